@@ -59,9 +59,10 @@ def draw(rng):
         kv = rng.choice([1, 2, 4, 8])
         heads = kv * rng.choice([1, 2, 4, 8] if kv < 8 else [1, 4])
         causal = rng.random() < 0.75
-        S = _log_int(rng, 1, 8192 if causal else 5700)
+        # (one token alone has no gradient by its scores: there is nothing to compare)
+        S = _log_int(rng, 2, 8192 if causal else 5700)
         return dict(kind=kind, B=rng.randint(1, max(1, min(8, 8192 // S))), S=S, heads=heads, kv=kv, d=d, causal=causal,
-                    docs=rng.choice([0, _log_int(rng, 20, 2000)]), prefix=rng.choice([0.0, 0.0, 0.4]) if causal else 0.0,
+                    docs=rng.choice([0, _log_int(rng, 20, 2000)]) if S >= 16 else 0, prefix=rng.choice([0.0, 0.0, 0.4]) if causal else 0.0,
                     cap=rng.choice([0.0, 0.0, 30.0, 50.0]), alibi=rng.random() < 0.3, grad=rng.random() < 0.75)
     if kind == "rope":
         S = _log_int(rng, 1, 8192)
@@ -175,12 +176,7 @@ def _prepare_attention(c, seed, r):
     if c["prefix"]:
         st["prefix"] = marks.cuda()
     if c["grad"]:
-        for n in ("q", "k", "v"):
-            st[n] = st[n].detach().requires_grad_(own)
-    if own and (c["docs"] or c["prefix"]):
-        from lightron_b200.ops import functional as OF
-        # built once per batch and used by every layer, forward and backward
-        st["mask"] = OF.attention_mask(documents=st["documents"], prefix=st["prefix"], causal=c["causal"])
+        st.update({n: st[n].detach().requires_grad_() for n in ("q", "k", "v")})
     return st
 
 
@@ -206,7 +202,7 @@ def _prepare_rope(c, seed, r):
             at += n
     rows = r(B, S, (h + 2) * d)                          # heads of a wider row, as of a fused projection
     x = rows.unflatten(2, (-1, d))[:, :, :h]
-    return dict(c=c, x=x.detach().requires_grad_(own), dy=r(B, S, h, d), cos=ang.cos().float(), sin=ang.sin().float(), positions=pos.cuda(), axes=_axes(d))
+    return dict(c=c, x=x.detach().requires_grad_(), dy=r(B, S, h, d), cos=ang.cos().float(), sin=ang.sin().float(), positions=pos.cuda(), axes=_axes(d))
 
 
 # ---- one pass ----------------------------------------------------------------------------------
@@ -214,80 +210,69 @@ def _prepare_rope(c, seed, r):
 
 def run(st):
     kind = st["c"]["kind"]
-    if kind == "attn":
-        return _attention_own(st) if own else _attention_plain(st)
-    if kind == "rope":
-        return _rope_own(st) if own else _rope_plain(st)
-    return _clip_own(st) if own else _clip_plain(st)
+    if own:
+        return {"attn": _attention_own, "rope": _rope_own, "clip": _clip_own}[kind](st)
+    with torch.no_grad():
+        return {"attn": _attention_plain, "rope": _rope_plain, "clip": _clip_plain}[kind](st)
 
 
 def _attention_own(st):
     from lightron_b200.ops import functional as OF
     q, k, v = st["q"], st["k"], st["v"]
-    o = OF.masked_attention(q, k, v, mask=st.get("mask"), causal=st["causal"], scale=st["scale"], softcap=st["cap"], slopes=st["slopes"])
+    mask = None
+    if st["documents"] is not None or st["prefix"] is not None:
+        # (a model makes it once per batch, for all of its layers)
+        mask = OF.attention_mask(documents=st["documents"], prefix=st["prefix"], causal=st["causal"])
+    o = OF.masked_attention(q, k, v, mask=mask, causal=st["causal"], scale=st["scale"], softcap=st["cap"], slopes=st["slopes"])
     if st["do"] is None:
         return o
     return (o, *torch.autograd.grad(o, (q, k, v), st["do"]))
 
 
 def _visible(st):
-    """[B, S, S]: whether query i sees key j."""
+    """[B, 1, 1, S, S]: whether query i sees key j."""
     c = st["c"]
-    B, S = c["B"], c["S"]
-    i = torch.arange(S, device="cuda")
-    see = (i[None, :] <= i[:, None]) if c["causal"] else torch.ones(S, S, dtype=torch.bool, device="cuda")
-    see = see.expand(B, S, S)
+    i = torch.arange(c["S"], device="cuda")
+    see = (i[None, :] <= i[:, None])[None] if c["causal"] else torch.ones(1, c["S"], c["S"], dtype=torch.bool, device="cuda")
     if st["prefix"] is not None:
         see = see | st["prefix"][:, None, :]
     if st["documents"] is not None:
         ids = st["documents"]
         see = see & (ids[:, :, None] == ids[:, None, :]) & (ids[:, :, None] >= 0)
-    return see
+    return see[:, None, None]
 
 
 def _attention_plain(st):
     c = st["c"]
-    B, S, hq, hkv, d = c["B"], c["S"], c["heads"], c["kv"], c["d"]
-    rep = hq // hkv
-    see = _visible(st)
-    grad = st["do"] is not None
-    i = torch.arange(S, device="cuda", dtype=torch.float32)
-    away = (i[:, None] - i[None, :]).abs()
-    o = torch.empty(B, S, hq, d, dtype=BF16, device="cuda")
-    if grad:
-        dq, dk, dv = torch.empty_like(o), torch.empty(B, S, hkv, d, dtype=BF16, device="cuda"), torch.empty(B, S, hkv, d, dtype=BF16, device="cuda")
-    for b in range(B):
-        for g in range(hkv):
-            hs = slice(g * rep, (g + 1) * rep)
-            q = st["q"][b, :, hs].float().transpose(0, 1)              # [rep, S, d]
-            k, v = st["k"][b, :, g].float(), st["v"][b, :, g].float()   # [S, d]
-            s = (q @ k.t()) * st["scale"]
-            if c["cap"]:
-                t = torch.tanh(s / c["cap"])
-                s = c["cap"] * t
-            if st["slopes"] is not None:
-                s = s - st["slopes"][hs, None, None] * away
-            s = s.masked_fill(~see[b], float("-inf"))
-            m = s.amax(dim=-1, keepdim=True).clamp_min(-3e38)
-            p = torch.exp(s - m)
-            del s
-            p = p / p.sum(dim=-1, keepdim=True).clamp_min(1e-38)
-            out = p @ v
-            o[b, :, hs] = out.transpose(0, 1).to(BF16)
-            if not grad:
-                continue
-            do = st["do"][b, :, hs].float().transpose(0, 1)
-            dv[b, :, g] = (p.transpose(1, 2) @ do).sum(0).to(BF16)
-            ds = do @ v.t()
-            ds = p * (ds - (out * do).sum(dim=-1, keepdim=True)) * st["scale"]
-            del p
-            if c["cap"]:
-                ds = ds * (1 - t * t)
-                del t
-            dq[b, :, hs] = (ds @ k).transpose(0, 1).to(BF16)
-            dk[b, :, g] = (ds.transpose(1, 2) @ q).sum(0).to(BF16)
-            del ds
-    return (o, dq, dk, dv) if grad else o
+    rep = c["heads"] // c["kv"]
+    q = st["q"].float().unflatten(2, (-1, rep)).permute(0, 2, 3, 1, 4)      # [B, kv, rep, S, d]
+    k, v = (st[n].float().permute(0, 2, 1, 3)[:, :, None] for n in ("k", "v"))      # [B, kv, 1, S, d]
+    s = (q @ k.transpose(-1, -2)).mul_(st["scale"])
+    if c["cap"]:
+        t = torch.tanh(s / c["cap"])
+        s = c["cap"] * t
+    if st["slopes"] is not None:
+        i = torch.arange(c["S"], device="cuda", dtype=torch.float32)
+        s -= st["slopes"].view(c["kv"], rep, 1, 1) * (i[:, None] - i[None, :]).abs()
+    s.masked_fill_(~_visible(st), float("-inf"))
+    p = torch.exp(s.sub_(s.amax(dim=-1, keepdim=True).clamp_min(-3e38)))
+    del s
+    p /= p.sum(dim=-1, keepdim=True).clamp_min(1e-38)
+    o = p @ v
+
+    def tokens_first(x):
+        return x.flatten(1, 2).transpose(1, 2).to(BF16)
+
+    if st["do"] is None:
+        return tokens_first(o)
+    do = st["do"].float().unflatten(2, (-1, rep)).permute(0, 2, 3, 1, 4)
+    dv = (p.transpose(-1, -2) @ do).sum(2, keepdim=True)
+    ds = (do @ v.transpose(-1, -2)).sub_((o * do).sum(dim=-1, keepdim=True)).mul_(p).mul_(st["scale"])
+    del p
+    if c["cap"]:
+        ds *= 1 - t * t
+    dq, dk = ds @ k, (ds.transpose(-1, -2) @ q).sum(2, keepdim=True)
+    return tuple(tokens_first(x) for x in (o, dq, dk, dv))
 
 
 def _rope_own(st):
@@ -323,8 +308,7 @@ def _clip_plain(st):
     if not st["c"]["clip"]:
         return norm
     scale = (st["max_norm"] / (norm + 1e-6)).clamp_max(1.0)
-    for g, o in zip(st["grads"], st["out"]):
-        o.copy_((g.float() * scale).to(g.dtype))
+    torch._foreach_copy_(st["out"], [(g.float() * scale).to(g.dtype) for g in st["grads"]])
     return [norm, *st["flat"]]
 
 
@@ -362,12 +346,7 @@ def work(c):
 
 
 def exact(c, seed):
-    global own
-    mine, own = own, False
-    try:
-        st = prepare(c, seed)
-    finally:
-        own = mine
+    st = prepare(c, seed)
     if c["kind"] == "attn":
         return _attention_exact(c, st)
     if c["kind"] == "rope":
