@@ -1,0 +1,304 @@
+// Attention under interval masks (attn_masked.cuh): the intervals of a batch, forward and backward.
+#include "attn_masked.cuh"
+
+namespace {
+
+constexpr int PLAN_THREADS = 1024;
+
+// Value of the nearest thread before (or, REVERSE, behind) this one that has one (>= 0); -1: none has.
+template <bool REVERSE>
+__device__ __forceinline__ int carry_in(int own, int* sh) {
+  const int t = REVERSE ? PLAN_THREADS - 1 - (int)threadIdx.x : (int)threadIdx.x;
+  const int lane = threadIdx.x & 31, w = t >> 5, l = REVERSE ? 31 - lane : lane;
+  int v = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = REVERSE ? __shfl_down_sync(0xffffffffu, v, o) : __shfl_up_sync(0xffffffffu, v, o);
+    if (l >= o && v < 0) v = x;
+  }
+  __syncthreads();
+  if (l == 31) sh[w] = v;
+  __syncthreads();
+  int before = REVERSE ? __shfl_down_sync(0xffffffffu, v, 1) : __shfl_up_sync(0xffffffffu, v, 1);
+  if (l == 0) before = -1;
+  for (int i = w - 1; i >= 0 && before < 0; i--) before = sh[i];
+  return before;
+}
+
+// Intervals of one sequence by one CTA, a run of positions per thread.  A document is a run of equal ids; ids below zero are padding, which sees nothing and
+// is seen by nothing (an empty interval at its own place keeps the ends in order).  The prefix of a document is the marked run at its start.
+template <typename Id>
+__global__ void __launch_bounds__(PLAN_THREADS) attn_mask_kernel(const Id* __restrict__ ids, const unsigned char* __restrict__ marks, const int* __restrict__ lens,
+                                                                 int S, int causal, int2* __restrict__ qb, int2* __restrict__ kb) {
+  __shared__ int sh[32];
+  grid_go();
+  grid_wait();
+  const long long base = (long long)blockIdx.x * S;
+  if (ids) ids += base;
+  if (marks) marks += base;
+  qb += base;
+  kb += base;
+  const int len = lens ? lens[blockIdx.x] : 0;
+  const int per = (S + PLAN_THREADS - 1) / PLAN_THREADS;
+  const int a = min(S, (int)threadIdx.x * per), e = min(S, a + per);
+  auto starts = [&](int i) { return i == 0 || (ids && ids[i] != ids[i - 1]); };
+  auto plain = [&](int i) { return marks ? marks[i] == 0 : i >= len; };          // outside the prefix part
+  int first_start = -1, last_start = -1, first_plain = -1;
+  for (int i = a; i < e; i++) {
+    if (starts(i)) { last_start = i; if (first_start < 0) first_start = i; }
+    if (first_plain < 0 && plain(i)) first_plain = i;
+  }
+  int end = carry_in<true>(first_start, sh), np = carry_in<true>(first_plain, sh), start = carry_in<false>(last_start, sh);
+  if (end < 0) end = S;
+  if (np < 0) np = S;
+  // backwards: end of the document, and the first position from here on that is not marked
+  for (int i = e - 1; i >= a; i--) {
+    if (plain(i)) np = i;
+    kb[i].y = end;
+    qb[i].y = np;
+    if (starts(i)) end = i;
+  }
+  __syncthreads();
+  int prefix = start >= 0 && a < e ? qb[start].y : 0;      // (unused where this thread's first position starts a document)
+  __syncthreads();
+  for (int i = a; i < e; i++) {
+    if (starts(i)) { start = i; prefix = qb[i].y; }
+    const int stop = kb[i].y, pe = min(prefix, stop);
+    if (ids && ids[i] < 0) {
+      qb[i] = kb[i] = make_int2(i, i);
+    } else {
+      qb[i] = make_int2(start, causal ? max(i + 1, pe) : stop);
+      kb[i] = make_int2(causal && i >= pe ? i : start, stop);
+    }
+  }
+}
+
+// ---- a warp per row: right for every size ---------------------------------------------------------
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float dot_row(const bf16* a, const bf16* b, int d) {
+  float s = 0.f;
+  for (int c = 0; c < d; c += 8) {
+    float x[8], y[8];
+    unpack8(*reinterpret_cast<const uint4*>(a + c), x);
+    unpack8(*reinterpret_cast<const uint4*>(b + c), y);
+#pragma unroll
+    for (int i = 0; i < 8; i++) s += x[i] * y[i];
+  }
+  return s;
+}
+__device__ __forceinline__ void load4(const bf16* p, float* f) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  const bf162* h = reinterpret_cast<const bf162*>(&u);
+  const float2 x = __bfloat1622float2(h[0]), y = __bfloat1622float2(h[1]);
+  f[0] = x.x; f[1] = x.y; f[2] = y.x; f[3] = y.y;
+}
+__device__ __forceinline__ void store4(bf16* p, const float* f) {
+  bf162 h[2] = {__floats2bfloat162_rn(f[0], f[1]), __floats2bfloat162_rn(f[2], f[3])};
+  *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(h);
+}
+// score, and its derivative by the uncapped score
+__device__ __forceinline__ float ma_score(const MaParams& p, float qk, int away, float slope, float& dcap) {
+  float s = qk * p.scale;
+  dcap = 1.f;
+  if (p.softcap > 0.f) {
+    const float t = tanhf(s / p.softcap);
+    s = p.softcap * t;
+    dcap = 1.f - t * t;
+  }
+  return s - slope * (float)abs(away);
+}
+
+__global__ void ma_fwd_rows_kernel(const MaParams p) {
+  const long long row = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (row >= (long long)p.B * p.hq * p.Sq) return;
+  const int lane = threadIdx.x & 31, i = (int)(row % p.Sq), h = (int)(row / p.Sq % p.hq), b = (int)(row / p.Sq / p.hq), g = h / (p.hq / p.hkv);
+  const bf16* q = p.q + b * p.qs.b + i * p.qs.s + h * p.qs.h;
+  const bf16 *k = p.k + b * p.ks.b + g * p.ks.h, *v = p.v + b * p.vs.b + g * p.vs.h;
+  const int2 r = ma_keys(p, b, i);
+  const float slope = p.slopes ? p.slopes[h] : 0.f;
+  const bool mine = lane * 4 < p.d;
+  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int j0 = r.x; j0 < r.y; j0 += 32) {
+    const int j = j0 + lane;
+    float s = -INFINITY, dc;
+    if (j < r.y) s = ma_score(p, dot_row(q, k + j * p.ks.s, p.d), i + p.Sk - p.Sq - j, slope, dc);
+    const float mn = fmaxf(m, warp_max(s));
+    const float e = j < r.y ? exp2f((s - mn) * LOG2E) : 0.f, c = m == -INFINITY ? 0.f : exp2f((m - mn) * LOG2E);
+    m = mn;
+    l = l * c + warp_sum(e);
+#pragma unroll
+    for (int x = 0; x < 4; x++) o[x] *= c;
+    for (int n = 0; n < min(32, r.y - j0); n++) {
+      const float pn = __shfl_sync(0xffffffffu, e, n);
+      if (mine) {
+        float f[4];
+        load4(v + (j0 + n) * p.vs.s + lane * 4, f);
+#pragma unroll
+        for (int x = 0; x < 4; x++) o[x] += pn * f[x];
+      }
+    }
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  if (mine) {
+    const long long at = (((long long)b * p.Sq + i) * p.hq + h) * p.d + lane * 4;
+    float hi[4];
+#pragma unroll
+    for (int x = 0; x < 4; x++) { o[x] *= inv; hi[x] = __bfloat162float(__float2bfloat16(o[x])); o[x] -= hi[x]; }
+    store4(p.o + at, hi);
+    if (p.o_lo) store4(p.o_lo + at, o);
+  }
+  if (lane == 0) p.lse[row] = r.x < r.y ? m + logf(l) : -INFINITY;
+}
+
+// D of a row, then dQ.
+__global__ void ma_bwd_rows_kernel(const MaBwdParams w) {
+  const MaParams& p = w.f;
+  const long long row = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (row >= (long long)p.B * p.hq * p.Sq) return;
+  const int lane = threadIdx.x & 31, i = (int)(row % p.Sq), h = (int)(row / p.Sq % p.hq), b = (int)(row / p.Sq / p.hq), g = h / (p.hq / p.hkv);
+  const bf16 *q = p.q + b * p.qs.b + i * p.qs.s + h * p.qs.h, *dout = w.dout + b * w.dos.b + i * w.dos.s + h * w.dos.h;
+  const bf16 *k = p.k + b * p.ks.b + g * p.ks.h, *v = p.v + b * p.vs.b + g * p.vs.h;
+  const int2 r = ma_keys(p, b, i);
+  const float slope = p.slopes ? p.slopes[h] : 0.f, lse = p.lse[row];
+  const bool mine = lane * 4 < p.d;
+  float D = 0.f, dq[4] = {0.f, 0.f, 0.f, 0.f};
+  if (mine) {
+    float x[4], y[4], z[4];
+    const long long at = (((long long)b * p.Sq + i) * p.hq + h) * p.d + lane * 4;
+    load4(p.o + at, x);
+    load4(p.o_lo + at, y);
+    load4(dout + lane * 4, z);
+#pragma unroll
+    for (int c = 0; c < 4; c++) D += (x[c] + y[c]) * z[c];
+  }
+  D = warp_sum(D);
+  if (lane == 0) w.stats[row] = D;
+  for (int j0 = r.x; j0 < r.y; j0 += 32) {
+    const int j = j0 + lane;
+    float ds = 0.f;
+    if (j < r.y) {
+      float dc;
+      const float s = ma_score(p, dot_row(q, k + j * p.ks.s, p.d), i + p.Sk - p.Sq - j, slope, dc);
+      ds = exp2f((s - lse) * LOG2E) * (dot_row(dout, v + j * p.vs.s, p.d) - D) * dc * p.scale;
+    }
+    for (int n = 0; n < min(32, r.y - j0); n++) {
+      const float x = __shfl_sync(0xffffffffu, ds, n);
+      if (mine) {
+        float f[4];
+        load4(k + (j0 + n) * p.ks.s + lane * 4, f);
+#pragma unroll
+        for (int c = 0; c < 4; c++) dq[c] += x * f[c];
+      }
+    }
+  }
+  if (mine) store4(w.dq + b * w.dqs.b + i * w.dqs.s + h * w.dqs.h + lane * 4, dq);
+}
+
+__global__ void ma_bwd_keys_kernel(const MaBwdParams w) {
+  const MaParams& p = w.f;
+  const long long row = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (row >= (long long)p.B * p.hkv * p.Sk) return;
+  const int lane = threadIdx.x & 31, j = (int)(row % p.Sk), g = (int)(row / p.Sk % p.hkv), b = (int)(row / p.Sk / p.hkv), rep = p.hq / p.hkv;
+  const bf16 *k = p.k + b * p.ks.b + j * p.ks.s + g * p.ks.h, *v = p.v + b * p.vs.b + j * p.vs.s + g * p.vs.h;
+  const int2 r = ma_queries(p, b, j);
+  const bool mine = lane * 4 < p.d;
+  float dk[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int h = g * rep; h < (g + 1) * rep; h++) {
+    const float slope = p.slopes ? p.slopes[h] : 0.f;
+    const bf16 *q = p.q + b * p.qs.b + h * p.qs.h, *dout = w.dout + b * w.dos.b + h * w.dos.h;
+    for (int i0 = r.x; i0 < r.y; i0 += 32) {
+      const int i = i0 + lane;
+      float ds = 0.f, e = 0.f;
+      if (i < r.y) {
+        float dc;
+        const long long at = ((long long)b * p.hq + h) * p.Sq + i;
+        const float s = ma_score(p, dot_row(q + i * p.qs.s, k, p.d), i + p.Sk - p.Sq - j, slope, dc);
+        e = exp2f((s - p.lse[at]) * LOG2E);
+        ds = e * (dot_row(dout + i * w.dos.s, v, p.d) - w.stats[at]) * dc * p.scale;
+      }
+      for (int n = 0; n < min(32, r.y - i0); n++) {
+        const float x = __shfl_sync(0xffffffffu, ds, n), y = __shfl_sync(0xffffffffu, e, n);
+        if (mine) {
+          float f[4], f2[4];
+          load4(q + (i0 + n) * p.qs.s + lane * 4, f);
+          load4(dout + (i0 + n) * w.dos.s + lane * 4, f2);
+#pragma unroll
+          for (int c = 0; c < 4; c++) { dk[c] += x * f[c]; dv[c] += y * f2[c]; }
+        }
+      }
+    }
+  }
+  if (mine) {
+    store4(w.dk + b * w.dks.b + j * w.dks.s + g * w.dks.h + lane * 4, dk);
+    store4(w.dv + b * w.dvs.b + j * w.dvs.s + g * w.dvs.h + lane * 4, dv);
+  }
+}
+
+bool bad_strides(const MaStrides& s) { return (s.b | s.s | s.h) % 8 != 0; }
+bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
+MaStrides strides_at(const long long* s) { return MaStrides{s[0], s[1], s[2]}; }
+
+int fill(MaParams& p, const void* q, const void* k, const void* v, void* o, void* o_lo, void* lse, int B, int Sq, int Sk, int hq, int hkv, int d, const long long* st,
+         float scale, int causal, float softcap, const void* slopes, const void* q_bounds, const void* k_bounds) {
+  if (B <= 0 || Sq <= 0 || Sk < Sq || hq <= 0 || hkv <= 0 || hq % hkv || d <= 0 || d % 8 || d > 128) return LB_ERR_SHAPE;
+  if (!q || !k || !v || !o || !lse || !st || !(softcap >= 0.f) || (!q_bounds) != (!k_bounds)) return LB_ERR_ARG;
+  if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(o) || misaligned(o_lo)) return LB_ERR_ARG;
+  p = MaParams{(const bf16*)q, (const bf16*)k, (const bf16*)v, strides_at(st), strides_at(st + 3), strides_at(st + 6), (bf16*)o, (bf16*)o_lo, (float*)lse, B, Sq, Sk, hq, hkv, d,
+               scale, causal, softcap, (const float*)slopes, (const int2*)q_bounds, (const int2*)k_bounds};
+  return bad_strides(p.qs) || bad_strides(p.ks) || bad_strides(p.vs) ? LB_ERR_SHAPE : LB_OK;
+}
+
+}  // namespace
+
+// Intervals of B sequences of S positions: q_bounds [B, S, 2] the keys that a position sees, k_bounds [B, S, 2] the positions that see a key.
+// ids: null or [B, S] of id_bytes (4 or 8) each; marks: null or [B, S] bytes, or lens: null or [B], the prefix part by its marks or its length.
+extern "C" int lb_attn_mask(const void* ids, int id_bytes, const void* marks, const void* lens, int B, int S, int causal, void* q_bounds, void* k_bounds, void* stream) {
+  if (B <= 0 || S <= 0) return LB_ERR_SHAPE;
+  if (!q_bounds || !k_bounds || (ids && id_bytes != 4 && id_bytes != 8) || (marks && lens)) return LB_ERR_ARG;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (id_bytes == 8)
+    LB_LAUNCH(attn_mask_kernel<long long>, B, PLAN_THREADS, 0, s, (const long long*)ids, (const unsigned char*)marks, (const int*)lens, S, causal, (int2*)q_bounds, (int2*)k_bounds);
+  else
+    LB_LAUNCH(attn_mask_kernel<int>, B, PLAN_THREADS, 0, s, (const int*)ids, (const unsigned char*)marks, (const int*)lens, S, causal, (int2*)q_bounds, (int2*)k_bounds);
+  return LB_OK;
+}
+
+// Forward.  strides: 3 x {batch, token, head} of q, k, v in elements, multiples of 8; o, o_lo (or null) [B, Sq, hq, d] and lse [B, hq, Sq] contiguous.
+// head_dim a multiple of 8 up to 128, Sk >= Sq; slopes null or fp32 [hq]; q_bounds / k_bounds of lb_attn_mask() over Sk positions, or null: causal or all keys.
+extern "C" int lb_masked_attn_fwd(const void* q, const void* k, const void* v, void* o, void* o_lo, void* lse, int B, int Sq, int Sk, int hq, int hkv, int d,
+                                  const long long* strides, float scale, int causal, float softcap, const void* slopes, const void* q_bounds, const void* k_bounds,
+                                  void* stream) {
+  MaParams p;
+  if (const int rc = fill(p, q, k, v, o, o_lo, lse, B, Sq, Sk, hq, hkv, d, strides, scale, causal, softcap, slopes, q_bounds, k_bounds)) return rc;
+  const long long rows = (long long)B * hq * Sq;
+  if ((rows + 3) / 4 > 2147483647LL) return LB_ERR_SHAPE;
+  ma_fwd_rows_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, (cudaStream_t)stream>>>(p);
+  LB_CHECK_LAUNCH();
+  return LB_OK;
+}
+
+extern "C" long long lb_masked_attn_bwd_ws_bytes(int B, int Sq, int Sk, int hq, int hkv, int d) {
+  (void)Sk; (void)hkv; (void)d;
+  return (long long)B * hq * Sq * (long long)sizeof(float);
+}
+
+// Backward.  strides: 7 x {batch, token, head} of q, k, v, dout, dq, dk, dv; o, o_lo, lse as the forward left them; ws: lb_masked_attn_bwd_ws_bytes(), 16-byte aligned.
+extern "C" int lb_masked_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_lo, const void* dout, const void* lse, void* ws, long long ws_bytes,
+                                  void* dq, void* dk, void* dv, int B, int Sq, int Sk, int hq, int hkv, int d, const long long* strides, float scale, int causal, float softcap,
+                                  const void* slopes, const void* q_bounds, const void* k_bounds, void* stream) {
+  MaBwdParams w;
+  if (const int rc = fill(w.f, q, k, v, const_cast<void*>(o), const_cast<void*>(o_lo), const_cast<void*>(lse), B, Sq, Sk, hq, hkv, d, strides, scale, causal, softcap, slopes, q_bounds, k_bounds)) return rc;
+  if (!o_lo || !dout || !ws || !dq || !dk || !dv || misaligned(dout) || misaligned(ws) || misaligned(dq) || misaligned(dk) || misaligned(dv)) return LB_ERR_ARG;
+  if (ws_bytes < lb_masked_attn_bwd_ws_bytes(B, Sq, Sk, hq, hkv, d)) return LB_ERR_CAPACITY;
+  w.dout = (const bf16*)dout; w.dq = (bf16*)dq; w.dk = (bf16*)dk; w.dv = (bf16*)dv; w.stats = (float*)ws;
+  w.dos = strides_at(strides + 9); w.dqs = strides_at(strides + 12); w.dks = strides_at(strides + 15); w.dvs = strides_at(strides + 18);
+  if (bad_strides(w.dos) || bad_strides(w.dqs) || bad_strides(w.dks) || bad_strides(w.dvs)) return LB_ERR_SHAPE;
+  const long long rows = (long long)B * hq * Sq, keys = (long long)B * hkv * Sk;
+  if ((rows + 3) / 4 > 2147483647LL || (keys + 3) / 4 > 2147483647LL) return LB_ERR_SHAPE;
+  ma_bwd_rows_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, (cudaStream_t)stream>>>(w);
+  LB_CHECK_LAUNCH();
+  ma_bwd_keys_kernel<<<(unsigned)((keys + 3) / 4), 128, 0, (cudaStream_t)stream>>>(w);
+  LB_CHECK_LAUNCH();
+  return LB_OK;
+}

@@ -1,0 +1,190 @@
+// Global norm of many tensors, and their scaling by it.
+//
+//     norm = sqrt(sum over all tensors of sum g^2)        g * min(1, max_norm / (norm + eps))
+//
+// Both are memory bound: the sum reads every element once, the scaling reads it again and writes it.  The tensors' addresses travel as
+// kernel parameters, so that a call uploads nothing and can be captured.  Every tensor is cut into chunks of CHUNK elements, chunk c belongs to CTA
+// c % grid, and a CTA leaves the fp32 sum of its squares in a place of its own; whoever needs the total adds those up in 64 bits, in their order: the
+// norm is the same bits in every run.
+#include <cuda_fp16.h>
+#include "common.cuh"
+
+namespace {
+
+constexpr int THREADS = 256, MAX_TENSORS = 768, CHUNK = 16384;
+enum : int { BF16 = 0, FP16 = 1, FP32 = 2 };
+
+struct Tensors {
+  int n, chunks;
+  const void* src[MAX_TENSORS];
+  void* dst[MAX_TENSORS];
+  long long count[MAX_TENSORS];
+  int first[MAX_TENSORS];                      // chunks ahead of a tensor's, with its type in the upper two bits
+};
+static_assert(sizeof(Tensors) <= 32000, "kernel parameters");
+
+__device__ __forceinline__ float to_f(bf16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f(float x) { return x; }
+template <typename T> __device__ __forceinline__ T from_f(float x);
+template <> __device__ __forceinline__ bf16 from_f<bf16>(float x) { return __float2bfloat16(x); }
+template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half(x); }
+template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
+
+// Sum over the CTA, in the same order in every run; to thread 0.
+__device__ __forceinline__ float block_sum(float s) {
+  __shared__ float sh[THREADS / 32];
+  s = warp_sum(s);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
+  __syncthreads();
+  float t = 0.f;
+  if (threadIdx.x == 0)
+    for (int i = 0; i < THREADS / 32; i++) t += sh[i];
+  return t;
+}
+
+// The chunk's tensor: the last whose first chunk is not behind it (empty tensors have none and are never the last).
+__device__ __forceinline__ int tensor_of(const Tensors& t, int chunk) {
+  int lo = 0, hi = t.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((t.first[mid] & 0x3fffffff) <= chunk) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <typename T>
+__device__ __forceinline__ float chunk_squares(const T* x, int n) {
+  float s = 0.f;
+  for (int i = threadIdx.x; i < n; i += THREADS) { const float f = to_f(x[i]); s += f * f; }
+  return s;
+}
+
+__global__ void __launch_bounds__(THREADS) grad_squares_kernel(const __grid_constant__ Tensors t, float* __restrict__ partial) {
+  grid_go();
+  grid_wait();
+  float s = 0.f;
+  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+    const int k = tensor_of(t, c), type = (unsigned)t.first[k] >> 30;
+    const long long at = (long long)(c - (t.first[k] & 0x3fffffff)) * CHUNK;
+    const int n = (int)min((long long)CHUNK, t.count[k] - at);
+    s += type == FP32 ? chunk_squares((const float*)t.src[k] + at, n) : type == BF16 ? chunk_squares((const bf16*)t.src[k] + at, n) : chunk_squares((const __half*)t.src[k] + at, n);
+  }
+  s = block_sum(s);
+  if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+// Sum of the parts in 64 bits, in an order of its own; to all threads.
+__device__ __forceinline__ double total_of(const float* partial, int n) {
+  __shared__ double sh[THREADS];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += THREADS) s += (double)partial[i];
+  sh[threadIdx.x] = s;
+  __syncthreads();
+#pragma unroll
+  for (int o = THREADS / 2; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
+    __syncthreads();
+  }
+  return sh[0];
+}
+
+__global__ void __launch_bounds__(THREADS) grad_total_kernel(const float* __restrict__ partial, int n, float* __restrict__ sumsq, float* __restrict__ norm) {
+  grid_go();
+  grid_wait();
+  const double s = total_of(partial, n);
+  if (threadIdx.x == 0) {
+    if (sumsq) *sumsq = (float)s;
+    if (norm) *norm = (float)sqrt(s);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void chunk_scale(const T* x, T* y, int n, float by) {
+  for (int i = threadIdx.x; i < n; i += THREADS) y[i] = from_f<T>(to_f(x[i]) * by);
+}
+
+__global__ void __launch_bounds__(THREADS) grad_scale_kernel(const __grid_constant__ Tensors t, const float* __restrict__ partial, int n_partial, float max_norm, float eps,
+                                                             float* __restrict__ norm_out) {
+  grid_go();
+  grid_wait();
+  const float norm = (float)sqrt(total_of(partial, n_partial));
+  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+  const float r = max_norm / (norm + eps), by = r > 1.f ? 1.f : r;       // (a NaN stays one)
+  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+    const int k = tensor_of(t, c), type = (unsigned)t.first[k] >> 30;
+    if (by == 1.f && t.src[k] == t.dst[k]) continue;
+    const long long at = (long long)(c - (t.first[k] & 0x3fffffff)) * CHUNK;
+    const int n = (int)min((long long)CHUNK, t.count[k] - at);
+    if (type == FP32) chunk_scale((const float*)t.src[k] + at, (float*)t.dst[k] + at, n, by);
+    else if (type == BF16) chunk_scale((const bf16*)t.src[k] + at, (bf16*)t.dst[k] + at, n, by);
+    else chunk_scale((const __half*)t.src[k] + at, (__half*)t.dst[k] + at, n, by);
+  }
+}
+
+int grid_of(int chunks) { const int most = lb_num_sms() * 8; return chunks < most ? chunks : most; }
+
+// The next tensors of a list, up to what one launch takes; `at` moves on.
+int next_tensors(Tensors& t, int n, int& at, const void* const* src, void* const* dst, const long long* counts, const int* types) {
+  t.n = t.chunks = 0;
+  for (; at < n && t.n < MAX_TENSORS; at++) {
+    if (counts[at] < 0 || (counts[at] && (!src[at] || (dst && !dst[at]))) || types[at] < BF16 || types[at] > FP32) return LB_ERR_ARG;
+    const long long chunks = (counts[at] + CHUNK - 1) / CHUNK;
+    if (!chunks) continue;
+    if (t.chunks + chunks >= (1LL << 30)) {
+      if (!t.n) return LB_ERR_SHAPE;
+      break;
+    }
+    t.src[t.n] = src[at];
+    t.dst[t.n] = dst ? dst[at] : nullptr;
+    t.count[t.n] = counts[at];
+    t.first[t.n++] = (int)((unsigned)t.chunks | (unsigned)types[at] << 30);
+    t.chunks += (int)chunks;
+  }
+  return LB_OK;
+}
+
+}  // namespace
+
+// Floats of `partial` that lb_grad_squares() of n tensors may fill.
+extern "C" int lb_grad_norm_parts(int n) { return n < 0 ? LB_ERR_ARG : (n / MAX_TENSORS + 1) * lb_num_sms() * 8; }
+
+// partial[0 .. *filled): sums of squares of parts of the n tensors (host arrays of device addresses, element counts and types: 0 bf16, 1 fp16, 2 fp32).
+extern "C" int lb_grad_squares(int n, const void* const* src, const long long* counts, const int* types, void* partial, int partials, int* filled, void* stream) {
+  if (n < 0 || !partial || !filled || (n && (!src || !counts || !types))) return LB_ERR_ARG;
+  static thread_local Tensors t;
+  *filled = 0;
+  for (int at = 0; at < n;) {
+    if (const int rc = next_tensors(t, n, at, src, nullptr, counts, types)) return rc;
+    if (!t.n) break;
+    const int grid = grid_of(t.chunks);
+    if (*filled + grid > partials) return LB_ERR_CAPACITY;
+    LB_LAUNCH(grad_squares_kernel, grid, THREADS, 0, (cudaStream_t)stream, t, (float*)partial + *filled);
+    *filled += grid;
+  }
+  return LB_OK;
+}
+
+// Total of n parts: its fp32 value and its root (either may be null).
+extern "C" int lb_grad_total(const void* partial, int n, void* sumsq, void* norm, void* stream) {
+  if (n < 0 || !partial) return LB_ERR_ARG;
+  LB_LAUNCH(grad_total_kernel, 1, THREADS, 0, (cudaStream_t)stream, (const float*)partial, n, (float*)sumsq, (float*)norm);
+  return LB_OK;
+}
+
+// dst = src * min(1, max_norm / (norm + eps)), norm the root of the total of the parts, also written to norm_out (null: not).  dst may be src, whose elements are
+// then left alone where the factor is 1.
+extern "C" int lb_grad_scale(int n, const void* const* src, void* const* dst, const long long* counts, const int* types, const void* partial, int n_partial, float max_norm,
+                             float eps, void* norm_out, void* stream) {
+  if (n < 0 || n_partial < 0 || !partial || (n && (!src || !dst || !counts || !types))) return LB_ERR_ARG;
+  static thread_local Tensors t;
+  for (int at = 0; at < n;) {
+    if (const int rc = next_tensors(t, n, at, src, dst, counts, types)) return rc;
+    if (!t.n) break;
+    LB_LAUNCH(grad_scale_kernel, grid_of(t.chunks), THREADS, 0, (cudaStream_t)stream, t, (const float*)partial, n_partial, max_norm, eps, (float*)norm_out);
+    norm_out = nullptr;
+  }
+  if (norm_out) return lb_grad_total(partial, n_partial, nullptr, norm_out, stream);
+  return LB_OK;
+}

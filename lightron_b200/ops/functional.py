@@ -727,6 +727,353 @@ def rope_attention_qkv(qkv: torch.Tensor, cos, sin, positions, B: int, S: int, h
 
 
 # --------------------------------------------------------------------------------------
+# Attention of packed batches: documents, prefixes, capped scores, a bias by distance
+# --------------------------------------------------------------------------------------
+
+
+class AttentionMask:
+    """Which keys each position of a packed batch sees (:func:`attention_mask`): per position the interval of keys, per key the interval of
+    positions, [batch, length, 2] int32.  Made once per batch, for all layers, forward and backward."""
+
+    __slots__ = ("q_bounds", "k_bounds", "causal")
+
+    def __init__(self, q_bounds: torch.Tensor, k_bounds: torch.Tensor, causal: bool):
+        self.q_bounds, self.k_bounds, self.causal = q_bounds, k_bounds, causal
+
+    @property
+    def batch(self) -> int:
+        return self.q_bounds.shape[0]
+
+    @property
+    def length(self) -> int:
+        return self.q_bounds.shape[1]
+
+
+def attention_mask(documents: Optional[torch.Tensor] = None, prefix: Optional[torch.Tensor] = None, causal: bool = True,
+                   length: Optional[int] = None) -> AttentionMask:
+    """``documents`` [B, S] int32 / int64: a document is a run of equal ids, whose positions see no other run's; negative ids are padding, which
+    sees nothing (its output is zero) and is seen by nothing.  ``prefix``: the leading part of each document that is seen both ways
+    in a causal mask, as [B, S] marks (bool / uint8; the marked run at the document's start counts) or as [B] int32 lengths from the sequence's
+    start (``length`` then gives S where there are no documents).  Values stay on the device.  (Values of padding are read all
+    the same, and multiplied by weights of zero: they have to be finite, as those of causal attention have to be.)"""
+    if documents is None and prefix is None:
+        raise ValueError("attention_mask needs documents or prefix (masked_attention takes causal=... alone)")
+    if documents is not None and (documents.dim() != 2 or documents.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"documents must be [B, S] int32 or int64, got {documents.dtype} {tuple(documents.shape)}")
+    marks = lens = None
+    if prefix is not None:
+        if not causal:
+            raise ValueError("a prefix has a meaning in a causal mask only")
+        if prefix.dim() == 2 and prefix.dtype in (torch.bool, torch.uint8):
+            marks = prefix
+        elif prefix.dim() == 1 and prefix.dtype in (torch.int32, torch.int64):
+            lens = prefix
+        else:
+            raise ValueError(f"prefix must be [B, S] bool / uint8 marks or [B] int32 / int64 lengths, got {prefix.dtype} {tuple(prefix.shape)}")
+    shaped = documents if documents is not None else marks
+    if shaped is None and length is None:
+        raise ValueError("prefix lengths alone need length=S")
+    B, S = shaped.shape if shaped is not None else (lens.shape[0], int(length))
+    if length is not None and int(length) != S:
+        raise ValueError(f"length {length} of a batch of {S} positions")
+    first = documents if documents is not None else prefix
+    if prefix is not None and (prefix.shape[0] != B or prefix.device != first.device or (marks is not None and marks.shape[1] != S)):
+        raise ValueError(f"prefix {tuple(prefix.shape)} on {prefix.device} does not belong to {B} sequences of {S} positions on {first.device}")
+    if not first.is_cuda or B == 0 or S == 0:
+        if B == 0 or S == 0:
+            empty = torch.zeros(B, S, 2, dtype=torch.int32, device=first.device)
+            return AttentionMask(empty, empty, causal)
+        return AttentionMask(*ref.mask_bounds(S, documents, prefix, causal), causal)
+    documents = None if documents is None else documents.contiguous()
+    marks = None if marks is None else marks.contiguous()
+    lens = None if lens is None else lens.to(torch.int32).contiguous()
+    qb = torch.empty(B, S, 2, dtype=torch.int32, device=first.device)
+    kb = torch.empty_like(qb)
+    with native.on_device(first):
+        native.call("lb_attn_mask", native.ptr(documents), documents.element_size() if documents is not None else 4, native.ptr(marks), native.ptr(lens), B, S,
+                    int(causal), qb.data_ptr(), kb.data_ptr(), native.stream_ptr())
+    return AttentionMask(qb, kb, causal)
+
+
+def _strided_ok(t: torch.Tensor) -> bool:
+    """Whether the masked attention kernels read [B, S, h, d] where it lies: rows of 16-byte aligned heads, in any order."""
+    if t.stride(3) != 1 or t.data_ptr() % 16:
+        return False
+    return all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:3], t.stride()[:3]))
+
+
+def _strided(t: torch.Tensor) -> torch.Tensor:
+    return t if _strided_ok(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(*ts: torch.Tensor):
+    """Strides {batch, token, head} of each tensor; those of single entries are never used, and made such that a tensor map takes them."""
+    import ctypes
+    flat = [s if n > 1 else t.shape[3] for t in ts for n, s in zip(t.shape[:3], t.stride()[:3])]
+    return (ctypes.c_longlong * len(flat))(*flat)
+
+
+def masked_fwd_native(q, k, v, causal: bool, scale: float, softcap: float, slopes, qb, kb, grad: bool):
+    """(o, what rounding o to bf16 left or None, lse): the backward's row sums of ``do * o`` need o to more than 8 bits where a row sees
+    few keys, for its score gradients are differences that then all but vanish."""
+    q, k, v = _strided(q), _strided(k), _strided(v)
+    B, Sq, hq, d = q.shape
+    Sk, hkv = k.shape[1], k.shape[2]
+    o = torch.empty(B, Sq, hq, d, dtype=q.dtype, device=q.device)
+    o_lo = torch.empty_like(o) if grad else None
+    lse = torch.empty(B, hq, Sq, dtype=torch.float32, device=q.device)
+    native.call("lb_masked_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), native.ptr(o_lo), lse.data_ptr(), B, Sq, Sk, hq, hkv, d,
+                _strides(q, k, v), scale, int(causal), softcap, native.ptr(slopes), native.ptr(qb), native.ptr(kb), native.stream_ptr())
+    return o, o_lo, lse
+
+
+def masked_bwd_native(q, k, v, o, o_lo, lse, do, causal: bool, scale: float, softcap: float, slopes, qb, kb, dq=None, dk=None, dv=None):
+    q, k, v, do = _strided(q), _strided(k), _strided(v), _strided(do)
+    B, Sq, hq, d = q.shape
+    Sk, hkv = k.shape[1], k.shape[2]
+    if dq is None:
+        dq, dk, dv = torch.empty_like(o), torch.empty(B, Sk, hkv, d, dtype=q.dtype, device=q.device), torch.empty(B, Sk, hkv, d, dtype=q.dtype, device=q.device)
+    ws = torch.empty(native.require().lb_masked_attn_bwd_ws_bytes(B, Sq, Sk, hq, hkv, d), dtype=torch.uint8, device=q.device)
+    native.call("lb_masked_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), o_lo.data_ptr(), do.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(),
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, Sq, Sk, hq, hkv, d, _strides(q, k, v, do, dq, dk, dv), scale, int(causal), softcap,
+                native.ptr(slopes), native.ptr(qb), native.ptr(kb), native.stream_ptr())
+    return dq, dk, dv
+
+
+class _MaskedAttn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, slopes, qb, kb, causal, scale, softcap):
+        with native.on_device(q):
+            o, o_lo, lse = masked_fwd_native(q, k, v, causal, scale, softcap, slopes, qb, kb, not isinstance(ctx, _NoGradCtx) and any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(q, k, v, o, o_lo, lse, slopes, qb, kb)
+        ctx.args = (causal, scale, softcap)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, o_lo, lse, slopes, qb, kb = ctx.saved_tensors
+        causal, scale, softcap = ctx.args
+        with native.on_device(q):
+            dq, dk, dv = masked_bwd_native(q, k, v, o, o_lo, lse, do, causal, scale, softcap, slopes, qb, kb)
+        return dq, dk, dv, None, None, None, None, None, None
+
+
+MASKED_MAX_HEAD_DIM = 128
+
+
+def _check_masked(q, k, v, mask, causal, softcap, slopes) -> bool:
+    """Refuses what does not fit together; returns whether the mask is causal."""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"masked_attention takes q [B, Sq, hq, d] and k, v [B, Sk, hkv, d]; got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, Sq, hq, d = q.shape
+    Sk, hkv = k.shape[1], k.shape[2]
+    if hkv == 0 or hq % hkv:
+        raise ValueError(f"{hq} query heads are not a multiple of {hkv} key heads")
+    if Sq > Sk:
+        raise ValueError(f"{Sq} queries at the end of {Sk} positions")
+    if not (k.dtype == v.dtype == q.dtype and k.device == v.device == q.device):
+        raise ValueError(f"q, k, v differ in type or device: {q.dtype} {q.device}, {k.dtype} {k.device}, {v.dtype} {v.device}")
+    if not (0.0 <= softcap < float("inf")):
+        raise ValueError(f"softcap must be zero (none) or positive and finite, got {softcap}")
+    if mask is not None:
+        if not isinstance(mask, AttentionMask):
+            raise ValueError(f"mask must come from attention_mask(), got {type(mask).__name__}")
+        if mask.batch != B or mask.length != Sk or mask.q_bounds.device != q.device:
+            raise ValueError(f"mask of {mask.batch} x {mask.length} positions on {mask.q_bounds.device} for keys {B} x {Sk} on {q.device}")
+        if causal is not None and bool(causal) != mask.causal:
+            raise ValueError(f"causal={causal} contradicts the mask, which was made with causal={mask.causal}")
+        causal = mask.causal
+    if slopes is not None:
+        if tuple(slopes.shape) != (hq,) or slopes.dtype != torch.float32 or slopes.device != q.device:
+            raise ValueError(f"slopes must be fp32 [{hq}] on {q.device}, got {slopes.dtype} {tuple(slopes.shape)} on {slopes.device}")
+        if slopes.requires_grad:
+            raise ValueError("slopes are constants: they get no gradient (detach them)")
+    return True if causal is None else bool(causal)
+
+
+def _check_masked_native(d: int) -> None:
+    if d % 8 or not 0 < d <= MASKED_MAX_HEAD_DIM:
+        raise ValueError(f"masked_attention on the GPU takes head sizes that are multiples of 8 up to {MASKED_MAX_HEAD_DIM}, got {d}")
+
+
+def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[AttentionMask] = None, causal: Optional[bool] = None,
+                     scale: Optional[float] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(s) v for q [B, Sq, hq, d] and k, v [B, Sk, hkv, d] in any order of the outer dimensions; query i sits at position i + Sk - Sq.
+    ``s = softcap * tanh(x / softcap) - slopes[h] * |distance|`` with ``x = scale * q.k`` (``softcap`` 0: x itself; ``slopes`` fp32 [hq], constants).
+    ``mask``: see :func:`attention_mask`; without one, ``causal`` (default) or all keys.  Rows that see nothing give zeros, and gradients of zero."""
+    causal = _check_masked(q, k, v, mask, causal, softcap, slopes)
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
+    qb, kb = (mask.q_bounds, mask.k_bounds) if mask is not None else (None, None)
+    if native.use_native(q) and q.numel() and k.numel():
+        _check_masked_native(q.shape[-1])
+        return _apply(_MaskedAttn, q, k, v, None if slopes is None else slopes.contiguous(), qb, kb, causal, scale, float(softcap))
+    return ref.masked_attention(q, k, v, qb, causal, scale, float(softcap), slopes)
+
+
+# --------------------------------------------------------------------------------------
+# Rotary positions with several axes
+# --------------------------------------------------------------------------------------
+
+
+def _rope_axes_native(x, out, cos, sin, positions, axes, inverse: bool) -> None:
+    """x [B, S, h, d] strided (:func:`_strided_ok`), out contiguous (or x itself, contiguous)."""
+    B, S, h, d = x.shape
+    pos_a, pos_b = positions.stride(0), positions.stride(1) if positions.dim() == 3 else 0
+    native.call("lb_rope_axes", x.data_ptr(), out.data_ptr(), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), bytes(axes), positions.shape[0], B, S, h, d,
+                cos.shape[0], _strides(x), pos_a, pos_b, int(inverse), native.stream_ptr())
+
+
+class _RopeAxes(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, cos, sin, positions, axes):
+        x = _strided(x)
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        with native.on_device(x):
+            _rope_axes_native(x, out, cos, sin, positions, axes, False)
+        ctx.save_for_backward(cos, sin, positions)
+        ctx.axes = axes
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        cos, sin, positions = ctx.saved_tensors
+        dy = _strided(dy)
+        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+        with native.on_device(dy):
+            _rope_axes_native(dy, dx, cos, sin, positions, ctx.axes, True)
+        return dx, None, None, None, None
+
+
+def _check_axes(B, S, d, cos, sin, positions, axes):
+    """(positions as int32 with unit stride over the tokens, axes as a tuple), or refuses them."""
+    axes = tuple(int(a) for a in axes)
+    if d % 2 or len(axes) != d // 2:
+        raise ValueError(f"axes name the axis of each of the {d // 2} pairs of a head, got {len(axes)}")
+    if positions.dim() not in (2, 3) or tuple(positions.shape[1:]) not in ((S,), (B, S)) or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"positions must be [axes, {B}, {S}] or [axes, {S}] int32 / int64, got {positions.dtype} {tuple(positions.shape)}")
+    if any(not 0 <= a < positions.shape[0] for a in axes):
+        raise ValueError(f"axes {sorted(set(axes))} of positions with {positions.shape[0]} axes")
+    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != d // 2 or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise ValueError(f"cos and sin must be fp32 [positions, {d // 2}], got {cos.dtype} {tuple(cos.shape)} and {sin.dtype} {tuple(sin.shape)}")
+    if not cos.device == sin.device == positions.device:
+        raise ValueError("cos, sin and positions are on different devices")
+    positions = positions.to(torch.int32)
+    return (positions if positions.stride(-1) == 1 else positions.contiguous()), axes
+
+
+def rope_axes(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, axes: Sequence[int]) -> torch.Tensor:
+    """x [B, S, h, d] -> rotated copy: pair i of every head turns by row ``positions[axes[i]]`` of the tables [*, d/2] (interleaved pairs, as
+    :func:`rope`).  ``positions`` [A, B, S] or [A, S]: time, height and width of every token, say; ``axes``: the axis of each of the d/2 pairs.  A position
+    outside the tables makes its pairs NaN."""
+    if x.dim() != 4:
+        raise ValueError(f"rope_axes takes x [B, S, h, d], got {tuple(x.shape)}")
+    B, S, _, d = x.shape
+    if cos.device != x.device:
+        raise ValueError(f"tables on {cos.device} for x on {x.device}")
+    positions, axes = _check_axes(B, S, d, cos, sin, positions, axes)
+    if native.use_native(x) and x.numel() and d % 8 == 0 and d <= 256 and positions.shape[0] <= 8:
+        return _apply(_RopeAxes, x, cos.contiguous(), sin.contiguous(), positions, axes)
+    return ref.rope_axes(x, cos, sin, positions, axes)
+
+
+# --------------------------------------------------------------------------------------
+# Global gradient norm and clipping
+# --------------------------------------------------------------------------------------
+
+_NORM_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _norm_list(tensors, what: str) -> List[torch.Tensor]:
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    for t in tensors:
+        if t.dtype not in _NORM_TYPES or t.layout != torch.strided:
+            raise ValueError(f"{what} must be dense bf16, fp16 or fp32, got {t.dtype} {t.layout}")
+        if t.device != tensors[0].device:
+            raise ValueError(f"{what} on {tensors[0].device} and {t.device}")
+    return tensors
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the elements fill one piece of memory, in whatever order."""
+    return t.is_contiguous() or (t.numel() > 0 and torch.ops.aten.is_non_overlapping_and_dense(t))
+
+
+def _norm_table(tensors):
+    import ctypes
+    n = len(tensors)
+    return (n, (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]), (ctypes.c_longlong * n)(*[t.numel() for t in tensors]),
+            (ctypes.c_int * n)(*[_NORM_TYPES[t.dtype] for t in tensors]))
+
+
+def _grad_parts(tensors, device):
+    """Sums of squares of parts of the tensors: (fp32 buffer, how many)."""
+    import ctypes
+    n, ptrs, counts, types = _norm_table([t if _dense(t) else t.contiguous() for t in tensors])
+    parts = torch.empty(native.require().lb_grad_norm_parts(n), dtype=torch.float32, device=device)
+    filled = ctypes.c_int(0)
+    native.call("lb_grad_squares", n, ptrs, counts, types, parts.data_ptr(), parts.numel(), ctypes.byref(filled), native.stream_ptr())
+    return parts, filled.value
+
+
+def _reduce_sumsq(sumsq: torch.Tensor, group) -> torch.Tensor:
+    if group is not None and dist.get_world_size(group) > 1:
+        dist.all_reduce(sumsq, group=group)
+    return sumsq
+
+
+@torch.no_grad()
+def grad_norm(tensors, group=None) -> torch.Tensor:
+    """2-norm of all elements of all tensors (bf16, fp16, fp32, mixed) together, a fp32 scalar on their device, without a host
+    synchronisation and the same bits in every run.  ``group``: the tensors are this rank's share of one whole."""
+    tensors = _norm_list(tensors, "tensors")
+    if not tensors or not tensors[0].is_cuda:
+        return _reduce_sumsq(ref.grad_sumsq(tensors), group).sqrt()
+    with native.on_device(tensors[0]):
+        parts, n = _grad_parts(tensors, tensors[0].device)
+        out = torch.empty((), dtype=torch.float32, device=tensors[0].device)
+        whole = group is None or dist.get_world_size(group) == 1
+        native.call("lb_grad_total", parts.data_ptr(), n, 0 if whole else out.data_ptr(), out.data_ptr() if whole else 0, native.stream_ptr())
+    return out if whole else _reduce_sumsq(out, group).sqrt()
+
+
+@torch.no_grad()
+def clip_grad_norm(tensors, max_norm: float, out=None, group=None, eps: float = 1e-6) -> torch.Tensor:
+    """Scales the tensors by ``min(1, max_norm / (norm + eps))`` and returns their norm (:func:`grad_norm`).  In place; or into ``out``, tensors of the same sizes
+    and types.  A norm that is not finite goes into the result as it would in the product: NaN stays NaN, an infinite norm gives zeros and NaN."""
+    tensors = _norm_list(tensors, "tensors")
+    if not (max_norm >= 0.0 and eps >= 0.0):
+        raise ValueError(f"max_norm {max_norm} and eps {eps} must not be negative")
+    outs = tensors if out is None else _norm_list(out, "out")
+    if len(outs) != len(tensors) or any(o.shape != t.shape or o.dtype != t.dtype or o.device != t.device for o, t in zip(outs, tensors)):
+        raise ValueError("out must be one tensor of the same size, type and device for each tensor")
+    if not tensors or not tensors[0].is_cuda:
+        norm = _reduce_sumsq(ref.grad_sumsq(tensors), group).sqrt()
+        by = (max_norm / (norm + eps)).clamp_max(1.0)
+        for t, o in zip(tensors, outs):
+            o.copy_((t.float() * by).to(t.dtype))
+        return norm
+    dev = tensors[0].device
+    with native.on_device(tensors[0]):
+        # (elements of the kernel's tensors lie in one piece, and in the same order in both)
+        src = [t if _dense(t) else t.contiguous() for t in tensors]
+        dst = [o if o is t or (o.stride() == t.stride() and _dense(o)) else torch.empty_like(t) for t, o in zip(src, outs)]
+        parts, n = _grad_parts(src, dev)
+        if group is not None and dist.get_world_size(group) > 1:
+            sumsq = torch.empty(1, dtype=torch.float32, device=dev)
+            native.call("lb_grad_total", parts.data_ptr(), n, sumsq.data_ptr(), 0, native.stream_ptr())
+            parts, n = _reduce_sumsq(sumsq, group), 1
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        k, sp, counts, types = _norm_table(src)
+        native.call("lb_grad_scale", k, sp, _norm_table(dst)[1], counts, types, parts.data_ptr(), n, float(max_norm), float(eps), norm.data_ptr(), native.stream_ptr())
+        for d, o in zip(dst, outs):
+            if d is not o:
+                o.copy_(d)
+    return norm
+
+
+# --------------------------------------------------------------------------------------
 # Embedding (optionally vocab-parallel)
 # --------------------------------------------------------------------------------------
 

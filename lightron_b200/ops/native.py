@@ -89,6 +89,15 @@ _SIGNATURES = {
     "lb_all_reduce_nvls": [_P, _P, _P, _P, _P, _L, _L, _I, _I, _I, _I, ctypes.c_uint, _P],
     "lb_dp_status": [_P],
     "lb_dp_adamw": [_P, _P, _P, _P, _P, _P, _P, _L, _L, _I, _I, ctypes.c_uint, _F, _F, _F, _F, _F, _F, _F, _F, _I, _P],
+    "lb_attn_mask": [_P, _I, _P, _P, _I, _I, _I, _P, _P, _P],
+    "lb_masked_attn_fwd": [_P] * 6 + [_I] * 6 + [_P, _F, _I, _F, _P, _P, _P, _P],
+    "lb_masked_attn_bwd": [_P] * 8 + [_L] + [_P] * 3 + [_I] * 6 + [_P, _F, _I, _F, _P, _P, _P, _P],
+    "lb_masked_attn_bwd_ws_bytes": [_I] * 6,
+    "lb_rope_axes": [_P] * 6 + [_I] * 6 + [_P, _L, _L, _I, _P],
+    "lb_grad_norm_parts": [_I],
+    "lb_grad_squares": [_I, _P, _P, _P, _P, _I, _P, _P],
+    "lb_grad_total": [_P, _I, _P, _P, _P],
+    "lb_grad_scale": [_I, _P, _P, _P, _P, _P, _I, _F, _F, _P, _P],
     "lb_flash_fwd": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _L, _L, _L, _L, _F, _I, _P],
     "lb_flash_fwd_tc": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _L, _L, _L, _L, _F, _I, _P],
     "lb_flash_status": [_P],
@@ -198,6 +207,24 @@ def stream_ptr() -> int:
     if _raw_stream is None:
         return torch.cuda.current_stream().cuda_stream
     return _raw_stream(_current_device())
+
+
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_HERE = _Here()
+
+
+def on_device(t: torch.Tensor):
+    """Context in which launches and ``stream_ptr()`` go to the tensor's device (nothing to do where it is the current one)."""
+    if t.device.index == (torch.cuda.current_device() if _raw_stream is None else _current_device()):
+        return _HERE
+    return torch.cuda.device(t.device)
 
 
 def flash_bwd_workspace(B: int, Sq: int, hq: int, d: int, device, kv=None) -> torch.Tensor:

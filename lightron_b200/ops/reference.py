@@ -93,6 +93,79 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     return o
 
 
+def mask_bounds(S: int, documents: Optional[torch.Tensor], prefix: Optional[torch.Tensor], causal: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Intervals of ``functional.attention_mask``: keys [lo, hi) that a position sees, positions [lo, hi) that see a key, both [B, S, 2] int32.
+    ``documents`` [B, S] ids or None, ``prefix`` [B, S] marks, [B] lengths or None."""
+    B, dev = (documents if documents is not None else prefix).shape[0], (documents if documents is not None else prefix).device
+    i = torch.arange(S, device=dev).expand(B, S)
+    ids = documents if documents is not None else torch.zeros(B, S, dtype=torch.int32, device=dev)
+    first = torch.ones(B, S, dtype=torch.bool, device=dev)
+    first[:, 1:] = ids[:, 1:] != ids[:, :-1]
+    start = torch.where(first, i, -1).cummax(dim=1).values
+    after = torch.cat((torch.where(first, i, S)[:, 1:], torch.full((B, 1), S, device=dev)), dim=1)
+    end = after.flip(1).cummin(dim=1).values.flip(1)
+    if prefix is None:
+        part = start
+    else:
+        marks = prefix.bool() if prefix.dim() == 2 else i < prefix[:, None]
+        plain = torch.where(marks, S, i).flip(1).cummin(dim=1).values.flip(1)          # first position from here on that is not marked
+        part = torch.minimum(plain.gather(1, start), end)
+    hi = torch.maximum(i + 1, part) if causal else end
+    q = torch.stack((start, hi), dim=-1)
+    k = torch.stack((torch.where(i < part, start, i) if causal else start, end), dim=-1)
+    pad = torch.stack((i, i), dim=-1)
+    hide = (ids < 0)[..., None]
+    return torch.where(hide, pad, q).int(), torch.where(hide, pad, k).int()
+
+
+def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bounds: Optional[torch.Tensor] = None, causal: bool = True,
+                     scale: Optional[float] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """q [B, Sq, hq, d], k / v [B, Sk, hkv, d]; query i sits at position i + Sk - Sq and sees the keys of ``bounds`` [B, Sk, 2] there (None:
+    all keys, with ``causal`` those up to its own).  Scores are ``softcap * tanh(x / softcap) - slopes[h] * distance``; fp32 math."""
+    B, Sq, hq, d = q.shape
+    Sk, hkv = k.shape[1], k.shape[2]
+    scale = 1.0 / math.sqrt(d) if scale is None else scale
+    dt = torch.float64 if q.dtype == torch.float64 else torch.float32
+    qf = q.to(dt).permute(0, 2, 1, 3).reshape(B, hkv, hq // hkv, Sq, d)
+    kf, vf = k.to(dt).permute(0, 2, 1, 3), v.to(dt).permute(0, 2, 1, 3)
+    s = torch.einsum("bgrqd,bgkd->bgrqk", qf, kf) * scale
+    if softcap:
+        s = softcap * torch.tanh(s / softcap)
+    at, key = torch.arange(Sk - Sq, Sk, device=q.device), torch.arange(Sk, device=q.device)
+    if slopes is not None:
+        s = s - slopes.to(dt).view(hkv, hq // hkv, 1, 1) * (at[:, None] - key[None, :]).abs()
+    if bounds is not None:
+        row = bounds[:, Sk - Sq:].to(q.device)
+        see = ((key >= row[..., :1]) & (key < row[..., 1:]))[:, None, None]
+    else:
+        see = (key[None, :] <= at[:, None]) if causal else torch.ones(Sq, Sk, dtype=torch.bool, device=q.device)
+        see = see[None, None, None]
+    s = s.masked_fill(~see, float("-inf"))
+    top = s.amax(dim=-1, keepdim=True).detach() if Sk else s.new_zeros(*s.shape[:-1], 1)
+    e = torch.exp(s - torch.where(top == float("-inf"), torch.zeros_like(top), top))
+    total = e.sum(dim=-1, keepdim=True)
+    p = e / torch.where(total == 0, torch.ones_like(total), total)                       # rows that see nothing: zero
+    o = torch.einsum("bgrqk,bgkd->bgrqd", p, vf)
+    return o.reshape(B, hq, Sq, d).permute(0, 2, 1, 3).to(q.dtype)
+
+
+def rope_axes(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, axes, inverse: bool = False) -> torch.Tensor:
+    """x [B, S, h, d]; pair i turns by the table row ``positions[axes[i]]`` ([A, B, S] or [A, S]) of its token."""
+    axis, pair = torch.as_tensor(axes, device=x.device), torch.arange(x.shape[-1] // 2, device=x.device)
+    at = positions.long()[axis]                                                          # [d/2, (B,) S]
+    at = (at if at.dim() == 3 else at[:, None]).permute(1, 2, 0)
+    c, s = cos[at, pair][:, :, None], sin[at, pair][:, :, None]
+    s = -s if inverse else s
+    a, b = x.to(c.dtype)[..., 0::2], x.to(c.dtype)[..., 1::2]
+    return torch.stack((a * c - b * s, a * s + b * c), dim=-1).flatten(-2).type_as(x)
+
+
+def grad_sumsq(tensors) -> torch.Tensor:
+    """Sum of the squares of all elements of all tensors, fp32."""
+    parts = [t.detach().float().square().sum() for t in tensors]
+    return torch.stack(parts).sum() if parts else torch.zeros(())
+
+
 def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
     """Token-mean NLL over [T, V] logits (fp32 math)."""
     return F.cross_entropy(logits.float(), targets, reduction="mean", ignore_index=ignore_index)
