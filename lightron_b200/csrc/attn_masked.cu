@@ -102,53 +102,11 @@ __device__ __forceinline__ float ma_score(const MaParams& p, float qk, int away,
   float s = qk * p.scale;
   dcap = 1.f;
   if (p.softcap > 0.f) {
-    const float t = tanhf(s / p.softcap);
+    const float t = 1.f - __fdividef(2.f, exp2f(s / p.softcap * (2.f * LOG2E)) + 1.f);
     s = p.softcap * t;
     dcap = 1.f - t * t;
   }
   return s - slope * (float)abs(away);
-}
-
-__global__ void ma_fwd_rows_kernel(const MaParams p) {
-  const long long row = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (row >= (long long)p.B * p.hq * p.Sq) return;
-  const int lane = threadIdx.x & 31, i = (int)(row % p.Sq), h = (int)(row / p.Sq % p.hq), b = (int)(row / p.Sq / p.hq), g = h / (p.hq / p.hkv);
-  const bf16* q = p.q + b * p.qs.b + i * p.qs.s + h * p.qs.h;
-  const bf16 *k = p.k + b * p.ks.b + g * p.ks.h, *v = p.v + b * p.vs.b + g * p.vs.h;
-  const int2 r = ma_keys(p, b, i);
-  const float slope = p.slopes ? p.slopes[h] : 0.f;
-  const bool mine = lane * 4 < p.d;
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int j0 = r.x; j0 < r.y; j0 += 32) {
-    const int j = j0 + lane;
-    float s = -INFINITY, dc;
-    if (j < r.y) s = ma_score(p, dot_row(q, k + j * p.ks.s, p.d), i + p.Sk - p.Sq - j, slope, dc);
-    const float mn = fmaxf(m, warp_max(s));
-    const float e = j < r.y ? exp2f((s - mn) * LOG2E) : 0.f, c = m == -INFINITY ? 0.f : exp2f((m - mn) * LOG2E);
-    m = mn;
-    l = l * c + warp_sum(e);
-#pragma unroll
-    for (int x = 0; x < 4; x++) o[x] *= c;
-    for (int n = 0; n < min(32, r.y - j0); n++) {
-      const float pn = __shfl_sync(0xffffffffu, e, n);
-      if (mine) {
-        float f[4];
-        load4(v + (j0 + n) * p.vs.s + lane * 4, f);
-#pragma unroll
-        for (int x = 0; x < 4; x++) o[x] += pn * f[x];
-      }
-    }
-  }
-  const float inv = l != 0.f ? 1.f / l : 0.f;
-  if (mine) {
-    const long long at = (((long long)b * p.Sq + i) * p.hq + h) * p.d + lane * 4;
-    float hi[4];
-#pragma unroll
-    for (int x = 0; x < 4; x++) { o[x] *= inv; hi[x] = __bfloat162float(__float2bfloat16(o[x])); o[x] -= hi[x]; }
-    store4(p.o + at, hi);
-    if (p.o_lo) store4(p.o_lo + at, o);
-  }
-  if (lane == 0) p.lse[row] = r.x < r.y ? m + logf(l) : -INFINITY;
 }
 
 // D of a row, then dQ.
@@ -271,11 +229,7 @@ extern "C" int lb_masked_attn_fwd(const void* q, const void* k, const void* v, v
                                   void* stream) {
   MaParams p;
   if (const int rc = fill(p, q, k, v, o, o_lo, lse, B, Sq, Sk, hq, hkv, d, strides, scale, causal, softcap, slopes, q_bounds, k_bounds)) return rc;
-  const long long rows = (long long)B * hq * Sq;
-  if ((rows + 3) / 4 > 2147483647LL) return LB_ERR_SHAPE;
-  ma_fwd_rows_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, (cudaStream_t)stream>>>(p);
-  LB_CHECK_LAUNCH();
-  return LB_OK;
+  return ma_launch_fwd(p, (cudaStream_t)stream);
 }
 
 extern "C" long long lb_masked_attn_bwd_ws_bytes(int B, int Sq, int Sk, int hq, int hkv, int d) {

@@ -32,6 +32,8 @@ struct MaBwdParams {
   float* stats;
 };
 
+int ma_launch_fwd(const MaParams& p, cudaStream_t s);
+
 // Keys [x, y) that query i of sequence b sees.
 __device__ __forceinline__ int2 ma_keys(const MaParams& p, int b, int i) {
   const int at = i + p.Sk - p.Sq;

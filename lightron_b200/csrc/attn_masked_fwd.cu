@@ -1,0 +1,618 @@
+// Forward of attention under interval masks (attn_masked.cuh) on the 5th-generation tensor cores, head_dim up to 128 (a multiple of 8, in
+// tiles of 64 or 128 columns).
+//
+// A CTA works on one tile of 128 queries of one (batch, head) at a time, two CTAs per SM; S = Q K^T and O += P V by tcgen05.mma with S, P and O in tensor
+// memory, a softmax thread per query row, K and V by TMA through a ring of 16 KB slots, further tiles by cluster launch control: the pipeline of the causal
+// forward (flash_fwd_tcgen05.cu has what each part of it is worth).  What is different here:
+//   * the keys of a tile run from the first key of its first row to the last key of its last (the ends never fall), from exactly there: blocks start
+//     at any key, so that a document of n keys takes ceil(n / 128) of them wherever it lies.  Blocks inside all 32 intervals of a warp are not masked.
+//   * with a cap the scores are known to lie within it.  Up to softcap * log2(e) = 80 exponentials are taken relative to zero instead of the running
+//     maximum: 2^+-80 and sums of them are far inside fp32 (and bf16 has the same exponents), nothing is ever rescaled, and the first half of
+//     P leaves before the second is looked at.  Above it the maximum is kept.
+//   * tanh: where no score of 32 rows x 64 columns is above 0.6 caps, x times a polynomial in x^2 on the FMA pipe, two at a time (relative error
+//     2.1e-6, found by least squares with re-weighted points; 7e-5 of a score at most); else by its definition with exp2, whose units the softmax needs itself.
+//   * the bias is an addend of the same FMA, counted up along the columns; only where a block holds keys on both sides of a row is its distance made per column.
+//   * a row's sum is that of its weights as they are rounded for P V.  A row that all but one key leave cold has o = v of that key then, and a D = do . o whose
+//     error is as small as the differences dP - D that the backward lives on (the weight's own rounding, 2^-9 of dP, would drown them).
+//   * o leaves twice: rounded, and what the rounding left (for the backward's row sums).
+// All waits are bounded; on expiry a status word is set and the CTA drains and frees its TMEM.
+#include "attn_masked.cuh"
+#include "tcgen05.cuh"
+
+static __device__ unsigned int g_ma_status[4] = {0, 0, 0, 0};
+
+namespace {
+using namespace bw;
+
+constexpr int THREADS = 256;
+// Registers per thread of the two warpgroups (two CTAs of 256 threads leave 128 per thread at launch).
+constexpr int REGS_ISSUE = 56, REGS_SOFTMAX = 200;
+static_assert(REGS_ISSUE + REGS_SOFTMAX <= 2 * 128, "a CTA has 256 x 128 registers");
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct FwdParams {
+  MaParams a;
+  int tiles_x;                   // query tiles (128 rows) per (batch, head)
+  int steal;                     // CTAs go on with entries that have not been started
+  int group;                     // (batch, head) pairs whose tiles are ordered together
+  FastDiv by_grp, by_group, by_last, by_hq, by_rep;    // entries of a group, heads of a group / of the last one, hq, hq / hkv
+  // scores in units of log2: x * scale_l2 without a cap; with one x * (c[0] + c[1] x^2 + ..) while |x| <= limit, else cap_l2 * tanh(x * by_cap)
+  float scale_l2, by_cap, cap_l2, limit, c[4];
+};
+
+enum : int { NO_CAP, CAP_ZERO, CAP_MAX };      // CAP_ZERO: exponentials relative to zero, CAP_MAX: to the running maximum
+
+template <int D>
+struct Cfg {
+  static constexpr int BM = 128, BN = 128;
+  static constexpr int ATOMS = D / 64;
+  static constexpr int SLOT_BYTES = 128 * 128;          // K: 128 keys x 64 columns; V: 128 keys x 64 columns or 64 keys x 128 columns
+  static constexpr int SLOTS = 6 - ATOMS;
+  static constexpr int UNITS = 2 * ATOMS;               // slots that a key block takes, K before V
+  // TMEM columns: S fp32 [128], O fp32 [D], P packed bf16 [64]; with 128 columns of O, P takes the first half of S's
+  static constexpr bool P_ALIAS = (D == 128);
+  static constexpr int COL_S = 0, COL_O = 128, COL_P = P_ALIAS ? 0 : 192, TMEM_COLS = 256;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_RING = OFF_Q + ATOMS * SLOT_BYTES;
+  static constexpr int OFF_OUT = OFF_RING + SLOTS * SLOT_BYTES;   // 64 columns of O on their way out, 4 KB per softmax warp
+  static constexpr int OFF_BAR = OFF_OUT + SLOT_BYTES;
+  static constexpr int NBAR = 2 + 2 * SLOTS + 9;
+  static constexpr int SMEM = OFF_BAR + 256;
+};
+static_assert(Cfg<64>::SMEM <= 115712 && Cfg<128>::SMEM <= 115712, "two CTAs per SM");
+
+// Bits [lo, hi) of 32 columns, of which column 0 is at `at`.
+__device__ __forceinline__ uint32_t visible_bits(int lo, int hi, int at) {
+  const int a = min(max(lo - at, 0), 32), e = min(max(hi - at, 0), 32);
+  const uint32_t below_e = e == 32 ? 0xffffffffu : (1u << e) - 1u, below_a = a == 32 ? 0xffffffffu : (1u << a) - 1u;
+  return below_e & ~below_a;
+}
+
+// 64 raw scores to units of log2, capped and lowered with distance.  `first`: key of column 0 less the row's position; `side`: the columns lie on the row's left (1),
+// on its right (-1) or on both sides (0), the same for all lanes.
+template <int CAP, bool BIAS>
+__device__ __forceinline__ void scores64(uint32_t* r, const FwdParams& p, float slope2, int side, int first) {
+  bool small = true;
+  if constexpr (CAP != NO_CAP) {
+    float top[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 64; i += 2) top[(i >> 1) & 3] = max3abs(top[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+    small = __all_sync(0xffffffffu, max2(max2(top[0], top[1]), max2(top[2], top[3])) <= p.limit);
+  }
+  const float slope = side < 0 ? -slope2 : slope2;
+  const float step1 = side ? 2.f * slope : 0.f;
+  const f32x2 step = pack2(step1, step1);
+#pragma unroll
+  for (int c0 = 0; c0 < 64; c0 += 32) {
+    // (counted up anew every 32 columns: its rounding errors do not pile up)
+    const float base = slope * (float)(first + c0);
+    f32x2 add = BIAS && side ? pack2(base, base + slope) : pack2(0.f, 0.f);
+    if (CAP == NO_CAP || small) {
+      const f32x2 k0 = pack2(p.c[0], p.c[0]), k1 = pack2(p.c[1], p.c[1]), k2 = pack2(p.c[2], p.c[2]), k3 = pack2(p.c[3], p.c[3]);
+#pragma unroll
+      for (int i = c0; i < c0 + 32; i += 2) {
+        const f32x2 x = pack2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+        f32x2 f = k0;
+        if constexpr (CAP != NO_CAP) {
+          const f32x2 w = mul2(x, x);
+          f = fma2(w, fma2(w, fma2(w, k3, k2), k1), k0);
+        }
+        f32x2 y;
+        if constexpr (BIAS) {
+          y = fma2(x, f, add);
+          add = add2(add, step);
+        } else {
+          y = mul2(x, f);
+        }
+        float y0, y1;
+        unpack2(y, y0, y1);
+        r[i] = __float_as_uint(y0);
+        r[i + 1] = __float_as_uint(y1);
+      }
+    } else if constexpr (CAP != NO_CAP) {
+      const float by = 2.f * LOG2E * p.by_cap;
+#pragma unroll
+      for (int i = c0; i < c0 + 32; i += 2) {
+        float a0, a1;
+        unpack2(add, a0, a1);
+        if constexpr (BIAS) add = add2(add, step);
+        // tanh u = 1 - 2 / (exp 2u + 1)
+        const float t0 = 1.f - __fdividef(2.f, exp2f(__uint_as_float(r[i]) * by) + 1.f), t1 = 1.f - __fdividef(2.f, exp2f(__uint_as_float(r[i + 1]) * by) + 1.f);
+        r[i] = __float_as_uint(fmaf(p.cap_l2, t0, a0));
+        r[i + 1] = __float_as_uint(fmaf(p.cap_l2, t1, a1));
+      }
+    }
+  }
+  if (BIAS && side == 0) {
+    const float d0 = (float)first;
+#pragma unroll
+    for (int i = 0; i < 64; i++) r[i] = __float_as_uint(fmaf(-slope2, fabsf(d0 + (float)i), __uint_as_float(r[i])));
+  }
+}
+
+template <int D, int CAP, bool BIAS>
+__global__ void __launch_bounds__(THREADS, 2)
+ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to,
+              const __grid_constant__ CUtensorMap to_lo, const __grid_constant__ FwdParams pp) {
+  using C = Cfg<D>;
+  constexpr bool MADE = CAP != NO_CAP || BIAS;        // scores are made in units of log2 ahead of the softmax
+  const MaParams& p = pp.a;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::NBAR + 5);     // behind two 16-byte answers
+  int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);     // {abort, extra wait in ms}: see bw::mbar_wait
+
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // (uniform over the warp)
+  const uint32_t sbase = smem_u32(smem);
+  if (sbase & 1023u) {                                       // the swizzled tiles need it; nothing has been started yet
+    if (threadIdx.x == 0) atomicExch(&g_ma_status[0], 4u);
+    return;
+  }
+  const uint32_t bar0 = smem_u32(bars);
+  const uint32_t q_full = bar0, q_empty = bar0 + 8;
+  auto full = [&](int s) { return bar0 + 8u * (2 + s); };
+  auto empty = [&](int s) { return bar0 + 8u * (2 + C::SLOTS + s); };
+  const uint32_t bar1 = bar0 + 8u * (2 + 2 * C::SLOTS);
+  const uint32_t s_full = bar1, s_free = bar1 + 8, p_half = bar1 + 16, p_full = bar1 + 24, pv_done = bar1 + 32;   // p_half: P of 64 keys
+  auto next_full = [&](int i) { return bar1 + 40u + 8u * i; };
+  auto next_empty = [&](int i) { return bar1 + 56u + 8u * i; };
+  const uint32_t next_slot = (bar0 + 8u * C::NBAR + 15u) & ~15u;
+
+  // One entry per (batch, head, query tile): the last tiles, which see most under a causal mask, of all heads of a group first; a group is as many heads as keep
+  // their K / V in L2 together.  A resident CTA goes on with entries that have not been started (cluster launch control).
+  volatile int* abort_flag = s_abort;
+  const int off = p.Sk - p.Sq;
+  struct Tile { int m0, b, h, hk, key0, nb; };
+  auto tile_of = [&](int cid) {
+    Tile t;
+    const int grp = pp.by_grp.div(cid);
+    const int in_grp = cid - grp * (int)pp.by_grp.d;
+    const FastDiv& heads = (grp + 1) * pp.group <= p.hq * p.B ? pp.by_group : pp.by_last;
+    const int row = heads.div(in_grp);
+    const int bh = grp * pp.group + in_grp - row * (int)heads.d;
+    t.m0 = (pp.tiles_x - 1 - row) * C::BM;
+    t.b = pp.by_hq.div(bh);
+    t.h = bh - t.b * p.hq;
+    t.hk = pp.by_rep.div(t.h);
+    t.key0 = ma_keys(p, t.b, t.m0).x;
+    // (a tile whose rows see nothing takes one block, all of it hidden)
+    t.nb = max((ma_keys(p, t.b, min(t.m0 + C::BM, p.Sq) - 1).y - t.key0 + C::BN - 1) / C::BN, 1);
+    return t;
+  };
+  // Entry n + 1 of this CTA: the answer to request n, or -1 at the end.
+  auto next_cta = [&](int n) -> int {
+    if (!pp.steal || !mbar_wait(next_full(n & 1), (uint32_t)(n >> 1) & 1u, abort_flag)) return -1;
+    const int cta = cancel_result(next_slot + 16u * (n & 1));
+    fence_proxy_async_smem();
+    return cta;
+  };
+
+  if (threadIdx.x == 0) {
+    s_abort[0] = s_abort[1] = 0;
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int s = 0; s < C::SLOTS; s++) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+    mbar_init(s_full, 1);
+    mbar_init(pv_done, 1);
+    mbar_init(s_free, 4);
+    mbar_init(p_half, 4);
+    mbar_init(p_full, 4);
+    for (int i = 0; i < 2; i++) { mbar_init(next_full(i), 1); mbar_init(next_empty(i), 5); }   // the issuer and four softmax warps read
+    mbar_init_fence();
+    prefetch_tmap(&tq); prefetch_tmap(&tk); prefetch_tmap(&tv); prefetch_tmap(&to); prefetch_tmap(&to_lo);
+  }
+  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  if (!pp.steal) grid_go();
+  grid_wait();
+
+  if (warp < 4) {
+    reg_dec<REGS_ISSUE>();
+    if (warp == 0) {
+      // ------------------------------- TMA producer -------------------------------
+      if (elect_one()) {
+        bool ok = true;
+        int slot = 0;
+        uint32_t phase = 0;
+        int asked = 0;
+        for (int n = 0, cta = (int)blockIdx.x; ok && cta >= 0; n++) {
+          if (pp.steal) {
+            if (!mbar_wait(next_empty(n & 1), ((uint32_t)(n >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+            mbar_expect_tx(next_full(n & 1), 16);
+            cancel_next(next_slot + 16u * (n & 1), next_full(n & 1));
+            asked = n + 1;
+          }
+          const Tile t = tile_of(cta);
+          if (!mbar_wait(q_empty, (uint32_t)(n & 1) ^ 1u, abort_flag)) { ok = false; break; }
+          mbar_expect_tx(q_full, C::ATOMS * C::SLOT_BYTES);
+#pragma unroll
+          for (int a = 0; a < C::ATOMS; a++) tma_load_4d(sbase + C::OFF_Q + a * C::SLOT_BYTES, &tq, a * 64, t.h, t.m0, t.b, q_full);
+          for (int j = 0; j < t.nb && ok; j++) {
+            const int key0 = t.key0 + j * C::BN;
+#pragma unroll
+            for (int u = 0; u < C::UNITS; u++) {
+              if (ok && !mbar_wait(empty(slot), phase ^ 1u, abort_flag)) ok = false;
+              if (!ok) break;
+              const uint32_t dst = sbase + C::OFF_RING + slot * C::SLOT_BYTES, bar = full(slot);
+              mbar_expect_tx(bar, C::SLOT_BYTES);
+              if (u < C::ATOMS) {
+                tma_load_4d(dst, &tk, u * 64, t.hk, key0, t.b, bar);              // box 128 keys x 64 columns
+              } else {
+                const int half = u - C::ATOMS;                                    // 128 columns: keys 0-63, then 64-127
+#pragma unroll
+                for (int a = 0; a < 2; a++)                                       // boxes 64 keys x 64 columns
+                  tma_load_4d(dst + a * 8192, &tv, D == 128 ? a * 64 : 0, t.hk, key0 + (D == 128 ? half * 64 : a * 64), t.b, bar);
+              }
+              if (++slot == C::SLOTS) { slot = 0; phase ^= 1u; }
+            }
+          }
+          if (ok) cta = next_cta(n);
+        }
+        if (!ok) {
+          atomicExch(&g_ma_status[0], 1u);
+          if (asked) mbar_wait(next_full((asked - 1) & 1), (uint32_t)((asked - 1) >> 1) & 1u, abort_flag);   // nothing arrives after the CTA's end
+        }
+      }
+    } else if (warp == 1) {
+      // ------------------------------- MMA issuer -------------------------------
+      // Per tile S(0); then per key block, 64 columns: S(j+1) as soon as the softmax threads hold S(j) in registers, and P(j) V in two halves as
+      // P(j) arrives; 128 columns: P(j) V, then S(j+1) into the columns that P(j) leaves.
+      if (elect_one()) {
+        const uint32_t idesc_s = make_idesc(C::BM, C::BN, 0, 0);
+        const uint32_t idesc_o = make_idesc(C::BM, D, 0, 1);
+        const uint64_t qa = make_desc(sbase + C::OFF_Q, 16, 1024);
+        const uint64_t dk0 = make_desc(sbase + C::OFF_RING, 16, 1024);
+        const uint64_t dv0 = make_desc(sbase + C::OFF_RING, 8192, 1024);
+        const uint32_t s_dst = tmem_base + C::COL_S, o_dst = tmem_base + C::COL_O, pa = tmem_base + C::COL_P;
+        bool ok = true;
+        // slots are taken in load order: K (ATOMS slots), then V of every block
+        auto ring = [&](int& slot, uint32_t& phase, int step) { slot += step; if (slot >= C::SLOTS) { slot -= C::SLOTS; phase ^= 1u; } };
+        int ks = 0, vs = C::ATOMS;                      // next slot of K and of V, and their phases
+        uint32_t kp = 0, vp = 0;
+        uint32_t g = 0;                                 // key blocks so far, over all tiles: the phase of the per-block barriers
+        auto k_ready = [&]() -> bool {                  // the next block's K has arrived
+          if (!mbar_wait(full(ks), kp, abort_flag)) return false;
+          if (C::ATOMS == 1) return true;
+          const bool wrap = ks + 1 == C::SLOTS;
+          return mbar_wait(full(wrap ? 0 : ks + 1), wrap ? kp ^ 1u : kp, abort_flag);
+        };
+        auto issue_s = [&](bool last) {                 // S = Q K^T of the next block (K is there), then release its slots of K (and Q)
+          fence_after();
+#pragma unroll
+          for (int a = 0; a < C::ATOMS; a++) {
+            const uint64_t ka = dk0 + (uint64_t)((ks * C::SLOT_BYTES) >> 4);
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+              umma_bf16(s_dst, qa + (uint64_t)((a * C::SLOT_BYTES + s * 32) >> 4), ka + (uint64_t)((s * 32) >> 4), idesc_s, (a | s) ? 1u : 0u);
+            if (a == C::ATOMS - 1) umma_commit(s_full);
+            umma_commit(empty(ks));
+            ring(ks, kp, a == C::ATOMS - 1 ? C::UNITS - C::ATOMS + 1 : 1);
+          }
+          if (last) umma_commit(q_empty);
+        };
+        auto issue_pv = [&](bool first, bool last) -> bool {      // O += P V of block g, then release its slots of V
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            if ((D == 128 || half == 0) && !mbar_wait(full(vs), vp, abort_flag)) return false;
+            if (half == 1 && C::P_ALIAS && !last && !k_ready()) return false;
+            if (!mbar_wait(half ? p_full : p_half, g & 1u, abort_flag)) return false;
+            fence_after();
+            const uint64_t va = dv0 + (uint64_t)((vs * C::SLOT_BYTES + (D == 128 ? 0 : half * 8192)) >> 4);
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+              umma_bf16_ta(o_dst, pa + 8u * (half * 4 + s), va + (uint64_t)((s * 2048) >> 4), idesc_o, (half | s) ? 1u : (first ? 0u : 1u));
+            if (half && (!C::P_ALIAS || last)) umma_commit(pv_done);
+            if (D == 128 || half) {
+              umma_commit(empty(vs));
+              ring(vs, vp, half ? C::ATOMS + 1 : 1);
+            }
+          }
+          return true;
+        };
+        for (int n = 0, cta = (int)blockIdx.x; ok && cta >= 0; n++) {
+          const Tile t = tile_of(cta);
+          ok = k_ready() && mbar_wait(q_full, (uint32_t)n & 1u, abort_flag);
+          if (ok && !C::P_ALIAS && n > 0) ok = mbar_wait(s_free, (g - 1) & 1u, abort_flag);
+          if (ok) issue_s(t.nb == 1);
+          for (int j = 0; j < t.nb && ok; j++, g++) {
+            const bool last = j + 1 == t.nb;
+            if (!C::P_ALIAS && !last) {
+              ok = k_ready() && mbar_wait(s_free, g & 1u, abort_flag);
+              if (ok) issue_s(j + 2 == t.nb);
+            }
+            if (ok) ok = issue_pv(j == 0, last);
+            if (C::P_ALIAS && ok && !last) issue_s(j + 2 == t.nb);
+          }
+          if (!ok) break;
+          cta = next_cta(n);
+          if (cta >= 0) mbar_arrive(next_empty(n & 1));
+        }
+        if (!ok) atomicExch(&g_ma_status[0], 2u);
+      }
+    }
+  } else {
+    // ------------------------------- softmax warps -------------------------------
+    reg_inc<REGS_SOFTMAX>();
+    const int quad = warp & 3;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16);
+    const uint32_t ts_addr = lane_addr + C::COL_S, to_addr = lane_addr + C::COL_O, tp_addr = lane_addr + C::COL_P;
+    const f32x2 sl2x2 = pack2(pp.scale_l2, pp.scale_l2);
+    bool ok = true;
+    auto arrive = [&](uint32_t bar) {              // once per warp
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    uint32_t g = 0;                                // key blocks so far, over all tiles
+    bool s_ready = false;                          // S of the next block was seen complete
+    for (int n = 0, cta = (int)blockIdx.x; ok && cta >= 0; n++) {
+      const Tile t = tile_of(cta);
+      const int nb = t.nb, row = t.m0 + quad * 32 + lane, warp_at = t.m0 + quad * 32 + off;      // the row's place is row + off
+      // (rows past the last one are never stored: they are left unmasked)
+      const int2 see = row < p.Sq ? ma_keys(p, t.b, row) : make_int2(0, 0x7fffffff);
+      [[maybe_unused]] float slope2 = 0.f;
+      [[maybe_unused]] bool left_only = true;      // no row of the warp sees a key behind its own
+      if constexpr (BIAS) {
+        slope2 = p.slopes ? p.slopes[t.h] * LOG2E : 0.f;
+        left_only = __all_sync(0xffffffffu, row >= p.Sq || see.y <= row + off + 1);
+      }
+      float m_i = -INFINITY, m_s = 0.f, l_i = 0.f;      // running maximum, and what exponentials are relative to
+      for (int j = 0; j < nb; j++, g++) {
+        if (!s_ready && !mbar_wait(s_full, g & 1u, abort_flag)) { ok = false; break; }
+        fence_after();
+        uint32_t r[128];
+        const int c0 = t.key0 + j * C::BN, lo = see.x - c0, hi = see.y - c0;       // visible columns
+        const bool need_mask = __any_sync(0xffffffffu, lo > 0 || hi < C::BN);
+        auto mask = [&](int i0) {
+          if (need_mask) {
+#pragma unroll
+            for (int w = i0; w < i0 + 64; w += 32) {
+              const uint32_t bits = visible_bits(lo, hi, w);
+#pragma unroll
+              for (int i = 0; i < 32; i++)
+                if (!(bits >> i & 1u)) r[w + i] = 0xff800000u;           // -inf
+            }
+          }
+        };
+        auto made = [&](int i0) {
+          if constexpr (MADE) {
+            const int side = left_only || c0 + i0 + 63 <= warp_at ? 1 : c0 + i0 >= warp_at + 31 ? -1 : 0;
+            scores64<CAP, BIAS>(r + i0, pp, slope2, side, c0 + i0 - (row + off));
+          }
+        };
+        // exponentials of 64 columns, packed as bf16 pairs (column c of P holds keys 2c, 2c+1)
+        auto exps = [&](int i0, uint32_t* pr, f32x2* rs2) {
+          const f32x2 nms2 = pack2(-m_s, -m_s);
+          rs2[0] = rs2[1] = pack2(0.f, 0.f);
+#pragma unroll
+          for (int c = 0; c < 32; c++) {
+            const int i = i0 + c * 2;
+            float e0 = __uint_as_float(r[i]), e1 = __uint_as_float(r[i + 1]);
+            // (the difference first: with the maximum scaled ahead and a fused product, what its rounding left would be the exponent of scores far from zero)
+            if constexpr (CAP != CAP_ZERO) {
+              f32x2 x = add2(pack2(e0, e1), nms2);
+              if constexpr (!MADE) x = mul2(x, sl2x2);
+              unpack2(x, e0, e1);
+            }
+            e0 = exp2f(e0);
+            e1 = exp2f(e1);
+            bf162 pk = __floats2bfloat162_rn(e0, e1);
+            pr[c] = *reinterpret_cast<uint32_t*>(&pk);
+            rs2[c & 1] = add2(rs2[c & 1], pack2(__uint_as_float(pr[c] << 16), __uint_as_float(pr[c] & 0xffff0000u)));
+          }
+        };
+        auto row_max = [&]() {                           // four independent chains
+          float mx4[4] = {m_i, m_i, m_i, m_i};
+#pragma unroll
+          for (int i = 0; i < 128; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+          return max2(max2(mx4[0], mx4[1]), max2(mx4[2], mx4[3]));
+        };
+        tmem_ld32(ts_addr, r);
+        tmem_ld32(ts_addr + 32, r + 32);
+        tmem_ld32(ts_addr + 64, r + 64);
+        tmem_ld32(ts_addr + 96, r + 96);
+        tmem_ld_wait();
+        if (!C::P_ALIAS) arrive(s_free);                 // S may be overwritten by the next key block
+        uint32_t pr[32];
+        f32x2 rs2[2], rt2[2];
+        const bool pv_ready = !C::P_ALIAS && j > 0 && mbar_test_wait(pv_done, (g - 1) & 1u);   // asked ahead of its use
+        bool any_grow = false;
+        float corr = 1.f;
+        made(0);
+        mask(0);
+        if constexpr (CAP == CAP_ZERO) {
+          exps(0, pr, rs2);
+        } else {
+          // Lazy reference maximum: the old one stays unless the new maximum is more than 2^8 above it, so that O and l rarely need rescaling.  So the
+          // first 64 exponentials are computed with the old one, and once more in the rare block where it may not stay.
+          made(64);
+          mask(64);
+          const float unit = MADE ? 1.f : pp.scale_l2;
+          if (j > 0) exps(0, pr, rs2);
+          float m_new = row_max();
+          const bool grow = !(m_i != -INFINITY && (m_new - m_i) * unit <= 8.f);
+          any_grow = __any_sync(0xffffffffu, grow);
+          if (any_grow) {
+            if (!grow) m_new = m_i;
+            // (a row with a score of +inf has no softmax: NaN, as inf - inf gives)
+            m_s = (m_new == -INFINITY) ? 0.f : (m_new == INFINITY ? __int_as_float(0x7fffffff) : m_new);
+            corr = (m_i == -INFINITY) ? 0.f : exp2f((m_i - m_s) * unit);
+            l_i *= corr;
+            m_i = m_new;
+            exps(0, pr, rs2);
+          }
+        }
+        if (j > 0) {
+          // previous P V finished: O is stable and the P columns may be overwritten.  (128 columns: S(j) was issued behind it by the same thread, so
+          // its completion says that P V has completed too.)
+          if (!C::P_ALIAS) {
+            if (!pv_ready && !mbar_wait(pv_done, (g - 1) & 1u, abort_flag)) { ok = false; break; }
+            fence_after();
+          }
+          if (CAP != CAP_ZERO && any_grow) {
+#pragma unroll 1
+            for (int c = 0; c < D / 32; c++) {
+              uint32_t o[32];
+              tmem_ld32(to_addr + c * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              tmem_st32(to_addr + c * 32, o);
+            }
+            tmem_st_wait();
+          }
+        }
+        // P goes back to TMEM, the first half in flight while the second is computed
+        tmem_st32(tp_addr, pr);
+        tmem_st_wait();
+        arrive(p_half);
+        s_ready = !C::P_ALIAS && j + 1 < nb && mbar_test_wait(s_full, (g + 1) & 1u);
+        if constexpr (CAP == CAP_ZERO) {
+          made(64);
+          mask(64);
+        }
+        exps(64, pr, rt2);
+        tmem_st32(tp_addr + 32, pr);
+        tmem_st_wait();
+        arrive(p_full);
+        rs2[0] = add2(rs2[0], rt2[0]);
+        rs2[1] = add2(rs2[1], rt2[1]);
+        float rs[4];
+        unpack2(rs2[0], rs[0], rs[1]);
+        unpack2(rs2[1], rs[2], rs[3]);
+        l_i += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+      }
+      if (ok) {
+        cta = next_cta(n);
+        __syncwarp();
+        if (lane == 0 && cta >= 0) mbar_arrive(next_empty(n & 1));
+      }
+      if (ok && !mbar_wait(pv_done, C::P_ALIAS ? (uint32_t)n & 1u : (g - 1) & 1u, abort_flag)) ok = false;
+      if (!ok) break;
+      fence_after();
+      const float inv = l_i != 0.f ? 1.f / l_i : 0.f;
+      // 64 columns at a time through shared memory and TMA stores, which leave out rows past the last and columns past head_dim
+      uint8_t* out = smem + C::OFF_OUT + quad * 4096;
+#pragma unroll
+      for (int c = 0; c < C::ATOMS; c++) {
+        uint32_t r[64];
+        tmem_ld32(to_addr + c * 64, r);
+        tmem_ld32(to_addr + c * 64 + 32, r + 32);
+        tmem_ld_wait();
+        auto leave = [&](const CUtensorMap* map) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && t.m0 + quad * 32 < p.Sq) {
+            tma_store_4d(map, smem_u32(out), c * 64, t.h, t.m0 + quad * 32, t.b);
+            bulk_commit();
+          }
+        };
+        if (lane == 0) bulk_wait_read_but<0>();
+        __syncwarp();
+#pragma unroll
+        for (int g8 = 0; g8 < 8; g8++) {
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) f[i] = __uint_as_float(r[g8 * 8 + i]) * inv;
+          const uint4 hi = pack8(f);
+          *reinterpret_cast<uint4*>(out + sw128_off(lane, g8)) = hi;
+          float back[8];
+          unpack8(hi, back);
+#pragma unroll
+          for (int i = 0; i < 8; i++) r[g8 * 8 + i] = __float_as_uint(f[i] - back[i]);
+        }
+        leave(&to);
+        if (p.o_lo) {
+          if (lane == 0) bulk_wait_read_but<0>();
+          __syncwarp();
+#pragma unroll
+          for (int g8 = 0; g8 < 8; g8++) *reinterpret_cast<uint4*>(out + sw128_off(lane, g8)) = pack8(reinterpret_cast<const float*>(r) + g8 * 8);
+          leave(&to_lo);
+        }
+      }
+      if (row < p.Sq) p.lse[((long long)t.b * p.hq + t.h) * p.Sq + row] = l_i != 0.f ? m_s * (MADE ? LN2 : p.scale) + logf(l_i) : -INFINITY;
+    }
+    if (lane == 0) bulk_wait_read_but<0>();        // nothing reads shared memory after the CTA's end
+    if (!ok && lane == 0) atomicExch(&g_ma_status[0], 3u);
+  }
+
+  fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    fence_after();
+    tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+template <int D, int CAP, bool BIAS>
+int launch(const CUtensorMap* maps, const FwdParams& p, unsigned grid, cudaStream_t s) {
+  using C = Cfg<D>;
+  auto fn = ma_fwd_kernel<D, CAP, BIAS>;
+  static bool attr = false;
+  if (!attr) {
+    // the register split must fit in what the launch allocates, or it would wait for registers that nobody gives back
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, fn) != cudaSuccess || (fa.numRegs + 7) / 8 * 8 * 2 < REGS_ISSUE + REGS_SOFTMAX) return LB_ERR_LAUNCH;
+    cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    attr = true;
+  }
+  return lb_launch(fn, grid, THREADS, C::SMEM, s, maps[0], maps[1], maps[2], maps[3], maps[4], p);
+}
+
+template <int D>
+int launch_fwd(const MaParams& a, cudaStream_t s) {
+  CUtensorMap maps[5];      // q, k, v, o, o_lo
+  int rc;
+  const uint64_t B = a.B, Sq = a.Sq, Sk = a.Sk, hq = a.hq, hkv = a.hkv, d = a.d;
+  if ((rc = make_map_bf16_4d(maps, a.q, d, hq, Sq, B, a.qs.h, a.qs.s, a.qs.b, 128))) return rc;
+  if ((rc = make_map_bf16_4d(maps + 1, a.k, d, hkv, Sk, B, a.ks.h, a.ks.s, a.ks.b, 128))) return rc;
+  if ((rc = make_map_bf16_4d(maps + 2, a.v, d, hkv, Sk, B, a.vs.h, a.vs.s, a.vs.b, 64))) return rc;
+  if ((rc = make_map_bf16_4d(maps + 3, a.o, d, hq, Sq, B, d, hq * d, Sq * hq * d, 32))) return rc;
+  if ((rc = make_map_bf16_4d(maps + 4, a.o_lo ? a.o_lo : a.o, d, hq, Sq, B, d, hq * d, Sq * hq * d, 32))) return rc;
+  FwdParams p;
+  p.a = a;
+  p.tiles_x = (a.Sq + 127) / 128;
+  // heads ordered together: as many as have their K / V in 48 MB (of 126 MB of L2), whole GQA groups
+  const long long kv_bytes = 4LL * D * a.Sk, pairs = (long long)a.hq * a.B;
+  const long long kv_heads = kv_bytes >= (48LL << 20) ? 1 : (48LL << 20) / kv_bytes;
+  p.group = (int)(kv_heads * (a.hq / a.hkv) < pairs ? kv_heads * (a.hq / a.hkv) : pairs);
+  const long long grid = p.tiles_x * pairs;
+  if (grid > 2147483647LL) return LB_ERR_SHAPE;
+  p.by_grp.set((unsigned)(p.tiles_x * p.group));
+  p.by_group.set((unsigned)p.group);
+  p.by_last.set((unsigned)(pairs % p.group ? pairs % p.group : p.group));
+  p.by_hq.set((unsigned)a.hq);
+  p.by_rep.set((unsigned)(a.hq / a.hkv));
+  p.steal = grid > 2 * lb_num_sms();      // (with all tiles resident at once there is none to take)
+  p.scale_l2 = p.c[0] = a.scale * LOG2E;
+  p.by_cap = p.cap_l2 = p.limit = p.c[1] = p.c[2] = p.c[3] = 0.f;
+  if (a.softcap > 0.f) {
+    const double by = (double)a.scale / a.softcap, l2 = (double)a.softcap * 1.4426950408889634;
+    const double k[4] = {0.9999978542327881, -0.33314040303230286, 0.13057856261730194, -0.04092942178249359};      // tanh(u) / u in u^2, |u| <= 0.6
+    p.by_cap = (float)by;
+    p.cap_l2 = (float)l2;
+    p.limit = (float)(0.6 / fabs(by));      // (a scale of zero: no limit)
+    double pw = by * l2;
+    for (int i = 0; i < 4; i++, pw *= by * by) p.c[i] = (float)(k[i] * pw);
+  }
+  const bool bias = a.slopes != nullptr;
+  if (a.softcap <= 0.f) return bias ? launch<D, NO_CAP, true>(maps, p, (unsigned)grid, s) : launch<D, NO_CAP, false>(maps, p, (unsigned)grid, s);
+  if (p.cap_l2 <= 80.f) return bias ? launch<D, CAP_ZERO, true>(maps, p, (unsigned)grid, s) : launch<D, CAP_ZERO, false>(maps, p, (unsigned)grid, s);
+  return launch<D, CAP_MAX, true>(maps, p, (unsigned)grid, s);
+}
+
+}  // namespace
+
+int ma_launch_fwd(const MaParams& p, cudaStream_t s) { return p.d <= 64 ? launch_fwd<64>(p, s) : launch_fwd<128>(p, s); }
+
+// Copies the status words of the forward to host memory and clears them.
+extern "C" int lb_masked_attn_status(void* out) {
+  cudaError_t e = cudaMemcpyFromSymbol(out, g_ma_status, sizeof(unsigned int) * 4);
+  if (e != cudaSuccess) { g_lb_last_cuda_error = (int)e; return LB_ERR_LAUNCH; }
+  unsigned int zeros[4] = {0, 0, 0, 0};
+  cudaMemcpyToSymbol(g_ma_status, zeros, sizeof(zeros));
+  return LB_OK;
+}

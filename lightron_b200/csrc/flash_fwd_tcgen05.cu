@@ -59,19 +59,6 @@ struct FaPush {
   bf16* v_dst[FA_MAX_RANKS];
   unsigned int* flags[FA_MAX_RANKS];                 // rank r's block counters [B][S_full / 128]
 };
-// Division of 0 <= x < 2^31 by a divisor that is fixed for the launch: a multiplication by a rounded-up reciprocal (division by invariant
-// integers, Granlund and Montgomery 1994; the host finds m, which is exact for such x).
-struct FastDiv {
-  unsigned int d, m, s;
-  void set(unsigned int div) {
-    d = div;
-    s = 0;
-    while (s < 31 && (1u << s) < div) s++;                                        // 2^(s-1) < d <= 2^s
-    m = (unsigned int)((((unsigned long long)1 << (31 + s)) + div - 1) / div);    // < 2^32
-  }
-  __device__ __forceinline__ int div(int x) const { return (int)(((unsigned long long)(unsigned)x * m) >> (31 + s)); }
-};
-
 struct FaFwdParams {
   bf16* o;
   float* lse;
@@ -88,18 +75,6 @@ struct FaFwdParams {
   unsigned long long wait_ns;    // limit of a wait on a key block's arrival flag
   FastDiv by_grp, by_group, by_last, by_hq, by_rep;    // entries of a group, heads of a group / of the last one, hq, hq / hkv
 };
-
-// Three-input maximum; a NaN in any input is the result.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.NaN.ftz.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-__device__ __forceinline__ float max2(float a, float b) {
-  float r;
-  asm("max.NaN.ftz.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 
 template <int D>
 struct FaCfg {

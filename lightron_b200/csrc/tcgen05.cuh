@@ -102,6 +102,12 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
 // The same box into L2 only: a hint, which may run while another kernel still writes the matrix.
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
@@ -110,6 +116,11 @@ __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, i
 // fence_proxy_async_smem() after filling the tile, bulk_commit() after the store, and bulk_wait_read_but<>() before reusing it.
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y), "r"(z),
+               "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(w),
                "r"(src)
                : "memory");
 }
@@ -365,6 +376,37 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
   return r;
 }
 
+// Three-input maximum; a NaN in any input is the result.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.ftz.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("max.NaN.ftz.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// The same of the absolute values.
+__device__ __forceinline__ float max3abs(float a, float b, float c) {
+  float r;
+  asm("max.ftz.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Division of 0 <= x < 2^31 by a divisor that is fixed for the launch: a multiplication by a rounded-up reciprocal (division by invariant
+// integers, Granlund and Montgomery 1994; the host finds m, which is exact for such x).
+struct FastDiv {
+  unsigned int d, m, s;
+  void set(unsigned int div) {
+    d = div;
+    s = 0;
+    while (s < 31 && (1u << s) < div) s++;                                        // 2^(s-1) < d <= 2^s
+    m = (unsigned int)((((unsigned long long)1 << (31 + s)) + div - 1) / div);    // < 2^32
+  }
+  __device__ __forceinline__ int div(int x) const { return (int)(((unsigned long long)(unsigned)x * m) >> (31 + s)); }
+};
+
 // Byte offset of 16-byte chunk `c16` (0..7) of row `r` inside a 128-byte-swizzled atom whose rows
 // are 128 B apart and whose base is 1024-byte aligned.
 __device__ __forceinline__ uint32_t sw128_off(int r, int c16) { return (uint32_t)(r * 128 + ((c16 ^ (r & 7)) << 4)); }
@@ -387,7 +429,7 @@ inline EncodeTiledFn get_encode() {
   return fn;
 }
 
-// bf16 tensor map of `rank` 2 or 3 with 128-byte swizzle.  Binds the CUDA context to the calling thread first (the
+// bf16 tensor map of `rank` 2 to 4 with 128-byte swizzle.  Binds the CUDA context to the calling thread first (the
 // driver call needs one; autograd worker threads may not have touched the runtime yet).
 inline int make_map_bf16_nd(CUtensorMap* m, const void* base, uint32_t rank, const cuuint64_t* dims, const cuuint64_t* strides,
                             const cuuint32_t* box) {
@@ -398,7 +440,7 @@ inline int make_map_bf16_nd(CUtensorMap* m, const void* base, uint32_t rank, con
   }
   EncodeTiledFn enc = get_encode();
   if (!enc) return LB_ERR_DRIVER;
-  cuuint32_t estr[3] = {1, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -421,6 +463,15 @@ inline int make_map_bf16_3d(CUtensorMap* m, const void* base, uint64_t inner, ui
   const cuuint64_t dims[3] = {inner, rows, batches}, strides[2] = {ld * 2, apart * ld * 2};
   const cuuint32_t box[3] = {box_inner, box_rows, 1};
   return make_map_bf16_nd(m, base, 3, dims, strides, box);
+}
+
+// [batches, rows, heads, d] with strides of sb, ss and sh elements (multiples of 8); box = box_rows rows of 64 columns of one head.  What lies outside of d or of
+// the rows is loaded as zeros and not stored.
+inline int make_map_bf16_4d(CUtensorMap* m, const void* base, uint64_t d, uint64_t heads, uint64_t rows, uint64_t batches, uint64_t sh, uint64_t ss, uint64_t sb,
+                            uint32_t box_rows) {
+  const cuuint64_t dims[4] = {d, heads, rows, batches}, strides[3] = {sh * 2, ss * 2, sb * 2};
+  const cuuint32_t box[4] = {64, 1, box_rows, 1};
+  return make_map_bf16_nd(m, base, 4, dims, strides, box);
 }
 
 }  // namespace bw
