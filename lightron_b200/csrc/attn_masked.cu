@@ -73,134 +73,18 @@ __global__ void __launch_bounds__(PLAN_THREADS) attn_mask_kernel(const Id* __res
   }
 }
 
-// ---- a warp per row: right for every size ---------------------------------------------------------
-constexpr float LOG2E = 1.4426950408889634f;
-
-__device__ __forceinline__ float dot_row(const bf16* a, const bf16* b, int d) {
-  float s = 0.f;
-  for (int c = 0; c < d; c += 8) {
-    float x[8], y[8];
-    unpack8(*reinterpret_cast<const uint4*>(a + c), x);
-    unpack8(*reinterpret_cast<const uint4*>(b + c), y);
-#pragma unroll
-    for (int i = 0; i < 8; i++) s += x[i] * y[i];
-  }
-  return s;
-}
-__device__ __forceinline__ void load4(const bf16* p, float* f) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  const bf162* h = reinterpret_cast<const bf162*>(&u);
-  const float2 x = __bfloat1622float2(h[0]), y = __bfloat1622float2(h[1]);
-  f[0] = x.x; f[1] = x.y; f[2] = y.x; f[3] = y.y;
-}
-__device__ __forceinline__ void store4(bf16* p, const float* f) {
-  bf162 h[2] = {__floats2bfloat162_rn(f[0], f[1]), __floats2bfloat162_rn(f[2], f[3])};
-  *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(h);
-}
-// score, and its derivative by the uncapped score
-__device__ __forceinline__ float ma_score(const MaParams& p, float qk, int away, float slope, float& dcap) {
-  float s = qk * p.scale;
-  dcap = 1.f;
-  if (p.softcap > 0.f) {
-    const float t = 1.f - __fdividef(2.f, exp2f(s / p.softcap * (2.f * LOG2E)) + 1.f);
-    s = p.softcap * t;
-    dcap = 1.f - t * t;
-  }
-  return s - slope * (float)abs(away);
-}
-
-// D of a row, then dQ.
-__global__ void ma_bwd_rows_kernel(const MaBwdParams w) {
-  const MaParams& p = w.f;
-  const long long row = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (row >= (long long)p.B * p.hq * p.Sq) return;
-  const int lane = threadIdx.x & 31, i = (int)(row % p.Sq), h = (int)(row / p.Sq % p.hq), b = (int)(row / p.Sq / p.hq), g = h / (p.hq / p.hkv);
-  const bf16 *q = p.q + b * p.qs.b + i * p.qs.s + h * p.qs.h, *dout = w.dout + b * w.dos.b + i * w.dos.s + h * w.dos.h;
-  const bf16 *k = p.k + b * p.ks.b + g * p.ks.h, *v = p.v + b * p.vs.b + g * p.vs.h;
-  const int2 r = ma_keys(p, b, i);
-  const float slope = p.slopes ? p.slopes[h] : 0.f, lse = p.lse[row];
-  const bool mine = lane * 4 < p.d;
-  float D = 0.f, dq[4] = {0.f, 0.f, 0.f, 0.f};
-  if (mine) {
-    float x[4], y[4], z[4];
-    const long long at = (((long long)b * p.Sq + i) * p.hq + h) * p.d + lane * 4;
-    load4(p.o + at, x);
-    load4(p.o_lo + at, y);
-    load4(dout + lane * 4, z);
-#pragma unroll
-    for (int c = 0; c < 4; c++) D += (x[c] + y[c]) * z[c];
-  }
-  D = warp_sum(D);
-  if (lane == 0) w.stats[row] = D;
-  for (int j0 = r.x; j0 < r.y; j0 += 32) {
-    const int j = j0 + lane;
-    float ds = 0.f;
-    if (j < r.y) {
-      float dc;
-      const float s = ma_score(p, dot_row(q, k + j * p.ks.s, p.d), i + p.Sk - p.Sq - j, slope, dc);
-      ds = exp2f((s - lse) * LOG2E) * (dot_row(dout, v + j * p.vs.s, p.d) - D) * dc * p.scale;
-    }
-    for (int n = 0; n < min(32, r.y - j0); n++) {
-      const float x = __shfl_sync(0xffffffffu, ds, n);
-      if (mine) {
-        float f[4];
-        load4(k + (j0 + n) * p.ks.s + lane * 4, f);
-#pragma unroll
-        for (int c = 0; c < 4; c++) dq[c] += x * f[c];
-      }
-    }
-  }
-  if (mine) store4(w.dq + b * w.dqs.b + i * w.dqs.s + h * w.dqs.h + lane * 4, dq);
-}
-
-__global__ void ma_bwd_keys_kernel(const MaBwdParams w) {
-  const MaParams& p = w.f;
-  const long long row = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (row >= (long long)p.B * p.hkv * p.Sk) return;
-  const int lane = threadIdx.x & 31, j = (int)(row % p.Sk), g = (int)(row / p.Sk % p.hkv), b = (int)(row / p.Sk / p.hkv), rep = p.hq / p.hkv;
-  const bf16 *k = p.k + b * p.ks.b + j * p.ks.s + g * p.ks.h, *v = p.v + b * p.vs.b + j * p.vs.s + g * p.vs.h;
-  const int2 r = ma_queries(p, b, j);
-  const bool mine = lane * 4 < p.d;
-  float dk[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int h = g * rep; h < (g + 1) * rep; h++) {
-    const float slope = p.slopes ? p.slopes[h] : 0.f;
-    const bf16 *q = p.q + b * p.qs.b + h * p.qs.h, *dout = w.dout + b * w.dos.b + h * w.dos.h;
-    for (int i0 = r.x; i0 < r.y; i0 += 32) {
-      const int i = i0 + lane;
-      float ds = 0.f, e = 0.f;
-      if (i < r.y) {
-        float dc;
-        const long long at = ((long long)b * p.hq + h) * p.Sq + i;
-        const float s = ma_score(p, dot_row(q + i * p.qs.s, k, p.d), i + p.Sk - p.Sq - j, slope, dc);
-        e = exp2f((s - p.lse[at]) * LOG2E);
-        ds = e * (dot_row(dout + i * w.dos.s, v, p.d) - w.stats[at]) * dc * p.scale;
-      }
-      for (int n = 0; n < min(32, r.y - i0); n++) {
-        const float x = __shfl_sync(0xffffffffu, ds, n), y = __shfl_sync(0xffffffffu, e, n);
-        if (mine) {
-          float f[4], f2[4];
-          load4(q + (i0 + n) * p.qs.s + lane * 4, f);
-          load4(dout + (i0 + n) * w.dos.s + lane * 4, f2);
-#pragma unroll
-          for (int c = 0; c < 4; c++) { dk[c] += x * f[c]; dv[c] += y * f2[c]; }
-        }
-      }
-    }
-  }
-  if (mine) {
-    store4(w.dk + b * w.dks.b + j * w.dks.s + g * w.dks.h + lane * 4, dk);
-    store4(w.dv + b * w.dvs.b + j * w.dvs.s + g * w.dvs.h + lane * 4, dv);
-  }
-}
-
 bool bad_strides(const MaStrides& s) { return (s.b | s.s | s.h) % 8 != 0; }
 bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
 MaStrides strides_at(const long long* s) { return MaStrides{s[0], s[1], s[2]}; }
 
+int check_sizes(int B, int Sq, int Sk, int hq, int hkv, int d) {
+  return B <= 0 || Sq <= 0 || Sk < Sq || hq <= 0 || hkv <= 0 || hq % hkv || d <= 0 || d % 8 || d > 128 ? LB_ERR_SHAPE : LB_OK;
+}
+
 int fill(MaParams& p, const void* q, const void* k, const void* v, void* o, void* o_lo, void* lse, int B, int Sq, int Sk, int hq, int hkv, int d, const long long* st,
          float scale, int causal, float softcap, const void* slopes, const void* q_bounds, const void* k_bounds) {
-  if (B <= 0 || Sq <= 0 || Sk < Sq || hq <= 0 || hkv <= 0 || hq % hkv || d <= 0 || d % 8 || d > 128) return LB_ERR_SHAPE;
-  if (!q || !k || !v || !o || !lse || !st || !(softcap >= 0.f) || (!q_bounds) != (!k_bounds)) return LB_ERR_ARG;
+  if (check_sizes(B, Sq, Sk, hq, hkv, d)) return LB_ERR_SHAPE;
+  if (!q || !k || !v || !o || !lse || !st || !(softcap >= 0.f && softcap < INFINITY) || !(scale >= 0.f && scale < INFINITY) || (!q_bounds) != (!k_bounds)) return LB_ERR_ARG;
   if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(o) || misaligned(o_lo)) return LB_ERR_ARG;
   p = MaParams{(const bf16*)q, (const bf16*)k, (const bf16*)v, strides_at(st), strides_at(st + 3), strides_at(st + 6), (bf16*)o, (bf16*)o_lo, (float*)lse, B, Sq, Sk, hq, hkv, d,
                scale, causal, softcap, (const float*)slopes, (const int2*)q_bounds, (const int2*)k_bounds};
@@ -232,9 +116,12 @@ extern "C" int lb_masked_attn_fwd(const void* q, const void* k, const void* v, v
   return ma_launch_fwd(p, (cudaStream_t)stream);
 }
 
-extern "C" long long lb_masked_attn_bwd_ws_bytes(int B, int Sq, int Sk, int hq, int hkv, int d) {
-  (void)Sk; (void)hkv; (void)d;
-  return (long long)B * hq * Sq * (long long)sizeof(float);
+// Bytes of the backward's workspace; 0 for sizes that it does not take.
+extern "C" long long lb_masked_attn_bwd_ws_bytes(int B, int Sq, int Sk, int hq, int hkv, int d, int causal) {
+  MaParams p{};
+  if (check_sizes(B, Sq, Sk, hq, hkv, d)) return 0;
+  p.B = B; p.Sq = Sq; p.Sk = Sk; p.hq = hq; p.hkv = hkv; p.d = d; p.causal = causal;
+  return ma_bwd_ws_bytes(p);
 }
 
 // Backward.  strides: 7 x {batch, token, head} of q, k, v, dout, dq, dk, dv; o, o_lo, lse as the forward left them; ws: lb_masked_attn_bwd_ws_bytes(), 16-byte aligned.
@@ -244,15 +131,9 @@ extern "C" int lb_masked_attn_bwd(const void* q, const void* k, const void* v, c
   MaBwdParams w;
   if (const int rc = fill(w.f, q, k, v, const_cast<void*>(o), const_cast<void*>(o_lo), const_cast<void*>(lse), B, Sq, Sk, hq, hkv, d, strides, scale, causal, softcap, slopes, q_bounds, k_bounds)) return rc;
   if (!o_lo || !dout || !ws || !dq || !dk || !dv || misaligned(dout) || misaligned(ws) || misaligned(dq) || misaligned(dk) || misaligned(dv)) return LB_ERR_ARG;
-  if (ws_bytes < lb_masked_attn_bwd_ws_bytes(B, Sq, Sk, hq, hkv, d)) return LB_ERR_CAPACITY;
+  if (ws_bytes < ma_bwd_ws_bytes(w.f)) return LB_ERR_CAPACITY;
   w.dout = (const bf16*)dout; w.dq = (bf16*)dq; w.dk = (bf16*)dk; w.dv = (bf16*)dv; w.stats = (float*)ws;
   w.dos = strides_at(strides + 9); w.dqs = strides_at(strides + 12); w.dks = strides_at(strides + 15); w.dvs = strides_at(strides + 18);
   if (bad_strides(w.dos) || bad_strides(w.dqs) || bad_strides(w.dks) || bad_strides(w.dvs)) return LB_ERR_SHAPE;
-  const long long rows = (long long)B * hq * Sq, keys = (long long)B * hkv * Sk;
-  if ((rows + 3) / 4 > 2147483647LL || (keys + 3) / 4 > 2147483647LL) return LB_ERR_SHAPE;
-  ma_bwd_rows_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, (cudaStream_t)stream>>>(w);
-  LB_CHECK_LAUNCH();
-  ma_bwd_keys_kernel<<<(unsigned)((keys + 3) / 4), 128, 0, (cudaStream_t)stream>>>(w);
-  LB_CHECK_LAUNCH();
-  return LB_OK;
+  return ma_launch_bwd(w, (cudaStream_t)stream);
 }

@@ -33,6 +33,24 @@ struct MaBwdParams {
 };
 
 int ma_launch_fwd(const MaParams& p, cudaStream_t s);
+int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s);
+long long ma_bwd_ws_bytes(const MaParams& p);
+
+// tanh(x * by) * times = x * (c[0] + c[1] x^2 + c[2] x^4 + c[3] x^6) while |x| <= limit, which is 0.6 / by: relative error 2.2e-6 (coefficients of tanh(u) / u in u^2, found
+// by least squares over Chebyshev points with weights that were raised where the error was largest).
+inline void ma_tanh_terms(double by, double times, float* limit, float* c) {
+  const double k[4] = {0.9999978542327881, -0.33314040303230286, 0.13057856261730194, -0.04092942178249359};
+  *limit = (float)(0.6 / by);      // (a scale of zero: no limit)
+  double pw = by * times;
+  for (int i = 0; i < 4; i++, pw *= by * by) c[i] = (float)(k[i] * pw);
+}
+
+// Bits [lo, hi) of 32 columns, of which column 0 is at `at`.
+__device__ __forceinline__ uint32_t ma_bits(int lo, int hi, int at) {
+  const int a = min(max(lo - at, 0), 32), e = min(max(hi - at, 0), 32);
+  const uint32_t below_e = e == 32 ? 0xffffffffu : (1u << e) - 1u, below_a = a == 32 ? 0xffffffffu : (1u << a) - 1u;
+  return below_e & ~below_a;
+}
 
 // Keys [x, y) that query i of sequence b sees.
 __device__ __forceinline__ int2 ma_keys(const MaParams& p, int b, int i) {

@@ -61,13 +61,6 @@ struct Cfg {
 };
 static_assert(Cfg<64>::SMEM <= 115712 && Cfg<128>::SMEM <= 115712, "two CTAs per SM");
 
-// Bits [lo, hi) of 32 columns, of which column 0 is at `at`.
-__device__ __forceinline__ uint32_t visible_bits(int lo, int hi, int at) {
-  const int a = min(max(lo - at, 0), 32), e = min(max(hi - at, 0), 32);
-  const uint32_t below_e = e == 32 ? 0xffffffffu : (1u << e) - 1u, below_a = a == 32 ? 0xffffffffu : (1u << a) - 1u;
-  return below_e & ~below_a;
-}
-
 // 64 raw scores to units of log2, capped and lowered with distance.  `first`: key of column 0 less the row's position; `side`: the columns lie on the row's left (1),
 // on its right (-1) or on both sides (0), the same for all lanes.
 template <int CAP, bool BIAS>
@@ -370,7 +363,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           if (need_mask) {
 #pragma unroll
             for (int w = i0; w < i0 + 64; w += 32) {
-              const uint32_t bits = visible_bits(lo, hi, w);
+              const uint32_t bits = ma_bits(lo, hi, w);
 #pragma unroll
               for (int i = 0; i < 32; i++)
                 if (!(bits >> i & 1u)) r[w + i] = 0xff800000u;           // -inf
@@ -591,12 +584,9 @@ int launch_fwd(const MaParams& a, cudaStream_t s) {
   p.by_cap = p.cap_l2 = p.limit = p.c[1] = p.c[2] = p.c[3] = 0.f;
   if (a.softcap > 0.f) {
     const double by = (double)a.scale / a.softcap, l2 = (double)a.softcap * 1.4426950408889634;
-    const double k[4] = {0.9999978542327881, -0.33314040303230286, 0.13057856261730194, -0.04092942178249359};      // tanh(u) / u in u^2, |u| <= 0.6
     p.by_cap = (float)by;
     p.cap_l2 = (float)l2;
-    p.limit = (float)(0.6 / fabs(by));      // (a scale of zero: no limit)
-    double pw = by * l2;
-    for (int i = 0; i < 4; i++, pw *= by * by) p.c[i] = (float)(k[i] * pw);
+    ma_tanh_terms(by, l2, &p.limit, p.c);
   }
   const bool bias = a.slopes != nullptr;
   if (a.softcap <= 0.f) return bias ? launch<D, NO_CAP, true>(maps, p, (unsigned)grid, s) : launch<D, NO_CAP, false>(maps, p, (unsigned)grid, s);

@@ -833,7 +833,7 @@ def masked_bwd_native(q, k, v, o, o_lo, lse, do, causal: bool, scale: float, sof
     Sk, hkv = k.shape[1], k.shape[2]
     if dq is None:
         dq, dk, dv = torch.empty_like(o), torch.empty(B, Sk, hkv, d, dtype=q.dtype, device=q.device), torch.empty(B, Sk, hkv, d, dtype=q.dtype, device=q.device)
-    ws = torch.empty(native.require().lb_masked_attn_bwd_ws_bytes(B, Sq, Sk, hq, hkv, d), dtype=torch.uint8, device=q.device)
+    ws = torch.empty(native.require().lb_masked_attn_bwd_ws_bytes(B, Sq, Sk, hq, hkv, d, int(causal)), dtype=torch.uint8, device=q.device)
     native.call("lb_masked_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), o_lo.data_ptr(), do.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(),
                 dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, Sq, Sk, hq, hkv, d, _strides(q, k, v, do, dq, dk, dv), scale, int(causal), softcap,
                 native.ptr(slopes), native.ptr(qb), native.ptr(kb), native.stream_ptr())
@@ -862,7 +862,7 @@ class _MaskedAttn(torch.autograd.Function):
 MASKED_MAX_HEAD_DIM = 128
 
 
-def _check_masked(q, k, v, mask, causal, softcap, slopes) -> bool:
+def _check_masked(q, k, v, mask, causal, scale, softcap, slopes) -> bool:
     """Refuses what does not fit together; returns whether the mask is causal."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError(f"masked_attention takes q [B, Sq, hq, d] and k, v [B, Sk, hkv, d]; got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -874,6 +874,8 @@ def _check_masked(q, k, v, mask, causal, softcap, slopes) -> bool:
         raise ValueError(f"{Sq} queries at the end of {Sk} positions")
     if not (k.dtype == v.dtype == q.dtype and k.device == v.device == q.device):
         raise ValueError(f"q, k, v differ in type or device: {q.dtype} {q.device}, {k.dtype} {k.device}, {v.dtype} {v.device}")
+    if scale is not None and not 0.0 <= scale < float("inf"):
+        raise ValueError(f"scale must be finite and not negative, got {scale}")
     if not (0.0 <= softcap < float("inf")):
         raise ValueError(f"softcap must be zero (none) or positive and finite, got {softcap}")
     if mask is not None:
@@ -902,7 +904,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Op
     """softmax(s) v for q [B, Sq, hq, d] and k, v [B, Sk, hkv, d] in any order of the outer dimensions; query i sits at position i + Sk - Sq.
     ``s = softcap * tanh(x / softcap) - slopes[h] * |distance|`` with ``x = scale * q.k`` (``softcap`` 0: x itself; ``slopes`` fp32 [hq], constants).
     ``mask``: see :func:`attention_mask`; without one, ``causal`` (default) or all keys.  Rows that see nothing give zeros, and gradients of zero."""
-    causal = _check_masked(q, k, v, mask, causal, softcap, slopes)
+    causal = _check_masked(q, k, v, mask, causal, scale, softcap, slopes)
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
     qb, kb = (mask.q_bounds, mask.k_bounds) if mask is not None else (None, None)
     if native.use_native(q) and q.numel() and k.numel():

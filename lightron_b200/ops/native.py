@@ -93,7 +93,8 @@ _SIGNATURES = {
     "lb_masked_attn_fwd": [_P] * 6 + [_I] * 6 + [_P, _F, _I, _F, _P, _P, _P, _P],
     "lb_masked_attn_status": [_P],
     "lb_masked_attn_bwd": [_P] * 8 + [_L] + [_P] * 3 + [_I] * 6 + [_P, _F, _I, _F, _P, _P, _P, _P],
-    "lb_masked_attn_bwd_ws_bytes": [_I] * 6,
+    "lb_masked_attn_bwd_ws_bytes": [_I] * 7,
+    "lb_masked_attn_bwd_status": [_P],
     "lb_rope_axes": [_P] * 6 + [_I] * 6 + [_P, _L, _L, _I, _P],
     "lb_grad_norm_parts": [_I],
     "lb_grad_squares": [_I, _P, _P, _P, _P, _I, _P, _P],
@@ -307,7 +308,7 @@ def _load_host_ops():
 _STATUS_READERS = (("lb_device_status", "GEMM / fused collective GEMM"), ("lb_gemm_grouped_status", "grouped GEMM"),
                    ("lb_gemm_split_status", "GEMM of small launches"),
                    ("lb_flash_status", "attention forward"), ("lb_flash_bwd_status", "attention backward"),
-                   ("lb_masked_attn_status", "masked attention forward"),
+                   ("lb_masked_attn_status", "masked attention forward"), ("lb_masked_attn_bwd_status", "masked attention backward"),
                    ("lb_dp_status", "data-parallel optimizer kernel"),
                    ("lb_moe_status", "expert-parallel routing / dispatch / combine"),
                    ("lb_coll_status", "stand-alone peer-memory collective"))
