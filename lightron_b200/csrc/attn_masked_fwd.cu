@@ -12,8 +12,9 @@
 //   * tanh: where no score of 32 rows x 64 columns is above 0.6 caps, x times a polynomial in x^2 on the FMA pipe, two at a time (relative error
 //     2.1e-6, found by least squares with re-weighted points; 7e-5 of a score at most); else by its definition with exp2, whose units the softmax needs itself.
 //   * the bias is an addend of the same FMA, counted up along the columns; only where a block holds keys on both sides of a row is its distance made per column.
-//   * a row's sum is that of its weights as they are rounded for P V.  A row that all but one key leave cold has o = v of that key then, and a D = do . o whose
-//     error is as small as the differences dP - D that the backward lives on (the weight's own rounding, 2^-9 of dP, would drown them).
+//   * o is divided by the sum of the weights as they are rounded for P V.  A row that all but one key leave cold has o = v of that key then, and a D = do . o whose
+//     error is as small as the differences dP - D that the backward lives on (the weight's own rounding, 2^-9 of dP, would drown them); lse is of the sum of the
+//     unrounded ones, from which the backward's P are made.
 //   * o leaves twice: rounded, and what the rounding left (for the backward's row sums).
 // All waits are bounded; on expiry a status word is set and the CTA drains and frees its TMEM.
 #include "attn_masked.cuh"
@@ -352,7 +353,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         slope2 = p.slopes ? p.slopes[t.h] * LOG2E : 0.f;
         left_only = __all_sync(0xffffffffu, row >= p.Sq || see.y <= row + off + 1);
       }
-      float m_i = -INFINITY, m_s = 0.f, l_i = 0.f;      // running maximum, and what exponentials are relative to
+      float m_i = -INFINITY, m_s = 0.f, l_i = 0.f, lp_i = 0.f;      // running maximum, what exponentials are relative to, their sums
       for (int j = 0; j < nb; j++, g++) {
         if (!s_ready && !mbar_wait(s_full, g & 1u, abort_flag)) { ok = false; break; }
         fence_after();
@@ -379,7 +380,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         // exponentials of 64 columns, packed as bf16 pairs (column c of P holds keys 2c, 2c+1)
         auto exps = [&](int i0, uint32_t* pr, f32x2* rs2) {
           const f32x2 nms2 = pack2(-m_s, -m_s);
-          rs2[0] = rs2[1] = pack2(0.f, 0.f);
+          rs2[0] = rs2[1] = pack2(0.f, 0.f);             // sums of the exponentials, and of them as P holds them
 #pragma unroll
           for (int c = 0; c < 32; c++) {
             const int i = i0 + c * 2;
@@ -394,7 +395,8 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             e1 = exp2f(e1);
             bf162 pk = __floats2bfloat162_rn(e0, e1);
             pr[c] = *reinterpret_cast<uint32_t*>(&pk);
-            rs2[c & 1] = add2(rs2[c & 1], pack2(__uint_as_float(pr[c] << 16), __uint_as_float(pr[c] & 0xffff0000u)));
+            rs2[0] = add2(rs2[0], pack2(e0, e1));
+            rs2[1] = add2(rs2[1], pack2(__uint_as_float(pr[c] << 16), __uint_as_float(pr[c] & 0xffff0000u)));
           }
         };
         auto row_max = [&]() {                           // four independent chains
@@ -434,6 +436,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             m_s = (m_new == -INFINITY) ? 0.f : (m_new == INFINITY ? __int_as_float(0x7fffffff) : m_new);
             corr = (m_i == -INFINITY) ? 0.f : exp2f((m_i - m_s) * unit);
             l_i *= corr;
+            lp_i *= corr;
             m_i = m_new;
             exps(0, pr, rs2);
           }
@@ -476,7 +479,8 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         float rs[4];
         unpack2(rs2[0], rs[0], rs[1]);
         unpack2(rs2[1], rs[2], rs[3]);
-        l_i += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+        l_i += rs[0] + rs[1];
+        lp_i += rs[2] + rs[3];
       }
       if (ok) {
         cta = next_cta(n);
@@ -486,7 +490,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       if (ok && !mbar_wait(pv_done, C::P_ALIAS ? (uint32_t)n & 1u : (g - 1) & 1u, abort_flag)) ok = false;
       if (!ok) break;
       fence_after();
-      const float inv = l_i != 0.f ? 1.f / l_i : 0.f;
+      const float inv = lp_i != 0.f ? 1.f / lp_i : 0.f;
       // 64 columns at a time through shared memory and TMA stores, which leave out rows past the last and columns past head_dim
       uint8_t* out = smem + C::OFF_OUT + quad * 4096;
 #pragma unroll
