@@ -21,6 +21,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <atomic>
 #include <climits>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 
@@ -52,6 +53,15 @@ struct Api {
   int (*lb_ce_loss)(P, W, P, P, W, W, int, float, int, W);
   int (*lb_ce_grad)(P, P, P, W, P, int, int, L, int, float, int, W);
   int (*lb_gemm_rope)(P, P, W, int, int, int, P, P, P, int, int, int, W);
+  int (*lb_attn_mask)(P, int, P, P, int, int, int, W, W, W);
+  int (*lb_masked_attn_fwd)(P, P, P, W, W, W, int, int, int, int, int, int, const L*, float, int, float, P, P, P, W);
+  L (*lb_masked_attn_bwd_ws_bytes)(int, int, int, int, int, int, int);
+  int (*lb_masked_attn_bwd)(P, P, P, P, P, P, P, W, L, W, W, W, int, int, int, int, int, int, const L*, float, int, float, P, P, P, W);
+  int (*lb_rope_axes)(P, W, P, P, P, const unsigned char*, int, int, int, int, int, int, const L*, L, L, int, W);
+  int (*lb_grad_norm_parts)(int);
+  int (*lb_grad_squares)(int, const P*, const L*, const int*, W, int, int*, W);
+  int (*lb_grad_total)(P, int, W, W, W);
+  int (*lb_grad_scale)(int, const P*, const W*, const L*, const int*, P, int, float, float, W, W);
 } api;
 PyObject* raise_error = nullptr;                 // (name, code): raises the error of ops/native.py
 PyObject* direct_grad = nullptr;                 // the attribute of a weight whose gradient the optimizer keeps
@@ -356,6 +366,97 @@ struct RopeAttention : Function<RopeAttention> {
                        {dout.const_data_ptr(), dout.stride(1)}, at_head(dqkv, 0, d), at_head(dqkv, hq, d), at_head(dqkv, hq + hkv, d), row, row, row, m);
     rope(dqkv, cos, sin, pos, S, hq + hkv, d, row, 1);
     return {dqkv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// ---- packed batches: masked attention, rotation by axes ------------------------------------------
+// [B, S, h, d] that the kernels read where it lies: 16-byte heads, outer dimensions in any order
+bool strided_ok(const Tensor& t) {
+  if (t.stride(3) != 1 || ((uintptr_t)t.const_data_ptr() & 15)) return false;
+  for (int i = 0; i < 3; i++)
+    if (t.size(i) != 1 && (t.stride(i) <= 0 || t.stride(i) % 8)) return false;
+  return true;
+}
+Tensor fix_strides(const Tensor& t) { return strided_ok(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+// (the stride of a single entry is never used, and made such that a tensor map takes it)
+void put_strides(L* at, const Tensor& t) {
+  for (int i = 0; i < 3; i++) at[i] = t.size(i) > 1 ? t.stride(i) : t.size(3);
+}
+P ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+struct MaskedArgs { bool causal, grad; double scale, softcap; };      // one argument to autograd
+struct MaskedAttention : Function<MaskedAttention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q0, const Tensor& k0, const Tensor& v0, const std::optional<Tensor>& slopes, const std::optional<Tensor>& qb,
+                        const std::optional<Tensor>& kb, MaskedArgs a) {
+    const Tensor q = fix_strides(q0), k = fix_strides(k0), v = fix_strides(v0), sl = slopes.value_or(Tensor()), qi = qb.value_or(Tensor()), ki = kb.value_or(Tensor());
+    const AttnDims m = dims_of(q, k, a.causal, a.scale);
+    Tensor o = at::empty({m.B, m.Sq, m.hq, m.d}, q.options()), lo, lse = empty_f32({m.B, m.hq, m.Sq}, q);
+    if (a.grad) lo = at::empty({m.B, m.Sq, m.hq, m.d}, q.options());
+    L st[9];
+    put_strides(st, q); put_strides(st + 3, k); put_strides(st + 6, v);
+    LB_CALL(lb_masked_attn_fwd, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.mutable_data_ptr(), const_cast<W>(ptr(lo)), lse.mutable_data_ptr(), m.B, m.Sq, m.Sk, m.hq,
+            m.hkv, m.d, st, m.scale, m.causal, (float)a.softcap, ptr(sl), ptr(qi), ptr(ki), stream());
+    if (a.grad) {
+      ctx->save_for_backward({q0, k0, v0, o, lo, lse, sl, qi, ki});
+      ctx->saved_data["causal"] = a.causal;
+      ctx->saved_data["scale"] = a.scale;
+      ctx->saved_data["softcap"] = a.softcap;
+    }
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor& g = grads[0];
+    check_saved(s[0], g, at::kBFloat16, g.numel(), g.size(3));
+    for (int i = 1; i < 3; i++) check_saved(s[i], g, at::kBFloat16, s[1].defined() ? s[1].numel() : -1, g.size(3));
+    TORCH_CHECK(s[0].sizes().equals(g.sizes()) && s[1].dim() == 4 && s[2].sizes().equals(s[1].sizes()) && s[1].size(0) == g.size(0) && s[1].numel() > 0 && g.size(2) % s[1].size(2) == 0,
+                "q, k or v saved for backward has come back with another shape");
+    const Tensor q = fix_strides(s[0]), k = fix_strides(s[1]), v = fix_strides(s[2]), dout = fix_strides(g);
+    const AttnDims m = dims_of(q, k, ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
+    const L rows = (L)m.B * m.Sq * m.hq, ends = 2L * m.B * m.Sk;
+    const Tensor o = operand(s[3], g, rows * m.d, -1), lo = operand(s[4], g, rows * m.d, -1), lse = operand(s[5], g, rows, m.Sq, at::kFloat);
+    const Tensor sl = s[6].defined() ? operand(s[6], g, m.hq, m.hq, at::kFloat) : Tensor(), qi = s[7].defined() ? operand(s[7], g, ends, 2, at::kInt) : Tensor();
+    const Tensor ki = s[8].defined() ? operand(s[8], g, ends, 2, at::kInt) : Tensor();
+    Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(k.sizes(), k.options());
+    const L bytes = api.lb_masked_attn_bwd_ws_bytes(m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d, m.causal);
+    Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+    L st[21];
+    const Tensor* ts[7] = {&q, &k, &v, &dout, &dq, &dk, &dv};
+    for (int i = 0; i < 7; i++) put_strides(st + 3 * i, *ts[i]);
+    LB_CALL(lb_masked_attn_bwd, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.const_data_ptr(), lo.const_data_ptr(), dout.const_data_ptr(), lse.const_data_ptr(),
+            ws.mutable_data_ptr(), bytes, dq.mutable_data_ptr(), dk.mutable_data_ptr(), dv.mutable_data_ptr(), m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d, st, m.scale, m.causal,
+            (float)ctx->saved_data["softcap"].toDouble(), ptr(sl), ptr(qi), ptr(ki), stream());
+    return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct Axes { unsigned char of[128]; int n; };      // axis of each pair, number of axes
+struct RopeAxes : Function<RopeAxes> {
+  static Tensor turn(const Tensor& x0, const Tensor& cos, const Tensor& sin, const Tensor& pos, const unsigned char* axes, int inverse) {
+    const Tensor x = fix_strides(x0);
+    Tensor y = at::empty(x.sizes(), x.options());
+    L st[3];
+    put_strides(st, x);
+    LB_CALL(lb_rope_axes, x.const_data_ptr(), y.mutable_data_ptr(), cos.const_data_ptr(), sin.const_data_ptr(), pos.const_data_ptr(), axes, (int)pos.size(0), (int)x.size(0), (int)x.size(1),
+            (int)x.size(2), (int)x.size(3), (int)cos.size(0), st, pos.stride(0), pos.dim() == 3 ? pos.stride(1) : 0, inverse, stream());
+    return y;
+  }
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& cos, const Tensor& sin, const Tensor& pos, Axes axes) {
+    Tensor y = turn(x, cos, sin, pos, axes.of, 0);
+    ctx->save_for_backward({cos, sin, pos});
+    ctx->saved_data["axes"] = std::string(reinterpret_cast<const char*>(axes.of), x.size(3) / 2);
+    ctx->saved_data["sizes"] = std::vector<int64_t>{cos.numel(), pos.numel(), pos.dim()};
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor& g = grads[0];
+    const std::vector<int64_t> n = ctx->saved_data["sizes"].toIntVector();
+    const Tensor cos = operand(s[0], g, n[0], g.size(3) / 2, at::kFloat), sin = operand(s[1], g, n[0], g.size(3) / 2, at::kFloat);
+    const Tensor pos = operand(s[2], g, n[1], g.size(1), at::kInt);
+    TORCH_CHECK(pos.dim() == n[2], "positions saved for backward have come back with another shape");
+    const std::string axes = ctx->saved_data["axes"].toStringRef();
+    return {turn(g, cos, sin, pos, reinterpret_cast<const unsigned char*>(axes.data()), 1), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -695,6 +796,181 @@ PyObject* py_decoder_layers(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- packed batches ------------------------------------------------------------------------------
+bool here(const Tensor& t) { return t.device().index() == c10::cuda::current_device(); }
+bool sized(const Tensor* t, const Tensor& like, at::ScalarType type) {      // dense, contiguous, on the same device, without a gradient of its own
+  return t && t->defined() && t->device() == like.device() && t->scalar_type() == type && t->layout() == at::kStrided && t->is_contiguous() && !t->requires_grad();
+}
+std::optional<Tensor> maybe(const Tensor* t) { return t ? std::optional<Tensor>(*t) : std::nullopt; }
+
+// attention_mask(documents or None, marks or None, causal) -> (q_bounds, k_bounds)
+PyObject* py_attention_mask(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 3 || !unobserved()) LB_NOT_PLAIN;
+  const Tensor *ids = a[0] == Py_None ? nullptr : tensor(a[0]), *marks = a[1] == Py_None ? nullptr : tensor(a[1]);
+  const bool causal = a[2] == Py_True;
+  if ((a[0] != Py_None && !ids) || (a[1] != Py_None && !marks) || (!ids && !marks) || (a[2] != Py_True && a[2] != Py_False) || (marks && !causal)) LB_NOT_PLAIN;
+  const Tensor& t = ids ? *ids : *marks;
+  if (!t.defined() || !t.is_cuda() || t.dim() != 2 || t.numel() == 0 || !here(t) || !fits_int({t.size(0), t.size(1)})) LB_NOT_PLAIN;
+  if (ids && !sized(ids, t, at::kInt) && !sized(ids, t, at::kLong)) LB_NOT_PLAIN;
+  if (marks && ((!sized(marks, t, at::kBool) && !sized(marks, t, at::kByte)) || !marks->sizes().equals(t.sizes()))) LB_NOT_PLAIN;
+  std::pair<Tensor, Tensor> r = unlocked([&] {
+    Tensor q = at::empty({t.size(0), t.size(1), 2}, t.options().dtype(at::kInt)), k = at::empty({t.size(0), t.size(1), 2}, t.options().dtype(at::kInt));
+    LB_CALL(lb_attn_mask, ids ? ids->const_data_ptr() : nullptr, ids ? (int)ids->element_size() : 4, marks ? marks->const_data_ptr() : nullptr, nullptr, (int)t.size(0), (int)t.size(1),
+            causal, q.mutable_data_ptr(), k.mutable_data_ptr(), stream());
+    return std::pair<Tensor, Tensor>(q, k);
+  });
+  PyObject* out = PyTuple_New(2);
+  if (!out) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(r.first)));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(r.second)));
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// masked_attention(q, k, v, q_bounds or None, k_bounds or None, slopes or None, causal, scale or None, softcap)
+PyObject* py_masked_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || !unobserved()) LB_NOT_PLAIN;
+  const Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]);
+  if (!plain(q, false) || !plain(k, false) || !plain(v, false) || q->dim() != 4 || k->dim() != 4 || !v->sizes().equals(k->sizes()) || !here(*q) || k->device() != q->device() ||
+      v->device() != q->device())
+    LB_NOT_PLAIN;
+  const int64_t B = q->size(0), Sq = q->size(1), hq = q->size(2), d = q->size(3), Sk = k->size(1), hkv = k->size(2);
+  if (k->size(0) != B || k->size(3) != d || hq % hkv || Sq > Sk || d % 8 || d > 128 || !fits_int({B, Sk, hq})) LB_NOT_PLAIN;
+  const Tensor *qb = nullptr, *kb = nullptr, *slopes = nullptr;
+  if (a[3] != Py_None) {
+    qb = tensor(a[3]);
+    kb = tensor(a[4]);
+    if (!sized(qb, *q, at::kInt) || !sized(kb, *q, at::kInt) || !qb->sizes().equals({B, Sk, 2}) || !kb->sizes().equals({B, Sk, 2})) LB_NOT_PLAIN;
+  }
+  if (a[5] != Py_None) {
+    slopes = tensor(a[5]);
+    if (!sized(slopes, *q, at::kFloat) || !slopes->sizes().equals({hq})) LB_NOT_PLAIN;
+  }
+  if (a[6] != Py_True && a[6] != Py_False) LB_NOT_PLAIN;
+  const double scale = a[7] == Py_None ? 1.0 / std::sqrt((double)d) : PyFloat_AsDouble(a[7]), softcap = PyFloat_AsDouble(a[8]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    LB_NOT_PLAIN;
+  }
+  if (!(scale >= 0.0 && scale < HUGE_VAL) || !(softcap >= 0.0 && softcap < HUGE_VAL)) LB_NOT_PLAIN;
+  const MaskedArgs m{a[6] == Py_True, at::GradMode::is_enabled() && (q->requires_grad() || k->requires_grad() || v->requires_grad()), scale, softcap};
+  return THPVariable_Wrap(unlocked([&, q_ = *q, k_ = *k, v_ = *v, sl = maybe(slopes), qi = maybe(qb), ki = maybe(kb)] { return MaskedAttention::apply(q_, k_, v_, sl, qi, ki, m); }));
+  END_HANDLE_TH_ERRORS
+}
+
+// rope_axes(x, cos, sin, positions, axes: list or tuple of ints)
+PyObject* py_rope_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || !unobserved()) LB_NOT_PLAIN;
+  const Tensor *x = tensor(a[0]), *cos = tensor(a[1]), *sin = tensor(a[2]), *pos = tensor(a[3]);
+  if (!plain(x, false) || x->dim() != 4 || !here(*x) || !(PyList_CheckExact(a[4]) || PyTuple_CheckExact(a[4]))) LB_NOT_PLAIN;
+  const int64_t B = x->size(0), S = x->size(1), d = x->size(3), pairs = d / 2;
+  if (d % 8 || d > 256 || !fits_int({B, S, x->size(2)})) LB_NOT_PLAIN;
+  if (!sized(cos, *x, at::kFloat) || !sized(sin, *x, at::kFloat) || !sized(pos, *x, at::kInt) || cos->dim() != 2 || cos->size(1) != pairs || !sin->sizes().equals(cos->sizes()) ||
+      cos->size(0) == 0 || !fits_int({cos->size(0)}) || ((uintptr_t)cos->const_data_ptr() & 15) || ((uintptr_t)sin->const_data_ptr() & 15))
+    LB_NOT_PLAIN;
+  const int64_t A = pos->dim() > 0 ? pos->size(0) : 0;
+  if (A < 1 || A > 8 || !(pos->sizes().equals({A, S}) || pos->sizes().equals({A, B, S}))) LB_NOT_PLAIN;
+  Axes axes;
+  axes.n = (int)A;
+  if (PySequence_Fast_GET_SIZE(a[4]) != pairs) LB_NOT_PLAIN;
+  for (int64_t i = 0; i < pairs; i++) {
+    PyObject* o = PySequence_Fast_GET_ITEM(a[4], i);
+    if (!PyLong_CheckExact(o)) LB_NOT_PLAIN;
+    const long v = PyLong_AsLong(o);
+    if (v < 0 || v >= A) {
+      PyErr_Clear();
+      LB_NOT_PLAIN;
+    }
+    axes.of[i] = (unsigned char)v;
+  }
+  return THPVariable_Wrap(unlocked([&, x_ = *x, c = *cos, s = *sin, p = *pos] { return RopeAxes::apply(x_, c, s, p, axes); }));
+  END_HANDLE_TH_ERRORS
+}
+
+// The list's tensors as the kernels take them: dense in one piece, all on the current device; false: not a plain list
+struct NormList {
+  std::vector<P> at;
+  std::vector<L> n;
+  std::vector<int> type;
+  std::vector<const Tensor*> t;
+  bool take(PyObject* list) {
+    if (!PyList_CheckExact(list) && !PyTuple_CheckExact(list)) return false;
+    const Py_ssize_t k = PySequence_Fast_GET_SIZE(list);
+    at.reserve(k); n.reserve(k); type.reserve(k); t.reserve(k);
+    for (Py_ssize_t i = 0; i < k; i++) {
+      const Tensor* x = tensor(PySequence_Fast_GET_ITEM(list, i));
+      if (!x || !x->defined() || !x->is_cuda() || x->layout() != at::kStrided || !x->is_contiguous() || x->is_neg() || x->_fw_grad(0).defined()) return false;
+      const at::ScalarType s = x->scalar_type();
+      if (s != at::kBFloat16 && s != at::kHalf && s != at::kFloat) return false;
+      if (i == 0 ? !here(*x) : x->device() != t[0]->device()) return false;
+      at.push_back(x->const_data_ptr());
+      n.push_back(x->numel());
+      type.push_back(s == at::kBFloat16 ? 0 : s == at::kHalf ? 1 : 2);
+      t.push_back(x);
+    }
+    return k > 0 && k < INT_MAX;
+  }
+};
+// Runs the sums of squares; the parts and how many
+std::pair<Tensor, int> norm_parts(const NormList& l) {
+  Tensor parts = empty_f32({api.lb_grad_norm_parts((int)l.at.size())}, *l.t[0]);
+  int filled = 0;
+  LB_CALL(lb_grad_squares, (int)l.at.size(), l.at.data(), l.n.data(), l.type.data(), parts.mutable_data_ptr(), (int)parts.numel(), &filled, stream());
+  return {parts, filled};
+}
+
+// grad_norm(list)
+PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NormList l;
+  if (n != 1 || !unobserved() || !l.take(a[0])) LB_NOT_PLAIN;
+  return THPVariable_Wrap(unlocked([&] {
+    at::NoGradGuard off;
+    const std::pair<Tensor, int> p = norm_parts(l);
+    Tensor norm = empty_f32({}, *l.t[0]);
+    LB_CALL(lb_grad_total, p.first.const_data_ptr(), p.second, nullptr, norm.mutable_data_ptr(), stream());
+    return norm;
+  }));
+  END_HANDLE_TH_ERRORS
+}
+
+// clip_grad_norm(list, max_norm, out list or None, eps)
+PyObject* py_clip_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NormList l, o;
+  if (n != 4 || !unobserved() || !l.take(a[0]) || (a[2] != Py_None && !o.take(a[2]))) LB_NOT_PLAIN;
+  const double max_norm = PyFloat_AsDouble(a[1]), eps = PyFloat_AsDouble(a[3]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    LB_NOT_PLAIN;
+  }
+  if (!(max_norm >= 0.0) || !(eps >= 0.0)) LB_NOT_PLAIN;
+  const NormList& to = a[2] == Py_None ? l : o;
+  if (to.at.size() != l.at.size() || to.t[0]->device() != l.t[0]->device()) LB_NOT_PLAIN;
+  for (size_t i = 0; i < l.at.size(); i++) {
+    if (to.type[i] != l.type[i] || !to.t[i]->sizes().equals(l.t[i]->sizes())) LB_NOT_PLAIN;
+    if (to.t[i]->requires_grad() && at::GradMode::is_enabled()) LB_NOT_PLAIN;
+  }
+  return THPVariable_Wrap(unlocked([&] {
+    at::NoGradGuard off;
+    const std::pair<Tensor, int> p = norm_parts(l);
+    Tensor norm = empty_f32({}, *l.t[0]);
+    std::vector<W> dst;
+    dst.reserve(to.at.size());
+    for (const Tensor* t : to.t) {
+      dst.push_back(t->mutable_data_ptr());
+      t->unsafeGetTensorImpl()->bump_version();
+    }
+    LB_CALL(lb_grad_scale, (int)l.at.size(), l.at.data(), dst.data(), l.n.data(), l.type.data(), p.first.const_data_ptr(), p.second, (float)max_norm, (float)eps, norm.mutable_data_ptr(),
+            stream());
+    return norm;
+  }));
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* py_launches(PyObject*, PyObject*) { return PyLong_FromUnsignedLongLong(g_launches.load(std::memory_order_relaxed)); }
 
 // init(addresses: dict of name -> int, raise_error): the kernels' entry points of the library that ops/native.py has loaded
@@ -712,6 +988,8 @@ PyObject* py_init(PyObject*, PyObject* args) {
   LB_TAKE(lb_rmsnorm_fwd); LB_TAKE(lb_rmsnorm_bwd_blocks); LB_TAKE(lb_rmsnorm_bwd); LB_TAKE(lb_rope); LB_TAKE(lb_gemm_grouped_epi);
   LB_TAKE(lb_flash_fwd_tc); LB_TAKE(lb_flash_bwd_ws_bytes_kv); LB_TAKE(lb_flash_bwd_tc_ws); LB_TAKE(lb_flash_bwd); LB_TAKE(lb_embedding_fwd); LB_TAKE(lb_clear);
   LB_TAKE(lb_embedding_bwd); LB_TAKE(lb_ce_stats); LB_TAKE(lb_ce_loss); LB_TAKE(lb_ce_grad); LB_TAKE(lb_gemm_rope);
+  LB_TAKE(lb_attn_mask); LB_TAKE(lb_masked_attn_fwd); LB_TAKE(lb_masked_attn_bwd_ws_bytes); LB_TAKE(lb_masked_attn_bwd); LB_TAKE(lb_rope_axes);
+  LB_TAKE(lb_grad_norm_parts); LB_TAKE(lb_grad_squares); LB_TAKE(lb_grad_total); LB_TAKE(lb_grad_scale);
   if (!ok) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "an entry point of the kernels is missing");
     return nullptr;
@@ -723,7 +1001,7 @@ PyObject* py_init(PyObject*, PyObject* args) {
 
 #define LB_FAST(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {LB_FAST(linear), LB_FAST(swiglu_mlp), LB_FAST(rmsnorm), LB_FAST(attention), LB_FAST(rope_attention), LB_FAST(embedding),
-                         LB_FAST(cross_entropy), LB_FAST(decoder_layers), {"launches", py_launches, METH_NOARGS, nullptr}, {"init", py_init, METH_VARARGS, nullptr},
+                         LB_FAST(cross_entropy), LB_FAST(decoder_layers), LB_FAST(attention_mask), LB_FAST(masked_attention), LB_FAST(rope_axes), LB_FAST(grad_norm), LB_FAST(clip_grad_norm), {"launches", py_launches, METH_NOARGS, nullptr}, {"init", py_init, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

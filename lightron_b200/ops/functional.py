@@ -756,6 +756,8 @@ def attention_mask(documents: Optional[torch.Tensor] = None, prefix: Optional[to
     in a causal mask, as [B, S] marks (bool / uint8; the marked run at the document's start counts) or as [B] int32 lengths from the sequence's
     start (``length`` then gives S where there are no documents).  Values stay on the device.  (Values of padding are read all
     the same, and multiplied by weights of zero: they have to be finite, as those of causal attention have to be.)"""
+    if length is None and (host := native.host_ops()) is not None and (bounds := host.attention_mask(documents, prefix, causal)) is not NotImplemented:
+        return AttentionMask(*bounds, causal)
     if documents is None and prefix is None:
         raise ValueError("attention_mask needs documents or prefix (masked_attention takes causal=... alone)")
     if documents is not None and (documents.dim() != 2 or documents.dtype not in (torch.int32, torch.int64)):
@@ -904,6 +906,10 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Op
     """softmax(s) v for q [B, Sq, hq, d] and k, v [B, Sk, hkv, d] in any order of the outer dimensions; query i sits at position i + Sk - Sq.
     ``s = softcap * tanh(x / softcap) - slopes[h] * |distance|`` with ``x = scale * q.k`` (``softcap`` 0: x itself; ``slopes`` fp32 [hq], constants).
     ``mask``: see :func:`attention_mask`; without one, ``causal`` (default) or all keys.  Rows that see nothing give zeros, and gradients of zero."""
+    if (host := native.host_ops()) is not None and (mask is None or (type(mask) is AttentionMask and causal in (None, mask.causal))):
+        qb, kb, one_way = (None, None, causal is None or causal) if mask is None else (mask.q_bounds, mask.k_bounds, mask.causal)
+        if (o := host.masked_attention(q, k, v, qb, kb, slopes, one_way, scale, softcap)) is not NotImplemented:
+            return o
     causal = _check_masked(q, k, v, mask, causal, scale, softcap, slopes)
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
     qb, kb = (mask.q_bounds, mask.k_bounds) if mask is not None else (None, None)
@@ -969,6 +975,8 @@ def rope_axes(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: 
     """x [B, S, h, d] -> rotated copy: pair i of every head turns by row ``positions[axes[i]]`` of the tables [*, d/2] (interleaved pairs, as
     :func:`rope`).  ``positions`` [A, B, S] or [A, S]: time, height and width of every token, say; ``axes``: the axis of each of the d/2 pairs.  A position
     outside the tables makes its pairs NaN."""
+    if (host := native.host_ops()) is not None and (y := host.rope_axes(x, cos, sin, positions, axes)) is not NotImplemented:
+        return y
     if x.dim() != 4:
         raise ValueError(f"rope_axes takes x [B, S, h, d], got {tuple(x.shape)}")
     B, S, _, d = x.shape
@@ -1029,6 +1037,8 @@ def _reduce_sumsq(sumsq: torch.Tensor, group) -> torch.Tensor:
 def grad_norm(tensors, group=None) -> torch.Tensor:
     """2-norm of all elements of all tensors (bf16, fp16, fp32, mixed) together, a fp32 scalar on their device, without a host
     synchronisation and the same bits in every run.  ``group``: the tensors are this rank's share of one whole."""
+    if group is None and (host := native.host_ops()) is not None and (norm := host.grad_norm(tensors)) is not NotImplemented:
+        return norm
     tensors = _norm_list(tensors, "tensors")
     if not tensors or not tensors[0].is_cuda:
         return _reduce_sumsq(ref.grad_sumsq(tensors), group).sqrt()
@@ -1044,6 +1054,8 @@ def grad_norm(tensors, group=None) -> torch.Tensor:
 def clip_grad_norm(tensors, max_norm: float, out=None, group=None, eps: float = 1e-6) -> torch.Tensor:
     """Scales the tensors by ``min(1, max_norm / (norm + eps))`` and returns their norm (:func:`grad_norm`).  In place; or into ``out``, tensors of the same sizes
     and types.  A norm that is not finite goes into the result as it would in the product: NaN stays NaN, an infinite norm gives zeros and NaN."""
+    if group is None and (host := native.host_ops()) is not None and (norm := host.clip_grad_norm(tensors, max_norm, out, eps)) is not NotImplemented:
+        return norm
     tensors = _norm_list(tensors, "tensors")
     if not (max_norm >= 0.0 and eps >= 0.0):
         raise ValueError(f"max_norm {max_norm} and eps {eps} must not be negative")
@@ -1072,6 +1084,8 @@ def clip_grad_norm(tensors, max_norm: float, out=None, group=None, eps: float = 
         for d, o in zip(dst, outs):
             if d is not o:
                 o.copy_(d)
+            else:
+                torch.autograd.graph.increment_version(o)
     return norm
 
 

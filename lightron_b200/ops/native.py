@@ -273,7 +273,8 @@ def call(name: str, *args) -> None:
 _HOST = False               # not looked for yet; then the extension module, or None
 _HOST_ENTRIES = ("lb_rmsnorm_fwd", "lb_rmsnorm_bwd_blocks", "lb_rmsnorm_bwd", "lb_rope", "lb_gemm_grouped_epi", "lb_flash_fwd_tc",
                  "lb_flash_bwd_ws_bytes_kv", "lb_flash_bwd_tc_ws", "lb_flash_bwd", "lb_embedding_fwd", "lb_clear", "lb_embedding_bwd", "lb_ce_stats",
-                 "lb_ce_loss", "lb_ce_grad", "lb_gemm_rope")
+                 "lb_ce_loss", "lb_ce_grad", "lb_gemm_rope", "lb_attn_mask", "lb_masked_attn_fwd", "lb_masked_attn_bwd_ws_bytes", "lb_masked_attn_bwd", "lb_rope_axes",
+                 "lb_grad_norm_parts", "lb_grad_squares", "lb_grad_total", "lb_grad_scale")
 
 
 def host_ops():

@@ -178,6 +178,47 @@ def test_attention_on_another_stream_and_in_a_graph():
         assert rel(a, w) < 2e-3 and rel(b, w) < 2e-3
 
 
+def test_nodes_in_python_and_in_cpp(monkeypatch):
+    """The autograd functions in Python and the C++ nodes: the same bits (dq beyond 128 keys: the same up to the order of its sums), the same version counts."""
+    from lightron_b200.ops import functional as OF
+    from lightron_b200.ops import native
+    from lightron_b200.ops import reference as ref
+    assert native.host_ops() is not None
+    q, k, v, do = _rand(2, 100, 4, 64, seed=1), _rand(2, 120, 2, 64, seed=2), _rand(2, 120, 2, 64, seed=3), _rand(2, 100, 4, 64, seed=4)
+    ids, slopes = documents(2, 120, 30, seed=1).cuda(), torch.rand(4, device="cuda")
+    cos, sin = ref.rope_tables(64, 200, device="cuda")
+    pos = torch.arange(100, device="cuda", dtype=torch.int32).expand(3, 100).contiguous()
+    grads = [_rand(100, 33, seed=5), _rand(7, seed=6, dtype=torch.float32)]
+
+    def everything():
+        mask = OF.attention_mask(documents=ids)
+        x = q.detach().requires_grad_()
+        y = OF.rope_axes(x, cos, sin, pos, [0, 1, 2, 0] * 8)
+        mine = [g.clone() for g in grads]
+        before = [g._version for g in mine]
+        norm = OF.clip_grad_norm(mine, 1.0)
+        assert [g._version - n for g, n in zip(mine, before)] == [1, 1]
+        with torch.no_grad():
+            alone = OF.masked_attention(q, k, v, mask=mask, softcap=20.0)
+        return [mask.q_bounds, mask.k_bounds, *_run(q, k, v, do, mask=mask, softcap=20.0, slopes=slopes), alone, y, *torch.autograd.grad(y, x, do), OF.grad_norm(grads), norm, *mine]
+    fast = everything()
+    monkeypatch.setattr(native, "_HOST", None)
+    for a, b in zip(fast, everything()):
+        assert torch.equal(a, b)
+
+
+def test_saved_tensors_that_come_back_otherwise():
+    from lightron_b200.ops import functional as OF
+    q = _rand(1, 50, 2, 64).requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t):            # copies are fine
+        o = OF.masked_attention(q, q, q)
+    o.sum().backward()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t[:, :10], lambda t: t):
+        o = OF.masked_attention(q, q, q)
+    with pytest.raises(RuntimeError):
+        o.sum().backward()
+
+
 def test_attention_refusals_on_the_gpu():
     from lightron_b200.ops import functional as OF
     q = _rand(1, 8, 2, 136)
