@@ -25,10 +25,10 @@ static __device__ unsigned int g_ma_status[4] = {0, 0, 0, 0};
 namespace {
 using namespace bw;
 
-constexpr int THREADS = 256;
-// Registers per thread of the two warpgroups (two CTAs of 256 threads leave 128 per thread at launch).
-constexpr int REGS_ISSUE = 56, REGS_SOFTMAX = 200;
-static_assert(REGS_ISSUE + REGS_SOFTMAX <= 2 * 128, "a CTA has 256 x 128 registers");
+constexpr int THREADS = 384;
+// Registers per thread of the issuing and of the two softmax warpgroups (two CTAs of 384 threads leave 80 per thread at launch).
+constexpr int REGS_LAUNCH = 80, REGS_ISSUE = 48, REGS_SOFTMAX = 96;
+static_assert(REGS_ISSUE + 2 * REGS_SOFTMAX <= 3 * REGS_LAUNCH, "a CTA has 384 x 80 registers");
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct FwdParams {
@@ -55,9 +55,10 @@ struct Cfg {
   static constexpr int COL_S = 0, COL_O = 128, COL_P = P_ALIAS ? 0 : 192, TMEM_COLS = 256;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_RING = OFF_Q + ATOMS * SLOT_BYTES;
-  static constexpr int OFF_OUT = OFF_RING + SLOTS * SLOT_BYTES;   // 64 columns of O on their way out, 4 KB per softmax warp
-  static constexpr int OFF_BAR = OFF_OUT + SLOT_BYTES;
-  static constexpr int NBAR = 2 + 2 * SLOTS + 9;
+  // 2 KB per softmax warp: 32 rows x 32 columns of O on their way out, and before that what the rows' two threads tell each other
+  static constexpr int OFF_OUT = OFF_RING + SLOTS * SLOT_BYTES;
+  static constexpr int OFF_BAR = OFF_OUT + 8 * 2048;
+  static constexpr int NBAR = 2 + 2 * SLOTS + 12;
   static constexpr int SMEM = OFF_BAR + 256;
 };
 static_assert(Cfg<64>::SMEM <= 115712 && Cfg<128>::SMEM <= 115712, "two CTAs per SM");
@@ -147,9 +148,10 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
   auto full = [&](int s) { return bar0 + 8u * (2 + s); };
   auto empty = [&](int s) { return bar0 + 8u * (2 + C::SLOTS + s); };
   const uint32_t bar1 = bar0 + 8u * (2 + 2 * C::SLOTS);
-  const uint32_t s_full = bar1, s_free = bar1 + 8, p_half = bar1 + 16, p_full = bar1 + 24, pv_done = bar1 + 32;   // p_half: P of 64 keys
-  auto next_full = [&](int i) { return bar1 + 40u + 8u * i; };
-  auto next_empty = [&](int i) { return bar1 + 56u + 8u * i; };
+  const uint32_t s_full = bar1, s_free = bar1 + 8, p_full = bar1 + 16, pv_done = bar1 + 24;
+  auto next_full = [&](int i) { return bar1 + 32u + 8u * i; };
+  auto next_empty = [&](int i) { return bar1 + 48u + 8u * i; };
+  auto pair_bar = [&](int quad) { return bar1 + 64u + 8u * quad; };
   const uint32_t next_slot = (bar0 + 8u * C::NBAR + 15u) & ~15u;
 
   // One entry per (batch, head, query tile): the last tiles, which see most under a causal mask, of all heads of a group first; a group is as many heads as keep
@@ -188,10 +190,10 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     for (int s = 0; s < C::SLOTS; s++) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
     mbar_init(s_full, 1);
     mbar_init(pv_done, 1);
-    mbar_init(s_free, 4);
-    mbar_init(p_half, 4);
-    mbar_init(p_full, 4);
-    for (int i = 0; i < 2; i++) { mbar_init(next_full(i), 1); mbar_init(next_empty(i), 5); }   // the issuer and four softmax warps read
+    mbar_init(s_free, 8);
+    mbar_init(p_full, 8);
+    for (int i = 0; i < 4; i++) mbar_init(pair_bar(i), 2);
+    for (int i = 0; i < 2; i++) { mbar_init(next_full(i), 1); mbar_init(next_empty(i), 9); }   // the issuer and eight softmax warps read
     mbar_init_fence();
     prefetch_tmap(&tq); prefetch_tmap(&tk); prefetch_tmap(&tv); prefetch_tmap(&to); prefetch_tmap(&to_lo);
   }
@@ -252,8 +254,8 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       }
     } else if (warp == 1) {
       // ------------------------------- MMA issuer -------------------------------
-      // Per tile S(0); then per key block, 64 columns: S(j+1) as soon as the softmax threads hold S(j) in registers, and P(j) V in two halves as
-      // P(j) arrives; 128 columns: P(j) V, then S(j+1) into the columns that P(j) leaves.
+      // Per tile S(0); then per key block, 64 columns: S(j+1) as soon as the softmax threads hold S(j) in registers, and P(j) V when P(j) is there; 128
+      // columns: P(j) V, then S(j+1) into the columns that P(j) leaves.
       if (elect_one()) {
         const uint32_t idesc_s = make_idesc(C::BM, C::BN, 0, 0);
         const uint32_t idesc_o = make_idesc(C::BM, D, 0, 1);
@@ -290,10 +292,16 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         auto issue_pv = [&](bool first, bool last) -> bool {      // O += P V of block g, then release its slots of V
 #pragma unroll
           for (int half = 0; half < 2; half++) {
-            if ((D == 128 || half == 0) && !mbar_wait(full(vs), vp, abort_flag)) return false;
-            if (half == 1 && C::P_ALIAS && !last && !k_ready()) return false;
-            if (!mbar_wait(half ? p_full : p_half, g & 1u, abort_flag)) return false;
-            fence_after();
+            if (half == 0 && !mbar_wait(full(vs), vp, abort_flag)) return false;
+            if (half == 0) {
+              if (D == 128) {                           // the second half of V, ahead of the wait that is the last to come
+                const bool wrap = vs + 1 == C::SLOTS;
+                if (!mbar_wait(full(wrap ? 0 : vs + 1), wrap ? vp ^ 1u : vp, abort_flag)) return false;
+              }
+              if (C::P_ALIAS && !last && !k_ready()) return false;
+              if (!mbar_wait(p_full, g & 1u, abort_flag)) return false;
+              fence_after();
+            }
             const uint64_t va = dv0 + (uint64_t)((vs * C::SLOT_BYTES + (D == 128 ? 0 : half * 8192)) >> 4);
 #pragma unroll
             for (int s = 0; s < 4; s++)
@@ -306,11 +314,18 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           }
           return true;
         };
-        for (int n = 0, cta = (int)blockIdx.x; ok && cta >= 0; n++) {
-          const Tile t = tile_of(cta);
+        Tile t = tile_of((int)blockIdx.x);
+        for (int n = 0; ok; n++) {
           ok = k_ready() && mbar_wait(q_full, (uint32_t)n & 1u, abort_flag);
           if (ok && !C::P_ALIAS && n > 0) ok = mbar_wait(s_free, (g - 1) & 1u, abort_flag);
           if (ok) issue_s(t.nb == 1);
+          // (the next tile's size is on its way while this one is worked on)
+          const int cta = ok ? next_cta(n) : -1;
+          Tile next = t;
+          if (cta >= 0) {
+            mbar_arrive(next_empty(n & 1));
+            next = tile_of(cta);
+          }
           for (int j = 0; j < t.nb && ok; j++, g++) {
             const bool last = j + 1 == t.nb;
             if (!C::P_ALIAS && !last) {
@@ -320,21 +335,34 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             if (ok) ok = issue_pv(j == 0, last);
             if (C::P_ALIAS && ok && !last) issue_s(j + 2 == t.nb);
           }
-          if (!ok) break;
-          cta = next_cta(n);
-          if (cta >= 0) mbar_arrive(next_empty(n & 1));
+          if (cta < 0) break;
+          t = next;
         }
         if (!ok) atomicExch(&g_ma_status[0], 2u);
       }
     }
   } else {
     // ------------------------------- softmax warps -------------------------------
+    // A row is two threads', in the warps quad and quad + 4 of the eight: 64 columns of a key block each, and half of the columns of O.
     reg_inc<REGS_SOFTMAX>();
-    const int quad = warp & 3;
+    const int quad = warp & 3, set = warp >= 8 ? 1 : 0;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16);
-    const uint32_t ts_addr = lane_addr + C::COL_S, to_addr = lane_addr + C::COL_O, tp_addr = lane_addr + C::COL_P;
+    const uint32_t ts_addr = lane_addr + C::COL_S + set * 64, to_addr = lane_addr + C::COL_O + set * (D / 2), tp_addr = lane_addr + C::COL_P + set * 32;
     const f32x2 sl2x2 = pack2(pp.scale_l2, pp.scale_l2);
+    uint8_t* const out = smem + C::OFF_OUT + (warp - 4) * 2048;
+    float2* const mine = reinterpret_cast<float2*>(out) + lane;
+    const float2* const other = reinterpret_cast<float2*>(smem + C::OFF_OUT + ((warp - 4) ^ 4) * 2048) + lane;
     bool ok = true;
+    uint32_t turn = 0;
+    // The row's two threads meet (in a wait that ends, as all do); what the other one has in y.  Two places in turn: nobody is more than one meeting ahead.
+    auto meet = [&](float2 x, float2& y) {
+      mine[turn * 32] = x;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pair_bar(quad));
+      if (!mbar_wait(pair_bar(quad), turn, abort_flag)) ok = false;
+      y = other[turn * 32];
+      turn ^= 1u;
+    };
     auto arrive = [&](uint32_t bar) {              // once per warp
       fence_before();
       __syncwarp();
@@ -342,95 +370,61 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     };
     uint32_t g = 0;                                // key blocks so far, over all tiles
     bool s_ready = false;                          // S of the next block was seen complete
-    for (int n = 0, cta = (int)blockIdx.x; ok && cta >= 0; n++) {
-      const Tile t = tile_of(cta);
+    Tile t = tile_of((int)blockIdx.x);
+    // (rows past the last one are never stored: they are left unmasked)
+    auto keys_of = [&](const Tile& at) { const int row = at.m0 + quad * 32 + lane; return row < p.Sq ? ma_keys(p, at.b, row) : make_int2(0, 0x7fffffff); };
+    int2 see = keys_of(t);
+    for (int n = 0; ok; n++) {
       const int nb = t.nb, row = t.m0 + quad * 32 + lane, warp_at = t.m0 + quad * 32 + off;      // the row's place is row + off
-      // (rows past the last one are never stored: they are left unmasked)
-      const int2 see = row < p.Sq ? ma_keys(p, t.b, row) : make_int2(0, 0x7fffffff);
       [[maybe_unused]] float slope2 = 0.f;
       [[maybe_unused]] bool left_only = true;      // no row of the warp sees a key behind its own
       if constexpr (BIAS) {
         slope2 = p.slopes ? p.slopes[t.h] * LOG2E : 0.f;
         left_only = __all_sync(0xffffffffu, row >= p.Sq || see.y <= row + off + 1);
       }
-      float m_i = -INFINITY, m_s = 0.f, l_i = 0.f, lp_i = 0.f;      // running maximum, what exponentials are relative to, their sums
+      if (lane == 0) bulk_wait_read_but<0>();      // the last tile's O has left the place of the meetings
+      __syncwarp();
+      float m_i = -INFINITY, m_s = 0.f, l_i = 0.f, lp_i = 0.f;      // the row's running maximum, what exponentials are relative to, this thread's sums of them
       for (int j = 0; j < nb; j++, g++) {
         if (!s_ready && !mbar_wait(s_full, g & 1u, abort_flag)) { ok = false; break; }
         fence_after();
-        uint32_t r[128];
-        const int c0 = t.key0 + j * C::BN, lo = see.x - c0, hi = see.y - c0;       // visible columns
-        const bool need_mask = __any_sync(0xffffffffu, lo > 0 || hi < C::BN);
-        auto mask = [&](int i0) {
-          if (need_mask) {
-#pragma unroll
-            for (int w = i0; w < i0 + 64; w += 32) {
-              const uint32_t bits = ma_bits(lo, hi, w);
-#pragma unroll
-              for (int i = 0; i < 32; i++)
-                if (!(bits >> i & 1u)) r[w + i] = 0xff800000u;           // -inf
-            }
-          }
-        };
-        auto made = [&](int i0) {
-          if constexpr (MADE) {
-            const int side = left_only || c0 + i0 + 63 <= warp_at ? 1 : c0 + i0 >= warp_at + 31 ? -1 : 0;
-            scores64<CAP, BIAS>(r + i0, pp, slope2, side, c0 + i0 - (row + off));
-          }
-        };
-        // exponentials of 64 columns, packed as bf16 pairs (column c of P holds keys 2c, 2c+1)
-        auto exps = [&](int i0, uint32_t* pr, f32x2* rs2) {
-          const f32x2 nms2 = pack2(-m_s, -m_s);
-          rs2[0] = rs2[1] = pack2(0.f, 0.f);             // sums of the exponentials, and of them as P holds them
-#pragma unroll
-          for (int c = 0; c < 32; c++) {
-            const int i = i0 + c * 2;
-            float e0 = __uint_as_float(r[i]), e1 = __uint_as_float(r[i + 1]);
-            // (the difference first: with the maximum scaled ahead and a fused product, what its rounding left would be the exponent of scores far from zero)
-            if constexpr (CAP != CAP_ZERO) {
-              f32x2 x = add2(pack2(e0, e1), nms2);
-              if constexpr (!MADE) x = mul2(x, sl2x2);
-              unpack2(x, e0, e1);
-            }
-            e0 = exp2f(e0);
-            e1 = exp2f(e1);
-            bf162 pk = __floats2bfloat162_rn(e0, e1);
-            pr[c] = *reinterpret_cast<uint32_t*>(&pk);
-            rs2[0] = add2(rs2[0], pack2(e0, e1));
-            rs2[1] = add2(rs2[1], pack2(__uint_as_float(pr[c] << 16), __uint_as_float(pr[c] & 0xffff0000u)));
-          }
-        };
-        auto row_max = [&]() {                           // four independent chains
-          float mx4[4] = {m_i, m_i, m_i, m_i};
-#pragma unroll
-          for (int i = 0; i < 128; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-          return max2(max2(mx4[0], mx4[1]), max2(mx4[2], mx4[3]));
-        };
+        uint32_t r[64];
+        const int c0 = t.key0 + j * C::BN + set * 64, lo = see.x - c0, hi = see.y - c0;       // visible columns
+        const bool need_mask = __any_sync(0xffffffffu, lo > 0 || hi < 64);
         tmem_ld32(ts_addr, r);
         tmem_ld32(ts_addr + 32, r + 32);
-        tmem_ld32(ts_addr + 64, r + 64);
-        tmem_ld32(ts_addr + 96, r + 96);
         tmem_ld_wait();
         if (!C::P_ALIAS) arrive(s_free);                 // S may be overwritten by the next key block
-        uint32_t pr[32];
-        f32x2 rs2[2], rt2[2];
         const bool pv_ready = !C::P_ALIAS && j > 0 && mbar_test_wait(pv_done, (g - 1) & 1u);   // asked ahead of its use
-        bool any_grow = false;
+        if constexpr (MADE) {
+          const int side = left_only || c0 + 63 <= warp_at ? 1 : c0 >= warp_at + 31 ? -1 : 0;
+          scores64<CAP, BIAS>(r, pp, slope2, side, c0 - (row + off));
+        }
+        if (need_mask) {
+#pragma unroll
+          for (int w = 0; w < 64; w += 32) {
+            const uint32_t bits = ma_bits(lo, hi, w);
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+              if (!(bits >> i & 1u)) r[w + i] = 0xff800000u;           // -inf
+          }
+        }
+        bool rescale = false;
         float corr = 1.f;
-        made(0);
-        mask(0);
-        if constexpr (CAP == CAP_ZERO) {
-          exps(0, pr, rs2);
-        } else {
-          // Lazy reference maximum: the old one stays unless the new maximum is more than 2^8 above it, so that O and l rarely need rescaling.  So the
-          // first 64 exponentials are computed with the old one, and once more in the rare block where it may not stay.
-          made(64);
-          mask(64);
+        if constexpr (CAP != CAP_ZERO) {
+          // Lazy reference maximum: the old one stays unless the new maximum is more than 2^8 above it, so that O and l rarely need rescaling.
           const float unit = MADE ? 1.f : pp.scale_l2;
-          if (j > 0) exps(0, pr, rs2);
-          float m_new = row_max();
+          float mx4[4] = {m_i, m_i, m_i, m_i};           // four independent chains
+#pragma unroll
+          for (int i = 0; i < 64; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+          float m_new = max2(max2(mx4[0], mx4[1]), max2(mx4[2], mx4[3]));
+          float2 theirs;
+          meet(make_float2(m_new, 0.f), theirs);
+          m_new = max2(m_new, theirs.x);
           const bool grow = !(m_i != -INFINITY && (m_new - m_i) * unit <= 8.f);
-          any_grow = __any_sync(0xffffffffu, grow);
-          if (any_grow) {
+          if (__any_sync(0xffffffffu, grow)) {
+            // (where a row has seen nothing yet there is nothing to rescale)
+            rescale = __any_sync(0xffffffffu, grow && m_i != -INFINITY);
             if (!grow) m_new = m_i;
             // (a row with a score of +inf has no softmax: NaN, as inf - inf gives)
             m_s = (m_new == -INFINITY) ? 0.f : (m_new == INFINITY ? __int_as_float(0x7fffffff) : m_new);
@@ -438,8 +432,27 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             l_i *= corr;
             lp_i *= corr;
             m_i = m_new;
-            exps(0, pr, rs2);
           }
+        }
+        // exponentials, packed as bf16 pairs (column c of P holds keys 2c, 2c+1)
+        uint32_t pr[32];
+        f32x2 sum = pack2(0.f, 0.f), sump = pack2(0.f, 0.f);
+        const f32x2 nms2 = pack2(-m_s, -m_s);
+#pragma unroll
+        for (int c = 0; c < 32; c++) {
+          float e0 = __uint_as_float(r[2 * c]), e1 = __uint_as_float(r[2 * c + 1]);
+          // (the difference first: with the maximum scaled ahead and a fused product, what its rounding left would be the exponent of scores far from zero)
+          if constexpr (CAP != CAP_ZERO) {
+            f32x2 x = add2(pack2(e0, e1), nms2);
+            if constexpr (!MADE) x = mul2(x, sl2x2);
+            unpack2(x, e0, e1);
+          }
+          e0 = exp2f(e0);
+          e1 = exp2f(e1);
+          bf162 pk = __floats2bfloat162_rn(e0, e1);
+          pr[c] = *reinterpret_cast<uint32_t*>(&pk);
+          sum = add2(sum, pack2(e0, e1));
+          sump = add2(sump, pack2(__uint_as_float(pr[c] << 16), __uint_as_float(pr[c] & 0xffff0000u)));
         }
         if (j > 0) {
           // previous P V finished: O is stable and the P columns may be overwritten.  (128 columns: S(j) was issued behind it by the same thread, so
@@ -448,89 +461,96 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             if (!pv_ready && !mbar_wait(pv_done, (g - 1) & 1u, abort_flag)) { ok = false; break; }
             fence_after();
           }
-          if (CAP != CAP_ZERO && any_grow) {
+          if (CAP != CAP_ZERO && rescale) {
 #pragma unroll 1
-            for (int c = 0; c < D / 32; c++) {
-              uint32_t o[32];
-              tmem_ld32(to_addr + c * 32, o);
+            for (int c = 0; c < D / 2; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(to_addr + c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-              tmem_st32(to_addr + c * 32, o);
+              for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              tmem_st16(to_addr + c, o);
             }
-            tmem_st_wait();
           }
         }
-        // P goes back to TMEM, the first half in flight while the second is computed
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        if (C::P_ALIAS) {
+          // P takes columns of S that the row's other thread reads: both have by now where maxima were exchanged
+          if constexpr (CAP == CAP_ZERO) {
+            float2 none;
+            meet(make_float2(0.f, 0.f), none);
+          }
+        }
         tmem_st32(tp_addr, pr);
         tmem_st_wait();
-        arrive(p_half);
-        s_ready = !C::P_ALIAS && j + 1 < nb && mbar_test_wait(s_full, (g + 1) & 1u);
-        if constexpr (CAP == CAP_ZERO) {
-          made(64);
-          mask(64);
-        }
-        exps(64, pr, rt2);
-        tmem_st32(tp_addr + 32, pr);
-        tmem_st_wait();
         arrive(p_full);
-        rs2[0] = add2(rs2[0], rt2[0]);
-        rs2[1] = add2(rs2[1], rt2[1]);
-        float rs[4];
-        unpack2(rs2[0], rs[0], rs[1]);
-        unpack2(rs2[1], rs[2], rs[3]);
-        l_i += rs[0] + rs[1];
-        lp_i += rs[2] + rs[3];
+        s_ready = !C::P_ALIAS && j + 1 < nb && mbar_test_wait(s_full, (g + 1) & 1u);
+        float s0, s1, p0, p1;
+        unpack2(sum, s0, s1);
+        unpack2(sump, p0, p1);
+        l_i += s0 + s1;
+        lp_i += p0 + p1;
       }
-      if (ok) {
-        cta = next_cta(n);
-        __syncwarp();
-        if (lane == 0 && cta >= 0) mbar_arrive(next_empty(n & 1));
-      }
-      if (ok && !mbar_wait(pv_done, C::P_ALIAS ? (uint32_t)n & 1u : (g - 1) & 1u, abort_flag)) ok = false;
       if (!ok) break;
+      const int cta = next_cta(n);
+      __syncwarp();
+      Tile next = t;
+      int2 see_next = see;
+      if (cta >= 0) {
+        if (lane == 0) mbar_arrive(next_empty(n & 1));
+        next = tile_of(cta);
+        see_next = keys_of(next);
+      }
+      float2 theirs;
+      meet(make_float2(l_i, lp_i), theirs);
+      l_i += theirs.x;
+      lp_i += theirs.y;
+      float2 none;
+      meet(theirs, none);                          // (O takes the place of what the other one has read by now)
+      if (!ok || !mbar_wait(pv_done, C::P_ALIAS ? (uint32_t)n & 1u : (g - 1) & 1u, abort_flag)) ok = false;
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       fence_after();
       const float inv = lp_i != 0.f ? 1.f / lp_i : 0.f;
-      // 64 columns at a time through shared memory and TMA stores, which leave out rows past the last and columns past head_dim
-      uint8_t* out = smem + C::OFF_OUT + quad * 4096;
-#pragma unroll
-      for (int c = 0; c < C::ATOMS; c++) {
-        uint32_t r[64];
-        tmem_ld32(to_addr + c * 64, r);
-        tmem_ld32(to_addr + c * 64 + 32, r + 32);
-        tmem_ld_wait();
-        auto leave = [&](const CUtensorMap* map) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0 && t.m0 + quad * 32 < p.Sq) {
-            tma_store_4d(map, smem_u32(out), c * 64, t.h, t.m0 + quad * 32, t.b);
-            bulk_commit();
-          }
-        };
+      // 32 columns at a time through shared memory and TMA stores, which leave out rows past the last and columns past head_dim
+      auto leave = [&](const CUtensorMap* map, const uint4* v, int col) {      // v: 32 columns of the lane's row
         if (lane == 0) bulk_wait_read_but<0>();
         __syncwarp();
 #pragma unroll
-        for (int g8 = 0; g8 < 8; g8++) {
-          float f[8];
+        for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(out + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = v[i];      // (64-byte swizzle)
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && t.m0 + quad * 32 < p.Sq) {
+          tma_store_4d(map, smem_u32(out), col, t.h, t.m0 + quad * 32, t.b);
+          bulk_commit();
+        }
+      };
+#pragma unroll 1
+      for (int c = 0; c < D / 2; c += 32) {
+        uint32_t r[32];
+        uint4 hi[4];
+        tmem_ld32(to_addr + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int g8 = 0; g8 < 4; g8++) {
+          float f[8], back[8];
 #pragma unroll
           for (int i = 0; i < 8; i++) f[i] = __uint_as_float(r[g8 * 8 + i]) * inv;
-          const uint4 hi = pack8(f);
-          *reinterpret_cast<uint4*>(out + sw128_off(lane, g8)) = hi;
-          float back[8];
-          unpack8(hi, back);
+          hi[g8] = pack8(f);
+          unpack8(hi[g8], back);
 #pragma unroll
           for (int i = 0; i < 8; i++) r[g8 * 8 + i] = __float_as_uint(f[i] - back[i]);
         }
-        leave(&to);
+        leave(&to, hi, set * (D / 2) + c);
         if (p.o_lo) {
-          if (lane == 0) bulk_wait_read_but<0>();
-          __syncwarp();
 #pragma unroll
-          for (int g8 = 0; g8 < 8; g8++) *reinterpret_cast<uint4*>(out + sw128_off(lane, g8)) = pack8(reinterpret_cast<const float*>(r) + g8 * 8);
-          leave(&to_lo);
+          for (int g8 = 0; g8 < 4; g8++) hi[g8] = pack8(reinterpret_cast<const float*>(r) + g8 * 8);
+          leave(&to_lo, hi, set * (D / 2) + c);
         }
       }
-      if (row < p.Sq) p.lse[((long long)t.b * p.hq + t.h) * p.Sq + row] = l_i != 0.f ? m_s * (MADE ? LN2 : p.scale) + logf(l_i) : -INFINITY;
+      if (set == 0 && row < p.Sq) p.lse[((long long)t.b * p.hq + t.h) * p.Sq + row] = l_i != 0.f ? m_s * (MADE ? LN2 : p.scale) + logf(l_i) : -INFINITY;
+      if (cta < 0) break;
+      t = next;
+      see = see_next;
     }
     if (lane == 0) bulk_wait_read_but<0>();        // nothing reads shared memory after the CTA's end
     if (!ok && lane == 0) atomicExch(&g_ma_status[0], 3u);
@@ -552,7 +572,7 @@ int launch(const CUtensorMap* maps, const FwdParams& p, unsigned grid, cudaStrea
   if (!attr) {
     // the register split must fit in what the launch allocates, or it would wait for registers that nobody gives back
     cudaFuncAttributes fa;
-    if (cudaFuncGetAttributes(&fa, fn) != cudaSuccess || (fa.numRegs + 7) / 8 * 8 * 2 < REGS_ISSUE + REGS_SOFTMAX) return LB_ERR_LAUNCH;
+    if (cudaFuncGetAttributes(&fa, fn) != cudaSuccess || (fa.numRegs + 7) / 8 * 8 < REGS_LAUNCH) return LB_ERR_LAUNCH;
     cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     attr = true;
   }
@@ -567,8 +587,8 @@ int launch_fwd(const MaParams& a, cudaStream_t s) {
   if ((rc = make_map_bf16_4d(maps, a.q, d, hq, Sq, B, a.qs.h, a.qs.s, a.qs.b, 128))) return rc;
   if ((rc = make_map_bf16_4d(maps + 1, a.k, d, hkv, Sk, B, a.ks.h, a.ks.s, a.ks.b, 128))) return rc;
   if ((rc = make_map_bf16_4d(maps + 2, a.v, d, hkv, Sk, B, a.vs.h, a.vs.s, a.vs.b, 64))) return rc;
-  if ((rc = make_map_bf16_4d(maps + 3, a.o, d, hq, Sq, B, d, hq * d, Sq * hq * d, 32))) return rc;
-  if ((rc = make_map_bf16_4d(maps + 4, a.o_lo ? a.o_lo : a.o, d, hq, Sq, B, d, hq * d, Sq * hq * d, 32))) return rc;
+  if ((rc = make_map_bf16_4d(maps + 3, a.o, d, hq, Sq, B, d, hq * d, Sq * hq * d, 32, 32))) return rc;
+  if ((rc = make_map_bf16_4d(maps + 4, a.o_lo ? a.o_lo : a.o, d, hq, Sq, B, d, hq * d, Sq * hq * d, 32, 32))) return rc;
   FwdParams p;
   p.a = a;
   p.tiles_x = (a.Sq + 127) / 128;

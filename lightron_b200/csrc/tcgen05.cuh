@@ -290,6 +290,18 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+                 "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // One thread of a converged warp, chosen by the hardware.  Where the issuing thread of MMAs and TMA loads is chosen this way (and not
@@ -429,10 +441,10 @@ inline EncodeTiledFn get_encode() {
   return fn;
 }
 
-// bf16 tensor map of `rank` 2 to 4 with 128-byte swizzle.  Binds the CUDA context to the calling thread first (the
+// bf16 tensor map of `rank` 2 to 4, by default with 128-byte swizzle.  Binds the CUDA context to the calling thread first (the
 // driver call needs one; autograd worker threads may not have touched the runtime yet).
 inline int make_map_bf16_nd(CUtensorMap* m, const void* base, uint32_t rank, const cuuint64_t* dims, const cuuint64_t* strides,
-                            const cuuint32_t* box) {
+                            const cuuint32_t* box, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   static thread_local bool ctx_bound = false;
   if (!ctx_bound) {
     cudaFree(0);
@@ -442,7 +454,7 @@ inline int make_map_bf16_nd(CUtensorMap* m, const void* base, uint32_t rank, con
   if (!enc) return LB_ERR_DRIVER;
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     g_lb_last_cuda_error = (int)r;
@@ -465,13 +477,13 @@ inline int make_map_bf16_3d(CUtensorMap* m, const void* base, uint64_t inner, ui
   return make_map_bf16_nd(m, base, 3, dims, strides, box);
 }
 
-// [batches, rows, heads, d] with strides of sb, ss and sh elements (multiples of 8); box = box_rows rows of 64 columns of one head.  What lies outside of d or of
+// [batches, rows, heads, d] with strides of sb, ss and sh elements (multiples of 8); box = box_rows rows of 64 columns of one head, or of 32 (64-byte swizzle).  What lies outside of d or of
 // the rows is loaded as zeros and not stored.
 inline int make_map_bf16_4d(CUtensorMap* m, const void* base, uint64_t d, uint64_t heads, uint64_t rows, uint64_t batches, uint64_t sh, uint64_t ss, uint64_t sb,
-                            uint32_t box_rows) {
+                            uint32_t box_rows, uint32_t box_cols = 64) {
   const cuuint64_t dims[4] = {d, heads, rows, batches}, strides[3] = {sh * 2, ss * 2, sb * 2};
-  const cuuint32_t box[4] = {64, 1, box_rows, 1};
-  return make_map_bf16_nd(m, base, 4, dims, strides, box);
+  const cuuint32_t box[4] = {box_cols, 1, box_rows, 1};
+  return make_map_bf16_nd(m, base, 4, dims, strides, box, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 }  // namespace bw
