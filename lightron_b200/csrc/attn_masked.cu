@@ -84,7 +84,7 @@ int check_sizes(int B, int Sq, int Sk, int hq, int hkv, int d) {
 int fill(MaParams& p, const void* q, const void* k, const void* v, void* o, void* o_lo, void* lse, int B, int Sq, int Sk, int hq, int hkv, int d, const long long* st,
          float scale, int causal, float softcap, const void* slopes, const void* q_bounds, const void* k_bounds) {
   if (check_sizes(B, Sq, Sk, hq, hkv, d)) return LB_ERR_SHAPE;
-  if (!q || !k || !v || !o || !lse || !st || !(softcap >= 0.f && softcap < INFINITY) || !(scale >= 0.f && scale < INFINITY) || (!q_bounds) != (!k_bounds)) return LB_ERR_ARG;
+  if (!q || !k || !v || !o || !lse || !st || !(softcap >= 0.f && softcap < INFINITY) || !(scale > 0.f && scale < INFINITY) || (!q_bounds) != (!k_bounds)) return LB_ERR_ARG;
   if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(o) || misaligned(o_lo)) return LB_ERR_ARG;
   p = MaParams{(const bf16*)q, (const bf16*)k, (const bf16*)v, strides_at(st), strides_at(st + 3), strides_at(st + 6), (bf16*)o, (bf16*)o_lo, (float*)lse, B, Sq, Sk, hq, hkv, d,
                scale, causal, softcap, (const float*)slopes, (const int2*)q_bounds, (const int2*)k_bounds};

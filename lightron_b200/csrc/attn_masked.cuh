@@ -36,14 +36,30 @@ int ma_launch_fwd(const MaParams& p, cudaStream_t s);
 int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s);
 long long ma_bwd_ws_bytes(const MaParams& p);
 
-// tanh(x * by) * times = x * (c[0] + c[1] x^2 + c[2] x^4 + c[3] x^6) while |x| <= limit, which is 0.6 / by: relative error 2.2e-6 (coefficients of tanh(u) / u in u^2, found
-// by least squares over Chebyshev points with weights that were raised where the error was largest).
-inline void ma_tanh_terms(double by, double times, float* limit, float* c) {
-  const double k[4] = {0.9999978542327881, -0.33314040303230286, 0.13057856261730194, -0.04092942178249359};
-  *limit = (float)(0.6 / by);      // (a scale of zero: no limit)
-  double pw = by * times;
-  for (int i = 0; i < 4; i++, pw *= by * by) c[i] = (float)(k[i] * pw);
-}
+// What the kernels need of the scores' form, in units of log2: x * scale without a cap; with one, tanh(x * by) * times = x * (c[0] + c[1] x^2 + c[2] x^4 + c[3] x^6) while
+// |x| <= limit, which is 0.6 / by: relative error 2.2e-6 (coefficients of tanh(u) / u in u^2, found by least squares over Chebyshev points with weights that were raised
+// where the error was largest).  Pairs hold a value twice.
+struct MaTerms {
+  unsigned long long scale, cap, c[4];
+  float scale1, cap1, by2, limit;       // by2: 2 * log2(e) * by, for tanh by its definition
+  void set(const MaParams& p, bool times_cap, unsigned long long (*twice)(float)) {
+    const double log2e = 1.4426950408889634, k[4] = {0.9999978542327881, -0.33314040303230286, 0.13057856261730194, -0.04092942178249359};
+    scale1 = (float)(p.scale * log2e);
+    cap1 = (float)(p.softcap * log2e);
+    scale = twice(scale1);
+    cap = twice(cap1);
+    by2 = limit = 0.f;
+    const double by = p.softcap > 0.f ? (double)p.scale / p.softcap : 0.0;
+    double pw = by * (times_cap ? p.softcap * log2e : 1.0);
+    for (int i = 0; i < 4; i++, pw *= by * by) c[i] = twice((float)(k[i] * pw));
+    if (p.softcap > 0.f) {
+      by2 = (float)(2.0 * log2e * by);
+      limit = (float)(0.6 / by);
+    } else {
+      c[0] = scale;
+    }
+  }
+};
 
 // Bits [lo, hi) of 32 columns, of which column 0 is at `at`.
 __device__ __forceinline__ uint32_t ma_bits(int lo, int hi, int at) {

@@ -16,6 +16,7 @@
 // Warp roles (512 threads): warp 0 TMA producer, warp 1 MMA issuer + TMEM owner, warps 4-11 math, 12-15 dQ drain.
 // All waits are bounded; on expiry a status word is set and the CTA drains and frees its TMEM.
 #include <algorithm>
+#include <type_traits>
 #include "attn_masked.cuh"
 #include "tcgen05.cuh"
 
@@ -30,8 +31,8 @@ struct BwdParams {
   MaBwdParams w;
   float *dq_acc, *dk_acc, *dv_acc;
   int parts;                     // CTAs of a key block
-  // tanh(x * by_cap) = x * (c[0] + c[1] x^2 + ..) while |x| <= limit
-  float scale_l2, by_cap, cap_l2, limit, c[4];
+  MaTerms f;
+  f32x2 scale2;                  // the scale, twice
 };
 
 // (batch, kv head) pairs whose key blocks are ordered together: enough to keep the chip busy to the end, few enough that several key blocks of a pair run
@@ -440,8 +441,6 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     const int key = n0 + rit;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16);
     const uint32_t ts = lane_addr + C::COL_S + wg * 64, tdp = lane_addr + C::COL_DP + wg * 64;
-    const f32x2 sl2 = pack2(pp.scale_l2, pp.scale_l2);
-    const f32x2 sc = pack2(p.scale, p.scale);
     uint8_t* sds = smem + C::OFF_DS + wg * C::ATOM_BYTES;
     const int2 see = key < p.Sk ? ma_queries(p, b, key) : make_int2(0, 0);
     [[maybe_unused]] bool behind_only = true;       // no key of the warp is seen by a query ahead of it
@@ -471,62 +470,76 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           float top[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int i = 0; i < 64; i += 2) top[(i >> 1) & 3] = max3abs(top[(i >> 1) & 3], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
-          small = __all_sync(0xffffffffu, max2(max2(top[0], top[1]), max2(top[2], top[3])) <= pp.limit);
+          small = __all_sync(0xffffffffu, max2(max2(top[0], top[1]), max2(top[2], top[3])) <= pp.f.limit);
         }
         // distance to the columns' places: 1 all behind the key, -1 all ahead of it, 0 both
         const int first = m0 + off - key;
         int side = 1;
         if constexpr (BIAS) side = behind_only || m0 + off >= n0 + quad * 32 + 31 ? 1 : m0 + off + 63 <= n0 + quad * 32 ? -1 : 0;
-        const float slope = side > 0 ? -slope2 : side < 0 ? slope2 : 0.f;
+        const float slope = side > 0 ? -slope2 : slope2;
         const f32x2 step = pack2(2.f * slope, 2.f * slope);
         uint32_t pp_[32];
+        // (32 columns at a time; what a warp decides for all of them is decided outside of their loops, which would else be one pair after the other)
 #pragma unroll
         for (int w = 0; w < 64; w += 32) {
+          if constexpr (CAP) {                      // tanh
+            if (small) {
+#pragma unroll
+              for (int i = w; i < w + 32; i += 2) {
+                const f32x2 x = pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), u = mul2(x, x);
+                float t0, t1;
+                unpack2(mul2(x, fma2(u, fma2(u, fma2(u, pp.f.c[3], pp.f.c[2]), pp.f.c[1]), pp.f.c[0])), t0, t1);
+                sr[i] = __float_as_uint(t0);
+                sr[i + 1] = __float_as_uint(t1);
+              }
+            } else {
+#pragma unroll
+              for (int i = w; i < w + 32; i++)      // tanh u = 1 - 2 / (exp 2u + 1)
+                sr[i] = __float_as_uint(1.f - __fdividef(2.f, exp2f(__uint_as_float(sr[i]) * pp.f.by2) + 1.f));
+            }
+          }
+          auto weights = [&](auto both) {           // both: the columns are on both sides of the key
+            f32x2 add = pack2(0.f, 0.f);
+            if constexpr (BIAS) { const float base = slope * (float)(first + w); add = pack2(base, base + slope); }
+#pragma unroll
+            for (int i = w; i < w + 32; i += 2) {
+              const float2 nl = reinterpret_cast<const float2*>(st)[i >> 1];
+              const f32x2 x = pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+              f32x2 to = pack2(nl.x, nl.y);
+              if constexpr (BIAS && !decltype(both)::value) {
+                to = add2(to, add);
+                add = add2(add, step);
+              } else if constexpr (BIAS) {
+                to = pack2(fmaf(-slope2, fabsf((float)(first + i)), nl.x), fmaf(-slope2, fabsf((float)(first + i + 1)), nl.y));
+              }
+              unpack2(fma2(x, CAP ? pp.f.cap : pp.f.scale, to), pf[i], pf[i + 1]);
+              pf[i] = exp2f(pf[i]);
+              pf[i + 1] = exp2f(pf[i + 1]);
+            }
+          };
+          if (BIAS && side == 0) weights(std::true_type{}); else weights(std::false_type{});
           const uint32_t bits = ma_bits(lo, hi, w);
-          f32x2 add = pack2(0.f, 0.f);
-          if constexpr (BIAS) { const float base = slope * (float)(first + w); add = pack2(base, base + slope); }
+          if (need_mask) {
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+              if (!(bits >> i & 1u)) pf[w + i] = 0.f;
+          }
 #pragma unroll
           for (int i = w; i < w + 32; i += 2) {
-            const float2 nl = reinterpret_cast<const float2*>(st)[i >> 1];
-            f32x2 x = pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), to = pack2(nl.x, nl.y);
-            if constexpr (BIAS) {
-              to = add2(to, add);
-              add = add2(add, step);
-              if (side == 0) {
-                float t0, t1;
-                unpack2(to, t0, t1);
-                to = pack2(fmaf(-slope2, fabsf((float)(first + i)), t0), fmaf(-slope2, fabsf((float)(first + i + 1)), t1));
-              }
-            }
-            [[maybe_unused]] f32x2 dc;
-            if constexpr (CAP) {
-              f32x2 t;
-              if (small) {
-                const f32x2 u = mul2(x, x);
-                t = mul2(x, fma2(u, fma2(u, fma2(u, pack2(pp.c[3], pp.c[3]), pack2(pp.c[2], pp.c[2])), pack2(pp.c[1], pp.c[1])), pack2(pp.c[0], pp.c[0])));
-              } else {
-                const float by = 2.f * LOG2E * pp.by_cap;        // tanh u = 1 - 2 / (exp 2u + 1)
-                t = pack2(1.f - __fdividef(2.f, exp2f(__uint_as_float(sr[i]) * by) + 1.f), 1.f - __fdividef(2.f, exp2f(__uint_as_float(sr[i + 1]) * by) + 1.f));
-              }
-              dc = fma2(mul2(t, pack2(-1.f, -1.f)), t, pack2(1.f, 1.f));
-              x = fma2(t, pack2(pp.cap_l2, pp.cap_l2), to);
-            } else {
-              x = fma2(x, sl2, to);
-            }
-            float e0, e1;
-            unpack2(x, e0, e1);
-            e0 = exp2f(e0);
-            e1 = exp2f(e1);
-            float g0 = e0, g1 = e1;
-            if constexpr (CAP) unpack2(mul2(pack2(e0, e1), dc), g0, g1);
-            if (need_mask) {
-              if (!(bits >> (i - w) & 1u)) e0 = g0 = 0.f;
-              if (!(bits >> (i - w + 1) & 1u)) e1 = g1 = 0.f;
-            }
-            bf162 pb = __floats2bfloat162_rn(e0, e1);
+            bf162 pb = __floats2bfloat162_rn(pf[i], pf[i + 1]);
             pp_[i >> 1] = *reinterpret_cast<uint32_t*>(&pb);
-            pf[i] = g0;
-            pf[i + 1] = g1;
+          }
+          if constexpr (CAP) {
+#pragma unroll
+            for (int i = w; i < w + 32; i += 2) {   // P (1 - t^2)
+              const f32x2 e = pack2(pf[i], pf[i + 1]), t = pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+              unpack2(sub2(e, mul2(mul2(e, t), t)), pf[i], pf[i + 1]);
+            }
+            if (need_mask) {                        // (a hidden NaN is one still)
+#pragma unroll
+              for (int i = 0; i < 32; i++)
+                if (!(bits >> i & 1u)) pf[w + i] = 0.f;
+            }
           }
         }
         tmem_st32(ts, pp_);
@@ -548,9 +561,9 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           const float4 nd = st[32 + half * 8 + c];
           const int i = half * 32 + c * 4;
           const f32x2 d01 = mul2(pack2(pf[i], pf[i + 1]),
-                                 fma2(pack2(__uint_as_float(dr[c * 4]), __uint_as_float(dr[c * 4 + 1])), sc, pack2(nd.x, nd.y)));
+                                 fma2(pack2(__uint_as_float(dr[c * 4]), __uint_as_float(dr[c * 4 + 1])), pp.scale2, pack2(nd.x, nd.y)));
           const f32x2 d23 = mul2(pack2(pf[i + 2], pf[i + 3]),
-                                 fma2(pack2(__uint_as_float(dr[c * 4 + 2]), __uint_as_float(dr[c * 4 + 3])), sc, pack2(nd.z, nd.w)));
+                                 fma2(pack2(__uint_as_float(dr[c * 4 + 2]), __uint_as_float(dr[c * 4 + 3])), pp.scale2, pack2(nd.z, nd.w)));
           float d[4];
           unpack2(d01, d[0], d[1]);
           unpack2(d23, d[2], d[3]);
@@ -729,14 +742,8 @@ int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s) {
   p.dq_acc = w.stats + stats_floats(a);
   p.dk_acc = p.dq_acc + dq_floats(a);
   p.dv_acc = p.dk_acc + part_floats(a, p.parts);
-  p.scale_l2 = a.scale * LOG2E;
-  p.by_cap = p.cap_l2 = p.limit = p.c[0] = p.c[1] = p.c[2] = p.c[3] = 0.f;
-  if (a.softcap > 0.f) {
-    const double by = (double)a.scale / a.softcap;
-    p.by_cap = (float)by;
-    p.cap_l2 = a.softcap * LOG2E;
-    ma_tanh_terms(by, 1.0, &p.limit, p.c);
-  }
+  p.f.set(a, false, twice);
+  p.scale2 = twice(a.scale);
   return a.d <= 64 ? launch_bwd<64>(p, s) : launch_bwd<128>(p, s);
 }
 

@@ -37,8 +37,7 @@ struct FwdParams {
   int steal;                     // CTAs go on with entries that have not been started
   int group;                     // (batch, head) pairs whose tiles are ordered together
   FastDiv by_grp, by_group, by_last, by_hq, by_rep;    // entries of a group, heads of a group / of the last one, hq, hq / hkv
-  // scores in units of log2: x * scale_l2 without a cap; with one x * (c[0] + c[1] x^2 + ..) while |x| <= limit, else cap_l2 * tanh(x * by_cap)
-  float scale_l2, by_cap, cap_l2, limit, c[4];
+  MaTerms f;
 };
 
 enum : int { NO_CAP, CAP_ZERO, CAP_MAX };      // CAP_ZERO: exponentials relative to zero, CAP_MAX: to the running maximum
@@ -72,7 +71,7 @@ __device__ __forceinline__ void scores64(uint32_t* r, const FwdParams& p, float 
     float top[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 64; i += 2) top[(i >> 1) & 3] = max3abs(top[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-    small = __all_sync(0xffffffffu, max2(max2(top[0], top[1]), max2(top[2], top[3])) <= p.limit);
+    small = __all_sync(0xffffffffu, max2(max2(top[0], top[1]), max2(top[2], top[3])) <= p.f.limit);
   }
   const float slope = side < 0 ? -slope2 : slope2;
   const float step1 = side ? 2.f * slope : 0.f;
@@ -83,14 +82,13 @@ __device__ __forceinline__ void scores64(uint32_t* r, const FwdParams& p, float 
     const float base = slope * (float)(first + c0);
     f32x2 add = BIAS && side ? pack2(base, base + slope) : pack2(0.f, 0.f);
     if (CAP == NO_CAP || small) {
-      const f32x2 k0 = pack2(p.c[0], p.c[0]), k1 = pack2(p.c[1], p.c[1]), k2 = pack2(p.c[2], p.c[2]), k3 = pack2(p.c[3], p.c[3]);
 #pragma unroll
       for (int i = c0; i < c0 + 32; i += 2) {
         const f32x2 x = pack2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-        f32x2 f = k0;
+        f32x2 f = p.f.c[0];
         if constexpr (CAP != NO_CAP) {
           const f32x2 w = mul2(x, x);
-          f = fma2(w, fma2(w, fma2(w, k3, k2), k1), k0);
+          f = fma2(w, fma2(w, fma2(w, p.f.c[3], p.f.c[2]), p.f.c[1]), p.f.c[0]);
         }
         f32x2 y;
         if constexpr (BIAS) {
@@ -105,7 +103,7 @@ __device__ __forceinline__ void scores64(uint32_t* r, const FwdParams& p, float 
         r[i + 1] = __float_as_uint(y1);
       }
     } else if constexpr (CAP != NO_CAP) {
-      const float by = 2.f * LOG2E * p.by_cap;
+      const float by = p.f.by2;
 #pragma unroll
       for (int i = c0; i < c0 + 32; i += 2) {
         float a0, a1;
@@ -113,8 +111,8 @@ __device__ __forceinline__ void scores64(uint32_t* r, const FwdParams& p, float 
         if constexpr (BIAS) add = add2(add, step);
         // tanh u = 1 - 2 / (exp 2u + 1)
         const float t0 = 1.f - __fdividef(2.f, exp2f(__uint_as_float(r[i]) * by) + 1.f), t1 = 1.f - __fdividef(2.f, exp2f(__uint_as_float(r[i + 1]) * by) + 1.f);
-        r[i] = __float_as_uint(fmaf(p.cap_l2, t0, a0));
-        r[i + 1] = __float_as_uint(fmaf(p.cap_l2, t1, a1));
+        r[i] = __float_as_uint(fmaf(p.f.cap1, t0, a0));
+        r[i + 1] = __float_as_uint(fmaf(p.f.cap1, t1, a1));
       }
     }
   }
@@ -348,7 +346,6 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     const int quad = warp & 3, set = warp >= 8 ? 1 : 0;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16);
     const uint32_t ts_addr = lane_addr + C::COL_S + set * 64, to_addr = lane_addr + C::COL_O + set * (D / 2), tp_addr = lane_addr + C::COL_P + set * 32;
-    const f32x2 sl2x2 = pack2(pp.scale_l2, pp.scale_l2);
     uint8_t* const out = smem + C::OFF_OUT + (warp - 4) * 2048;
     float2* const mine = reinterpret_cast<float2*>(out) + lane;
     const float2* const other = reinterpret_cast<float2*>(smem + C::OFF_OUT + ((warp - 4) ^ 4) * 2048) + lane;
@@ -413,7 +410,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         float corr = 1.f;
         if constexpr (CAP != CAP_ZERO) {
           // Lazy reference maximum: the old one stays unless the new maximum is more than 2^8 above it, so that O and l rarely need rescaling.
-          const float unit = MADE ? 1.f : pp.scale_l2;
+          const float unit = MADE ? 1.f : pp.f.scale1;
           float mx4[4] = {m_i, m_i, m_i, m_i};           // four independent chains
 #pragma unroll
           for (int i = 0; i < 64; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
@@ -444,7 +441,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           // (the difference first: with the maximum scaled ahead and a fused product, what its rounding left would be the exponent of scores far from zero)
           if constexpr (CAP != CAP_ZERO) {
             f32x2 x = add2(pack2(e0, e1), nms2);
-            if constexpr (!MADE) x = mul2(x, sl2x2);
+            if constexpr (!MADE) x = mul2(x, pp.f.scale);
             unpack2(x, e0, e1);
           }
           e0 = exp2f(e0);
@@ -604,17 +601,10 @@ int launch_fwd(const MaParams& a, cudaStream_t s) {
   p.by_hq.set((unsigned)a.hq);
   p.by_rep.set((unsigned)(a.hq / a.hkv));
   p.steal = grid > 2 * lb_num_sms();      // (with all tiles resident at once there is none to take)
-  p.scale_l2 = p.c[0] = a.scale * LOG2E;
-  p.by_cap = p.cap_l2 = p.limit = p.c[1] = p.c[2] = p.c[3] = 0.f;
-  if (a.softcap > 0.f) {
-    const double by = (double)a.scale / a.softcap, l2 = (double)a.softcap * 1.4426950408889634;
-    p.by_cap = (float)by;
-    p.cap_l2 = (float)l2;
-    ma_tanh_terms(by, l2, &p.limit, p.c);
-  }
+  p.f.set(a, true, twice);
   const bool bias = a.slopes != nullptr;
   if (a.softcap <= 0.f) return bias ? launch<D, NO_CAP, true>(maps, p, (unsigned)grid, s) : launch<D, NO_CAP, false>(maps, p, (unsigned)grid, s);
-  if (p.cap_l2 <= 80.f) return bias ? launch<D, CAP_ZERO, true>(maps, p, (unsigned)grid, s) : launch<D, CAP_ZERO, false>(maps, p, (unsigned)grid, s);
+  if (p.f.cap1 <= 80.f) return bias ? launch<D, CAP_ZERO, true>(maps, p, (unsigned)grid, s) : launch<D, CAP_ZERO, false>(maps, p, (unsigned)grid, s);
   return launch<D, CAP_MAX, true>(maps, p, (unsigned)grid, s);
 }
 

@@ -388,6 +388,17 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
   return r;
 }
 
+__device__ __forceinline__ f32x2 sub2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("sub.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// A value for both halves, as a kernel parameter: the instructions above take it from there, where two of a scalar would be moved into registers for each use.
+inline f32x2 twice(float v) {
+  union { float f[2]; f32x2 x; } u = {{v, v}};
+  return u.x;
+}
+
 // Three-input maximum; a NaN in any input is the result.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;

@@ -876,8 +876,8 @@ def _check_masked(q, k, v, mask, causal, scale, softcap, slopes) -> bool:
         raise ValueError(f"{Sq} queries at the end of {Sk} positions")
     if not (k.dtype == v.dtype == q.dtype and k.device == v.device == q.device):
         raise ValueError(f"q, k, v differ in type or device: {q.dtype} {q.device}, {k.dtype} {k.device}, {v.dtype} {v.device}")
-    if scale is not None and not 0.0 <= scale < float("inf"):
-        raise ValueError(f"scale must be finite and not negative, got {scale}")
+    if scale is not None and not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
     if not (0.0 <= softcap < float("inf")):
         raise ValueError(f"softcap must be zero (none) or positive and finite, got {softcap}")
     if mask is not None:
