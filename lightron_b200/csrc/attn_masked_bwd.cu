@@ -130,8 +130,7 @@ __global__ void ma_bwd_prep_kernel(const __grid_constant__ BwdParams pp, const i
 }
 
 // fp32 accumulator layout: dQ tile (b, h, block of 128 rows), or dK / dV tile of a part -> 4 row quads -> D / 4 pieces of 4 columns -> 32 rows: the 16-byte stores of a
-// drain warp (a row per lane) are contiguous, and so are the 16-byte loads of a warp here.  A thread converts 32 columns of a row of dQ, or adds the parts of 8
-// columns of dK or dV.
+// drain warp (a row per lane) are contiguous.  A thread converts 8 columns of four rows of dQ, or adds the parts of 8 columns of a row of dK or dV.
 template <int D, bool CUT>
 __global__ void ma_convert_kernel(const __grid_constant__ BwdParams pp) {
   grid_go();
@@ -174,30 +173,32 @@ __global__ void ma_convert_kernel(const __grid_constant__ BwdParams pp) {
     }
     start -= 32 * pieces;                                      // dQ's pieces come next
   }
-  constexpr int CPR = D / 32;                                  // 32-column chunks per row
-  const long long total = (long long)p.B * p.hq * n_mblocks * 128 * CPR;
-  for (long long idx = start; idx < total; idx += threads) {
-    const int lane = (int)(idx & 31);
-    const long long w = idx >> 5;                              // (tile, quad, chunk): the accumulator's order
-    const int chunk = (int)(w % CPR), quad = (int)((w / CPR) & 3);
-    const long long tile = w / (CPR * 4);
-    const int mblock = (int)(tile % n_mblocks);
-    const long long bh = tile / n_mblocks;
-    const int row = mblock * 128 + quad * 32 + lane;
-    if (row >= p.Sq) continue;
-    const int h = (int)(bh % p.hq);
-    const long long b = bh / p.hq;
-    const float4* at = reinterpret_cast<const float4*>(pp.dq_acc) + (w * 8) * 32 + lane;
-    bf16* o = pp.w.dq + b * pp.w.dqs.b + row * pp.w.dqs.s + h * pp.w.dqs.h + chunk * 32;
-    float f[32];
+  // A warp takes RW rows at a time, whole: its stores are whole lines, its loads 16 bytes of RW neighbouring rows, all of four rounds in flight.  (A lane per row with 32
+  // columns, contiguous loads but stores of 16 bytes in 32 rows: 8 x 2048, 32 heads, d 64 54 us.)
+  constexpr int TPR = D / 8, RW = 32 / TPR, UNITS = 128 / (4 * RW);
+  const int lane = threadIdx.x & 31, c = lane % TPR, sub = lane / TPR;
+  const long long total = (long long)p.B * p.hq * n_mblocks * UNITS;
+  for (long long w = start >> 5; w < total; w += threads >> 5) {
+    const long long tile = w / UNITS;
+    const int first = (int)(w % UNITS) * 4 * RW + sub;          // row of the tile
+    const int mblock = (int)(tile % n_mblocks), h = (int)(tile / n_mblocks % p.hq), b = (int)(tile / n_mblocks / p.hq);
+    const float4* at = reinterpret_cast<const float4*>(pp.dq_acc) + tile * (32 * D) + 2 * c * 32;
+    float4 x[4][2];
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-      const float4 v = at[k * 32];
-      f[4 * k] = v.x; f[4 * k + 1] = v.y; f[4 * k + 2] = v.z; f[4 * k + 3] = v.w;
+    for (int k = 0; k < 4; k++) {
+      const int r = first + k * RW;
+      if (mblock * 128 + r < p.Sq && c * 8 < p.d) {
+        const float4* a = at + (r >> 5) * (8 * D) + (r & 31);
+        x[k][0] = __ldcs(a);
+        x[k][1] = __ldcs(a + 32);
+      }
     }
+    bf16* o = pp.w.dq + b * pp.w.dqs.b + h * pp.w.dqs.h + c * 8;
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-      if (chunk * 32 + k * 8 < p.d) *reinterpret_cast<uint4*>(o + k * 8) = pack8(f + k * 8);
+    for (int k = 0; k < 4; k++) {
+      const int row = mblock * 128 + first + k * RW;
+      if (row < p.Sq && c * 8 < p.d) *reinterpret_cast<uint4*>(o + row * pp.w.dqs.s) = pack8(reinterpret_cast<const float*>(x[k]));
+    }
   }
 }
 
@@ -716,7 +717,7 @@ int launch_bwd(BwdParams& p, cudaStream_t s) {
   rc = p.parts > 1 ? launch_form<D, PARTS>(m, p, (unsigned)grid, s) : alone ? launch_form<D, ALONE>(m, p, (unsigned)grid, s) : launch_form<D, WHOLE>(m, p, (unsigned)grid, s);
   if (rc || alone) return rc;
   const long long part_rows = p.parts > 1 ? 2LL * a.B * ((a.Sk + 127) / 128 * 128) * a.hkv : 0;
-  const long long cblocks = (rows * (D / 32) + part_rows * (D / 8) + 255) / 256;
+  const long long cblocks = (rows * (D / 32) + part_rows * (D / 8) + 255) / 256;      // (a thread takes 32 values of dQ)
   LB_LAUNCH(p.parts > 1 ? ma_convert_kernel<D, true> : ma_convert_kernel<D, false>, (int)(cblocks < cap ? cblocks : cap), 256, 0, s, p);
   return LB_OK;
 }

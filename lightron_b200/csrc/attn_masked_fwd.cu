@@ -346,6 +346,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     const int quad = warp & 3, set = warp >= 8 ? 1 : 0;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16);
     const uint32_t ts_addr = lane_addr + C::COL_S + set * 64, to_addr = lane_addr + C::COL_O + set * (D / 2), tp_addr = lane_addr + C::COL_P + set * 32;
+    [[maybe_unused]] const f32x2 scale2 = MADE ? 0 : kept(pp.f.scale);
     uint8_t* const out = smem + C::OFF_OUT + (warp - 4) * 2048;
     float2* const mine = reinterpret_cast<float2*>(out) + lane;
     const float2* const other = reinterpret_cast<float2*>(smem + C::OFF_OUT + ((warp - 4) ^ 4) * 2048) + lane;
@@ -433,7 +434,8 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         }
         // exponentials, packed as bf16 pairs (column c of P holds keys 2c, 2c+1)
         uint32_t pr[32];
-        f32x2 sum = pack2(0.f, 0.f), sump = pack2(0.f, 0.f);
+        f32x2 sum = pack2(0.f, 0.f);
+        float p0 = 0.f, p1 = 0.f;
         const f32x2 nms2 = pack2(-m_s, -m_s);
 #pragma unroll
         for (int c = 0; c < 32; c++) {
@@ -441,7 +443,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           // (the difference first: with the maximum scaled ahead and a fused product, what its rounding left would be the exponent of scores far from zero)
           if constexpr (CAP != CAP_ZERO) {
             f32x2 x = add2(pack2(e0, e1), nms2);
-            if constexpr (!MADE) x = mul2(x, pp.f.scale);
+            if constexpr (!MADE) x = mul2(x, scale2);
             unpack2(x, e0, e1);
           }
           e0 = exp2f(e0);
@@ -449,7 +451,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           bf162 pk = __floats2bfloat162_rn(e0, e1);
           pr[c] = *reinterpret_cast<uint32_t*>(&pk);
           sum = add2(sum, pack2(e0, e1));
-          sump = add2(sump, pack2(__uint_as_float(pr[c] << 16), __uint_as_float(pr[c] & 0xffff0000u)));
+          add_halves(pr[c], p0, p1);
         }
         if (j > 0) {
           // previous P V finished: O is stable and the P columns may be overwritten.  (128 columns: S(j) was issued behind it by the same thread, so
@@ -482,9 +484,8 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         tmem_st_wait();
         arrive(p_full);
         s_ready = !C::P_ALIAS && j + 1 < nb && mbar_test_wait(s_full, (g + 1) & 1u);
-        float s0, s1, p0, p1;
+        float s0, s1;
         unpack2(sum, s0, s1);
-        unpack2(sump, p0, p1);
         l_i += s0 + s1;
         lp_i += p0 + p1;
       }

@@ -399,6 +399,16 @@ inline f32x2 twice(float v) {
   return u.x;
 }
 
+// Adds the two halves of a packed bf16 pair to two sums.
+__device__ __forceinline__ void add_halves(uint32_t pair, float& lo, float& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.bf16 %0, l, %0;\n\tadd.rn.f32.bf16 %1, h, %1;\n\t}" : "+f"(lo), "+f"(hi) : "r"(pair));
+}
+// A value that stays in registers: the compiler would else fetch a kernel parameter anew for each use.
+__device__ __forceinline__ f32x2 kept(f32x2 x) {
+  asm volatile("" : "+l"(x));
+  return x;
+}
+
 // Three-input maximum; a NaN in any input is the result.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
