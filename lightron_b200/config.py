@@ -43,8 +43,19 @@ class ModelArgs:
     ep_size: int = 1
     sequence_parallel: bool = False
     cp_mode: str = "ring"                     # "ring" | "allgather" (both zig-zag causal) | "ulysses"
+    attn_softcap: float = 0.0                 # scores are capped at softcap * tanh(score / softcap); 0: not
+    attn_alibi: bool = False                  # scores fall with distance, head h by 2^(-8 (h + 1) / n_heads) a token
+    rope_sections: Optional[tuple] = None     # pairs of a head that turn by each axis of positions [axes, B, S]
 
     def __post_init__(self):
+        if self.rope_sections is not None:
+            self.rope_sections = tuple(int(n) for n in self.rope_sections)
+            if min(self.rope_sections, default=0) < 0 or sum(self.rope_sections) * 2 != self.head_dim:
+                raise ValueError(f"rope_sections {self.rope_sections} do not add up to the {self.head_dim // 2} pairs of a head")
+        if not 0.0 <= self.attn_softcap < float("inf"):
+            raise ValueError(f"attn_softcap must be zero (none) or positive and finite, got {self.attn_softcap}")
+        if self.cp_size > 1 and self.packed_attention:
+            raise ValueError("attn_softcap, attn_alibi and rope_sections are not built for context parallelism")
         if self.n_kv_heads is None:
             self.n_kv_heads = self.n_heads
         if self.dim % self.n_heads:
@@ -53,6 +64,11 @@ class ModelArgs:
             raise ValueError("n_heads must be a multiple of n_kv_heads")
         if self.cp_mode not in ("ring", "ulysses", "allgather"):
             raise ValueError(f"cp_mode must be ring|ulysses|allgather, got {self.cp_mode}")
+
+    @property
+    def packed_attention(self) -> bool:
+        """Whether the attention differs from plain causal attention with rotary positions on one axis."""
+        return bool(self.attn_softcap or self.attn_alibi or self.rope_sections)
 
     @property
     def head_dim(self) -> int:

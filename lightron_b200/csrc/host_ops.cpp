@@ -435,8 +435,9 @@ struct RopeAxes : Function<RopeAxes> {
   static Tensor turn(const Tensor& x0, const Tensor& cos, const Tensor& sin, const Tensor& pos, const unsigned char* axes, int inverse) {
     const Tensor x = fix_strides(x0);
     Tensor y = at::empty(x.sizes(), x.options());
-    L st[3];
+    L st[6];
     put_strides(st, x);
+    put_strides(st + 3, y);
     LB_CALL(lb_rope_axes, x.const_data_ptr(), y.mutable_data_ptr(), cos.const_data_ptr(), sin.const_data_ptr(), pos.const_data_ptr(), axes, (int)pos.size(0), (int)x.size(0), (int)x.size(1),
             (int)x.size(2), (int)x.size(3), (int)cos.size(0), st, pos.stride(0), pos.dim() == 3 ? pos.stride(1) : 0, inverse, stream());
     return y;

@@ -10,7 +10,7 @@ struct RopeAxesParams {
   bf16* y;
   const float *cosT, *sinT;
   const int* positions;          // [axes, B, S], or [axes, S] with pos_b = 0
-  long long xb, xs, xh, pos_a, pos_b;
+  long long xb, xs, xh, yb, ys, yh, pos_a, pos_b;
   int B, S, h, d, rows, inverse;
   int share;                     // heads of a warp
   unsigned char axis[MAX_PAIRS];
@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const __grid_constant__ 
   const int b = (int)(tok / p.S), s = (int)(tok - (long long)b * p.S);
   const int h0 = (int)blockIdx.y * p.share, h1 = min(p.h, h0 + p.share);
   const bf16* x = p.x + b * p.xb + s * p.xs + v * 8;
-  bf16* y = p.y + tok * p.h * p.d + v * 8;
+  bf16* y = p.y + b * p.yb + s * p.ys + v * 8;
   uint4 a[AHEAD];
   auto load = [&](int h) {
 #pragma unroll
@@ -53,21 +53,22 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const __grid_constant__ 
         float f[8];
         unpack8(a[i], f);
         rope_rotate8(cs, f, p.inverse != 0);
-        *reinterpret_cast<uint4*>(y + (long long)(h + i * G) * p.d) = pack8(f);
+        *reinterpret_cast<uint4*>(y + (h + i * G) * p.yh) = pack8(f);
       }
   }
 }
 
 }  // namespace
 
-// y [B, S, h, d] = x turned (back, with inverse).  x: strides {batch, token, head} in elements, multiples of 8, innermost contiguous; cos, sin fp32 [rows, d / 2];
+// y = x [B, S, h, d] turned (back, with inverse).  strides: {batch, token, head} of x, then of y, in elements, multiples of 8, innermost contiguous; y may be x; cos, sin fp32 [rows, d / 2];
 // positions int32, axis a of token (b, s) at a * pos_a + b * pos_b + s; axes: host bytes, the axis (0 to n_axes - 1) of each of the d / 2 pairs.
 extern "C" int lb_rope_axes(const void* x, void* y, const void* cosT, const void* sinT, const void* positions, const unsigned char* axes, int n_axes, int B, int S, int h, int d,
                             int rows, const long long* strides, long long pos_a, long long pos_b, int inverse, void* stream) {
   if (B <= 0 || S <= 0 || h <= 0 || rows <= 0 || d <= 0 || d % 8 || d > 2 * MAX_PAIRS || n_axes <= 0 || n_axes > MAX_AXES) return LB_ERR_SHAPE;
   if (!x || !y || !cosT || !sinT || !positions || !axes || !strides || ((uintptr_t)x | (uintptr_t)y | (uintptr_t)cosT | (uintptr_t)sinT) & 15) return LB_ERR_ARG;
-  if ((strides[0] | strides[1] | strides[2]) % 8) return LB_ERR_SHAPE;
-  RopeAxesParams p{(const bf16*)x, (bf16*)y, (const float*)cosT, (const float*)sinT, (const int*)positions, strides[0], strides[1], strides[2], pos_a, pos_b, B, S, h, d, rows, inverse, h, {}};
+  for (int i = 0; i < 6; i++)
+    if (strides[i] % 8) return LB_ERR_SHAPE;
+  RopeAxesParams p{(const bf16*)x, (bf16*)y, (const float*)cosT, (const float*)sinT, (const int*)positions, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], pos_a, pos_b, B, S, h, d, rows, inverse, h, {}};
   for (int i = 0; i < d / 2; i++) {
     if (axes[i] >= n_axes) return LB_ERR_ARG;
     p.axis[i] = axes[i];

@@ -113,15 +113,31 @@ class Attention(nn.Module):
         self.wk = _col(args, args.dim, args.n_kv_heads * d, ctx, **kw)
         self.wv = _col(args, args.dim, args.n_kv_heads * d, ctx, **kw)
         self.wo = _row(args, args.n_heads * d, args.dim, ctx, **kw)
+        self.packed = args.packed_attention
+        self.softcap = args.attn_softcap
+        self.axes = None if args.rope_sections is None else tuple(a for a, n in enumerate(args.rope_sections) for _ in range(n))
+        self._slopes = None
+        if args.attn_alibi:           # of this rank's heads
+            first = ctx.tp_rank * self.n_heads if tp > 1 else 0
+            self._slopes = 2.0 ** (-8.0 * (torch.arange(first, first + self.n_heads, dtype=torch.float32) + 1) / args.n_heads)
 
-    def forward(self, x: torch.Tensor, B: int, S: int, cos, sin, positions) -> torch.Tensor:
-        """x [T(/tp if SP), H] -> [T(/tp), H]; T = B*S with S the local (per-CP-rank) length."""
+    def slopes(self, device) -> Optional[torch.Tensor]:
+        if self._slopes is not None and self._slopes.device != device:
+            self._slopes = self._slopes.to(device)
+        return self._slopes
+
+    def forward(self, x: torch.Tensor, B: int, S: int, cos, sin, positions, mask=None) -> torch.Tensor:
+        """x [T(/tp if SP), H] -> [T(/tp), H]; T = B*S with S the local (per-CP-rank) length.  ``mask``: ``ops.functional.attention_mask`` of a packed batch."""
         if self.sp:
             qkv = fused.all_gather_linear(x, (self.wq.weight, self.wk.weight, self.wv.weight), self.tp_group)
         else:
             qkv = OF.linear(comm.copy_to_group(x, self.tp_group), self.wq.weight, self.wk.weight, self.wv.weight)
         hq, hkv, d = self.n_heads, self.n_kv_heads, self.head_dim
-        if self.cp_group is None:
+        if self.cp_group is None and (self.packed or mask is not None or (positions is not None and positions.dim() > 1)):
+            o = OF.packed_attention_qkv(qkv, cos, sin, positions, B, S, hq, hkv, d, axes=self.axes, mask=mask, softcap=self.softcap, slopes=self.slopes(qkv.device))
+        elif mask is not None:
+            raise ValueError("packed batches are not built for context parallelism")
+        elif self.cp_group is None:
             o = OF.rope_attention_qkv(qkv, cos, sin, positions, B, S, hq, hkv, d)
         else:
             from ..parallel import cp
@@ -144,14 +160,14 @@ class TransformerBlock(nn.Module):
         self.attention_norm = RMSNorm(args.dim, eps=args.norm_eps, **kw)
         self.ffn_norm = RMSNorm(args.dim, eps=args.norm_eps, **kw)
 
-    def forward(self, h, delta, B, S, cos, sin, positions):
+    def forward(self, h, delta, B, S, cos, sin, positions, mask=None):
         """Carries the residual stream as (h, delta) with h + delta pending, so that each add is
         fused with the following norm.  Returns the next (h, delta)."""
         if delta is None:
             x = OF.rmsnorm(h, self.attention_norm.weight, self.attention_norm.eps)
         else:
             h, x = OF.add_rmsnorm(delta, h, self.attention_norm.weight, self.attention_norm.eps)
-        a = self.attention(x, B, S, cos, sin, positions)
+        a = self.attention(x, B, S, cos, sin, positions) if mask is None else self.attention(x, B, S, cos, sin, positions, mask=mask)
         h, x = OF.add_rmsnorm(a, h, self.ffn_norm.weight, self.ffn_norm.eps)
         f = self.feed_forward(x)
         return h, f
@@ -173,7 +189,7 @@ def _plain_layers(layers: nn.ModuleDict):
         att, ff = mods.get("attention"), mods.get("feed_forward")
         if type(blk) is not TransformerBlock or type(att) is not Attention or type(ff) is not MLP:
             return None
-        if att.tp_group is not None or att.cp_group is not None or ff.tp_group is not None:
+        if att.tp_group is not None or att.cp_group is not None or ff.tp_group is not None or att.packed:
             return None
         for m in (blk, att, ff):
             if m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks or "forward" in m.__dict__:
@@ -243,15 +259,16 @@ class LightronTransformer(nn.Module):
             return comm.reduce_from_group(part, self.tp_group)
         return OF.embedding(flat, self.tok_embeddings.weight, 0)
 
-    def run_layers(self, h, delta, B, S, positions):
+    def run_layers(self, h, delta, B, S, positions, mask=None):
         cos, sin = self.rope_tables(h.device)
         if positions is not None and h.is_cuda:
             positions = positions.to(device=h.device, dtype=torch.int32)
-        if not torch.is_grad_enabled() and (host := native.host_ops()) is not None and (run := _plain_layers(self.layers)) is not None:
+        plain = mask is None and (positions is None or positions.dim() == 1)
+        if plain and not torch.is_grad_enabled() and (host := native.host_ops()) is not None and (run := _plain_layers(self.layers)) is not None:
             if (out := host.decoder_layers(h, delta, cos, sin, positions, B, S, *run)) is not NotImplemented:
                 return out
         for blk in self.layers.values():
-            h, delta = blk(h, delta, B, S, cos, sin, positions)
+            h, delta = blk(h, delta, B, S, cos, sin, positions) if mask is None else blk(h, delta, B, S, cos, sin, positions, mask=mask)
         return h, delta
 
     def head(self, h, delta) -> torch.Tensor:
@@ -265,12 +282,12 @@ class LightronTransformer(nn.Module):
         return OF.linear(comm.copy_to_group(x, self.tp_group), self.output.weight)
 
     # ---- stage-level API (pipeline parallel uses this directly) --------------------------
-    def forward_stage(self, x: torch.Tensor, B: int, S: int, positions=None) -> torch.Tensor:
+    def forward_stage(self, x: torch.Tensor, B: int, S: int, positions=None, mask=None) -> torch.Tensor:
         """First stage: x = tokens [B,S]; other stages: x = hidden [T(/tp), H].
         Returns hidden [T(/tp), H], or local logits [T, V/tp] on the last stage."""
         self.aux_losses = []
         h = self.embed(x) if self.first_stage else x
-        h, delta = self.run_layers(h, None, B, S, positions)
+        h, delta = self.run_layers(h, None, B, S, positions, mask)
         if self.last_stage:
             return self.head(h, delta)
         return h if delta is None else h + delta
@@ -292,20 +309,21 @@ class LightronTransformer(nn.Module):
         return aux
 
     # ---- user-level API ---------------------------------------------------------------------
-    def forward(self, tokens: torch.Tensor, positions=None) -> torch.Tensor:
+    def forward(self, tokens: torch.Tensor, positions=None, mask=None) -> torch.Tensor:
         """tokens [B, S] -> logits [B, S, V] (full vocab on every TP rank, as the reference's
         ``gather_output=True`` head, model/model.py:243)."""
         assert self.first_stage and self.last_stage, "forward() needs the whole model; use forward_stage under PP"
         B, S = tokens.shape
-        logits = self.forward_stage(tokens, B, S, positions)
+        logits = self.forward_stage(tokens, B, S, positions, mask)
         logits = comm.gather_cols(logits, self.tp_group)
         return logits.view(B, S, -1)
 
     def loss(self, tokens: torch.Tensor, targets: torch.Tensor, positions=None,
-             n_tokens: Optional[int] = None) -> torch.Tensor:
-        """Token-mean next-token NLL (+ MoE aux loss) without materialising gathered logits."""
+             n_tokens: Optional[int] = None, mask=None) -> torch.Tensor:
+        """Token-mean next-token NLL (+ MoE aux loss) without materialising gathered logits.  Packed batches: ``mask`` of
+        ``ops.functional.attention_mask``, ``positions`` [B, S], or [axes, B, S] with ``rope_sections``, and ``n_tokens``, the number of targets that are not -100."""
         B, S = tokens.shape
-        logits = self.forward_stage(tokens, B, S, positions)
+        logits = self.forward_stage(tokens, B, S, positions, mask)
         loss = self.loss_from_logits(logits, targets, n_tokens)
         aux = self.collect_aux_loss()
         if aux is not None:

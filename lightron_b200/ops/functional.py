@@ -925,11 +925,11 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Op
 
 
 def _rope_axes_native(x, out, cos, sin, positions, axes, inverse: bool) -> None:
-    """x [B, S, h, d] strided (:func:`_strided_ok`), out contiguous (or x itself, contiguous)."""
+    """x and out [B, S, h, d] strided (:func:`_strided_ok`); out may be x."""
     B, S, h, d = x.shape
     pos_a, pos_b = positions.stride(0), positions.stride(1) if positions.dim() == 3 else 0
     native.call("lb_rope_axes", x.data_ptr(), out.data_ptr(), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), bytes(axes), positions.shape[0], B, S, h, d,
-                cos.shape[0], _strides(x), pos_a, pos_b, int(inverse), native.stream_ptr())
+                cos.shape[0], _strides(x, out), pos_a, pos_b, int(inverse), native.stream_ptr())
 
 
 class _RopeAxes(torch.autograd.Function):
@@ -988,6 +988,64 @@ def rope_axes(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: 
     return ref.rope_axes(x, cos, sin, positions, axes)
 
 
+class _PackedAttnQKV(torch.autograd.Function):
+    """Rotation by axes + masked attention straight on the fused projection output, as :class:`_RopeAttnQKV`: q and k are rotated in place inside ``qkv``, which the caller
+    hands over, and backward writes one dqkv tensor whose q, k columns it turns back in place."""
+
+    @staticmethod
+    def _views(t, B, S, hq, hkv, d):
+        heads = t.view(B, S, hq + 2 * hkv, d)
+        return heads[:, :, :hq + hkv], heads[:, :, :hq], heads[:, :, hq:hq + hkv], heads[:, :, hq + hkv:]
+
+    @staticmethod
+    def forward(ctx, qkv, cos, sin, positions, slopes, qb, kb, axes, dims, causal, scale, softcap):
+        qk, q, k, v = _PackedAttnQKV._views(qkv, *dims)
+        with native.on_device(qkv):
+            _rope_axes_native(qk, qk, cos, sin, positions, axes, False)
+            o, o_lo, lse = masked_fwd_native(q, k, v, causal, scale, softcap, slopes, qb, kb, not isinstance(ctx, _NoGradCtx) and ctx.needs_input_grad[0])
+        ctx.save_for_backward(qkv, o, o_lo, lse, cos, sin, positions, slopes, qb, kb)
+        ctx.args = (axes, dims, causal, scale, softcap)
+        return o.view(qkv.shape[0], -1)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        qkv, o, o_lo, lse, cos, sin, positions, slopes, qb, kb = ctx.saved_tensors
+        axes, dims, causal, scale, softcap = ctx.args
+        dqkv = torch.empty_like(qkv)
+        _, q, k, v = _PackedAttnQKV._views(qkv, *dims)
+        dqk, dq, dk, dv = _PackedAttnQKV._views(dqkv, *dims)
+        with native.on_device(qkv):
+            masked_bwd_native(q, k, v, o, o_lo, lse, do.reshape(o.shape), causal, scale, softcap, slopes, qb, kb, dq, dk, dv)
+            _rope_axes_native(dqk, dqk, cos, sin, positions, axes, True)
+        return (dqkv,) + (None,) * 11
+
+
+def packed_attention_qkv(qkv: torch.Tensor, cos, sin, positions, B: int, S: int, hq: int, hkv: int, d: int, axes: Optional[Sequence[int]] = None,
+                         mask: Optional[AttentionMask] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`rope_attention_qkv` for packed batches: qkv [B*S, (hq+2hkv)*d] -> [B*S, hq*d] by :func:`rope_axes` on q and k and :func:`masked_attention`.
+    ``positions``: None (each token's place), [S], [B, S] (as of documents that count from zero) or, with ``axes``, [A, B, S] or [A, S]."""
+    if positions is None:
+        positions = torch.arange(S, device=qkv.device, dtype=torch.int32)
+    if axes is None:
+        positions, axes = positions[None], (0,) * (d // 2)
+    if qkv.dim() != 2 or qkv.shape != (B * S, (hq + 2 * hkv) * d):
+        raise ValueError(f"qkv {tuple(qkv.shape)} is not [{B} * {S}, ({hq} + 2 * {hkv}) * {d}]")
+    positions, axes = _check_axes(B, S, d, cos, sin, positions, axes)
+    heads = qkv.view(B, S, hq + 2 * hkv, d)
+    q, k, v = heads[:, :, :hq], heads[:, :, hq:hq + hkv], heads[:, :, hq + hkv:]
+    causal = _check_masked(q, k, v, mask, None, None, softcap, slopes)
+    if native.use_native(qkv) and qkv.numel() and positions.shape[0] <= 8:
+        _check_masked_native(d)
+        if not qkv.is_contiguous() or qkv.data_ptr() % 16:
+            qkv = qkv.clone(memory_format=torch.contiguous_format)
+        qb, kb = (mask.q_bounds, mask.k_bounds) if mask is not None else (None, None)
+        return _apply(_PackedAttnQKV, qkv, cos.contiguous(), sin.contiguous(), positions, None if slopes is None else slopes.contiguous(), qb, kb, axes, (B, S, hq, hkv, d), causal,
+                      1.0 / math.sqrt(d), float(softcap))
+    q, k = rope_axes(q, cos, sin, positions, axes), rope_axes(k, cos, sin, positions, axes)
+    return masked_attention(q, k, v, mask=mask, softcap=softcap, slopes=slopes).reshape(B * S, hq * d)
+
+
 # --------------------------------------------------------------------------------------
 # Global gradient norm and clipping
 # --------------------------------------------------------------------------------------
@@ -1027,34 +1085,42 @@ def _grad_parts(tensors, device):
     return parts, filled.value
 
 
-def _reduce_sumsq(sumsq: torch.Tensor, group) -> torch.Tensor:
-    if group is not None and dist.get_world_size(group) > 1:
-        dist.all_reduce(sumsq, group=group)
+def _norm_groups(group) -> list:
+    groups = [] if group is None else list(group) if isinstance(group, (list, tuple)) else [group]
+    return [g for g in groups if g is not None and dist.get_world_size(g) > 1]
+
+
+def _reduce_sumsq(sumsq: torch.Tensor, groups) -> torch.Tensor:
+    for g in groups:
+        dist.all_reduce(sumsq, group=g)
     return sumsq
 
 
 @torch.no_grad()
 def grad_norm(tensors, group=None) -> torch.Tensor:
     """2-norm of all elements of all tensors (bf16, fp16, fp32, mixed) together, a fp32 scalar on their device, without a host
-    synchronisation and the same bits in every run.  ``group``: the tensors are this rank's share of one whole."""
-    if group is None and (host := native.host_ops()) is not None and (norm := host.grad_norm(tensors)) is not NotImplemented:
+    synchronisation and the same bits in every run.  ``group``: the tensors are this rank's share of one whole (a process group, or
+    several over which the squares are summed one after the other)."""
+    groups = _norm_groups(group)
+    if not groups and (host := native.host_ops()) is not None and (norm := host.grad_norm(tensors)) is not NotImplemented:
         return norm
     tensors = _norm_list(tensors, "tensors")
     if not tensors or not tensors[0].is_cuda:
-        return _reduce_sumsq(ref.grad_sumsq(tensors), group).sqrt()
+        return _reduce_sumsq(ref.grad_sumsq(tensors), groups).sqrt()
     with native.on_device(tensors[0]):
         parts, n = _grad_parts(tensors, tensors[0].device)
         out = torch.empty((), dtype=torch.float32, device=tensors[0].device)
-        whole = group is None or dist.get_world_size(group) == 1
+        whole = not groups
         native.call("lb_grad_total", parts.data_ptr(), n, 0 if whole else out.data_ptr(), out.data_ptr() if whole else 0, native.stream_ptr())
-    return out if whole else _reduce_sumsq(out, group).sqrt()
+    return out if whole else _reduce_sumsq(out, groups).sqrt()
 
 
 @torch.no_grad()
 def clip_grad_norm(tensors, max_norm: float, out=None, group=None, eps: float = 1e-6) -> torch.Tensor:
     """Scales the tensors by ``min(1, max_norm / (norm + eps))`` and returns their norm (:func:`grad_norm`).  In place; or into ``out``, tensors of the same sizes
     and types.  A norm that is not finite goes into the result as it would in the product: NaN stays NaN, an infinite norm gives zeros and NaN."""
-    if group is None and (host := native.host_ops()) is not None and (norm := host.clip_grad_norm(tensors, max_norm, out, eps)) is not NotImplemented:
+    groups = _norm_groups(group)
+    if not groups and (host := native.host_ops()) is not None and (norm := host.clip_grad_norm(tensors, max_norm, out, eps)) is not NotImplemented:
         return norm
     tensors = _norm_list(tensors, "tensors")
     if not (max_norm >= 0.0 and eps >= 0.0):
@@ -1063,7 +1129,7 @@ def clip_grad_norm(tensors, max_norm: float, out=None, group=None, eps: float = 
     if len(outs) != len(tensors) or any(o.shape != t.shape or o.dtype != t.dtype or o.device != t.device for o, t in zip(outs, tensors)):
         raise ValueError("out must be one tensor of the same size, type and device for each tensor")
     if not tensors or not tensors[0].is_cuda:
-        norm = _reduce_sumsq(ref.grad_sumsq(tensors), group).sqrt()
+        norm = _reduce_sumsq(ref.grad_sumsq(tensors), groups).sqrt()
         by = (max_norm / (norm + eps)).clamp_max(1.0)
         for t, o in zip(tensors, outs):
             o.copy_((t.float() * by).to(t.dtype))
@@ -1074,10 +1140,10 @@ def clip_grad_norm(tensors, max_norm: float, out=None, group=None, eps: float = 
         src = [t if _dense(t) else t.contiguous() for t in tensors]
         dst = [o if o is t or (o.stride() == t.stride() and _dense(o)) else torch.empty_like(t) for t, o in zip(src, outs)]
         parts, n = _grad_parts(src, dev)
-        if group is not None and dist.get_world_size(group) > 1:
+        if groups:
             sumsq = torch.empty(1, dtype=torch.float32, device=dev)
             native.call("lb_grad_total", parts.data_ptr(), n, sumsq.data_ptr(), 0, native.stream_ptr())
-            parts, n = _reduce_sumsq(sumsq, group), 1
+            parts, n = _reduce_sumsq(sumsq, groups), 1
         norm = torch.empty((), dtype=torch.float32, device=dev)
         k, sp, counts, types = _norm_table(src)
         native.call("lb_grad_scale", k, sp, _norm_table(dst)[1], counts, types, parts.data_ptr(), n, float(max_norm), float(eps), norm.data_ptr(), native.stream_ptr())

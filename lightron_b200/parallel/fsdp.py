@@ -227,8 +227,11 @@ class FSDPOptimizer:
     ``torch.optim.AdamW`` on the fp32 master shards): the same small interface as
     ``optim.DistributedAdamW`` and ``fsdp_native.NativeFSDP``."""
 
-    def __init__(self, model: nn.Module, lr: float, weight_decay: float, betas=(0.9, 0.999), eps: float = 1e-8):
+    def __init__(self, model: nn.Module, lr: float, weight_decay: float, betas=(0.9, 0.999), eps: float = 1e-8, grad_clip: float = 0.0, groups=()):
+        """``grad_clip``: limit of the gradients' global norm (0: none), whose squares are summed over ``groups``, the process groups that hold
+        different shards."""
         self.model, self.state = model, model._fsdp
+        self.grad_clip, self.groups, self.last_grad_norm = grad_clip, list(groups), None
         self.opt = self.state.make_optimizer(lr=lr, weight_decay=weight_decay, betas=betas, eps=eps)
         self.step_count = 0
         self.shard_numel = sum(u.shard_len for u in self.state.units)
@@ -243,6 +246,9 @@ class FSDPOptimizer:
         pass
 
     def step(self) -> None:
+        if self.grad_clip > 0:
+            from ..ops import functional as OF
+            self.last_grad_norm = OF.clip_grad_norm([u.shard.grad for u in self.state.units if u.shard.grad is not None], self.grad_clip, group=self.groups)
         self.opt.step()
         self.step_count += 1
 

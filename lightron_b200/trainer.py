@@ -138,7 +138,8 @@ class Trainer:
             if d.pp_size == 1 and not any(getattr(p, "is_expert", False) for p in net.parameters()):
                 self.engine = f"fsdp (library collectives: {why_not})"
                 fsdp_lib.apply_fsdp2(net, ctx=ctx, param_dtype=self.dtype)
-                return fsdp_lib.FSDPOptimizer(net, lr=t.learning_rate, weight_decay=t.weight_decay, betas=t.betas, eps=t.eps)
+                return fsdp_lib.FSDPOptimizer(net, lr=t.learning_rate, weight_decay=t.weight_decay, betas=t.betas, eps=t.eps, grad_clip=t.grad_clip,
+                                              groups=(ctx.dpcp_group, ctx.tp_group))
             if ctx.rank == 0:
                 print(f"[lightron] distributed.fsdp ignored for this layout ({why_not}); using the sharded-optimizer engine",
                       flush=True)

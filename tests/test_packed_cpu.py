@@ -109,6 +109,101 @@ def test_norm_and_clip():
     assert float(OF.grad_norm([])) == 0.0 and float(OF.clip_grad_norm([], 1.0)) == 0.0
 
 
+def _packed_model(**kw):
+    from lightron_b200 import mesh
+    from lightron_b200.config import ModelArgs
+    from lightron_b200.models import LightronTransformer, init_weights
+    mesh.set_context(None)
+    args = ModelArgs(dim=32, n_layers=2, n_heads=4, n_kv_heads=2, vocab_size=64, intermediate_size=48, max_seq_len=64, **kw)
+    model = LightronTransformer(args, dtype=torch.float32, device="cpu")
+    init_weights(model, 0, std=0.2)
+    return model
+
+
+@pytest.mark.parametrize("kw", [{}, dict(attn_softcap=5.0), dict(attn_alibi=True), dict(rope_sections=(2, 1, 1), attn_softcap=3.0)])
+def test_packed_model_is_its_documents(kw):
+    """Logits of documents packed into one sequence, with positions of their own: those of each document alone."""
+    model = _packed_model(**kw)
+    lens = [5, 9, 3]
+    tokens = torch.randint(0, 64, (1, sum(lens)), generator=torch.Generator().manual_seed(0))
+    ids = torch.cat([torch.full((n,), i) for i, n in enumerate(lens)])[None]
+    pos = torch.cat([torch.arange(n) for n in lens])[None]
+    if "rope_sections" in kw:
+        pos = torch.stack([pos, pos // 2, pos % 3])
+    packed = model(tokens, positions=pos, mask=OF.attention_mask(documents=ids))
+    at = 0
+    for n in lens:
+        alone = model(tokens[:, at:at + n], positions=pos[..., at:at + n])
+        assert torch.allclose(packed[:, at:at + n], alone, atol=1e-5)
+        at += n
+    loss = model.loss(tokens, tokens, positions=pos, mask=OF.attention_mask(documents=ids))
+    loss.backward()
+    assert all(torch.isfinite(p.grad).all() for p in model.parameters())
+
+
+def _example():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "packed_documents.py")
+    spec = importlib.util.spec_from_file_location("packed_documents", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def test_example_runs():
+    losses = _example().main(["--steps", "4", "--batch", "2", "--seq-length", "96", "--dim", "64", "--layers", "1", "--device", "cpu"])
+    assert len(losses) == 4 and all(0 < x < 20 for x in losses)
+
+
+@pytest.mark.gpu
+def test_example_learns_on_the_gpu():
+    losses = _example().main(["--steps", "30", "--device", "cuda"])
+    assert losses[-1] < losses[0] - 0.3
+
+
+def test_model_arguments_are_checked():
+    from lightron_b200.config import ModelArgs
+    for bad in (dict(rope_sections=(2, 1)), dict(attn_softcap=-1.0), dict(attn_alibi=True, cp_size=2)):
+        with pytest.raises(ValueError):
+            ModelArgs(dim=32, n_heads=4, **bad)
+
+
+def _clipped_worker(rank, world, clip):
+    from lightron_b200 import mesh
+    from lightron_b200.parallel import apply_fsdp2
+    from lightron_b200.parallel.fsdp import FSDPOptimizer
+    ctx = mesh.setup_distributed(dp_size=world, backend="gloo")
+    model = _packed_model()
+    apply_fsdp2(model, ctx=ctx, param_dtype=torch.float32)
+    opt = FSDPOptimizer(model, lr=1e-2, weight_decay=0.0, grad_clip=clip, groups=(ctx.dpcp_group, ctx.tp_group))
+    tokens = torch.randint(0, 64, (2, 8), generator=torch.Generator().manual_seed(1))
+    norms = []
+    for _ in range(2):
+        opt.zero_grad()
+        model.loss(tokens[rank % 2:rank % 2 + 1], tokens[rank % 2:rank % 2 + 1].roll(-1, 1)).backward()
+        opt.step()
+        norms.append(float(opt.last_grad_norm))
+    return {k: v.numpy().copy() for k, v in model._fsdp.full_state_dict().items()}, norms
+
+
+def test_sharded_optimizer_clips_by_the_global_norm():
+    from dist_utils import run_distributed
+    (got, norms), (_, other) = run_distributed(_clipped_worker, 2, 0.05)
+    assert norms == other
+    model = _packed_model()
+    opt = torch.optim.AdamW(model.parameters(), lr=1e-2, weight_decay=0.0)
+    tokens = torch.randint(0, 64, (2, 8), generator=torch.Generator().manual_seed(1))
+    for n in norms:
+        opt.zero_grad()
+        model.loss(tokens, tokens.roll(-1, 1)).backward()
+        want = torch.nn.utils.clip_grad_norm_(model.parameters(), 0.05)
+        assert abs(n / float(want) - 1) < 1e-4
+        opt.step()
+    for k, v in model.state_dict().items():
+        assert torch.allclose(torch.from_numpy(got[k]), v, atol=1e-4), k
+
+
 def _attn(**kw):
     a = dict(q=torch.zeros(2, 4, 4, 8), k=torch.zeros(2, 4, 2, 8), v=torch.zeros(2, 4, 2, 8))
     a.update(kw)

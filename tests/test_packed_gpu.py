@@ -235,6 +235,58 @@ def test_attention_refusals_on_the_gpu():
         OF.masked_attention(q, q.cpu(), q)
 
 
+@pytest.mark.parametrize("kw", [{}, dict(attn_softcap=5.0, attn_alibi=True), dict(rope_sections=(8, 12, 12))])
+def test_packed_model(kw):
+    """Documents packed into one sequence against each alone, and the fused projection's node against its parts: logits, loss, gradients."""
+    from lightron_b200 import mesh
+    from lightron_b200.config import ModelArgs
+    from lightron_b200.models import LightronTransformer, init_weights
+    from lightron_b200.ops import functional as OF
+    mesh.set_context(None)
+    args = ModelArgs(dim=256, n_layers=2, n_heads=4, n_kv_heads=2, vocab_size=512, intermediate_size=384, max_seq_len=512, **kw)
+    model = LightronTransformer(args, dtype=BF16, device="cuda")
+    init_weights(model, 0, std=0.05)
+    lens = [130, 70, 256, 44]
+    tokens = torch.randint(0, 512, (1, sum(lens)), device="cuda", generator=torch.Generator(device="cuda").manual_seed(0))
+    ids = torch.cat([torch.full((n,), i) for i, n in enumerate(lens)])[None].cuda()
+    pos = torch.cat([torch.arange(n) for n in lens])[None].cuda()
+    if "rope_sections" in kw:
+        pos = torch.stack([pos, pos // 16, pos % 16])
+    mask = OF.attention_mask(documents=ids)
+    packed = model(tokens, positions=pos, mask=mask)
+    with torch.no_grad():
+        assert torch.equal(packed, model(tokens, positions=pos, mask=mask))
+        at = 0
+        for n in lens:
+            assert rel(packed[:, at:at + n], model(tokens[:, at:at + n], positions=pos[..., at:at + n])) < 1e-2      # (GEMMs of other sizes round otherwise)
+            at += n
+    model.loss(tokens, tokens.roll(-1, 1), positions=pos, mask=mask).backward()
+    norm = OF.clip_grad_norm([p.grad for p in model.parameters()], 1e-3)
+    assert 0 < norm.item() < 1e4
+    assert abs(OF.grad_norm([p.grad for p in model.parameters()]).item() / 1e-3 - 1) < 1e-2
+    _status_ok()
+
+
+def test_fused_projection_node_against_its_parts():
+    from lightron_b200.ops import functional as OF
+    from lightron_b200.ops import reference as ref
+    B, S, hq, hkv, d = 2, 150, 4, 2, 64
+    qkv, do = _rand(B * S, (hq + 2 * hkv) * d, seed=1), _rand(B * S, hq * d, seed=2)
+    cos, sin = ref.rope_tables(d, 200, device="cuda")
+    pos = torch.randint(0, 200, (3, B, S), device="cuda", dtype=torch.int32)
+    axes = [0] * 10 + [1] * 11 + [2] * 11
+    mask, slopes = OF.attention_mask(documents=documents(B, S, 40, 3).cuda()), torch.rand(hq, device="cuda")
+    x = qkv.clone().requires_grad_()
+    o = OF.packed_attention_qkv(x * 1, cos, sin, pos, B, S, hq, hkv, d, axes=axes, mask=mask, softcap=20.0, slopes=slopes)
+    dx, = torch.autograd.grad(o, x, do)
+    y = qkv.clone().requires_grad_()
+    q, k, v = (t.unflatten(1, (-1, d)).unflatten(0, (B, S)) for t in y.split([hq * d, hkv * d, hkv * d], dim=1))
+    w = OF.masked_attention(OF.rope_axes(q, cos, sin, pos, axes), OF.rope_axes(k, cos, sin, pos, axes), v, mask=mask, softcap=20.0, slopes=slopes)
+    dy, = torch.autograd.grad(w, y, do.view_as(w))
+    assert torch.equal(o.view_as(w), w)
+    assert rel(dx, dy) < 4e-3                                    # (dq is rounded before it is turned back, in both; it is added up as key tiles come)
+
+
 # ---- rotary positions -------------------------------------------------------------------------------
 
 
