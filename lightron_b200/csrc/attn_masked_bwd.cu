@@ -31,6 +31,7 @@ struct BwdParams {
   MaBwdParams w;
   float *dq_acc, *dk_acc, *dv_acc;
   int parts;                     // CTAs of a key block
+  int acc_d;                     // columns of dq_acc: head_dim in whole pieces of 32
   MaTerms f;
   f32x2 scale2;                  // the scale, twice
 };
@@ -103,8 +104,8 @@ __global__ void ma_bwd_prep_kernel(const __grid_constant__ BwdParams pp, const i
       const long long bi = idx / p.hq;
       b = (int)(bi / Sp);
       i = (int)(bi % Sp);
-      if (clear) {
-        float4* z = reinterpret_cast<float4*>(pp.dq_acc + (idx * TPR + sub) * 8);
+      if (clear && sub * 8 < pp.acc_d) {
+        float4* z = reinterpret_cast<float4*>(pp.dq_acc + idx * pp.acc_d + sub * 8);
         z[0] = make_float4(0.f, 0.f, 0.f, 0.f);
         z[1] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
@@ -129,7 +130,7 @@ __global__ void ma_bwd_prep_kernel(const __grid_constant__ BwdParams pp, const i
   }
 }
 
-// fp32 accumulator layout: dQ tile (b, h, block of 128 rows), or dK / dV tile of a part -> 4 row quads -> D / 4 pieces of 4 columns -> 32 rows: the 16-byte stores of a
+// fp32 accumulator layout: dQ tile (b, h, block of 128 rows), or dK / dV tile of a part -> 4 row quads -> acc_d / 4 (D / 4) pieces of 4 columns -> 32 rows: the 16-byte stores of a
 // drain warp (a row per lane) are contiguous.  A thread converts 8 columns of four rows of dQ, or adds the parts of 8 columns of a row of dK or dV.
 template <int D, bool CUT>
 __global__ void ma_convert_kernel(const __grid_constant__ BwdParams pp) {
@@ -182,13 +183,13 @@ __global__ void ma_convert_kernel(const __grid_constant__ BwdParams pp) {
     const long long tile = w / UNITS;
     const int first = (int)(w % UNITS) * 4 * RW + sub;          // row of the tile
     const int mblock = (int)(tile % n_mblocks), h = (int)(tile / n_mblocks % p.hq), b = (int)(tile / n_mblocks / p.hq);
-    const float4* at = reinterpret_cast<const float4*>(pp.dq_acc) + tile * (32 * D) + 2 * c * 32;
+    const float4* at = reinterpret_cast<const float4*>(pp.dq_acc) + tile * (32 * pp.acc_d) + 2 * c * 32;
     float4 x[4][2];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       const int r = first + k * RW;
       if (mblock * 128 + r < p.Sq && c * 8 < p.d) {
-        const float4* a = at + (r >> 5) * (8 * D) + (r & 31);
+        const float4* a = at + (r >> 5) * (8 * pp.acc_d) + (r & 31);
         x[k][0] = __ldcs(a);
         x[k][1] = __ldcs(a + 32);
       }
@@ -319,8 +320,9 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     // ------------------------------- MMA issuer -------------------------------
     if (total_it > 0 && elect_one()) {
       const uint32_t idesc_s = make_idesc(128, 128, 0, 0);     // S^T, dP^T: K-major A and B
-      const uint32_t idesc_kv = make_idesc(128, D, 0, 1);      // dV, dK: A in TMEM, MN-major B
-      const uint32_t idesc_dq = make_idesc(128, D, 1, 1);      // dQ: MN-major A and B
+      const int slices = (p.d + 15) / 16;                      // of 16 columns: those past head_dim are zeros, and left out of all products
+      const uint32_t idesc_kv = make_idesc(128, slices * 16, 0, 1);      // dV, dK: A in TMEM, MN-major B
+      const uint32_t idesc_dq = make_idesc(128, slices * 16, 1, 1);      // dQ: MN-major A and B
       const uint64_t kK = make_desc(sbase + C::OFF_K, 16, 1024), kV = make_desc(sbase + C::OFF_V, 16, 1024);
       const uint64_t kQ = make_desc(sbase + C::OFF_Q, 16, 1024), kDO = make_desc(sbase + C::OFF_DO, 16, 1024);
       const uint64_t mK = make_desc(sbase + C::OFF_K, C::ATOM_BYTES, 1024), mDS = make_desc(sbase + C::OFF_DS, C::ATOM_BYTES, 1024);
@@ -329,7 +331,7 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
 #pragma unroll
         for (int s = 0; s < D / 16; s++) {
           const uint64_t o = (uint64_t)(((s >> 2) * C::ATOM_BYTES + (s & 3) * 32) >> 4);
-          umma_bf16(tmem_base + col, a + o, bq + o, idesc_s, s ? 1u : 0u);
+          if (s < slices) umma_bf16(tmem_base + col, a + o, bq + o, idesc_s, s ? 1u : 0u);
         }
       };
       // A (P^T or dS^T): 16 queries of a warpgroup's 64 are 8 columns; the second warpgroup's start 64 columns on
@@ -411,9 +413,10 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             if (k * 8 < p.d) *reinterpret_cast<uint4*>(o + k * 8) = pack8(reinterpret_cast<const float*>(r) + k * 8);
         }
       } else {
-        float* tile = pp.dq_acc + (((long long)b * p.hq + h) * n_mblocks + mb) * (128 * D) + quad * (32 * D);
+        float* tile = pp.dq_acc + (((long long)b * p.hq + h) * n_mblocks + mb) * (128 * pp.acc_d) + quad * (32 * pp.acc_d);
 #pragma unroll
         for (int c = 0; c < D / 32; c++) {
+          if (c * 32 >= p.d) break;
           uint8_t* sp = stg + (c & 1) * C::STG_BYTES;
           if (lane == 0) bulk_wait_read_but<1>();      // this half of the staging has been read
           __syncwarp();
@@ -595,7 +598,7 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       float* sum = (wg ? pp.dk_acc : pp.dv_acc) + (((long long)nblk * p.hkv * p.B + pair) * pp.parts + part) * (128 * D) + quad * (32 * D);
       uint8_t* out = smem + (wg ? C::OFF_V : C::OFF_K) + quad * C::STG_BYTES;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; c++) {
+      for (int c = 0; c < D / 32 && c * 32 < p.d; c++) {
         uint32_t r[32];
         tmem_ld32(lane_addr + (wg ? C::COL_DK : C::COL_DV) + c * 32, r);
         tmem_ld_wait();
@@ -724,7 +727,8 @@ int launch_bwd(BwdParams& p, cudaStream_t s) {
 
 // Bytes of the workspace: row statistics, fp32 dQ (up to 128 keys: none), fp32 dK and dV of the parts.
 long long stats_floats(const MaParams& p) { return (long long)p.B * p.hq * ((p.Sq + 127) / 128) * 256; }
-long long dq_floats(const MaParams& p) { return p.Sk <= 128 ? 0 : stats_floats(p) / 2 * (p.d <= 64 ? 64 : 128); }
+int acc_columns(int d) { return (d + 31) / 32 * 32; }
+long long dq_floats(const MaParams& p) { return p.Sk <= 128 ? 0 : stats_floats(p) / 2 * acc_columns(p.d); }
 long long part_floats(const MaParams& p, int parts) {
   return parts > 1 ? (long long)p.B * p.hkv * ((p.Sk + 127) / 128) * parts * 128 * (p.d <= 64 ? 64 : 128) : 0;
 }
@@ -740,6 +744,7 @@ int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s) {
   BwdParams p;
   p.w = w;
   p.parts = parts_of(a.B, a.Sq, a.Sk, a.hq, a.hkv, a.causal, lb_num_sms());
+  p.acc_d = acc_columns(a.d);
   p.dq_acc = w.stats + stats_floats(a);
   p.dk_acc = p.dq_acc + dq_floats(a);
   p.dv_acc = p.dk_acc + part_floats(a, p.parts);

@@ -256,7 +256,8 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       // columns: P(j) V, then S(j+1) into the columns that P(j) leaves.
       if (elect_one()) {
         const uint32_t idesc_s = make_idesc(C::BM, C::BN, 0, 0);
-        const uint32_t idesc_o = make_idesc(C::BM, D, 0, 1);
+        const int slices = (p.d + 15) / 16;             // of 16 columns: those past head_dim are zeros, and left out of both products
+        const uint32_t idesc_o = make_idesc(C::BM, slices * 16, 0, 1);
         const uint64_t qa = make_desc(sbase + C::OFF_Q, 16, 1024);
         const uint64_t dk0 = make_desc(sbase + C::OFF_RING, 16, 1024);
         const uint64_t dv0 = make_desc(sbase + C::OFF_RING, 8192, 1024);
@@ -280,7 +281,8 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             const uint64_t ka = dk0 + (uint64_t)((ks * C::SLOT_BYTES) >> 4);
 #pragma unroll
             for (int s = 0; s < 4; s++)
-              umma_bf16(s_dst, qa + (uint64_t)((a * C::SLOT_BYTES + s * 32) >> 4), ka + (uint64_t)((s * 32) >> 4), idesc_s, (a | s) ? 1u : 0u);
+              if (a * 4 + s < slices)
+                umma_bf16(s_dst, qa + (uint64_t)((a * C::SLOT_BYTES + s * 32) >> 4), ka + (uint64_t)((s * 32) >> 4), idesc_s, (a | s) ? 1u : 0u);
             if (a == C::ATOMS - 1) umma_commit(s_full);
             umma_commit(empty(ks));
             ring(ks, kp, a == C::ATOMS - 1 ? C::UNITS - C::ATOMS + 1 : 1);
@@ -523,7 +525,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         }
       };
 #pragma unroll 1
-      for (int c = 0; c < D / 2; c += 32) {
+      for (int c = 0; c < D / 2 && set * (D / 2) + c < p.d; c += 32) {
         uint32_t r[32];
         uint4 hi[4];
         tmem_ld32(to_addr + c, r);

@@ -812,7 +812,7 @@ PyObject* py_attention_mask(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const bool causal = a[2] == Py_True;
   if ((a[0] != Py_None && !ids) || (a[1] != Py_None && !marks) || (!ids && !marks) || (a[2] != Py_True && a[2] != Py_False) || (marks && !causal)) LB_NOT_PLAIN;
   const Tensor& t = ids ? *ids : *marks;
-  if (!t.defined() || !t.is_cuda() || t.dim() != 2 || t.numel() == 0 || !here(t) || !fits_int({t.size(0), t.size(1)})) LB_NOT_PLAIN;
+  if (!t.defined() || !t.is_cuda() || t.dim() != 2 || t.numel() == 0 || !here(t) || t.size(0) > 65535 || t.size(1) > 327680) LB_NOT_PLAIN;
   if (ids && !sized(ids, t, at::kInt) && !sized(ids, t, at::kLong)) LB_NOT_PLAIN;
   if (marks && ((!sized(marks, t, at::kBool) && !sized(marks, t, at::kByte)) || !marks->sizes().equals(t.sizes()))) LB_NOT_PLAIN;
   std::pair<Tensor, Tensor> r = unlocked([&] {

@@ -749,6 +749,9 @@ class AttentionMask:
         return self.q_bounds.shape[1]
 
 
+MASK_MAX_LENGTH = 327680
+
+
 def attention_mask(documents: Optional[torch.Tensor] = None, prefix: Optional[torch.Tensor] = None, causal: bool = True,
                    length: Optional[int] = None) -> AttentionMask:
     """``documents`` [B, S] int32 / int64: a document is a run of equal ids, whose positions see no other run's; negative ids are padding, which
@@ -786,6 +789,8 @@ def attention_mask(documents: Optional[torch.Tensor] = None, prefix: Optional[to
             empty = torch.zeros(B, S, 2, dtype=torch.int32, device=first.device)
             return AttentionMask(empty, empty, causal)
         return AttentionMask(*ref.mask_bounds(S, documents, prefix, causal), causal)
+    if S > MASK_MAX_LENGTH or B > 65535:
+        raise ValueError(f"attention_mask on the GPU takes up to 65535 sequences of up to {MASK_MAX_LENGTH} positions, got {B} x {S}")
     documents = None if documents is None else documents.contiguous()
     marks = None if marks is None else marks.contiguous()
     lens = None if lens is None else lens.to(torch.int32).contiguous()

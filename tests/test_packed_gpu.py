@@ -41,7 +41,7 @@ def _run(q, k, v, do, **kw):
     return (o.detach(), *torch.autograd.grad(o, (q, k, v), do))
 
 
-@pytest.mark.parametrize("S", [1, 2, 31, 1000, 1024, 1025, 5000])
+@pytest.mark.parametrize("S", [1, 2, 31, 1000, 1024, 1025, 5000, 40001, 327680])
 @pytest.mark.parametrize("docs,prefix,causal", [(3, "none", True), (700, "marks", True), (0, "marks", True), (0, "lengths", True), (40, "none", False), (40, "lengths", True)])
 def test_intervals(S, docs, prefix, causal):
     from lightron_b200.ops import functional as OF
@@ -227,6 +227,8 @@ def test_attention_refusals_on_the_gpu():
     q = _rand(1, 8, 2, 20)
     with pytest.raises(ValueError):
         OF.masked_attention(q, q, q)                             # not a multiple of 8
+    with pytest.raises(ValueError):
+        OF.attention_mask(documents=torch.zeros(1, 327681, dtype=torch.int32, device="cuda"))
     q = _rand(1, 8, 2, 64)
     cpu = OF.attention_mask(documents=torch.zeros(1, 8, dtype=torch.int32))
     with pytest.raises(ValueError):
