@@ -57,8 +57,8 @@ struct Cfg {
   // 2 KB per softmax warp: 32 rows x 32 columns of O on their way out, and before that what the rows' two threads tell each other
   static constexpr int OFF_OUT = OFF_RING + SLOTS * SLOT_BYTES;
   static constexpr int OFF_BAR = OFF_OUT + 8 * 2048;
-  static constexpr int NBAR = 2 + 2 * SLOTS + 12;
-  static constexpr int SMEM = OFF_BAR + 256;
+  static constexpr int NBAR = 2 + 2 * SLOTS + 14;
+  static constexpr int SMEM = OFF_BAR + 288;
 };
 static_assert(Cfg<64>::SMEM <= 115712 && Cfg<128>::SMEM <= 115712, "two CTAs per SM");
 
@@ -129,6 +129,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
               const __grid_constant__ CUtensorMap to_lo, const __grid_constant__ FwdParams pp) {
   using C = Cfg<D>;
   constexpr bool MADE = CAP != NO_CAP || BIAS;        // scores are made in units of log2 ahead of the softmax
+  constexpr bool SPLIT = D == 128 && CAP == CAP_ZERO;
   const MaParams& p = pp.a;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
@@ -150,6 +151,9 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
   auto next_full = [&](int i) { return bar1 + 32u + 8u * i; };
   auto next_empty = [&](int i) { return bar1 + 48u + 8u * i; };
   auto pair_bar = [&](int quad) { return bar1 + 64u + 8u * quad; };
+  // SPLIT: scores and P of the second 64 keys of a block have barriers of their own
+  auto s_full_of = [&](int half) { return SPLIT && half ? bar1 + 96u : s_full; };
+  auto p_full_of = [&](int half) { return SPLIT && half ? bar1 + 104u : p_full; };
   const uint32_t next_slot = (bar0 + 8u * C::NBAR + 15u) & ~15u;
 
   // One entry per (batch, head, query tile): the last tiles, which see most under a causal mask, of all heads of a group first; a group is as many heads as keep
@@ -189,7 +193,9 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     mbar_init(s_full, 1);
     mbar_init(pv_done, 1);
     mbar_init(s_free, 8);
-    mbar_init(p_full, 8);
+    mbar_init(p_full, SPLIT ? 4 : 8);
+    mbar_init(s_full_of(1), 1);
+    mbar_init(p_full_of(1), SPLIT ? 4 : 8);
     for (int i = 0; i < 4; i++) mbar_init(pair_bar(i), 2);
     for (int i = 0; i < 2; i++) { mbar_init(next_full(i), 1); mbar_init(next_empty(i), 9); }   // the issuer and eight softmax warps read
     mbar_init_fence();
@@ -274,8 +280,35 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           const bool wrap = ks + 1 == C::SLOTS;
           return mbar_wait(full(wrap ? 0 : ks + 1), wrap ? kp ^ 1u : kp, abort_flag);
         };
+        // SPLIT: S of the next block's keys 64 * half and on, into the columns that P of such keys has left; the second half releases K (and Q)
+        const uint32_t idesc_half = make_idesc(C::BM, 64, 0, 0);
+        auto issue_half = [&](int half, bool last) {
+#pragma unroll
+          for (int a = 0; a < C::ATOMS; a++) {
+            const int slot = ks + a >= C::SLOTS ? ks + a - C::SLOTS : ks + a;
+            const uint64_t ka = dk0 + (uint64_t)((slot * C::SLOT_BYTES + half * 8192) >> 4);
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+              if (a * 4 + s < slices)
+                umma_bf16(s_dst + 64 * half, qa + (uint64_t)((a * C::SLOT_BYTES + s * 32) >> 4), ka + (uint64_t)((s * 32) >> 4), idesc_half, (a | s) ? 1u : 0u);
+          }
+          umma_commit(s_full_of(half));
+          if (half) {
+#pragma unroll
+            for (int a = 0; a < C::ATOMS; a++) {
+              umma_commit(empty(ks));
+              ring(ks, kp, a == C::ATOMS - 1 ? C::UNITS - C::ATOMS + 1 : 1);
+            }
+            if (last) umma_commit(q_empty);
+          }
+        };
         auto issue_s = [&](bool last) {                 // S = Q K^T of the next block (K is there), then release its slots of K (and Q)
           fence_after();
+          if constexpr (SPLIT) {
+            issue_half(0, last);
+            issue_half(1, last);
+            return;
+          }
 #pragma unroll
           for (int a = 0; a < C::ATOMS; a++) {
             const uint64_t ka = dk0 + (uint64_t)((ks * C::SLOT_BYTES) >> 4);
@@ -288,6 +321,27 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             ring(ks, kp, a == C::ATOMS - 1 ? C::UNITS - C::ATOMS + 1 : 1);
           }
           if (last) umma_commit(q_empty);
+        };
+        // SPLIT: O += P V by halves of 64 keys, each with S of the next block's behind it: the softmax threads of one half work while the products of the other run.
+        // (The first P V of a tile waits for both: until then the last tile's O is still being read.)
+        auto issue_halves = [&](bool first, bool last, bool last_s) -> bool {
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            if (!mbar_wait(full(vs), vp, abort_flag)) return false;
+            if (half == 0 && !last && !k_ready()) return false;
+            if (half == 0 && first && !mbar_wait(p_full_of(1), g & 1u, abort_flag)) return false;
+            if (!mbar_wait(p_full_of(half), g & 1u, abort_flag)) return false;
+            fence_after();
+            const uint64_t va = dv0 + (uint64_t)((vs * C::SLOT_BYTES) >> 4);
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+              umma_bf16_ta(o_dst, pa + 64u * half + 8u * s, va + (uint64_t)((s * 2048) >> 4), idesc_o, (half | s) ? 1u : (first ? 0u : 1u));
+            if (half && last) umma_commit(pv_done);
+            umma_commit(empty(vs));
+            ring(vs, vp, half ? C::ATOMS + 1 : 1);
+            if (!last) issue_half(half, last_s);
+          }
+          return true;
         };
         auto issue_pv = [&](bool first, bool last) -> bool {      // O += P V of block g, then release its slots of V
 #pragma unroll
@@ -328,6 +382,10 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           }
           for (int j = 0; j < t.nb && ok; j++, g++) {
             const bool last = j + 1 == t.nb;
+            if constexpr (SPLIT) {
+              ok = issue_halves(j == 0, last, j + 2 == t.nb);
+              continue;
+            }
             if (!C::P_ALIAS && !last) {
               ok = k_ready() && mbar_wait(s_free, g & 1u, abort_flag);
               if (ok) issue_s(j + 2 == t.nb);
@@ -347,7 +405,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     reg_inc<REGS_SOFTMAX>();
     const int quad = warp & 3, set = warp >= 8 ? 1 : 0;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16);
-    const uint32_t ts_addr = lane_addr + C::COL_S + set * 64, to_addr = lane_addr + C::COL_O + set * (D / 2), tp_addr = lane_addr + C::COL_P + set * 32;
+    const uint32_t ts_addr = lane_addr + C::COL_S + set * 64, to_addr = lane_addr + C::COL_O + set * (D / 2), tp_addr = lane_addr + C::COL_P + set * (SPLIT ? 64 : 32);
     [[maybe_unused]] const f32x2 scale2 = MADE ? 0 : kept(pp.f.scale);
     uint8_t* const out = smem + C::OFF_OUT + (warp - 4) * 2048;
     float2* const mine = reinterpret_cast<float2*>(out) + lane;
@@ -386,7 +444,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       __syncwarp();
       float m_i = -INFINITY, m_s = 0.f, l_i = 0.f, lp_i = 0.f;      // the row's running maximum, what exponentials are relative to, this thread's sums of them
       for (int j = 0; j < nb; j++, g++) {
-        if (!s_ready && !mbar_wait(s_full, g & 1u, abort_flag)) { ok = false; break; }
+        if (!s_ready && !mbar_wait(s_full_of(set), g & 1u, abort_flag)) { ok = false; break; }
         fence_after();
         uint32_t r[64];
         const int c0 = t.key0 + j * C::BN + set * 64, lo = see.x - c0, hi = see.y - c0;       // visible columns
@@ -475,16 +533,10 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           }
         }
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        if (C::P_ALIAS) {
-          // P takes columns of S that the row's other thread reads: both have by now where maxima were exchanged
-          if constexpr (CAP == CAP_ZERO) {
-            float2 none;
-            meet(make_float2(0.f, 0.f), none);
-          }
-        }
+        // (128 columns: P takes columns of S that the row's other thread reads; both have, where maxima were exchanged.  SPLIT: its own.)
         tmem_st32(tp_addr, pr);
         tmem_st_wait();
-        arrive(p_full);
+        arrive(p_full_of(set));
         s_ready = !C::P_ALIAS && j + 1 < nb && mbar_test_wait(s_full, (g + 1) & 1u);
         float s0, s1;
         unpack2(sum, s0, s1);
