@@ -30,6 +30,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 struct BwdParams {
   MaBwdParams w;
   float *dq_acc, *dk_acc, *dv_acc;
+  int* order;                    // null, or the key blocks (sequence * blocks + block) in the order of their CTAs
   int parts;                     // CTAs of a key block
   int acc_d;                     // columns of dq_acc: head_dim in whole pieces of 32
   MaTerms f;
@@ -83,18 +84,52 @@ __device__ __forceinline__ int2 query_blocks(const MaParams& p, int b, int n0, b
 
 // Row statistics, one 1 KB record per (b, h, 128-query block): 128 x -lse * log2(e), then 128 x -scale * D.  Rows without a sum, and rows past Sq, get (-inf, 0), which
 // makes their P and dS zero.  Also clears dQ's accumulator.  D/8 threads per (token, head).
+// With `order`, the last CTA instead sorts the key blocks by the query blocks that see them, most first, for the longest walks to begin first whatever the documents are
+// (walks of more than MOST blocks count as equal).  Against the order of a causal mask, main kernel: 8 x 2048, documents of 300, 32 / 4 heads, d 64 199 -> 188 us; 3 x 1531 of
+// 500, 32 / 8 heads, d 128 95 -> 86.
+constexpr int MOST = 1023;
 template <int D>
 __global__ void ma_bwd_prep_kernel(const __grid_constant__ BwdParams pp, const int clear) {
   grid_go();
   grid_wait();
   const MaParams& p = pp.w.f;
+  const int workers = (int)gridDim.x - (pp.order ? 1 : 0);
+  if ((int)blockIdx.x == workers) {
+    __shared__ int count[MOST + 2];
+    const int n_nblk = (p.Sk + 127) / 128, n = p.B * n_nblk;
+    auto size = [&](int e) {
+      const int2 mb = query_blocks(p, e / n_nblk, (e % n_nblk) * 128, false);
+      return MOST - min(mb.y - mb.x, MOST);                    // ascending: most first
+    };
+    for (int i = threadIdx.x; i < MOST + 2; i += blockDim.x) count[i] = 0;
+    __syncthreads();
+    for (int e = threadIdx.x; e < n; e += blockDim.x) atomicAdd(&count[size(e) + 1], 1);
+    __syncthreads();
+    if (threadIdx.x < 32) {                                    // entries ahead of each size
+      int run = 0;
+      for (int k = 0; k < MOST + 2; k += 32) {
+        const int i = k + (int)threadIdx.x;
+        int v = i < MOST + 2 ? count[i] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, v, o);
+          if ((int)threadIdx.x >= o) v += x;
+        }
+        if (i < MOST + 2) count[i] = run + v;
+        run += __shfl_sync(0xffffffffu, v, 31);
+      }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < n; e += blockDim.x) pp.order[atomicAdd(&count[size(e)], 1)] = e;
+    return;
+  }
   constexpr int TPR = D / 8;                                   // threads per row: 8 or 16
   const int n_mblocks = (p.Sq + 127) / 128, Sp = n_mblocks * 128;
   const long long total = (long long)p.B * Sp * p.hq;
   const int rpb = blockDim.x / TPR;                            // rows per block and iteration
   const int sub = threadIdx.x % TPR;
   // every thread of the block runs the same number of iterations, so the shuffles see whole warps
-  for (long long base = (long long)blockIdx.x * rpb; base < total; base += (long long)gridDim.x * rpb) {
+  for (long long base = (long long)blockIdx.x * rpb; base < total; base += (long long)workers * rpb) {
     const long long idx = base + threadIdx.x / TPR;
     const bool live = idx < total;
     float s = 0.f;
@@ -229,8 +264,8 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
   const uint32_t bar1 = bar0 + 8u * (1 + 2 * C::QS + 2 * C::DS);
   const uint32_t s_full = bar1, dp_full = bar1 + 8, p_full = bar1 + 16, ds_full = bar1 + 24, dq_full = bar1 + 32, dq_free = bar1 + 40;
 
-  // The first key blocks of all (batch, kv head) pairs of a group first: under a causal mask they take longest.  In parts: those of the first key block of all
-  // pairs, then the next.
+  // The first key blocks of all (batch, kv head) pairs of a group first: under a causal mask they take longest (with documents: in the order that has been
+  // found).  In parts: those of the first key block of all pairs, then the next.
   const int n_nblk = (p.Sk + C::BN - 1) / C::BN;
   int nblk, pair, part = 0;
   if constexpr (FORM == PARTS) {
@@ -245,8 +280,6 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     nblk = in_grp / gsize;
     pair = grp * GROUP + in_grp % gsize;
   }
-  const int hk = pair % p.hkv, b = pair / p.hkv;
-  const int n0 = nblk * C::BN;
   const int off = p.Sk - p.Sq;
   const int rep = p.hq / p.hkv;
   const int n_mblocks = (p.Sq + C::BM - 1) / C::BM;
@@ -273,6 +306,13 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
   volatile int* abort_flag = s_abort;
   grid_wait();
 
+  if (FORM == WHOLE && pp.order) {
+    const int e = pp.order[(int)blockIdx.x / p.hkv];
+    nblk = e % n_nblk;
+    pair = e / n_nblk * p.hkv + (int)blockIdx.x % p.hkv;
+  }
+  const int hk = pair % p.hkv, b = pair / p.hkv;
+  const int n0 = nblk * C::BN;
   // query blocks of every head of the group, head by head; a part takes an equal share of them
   const int2 seen_by = query_blocks(p, b, n0, FORM == ALONE);
   const int mb_first = seen_by.x, mb_end = seen_by.y, per_head = mb_end - mb_first;
@@ -716,7 +756,7 @@ int launch_bwd(BwdParams& p, cudaStream_t s) {
   const long long rows = (long long)a.B * ((a.Sq + 127) / 128 * 128) * a.hq;
   const long long rows_per_block = 256 / (D / 8), cap = lb_num_sms() * 16;
   const long long pblocks = (rows + rows_per_block - 1) / rows_per_block;
-  LB_LAUNCH(ma_bwd_prep_kernel<D>, (int)(pblocks < cap ? pblocks : cap), 256, 0, s, p, !alone);
+  LB_LAUNCH(ma_bwd_prep_kernel<D>, (int)(pblocks < cap ? pblocks : cap) + (p.order ? 1 : 0), 256, 0, s, p, !alone);
   rc = p.parts > 1 ? launch_form<D, PARTS>(m, p, (unsigned)grid, s) : alone ? launch_form<D, ALONE>(m, p, (unsigned)grid, s) : launch_form<D, WHOLE>(m, p, (unsigned)grid, s);
   if (rc || alone) return rc;
   const long long part_rows = p.parts > 1 ? 2LL * a.B * ((a.Sk + 127) / 128 * 128) * a.hkv : 0;
@@ -725,7 +765,7 @@ int launch_bwd(BwdParams& p, cudaStream_t s) {
   return LB_OK;
 }
 
-// Bytes of the workspace: row statistics, fp32 dQ (up to 128 keys: none), fp32 dK and dV of the parts.
+// Bytes of the workspace: row statistics, fp32 dQ (up to 128 keys: none), fp32 dK and dV of the parts, the order of the key blocks.
 long long stats_floats(const MaParams& p) { return (long long)p.B * p.hq * ((p.Sq + 127) / 128) * 256; }
 int acc_columns(int d) { return (d + 31) / 32 * 32; }
 long long dq_floats(const MaParams& p) { return p.Sk <= 128 ? 0 : stats_floats(p) / 2 * acc_columns(p.d); }
@@ -733,10 +773,12 @@ long long part_floats(const MaParams& p, int parts) {
   return parts > 1 ? (long long)p.B * p.hkv * ((p.Sk + 127) / 128) * parts * 128 * (p.d <= 64 ? 64 : 128) : 0;
 }
 
+long long order_ints(const MaParams& p) { return (long long)p.B * ((p.Sk + 127) / 128); }
+
 }  // namespace
 
 long long ma_bwd_ws_bytes(const MaParams& p) {
-  return (stats_floats(p) + dq_floats(p) + 2 * part_floats(p, parts_of(p.B, p.Sq, p.Sk, p.hq, p.hkv, p.causal, lb_num_sms()))) * (long long)sizeof(float);
+  return (stats_floats(p) + dq_floats(p) + 2 * part_floats(p, parts_of(p.B, p.Sq, p.Sk, p.hq, p.hkv, p.causal, lb_num_sms())) + order_ints(p)) * (long long)sizeof(float);
 }
 
 int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s) {
@@ -748,6 +790,7 @@ int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s) {
   p.dq_acc = w.stats + stats_floats(a);
   p.dk_acc = p.dq_acc + dq_floats(a);
   p.dv_acc = p.dk_acc + part_floats(a, p.parts);
+  p.order = a.kb && p.parts == 1 && a.Sk > 128 ? reinterpret_cast<int*>(p.dv_acc + part_floats(a, p.parts)) : nullptr;
   p.f.set(a, false, twice);
   p.scale2 = twice(a.scale);
   return a.d <= 64 ? launch_bwd<64>(p, s) : launch_bwd<128>(p, s);
