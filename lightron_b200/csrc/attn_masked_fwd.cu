@@ -47,7 +47,8 @@ struct Cfg {
   static constexpr int BM = 128, BN = 128;
   static constexpr int ATOMS = D / 64;
   static constexpr int SLOT_BYTES = 128 * 128;          // K: 128 keys x 64 columns; V: 128 keys x 64 columns or 64 keys x 128 columns
-  static constexpr int SLOTS = 6 - ATOMS;
+  static constexpr int SLOTS = 4;
+  static constexpr int OUT_BYTES = (D == 64) ? 4096 : 2048;      // of a softmax warp
   static constexpr int UNITS = 2 * ATOMS;               // slots that a key block takes, K before V
   // TMEM columns: S fp32 [128], O fp32 [D], P packed bf16 [64]; with 128 columns of O, P takes the first half of S's
   static constexpr bool P_ALIAS = (D == 128);
@@ -56,7 +57,7 @@ struct Cfg {
   static constexpr int OFF_RING = OFF_Q + ATOMS * SLOT_BYTES;
   // 2 KB per softmax warp: 32 rows x 32 columns of O on their way out, and before that what the rows' two threads tell each other
   static constexpr int OFF_OUT = OFF_RING + SLOTS * SLOT_BYTES;
-  static constexpr int OFF_BAR = OFF_OUT + 8 * 2048;
+  static constexpr int OFF_BAR = OFF_OUT + 8 * OUT_BYTES;
   static constexpr int NBAR = 2 + 2 * SLOTS + 14;
   static constexpr int SMEM = OFF_BAR + 288;
 };
@@ -407,9 +408,9 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16);
     const uint32_t ts_addr = lane_addr + C::COL_S + set * 64, to_addr = lane_addr + C::COL_O + set * (D / 2), tp_addr = lane_addr + C::COL_P + set * (SPLIT ? 64 : 32);
     [[maybe_unused]] const f32x2 scale2 = MADE ? 0 : kept(pp.f.scale);
-    uint8_t* const out = smem + C::OFF_OUT + (warp - 4) * 2048;
+    uint8_t* const out = smem + C::OFF_OUT + (warp - 4) * C::OUT_BYTES;
     float2* const mine = reinterpret_cast<float2*>(out) + lane;
-    const float2* const other = reinterpret_cast<float2*>(smem + C::OFF_OUT + ((warp - 4) ^ 4) * 2048) + lane;
+    const float2* const other = reinterpret_cast<float2*>(smem + C::OFF_OUT + ((warp - 4) ^ 4) * C::OUT_BYTES) + lane;
     bool ok = true;
     uint32_t turn = 0;
     // The row's two threads meet (in a wait that ends, as all do); what the other one has in y.  Two places in turn: nobody is more than one meeting ahead.
@@ -564,15 +565,17 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       fence_after();
       const float inv = lp_i != 0.f ? 1.f / lp_i : 0.f;
       // 32 columns at a time through shared memory and TMA stores, which leave out rows past the last and columns past head_dim
-      auto leave = [&](const CUtensorMap* map, const uint4* v, int col) {      // v: 32 columns of the lane's row
-        if (lane == 0) bulk_wait_read_but<0>();
-        __syncwarp();
+      auto leave = [&](const CUtensorMap* map, const uint4* v, int col, int at) {      // v: 32 columns of the lane's row
+        if (C::OUT_BYTES == 2048) {
+          if (lane == 0) bulk_wait_read_but<0>();
+          __syncwarp();
+        }
 #pragma unroll
-        for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(out + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = v[i];      // (64-byte swizzle)
+        for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(out + at + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = v[i];      // (64-byte swizzle)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0 && t.m0 + quad * 32 < p.Sq) {
-          tma_store_4d(map, smem_u32(out), col, t.h, t.m0 + quad * 32, t.b);
+          tma_store_4d(map, smem_u32(out) + at, col, t.h, t.m0 + quad * 32, t.b);
           bulk_commit();
         }
       };
@@ -592,11 +595,11 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
 #pragma unroll
           for (int i = 0; i < 8; i++) r[g8 * 8 + i] = __float_as_uint(f[i] - back[i]);
         }
-        leave(&to, hi, set * (D / 2) + c);
+        leave(&to, hi, set * (D / 2) + c, 0);
         if (p.o_lo) {
 #pragma unroll
           for (int g8 = 0; g8 < 4; g8++) hi[g8] = pack8(reinterpret_cast<const float*>(r) + g8 * 8);
-          leave(&to_lo, hi, set * (D / 2) + c);
+          leave(&to_lo, hi, set * (D / 2) + c, C::OUT_BYTES - 2048);
         }
       }
       if (set == 0 && row < p.Sq) p.lse[((long long)t.b * p.hq + t.h) * p.Sq + row] = l_i != 0.f ? m_s * (MADE ? LN2 : p.scale) + logf(l_i) : -INFINITY;
