@@ -11,17 +11,18 @@
 
 namespace {
 
-constexpr int THREADS = 256, MAX_TENSORS = 768, CHUNK = 16384;
+constexpr int THREADS = 256, MAX_TENSORS = 768, FEW_TENSORS = 96, CHUNK = 16384;
 enum : int { BF16 = 0, FP16 = 1, FP32 = 2 };
 
+template <int N>
 struct Tensors {
   int n, chunks;
-  const void* src[MAX_TENSORS];
-  void* dst[MAX_TENSORS];
-  long long count[MAX_TENSORS];
-  int first[MAX_TENSORS];                      // chunks ahead of a tensor's, with its type in the upper two bits
+  const void* src[N];
+  void* dst[N];
+  long long count[N];
+  int first[N];                                // chunks ahead of a tensor's, with its type in the upper two bits
 };
-static_assert(sizeof(Tensors) <= 32000, "kernel parameters");
+static_assert(sizeof(Tensors<MAX_TENSORS>) <= 32000 && sizeof(Tensors<FEW_TENSORS>) <= 4000, "kernel parameters: 32 KB, or 4 KB in the quicker way");
 
 __device__ __forceinline__ float to_f(bf16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
@@ -45,7 +46,8 @@ __device__ __forceinline__ float block_sum(float s) {
 }
 
 // The chunk's tensor: the last whose first chunk is not behind it (empty tensors have none and are never the last).
-__device__ __forceinline__ int tensor_of(const Tensors& t, int chunk) {
+template <int N>
+__device__ __forceinline__ int tensor_of(const Tensors<N>& t, int chunk) {
   int lo = 0, hi = t.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -93,7 +95,8 @@ __device__ __forceinline__ float chunk_squares(const T* x, int n) {
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-__global__ void __launch_bounds__(THREADS) grad_squares_kernel(const __grid_constant__ Tensors t, float* __restrict__ partial) {
+template <int N>
+__global__ void __launch_bounds__(THREADS) grad_squares_kernel(const __grid_constant__ Tensors<N> t, float* __restrict__ partial) {
   grid_go();
   grid_wait();
   float s = 0.f;
@@ -189,7 +192,8 @@ __device__ __forceinline__ void chunk_scale(const T* x, T* y, int n, float by) {
   if (i < n && (i < lead || i >= rest)) y[i] = from_f<T>(to_f(x[i]) * by);
 }
 
-__global__ void __launch_bounds__(THREADS) grad_scale_kernel(const __grid_constant__ Tensors t, const float* __restrict__ partial, int n_partial, float max_norm, float eps,
+template <int N>
+__global__ void __launch_bounds__(THREADS) grad_scale_kernel(const __grid_constant__ Tensors<N> t, const float* __restrict__ partial, int n_partial, float max_norm, float eps,
                                                              float* __restrict__ norm_out) {
   grid_go();
   grid_wait();
@@ -211,9 +215,10 @@ __global__ void __launch_bounds__(THREADS) grad_scale_kernel(const __grid_consta
 int grid_of(int chunks) { const int most = lb_num_sms() * 8; return chunks < most ? chunks : most; }
 
 // The next tensors of a list, up to what one launch takes; `at` moves on.
-int next_tensors(Tensors& t, int n, int& at, const void* const* src, void* const* dst, const long long* counts, const int* types) {
+template <int N>
+int next_tensors(Tensors<N>& t, int n, int& at, const void* const* src, void* const* dst, const long long* counts, const int* types) {
   t.n = t.chunks = 0;
-  for (; at < n && t.n < MAX_TENSORS; at++) {
+  for (; at < n && t.n < N; at++) {
     if (counts[at] < 0 || (counts[at] && (!src[at] || (dst && !dst[at]))) || types[at] < BF16 || types[at] > FP32) return LB_ERR_ARG;
     const long long chunks = (counts[at] + CHUNK - 1) / CHUNK;
     if (!chunks) continue;
@@ -230,6 +235,33 @@ int next_tensors(Tensors& t, int n, int& at, const void* const* src, void* const
   return LB_OK;
 }
 
+template <int N>
+int squares(int n, const void* const* src, const long long* counts, const int* types, float* partial, int partials, int* filled, cudaStream_t s) {
+  static thread_local Tensors<N> t;
+  for (int at = 0; at < n;) {
+    if (const int rc = next_tensors(t, n, at, src, nullptr, counts, types)) return rc;
+    if (!t.n) break;
+    const int grid = grid_of(t.chunks);
+    if (*filled + grid > partials) return LB_ERR_CAPACITY;
+    LB_LAUNCH(grad_squares_kernel<N>, grid, THREADS, 0, s, t, partial + *filled);
+    *filled += grid;
+  }
+  return LB_OK;
+}
+
+template <int N>
+int scale(int n, const void* const* src, void* const* dst, const long long* counts, const int* types, const float* partial, int n_partial, float max_norm, float eps, float*& norm_out,
+          cudaStream_t s) {
+  static thread_local Tensors<N> t;
+  for (int at = 0; at < n;) {
+    if (const int rc = next_tensors(t, n, at, src, dst, counts, types)) return rc;
+    if (!t.n) break;
+    LB_LAUNCH(grad_scale_kernel<N>, grid_of(t.chunks), THREADS, 0, s, t, partial, n_partial, max_norm, eps, norm_out);
+    norm_out = nullptr;
+  }
+  return LB_OK;
+}
+
 }  // namespace
 
 // Floats of `partial` that lb_grad_squares() of n tensors may fill.
@@ -238,17 +270,10 @@ extern "C" int lb_grad_norm_parts(int n) { return n < 0 ? LB_ERR_ARG : (n / MAX_
 // partial[0 .. *filled): sums of squares of parts of the n tensors (host arrays of device addresses, element counts and types: 0 bf16, 1 fp16, 2 fp32).
 extern "C" int lb_grad_squares(int n, const void* const* src, const long long* counts, const int* types, void* partial, int partials, int* filled, void* stream) {
   if (n < 0 || !partial || !filled || (n && (!src || !counts || !types))) return LB_ERR_ARG;
-  static thread_local Tensors t;
   *filled = 0;
-  for (int at = 0; at < n;) {
-    if (const int rc = next_tensors(t, n, at, src, nullptr, counts, types)) return rc;
-    if (!t.n) break;
-    const int grid = grid_of(t.chunks);
-    if (*filled + grid > partials) return LB_ERR_CAPACITY;
-    LB_LAUNCH(grad_squares_kernel, grid, THREADS, 0, (cudaStream_t)stream, t, (float*)partial + *filled);
-    *filled += grid;
-  }
-  return LB_OK;
+  cudaStream_t s = (cudaStream_t)stream;
+  return n <= FEW_TENSORS ? squares<FEW_TENSORS>(n, src, counts, types, (float*)partial, partials, filled, s)
+                          : squares<MAX_TENSORS>(n, src, counts, types, (float*)partial, partials, filled, s);
 }
 
 // Total of n parts: its fp32 value and its root (either may be null).
@@ -263,13 +288,11 @@ extern "C" int lb_grad_total(const void* partial, int n, void* sumsq, void* norm
 extern "C" int lb_grad_scale(int n, const void* const* src, void* const* dst, const long long* counts, const int* types, const void* partial, int n_partial, float max_norm,
                              float eps, void* norm_out, void* stream) {
   if (n < 0 || n_partial < 0 || !partial || (n && (!src || !dst || !counts || !types))) return LB_ERR_ARG;
-  static thread_local Tensors t;
-  for (int at = 0; at < n;) {
-    if (const int rc = next_tensors(t, n, at, src, dst, counts, types)) return rc;
-    if (!t.n) break;
-    LB_LAUNCH(grad_scale_kernel, grid_of(t.chunks), THREADS, 0, (cudaStream_t)stream, t, (const float*)partial, n_partial, max_norm, eps, (float*)norm_out);
-    norm_out = nullptr;
-  }
-  if (norm_out) return lb_grad_total(partial, n_partial, nullptr, norm_out, stream);
+  float* norm = (float*)norm_out;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (const int rc = n <= FEW_TENSORS ? scale<FEW_TENSORS>(n, src, dst, counts, types, (const float*)partial, n_partial, max_norm, eps, norm, s)
+                                      : scale<MAX_TENSORS>(n, src, dst, counts, types, (const float*)partial, n_partial, max_norm, eps, norm, s))
+    return rc;
+  if (norm) return lb_grad_total(partial, n_partial, nullptr, norm, stream);      // (nothing to scale)
   return LB_OK;
 }

@@ -112,6 +112,19 @@ def test_gradients_against_differences(cap, alibi):
         assert abs(((f[0] - f[1]) / (2 * eps) / u.square().sum()).item() - 1) < 5e-3, name
 
 
+@pytest.mark.parametrize("B,S,hq,hkv,d", [(1, 500, 8, 1, 64), (6, 300, 8, 4, 128)])
+def test_attention_repeats_its_bits(B, S, hq, hkv, d):
+    """o, dk and dv are summed in a fixed order, also where a key block's walk is cut into parts (the first); so is dq up to 128 keys."""
+    q, k, v, do = _rand(B, S, hq, d, seed=1), _rand(B, S, hkv, d, seed=2), _rand(B, S, hkv, d, seed=3), _rand(B, S, hq, d, seed=4)
+    mask, _, _ = _mask(B, S, True, 90, False, seed=1)
+    first = _run(q, k, v, do, mask=mask, softcap=30.0)
+    for _ in range(3):
+        again = _run(q, k, v, do, mask=mask, softcap=30.0)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[2], again[2]) and torch.equal(first[3], again[3])
+    short = [t[:, :120] for t in (q, k, v, do)]
+    assert torch.equal(_run(*short)[1], _run(*short)[1])
+
+
 def test_attention_strides():
     """Heads ahead of tokens, a fused projection's columns, every other token, an expanded gradient: the same bits as contiguous copies."""
     B, S, hq, hkv, d = 2, 150, 4, 2, 64
