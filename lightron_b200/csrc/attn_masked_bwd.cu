@@ -502,34 +502,35 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       fence_after();
       float pf[64];                                 // P, then P times the cap's derivative
       {
-        uint32_t sr[64];
-        tmem_ld32(ts, sr);
-        tmem_ld32(ts + 32, sr + 32);
-        tmem_ld_wait();
         // the key is seen by queries lo to hi - 1 of these columns
         const int lo = see.x - m0, hi = see.y - m0;
         const bool need_mask = __any_sync(0xffffffffu, lo > 0 || hi < 64);
-        bool small = true;
-        if constexpr (CAP) {
-          float top[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int i = 0; i < 64; i += 2) top[(i >> 1) & 3] = max3abs(top[(i >> 1) & 3], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
-          small = __all_sync(0xffffffffu, max2(max2(top[0], top[1]), max2(top[2], top[3])) <= pp.f.limit);
-        }
         // distance to the columns' places: 1 all behind the key, -1 all ahead of it, 0 both
         const int first = m0 + off - key;
         int side = 1;
         if constexpr (BIAS) side = behind_only || m0 + off >= n0 + quad * 32 + 31 ? 1 : m0 + off + 63 <= n0 + quad * 32 ? -1 : 0;
         const float slope = side > 0 ? -slope2 : slope2;
         const f32x2 step = pack2(2.f * slope, 2.f * slope);
-        uint32_t pp_[32];
-        // (32 columns at a time; what a warp decides for all of them is decided outside of their loops, which would else be one pair after the other)
+        // 32 columns at a time.  With 128 columns of head_dim they are loaded so, too: all 64 do not fit into the registers beside P (1 x 8192, capped, both ways in
+        // turn: 1675 to 1692 us, now 1605 to 1626).  What a warp decides for all columns is decided outside of their loops, which would else be one pair after the other.
+        constexpr int AT_ONCE = (D == 64) ? 64 : 32;
+        uint32_t all[AT_ONCE];
 #pragma unroll
         for (int w = 0; w < 64; w += 32) {
-          if constexpr (CAP) {                      // tanh
-            if (small) {
+          uint32_t pp_[16];
+          if (w % AT_ONCE == 0) {
 #pragma unroll
-              for (int i = w; i < w + 32; i += 2) {
+            for (int c = 0; c < AT_ONCE; c += 32) tmem_ld32(ts + w + c, all + c);
+            tmem_ld_wait();
+          }
+          uint32_t* const sr = all + w % AT_ONCE;
+          if constexpr (CAP) {                      // tanh
+            float top[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) top[(i >> 1) & 3] = max3abs(top[(i >> 1) & 3], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+            if (__all_sync(0xffffffffu, max2(max2(top[0], top[1]), max2(top[2], top[3])) <= pp.f.limit)) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
                 const f32x2 x = pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), u = mul2(x, x);
                 float t0, t1;
                 unpack2(mul2(x, fma2(u, fma2(u, fma2(u, pp.f.c[3], pp.f.c[2]), pp.f.c[1]), pp.f.c[0])), t0, t1);
@@ -538,7 +539,7 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
               }
             } else {
 #pragma unroll
-              for (int i = w; i < w + 32; i++)      // tanh u = 1 - 2 / (exp 2u + 1)
+              for (int i = 0; i < 32; i++)          // tanh u = 1 - 2 / (exp 2u + 1)
                 sr[i] = __float_as_uint(1.f - __fdividef(2.f, exp2f(__uint_as_float(sr[i]) * pp.f.by2) + 1.f));
             }
           }
@@ -546,19 +547,19 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             f32x2 add = pack2(0.f, 0.f);
             if constexpr (BIAS) { const float base = slope * (float)(first + w); add = pack2(base, base + slope); }
 #pragma unroll
-            for (int i = w; i < w + 32; i += 2) {
-              const float2 nl = reinterpret_cast<const float2*>(st)[i >> 1];
+            for (int i = 0; i < 32; i += 2) {
+              const float2 nl = reinterpret_cast<const float2*>(st)[(w + i) >> 1];
               const f32x2 x = pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
               f32x2 to = pack2(nl.x, nl.y);
               if constexpr (BIAS && !decltype(both)::value) {
                 to = add2(to, add);
                 add = add2(add, step);
               } else if constexpr (BIAS) {
-                to = pack2(fmaf(-slope2, fabsf((float)(first + i)), nl.x), fmaf(-slope2, fabsf((float)(first + i + 1)), nl.y));
+                to = pack2(fmaf(-slope2, fabsf((float)(first + w + i)), nl.x), fmaf(-slope2, fabsf((float)(first + w + i + 1)), nl.y));
               }
-              unpack2(fma2(x, CAP ? pp.f.cap : pp.f.scale, to), pf[i], pf[i + 1]);
-              pf[i] = exp2f(pf[i]);
-              pf[i + 1] = exp2f(pf[i + 1]);
+              unpack2(fma2(x, CAP ? pp.f.cap : pp.f.scale, to), pf[w + i], pf[w + i + 1]);
+              pf[w + i] = exp2f(pf[w + i]);
+              pf[w + i + 1] = exp2f(pf[w + i + 1]);
             }
           };
           if (BIAS && side == 0) weights(std::true_type{}); else weights(std::false_type{});
@@ -569,15 +570,16 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
               if (!(bits >> i & 1u)) pf[w + i] = 0.f;
           }
 #pragma unroll
-          for (int i = w; i < w + 32; i += 2) {
-            bf162 pb = __floats2bfloat162_rn(pf[i], pf[i + 1]);
+          for (int i = 0; i < 32; i += 2) {
+            bf162 pb = __floats2bfloat162_rn(pf[w + i], pf[w + i + 1]);
             pp_[i >> 1] = *reinterpret_cast<uint32_t*>(&pb);
           }
+          tmem_st16(ts + w / 2, pp_);
           if constexpr (CAP) {
 #pragma unroll
-            for (int i = w; i < w + 32; i += 2) {   // P (1 - t^2)
-              const f32x2 e = pack2(pf[i], pf[i + 1]), t = pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
-              unpack2(sub2(e, mul2(mul2(e, t), t)), pf[i], pf[i + 1]);
+            for (int i = 0; i < 32; i += 2) {       // P (1 - t^2)
+              const f32x2 e = pack2(pf[w + i], pf[w + i + 1]), t = pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+              unpack2(sub2(e, mul2(mul2(e, t), t)), pf[w + i], pf[w + i + 1]);
             }
             if (need_mask) {                        // (a hidden NaN is one still)
 #pragma unroll
@@ -586,7 +588,6 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             }
           }
         }
-        tmem_st32(ts, pp_);
         tmem_st_wait();
       }
       fence_before();
