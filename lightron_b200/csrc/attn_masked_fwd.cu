@@ -2,13 +2,15 @@
 // tiles of 64 or 128 columns).
 //
 // A CTA works on one tile of 128 queries of one (batch, head) at a time, two CTAs per SM; S = Q K^T and O += P V by tcgen05.mma with S, P and O in tensor
-// memory, a softmax thread per query row, K and V by TMA through a ring of 16 KB slots, further tiles by cluster launch control: the pipeline of the causal
+// memory, K and V by TMA through a ring of 16 KB slots, further tiles by cluster launch control: the pipeline of the causal
 // forward (flash_fwd_tcgen05.cu has what each part of it is worth).  What is different here:
+//   * a row is two threads', 64 columns of a key block each, in eight softmax warps, which tell each other maxima and sums through shared memory.  (One thread a row / two, 8 x 2048,
+//     32 / 4 heads, d 64: causal 268 / 254 us, bias 470 / 312, cap 363 / 305, documents 178 / 134; 1 x 8192, 32 / 8 heads, d 128: 632 / 595, bias 974 / 727, cap 720 / 722.)
 //   * the keys of a tile run from the first key of its first row to the last key of its last (the ends never fall), from exactly there: blocks start
 //     at any key, so that a document of n keys takes ceil(n / 128) of them wherever it lies.  Blocks inside all 32 intervals of a warp are not masked.
 //   * with a cap the scores are known to lie within it.  Up to softcap * log2(e) = 80 exponentials are taken relative to zero instead of the running
-//     maximum: 2^+-80 and sums of them are far inside fp32 (and bf16 has the same exponents), nothing is ever rescaled, and the first half of
-//     P leaves before the second is looked at.  Above it the maximum is kept.
+//     maximum: 2^+-80 and sums of them are far inside fp32 (and bf16 has the same exponents), and nothing is ever rescaled.  With 128 columns the two halves of a
+//     block then have nothing to tell each other, and their scores, P and products run apart (d 128, cap: 700 -> 640 us).  Above 80 the maximum is kept.
 //   * tanh: where no score of 32 rows x 64 columns is above 0.6 caps, x times a polynomial in x^2 on the FMA pipe, two at a time (relative error
 //     2.1e-6, found by least squares with re-weighted points; 7e-5 of a score at most); else by its definition with exp2, whose units the softmax needs itself.
 //   * the bias is an addend of the same FMA, counted up along the columns; only where a block holds keys on both sides of a row is its distance made per column.
@@ -16,6 +18,8 @@
 //     error is as small as the differences dP - D that the backward lives on (the weight's own rounding, 2^-9 of dP, would drown them); lse is of the sum of the
 //     unrounded ones, from which the backward's P are made.
 //   * o leaves twice: rounded, and what the rounding left (for the backward's row sums).
+// What bounds it: latency, with instructions close behind.  Of the active cycles 61 % of the issue slots and 41 to 52 % of the exponentials' unit (d 64, two tiles per SM), 39 %
+// of the tensor pipe (d 128); a block takes 1960 (d 64) / 2400 cycles (d 128, cap) of an SM, 2530 with documents, whose loops are short and whose blocks are nearly all masked.
 // All waits are bounded; on expiry a status word is set and the CTA drains and frees its TMEM.
 #include "attn_masked.cuh"
 #include "tcgen05.cuh"
