@@ -13,7 +13,10 @@
 //     block then have nothing to tell each other, and their scores, P and products run apart (d 128, cap: 700 -> 640 us).  Above 80 the maximum is kept.
 //   * tanh: where no score of 32 rows x 64 columns is above 0.6 caps, x times a polynomial in x^2 on the FMA pipe, two at a time (relative error
 //     2.1e-6, found by least squares with re-weighted points; 7e-5 of a score at most); else by its definition with exp2, whose units the softmax needs itself.
-//   * the bias is an addend of the same FMA, counted up along the columns; only where a block holds keys on both sides of a row is its distance made per column.
+//   * the bias is an addend of the FMA that scales a score (or evaluates its polynomial), counted up along the columns; only where a block holds keys on both sides of a row is its
+//     distance made per column.  Without a cap the exponentials' reference is a bound, not the maximum itself: what they are relative to cancels, as long as it is within 2^60
+//     or so of the maximum.  The nearest key blocks come first, or the maximum would grow from block to block and O be rescaled in each (both together: 1 x 8192, 32 / 8 heads,
+//     d 128 780 -> 632 us, 8 x 2048, 32 / 4 heads, d 64 303 -> 287).
 //   * o is divided by the sum of the weights as they are rounded for P V.  A row that all but one key leave cold has o = v of that key then, and a D = do . o whose
 //     error is as small as the differences dP - D that the backward lives on (the weight's own rounding, 2^-9 of dP, would drown them); lse is of the sum of the
 //     unrounded ones, from which the backward's P are made.
@@ -133,8 +136,10 @@ __global__ void __launch_bounds__(THREADS, 2)
 ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to,
               const __grid_constant__ CUtensorMap to_lo, const __grid_constant__ FwdParams pp) {
   using C = Cfg<D>;
-  constexpr bool MADE = CAP != NO_CAP || BIAS;        // scores are made in units of log2 ahead of the softmax
+  constexpr bool MADE = CAP != NO_CAP;                // scores are made in units of log2 ahead of the softmax
+  constexpr bool LINEAR = BIAS && !MADE;              // the bias is added where the exponentials are taken
   constexpr bool SPLIT = D == 128 && CAP == CAP_ZERO;
+  constexpr bool BACKWARDS = BIAS && CAP != CAP_ZERO;      // the nearest keys first: on the way to them the maximum would grow in every block, and O be rescaled
   const MaParams& p = pp.a;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
@@ -236,7 +241,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
 #pragma unroll
           for (int a = 0; a < C::ATOMS; a++) tma_load_4d(sbase + C::OFF_Q + a * C::SLOT_BYTES, &tq, a * 64, t.h, t.m0, t.b, q_full);
           for (int j = 0; j < t.nb && ok; j++) {
-            const int key0 = t.key0 + j * C::BN;
+            const int key0 = t.key0 + (BACKWARDS ? t.nb - 1 - j : j) * C::BN;
 #pragma unroll
             for (int u = 0; u < C::UNITS; u++) {
               if (ok && !mbar_wait(empty(slot), phase ^ 1u, abort_flag)) ok = false;
@@ -452,7 +457,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         if (!s_ready && !mbar_wait(s_full_of(set), g & 1u, abort_flag)) { ok = false; break; }
         fence_after();
         uint32_t r[64];
-        const int c0 = t.key0 + j * C::BN + set * 64, lo = see.x - c0, hi = see.y - c0;       // visible columns
+        const int c0 = t.key0 + (BACKWARDS ? nb - 1 - j : j) * C::BN + set * 64, lo = see.x - c0, hi = see.y - c0;       // visible columns
         const bool need_mask = __any_sync(0xffffffffu, lo > 0 || hi < 64);
         tmem_ld32(ts_addr, r);
         tmem_ld32(ts_addr + 32, r + 32);
@@ -472,15 +477,46 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
               if (!(bits >> i & 1u)) r[w + i] = 0xff800000u;           // -inf
           }
         }
+        // LINEAR: bias at column i is slope * (c0 + i - place); with keys on both sides of a row (slope 0) it is in r from here on
+        [[maybe_unused]] float slope = 0.f;
+        if constexpr (LINEAR) {
+          slope = left_only || c0 + 63 <= warp_at ? slope2 : c0 >= warp_at + 31 ? -slope2 : 0.f;
+          if (slope == 0.f) {
+            const float by = -__fdividef(slope2, pp.f.scale1), d0 = (float)(c0 - (row + off));
+#pragma unroll
+            for (int i = 0; i < 64; i++) r[i] = __float_as_uint(fmaf(by, fabsf(d0 + (float)i), __uint_as_float(r[i])));
+          }
+        }
         bool rescale = false;
         float corr = 1.f;
         if constexpr (CAP != CAP_ZERO) {
           // Lazy reference maximum: the old one stays unless the new maximum is more than 2^8 above it, so that O and l rarely need rescaling.
-          const float unit = MADE ? 1.f : pp.f.scale1;
-          float mx4[4] = {m_i, m_i, m_i, m_i};           // four independent chains
+          const float unit = MADE || LINEAR ? 1.f : pp.f.scale1;
+          const float from = LINEAR ? -INFINITY : m_i;
+          float mx4[4] = {from, from, from, from};       // four independent chains
+          float m_new = m_i;
+          if constexpr (LINEAR) {
+            // A bound instead of the maximum: of 32 columns the largest score with the smallest distance, at most 31 slopes above it.  (Where that is more than 2^60 the
+            // biased scores are looked at one by one.)
 #pragma unroll
-          for (int i = 0; i < 64; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-          float m_new = max2(max2(mx4[0], mx4[1]), max2(mx4[2], mx4[3]));
+            for (int w = 0; w < 64; w += 32) {
+              const int to_left = row + off - (c0 + w + 31), to_right = c0 + w - (row + off);
+              const float steep = fabsf(slope);
+              if (steep <= 60.f / 31.f) {
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = w; i < w + 32; i += 2) top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+                m_new = max2(m_new, fmaf(max2(top[0], top[1]), pp.f.scale1, -steep * (float)max(max(to_left, to_right), 0)));
+              } else {
+#pragma unroll
+                for (int i = w; i < w + 32; i++) m_new = max2(m_new, fmaf(__uint_as_float(r[i]), pp.f.scale1, -steep * fabsf((float)(to_right + (i - w)))));
+              }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 64; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+            m_new = max2(max2(mx4[0], mx4[1]), max2(mx4[2], mx4[3]));
+          }
           float2 theirs;
           meet(make_float2(m_new, 0.f), theirs);
           m_new = max2(m_new, theirs.x);
@@ -489,9 +525,10 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             // (where a row has seen nothing yet there is nothing to rescale)
             rescale = __any_sync(0xffffffffu, grow && m_i != -INFINITY);
             if (!grow) m_new = m_i;
+            const float m_r = m_s;
             // (a row with a score of +inf has no softmax: NaN, as inf - inf gives)
-            m_s = (m_new == -INFINITY) ? 0.f : (m_new == INFINITY ? __int_as_float(0x7fffffff) : m_new);
-            corr = (m_i == -INFINITY) ? 0.f : exp2f((m_i - m_s) * unit);
+            m_s = (m_new == -INFINITY) ? 0.f : (m_new == INFINITY ? __int_as_float(0x7fffffff) : LINEAR ? fmaf(fabsf(m_new), 0x1p-22f, m_new) : m_new);
+            corr = (m_i == -INFINITY) ? 0.f : exp2f((m_r - m_s) * unit);
             l_i *= corr;
             lp_i *= corr;
             m_i = m_new;
@@ -502,11 +539,20 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         f32x2 sum = pack2(0.f, 0.f);
         float p0 = 0.f, p1 = 0.f;
         const f32x2 nms2 = pack2(-m_s, -m_s);
+        [[maybe_unused]] f32x2 add = nms2, step = nms2;
+        if constexpr (LINEAR) step = pack2(2.f * slope, 2.f * slope);
 #pragma unroll
         for (int c = 0; c < 32; c++) {
           float e0 = __uint_as_float(r[2 * c]), e1 = __uint_as_float(r[2 * c + 1]);
           // (the difference first: with the maximum scaled ahead and a fused product, what its rounding left would be the exponent of scores far from zero)
-          if constexpr (CAP != CAP_ZERO) {
+          if constexpr (LINEAR) {
+            if (c % 16 == 0) {                           // (counted up anew every 32 columns: its rounding errors do not pile up)
+              const float base = fmaf(slope, (float)(c0 + 2 * c - (row + off)), -m_s);
+              add = pack2(base, base + slope);
+            }
+            unpack2(fma2(pack2(e0, e1), scale2, add), e0, e1);
+            add = add2(add, step);
+          } else if constexpr (CAP != CAP_ZERO) {
             f32x2 x = add2(pack2(e0, e1), nms2);
             if constexpr (!MADE) x = mul2(x, scale2);
             unpack2(x, e0, e1);
@@ -606,7 +652,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           leave(&to_lo, hi, set * (D / 2) + c, C::OUT_BYTES - 2048);
         }
       }
-      if (set == 0 && row < p.Sq) p.lse[((long long)t.b * p.hq + t.h) * p.Sq + row] = l_i != 0.f ? m_s * (MADE ? LN2 : p.scale) + logf(l_i) : -INFINITY;
+      if (set == 0 && row < p.Sq) p.lse[((long long)t.b * p.hq + t.h) * p.Sq + row] = l_i != 0.f ? m_s * (MADE || LINEAR ? LN2 : p.scale) + logf(l_i) : -INFINITY;
       if (cta < 0) break;
       t = next;
       see = see_next;

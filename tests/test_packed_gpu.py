@@ -112,6 +112,19 @@ def test_gradients_against_differences(cap, alibi):
         assert abs(((f[0] - f[1]) / (2 * eps) / u.square().sum()).item() - 1) < 5e-3, name
 
 
+@pytest.mark.parametrize("cap", [0.0, 20.0, 200.0])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("S,d", [(300, 64), (500, 128)])
+def test_attention_slopes(S, d, causal, cap):
+    """From no slope to slopes that leave a row its own key alone, with scores that are large enough for far keys to count."""
+    slopes = torch.tensor([0.0, 0.01, 1.3, 1.4, 5.0, 100.0], device="cuda")
+    q, k, v, do = _rand(1, S, 6, d, scale=6.0, seed=1), _rand(1, S, 2, d, seed=2), _rand(1, S, 2, d, seed=3), _rand(1, S, 6, d, seed=4)
+    got = _run(q, k, v, do, causal=causal, softcap=cap, slopes=slopes)
+    _status_ok()
+    for name, g, w in zip(("o", "dq", "dk", "dv"), got, attention64(q, k, v, visible(1, S, S, causal), d ** -0.5, cap, slopes, do)):
+        assert torch.isfinite(g).all() and rel(g, w) < 5e-3, name
+
+
 @pytest.mark.parametrize("B,S,hq,hkv,d", [(1, 500, 8, 1, 64), (6, 300, 8, 4, 128)])
 def test_attention_repeats_its_bits(B, S, hq, hkv, d):
     """o, dk and dv are summed in a fixed order, also where a key block's walk is cut into parts (the first); so is dq up to 128 keys."""
