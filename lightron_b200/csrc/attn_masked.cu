@@ -154,14 +154,23 @@ extern "C" int lb_attn_mask(const void* ids, int id_bytes, const void* marks, co
   return LB_OK;
 }
 
+// Bytes of the forward's workspace: 0 where it uses none, as for sizes that it does not take.
+extern "C" long long lb_masked_attn_fwd_ws_bytes(int B, int Sq, int Sk, int hq, int hkv, int d) {
+  MaParams p{};
+  if (check_sizes(B, Sq, Sk, hq, hkv, d)) return 0;
+  p.B = B; p.Sq = Sq; p.Sk = Sk; p.hq = hq; p.hkv = hkv; p.d = d;
+  return ma_fwd_ws_bytes(p);
+}
+
 // Forward.  strides: 3 x {batch, token, head} of q, k, v in elements, multiples of 8; o, o_lo (or null) [B, Sq, hq, d] and lse [B, hq, Sq] contiguous.
 // head_dim a multiple of 8 up to 128, Sk >= Sq; slopes null or fp32 [hq]; q_bounds / k_bounds of lb_attn_mask() over Sk positions, or null: causal or all keys.
-extern "C" int lb_masked_attn_fwd(const void* q, const void* k, const void* v, void* o, void* o_lo, void* lse, int B, int Sq, int Sk, int hq, int hkv, int d,
-                                  const long long* strides, float scale, int causal, float softcap, const void* slopes, const void* q_bounds, const void* k_bounds,
-                                  void* stream) {
+// ws: lb_masked_attn_fwd_ws_bytes(), 16-byte aligned, not initialised (with less, or null, few tiles are not split over their keys).
+extern "C" int lb_masked_attn_fwd(const void* q, const void* k, const void* v, void* o, void* o_lo, void* lse, void* ws, long long ws_bytes, int B, int Sq, int Sk, int hq, int hkv,
+                                  int d, const long long* strides, float scale, int causal, float softcap, const void* slopes, const void* q_bounds, const void* k_bounds, void* stream) {
   MaParams p;
   if (const int rc = fill(p, q, k, v, o, o_lo, lse, B, Sq, Sk, hq, hkv, d, strides, scale, causal, softcap, slopes, q_bounds, k_bounds)) return rc;
-  return ma_launch_fwd(p, (cudaStream_t)stream);
+  if (misaligned(ws)) return LB_ERR_ARG;
+  return ma_launch_fwd(p, ws, ws ? ws_bytes : 0, (cudaStream_t)stream);
 }
 
 // Bytes of the backward's workspace; 0 for sizes that it does not take.

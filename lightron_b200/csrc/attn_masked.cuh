@@ -32,7 +32,8 @@ struct MaBwdParams {
   float* stats;
 };
 
-int ma_launch_fwd(const MaParams& p, cudaStream_t s);
+int ma_launch_fwd(const MaParams& p, void* ws, long long ws_bytes, cudaStream_t s);
+long long ma_fwd_ws_bytes(const MaParams& p);
 int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s);
 long long ma_bwd_ws_bytes(const MaParams& p);
 

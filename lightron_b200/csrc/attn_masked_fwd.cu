@@ -20,6 +20,7 @@
 //   * o is divided by the sum of the weights as they are rounded for P V.  A row that all but one key leave cold has o = v of that key then, and a D = do . o whose
 //     error is as small as the differences dP - D that the backward lives on (the weight's own rounding, 2^-9 of dP, would drown them); lse is of the sum of the
 //     unrounded ones, from which the backward's P are made.
+//   * few tiles share their key blocks between CTAs, which leave O in fp32 with its reference and sums; another kernel joins them.
 //   * o leaves twice: rounded, and what the rounding left (for the backward's row sums).
 // What bounds it: latency, with instructions close behind.  Of the active cycles 61 % of the issue slots and 41 to 52 % of the exponentials' unit (d 64, two tiles per SM), 39 %
 // of the tensor pipe (d 128); a block takes 1960 (d 64) / 2400 cycles (d 128, cap) of an SM, 2530 with documents, whose loops are short and whose blocks are nearly all masked.
@@ -45,6 +46,8 @@ struct FwdParams {
   int group;                     // (batch, head) pairs whose tiles are ordered together
   FastDiv by_grp, by_group, by_last, by_hq, by_rep;    // entries of a group, heads of a group / of the last one, hq, hq / hkv
   MaTerms f;
+  int splits;                    // CTAs of a tile, each with a share of its key blocks, which leave parts
+  float *part_o, *part_s;        // [tile][split] x [D / 4][128 rows][4] fp32, and x [reference, sum, rounded sum][128 rows]
 };
 
 enum : int { NO_CAP, CAP_ZERO, CAP_MAX };      // CAP_ZERO: exponentials relative to zero, CAP_MAX: to the running maximum
@@ -170,9 +173,11 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
   // their K / V in L2 together.  A resident CTA goes on with entries that have not been started (cluster launch control).
   volatile int* abort_flag = s_abort;
   const int off = p.Sk - p.Sq;
-  struct Tile { int m0, b, h, hk, key0, nb; };
+  struct Tile { int m0, b, h, hk, key0, nb, split; };
   auto tile_of = [&](int cid) {
     Tile t;
+    t.split = 0;
+    if (pp.splits > 1) { t.split = cid % pp.splits; cid /= pp.splits; }
     const int grp = pp.by_grp.div(cid);
     const int in_grp = cid - grp * (int)pp.by_grp.d;
     const FastDiv& heads = (grp + 1) * pp.group <= p.hq * p.B ? pp.by_group : pp.by_last;
@@ -185,6 +190,12 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     t.key0 = ma_keys(p, t.b, t.m0).x;
     // (a tile whose rows see nothing takes one block, all of it hidden)
     t.nb = max((ma_keys(p, t.b, min(t.m0 + C::BM, p.Sq) - 1).y - t.key0 + C::BN - 1) / C::BN, 1);
+    if (pp.splits > 1) {
+      // (a share behind the tile's last block is one block that all rows' intervals hide)
+      const int share = (t.nb + pp.splits - 1) / pp.splits, first = min(t.split * share, t.nb);
+      t.key0 += first * C::BN;
+      t.nb = max(min(share, t.nb - first), 1);
+    }
     return t;
   };
   // Entry n + 1 of this CTA: the answer to request n, or -1 at the end.
@@ -317,20 +328,20 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           if constexpr (SPLIT) {
             issue_half(0, last);
             issue_half(1, last);
-            return;
-          }
+          } else {
 #pragma unroll
-          for (int a = 0; a < C::ATOMS; a++) {
-            const uint64_t ka = dk0 + (uint64_t)((ks * C::SLOT_BYTES) >> 4);
+            for (int a = 0; a < C::ATOMS; a++) {
+              const uint64_t ka = dk0 + (uint64_t)((ks * C::SLOT_BYTES) >> 4);
 #pragma unroll
-            for (int s = 0; s < 4; s++)
-              if (a * 4 + s < slices)
-                umma_bf16(s_dst, qa + (uint64_t)((a * C::SLOT_BYTES + s * 32) >> 4), ka + (uint64_t)((s * 32) >> 4), idesc_s, (a | s) ? 1u : 0u);
-            if (a == C::ATOMS - 1) umma_commit(s_full);
-            umma_commit(empty(ks));
-            ring(ks, kp, a == C::ATOMS - 1 ? C::UNITS - C::ATOMS + 1 : 1);
+              for (int s = 0; s < 4; s++)
+                if (a * 4 + s < slices)
+                  umma_bf16(s_dst, qa + (uint64_t)((a * C::SLOT_BYTES + s * 32) >> 4), ka + (uint64_t)((s * 32) >> 4), idesc_s, (a | s) ? 1u : 0u);
+              if (a == C::ATOMS - 1) umma_commit(s_full);
+              umma_commit(empty(ks));
+              ring(ks, kp, a == C::ATOMS - 1 ? C::UNITS - C::ATOMS + 1 : 1);
+            }
+            if (last) umma_commit(q_empty);
           }
-          if (last) umma_commit(q_empty);
         };
         // SPLIT: O += P V by halves of 64 keys, each with S of the next block's behind it: the softmax threads of one half work while the products of the other run.
         // (The first P V of a tile waits for both: until then the last tile's O is still being read.)
@@ -613,6 +624,25 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       if (!ok || !mbar_wait(pv_done, C::P_ALIAS ? (uint32_t)n & 1u : (g - 1) & 1u, abort_flag)) ok = false;
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       fence_after();
+      if (pp.splits > 1) {                         // (one tile per CTA)
+        const long long part = (((long long)t.b * p.hq + t.h) * pp.tiles_x + t.m0 / C::BM) * pp.splits + t.split;
+        float4* o = reinterpret_cast<float4*>(pp.part_o + part * (C::BM * D)) + set * (D / 8) * C::BM + quad * 32 + lane;
+#pragma unroll 1
+        for (int c = 0; c < D / 2; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(to_addr + c, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 8; i++) o[(c / 4 + i) * C::BM] = reinterpret_cast<const float4*>(r)[i];
+        }
+        if (set == 0) {
+          float* s = pp.part_s + part * (3 * C::BM) + quad * 32 + lane;
+          s[0] = l_i != 0.f ? m_s * (MADE || LINEAR ? 1.f : pp.f.scale1) : -INFINITY;
+          s[C::BM] = l_i;
+          s[2 * C::BM] = lp_i;
+        }
+        break;
+      }
       const float inv = lp_i != 0.f ? 1.f / lp_i : 0.f;
       // 32 columns at a time through shared memory and TMA stores, which leave out rows past the last and columns past head_dim
       auto leave = [&](const CUtensorMap* map, const uint4* v, int col, int at) {      // v: 32 columns of the lane's row
@@ -669,6 +699,66 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
   }
 }
 
+// Adds up the parts of a tile's rows: weights by their references, the order of the splits.  A thread has 8 columns of a row; a warp's stores are whole rows.
+template <int D>
+__global__ void ma_join_kernel(const __grid_constant__ FwdParams pp) {
+  grid_go();
+  grid_wait();
+  const MaParams& p = pp.a;
+  constexpr int TPR = D / 8;
+  const int c = threadIdx.x % TPR, rows = blockDim.x / TPR;
+  const long long total = (long long)p.B * p.hq * p.Sq;
+  for (long long at = (long long)blockIdx.x * rows + threadIdx.x / TPR; at < total; at += (long long)gridDim.x * rows) {
+    const int i = (int)(at % p.Sq), h = (int)(at / p.Sq % p.hq), b = (int)(at / p.Sq / p.hq), r = i & 127;
+    const long long part = (((long long)b * p.hq + h) * pp.tiles_x + i / 128) * pp.splits;
+    const float* s = pp.part_s + part * 384 + r;
+    float m = -INFINITY;
+    for (int k = 0; k < pp.splits; k++) m = max2(m, s[k * 384]);
+    float l = 0.f, lp = 0.f, f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const float4* o = reinterpret_cast<const float4*>(pp.part_o + part * (128 * D)) + 2 * c * 128 + r;
+    for (int k = 0; k < pp.splits; k++) {
+      const float from = s[k * 384];
+      if (from == -INFINITY) continue;                       // (has seen nothing)
+      const float w = exp2f(from - m);
+      const float4 x = o[(long long)k * (32 * D)], y = o[(long long)k * (32 * D) + 128];
+      l += w * s[k * 384 + 128];
+      lp += w * s[k * 384 + 256];
+      f[0] += w * x.x; f[1] += w * x.y; f[2] += w * x.z; f[3] += w * x.w;
+      f[4] += w * y.x; f[5] += w * y.y; f[6] += w * y.z; f[7] += w * y.w;
+    }
+    const float inv = lp != 0.f ? 1.f / lp : 0.f;
+    if (c * 8 < p.d) {
+      const long long to = (((long long)b * p.Sq + i) * p.hq + h) * p.d + c * 8;
+      float back[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) f[k] *= inv;
+      const uint4 hi = pack8(f);
+      *reinterpret_cast<uint4*>(p.o + to) = hi;
+      if (p.o_lo) {
+        unpack8(hi, back);
+#pragma unroll
+        for (int k = 0; k < 8; k++) f[k] -= back[k];
+        *reinterpret_cast<uint4*>(p.o_lo + to) = pack8(f);
+      }
+    }
+    if (c == 0) p.lse[at] = l != 0.f ? m * LN2 + logf(l) : -INFINITY;
+  }
+}
+
+// CTAs of a tile: one where there is a tile for each SM, else as many as find room (two per SM), with four key blocks or more each.  Whole / split, us, causal: 8192 queries and keys, 1 head,
+// d 64 97 / 45; 2 heads, d 128, cap 121 / 74; 4 x 4096 of 4 heads, d 128, cap 68 / 46; 2048, 4 heads, d 64 27 / 22; one query, 32 / 8 heads, d 128, 8192 keys 118 / 37, 4 x 32768 keys
+// 557 / 296; left whole 1024, 8 heads, d 128 19.7 / 20.4 and 2 x 1024, 8 heads, d 64 19.5 / 19.2.  (Where the mask comes from the device the length of the walks is not known here: that of all keys is taken.)
+int splits_of(int B, int Sq, int Sk, int hq, int sms) {
+  const long long tiles = (long long)((Sq + 127) / 128) * hq * B;
+  const int blocks = (Sk + 127) / 128;
+  if (tiles > sms || blocks <= 8) return 1;
+  const long long room = 2LL * sms / tiles;
+  return (int)(room < blocks / 4 ? room : blocks / 4);
+}
+long long part_floats(int B, int Sq, int hq, int d, int splits) {
+  return splits > 1 ? (long long)((Sq + 127) / 128) * hq * B * splits * 128 : 0;
+}
+
 template <int D, int CAP, bool BIAS>
 int launch(const CUtensorMap* maps, const FwdParams& p, unsigned grid, cudaStream_t s) {
   using C = Cfg<D>;
@@ -681,11 +771,16 @@ int launch(const CUtensorMap* maps, const FwdParams& p, unsigned grid, cudaStrea
     cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     attr = true;
   }
-  return lb_launch(fn, grid, THREADS, C::SMEM, s, maps[0], maps[1], maps[2], maps[3], maps[4], p);
+  LB_LAUNCH(fn, grid, THREADS, C::SMEM, s, maps[0], maps[1], maps[2], maps[3], maps[4], p);
+  if (p.splits > 1) {
+    const long long blocks = ((long long)p.a.B * p.a.hq * p.a.Sq * (D / 8) + 255) / 256, cap = lb_num_sms() * 16;
+    LB_LAUNCH(ma_join_kernel<D>, (unsigned)(blocks < cap ? blocks : cap), 256, 0, s, p);
+  }
+  return LB_OK;
 }
 
 template <int D>
-int launch_fwd(const MaParams& a, cudaStream_t s) {
+int launch_fwd(const MaParams& a, void* ws, long long ws_bytes, cudaStream_t s) {
   CUtensorMap maps[5];      // q, k, v, o, o_lo
   int rc;
   const uint64_t B = a.B, Sq = a.Sq, Sk = a.Sk, hq = a.hq, hkv = a.hkv, d = a.d;
@@ -701,14 +796,17 @@ int launch_fwd(const MaParams& a, cudaStream_t s) {
   const long long kv_bytes = 4LL * D * a.Sk, pairs = (long long)a.hq * a.B;
   const long long kv_heads = kv_bytes >= (48LL << 20) ? 1 : (48LL << 20) / kv_bytes;
   p.group = (int)(kv_heads * (a.hq / a.hkv) < pairs ? kv_heads * (a.hq / a.hkv) : pairs);
-  const long long grid = p.tiles_x * pairs;
+  p.splits = ws_bytes > 0 && ws_bytes >= ma_fwd_ws_bytes(a) ? splits_of(a.B, a.Sq, a.Sk, a.hq, lb_num_sms()) : 1;
+  p.part_o = (float*)ws;
+  p.part_s = p.part_o + part_floats(a.B, a.Sq, a.hq, a.d, p.splits) * D;
+  const long long grid = p.tiles_x * pairs * p.splits;
   if (grid > 2147483647LL) return LB_ERR_SHAPE;
   p.by_grp.set((unsigned)(p.tiles_x * p.group));
   p.by_group.set((unsigned)p.group);
   p.by_last.set((unsigned)(pairs % p.group ? pairs % p.group : p.group));
   p.by_hq.set((unsigned)a.hq);
   p.by_rep.set((unsigned)(a.hq / a.hkv));
-  p.steal = grid > 2 * lb_num_sms();      // (with all tiles resident at once there is none to take)
+  p.steal = p.splits == 1 && grid > 2 * lb_num_sms();      // (with all tiles resident at once there is none to take)
   p.f.set(a, true, twice);
   const bool bias = a.slopes != nullptr;
   if (a.softcap <= 0.f) return bias ? launch<D, NO_CAP, true>(maps, p, (unsigned)grid, s) : launch<D, NO_CAP, false>(maps, p, (unsigned)grid, s);
@@ -718,7 +816,15 @@ int launch_fwd(const MaParams& a, cudaStream_t s) {
 
 }  // namespace
 
-int ma_launch_fwd(const MaParams& p, cudaStream_t s) { return p.d <= 64 ? launch_fwd<64>(p, s) : launch_fwd<128>(p, s); }
+// Bytes of the parts' workspace: 0 where tiles are not split.
+long long ma_fwd_ws_bytes(const MaParams& p) {
+  const int splits = splits_of(p.B, p.Sq, p.Sk, p.hq, lb_num_sms());
+  return part_floats(p.B, p.Sq, p.hq, p.d, splits) * ((p.d <= 64 ? 64 : 128) + 3) * (long long)sizeof(float);
+}
+
+int ma_launch_fwd(const MaParams& p, void* ws, long long ws_bytes, cudaStream_t s) {
+  return p.d <= 64 ? launch_fwd<64>(p, ws, ws_bytes, s) : launch_fwd<128>(p, ws, ws_bytes, s);
+}
 
 // Copies the status words of the forward to host memory and clears them.
 extern "C" int lb_masked_attn_status(void* out) {

@@ -54,7 +54,8 @@ struct Api {
   int (*lb_ce_grad)(P, P, P, W, P, int, int, L, int, float, int, W);
   int (*lb_gemm_rope)(P, P, W, int, int, int, P, P, P, int, int, int, W);
   int (*lb_attn_mask)(P, int, P, P, int, int, int, W, W, W);
-  int (*lb_masked_attn_fwd)(P, P, P, W, W, W, int, int, int, int, int, int, const L*, float, int, float, P, P, P, W);
+  L (*lb_masked_attn_fwd_ws_bytes)(int, int, int, int, int, int);
+  int (*lb_masked_attn_fwd)(P, P, P, W, W, W, W, L, int, int, int, int, int, int, const L*, float, int, float, P, P, P, W);
   L (*lb_masked_attn_bwd_ws_bytes)(int, int, int, int, int, int, int);
   int (*lb_masked_attn_bwd)(P, P, P, P, P, P, P, W, L, W, W, W, int, int, int, int, int, int, const L*, float, int, float, P, P, P, W);
   int (*lb_rope_axes)(P, W, P, P, P, const unsigned char*, int, int, int, int, int, int, const L*, L, L, int, W);
@@ -394,7 +395,10 @@ struct MaskedAttention : Function<MaskedAttention> {
     if (a.grad) lo = at::empty({m.B, m.Sq, m.hq, m.d}, q.options());
     L st[9];
     put_strides(st, q); put_strides(st + 3, k); put_strides(st + 6, v);
-    LB_CALL(lb_masked_attn_fwd, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.mutable_data_ptr(), const_cast<W>(ptr(lo)), lse.mutable_data_ptr(), m.B, m.Sq, m.Sk, m.hq,
+    const L bytes = api.lb_masked_attn_fwd_ws_bytes(m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d);
+    Tensor ws;
+    if (bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte));
+    LB_CALL(lb_masked_attn_fwd, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.mutable_data_ptr(), const_cast<W>(ptr(lo)), lse.mutable_data_ptr(), const_cast<W>(ptr(ws)), bytes, m.B, m.Sq, m.Sk, m.hq,
             m.hkv, m.d, st, m.scale, m.causal, (float)a.softcap, ptr(sl), ptr(qi), ptr(ki), stream());
     if (a.grad) {
       ctx->save_for_backward({q0, k0, v0, o, lo, lse, sl, qi, ki});
@@ -989,7 +993,7 @@ PyObject* py_init(PyObject*, PyObject* args) {
   LB_TAKE(lb_rmsnorm_fwd); LB_TAKE(lb_rmsnorm_bwd_blocks); LB_TAKE(lb_rmsnorm_bwd); LB_TAKE(lb_rope); LB_TAKE(lb_gemm_grouped_epi);
   LB_TAKE(lb_flash_fwd_tc); LB_TAKE(lb_flash_bwd_ws_bytes_kv); LB_TAKE(lb_flash_bwd_tc_ws); LB_TAKE(lb_flash_bwd); LB_TAKE(lb_embedding_fwd); LB_TAKE(lb_clear);
   LB_TAKE(lb_embedding_bwd); LB_TAKE(lb_ce_stats); LB_TAKE(lb_ce_loss); LB_TAKE(lb_ce_grad); LB_TAKE(lb_gemm_rope);
-  LB_TAKE(lb_attn_mask); LB_TAKE(lb_masked_attn_fwd); LB_TAKE(lb_masked_attn_bwd_ws_bytes); LB_TAKE(lb_masked_attn_bwd); LB_TAKE(lb_rope_axes);
+  LB_TAKE(lb_attn_mask); LB_TAKE(lb_masked_attn_fwd_ws_bytes); LB_TAKE(lb_masked_attn_fwd); LB_TAKE(lb_masked_attn_bwd_ws_bytes); LB_TAKE(lb_masked_attn_bwd); LB_TAKE(lb_rope_axes);
   LB_TAKE(lb_grad_norm_parts); LB_TAKE(lb_grad_squares); LB_TAKE(lb_grad_total); LB_TAKE(lb_grad_scale);
   if (!ok) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "an entry point of the kernels is missing");

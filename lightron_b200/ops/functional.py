@@ -829,7 +829,9 @@ def masked_fwd_native(q, k, v, causal: bool, scale: float, softcap: float, slope
     o = torch.empty(B, Sq, hq, d, dtype=q.dtype, device=q.device)
     o_lo = torch.empty_like(o) if grad else None
     lse = torch.empty(B, hq, Sq, dtype=torch.float32, device=q.device)
-    native.call("lb_masked_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), native.ptr(o_lo), lse.data_ptr(), B, Sq, Sk, hq, hkv, d,
+    nbytes = native.require().lb_masked_attn_fwd_ws_bytes(B, Sq, Sk, hq, hkv, d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    native.call("lb_masked_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), native.ptr(o_lo), lse.data_ptr(), native.ptr(ws), nbytes, B, Sq, Sk, hq, hkv, d,
                 _strides(q, k, v), scale, int(causal), softcap, native.ptr(slopes), native.ptr(qb), native.ptr(kb), native.stream_ptr())
     return o, o_lo, lse
 

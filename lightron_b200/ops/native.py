@@ -90,7 +90,8 @@ _SIGNATURES = {
     "lb_dp_status": [_P],
     "lb_dp_adamw": [_P, _P, _P, _P, _P, _P, _P, _L, _L, _I, _I, ctypes.c_uint, _F, _F, _F, _F, _F, _F, _F, _F, _I, _P],
     "lb_attn_mask": [_P, _I, _P, _P, _I, _I, _I, _P, _P, _P],
-    "lb_masked_attn_fwd": [_P] * 6 + [_I] * 6 + [_P, _F, _I, _F, _P, _P, _P, _P],
+    "lb_masked_attn_fwd_ws_bytes": [_I] * 6,
+    "lb_masked_attn_fwd": [_P] * 7 + [_L] + [_I] * 6 + [_P, _F, _I, _F, _P, _P, _P, _P],
     "lb_masked_attn_status": [_P],
     "lb_masked_attn_bwd": [_P] * 8 + [_L] + [_P] * 3 + [_I] * 6 + [_P, _F, _I, _F, _P, _P, _P, _P],
     "lb_masked_attn_bwd_ws_bytes": [_I] * 7,
@@ -273,7 +274,7 @@ def call(name: str, *args) -> None:
 _HOST = False               # not looked for yet; then the extension module, or None
 _HOST_ENTRIES = ("lb_rmsnorm_fwd", "lb_rmsnorm_bwd_blocks", "lb_rmsnorm_bwd", "lb_rope", "lb_gemm_grouped_epi", "lb_flash_fwd_tc",
                  "lb_flash_bwd_ws_bytes_kv", "lb_flash_bwd_tc_ws", "lb_flash_bwd", "lb_embedding_fwd", "lb_clear", "lb_embedding_bwd", "lb_ce_stats",
-                 "lb_ce_loss", "lb_ce_grad", "lb_gemm_rope", "lb_attn_mask", "lb_masked_attn_fwd", "lb_masked_attn_bwd_ws_bytes", "lb_masked_attn_bwd", "lb_rope_axes",
+                 "lb_ce_loss", "lb_ce_grad", "lb_gemm_rope", "lb_attn_mask", "lb_masked_attn_fwd_ws_bytes", "lb_masked_attn_fwd", "lb_masked_attn_bwd_ws_bytes", "lb_masked_attn_bwd", "lb_rope_axes",
                  "lb_grad_norm_parts", "lb_grad_squares", "lb_grad_total", "lb_grad_scale")
 
 

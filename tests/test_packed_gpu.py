@@ -112,6 +112,23 @@ def test_gradients_against_differences(cap, alibi):
         assert abs(((f[0] - f[1]) / (2 * eps) / u.square().sum()).item() - 1) < 5e-3, name
 
 
+@pytest.mark.parametrize("d", [64, 128, 40])
+@pytest.mark.parametrize("B,Sq,Sk,hq,hkv,causal,docs,prefix,cap,alibi,scale", [
+    (1, 1, 2300, 2, 1, True, 0, False, 0.0, False, 4.0),         # one query over many keys
+    (3, 1, 1030, 4, 2, True, 200, False, 30.0, True, 2.0),
+    (1, 70, 2300, 2, 2, True, 0, False, 0.0, True, 4.0),
+    (1, 1300, 1300, 2, 1, True, 0, False, 0.0, False, 8.0),      # tiles of which some shares hold nothing
+    (1, 1300, 1300, 1, 1, True, 150, True, 50.0, False, 4.0),
+    (1, 1100, 1100, 2, 1, False, 400, False, 200.0, True, 4.0),
+    (2, 1025, 1025, 2, 2, True, 300, False, 0.0, False, 2.0),    # padding: rows that no share sees
+])
+def test_attention_split_over_keys(B, Sq, Sk, hq, hkv, causal, docs, prefix, cap, alibi, scale, d):
+    """Few tiles: their key blocks are shared between CTAs and the parts joined."""
+    from lightron_b200.ops import native
+    assert native.require().lb_masked_attn_fwd_ws_bytes(B, Sq, Sk, hq, hkv, d) > 0
+    test_attention(B, Sq, Sk, hq, hkv, causal, docs, prefix, cap, alibi, scale, d)
+
+
 @pytest.mark.parametrize("cap", [0.0, 20.0, 200.0])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("S,d", [(300, 64), (500, 128)])
