@@ -724,7 +724,8 @@ int launch_form(const CUtensorMap* m, const BwdParams& p, unsigned grid, cudaStr
 
 // CTAs of a key block, for its walk over query blocks of all heads of the group.  In query blocks: a CTA's fixed part is some 6, leaving dK / dV in fp32 instead of
 // writing them 3 and their conversion 2 more (the figures of the causal backward's model); where the mask comes from the device its lengths are not known
-// here, and those of a causal mask are taken.
+// here, and those of a causal mask are taken.  Whole / parts, all kernels as a graph, us, causal: 2 x 2000, 16 / 2 heads, d 64 213 / 78; 1 x 2000, 16 / 4, d 128 156 / 79; 1 x 8192, 8 / 2, d 128
+// 577 / 341; 4 x 500, 16 / 4, d 64 41 / 35; 2 x 1000, 16 / 4, d 96 80 / 51; 1 x 300, 8 / 2, d 64 30 / 14; left whole 8 x 2048, 32 / 4, d 64.
 int parts_of(int B, int Sq, int Sk, int hq, int hkv, int causal, int sms) {
   const int n_mblocks = (Sq + 127) / 128, n_nblk = (Sk + 127) / 128, rep = hq / hkv, off = Sk - Sq;
   const long long pairs = (long long)hkv * B;
@@ -754,6 +755,8 @@ int launch_bwd(BwdParams& p, cudaStream_t s) {
   if ((rc = make_map_bf16_4d(m + 3, w.dout, d, hq, Sq, B, w.dos.h, w.dos.s, w.dos.b, 128))) return rc;
   if ((rc = make_map_bf16_4d(m + 4, w.dk, d, hkv, Sk, B, w.dks.h, w.dks.s, w.dks.b, 32))) return rc;
   if ((rc = make_map_bf16_4d(m + 5, w.dv, d, hkv, Sk, B, w.dvs.h, w.dvs.s, w.dvs.b, 32))) return rc;
+  // Up to 128 keys a query block's dQ comes from one CTA, which writes it: nothing to clear, to add to and to convert.  Added / written, as a graph, us: 4 x 128, 12 heads, d 64 13.2 / 10.3,
+  // 8 x 128, 32 heads 24.6 / 18.5, 32 x 128, 32 / 8 heads 54 / 41; 8 x 100, 16 heads, d 128 18.6 / 14.4.
   const bool alone = a.Sk <= 128;
   const long long grid = (long long)((a.Sk + 127) / 128) * a.hkv * a.B * p.parts;
   if (grid > 2147483647LL) return LB_ERR_SHAPE;

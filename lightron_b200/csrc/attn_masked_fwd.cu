@@ -9,7 +9,7 @@
 //   * the keys of a tile run from the first key of its first row to the last key of its last (the ends never fall), from exactly there: blocks start
 //     at any key, so that a document of n keys takes ceil(n / 128) of them wherever it lies.  Blocks inside all 32 intervals of a warp are not masked.
 //   * with a cap the scores are known to lie within it.  Up to softcap * log2(e) = 80 exponentials are taken relative to zero instead of the running
-//     maximum: 2^+-80 and sums of them are far inside fp32 (and bf16 has the same exponents), and nothing is ever rescaled.  With 128 columns the two halves of a
+//     maximum: 2^+-80 and sums of them are far inside fp32 (and bf16 has the same exponents), and nothing is ever rescaled (8 x 2048, d 64 with the maximum / without 400 / 304 us, 1 x 8192, d 128 828 / 566).  With 128 columns the two halves of a
 //     block then have nothing to tell each other, and their scores, P and products run apart (d 128, cap: 700 -> 640 us).  Above 80 the maximum is kept.
 //   * tanh: where no score of 32 rows x 64 columns is above 0.6 caps, x times a polynomial in x^2 on the FMA pipe, two at a time (relative error
 //     2.1e-6, found by least squares with re-weighted points; 7e-5 of a score at most); else by its definition with exp2, whose units the softmax needs itself.

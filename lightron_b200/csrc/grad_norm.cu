@@ -23,7 +23,7 @@ struct Tensors {
   long long count[N];
   int first[N];                                // chunks ahead of a tensor's, with its type in the upper two bits
 };
-static_assert(sizeof(Tensors<MAX_TENSORS>) <= 32000 && sizeof(Tensors<FEW_TENSORS>) <= 4000, "kernel parameters: 32 KB, or 4 KB in the quicker way");
+static_assert(sizeof(Tensors<MAX_TENSORS>) <= 32000 && sizeof(Tensors<FEW_TENSORS>) <= 4000, "kernel parameters: 32 KB, or 4 KB, which a launch takes 3 us less for");
 
 __device__ __forceinline__ float to_f(bf16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }

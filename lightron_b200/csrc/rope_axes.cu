@@ -75,7 +75,8 @@ extern "C" int lb_rope_axes(const void* x, void* y, const void* cosT, const void
     if (axes[i] >= n_axes) return LB_ERR_ARG;
     p.axis[i] = axes[i];
   }
-  // all heads of a token by one warp, or by several where there are few tokens: at least one round of loads each, eight warps per SM
+  // all heads of a token by one warp, or by several where there are few tokens: at least one round of loads each, eight warps per SM (1 and 20 tokens, 40 heads of 128, as a graph, one warp /
+  // several, us: 6.2 / 4.1; 300 and 1000 tokens 6.2 in both)
   const long long tokens = (long long)B * S, blocks = (tokens + 7) / 8;
   if (blocks > 2147483647LL) return LB_ERR_SHAPE;
   const int round = 32 / (d / 8) * AHEAD, most = (h + round - 1) / round;
