@@ -12,6 +12,7 @@
 
 namespace {
 
+// (Lists of few tensors in fewer parameters: clipping 38 of them, alone on the GPU, 38 -> 35 us.)
 constexpr int THREADS = 256, MAX_TENSORS = 768, FEW_TENSORS = 96, CHUNK = 16384;
 enum : int { BF16 = 0, FP16 = 1, FP32 = 2 };
 
@@ -23,7 +24,7 @@ struct Tensors {
   long long count[N];
   int first[N];                                // chunks ahead of a tensor's, with its type in the upper two bits
 };
-static_assert(sizeof(Tensors<MAX_TENSORS>) <= 32000 && sizeof(Tensors<FEW_TENSORS>) <= 4000, "kernel parameters: 32 KB, or 4 KB, which a launch takes 3 us less for");
+static_assert(sizeof(Tensors<MAX_TENSORS>) <= 32000 && sizeof(Tensors<FEW_TENSORS>) <= 4000, "kernel parameters: 32 KB, or 4 KB");
 
 __device__ __forceinline__ float to_f(bf16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
