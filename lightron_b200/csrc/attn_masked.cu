@@ -121,7 +121,7 @@ int check_sizes(int B, int Sq, int Sk, int hq, int hkv, int d) {
 int fill(MaParams& p, const void* q, const void* k, const void* v, void* o, void* o_lo, void* lse, int B, int Sq, int Sk, int hq, int hkv, int d, const long long* st,
          float scale, int causal, float softcap, const void* slopes, const void* q_bounds, const void* k_bounds) {
   if (check_sizes(B, Sq, Sk, hq, hkv, d)) return LB_ERR_SHAPE;
-  if (!q || !k || !v || !o || !lse || !st || !(softcap >= 0.f && softcap < INFINITY) || !(scale > 0.f && scale < INFINITY) || (!q_bounds) != (!k_bounds)) return LB_ERR_ARG;
+  if (!q || !k || !v || !o || (!o_lo) != (!lse) || !st || !(softcap >= 0.f && softcap < INFINITY) || !(scale > 0.f && scale < INFINITY) || (!q_bounds) != (!k_bounds)) return LB_ERR_ARG;
   if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(o) || misaligned(o_lo)) return LB_ERR_ARG;
   p = MaParams{(const bf16*)q, (const bf16*)k, (const bf16*)v, strides_at(st), strides_at(st + 3), strides_at(st + 6), (bf16*)o, (bf16*)o_lo, (float*)lse, B, Sq, Sk, hq, hkv, d,
                scale, causal, softcap, (const float*)slopes, (const int2*)q_bounds, (const int2*)k_bounds};
@@ -162,7 +162,8 @@ extern "C" long long lb_masked_attn_fwd_ws_bytes(int B, int Sq, int Sk, int hq, 
   return ma_fwd_ws_bytes(p);
 }
 
-// Forward.  strides: 3 x {batch, token, head} of q, k, v in elements, multiples of 8; o, o_lo (or null) [B, Sq, hq, d] and lse [B, hq, Sq] contiguous.
+// Forward.  strides: 3 x {batch, token, head} of q, k, v in elements, multiples of 8; o [B, Sq, hq, d] contiguous, as are, for the backward, o_lo [B, Sq, hq, d] and lse
+// [B, hq, Sq] (both, or both null).
 // head_dim a multiple of 8 up to 128, Sk >= Sq; slopes null or fp32 [hq]; q_bounds / k_bounds of lb_attn_mask() over Sk positions, or null: causal or all keys.
 // ws: lb_masked_attn_fwd_ws_bytes(), 16-byte aligned, not initialised (with less, or null, few tiles are not split over their keys).
 extern "C" int lb_masked_attn_fwd(const void* q, const void* k, const void* v, void* o, void* o_lo, void* lse, void* ws, long long ws_bytes, int B, int Sq, int Sk, int hq, int hkv,

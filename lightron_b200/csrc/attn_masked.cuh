@@ -14,7 +14,7 @@ struct MaParams {
   const bf16 *q, *k, *v;
   MaStrides qs, ks, vs;
   bf16 *o, *o_lo;                // [B, Sq, hq, d]; o_lo: null, or what rounding o to bf16 left
-  float* lse;                    // [B, hq, Sq]; -inf: a row that sees nothing
+  float* lse;                    // [B, hq, Sq], with o_lo; -inf: a row that sees nothing
   int B, Sq, Sk, hq, hkv, d;
   float scale;
   int causal;

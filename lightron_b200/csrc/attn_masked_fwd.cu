@@ -134,7 +134,8 @@ __device__ __forceinline__ void scores64(uint32_t* r, const FwdParams& p, float 
   }
 }
 
-template <int D, int CAP, bool BIAS>
+// GRAD: o_lo and lse are wanted
+template <int D, int CAP, bool BIAS, bool GRAD>
 __global__ void __launch_bounds__(THREADS, 2)
 ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to,
               const __grid_constant__ CUtensorMap to_lo, const __grid_constant__ FwdParams pp) {
@@ -572,7 +573,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           e1 = exp2f(e1);
           bf162 pk = __floats2bfloat162_rn(e0, e1);
           pr[c] = *reinterpret_cast<uint32_t*>(&pk);
-          sum = add2(sum, pack2(e0, e1));
+          if constexpr (GRAD) sum = add2(sum, pack2(e0, e1));
           add_halves(pr[c], p0, p1);
         }
         if (j > 0) {
@@ -637,7 +638,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         }
         if (set == 0) {
           float* s = pp.part_s + part * (3 * C::BM) + quad * 32 + lane;
-          s[0] = l_i != 0.f ? m_s * (MADE || LINEAR ? 1.f : pp.f.scale1) : -INFINITY;
+          s[0] = lp_i != 0.f ? m_s * (MADE || LINEAR ? 1.f : pp.f.scale1) : -INFINITY;
           s[C::BM] = l_i;
           s[2 * C::BM] = lp_i;
         }
@@ -676,13 +677,13 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           for (int i = 0; i < 8; i++) r[g8 * 8 + i] = __float_as_uint(f[i] - back[i]);
         }
         leave(&to, hi, set * (D / 2) + c, 0);
-        if (p.o_lo) {
+        if constexpr (GRAD) {
 #pragma unroll
           for (int g8 = 0; g8 < 4; g8++) hi[g8] = pack8(reinterpret_cast<const float*>(r) + g8 * 8);
           leave(&to_lo, hi, set * (D / 2) + c, C::OUT_BYTES - 2048);
         }
       }
-      if (set == 0 && row < p.Sq) p.lse[((long long)t.b * p.hq + t.h) * p.Sq + row] = l_i != 0.f ? m_s * (MADE || LINEAR ? LN2 : p.scale) + logf(l_i) : -INFINITY;
+      if (GRAD && set == 0 && row < p.Sq) p.lse[((long long)t.b * p.hq + t.h) * p.Sq + row] = l_i != 0.f ? m_s * (MADE || LINEAR ? LN2 : p.scale) + logf(l_i) : -INFINITY;
       if (cta < 0) break;
       t = next;
       see = see_next;
@@ -741,7 +742,7 @@ __global__ void ma_join_kernel(const __grid_constant__ FwdParams pp) {
         *reinterpret_cast<uint4*>(p.o_lo + to) = pack8(f);
       }
     }
-    if (c == 0) p.lse[at] = l != 0.f ? m * LN2 + logf(l) : -INFINITY;
+    if (p.lse && c == 0) p.lse[at] = l != 0.f ? m * LN2 + logf(l) : -INFINITY;
   }
 }
 
@@ -759,10 +760,10 @@ long long part_floats(int B, int Sq, int hq, int d, int splits) {
   return splits > 1 ? (long long)((Sq + 127) / 128) * hq * B * splits * 128 : 0;
 }
 
-template <int D, int CAP, bool BIAS>
-int launch(const CUtensorMap* maps, const FwdParams& p, unsigned grid, cudaStream_t s) {
+template <int D, int CAP, bool BIAS, bool GRAD>
+int launch_form(const CUtensorMap* maps, const FwdParams& p, unsigned grid, cudaStream_t s) {
   using C = Cfg<D>;
-  auto fn = ma_fwd_kernel<D, CAP, BIAS>;
+  auto fn = ma_fwd_kernel<D, CAP, BIAS, GRAD>;
   static bool attr = false;
   if (!attr) {
     // the register split must fit in what the launch allocates, or it would wait for registers that nobody gives back
@@ -777,6 +778,12 @@ int launch(const CUtensorMap* maps, const FwdParams& p, unsigned grid, cudaStrea
     LB_LAUNCH(ma_join_kernel<D>, (unsigned)(blocks < cap ? blocks : cap), 256, 0, s, p);
   }
   return LB_OK;
+}
+
+// (Without gradients the sum of the unrounded weights is left out: 2 x 4099, cap 30, d 64 124 -> 118 us, 8 x 2048, documents of 300, d 64 133 -> 131.)
+template <int D, int CAP, bool BIAS>
+int launch(const CUtensorMap* maps, const FwdParams& p, unsigned grid, cudaStream_t s) {
+  return p.a.o_lo ? launch_form<D, CAP, BIAS, true>(maps, p, grid, s) : launch_form<D, CAP, BIAS, false>(maps, p, grid, s);
 }
 
 template <int D>

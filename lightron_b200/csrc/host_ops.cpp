@@ -391,14 +391,17 @@ struct MaskedAttention : Function<MaskedAttention> {
                         const std::optional<Tensor>& kb, MaskedArgs a) {
     const Tensor q = fix_strides(q0), k = fix_strides(k0), v = fix_strides(v0), sl = slopes.value_or(Tensor()), qi = qb.value_or(Tensor()), ki = kb.value_or(Tensor());
     const AttnDims m = dims_of(q, k, a.causal, a.scale);
-    Tensor o = at::empty({m.B, m.Sq, m.hq, m.d}, q.options()), lo, lse = empty_f32({m.B, m.hq, m.Sq}, q);
-    if (a.grad) lo = at::empty({m.B, m.Sq, m.hq, m.d}, q.options());
+    Tensor o = at::empty({m.B, m.Sq, m.hq, m.d}, q.options()), lo, lse;
+    if (a.grad) {
+      lo = at::empty({m.B, m.Sq, m.hq, m.d}, q.options());
+      lse = empty_f32({m.B, m.hq, m.Sq}, q);
+    }
     L st[9];
     put_strides(st, q); put_strides(st + 3, k); put_strides(st + 6, v);
     const L bytes = api.lb_masked_attn_fwd_ws_bytes(m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d);
     Tensor ws;
     if (bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte));
-    LB_CALL(lb_masked_attn_fwd, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.mutable_data_ptr(), const_cast<W>(ptr(lo)), lse.mutable_data_ptr(), const_cast<W>(ptr(ws)), bytes, m.B, m.Sq, m.Sk, m.hq,
+    LB_CALL(lb_masked_attn_fwd, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.mutable_data_ptr(), const_cast<W>(ptr(lo)), const_cast<W>(ptr(lse)), const_cast<W>(ptr(ws)), bytes, m.B, m.Sq, m.Sk, m.hq,
             m.hkv, m.d, st, m.scale, m.causal, (float)a.softcap, ptr(sl), ptr(qi), ptr(ki), stream());
     if (a.grad) {
       ctx->save_for_backward({q0, k0, v0, o, lo, lse, sl, qi, ki});

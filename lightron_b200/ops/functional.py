@@ -821,17 +821,17 @@ def _strides(*ts: torch.Tensor):
 
 
 def masked_fwd_native(q, k, v, causal: bool, scale: float, softcap: float, slopes, qb, kb, grad: bool):
-    """(o, what rounding o to bf16 left or None, lse): the backward's row sums of ``do * o`` need o to more than 8 bits where a row sees
+    """(o, what rounding o to bf16 left, lse; both None without gradients): the backward's row sums of ``do * o`` need o to more than 8 bits where a row sees
     few keys, for its score gradients are differences that then all but vanish."""
     q, k, v = _strided(q), _strided(k), _strided(v)
     B, Sq, hq, d = q.shape
     Sk, hkv = k.shape[1], k.shape[2]
     o = torch.empty(B, Sq, hq, d, dtype=q.dtype, device=q.device)
     o_lo = torch.empty_like(o) if grad else None
-    lse = torch.empty(B, hq, Sq, dtype=torch.float32, device=q.device)
+    lse = torch.empty(B, hq, Sq, dtype=torch.float32, device=q.device) if grad else None
     nbytes = native.require().lb_masked_attn_fwd_ws_bytes(B, Sq, Sk, hq, hkv, d)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    native.call("lb_masked_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), native.ptr(o_lo), lse.data_ptr(), native.ptr(ws), nbytes, B, Sq, Sk, hq, hkv, d,
+    native.call("lb_masked_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), native.ptr(o_lo), native.ptr(lse), native.ptr(ws), nbytes, B, Sq, Sk, hq, hkv, d,
                 _strides(q, k, v), scale, int(causal), softcap, native.ptr(slopes), native.ptr(qb), native.ptr(kb), native.stream_ptr())
     return o, o_lo, lse
 
