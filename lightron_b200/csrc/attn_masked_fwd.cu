@@ -780,7 +780,8 @@ int launch_form(const CUtensorMap* maps, const FwdParams& p, unsigned grid, cuda
   return LB_OK;
 }
 
-// (Without gradients the sum of the unrounded weights is left out: 2 x 4099, cap 30, d 64 124 -> 118 us, 8 x 2048, documents of 300, d 64 133 -> 131.)
+// (Without gradients the sum of the unrounded weights, lse and o_lo are left out: 2 x 4099 both ways, cap 30, 16 heads, d 64 118.7 -> 115.3 us, 8 x 2048, documents of 300, 32 / 4 heads,
+// d 64 137 -> 121.)
 template <int D, int CAP, bool BIAS>
 int launch(const CUtensorMap* maps, const FwdParams& p, unsigned grid, cudaStream_t s) {
   return p.a.o_lo ? launch_form<D, CAP, BIAS, true>(maps, p, grid, s) : launch_form<D, CAP, BIAS, false>(maps, p, grid, s);
