@@ -1085,7 +1085,9 @@ def _norm_table(tensors):
 def _grad_parts(tensors, device):
     """Sums of squares of parts of the tensors: (fp32 buffer, how many)."""
     import ctypes
-    n, ptrs, counts, types = _norm_table([t if _dense(t) else t.contiguous() for t in tensors])
+    # (held until the launch: a copy that went away here would give its memory to the next allocation, which is that of the sums)
+    src = [t if _dense(t) else t.contiguous() for t in tensors]
+    n, ptrs, counts, types = _norm_table(src)
     parts = torch.empty(native.require().lb_grad_norm_parts(n), dtype=torch.float32, device=device)
     filled = ctypes.c_int(0)
     native.call("lb_grad_squares", n, ptrs, counts, types, parts.data_ptr(), parts.numel(), ctypes.byref(filled), native.stream_ptr())

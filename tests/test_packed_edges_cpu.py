@@ -1,0 +1,49 @@
+"""Operators of packed batches where they can go wrong, on the CPU: what a launch is given, positions outside of tables, text for a model with several axes,
+norms of sharded gradients."""
+import gc
+import weakref
+
+import pytest
+import torch
+
+from lightron_b200.ops import functional as OF
+from lightron_b200.ops import native
+from lightron_b200.ops import reference as ref
+
+
+class _Library:
+    """Stands in for the kernels' library."""
+
+    def lb_grad_norm_parts(self, n):
+        return 8
+
+    def lb_masked_attn_fwd_ws_bytes(self, *sizes):
+        return 0
+
+
+def _fake_launches(monkeypatch, call):
+    monkeypatch.setattr(native, "require", lambda: _Library())
+    monkeypatch.setattr(native, "use_native", lambda t: True)
+    monkeypatch.setattr(native, "host_ops", lambda: None)
+    monkeypatch.setattr(native, "on_device", lambda t: native._HERE)
+    monkeypatch.setattr(native, "stream_ptr", lambda: 0)
+    monkeypatch.setattr(native, "call", call)
+
+
+def test_copies_live_until_their_launch(monkeypatch):
+    """A tensor that is not dense is copied for the sum of squares: the copy's address is not handed over without the copy."""
+    copies, alive, contiguous = [], [], torch.Tensor.contiguous
+
+    def copying(t, *a, **kw):
+        c = contiguous(t, *a, **kw)
+        if c is not t:
+            copies.append(weakref.ref(c))
+        return c
+
+    def call(name, *args):
+        gc.collect()
+        alive.append((name, [c() is not None for c in copies]))
+    _fake_launches(monkeypatch, call)
+    monkeypatch.setattr(torch.Tensor, "contiguous", copying)
+    OF._grad_parts([torch.randn(8, 8)[:, 1:5], torch.randn(6), torch.randn(9, 4)[::2]], torch.device("cpu"))
+    assert alive == [("lb_grad_squares", [True, True])]

@@ -1,0 +1,64 @@
+"""Operators of packed batches where they can go wrong: biases that rise with distance, caps near zero, heads in several groups, scores out of range,
+two streams, arguments that are written to, lists that change meanwhile.
+
+Bounds as in the tests of the same kernels beside this file: 5e-3 in the 2-norm for attention (one rounding to bf16 of the result, of P and of dS: 1.7e-3 each, with
+room); 1e-6 for norms.  A bias of up to 4000 in units of log2 rounds exponents by 2^-13 at most, which leaves the bound as it is.
+"""
+import threading
+
+import pytest
+import torch
+
+from packed_oracle import attention64, documents, rel, visible
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def _rand(*shape, scale=1.0, seed=0, dtype=BF16):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda", dtype=torch.float32) * scale).to(dtype)
+
+
+def _status_ok():
+    from lightron_b200.ops import native
+    assert native.device_status() == {}
+
+
+def _run(q, k, v, do, **kw):
+    from lightron_b200.ops import functional as OF
+    q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+    o = OF.masked_attention(q, k, v, **kw)
+    return (o.detach(), *torch.autograd.grad(o, (q, k, v), do))
+
+
+def _see(Sq, Sk, causal):
+    at, key = torch.arange(Sk - Sq, Sk, device="cuda"), torch.arange(Sk, device="cuda")
+    return (key[None, :] <= at[:, None] if causal else torch.ones(Sq, Sk, dtype=torch.bool, device="cuda"))[None]
+
+
+def _close(got, want, bound=5e-3):
+    for name, g, w in zip(("o", "dq", "dk", "dv"), got, want):
+        assert torch.isfinite(g).all(), name
+        assert rel(g, w) < bound, (name, rel(g, w))
+
+
+# ---- norm and clipping ---------------------------------------------------------------------------------
+
+
+def _norm64(ts):
+    return sum(t.double().square().sum() for t in ts).sqrt().item()
+
+
+def test_norm_of_views_that_are_not_dense():
+    """Their copies live until the sums are made: beside lists that take many rounds of the CTAs, and more than one launch."""
+    from lightron_b200.ops import functional as OF
+    base = _rand(120, 90, seed=1, dtype=torch.float32)
+    views = [base[:, 3:77], base[::2], base.t()[5:50, ::3]]
+    large = _rand(60_000_000, seed=2)
+    many = [_rand(40, seed=i) for i in range(800)]
+    for ts in (views, [large] + views, many + views, views + many + [large] + views):
+        want = _norm64(ts)
+        first = OF.grad_norm(ts)
+        assert abs(first.item() / want - 1) < 1e-6
+        assert all(torch.equal(OF.grad_norm(ts), first) for _ in range(3))
