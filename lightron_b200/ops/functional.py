@@ -1038,6 +1038,8 @@ def packed_attention_qkv(qkv: torch.Tensor, cos, sin, positions, B: int, S: int,
         positions, axes = positions[None], (0,) * (d // 2)
     if qkv.dim() != 2 or qkv.shape != (B * S, (hq + 2 * hkv) * d):
         raise ValueError(f"qkv {tuple(qkv.shape)} is not [{B} * {S}, ({hq} + 2 * {hkv}) * {d}]")
+    if cos.device != qkv.device:
+        raise ValueError(f"tables on {cos.device} for qkv on {qkv.device}")
     positions, axes = _check_axes(B, S, d, cos, sin, positions, axes)
     heads = qkv.view(B, S, hq + 2 * hkv, d)
     q, k, v = heads[:, :, :hq], heads[:, :, hq:hq + hkv], heads[:, :, hq + hkv:]

@@ -47,3 +47,17 @@ def test_copies_live_until_their_launch(monkeypatch):
     monkeypatch.setattr(torch.Tensor, "contiguous", copying)
     OF._grad_parts([torch.randn(8, 8)[:, 1:5], torch.randn(6), torch.randn(9, 4)[::2]], torch.device("cpu"))
     assert alive == [("lb_grad_squares", [True, True])]
+
+
+def test_tables_of_another_device_are_refused(monkeypatch):
+    """Tables and positions that do not lie where ``qkv`` does never reach a kernel."""
+    def call(name, *args):
+        raise AssertionError(f"{name} was launched")
+    _fake_launches(monkeypatch, call)
+    qkv, cos, sin = torch.zeros(8, 4 * 8), *ref.rope_tables(8, 16)
+    pos = torch.zeros(1, 8, dtype=torch.int32)
+    for tables in ((cos.to("meta"), sin.to("meta"), pos.to("meta")), (cos, sin, pos.to("meta")), (cos, sin.to("meta"), pos), (cos.to("meta"), sin.to("meta"), pos)):
+        with pytest.raises(ValueError):
+            OF.packed_attention_qkv(qkv, *tables, 1, 8, 2, 1, 8, axes=[0] * 4)
+        with pytest.raises(ValueError):
+            OF.rope_axes(qkv.view(1, 8, 4, 8), *tables, [0] * 4)
