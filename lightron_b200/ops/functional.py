@@ -972,6 +972,8 @@ def _check_axes(B, S, d, cos, sin, positions, axes):
         raise ValueError(f"axes {sorted(set(axes))} of positions with {positions.shape[0]} axes")
     if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != d // 2 or cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise ValueError(f"cos and sin must be fp32 [positions, {d // 2}], got {cos.dtype} {tuple(cos.shape)} and {sin.dtype} {tuple(sin.shape)}")
+    if cos.shape[0] == 0 and positions.numel():
+        raise ValueError("cos and sin have no rows")
     if not cos.device == sin.device == positions.device:
         raise ValueError("cos, sin and positions are on different devices")
     positions = positions.to(torch.int32)

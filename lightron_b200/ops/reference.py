@@ -150,11 +150,12 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bounds: 
 
 
 def rope_axes(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, axes, inverse: bool = False) -> torch.Tensor:
-    """x [B, S, h, d]; pair i turns by the table row ``positions[axes[i]]`` ([A, B, S] or [A, S]) of its token."""
+    """x [B, S, h, d]; pair i turns by the table row ``positions[axes[i]]`` ([A, B, S] or [A, S]) of its token, and is NaN where there is none."""
     axis, pair = torch.as_tensor(axes, device=x.device), torch.arange(x.shape[-1] // 2, device=x.device)
     at = positions.long()[axis]                                                          # [d/2, (B,) S]
     at = (at if at.dim() == 3 else at[:, None]).permute(1, 2, 0)
-    c, s = cos[at, pair][:, :, None], sin[at, pair][:, :, None]
+    away, at = (at < 0) | (at >= cos.shape[0]), at.clamp(0, max(cos.shape[0] - 1, 0))    # (an index outside of the table would be refused, or on a GPU end the process)
+    c, s = (t[at, pair].masked_fill(away, float("nan"))[:, :, None] for t in (cos, sin))
     s = -s if inverse else s
     a, b = x.to(c.dtype)[..., 0::2], x.to(c.dtype)[..., 1::2]
     return torch.stack((a * c - b * s, a * s + b * c), dim=-1).flatten(-2).type_as(x)

@@ -61,3 +61,17 @@ def test_tables_of_another_device_are_refused(monkeypatch):
             OF.packed_attention_qkv(qkv, *tables, 1, 8, 2, 1, 8, axes=[0] * 4)
         with pytest.raises(ValueError):
             OF.rope_axes(qkv.view(1, 8, 4, 8), *tables, [0] * 4)
+
+
+@pytest.mark.parametrize("outside", [16, -1, -16, 1000])
+def test_positions_outside_the_tables(outside):
+    """NaN in the pairs of that axis, values elsewhere, on every path; no access, which on a GPU would end the process."""
+    cos, sin = ref.rope_tables(8, 16)
+    x = torch.randn(1, 3, 2, 8, generator=torch.Generator().manual_seed(0), requires_grad=True)
+    pos = torch.tensor([[0, 15, 3], [0, 15, outside]], dtype=torch.int32)
+    y = OF.rope_axes(x, cos, sin, pos, [0, 1, 0, 1])
+    away = torch.zeros(1, 3, 2, 8, dtype=torch.bool)
+    away[:, 2, :, [2, 3, 6, 7]] = True
+    assert torch.equal(torch.isnan(y), away)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert torch.equal(torch.isnan(dx), away)

@@ -62,3 +62,14 @@ def test_norm_of_views_that_are_not_dense():
         first = OF.grad_norm(ts)
         assert abs(first.item() / want - 1) < 1e-6
         assert all(torch.equal(OF.grad_norm(ts), first) for _ in range(3))
+
+
+def test_rope_axes_outside_the_tables_in_the_form_for_other_types():
+    """fp32, odd head sizes and more than eight axes are rotated by PyTorch operations: NaN there, too, and no access."""
+    from lightron_b200.ops import functional as OF
+    from lightron_b200.ops import reference as ref
+    for d, axes, dtype in ((16, 2, torch.float32), (12, 2, BF16), (32, 9, BF16)):
+        cos, sin = ref.rope_tables(d, 10, device="cuda")
+        pos = torch.tensor([[0, 9, 10, -1]] * axes, device="cuda", dtype=torch.int32)
+        y = OF.rope_axes(_rand(1, 4, 2, d, dtype=dtype), cos, sin, pos, [i % axes for i in range(d // 2)])
+        assert torch.isfinite(y[:, :2]).all() and torch.isnan(y[:, 2:]).all()
