@@ -898,12 +898,13 @@ PyObject* py_rope_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// The list's tensors as the kernels take them: dense in one piece, all on the current device; false: not a plain list
+// The list's tensors as the kernels take them: dense in one piece, all on the current device; false: not a plain list.  They are held: without the interpreter's lock
+// another thread may change the list.
 struct NormList {
   std::vector<P> at;
   std::vector<L> n;
   std::vector<int> type;
-  std::vector<const Tensor*> t;
+  std::vector<Tensor> t;
   bool take(PyObject* list) {
     if (!PyList_CheckExact(list) && !PyTuple_CheckExact(list)) return false;
     const Py_ssize_t k = PySequence_Fast_GET_SIZE(list);
@@ -913,18 +914,18 @@ struct NormList {
       if (!x || !x->defined() || !x->is_cuda() || x->layout() != at::kStrided || !x->is_contiguous() || x->is_neg() || x->_fw_grad(0).defined()) return false;
       const at::ScalarType s = x->scalar_type();
       if (s != at::kBFloat16 && s != at::kHalf && s != at::kFloat) return false;
-      if (i == 0 ? !here(*x) : x->device() != t[0]->device()) return false;
+      if (i == 0 ? !here(*x) : x->device() != t[0].device()) return false;
       at.push_back(x->const_data_ptr());
       n.push_back(x->numel());
       type.push_back(s == at::kBFloat16 ? 0 : s == at::kHalf ? 1 : 2);
-      t.push_back(x);
+      t.push_back(*x);
     }
     return k > 0 && k < INT_MAX;
   }
 };
 // Runs the sums of squares; the parts and how many
 std::pair<Tensor, int> norm_parts(const NormList& l) {
-  Tensor parts = empty_f32({api.lb_grad_norm_parts((int)l.at.size())}, *l.t[0]);
+  Tensor parts = empty_f32({api.lb_grad_norm_parts((int)l.at.size())}, l.t[0]);
   int filled = 0;
   LB_CALL(lb_grad_squares, (int)l.at.size(), l.at.data(), l.n.data(), l.type.data(), parts.mutable_data_ptr(), (int)parts.numel(), &filled, stream());
   return {parts, filled};
@@ -938,7 +939,7 @@ PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return THPVariable_Wrap(unlocked([&] {
     at::NoGradGuard off;
     const std::pair<Tensor, int> p = norm_parts(l);
-    Tensor norm = empty_f32({}, *l.t[0]);
+    Tensor norm = empty_f32({}, l.t[0]);
     LB_CALL(lb_grad_total, p.first.const_data_ptr(), p.second, nullptr, norm.mutable_data_ptr(), stream());
     return norm;
   }));
@@ -957,20 +958,20 @@ PyObject* py_clip_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   if (!(max_norm >= 0.0) || !(eps >= 0.0)) LB_NOT_PLAIN;
   const NormList& to = a[2] == Py_None ? l : o;
-  if (to.at.size() != l.at.size() || to.t[0]->device() != l.t[0]->device()) LB_NOT_PLAIN;
+  if (to.at.size() != l.at.size() || to.t[0].device() != l.t[0].device()) LB_NOT_PLAIN;
   for (size_t i = 0; i < l.at.size(); i++) {
-    if (to.type[i] != l.type[i] || !to.t[i]->sizes().equals(l.t[i]->sizes())) LB_NOT_PLAIN;
-    if (to.t[i]->requires_grad() && at::GradMode::is_enabled()) LB_NOT_PLAIN;
+    if (to.type[i] != l.type[i] || !to.t[i].sizes().equals(l.t[i].sizes())) LB_NOT_PLAIN;
+    if (to.t[i].requires_grad() && at::GradMode::is_enabled()) LB_NOT_PLAIN;
   }
   return THPVariable_Wrap(unlocked([&] {
     at::NoGradGuard off;
     const std::pair<Tensor, int> p = norm_parts(l);
-    Tensor norm = empty_f32({}, *l.t[0]);
+    Tensor norm = empty_f32({}, l.t[0]);
     std::vector<W> dst;
     dst.reserve(to.at.size());
-    for (const Tensor* t : to.t) {
-      dst.push_back(t->mutable_data_ptr());
-      t->unsafeGetTensorImpl()->bump_version();
+    for (const Tensor& t : to.t) {
+      dst.push_back(t.mutable_data_ptr());
+      t.unsafeGetTensorImpl()->bump_version();
     }
     LB_CALL(lb_grad_scale, (int)l.at.size(), l.at.data(), dst.data(), l.n.data(), l.type.data(), p.first.const_data_ptr(), p.second, (float)max_norm, (float)eps, norm.mutable_data_ptr(),
             stream());

@@ -73,3 +73,25 @@ def test_rope_axes_outside_the_tables_in_the_form_for_other_types():
         pos = torch.tensor([[0, 9, 10, -1]] * axes, device="cuda", dtype=torch.int32)
         y = OF.rope_axes(_rand(1, 4, 2, d, dtype=dtype), cos, sin, pos, [i % axes for i in range(d // 2)])
         assert torch.isfinite(y[:, :2]).all() and torch.isnan(y[:, 2:]).all()
+
+
+def test_list_that_changes_meanwhile():
+    """Another thread empties and refills the list while it is clipped: each call sees one whole list."""
+    from lightron_b200.ops import functional as OF
+    grads = [torch.ones(100 + i, device="cuda") for i in range(60)]
+    total = sum(t.numel() for t in grads) ** 0.5
+    box, stop = list(grads), threading.Event()
+
+    def turn():
+        while not stop.is_set():
+            box[:] = [t.clone() for t in grads]
+    side = threading.Thread(target=turn)
+    side.start()
+    try:
+        for _ in range(300):
+            assert abs(OF.grad_norm(box).item() / total - 1) < 1e-6
+            assert abs(OF.clip_grad_norm(box, 1e9).item() / total - 1) < 1e-6
+    finally:
+        stop.set()
+        side.join()
+    torch.cuda.synchronize()
