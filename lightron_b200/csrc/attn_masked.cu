@@ -138,11 +138,13 @@ extern "C" int lb_attn_mask(const void* ids, int id_bytes, const void* marks, co
   cudaStream_t s = (cudaStream_t)stream;
   if (S > MAX_MASK_LENGTH) return LB_ERR_SHAPE;
   const int smem = (S + 31) / 32 * 20;
-  static bool attr = false;
-  if (!attr) {
+  static MaOnce once;
+  bool* const set = once.here();
+  if (!set) return LB_ERR_LAUNCH;
+  if (!*set) {
     cudaFuncSetAttribute(attn_mask_kernel<int>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_MASK_LENGTH / 32 * 20);
     cudaFuncSetAttribute(attn_mask_kernel<long long>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_MASK_LENGTH / 32 * 20);
-    attr = true;
+    *set = true;
   }
   // four positions a thread, where the sequences leave room for as many CTAs
   const int most = (S + 4 * PLAN_THREADS - 1) / (4 * PLAN_THREADS), room = lb_num_sms() / B;

@@ -32,6 +32,15 @@ struct MaBwdParams {
   float* stats;
 };
 
+// A kernel's attributes count on the device where they were set: the flag of the current one (null: none, or not among the first 64).
+struct MaOnce {
+  bool done[64] = {false};
+  bool* here() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? done + dev : nullptr;
+  }
+};
+
 int ma_launch_fwd(const MaParams& p, void* ws, long long ws_bytes, cudaStream_t s);
 long long ma_fwd_ws_bytes(const MaParams& p);
 int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s);

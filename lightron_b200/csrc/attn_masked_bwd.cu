@@ -705,13 +705,15 @@ template <int D, int FORM, bool CAP, bool BIAS>
 int launch(const CUtensorMap* m, const BwdParams& p, unsigned grid, cudaStream_t s) {
   using C = Cfg<D>;
   auto fn = ma_bwd_kernel<D, FORM, CAP, BIAS>;
-  static bool attr = false;
-  if (!attr) {
+  static MaOnce once;
+  bool* const set = once.here();
+  if (!set) return LB_ERR_LAUNCH;
+  if (!*set) {
     // the register split must fit in what the launch allocates, or it would wait for registers that nobody gives back
     cudaFuncAttributes fa;
     if (cudaFuncGetAttributes(&fa, fn) != cudaSuccess || (fa.numRegs + 7) / 8 * 8 != 128) return LB_ERR_LAUNCH;
     cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    attr = true;
+    *set = true;
   }
   return lb_launch(fn, grid, C::NTHREADS, C::SMEM, s, m[0], m[1], m[2], m[3], m[4], m[5], p);
 }

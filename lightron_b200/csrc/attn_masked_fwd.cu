@@ -764,13 +764,15 @@ template <int D, int CAP, bool BIAS, bool GRAD>
 int launch_form(const CUtensorMap* maps, const FwdParams& p, unsigned grid, cudaStream_t s) {
   using C = Cfg<D>;
   auto fn = ma_fwd_kernel<D, CAP, BIAS, GRAD>;
-  static bool attr = false;
-  if (!attr) {
+  static MaOnce once;
+  bool* const set = once.here();
+  if (!set) return LB_ERR_LAUNCH;
+  if (!*set) {
     // the register split must fit in what the launch allocates, or it would wait for registers that nobody gives back
     cudaFuncAttributes fa;
     if (cudaFuncGetAttributes(&fa, fn) != cudaSuccess || (fa.numRegs + 7) / 8 * 8 < REGS_LAUNCH) return LB_ERR_LAUNCH;
     cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    attr = true;
+    *set = true;
   }
   LB_LAUNCH(fn, grid, THREADS, C::SMEM, s, maps[0], maps[1], maps[2], maps[3], maps[4], p);
   if (p.splits > 1) {

@@ -95,3 +95,14 @@ def test_list_that_changes_meanwhile():
         stop.set()
         side.join()
     torch.cuda.synchronize()
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs in one process")
+def test_second_device_of_a_process():
+    from lightron_b200.ops import functional as OF
+    outs = []
+    for dev in ("cuda:0", "cuda:1"):
+        q, k, v, do = (_rand(2, 700, 4, 64, seed=i).to(dev) for i in range(4))
+        ids = documents(2, 700, 150, seed=1).to(dev)
+        outs.append([t.cpu() for t in _run(q, k, v, do, mask=OF.attention_mask(documents=ids), softcap=20.0)])
+    assert all(torch.equal(outs[0][i], outs[1][i]) for i in (0, 2, 3))
