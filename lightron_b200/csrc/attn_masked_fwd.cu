@@ -17,6 +17,9 @@
 //     distance made per column.  Without a cap the exponentials' reference is a bound, not the maximum itself: what they are relative to cancels, as long as it is within 2^60
 //     or so of the maximum.  The nearest key blocks come first, or the maximum would grow from block to block and O be rescaled in each (both together: 1 x 8192, 32 / 8 heads,
 //     d 128 780 -> 632 us, 8 x 2048, 32 / 4 heads, d 64 303 -> 287).
+//   * slopes below zero, whose scores rise with distance, are told apart on the device, by head: the bound takes the largest distance, and what exponentials under a cap are
+//     relative to is the bias at the row's farthest key instead of zero.  (For all biased forms under a cap 0 to 3 %: 1 x 4096, 32 / 8 heads, d 128, cap 50 210 -> 216 us, without
+//     gradients 177 -> 178, 4 x 2048, 32 / 4 heads, d 64 191 -> 193; without a cap nothing.)
 //   * o is divided by the sum of the weights as they are rounded for P V.  A row that all but one key leave cold has o = v of that key then, and a D = do . o whose
 //     error is as small as the differences dP - D that the backward lives on (the weight's own rounding, 2^-9 of dP, would drown them); lse is of the sum of the
 //     unrounded ones, from which the backward's P are made.
@@ -74,9 +77,9 @@ struct Cfg {
 static_assert(Cfg<64>::SMEM <= 115712 && Cfg<128>::SMEM <= 115712, "two CTAs per SM");
 
 // 64 raw scores to units of log2, capped and lowered with distance.  `first`: key of column 0 less the row's position; `side`: the columns lie on the row's left (1),
-// on its right (-1) or on both sides (0), the same for all lanes.
+// on its right (-1) or on both sides (0), the same for all lanes; `at`: what the row's exponentials are relative to, taken off with the bias.
 template <int CAP, bool BIAS>
-__device__ __forceinline__ void scores64(uint32_t* r, const FwdParams& p, float slope2, int side, int first) {
+__device__ __forceinline__ void scores64(uint32_t* r, const FwdParams& p, float slope2, int side, int first, float at) {
   bool small = true;
   if constexpr (CAP != NO_CAP) {
     float top[4] = {0.f, 0.f, 0.f, 0.f};
@@ -90,8 +93,8 @@ __device__ __forceinline__ void scores64(uint32_t* r, const FwdParams& p, float 
 #pragma unroll
   for (int c0 = 0; c0 < 64; c0 += 32) {
     // (counted up anew every 32 columns: its rounding errors do not pile up)
-    const float base = slope * (float)(first + c0);
-    f32x2 add = BIAS && side ? pack2(base, base + slope) : pack2(0.f, 0.f);
+    const float base = fmaf(slope, (float)(first + c0), -at);
+    f32x2 add = !BIAS ? pack2(0.f, 0.f) : side ? pack2(base, base + slope) : pack2(-at, -at);
     if (CAP == NO_CAP || small) {
 #pragma unroll
       for (int i = c0; i < c0 + 32; i += 2) {
@@ -464,7 +467,11 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       }
       if (lane == 0) bulk_wait_read_but<0>();      // the last tile's O has left the place of the meetings
       __syncwarp();
-      float m_i = -INFINITY, m_s = 0.f, l_i = 0.f, lp_i = 0.f;      // the row's running maximum, what exponentials are relative to, this thread's sums of them
+      [[maybe_unused]] float top = 0.f;
+      // (a slope below zero lifts scores over the cap, up to its value at the farthest key that the row sees: exponentials are relative to that, and one of them is 2^-80 or more)
+      if constexpr (BIAS && CAP == CAP_ZERO)
+        if (slope2 < 0.f && row < p.Sq) top = -slope2 * (float)max(max(row + off - see.x, see.y - 1 - (row + off)), 0);
+      float m_i = -INFINITY, m_s = top, l_i = 0.f, lp_i = 0.f;      // the row's running maximum, what exponentials are relative to, this thread's sums of them
       for (int j = 0; j < nb; j++, g++) {
         if (!s_ready && !mbar_wait(s_full_of(set), g & 1u, abort_flag)) { ok = false; break; }
         fence_after();
@@ -478,7 +485,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         const bool pv_ready = !C::P_ALIAS && j > 0 && mbar_test_wait(pv_done, (g - 1) & 1u);   // asked ahead of its use
         if constexpr (MADE) {
           const int side = left_only || c0 + 63 <= warp_at ? 1 : c0 >= warp_at + 31 ? -1 : 0;
-          scores64<CAP, BIAS>(r, pp, slope2, side, c0 - (row + off));
+          scores64<CAP, BIAS>(r, pp, slope2, side, c0 - (row + off), top);
         }
         if (need_mask) {
 #pragma unroll
@@ -508,20 +515,20 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           float mx4[4] = {from, from, from, from};       // four independent chains
           float m_new = m_i;
           if constexpr (LINEAR) {
-            // A bound instead of the maximum: of 32 columns the largest score with the smallest distance, at most 31 slopes above it.  (Where that is more than 2^60 the
-            // biased scores are looked at one by one.)
+            // A bound instead of the maximum: of 32 columns the largest score with the smallest distance (with the largest where the slope is below zero and scores rise with
+            // it), at most 31 slopes above it.  (Where that is more than 2^60 the biased scores are looked at one by one.)
 #pragma unroll
             for (int w = 0; w < 64; w += 32) {
               const int to_left = row + off - (c0 + w + 31), to_right = c0 + w - (row + off);
-              const float steep = fabsf(slope);
+              const float steep = fabsf(slope), rise = slope2 < 0.f ? steep : -steep;      // (0 where the bias is in r)
               if (steep <= 60.f / 31.f) {
                 float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int i = w; i < w + 32; i += 2) top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-                m_new = max2(m_new, fmaf(max2(top[0], top[1]), pp.f.scale1, -steep * (float)max(max(to_left, to_right), 0)));
+                m_new = max2(m_new, fmaf(max2(top[0], top[1]), pp.f.scale1, rise * (float)(slope2 < 0.f ? max(to_left, to_right) + 31 : max(max(to_left, to_right), 0))));
               } else {
 #pragma unroll
-                for (int i = w; i < w + 32; i++) m_new = max2(m_new, fmaf(__uint_as_float(r[i]), pp.f.scale1, -steep * fabsf((float)(to_right + (i - w)))));
+                for (int i = w; i < w + 32; i++) m_new = max2(m_new, fmaf(__uint_as_float(r[i]), pp.f.scale1, rise * fabsf((float)(to_right + (i - w)))));
               }
             }
           } else {

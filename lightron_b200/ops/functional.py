@@ -911,7 +911,7 @@ def _check_masked_native(d: int) -> None:
 def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[AttentionMask] = None, causal: Optional[bool] = None,
                      scale: Optional[float] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
     """softmax(s) v for q [B, Sq, hq, d] and k, v [B, Sk, hkv, d] in any order of the outer dimensions; query i sits at position i + Sk - Sq.
-    ``s = softcap * tanh(x / softcap) - slopes[h] * |distance|`` with ``x = scale * q.k`` (``softcap`` 0: x itself; ``slopes`` fp32 [hq], constants).
+    ``s = softcap * tanh(x / softcap) - slopes[h] * |distance|`` with ``x = scale * q.k`` (``softcap`` 0: x itself; ``slopes`` fp32 [hq], constants of either sign).
     ``mask``: see :func:`attention_mask`; without one, ``causal`` (default) or all keys.  Rows that see nothing give zeros, and gradients of zero."""
     if (host := native.host_ops()) is not None and (mask is None or (type(mask) is AttentionMask and causal in (None, mask.causal))):
         qb, kb, one_way = (None, None, causal is None or causal) if mask is None else (mask.q_bounds, mask.k_bounds, mask.causal)

@@ -106,3 +106,40 @@ def test_second_device_of_a_process():
         ids = documents(2, 700, 150, seed=1).to(dev)
         outs.append([t.cpu() for t in _run(q, k, v, do, mask=OF.attention_mask(documents=ids), softcap=20.0)])
     assert all(torch.equal(outs[0][i], outs[1][i]) for i in (0, 2, 3))
+
+
+# ---- slopes below zero ------------------------------------------------------------------------------
+
+
+RISING = [-0.01, -0.3, -1.3, -1.4, -5.0, 0.25]
+
+
+@pytest.mark.parametrize("cap", [0.0, 20.0, 200.0])
+@pytest.mark.parametrize("Sq,Sk,d,causal,docs,prefix", [
+    (300, 300, 64, True, 0, False),
+    (500, 500, 128, False, 0, False),
+    (700, 700, 96, True, 0, False),
+    (640, 640, 64, True, 200, True),          # documents with prefixes, padding
+    (100, 400, 128, True, 0, False),          # the last queries of a longer sequence
+    (1, 2300, 64, True, 0, False),            # split over keys
+    (70, 1100, 128, False, 400, False),
+])
+def test_slopes_below_zero(Sq, Sk, d, causal, docs, prefix, cap):
+    """Scores that rise with distance: the formula holds for every sign."""
+    from lightron_b200.ops import functional as OF
+    hq, hkv = 6, 2
+    q, k, v, do = _rand(1, Sq, hq, d, scale=4.0, seed=1), _rand(1, Sk, hkv, d, seed=2), _rand(1, Sk, hkv, d, seed=3), _rand(1, Sq, hq, d, seed=4)
+    mask, see = None, _see(Sq, Sk, causal)
+    if docs:
+        ids = documents(1, Sk, docs, seed=7)
+        marks = torch.rand(1, Sk, generator=torch.Generator().manual_seed(7)) < 0.95 if prefix else None
+        mask = OF.attention_mask(documents=ids.cuda(), prefix=None if marks is None else marks.cuda(), causal=causal)
+        see = visible(1, Sq, Sk, causal, ids, marks)
+    slopes = torch.tensor(RISING, device="cuda")
+    got = _run(q, k, v, do, mask=mask, causal=causal, softcap=cap, slopes=slopes)
+    with torch.no_grad():
+        alone = OF.masked_attention(q, k, v, mask=mask, causal=causal, softcap=cap, slopes=slopes)
+    _status_ok()
+    want = attention64(q, k, v, see, d ** -0.5, cap, slopes, do)
+    _close(got, want)
+    assert rel(alone, want[0]) < 5e-3
