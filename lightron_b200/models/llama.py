@@ -263,6 +263,8 @@ class LightronTransformer(nn.Module):
         cos, sin = self.rope_tables(h.device)
         if positions is not None and h.is_cuda:
             positions = positions.to(device=h.device, dtype=torch.int32)
+        if self.args.rope_sections is not None and positions is not None and positions.dim() == 2 and positions.shape[0] == B:
+            positions = positions.expand(len(self.args.rope_sections), -1, -1)      # [B, S]: text, which counts on all axes together
         plain = mask is None and (positions is None or positions.dim() == 1)
         if plain and not torch.is_grad_enabled() and (host := native.host_ops()) is not None and (run := _plain_layers(self.layers)) is not None:
             if (out := host.decoder_layers(h, delta, cos, sin, positions, B, S, *run)) is not NotImplemented:
@@ -321,7 +323,8 @@ class LightronTransformer(nn.Module):
     def loss(self, tokens: torch.Tensor, targets: torch.Tensor, positions=None,
              n_tokens: Optional[int] = None, mask=None) -> torch.Tensor:
         """Token-mean next-token NLL (+ MoE aux loss) without materialising gathered logits.  Packed batches: ``mask`` of
-        ``ops.functional.attention_mask``, ``positions`` [B, S], or [axes, B, S] with ``rope_sections``, and ``n_tokens``, the number of targets that are not -100."""
+        ``ops.functional.attention_mask``, ``positions`` [B, S], and ``n_tokens``, the number of targets that are not -100.  With ``rope_sections`` ``positions`` may be
+        [axes, B, S], or [axes, S] where there are not as many sequences as axes; None, [S] and [B, S] are text, which counts on all axes together."""
         B, S = tokens.shape
         logits = self.forward_stage(tokens, B, S, positions, mask)
         loss = self.loss_from_logits(logits, targets, n_tokens)

@@ -1033,11 +1033,15 @@ class _PackedAttnQKV(torch.autograd.Function):
 def packed_attention_qkv(qkv: torch.Tensor, cos, sin, positions, B: int, S: int, hq: int, hkv: int, d: int, axes: Optional[Sequence[int]] = None,
                          mask: Optional[AttentionMask] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`rope_attention_qkv` for packed batches: qkv [B*S, (hq+2hkv)*d] -> [B*S, hq*d] by :func:`rope_axes` on q and k and :func:`masked_attention`.
-    ``positions``: None (each token's place), [S], [B, S] (as of documents that count from zero) or, with ``axes``, [A, B, S] or [A, S]."""
+    ``positions``: None (each token's place), [S], [B, S] (as of documents that count from zero).  With ``axes``: None or [S], which count on all axes together as text
+    does, [A, B, S] or [A, S] (two dimensions are axes and tokens then, never sequences and tokens)."""
     if positions is None:
         positions = torch.arange(S, device=qkv.device, dtype=torch.int32)
     if axes is None:
         positions, axes = positions[None], (0,) * (d // 2)
+    elif positions.dim() == 1:
+        axes = tuple(axes)
+        positions = positions.expand(max(axes, default=0) + 1, -1)
     if qkv.dim() != 2 or qkv.shape != (B * S, (hq + 2 * hkv) * d):
         raise ValueError(f"qkv {tuple(qkv.shape)} is not [{B} * {S}, ({hq} + 2 * {hkv}) * {d}]")
     if cos.device != qkv.device:

@@ -75,3 +75,57 @@ def test_positions_outside_the_tables(outside):
     assert torch.equal(torch.isnan(y), away)
     dx, = torch.autograd.grad(y, x, torch.ones_like(y))
     assert torch.equal(torch.isnan(dx), away)
+
+
+# ---- a model whose rotary positions have several axes, on plain text ---------------------------------
+
+
+def _model(**kw):
+    from lightron_b200 import mesh
+    from lightron_b200.config import ModelArgs
+    from lightron_b200.models import LightronTransformer, init_weights
+    mesh.set_context(None)
+    model = LightronTransformer(ModelArgs(dim=32, n_layers=2, n_heads=4, n_kv_heads=2, vocab_size=64, intermediate_size=48, max_seq_len=64, **kw),
+                                dtype=torch.float32, device="cpu")
+    init_weights(model, 0, std=0.2)
+    return model
+
+
+@pytest.mark.parametrize("B", [1, 2, 3, 4])
+def test_text_counts_on_all_axes(B):
+    """Without positions, with [S] and with [B, S] (three sequences as well as three axes): the ordinary rotation."""
+    plain, axes = _model(), _model(rope_sections=(2, 1, 1))
+    tokens = torch.randint(0, 64, (B, 9), generator=torch.Generator().manual_seed(0))
+    own = torch.stack([torch.arange(9) + 3 * b for b in range(B)])
+    for pos in (None, torch.arange(9), torch.arange(5, 14), own):
+        want = plain(tokens, positions=pos)
+        assert torch.allclose(axes(tokens, positions=pos), want, atol=1e-5)
+    three = own.expand(3, B, 9)
+    assert torch.allclose(axes(tokens, positions=three), plain(tokens, positions=own), atol=1e-5)
+    loss = axes.loss(tokens, tokens)
+    loss.backward()
+    assert torch.isfinite(loss)
+
+
+def test_packed_attention_without_positions():
+    B, S, hq, hkv, d = 2, 5, 2, 1, 8
+    cos, sin = ref.rope_tables(d, 16)
+    qkv = torch.randn(B * S, (hq + 2 * hkv) * d, generator=torch.Generator().manual_seed(0))
+    want = OF.packed_attention_qkv(qkv, cos, sin, None, B, S, hq, hkv, d)
+    for pos in (None, torch.arange(S), torch.arange(S).expand(3, S), torch.arange(S).expand(3, B, S)):
+        assert torch.equal(OF.packed_attention_qkv(qkv, cos, sin, pos, B, S, hq, hkv, d, axes=[0, 1, 2, 2]), want)
+
+
+def test_trainer_takes_rope_sections():
+    """The key of the configuration, through the trainer's own data: the losses of one axis."""
+    from lightron_b200 import mesh
+    from lightron_b200.config import parse_config
+    from lightron_b200.trainer import Trainer
+    losses = []
+    for model in ({}, {"rope_sections": [2, 4, 2]}):
+        mesh.set_context(None)
+        trainer = Trainer(parse_config({"distributed": {}, "model": {"name": "tiny", "dim": 64, "n_heads": 4, "n_kv_heads": 2, **model}, "dataset": {"name": "synthetic"},
+                                        "training": {"micro_batch_size": 4, "gradient_accumulation_steps": 1, "seq_length": 64, "learning_rate": 3e-4, "total_steps": 2, "seed": 0,
+                                                     "dtype": "fp32", "log_interval": 1000}}, env={}))
+        losses.append([float(trainer.train_step()) for _ in range(2)])
+    assert losses[1] == pytest.approx(losses[0], rel=1e-5)

@@ -143,3 +143,22 @@ def test_slopes_below_zero(Sq, Sk, d, causal, docs, prefix, cap):
     want = attention64(q, k, v, see, d ** -0.5, cap, slopes, do)
     _close(got, want)
     assert rel(alone, want[0]) < 5e-3
+
+
+def test_text_counts_on_all_axes():
+    """Positions of one dimension, or none, on several axes: the bits of the same positions written out for each."""
+    from lightron_b200.ops import functional as OF
+    from lightron_b200.ops import reference as ref
+    B, S, hq, hkv, d = 2, 150, 4, 2, 64
+    qkv, do = _rand(B * S, (hq + 2 * hkv) * d, seed=1), _rand(B * S, hq * d, seed=2)
+    cos, sin = ref.rope_tables(d, 200, device="cuda")
+    axes = [0] * 10 + [1] * 11 + [2] * 11
+
+    def both(pos, **kw):
+        x = qkv.clone().requires_grad_()
+        o = OF.packed_attention_qkv(x * 1, cos, sin, pos, B, S, hq, hkv, d, **kw)
+        return o.detach(), torch.autograd.grad(o, x, do)[0]
+    text = torch.arange(S, device="cuda", dtype=torch.int32)
+    want = both(text.expand(3, B, S).contiguous(), axes=axes)
+    for got in (both(None, axes=axes), both(text, axes=axes), both(text.long(), axes=axes), both(text.expand(3, S), axes=axes), both(None)):
+        assert torch.equal(got[0], want[0]) and rel(got[1], want[1]) < 2e-3         # (dq is added up as key tiles come)
