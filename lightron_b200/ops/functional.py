@@ -1011,8 +1011,10 @@ class _PackedAttnQKV(torch.autograd.Function):
         qk, q, k, v = _PackedAttnQKV._views(qkv, *dims)
         with native.on_device(qkv):
             _rope_axes_native(qk, qk, cos, sin, positions, axes, False)
+            torch.autograd.graph.increment_version(qkv)
             o, o_lo, lse = masked_fwd_native(q, k, v, causal, scale, softcap, slopes, qb, kb, not isinstance(ctx, _NoGradCtx) and ctx.needs_input_grad[0])
-        ctx.save_for_backward(qkv, o, o_lo, lse, cos, sin, positions, slopes, qb, kb)
+        # (detached: the version still counts, but nobody asks how a view that was written to was made)
+        ctx.save_for_backward(qkv.detach(), o, o_lo, lse, cos, sin, positions, slopes, qb, kb)
         ctx.args = (axes, dims, causal, scale, softcap)
         return o.view(qkv.shape[0], -1)
 
@@ -1034,7 +1036,8 @@ def packed_attention_qkv(qkv: torch.Tensor, cos, sin, positions, B: int, S: int,
                          mask: Optional[AttentionMask] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`rope_attention_qkv` for packed batches: qkv [B*S, (hq+2hkv)*d] -> [B*S, hq*d] by :func:`rope_axes` on q and k and :func:`masked_attention`.
     ``positions``: None (each token's place), [S], [B, S] (as of documents that count from zero).  With ``axes``: None or [S], which count on all axes together as text
-    does, [A, B, S] or [A, S] (two dimensions are axes and tokens then, never sequences and tokens)."""
+    does, [A, B, S] or [A, S] (two dimensions are axes and tokens then, never sequences and tokens).  On the GPU the caller hands ``qkv`` over: q and k are rotated where
+    they lie (its version counts up); only a leaf that requires a gradient, or one whose memory does not suit the kernels, is copied first and stays as it was."""
     if positions is None:
         positions = torch.arange(S, device=qkv.device, dtype=torch.int32)
     if axes is None:
@@ -1052,7 +1055,7 @@ def packed_attention_qkv(qkv: torch.Tensor, cos, sin, positions, B: int, S: int,
     causal = _check_masked(q, k, v, mask, None, None, softcap, slopes)
     if native.use_native(qkv) and qkv.numel() and positions.shape[0] <= 8:
         _check_masked_native(d)
-        if not qkv.is_contiguous() or qkv.data_ptr() % 16:
+        if not qkv.is_contiguous() or qkv.data_ptr() % 16 or (qkv.requires_grad and qkv.is_leaf):
             qkv = qkv.clone(memory_format=torch.contiguous_format)
         qb, kb = (mask.q_bounds, mask.k_bounds) if mask is not None else (None, None)
         return _apply(_PackedAttnQKV, qkv, cos.contiguous(), sin.contiguous(), positions, None if slopes is None else slopes.contiguous(), qb, kb, axes, (B, S, hq, hkv, d), causal,

@@ -162,3 +162,43 @@ def test_text_counts_on_all_axes():
     want = both(text.expand(3, B, S).contiguous(), axes=axes)
     for got in (both(None, axes=axes), both(text, axes=axes), both(text.long(), axes=axes), both(text.expand(3, S), axes=axes), both(None)):
         assert torch.equal(got[0], want[0]) and rel(got[1], want[1]) < 2e-3         # (dq is added up as key tiles come)
+
+
+# ---- packed_attention_qkv writes to its argument -----------------------------------------------------
+
+
+def _packed(B=1, S=40, hq=2, hkv=1, d=64):
+    from lightron_b200.ops import functional as OF
+    from lightron_b200.ops import reference as ref
+    cos, sin = ref.rope_tables(d, 64, device="cuda")
+    return _rand(B * S, (hq + 2 * hkv) * d, seed=1), lambda t: OF.packed_attention_qkv(t, cos, sin, None, B, S, hq, hkv, d)
+
+
+def test_packed_attention_counts_its_writing():
+    """The rotation of q and k inside the argument is seen by whoever has saved it; a leaf that asks for a gradient is not written to."""
+    qkv, call = _packed()
+    x = qkv.clone()
+    before = x._version
+    call(x)
+    assert x._version > before
+    w = qkv.clone().requires_grad_()
+    y = w * 1
+    z = y * y                                                     # saves y
+    call(y)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+    leaf = qkv.clone().requires_grad_()
+    first = call(leaf)
+    assert torch.equal(leaf, qkv) and torch.equal(call(leaf), first)
+    grad, = torch.autograd.grad(first.float().sum(), leaf)
+    other = qkv.clone().requires_grad_()
+    assert torch.equal(grad[:, 3 * 64:], torch.autograd.grad(call(other * 1).float().sum(), other)[0][:, 3 * 64:])      # dv: the same bits
+
+
+def test_packed_attention_without_gradients():
+    qkv, call = _packed()
+    want = call(qkv.clone())
+    with torch.no_grad():
+        assert torch.equal(call(qkv.clone()), want)
+    with torch.inference_mode():
+        assert torch.equal(call(qkv.clone()), want)
