@@ -184,10 +184,11 @@ def _wrap(module: nn.Module, unit: _ShardedUnit, checkpoint: bool) -> None:
 def apply_fsdp2(model: nn.Module, ctx: Optional[_mesh.ParallelContext] = None, param_dtype: Optional[torch.dtype] = None,
                 reduce_dtype: torch.dtype = torch.float32, reshard_after_forward: bool = True,
                 activation_checkpointing: bool = False) -> nn.Module:
-    """Shard every transformer block, then the remaining (root) parameters, over the DP group.
+    """Shard every transformer block, then the remaining (root) parameters, over the ranks that hold the same parameters: the DP group, with context
+    parallelism the DP x CP group (CP ranks see other tokens of the same sequences, and their gradients are averaged, too).
     Optimise ``model._fsdp.parameters()`` (fp32 master shards)."""
     ctx = ctx or getattr(model, "ctx", None) or _mesh.get_context()
-    group = ctx.dp_group
+    group = ctx.dp_group if ctx.cp_size == 1 else ctx.dpcp_group
     state = FSDPState()
     seen = set()
     param_dtype = param_dtype or next(model.parameters()).dtype

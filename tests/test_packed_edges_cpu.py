@@ -129,3 +129,54 @@ def test_trainer_takes_rope_sections():
                                                      "dtype": "fp32", "log_interval": 1000}}, env={}))
         losses.append([float(trainer.train_step()) for _ in range(2)])
     assert losses[1] == pytest.approx(losses[0], rel=1e-5)
+
+
+# ---- the sharded engine over library collectives -------------------------------------------------------
+
+
+def _engine(dist_kw, clip):
+    return {"distributed": dist_kw, "model": {"name": "tiny"}, "dataset": {"name": "synthetic"},
+            "training": {"micro_batch_size": 4, "gradient_accumulation_steps": 1, "seq_length": 64, "learning_rate": 3e-4, "total_steps": 4, "seed": 0, "dtype": "fp32",
+                         "log_interval": 1000, "grad_clip": clip}}
+
+
+def _engine_steps(raw, steps=3):
+    """(losses, norms before clipping, replicated parameters after the steps)"""
+    from lightron_b200.config import parse_config
+    from lightron_b200.trainer import Trainer
+    trainer = Trainer(parse_config(raw, env={}))
+    losses, norms = [], []
+    for _ in range(steps):
+        losses.append(float(trainer.train_step()))
+        norms.append(float(trainer.optimizer.last_grad_norm) if raw["training"]["grad_clip"] else 0.0)
+    state = trainer.net._fsdp.full_state_dict() if hasattr(trainer.net, "_fsdp") else trainer.net.state_dict()
+    return losses, norms, {k: v.float().numpy().copy() for k, v in state.items() if v.dim() == 1}
+
+
+def _engine_worker(rank, world, raw):
+    return _engine_steps(raw)
+
+
+def _against_one_process(dist_kw, world, clip, norm_bound=2e-5):
+    from dist_utils import run_distributed
+    from lightron_b200 import mesh
+    mesh.set_context(None)
+    one = _engine({}, clip)
+    one["training"]["gradient_accumulation_steps"] = dist_kw.get("dp_size", 1)      # one process sees the whole batch
+    losses, norms, params = _engine_steps(one)
+    mesh.set_context(None)
+    ranks = run_distributed(_engine_worker, world, _engine({"fsdp": True, **dist_kw}, clip))
+    for i in range(3):
+        mean = sum(r[0][i] for r in ranks) / world
+        assert abs(mean - losses[i]) < 2e-4 * losses[i]
+        for r in ranks:
+            assert abs(r[1][i] - norms[i]) <= norm_bound * norms[i], (r[1], norms)
+    for r in ranks:
+        for k, v in params.items():
+            assert abs(r[2][k] - ranks[0][2][k]).max() == 0, k                     # every rank holds the same
+            assert abs(r[2][k] - v).max() < 1e-4, k                                # (a step of AdamW is 3e-4)
+
+
+def test_sharded_engine_with_context_parallelism():
+    """Ranks of a sequence's parts hold the same parameters: gradients are averaged over them, and count once in the norm."""
+    _against_one_process({"cp_size": 2}, 2, 0.5)
