@@ -38,7 +38,9 @@ _ALIGN = 128
 
 class _ShardedUnit:
     def __init__(self, name: str, params: List[nn.Parameter], names: List[str], group, param_dtype, reduce_dtype,
-                 reshard_after_forward: bool, keep_resident: bool = False):
+                 reshard_after_forward: bool, keep_resident: bool = False, partial_group=None):
+        """``partial_group``: TP group whose ranks each have a part of the gradients of vectors (norm weights under sequence parallelism)."""
+        self.partial_group = partial_group
         self.name, self.params, self.names, self.group = name, params, names, group
         self.keep_resident = keep_resident      # root unit: used outside module calls, never freed
         self.n, self.rank = comm.group_size(group), comm.group_rank(group)
@@ -108,6 +110,12 @@ class _ShardedUnit:
             if p.grad is not None:
                 flat[off:off + p.numel()].copy_(p.grad.reshape(-1))
                 p.grad = None
+        if self.partial_group is not None:
+            parts = [flat[off:off + p.numel()] for p, off in zip(self.params, self.offsets) if p.dim() == 1]
+            if parts:
+                buf = torch.cat(parts)
+                dist.all_reduce(buf, group=self.partial_group)
+                torch._foreach_copy_(parts, list(buf.split([t.numel() for t in parts])))
         if self.n > 1:
             g = comm.reduce_scatter_rows(flat.view(self.n, self.shard_len), self.group).view(-1) / self.n
         else:
@@ -189,6 +197,7 @@ def apply_fsdp2(model: nn.Module, ctx: Optional[_mesh.ParallelContext] = None, p
     Optimise ``model._fsdp.parameters()`` (fp32 master shards)."""
     ctx = ctx or getattr(model, "ctx", None) or _mesh.get_context()
     group = ctx.dp_group if ctx.cp_size == 1 else ctx.dpcp_group
+    partial = ctx.tp_group if ctx.tp_size > 1 and getattr(getattr(model, "args", None), "sequence_parallel", False) else None
     state = FSDPState()
     seen = set()
     param_dtype = param_dtype or next(model.parameters()).dtype
@@ -198,14 +207,14 @@ def apply_fsdp2(model: nn.Module, ctx: Optional[_mesh.ParallelContext] = None, p
     for blk in blocks:
         named = [(f"{prefix_of[id(blk)]}.{n}", p) for n, p in blk.named_parameters()]
         unit = _ShardedUnit(prefix_of[id(blk)], [p for _, p in named], [n for n, _ in named], group, param_dtype,
-                            reduce_dtype, reshard_after_forward)
+                            reduce_dtype, reshard_after_forward, partial_group=partial)
         seen.update(id(p) for _, p in named)
         _wrap(blk, unit, activation_checkpointing)
         state.units.append(unit)
     rest = [(n, p) for n, p in model.named_parameters() if id(p) not in seen]
     if rest:
         unit = _ShardedUnit("root", [p for _, p in rest], [n for n, _ in rest], group, param_dtype, reduce_dtype,
-                            reshard_after_forward=False, keep_resident=True)   # embedding / head / final norm
+                            reshard_after_forward=False, keep_resident=True, partial_group=partial)   # embedding / head / final norm
         unit.unshard(force=True)
         state.units.append(unit)
     model._fsdp = state

@@ -180,3 +180,8 @@ def _against_one_process(dist_kw, world, clip, norm_bound=2e-5):
 def test_sharded_engine_with_context_parallelism():
     """Ranks of a sequence's parts hold the same parameters: gradients are averaged over them, and count once in the norm."""
     _against_one_process({"cp_size": 2}, 2, 0.5)
+
+
+def test_sharded_engine_sums_partial_gradients():
+    """Norm weights under sequence parallelism: every rank of the TP group has seen its own rows only."""
+    _against_one_process({"dp_size": 2, "tp_size": 2, "sequence_parallel": True}, 4, 0.0)
