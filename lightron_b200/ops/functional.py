@@ -1136,11 +1136,11 @@ def grad_norm(tensors, group=None) -> torch.Tensor:
 
 
 @torch.no_grad()
-def clip_grad_norm(tensors, max_norm: float, out=None, group=None, eps: float = 1e-6) -> torch.Tensor:
+def clip_grad_norm(tensors, max_norm: float, out=None, group=None, eps: float = 1e-6, counted=None) -> torch.Tensor:
     """Scales the tensors by ``min(1, max_norm / (norm + eps))`` and returns their norm (:func:`grad_norm`).  In place; or into ``out``, tensors of the same sizes
-    and types.  A norm that is not finite goes into the result as it would in the product: NaN stays NaN, an infinite norm gives zeros and NaN."""
+    and types.  ``counted``: tensors whose norm it is instead, as where other ranks of ``group`` hold some of the tensors, too, and they are to count once.  A norm that is not finite goes into the result as it would in the product: NaN stays NaN, an infinite norm gives zeros and NaN."""
     groups = _norm_groups(group)
-    if not groups and (host := native.host_ops()) is not None and (norm := host.clip_grad_norm(tensors, max_norm, out, eps)) is not NotImplemented:
+    if not groups and counted is None and (host := native.host_ops()) is not None and (norm := host.clip_grad_norm(tensors, max_norm, out, eps)) is not NotImplemented:
         return norm
     tensors = _norm_list(tensors, "tensors")
     if not (max_norm >= 0.0 and eps >= 0.0):
@@ -1148,8 +1148,11 @@ def clip_grad_norm(tensors, max_norm: float, out=None, group=None, eps: float = 
     outs = tensors if out is None else _norm_list(out, "out")
     if len(outs) != len(tensors) or any(o.shape != t.shape or o.dtype != t.dtype or o.device != t.device for o, t in zip(outs, tensors)):
         raise ValueError("out must be one tensor of the same size, type and device for each tensor")
+    counted = tensors if counted is None else _norm_list(counted, "counted")
+    if tensors and any(t.device != tensors[0].device for t in counted):
+        raise ValueError(f"counted tensors are not on {tensors[0].device}")
     if not tensors or not tensors[0].is_cuda:
-        norm = _reduce_sumsq(ref.grad_sumsq(tensors), groups).sqrt()
+        norm = _reduce_sumsq(ref.grad_sumsq(counted), groups).sqrt()
         by = (max_norm / (norm + eps)).clamp_max(1.0)
         for t, o in zip(tensors, outs):
             o.copy_((t.float() * by).to(t.dtype))
@@ -1159,7 +1162,7 @@ def clip_grad_norm(tensors, max_norm: float, out=None, group=None, eps: float = 
         # (elements of the kernel's tensors lie in one piece, and in the same order in both)
         src = [t if _dense(t) else t.contiguous() for t in tensors]
         dst = [o if o is t or (o.stride() == t.stride() and _dense(o)) else torch.empty_like(t) for t, o in zip(src, outs)]
-        parts, n = _grad_parts(src, dev)
+        parts, n = _grad_parts(src if counted is tensors else counted, dev)
         if groups:
             sumsq = torch.empty(1, dtype=torch.float32, device=dev)
             native.call("lb_grad_total", parts.data_ptr(), n, sumsq.data_ptr(), 0, native.stream_ptr())

@@ -70,6 +70,16 @@ class _ShardedUnit:
         self.unshard(force=True)
         self.reshard()
 
+    def without(self, t: torch.Tensor, skip) -> List[torch.Tensor]:
+        """The pieces of a tensor over this rank's shard that belong to no parameter for which ``skip(parameter)`` holds."""
+        start, pieces, at = self.rank * self.shard_len, [], 0
+        for p, off in zip(self.params, self.offsets):
+            if skip(p):
+                lo, hi = (min(max(x - start, at), self.shard_len) for x in (off, off + p.numel()))
+                pieces.append(t[at:lo])
+                at = hi
+        return [x for x in (*pieces, t[at:]) if x.numel()]
+
     # ---- parameter lifetime ------------------------------------------------------------------
     def unshard(self, force: bool = False) -> None:
         if not self.sharded and not force:
@@ -238,9 +248,11 @@ class FSDPOptimizer:
     ``optim.DistributedAdamW`` and ``fsdp_native.NativeFSDP``."""
 
     def __init__(self, model: nn.Module, lr: float, weight_decay: float, betas=(0.9, 0.999), eps: float = 1e-8, grad_clip: float = 0.0, groups=()):
-        """``grad_clip``: limit of the gradients' global norm (0: none), whose squares are summed over ``groups``, the process groups that hold
-        different shards."""
+        """``grad_clip``: limit of the gradients' global norm (0: none), whose squares are summed over ``groups``: the ranks that shard the parameters, and the TP
+        group.  Parameters that all ranks of the TP group hold whole count on its first rank."""
         self.model, self.state = model, model._fsdp
+        ctx = getattr(model, "ctx", None) or _mesh.get_context()
+        self.count_replicated = ctx.tp_group is None or ctx.tp_group not in groups or comm.group_rank(ctx.tp_group) == 0
         self.grad_clip, self.groups, self.last_grad_norm = grad_clip, list(groups), None
         self.opt = self.state.make_optimizer(lr=lr, weight_decay=weight_decay, betas=betas, eps=eps)
         self.step_count = 0
@@ -258,7 +270,9 @@ class FSDPOptimizer:
     def step(self) -> None:
         if self.grad_clip > 0:
             from ..ops import functional as OF
-            self.last_grad_norm = OF.clip_grad_norm([u.shard.grad for u in self.state.units if u.shard.grad is not None], self.grad_clip, group=self.groups)
+            units = [u for u in self.state.units if u.shard.grad is not None]
+            counted = None if self.count_replicated else [t for u in units for t in u.without(u.shard.grad, lambda p: not hasattr(p, "tp_shard_dim"))]
+            self.last_grad_norm = OF.clip_grad_norm([u.shard.grad for u in units], self.grad_clip, group=self.groups, counted=counted)
         self.opt.step()
         self.step_count += 1
 

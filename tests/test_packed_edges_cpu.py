@@ -185,3 +185,24 @@ def test_sharded_engine_with_context_parallelism():
 def test_sharded_engine_sums_partial_gradients():
     """Norm weights under sequence parallelism: every rank of the TP group has seen its own rows only."""
     _against_one_process({"dp_size": 2, "tp_size": 2, "sequence_parallel": True}, 4, 0.0)
+
+
+@pytest.mark.parametrize("sp", [False, True])
+def test_sharded_engine_counts_replicated_parameters_once(sp):
+    """Parameters that all ranks of a TP group hold, in the global norm."""
+    _against_one_process({"dp_size": 2, "tp_size": 2, "sequence_parallel": sp}, 4, 0.5)
+
+
+def test_clip_by_the_norm_of_others():
+    g = torch.Generator().manual_seed(0)
+    ts = [torch.randn(30, generator=g), torch.randn(4, 5, generator=g)]
+    own = [t.clone() for t in ts]
+    norm = OF.clip_grad_norm(own, 0.5, counted=ts[:1])
+    assert torch.equal(norm, OF.grad_norm(ts[:1]))
+    for t, o in zip(ts, own):
+        assert torch.allclose(o, t * 0.5 / (norm + 1e-6), rtol=1e-6)
+    assert float(OF.clip_grad_norm(own, 0.5, counted=[])) == 0.0
+    with pytest.raises(ValueError):
+        OF.clip_grad_norm(own, 0.5, counted=[torch.zeros(2, dtype=torch.int32)])
+    with pytest.raises(ValueError):
+        OF.clip_grad_norm(own, 0.5, counted=[torch.zeros(2, device="meta")])

@@ -202,3 +202,16 @@ def test_packed_attention_without_gradients():
         assert torch.equal(call(qkv.clone()), want)
     with torch.inference_mode():
         assert torch.equal(call(qkv.clone()), want)
+
+
+def test_clip_by_the_norm_of_others():
+    """``counted``: pieces of the tensors, none, and pieces that are not dense."""
+    from lightron_b200.ops import functional as OF
+    ts = [_rand(3000, seed=1, dtype=torch.float32), _rand(40, 70, seed=2)]
+    for counted in ([ts[0][5:1000], ts[0][2000:]], [ts[1][:, 3:50]], []):
+        own = [t.clone() for t in ts]
+        norm = OF.clip_grad_norm(own, 0.5, counted=counted)
+        assert torch.equal(norm, OF.grad_norm(counted).to(norm.device))
+        by = min(1.0, 0.5 / (norm.item() + 1e-6))
+        for t, o, e in zip(ts, own, (2.0 ** -22, 2.0 ** -8)):
+            assert ((o.double() - t.double() * by).abs() <= e * (t.double() * by).abs()).all()
