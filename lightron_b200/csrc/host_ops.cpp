@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
+#include <algorithm>
 #include <atomic>
 #include <climits>
 #include <cmath>
@@ -923,6 +924,27 @@ struct NormList {
     return k > 0 && k < INT_MAX;
   }
 };
+// Whether a result lies on another result or on a tensor that is not its own
+bool shares_memory(const NormList& from, const NormList& to) {
+  struct Piece { uintptr_t lo, hi; bool written; };
+  std::vector<Piece> v;
+  v.reserve(2 * to.at.size());
+  for (size_t i = 0; i < to.at.size(); i++) {
+    const uintptr_t bytes = (uintptr_t)to.n[i] * (to.type[i] == 2 ? 4 : 2), w = (uintptr_t)to.at[i], r = (uintptr_t)from.at[i];
+    if (!bytes) continue;
+    v.push_back({w, w + bytes, true});
+    if (r != w) v.push_back({r, r + bytes, false});
+  }
+  const auto before = [](const Piece& a, const Piece& b) { return a.lo < b.lo; };
+  if (!std::is_sorted(v.begin(), v.end(), before)) std::sort(v.begin(), v.end(), before);
+  uintptr_t end = 0, end_written = 0;
+  for (const Piece& x : v) {
+    if (x.lo < (x.written ? end : end_written)) return true;
+    end = std::max(end, x.hi);
+    if (x.written) end_written = std::max(end_written, x.hi);
+  }
+  return false;
+}
 // Runs the sums of squares; the parts and how many
 std::pair<Tensor, int> norm_parts(const NormList& l) {
   Tensor parts = empty_f32({api.lb_grad_norm_parts((int)l.at.size())}, l.t[0]);
@@ -963,6 +985,7 @@ PyObject* py_clip_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (to.type[i] != l.type[i] || !to.t[i].sizes().equals(l.t[i].sizes())) LB_NOT_PLAIN;
     if (to.t[i].requires_grad() && at::GradMode::is_enabled()) LB_NOT_PLAIN;
   }
+  if (shares_memory(l, to)) LB_NOT_PLAIN;
   return THPVariable_Wrap(unlocked([&] {
     at::NoGradGuard off;
     const std::pair<Tensor, int> p = norm_parts(l);

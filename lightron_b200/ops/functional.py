@@ -1086,6 +1086,23 @@ def _dense(t: torch.Tensor) -> bool:
     return t.is_contiguous() or (t.numel() > 0 and torch.ops.aten.is_non_overlapping_and_dense(t))
 
 
+def _shares_memory(tensors, outs) -> bool:
+    """Whether a result in one piece lies on another result or on a tensor that is not its own: CTAs, which run in any order, would read what others have written."""
+    pieces = []
+    for t, o in zip(tensors, outs):
+        own = o is t or (o.data_ptr() == t.data_ptr() and o.stride() == t.stride())
+        for x, written in ((o, True),) if own else ((o, True), (t, False)):
+            if x.numel() and _dense(x):
+                pieces.append((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size(), written))
+    end = end_written = 0
+    for lo, hi, written in sorted(pieces):
+        if lo < (end if written else end_written):
+            return True
+        end = max(end, hi)
+        end_written = max(end_written, hi) if written else end_written
+    return False
+
+
 def _norm_table(tensors):
     import ctypes
     n = len(tensors)
@@ -1138,7 +1155,7 @@ def grad_norm(tensors, group=None) -> torch.Tensor:
 @torch.no_grad()
 def clip_grad_norm(tensors, max_norm: float, out=None, group=None, eps: float = 1e-6, counted=None) -> torch.Tensor:
     """Scales the tensors by ``min(1, max_norm / (norm + eps))`` and returns their norm (:func:`grad_norm`).  In place; or into ``out``, tensors of the same sizes
-    and types.  ``counted``: tensors whose norm it is instead, as where other ranks of ``group`` hold some of the tensors, too, and they are to count once.  A norm that is not finite goes into the result as it would in the product: NaN stays NaN, an infinite norm gives zeros and NaN."""
+    and types, which share no memory with each other or with other tensors.  ``counted``: tensors whose norm it is instead, as where other ranks of ``group`` hold some of the tensors, too, and they are to count once.  A norm that is not finite goes into the result as it would in the product: NaN stays NaN, an infinite norm gives zeros and NaN."""
     groups = _norm_groups(group)
     if not groups and counted is None and (host := native.host_ops()) is not None and (norm := host.clip_grad_norm(tensors, max_norm, out, eps)) is not NotImplemented:
         return norm
@@ -1148,6 +1165,8 @@ def clip_grad_norm(tensors, max_norm: float, out=None, group=None, eps: float = 
     outs = tensors if out is None else _norm_list(out, "out")
     if len(outs) != len(tensors) or any(o.shape != t.shape or o.dtype != t.dtype or o.device != t.device for o, t in zip(outs, tensors)):
         raise ValueError("out must be one tensor of the same size, type and device for each tensor")
+    if _shares_memory(tensors, outs):
+        raise ValueError("tensors that are scaled share memory with each other, or results with other tensors")
     counted = tensors if counted is None else _norm_list(counted, "counted")
     if tensors and any(t.device != tensors[0].device for t in counted):
         raise ValueError(f"counted tensors are not on {tensors[0].device}")

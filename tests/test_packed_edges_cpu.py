@@ -206,3 +206,18 @@ def test_clip_by_the_norm_of_others():
         OF.clip_grad_norm(own, 0.5, counted=[torch.zeros(2, dtype=torch.int32)])
     with pytest.raises(ValueError):
         OF.clip_grad_norm(own, 0.5, counted=[torch.zeros(2, device="meta")])
+
+
+def test_clip_refuses_memory_that_overlaps():
+    """As on the GPU, where two entries that share memory would be scaled once or twice, as it comes."""
+    a, b, buf = torch.ones(100), torch.ones(50), torch.zeros(200)
+    for ts, out in (([a, b, a], None), ([a[:60], a[40:]], None), ([a, b], [buf[:100], buf[60:110]]), ([a[:50], a[50:]], [a[50:], a[:50]]), ([a[:99], b], [a[1:], buf[:50]])):
+        with pytest.raises(ValueError):
+            OF.clip_grad_norm(ts, 1e-3, out=out)
+    assert (a == 1).all() and (b == 1).all() and (buf == 0).all()
+    OF.clip_grad_norm([a[:50], a[50:], b, a[:0], a[:0]], 1.0)
+    OF.clip_grad_norm([a, b], 1.0, out=[a, b])
+    # columns of one matrix lie between each other, and share nothing
+    m = torch.ones(10, 4)
+    norm = OF.clip_grad_norm([m[:, :2], m[:, 2:]], 1.0)
+    assert abs(float(norm) - 40 ** 0.5) < 1e-5 and torch.allclose(m, torch.full((10, 4), 40 ** -0.5))

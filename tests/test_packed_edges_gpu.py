@@ -215,3 +215,19 @@ def test_clip_by_the_norm_of_others():
         by = min(1.0, 0.5 / (norm.item() + 1e-6))
         for t, o, e in zip(ts, own, (2.0 ** -22, 2.0 ** -8)):
             assert ((o.double() - t.double() * by).abs() <= e * (t.double() * by).abs()).all()
+
+
+def test_clip_refuses_memory_that_overlaps():
+    """Two entries that share memory would be scaled once or twice, as it comes: refused, with nothing written."""
+    from lightron_b200.ops import functional as OF
+    a = torch.ones(100, device="cuda")
+    b = torch.ones(50, device="cuda")
+    buf = torch.zeros(200, device="cuda")
+    for ts, out in (([a, b, a], None), ([a[:60], a[40:]], None), ([a, b], [buf[:100], buf[60:110]]), ([a[:50], a[50:]], [a[50:], a[:50]]), ([a[:99], b], [a[1:], buf[:50]])):
+        with pytest.raises(ValueError):
+            OF.clip_grad_norm(ts, 1e-3, out=out)
+    assert (a == 1).all() and (b == 1).all() and (buf == 0).all()
+    # neighbours, and the same list as its own result, are not that
+    OF.clip_grad_norm([a[:50], a[50:], b, a[:0], a[:0]], 1.0)
+    OF.clip_grad_norm([a, b], 1.0, out=[a, b])
+    assert abs(_norm64([a, b]) - 1) < 1e-5
