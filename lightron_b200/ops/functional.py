@@ -1074,6 +1074,8 @@ _NORM_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 def _norm_list(tensors, what: str) -> List[torch.Tensor]:
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{what} must be tensors, got {type(t).__name__} (gradients that are missing are left out of the list)")
         if t.dtype not in _NORM_TYPES or t.layout != torch.strided:
             raise ValueError(f"{what} must be dense bf16, fp16 or fp32, got {t.dtype} {t.layout}")
         if t.device != tensors[0].device:

@@ -221,3 +221,11 @@ def test_clip_refuses_memory_that_overlaps():
     m = torch.ones(10, 4)
     norm = OF.clip_grad_norm([m[:, :2], m[:, 2:]], 1.0)
     assert abs(float(norm) - 40 ** 0.5) < 1e-5 and torch.allclose(m, torch.full((10, 4), 40 ** -0.5))
+
+
+@pytest.mark.parametrize("bad", [[torch.ones(3), None], [None], [1.0]])
+def test_gradients_that_are_missing_are_refused(bad):
+    with pytest.raises(ValueError):
+        OF.grad_norm(bad)
+    with pytest.raises(ValueError):
+        OF.clip_grad_norm(bad, 1.0)

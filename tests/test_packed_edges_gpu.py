@@ -231,3 +231,12 @@ def test_clip_refuses_memory_that_overlaps():
     OF.clip_grad_norm([a[:50], a[50:], b, a[:0], a[:0]], 1.0)
     OF.clip_grad_norm([a, b], 1.0, out=[a, b])
     assert abs(_norm64([a, b]) - 1) < 1e-5
+
+
+def test_gradients_that_are_missing_are_refused():
+    from lightron_b200.ops import functional as OF
+    for ts in ([torch.ones(3, device="cuda"), None], [None]):
+        with pytest.raises(ValueError):
+            OF.grad_norm(ts)
+        with pytest.raises(ValueError):
+            OF.clip_grad_norm(ts, 1.0)
