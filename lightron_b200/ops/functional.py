@@ -1131,6 +1131,8 @@ def _norm_groups(group) -> list:
 
 def _reduce_sumsq(sumsq: torch.Tensor, groups) -> torch.Tensor:
     for g in groups:
+        if not sumsq.is_cuda and "nccl" in dist.get_backend(g) and torch.cuda.is_available():      # a rank that holds nothing takes part, where the others do
+            sumsq = sumsq.cuda()
         dist.all_reduce(sumsq, group=g)
     return sumsq
 

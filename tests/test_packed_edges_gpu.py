@@ -240,3 +240,16 @@ def test_gradients_that_are_missing_are_refused():
             OF.grad_norm(ts)
         with pytest.raises(ValueError):
             OF.clip_grad_norm(ts, 1.0)
+
+
+def test_a_rank_that_holds_nothing_takes_part(monkeypatch):
+    """An empty list has no device: its zero is added where the group's backend works."""
+    import torch.distributed as dist
+    from lightron_b200.ops import functional as OF
+    seen = []
+    monkeypatch.setattr(dist, "get_world_size", lambda g=None: 2)
+    monkeypatch.setattr(dist, "get_backend", lambda g=None: "nccl")
+    monkeypatch.setattr(dist, "all_reduce", lambda t, group=None: seen.append(t.device.type) or t.add_(9.0))
+    for call in (OF.grad_norm, lambda ts, group: OF.clip_grad_norm(ts, 1.0, group=group)):
+        assert call([], group="others").item() == 3.0
+    assert seen == ["cuda", "cuda"]
