@@ -793,7 +793,7 @@ def attention_mask(documents: Optional[torch.Tensor] = None, prefix: Optional[to
         raise ValueError(f"attention_mask on the GPU takes up to 65535 sequences of up to {MASK_MAX_LENGTH} positions, got {B} x {S}")
     documents = None if documents is None else documents.contiguous()
     marks = None if marks is None else marks.contiguous()
-    lens = None if lens is None else lens.to(torch.int32).contiguous()
+    lens = None if lens is None else lens.clamp(0, S).to(torch.int32).contiguous()
     qb = torch.empty(B, S, 2, dtype=torch.int32, device=first.device)
     kb = torch.empty_like(qb)
     with native.on_device(first):
@@ -976,7 +976,8 @@ def _check_axes(B, S, d, cos, sin, positions, axes):
         raise ValueError("cos and sin have no rows")
     if not cos.device == sin.device == positions.device:
         raise ValueError("cos, sin and positions are on different devices")
-    positions = positions.to(torch.int32)
+    if positions.dtype == torch.int64:              # (what is outside of the tables stays outside in 32 bits)
+        positions = positions.clamp(-1, cos.shape[0]).to(torch.int32)
     return (positions if positions.stride(-1) == 1 else positions.contiguous()), axes
 
 

@@ -229,3 +229,10 @@ def test_gradients_that_are_missing_are_refused(bad):
         OF.grad_norm(bad)
     with pytest.raises(ValueError):
         OF.clip_grad_norm(bad, 1.0)
+
+
+def test_positions_beyond_32_bits():
+    cos, sin = ref.rope_tables(8, 16)
+    x = torch.randn(1, 3, 1, 8, generator=torch.Generator().manual_seed(0))
+    y = OF.rope_axes(x, cos, sin, torch.tensor([[1, 2 ** 32 + 1, -2 ** 32]]), [0] * 4)
+    assert torch.isfinite(y[:, 0]).all() and torch.isnan(y[:, 1:]).all()

@@ -253,3 +253,17 @@ def test_a_rank_that_holds_nothing_takes_part(monkeypatch):
     for call in (OF.grad_norm, lambda ts, group: OF.clip_grad_norm(ts, 1.0, group=group)):
         assert call([], group="others").item() == 3.0
     assert seen == ["cuda", "cuda"]
+
+
+def test_whole_numbers_beyond_32_bits():
+    """Positions past the tables, prefix lengths past the sequence: as such, not what their low 32 bits say."""
+    from lightron_b200.ops import functional as OF
+    from lightron_b200.ops import reference as ref
+    cos, sin = ref.rope_tables(16, 10, device="cuda")
+    pos = torch.tensor([[0, 9, 2 ** 32 + 1, -2 ** 32]] * 2, device="cuda")
+    y = OF.rope_axes(_rand(1, 4, 2, 16), cos, sin, pos, [0, 1] * 4)
+    assert torch.isfinite(y[:, :2]).all() and torch.isnan(y[:, 2:]).all()
+    lens = torch.tensor([2 ** 32, -2 ** 32 + 3, 2], device="cuda")
+    mask = OF.attention_mask(prefix=lens, length=5)
+    want = ref.mask_bounds(5, None, lens.cpu(), True)
+    assert torch.equal(mask.q_bounds.cpu(), want[0]) and torch.equal(mask.k_bounds.cpu(), want[1])
