@@ -48,7 +48,8 @@ long long ma_bwd_ws_bytes(const MaParams& p);
 
 // What the kernels need of the scores' form, in units of log2: x * scale without a cap; with one, tanh(x * by) * times = x * (c[0] + c[1] x^2 + c[2] x^4 + c[3] x^6) while
 // |x| <= limit, which is 0.6 / by: relative error 2.2e-6 (coefficients of tanh(u) / u in u^2, found by least squares over Chebyshev points with weights that were raised
-// where the error was largest).  Pairs hold a value twice.
+// where the error was largest).  Where a coefficient leaves fp32 (caps below some 1e-7 times the scale) the definition is taken for every score: infinity times the square
+// of a score that is exactly zero would be NaN.  Pairs hold a value twice.
 struct MaTerms {
   unsigned long long scale, cap, c[4];
   float scale1, cap1, by2, limit;       // by2: 2 * log2(e) * by, for tanh by its definition
@@ -61,10 +62,14 @@ struct MaTerms {
     by2 = limit = 0.f;
     const double by = p.softcap > 0.f ? (double)p.scale / p.softcap : 0.0;
     double pw = by * (times_cap ? p.softcap * log2e : 1.0);
-    for (int i = 0; i < 4; i++, pw *= by * by) c[i] = twice((float)(k[i] * pw));
+    bool fits = true;
+    for (int i = 0; i < 4; i++, pw *= by * by) {
+      c[i] = twice((float)(k[i] * pw));
+      fits = fits && pw < 3e38;
+    }
     if (p.softcap > 0.f) {
-      by2 = (float)(2.0 * log2e * by);
-      limit = (float)(0.6 / by);
+      by2 = (float)(2.0 * log2e * by < 3e38 ? 2.0 * log2e * by : 3e38);
+      limit = fits ? (float)(0.6 / by) : -1.f;
     } else {
       c[0] = scale;
     }

@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <cfloat>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -863,7 +864,7 @@ PyObject* py_masked_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     PyErr_Clear();
     LB_NOT_PLAIN;
   }
-  if (!(scale > 0.0 && scale < HUGE_VAL) || !(softcap >= 0.0 && softcap < HUGE_VAL)) LB_NOT_PLAIN;
+  if (!(scale >= FLT_MIN && scale <= FLT_MAX) || !(softcap == 0.0 || (softcap >= FLT_MIN && softcap <= FLT_MAX))) LB_NOT_PLAIN;
   const MaskedArgs m{a[6] == Py_True, at::GradMode::is_enabled() && (q->requires_grad() || k->requires_grad() || v->requires_grad()), scale, softcap};
   return THPVariable_Wrap(unlocked([&, q_ = *q, k_ = *k, v_ = *v, sl = maybe(slopes), qi = maybe(qb), ki = maybe(kb)] { return MaskedAttention::apply(q_, k_, v_, sl, qi, ki, m); }));
   END_HANDLE_TH_ERRORS

@@ -869,6 +869,7 @@ class _MaskedAttn(torch.autograd.Function):
 
 
 MASKED_MAX_HEAD_DIM = 128
+_FP32_TINY, _FP32_MAX = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 
 
 def _check_masked(q, k, v, mask, causal, scale, softcap, slopes) -> bool:
@@ -883,10 +884,10 @@ def _check_masked(q, k, v, mask, causal, scale, softcap, slopes) -> bool:
         raise ValueError(f"{Sq} queries at the end of {Sk} positions")
     if not (k.dtype == v.dtype == q.dtype and k.device == v.device == q.device):
         raise ValueError(f"q, k, v differ in type or device: {q.dtype} {q.device}, {k.dtype} {k.device}, {v.dtype} {v.device}")
-    if scale is not None and not 0.0 < scale < float("inf"):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
-    if not (0.0 <= softcap < float("inf")):
-        raise ValueError(f"softcap must be zero (none) or positive and finite, got {softcap}")
+    if scale is not None and not _FP32_TINY <= scale <= _FP32_MAX:
+        raise ValueError(f"scale must be positive and finite, in 32 bits, got {scale}")
+    if not (softcap == 0.0 or _FP32_TINY <= softcap <= _FP32_MAX):
+        raise ValueError(f"softcap must be zero (none) or positive and finite, in 32 bits, got {softcap}")
     if mask is not None:
         if not isinstance(mask, AttentionMask):
             raise ValueError(f"mask must come from attention_mask(), got {type(mask).__name__}")

@@ -236,3 +236,11 @@ def test_positions_beyond_32_bits():
     x = torch.randn(1, 3, 1, 8, generator=torch.Generator().manual_seed(0))
     y = OF.rope_axes(x, cos, sin, torch.tensor([[1, 2 ** 32 + 1, -2 ** 32]]), [0] * 4)
     assert torch.isfinite(y[:, 0]).all() and torch.isnan(y[:, 1:]).all()
+
+
+@pytest.mark.parametrize("kw", [dict(softcap=1e-45), dict(softcap=1e-50), dict(softcap=1e39), dict(scale=1e-46), dict(scale=1e39)])
+def test_numbers_that_32_bits_do_not_hold_are_refused(kw):
+    """A cap that became zero would be no cap at all."""
+    q = torch.zeros(1, 4, 2, 8)
+    with pytest.raises(ValueError):
+        OF.masked_attention(q, q, q, **kw)

@@ -267,3 +267,18 @@ def test_whole_numbers_beyond_32_bits():
     mask = OF.attention_mask(prefix=lens, length=5)
     want = ref.mask_bounds(5, None, lens.cpu(), True)
     assert torch.equal(mask.q_bounds.cpu(), want[0]) and torch.equal(mask.k_bounds.cpu(), want[1])
+
+
+# ---- caps near zero ---------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("cap", [1e-6, 1e-9, 1e-20])
+@pytest.mark.parametrize("d", [64, 128])
+def test_caps_near_zero(d, cap):
+    """Scores of exactly zero beside others that are all at the cap."""
+    S = 256
+    q, k, v, do = _rand(1, S, 2, d, seed=1), _rand(1, S, 1, d, seed=2), _rand(1, S, 1, d, seed=3), _rand(1, S, 2, d, seed=4)
+    q[:, :128] = 0
+    got = _run(q, k, v, do, softcap=cap)
+    _status_ok()
+    _close(got, attention64(q, k, v, _see(S, S, True), d ** -0.5, cap, None, do))
