@@ -879,7 +879,7 @@ PyObject* py_rope_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t B = x->size(0), S = x->size(1), d = x->size(3), pairs = d / 2;
   if (d % 8 || d > 256 || !fits_int({B, S, x->size(2)})) LB_NOT_PLAIN;
   if (!sized(cos, *x, at::kFloat) || !sized(sin, *x, at::kFloat) || !sized(pos, *x, at::kInt) || cos->dim() != 2 || cos->size(1) != pairs || !sin->sizes().equals(cos->sizes()) ||
-      cos->size(0) == 0 || !fits_int({cos->size(0)}) || ((uintptr_t)cos->const_data_ptr() & 15) || ((uintptr_t)sin->const_data_ptr() & 15))
+      cos->size(0) == 0 || !fits_int({cos->size(0)}))
     LB_NOT_PLAIN;
   const int64_t A = pos->dim() > 0 ? pos->size(0) : 0;
   if (A < 1 || A > 8 || !(pos->sizes().equals({A, S}) || pos->sizes().equals({A, B, S}))) LB_NOT_PLAIN;

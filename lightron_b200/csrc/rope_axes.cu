@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const __grid_constant__ 
 extern "C" int lb_rope_axes(const void* x, void* y, const void* cosT, const void* sinT, const void* positions, const unsigned char* axes, int n_axes, int B, int S, int h, int d,
                             int rows, const long long* strides, long long pos_a, long long pos_b, int inverse, void* stream) {
   if (B <= 0 || S <= 0 || h <= 0 || rows <= 0 || d <= 0 || d % 8 || d > 2 * MAX_PAIRS || n_axes <= 0 || n_axes > MAX_AXES) return LB_ERR_SHAPE;
-  if (!x || !y || !cosT || !sinT || !positions || !axes || !strides || ((uintptr_t)x | (uintptr_t)y | (uintptr_t)cosT | (uintptr_t)sinT) & 15) return LB_ERR_ARG;
+  if (!x || !y || !cosT || !sinT || !positions || !axes || !strides || ((uintptr_t)x | (uintptr_t)y) & 15) return LB_ERR_ARG;
   for (int i = 0; i < 6; i++)
     if (strides[i] % 8) return LB_ERR_SHAPE;
   RopeAxesParams p{(const bf16*)x, (bf16*)y, (const float*)cosT, (const float*)sinT, (const int*)positions, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], pos_a, pos_b, B, S, h, d, rows, inverse, h, {}};

@@ -282,3 +282,18 @@ def test_caps_near_zero(d, cap):
     got = _run(q, k, v, do, softcap=cap)
     _status_ok()
     _close(got, attention64(q, k, v, _see(S, S, True), d ** -0.5, cap, None, do))
+
+
+# ---- rotation -----------------------------------------------------------------------------------------
+
+
+def test_rope_axes_tables_of_any_alignment():
+    from lightron_b200.ops import functional as OF
+    from lightron_b200.ops import reference as ref
+    cos, sin = ref.rope_tables(64, 50, device="cuda")
+    flat = torch.empty(2 * cos.numel() + 1, device="cuda")
+    c, s = flat[1:1 + cos.numel()].view(cos.shape).copy_(cos), flat[1 + cos.numel():].view(cos.shape).copy_(sin)
+    assert c.data_ptr() % 16 and c.is_contiguous()
+    pos = torch.arange(20, device="cuda", dtype=torch.int32).expand(2, 20).contiguous()
+    x = _rand(1, 20, 3, 64)
+    assert torch.equal(OF.rope_axes(x, c, s, pos, [0, 1] * 16), OF.rope_axes(x, cos, sin, pos, [0, 1] * 16))
