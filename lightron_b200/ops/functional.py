@@ -757,8 +757,9 @@ def attention_mask(documents: Optional[torch.Tensor] = None, prefix: Optional[to
     """``documents`` [B, S] int32 / int64: a document is a run of equal ids, whose positions see no other run's; negative ids are padding, which
     sees nothing (its output is zero) and is seen by nothing.  ``prefix``: the leading part of each document that is seen both ways
     in a causal mask, as [B, S] marks (bool / uint8; the marked run at the document's start counts) or as [B] int32 lengths from the sequence's
-    start (``length`` then gives S where there are no documents).  Values stay on the device.  (Values of padding are read all
-    the same, and multiplied by weights of zero: they have to be finite, as those of causal attention have to be.)"""
+    start (``length`` then gives S where there are no documents).  Values stay on the device.  (What queries, keys, values
+    and the output's gradient hold at hidden positions is read all the same, and multiplied by weights of zero: it has to be finite, as for causal attention.  The scores that it
+    makes with visible positions may be anything.)"""
     if length is None and (host := native.host_ops()) is not None and (bounds := host.attention_mask(documents, prefix, causal)) is not NotImplemented:
         return AttentionMask(*bounds, causal)
     if documents is None and prefix is None:

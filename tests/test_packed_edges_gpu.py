@@ -297,3 +297,88 @@ def test_rope_axes_tables_of_any_alignment():
     pos = torch.arange(20, device="cuda", dtype=torch.int32).expand(2, 20).contiguous()
     x = _rand(1, 20, 3, 64)
     assert torch.equal(OF.rope_axes(x, c, s, pos, [0, 1] * 16), OF.rope_axes(x, cos, sin, pos, [0, 1] * 16))
+
+
+# ---- hidden scores out of range ---------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("cap,alibi", [(0.0, False), (0.0, True), (30.0, False), (200.0, True)])
+def test_hidden_scores_out_of_range(cap, alibi):
+    """Finite queries and keys of two documents whose scores across them pass fp32: infinite, and NaN where infinities meet.  Both documents as if alone."""
+    from lightron_b200.ops import functional as OF
+    S, cut, h, d = 256, 100, 2, 64
+    q, k, v, do = (_rand(1, S, h, d, seed=i) for i in range(1, 5))
+    up = torch.ones(S, 1, 1, device="cuda")
+    up[:cut], up[cut:] = 2.0 ** 60, 2.0 ** -100
+    q, k = (q.float() * up).to(BF16), (k.float() / up).to(BF16)
+    ids = torch.zeros(1, S, dtype=torch.int32, device="cuda")
+    ids[:, cut:] = 1
+    slopes = torch.tensor([0.1, 0.02], device="cuda") if alibi else None
+    got = _run(q, k, v, do, mask=OF.attention_mask(documents=ids), softcap=cap, slopes=slopes)
+    _status_ok()
+    for part in (slice(0, cut), slice(cut, S)):
+        n = part.stop - part.start
+        want = attention64(q[:, part], k[:, part], v[:, part], _see(n, n, True), d ** -0.5, cap, slopes, do[:, part])
+        _close([g[:, part] for g in got], want)
+
+
+# ---- heads in several groups ------------------------------------------------------------------------
+
+
+def test_heads_in_several_groups_forward():
+    """K and V of more heads than are kept in L2 together: groups of 4, 4 and 2 of ten heads."""
+    from lightron_b200.ops import functional as OF
+    from lightron_b200.ops import native
+    Sq, Sk, h, d = 2000, 40960, 10, 64
+    assert native.require().lb_masked_attn_fwd_ws_bytes(1, Sq, Sk, h, h, d) == 0          # (not split)
+    q, k, v = _rand(1, Sq, h, d, seed=1), _rand(1, Sk, h, d, seed=2), _rand(1, Sk, h, d, seed=3)
+    with torch.no_grad():
+        o = OF.masked_attention(q, k, v)
+    _status_ok()
+    see = _see(Sq, Sk, True)
+    for i in range(h):
+        w = attention64(*(t[:, :, i:i + 1] for t in (q, k, v)), see, d ** -0.5)
+        assert rel(o[:, :, i:i + 1], w) < 5e-3, i
+
+
+def test_heads_in_several_groups_backward():
+    """236 pairs of batch and key head in groups of 32, the last one smaller."""
+    B, S, h, d = 59, 400, 4, 64
+    q, k, v, do = (_rand(B, S, h, d, seed=i) for i in range(1, 5))
+    got = _run(q, k, v, do)
+    _status_ok()
+    _close(got, attention64(q, k, v, _see(S, S, True), d ** -0.5, 0.0, None, do))
+
+
+# ---- two streams at a time --------------------------------------------------------------------------
+
+
+def test_two_streams_at_a_time():
+    from lightron_b200.ops import functional as OF
+
+    def work(i):
+        q, k, v, do = (_rand(2, 700, 4, 64, seed=10 * i + j) for j in range(4))
+        grads = [_rand(300 + i, 77, seed=i), _rand(5000, seed=i, dtype=torch.float32)]
+        ids = documents(2, 700, 150, seed=i).cuda()
+        torch.cuda.synchronize()
+
+        def step():
+            mask = OF.attention_mask(documents=ids)
+            out = _run(q, k, v, do, mask=mask, softcap=20.0)
+            outs = [torch.empty_like(g) for g in grads]
+            return [out[0], out[2], out[3], OF.clip_grad_norm(grads, 1.0, out=outs), *outs]
+        return step
+    steps = [work(1), work(2)]
+    want = [s() for s in steps]
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (s, st) in enumerate(zip(steps, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(s())
+    torch.cuda.synchronize()
+    _status_ok()
+    for w, runs in zip(want, got):
+        for g in runs:
+            assert all(torch.equal(a, b) for a, b in zip(g, w))
