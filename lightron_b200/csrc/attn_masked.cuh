@@ -46,10 +46,13 @@ long long ma_fwd_ws_bytes(const MaParams& p);
 int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s);
 long long ma_bwd_ws_bytes(const MaParams& p);
 
-// What the kernels need of the scores' form, in units of log2: x * scale without a cap; with one, tanh(x * by) * times = x * (c[0] + c[1] x^2 + c[2] x^4 + c[3] x^6) while
-// |x| <= limit, which is 0.6 / by: relative error 2.2e-6 (coefficients of tanh(u) / u in u^2, found by least squares over Chebyshev points with weights that were raised
-// where the error was largest).  Where a coefficient leaves fp32 (caps below some 1e-7 times the scale) the definition is taken for every score: infinity times the square
-// of a score that is exactly zero would be NaN.  Pairs hold a value twice.
+// What the kernels need of the scores' form, in units of log2: x * scale without a cap; with one, tanh(u) * times, u = x * by, as x * (c[0] + c[1] x^2 + c[2] x^4 + c[3] x^6) while
+// |x| <= limit: relative error 2.2e-6 up to u = 0.6 (coefficients of tanh(u) / u in u^2, found by least squares over Chebyshev points with weights that were raised
+// where the error was largest).  The limit is u = 0.6 or less:
+//   * 33 / cap, that is scores of 33, where the error is 7e-5 of a score; the definition's, some 1.3e-7 caps wherever the score lies, is reached at u = 0.06, which is the least;
+//   * coefficients that fp32 holds as zero (small scales, large caps: powers of by) have to be small against the error where they are missing: 0.041 u^6, 0.13 u^4, u^2 / 3;
+//   * where one overflows (caps below some 1e-7 times the scale) the definition is taken for every score: infinity times the square of a score that is exactly zero would be NaN.
+// Pairs hold a value twice.
 struct MaTerms {
   unsigned long long scale, cap, c[4];
   float scale1, cap1, by2, limit;       // by2: 2 * log2(e) * by, for tanh by its definition
@@ -62,14 +65,16 @@ struct MaTerms {
     by2 = limit = 0.f;
     const double by = p.softcap > 0.f ? (double)p.scale / p.softcap : 0.0;
     double pw = by * (times_cap ? p.softcap * log2e : 1.0);
-    bool fits = true;
+    constexpr double missing[4] = {0.0, 0.0025, 0.06, 0.1};      // u up to which c[i] may be left out: 2.1e-6, 1.7e-6, 4.1e-8
+    double most = p.softcap > 55.f ? fmax(33.0 / p.softcap, 0.06) : 0.6;
     for (int i = 0; i < 4; i++, pw *= by * by) {
       c[i] = twice((float)(k[i] * pw));
-      fits = fits && pw < 3e38;
+      if (!(pw < 3e38)) most = -1.0;
+      if (fabs(k[i] * pw) < 1.2e-38) most = fmin(most, missing[i]);
     }
     if (p.softcap > 0.f) {
       by2 = (float)(2.0 * log2e * by < 3e38 ? 2.0 * log2e * by : 3e38);
-      limit = fits ? (float)(0.6 / by) : -1.f;
+      limit = most < 0.0 ? -1.f : (float)(most / by);
     } else {
       c[0] = scale;
     }

@@ -11,8 +11,8 @@
 //   * with a cap the scores are known to lie within it.  Up to softcap * log2(e) = 80 exponentials are taken relative to zero instead of the running
 //     maximum: 2^+-80 and sums of them are far inside fp32 (and bf16 has the same exponents), and nothing is ever rescaled (8 x 2048, d 64 with the maximum / without 400 / 304 us, 1 x 8192, d 128 828 / 566).  With 128 columns the two halves of a
 //     block then have nothing to tell each other, and their scores, P and products run apart (d 128, cap: 700 -> 640 us).  Above 80 the maximum is kept.
-//   * tanh: where no score of 32 rows x 64 columns is above 0.6 caps, x times a polynomial in x^2 on the FMA pipe, two at a time (relative error
-//     2.1e-6, found by least squares with re-weighted points; 7e-5 of a score at most); else by its definition with exp2, whose units the softmax needs itself.
+//   * tanh: where no score of 32 rows x 64 columns is above 0.6 caps (33 at caps above 55: MaTerms), x times a polynomial in x^2 on the FMA pipe, two at a time
+//     (7e-5 of a score at most, at caps above 550 1.3e-7 caps); else by its definition with exp2, whose units the softmax needs itself.
 //   * the bias is an addend of the FMA that scales a score (or evaluates its polynomial), counted up along the columns; only where a block holds keys on both sides of a row is its
 //     distance made per column.  Without a cap the exponentials' reference is a bound, not the maximum itself: what they are relative to cancels, as long as it is within 2^60
 //     or so of the maximum.  The nearest key blocks come first, or the maximum would grow from block to block and O be rescaled in each (both together: 1 x 8192, 32 / 8 heads,
