@@ -413,3 +413,21 @@ def test_scales_of_any_size(d, scale, cap):
     got = _run(q, k, v, do, softcap=cap, scale=scale)
     _status_ok()
     _close(got, attention64(q, k, v, _see(S, S, True), scale, cap, None, do))
+
+
+@pytest.mark.parametrize("d", [8, 24, 32, 40, 64, 72, 80, 96, 104, 128])
+@pytest.mark.parametrize("B,S,hq,hkv,docs", [(2, 1300, 8, 2, 0), (3, 400, 4, 4, 60)])
+def test_query_gradients_of_every_head_size(B, S, hq, hkv, docs, d):
+    """dQ leaves in pieces of 32 columns, an odd or even number of them, through two places in turn."""
+    from lightron_b200.ops import functional as OF
+    q, k, v, do = _rand(B, S, hq, d, seed=1), _rand(B, S, hkv, d, seed=2), _rand(B, S, hkv, d, seed=3), _rand(B, S, hq, d, seed=4)
+    mask, see = None, _see(S, S, True)
+    if docs:
+        ids = documents(B, S, docs, seed=7)
+        mask = OF.attention_mask(documents=ids.cuda())
+        at = torch.arange(S, device="cuda")
+        see = (at >= mask.q_bounds[..., :1]) & (at < mask.q_bounds[..., 1:])
+    want = attention64(q, k, v, see, d ** -0.5, 0.0, None, do)
+    for _ in range(8):
+        _close(_run(q, k, v, do, mask=mask), want)
+    _status_ok()
