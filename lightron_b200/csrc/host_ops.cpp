@@ -17,6 +17,7 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <algorithm>
@@ -387,6 +388,15 @@ void put_strides(L* at, const Tensor& t) {
 }
 P ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
+// Gradients of a node's backward.  Where they are to be differentiated themselves (create_graph), an error in place of that: as constants their part would silently be missing.
+variable_list only_once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& g : grads)
+    if (g.defined()) g = g.detach().set_requires_grad(true);
+  auto err = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function whose gradients are made by kernels", (int64_t)grads.size());
+  return (*err)(std::move(grads));
+}
+
 struct MaskedArgs { bool causal, grad; double scale, softcap; };      // one argument to autograd
 struct MaskedAttention : Function<MaskedAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q0, const Tensor& k0, const Tensor& v0, const std::optional<Tensor>& slopes, const std::optional<Tensor>& qb,
@@ -435,7 +445,7 @@ struct MaskedAttention : Function<MaskedAttention> {
     LB_CALL(lb_masked_attn_bwd, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.const_data_ptr(), lo.const_data_ptr(), dout.const_data_ptr(), lse.const_data_ptr(),
             ws.mutable_data_ptr(), bytes, dq.mutable_data_ptr(), dk.mutable_data_ptr(), dv.mutable_data_ptr(), m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d, st, m.scale, m.causal,
             (float)ctx->saved_data["softcap"].toDouble(), ptr(sl), ptr(qi), ptr(ki), stream());
-    return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
+    return only_once({dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
@@ -466,7 +476,7 @@ struct RopeAxes : Function<RopeAxes> {
     const Tensor pos = operand(s[2], g, n[1], g.size(1), at::kInt);
     TORCH_CHECK(pos.dim() == n[2], "positions saved for backward have come back with another shape");
     const std::string axes = ctx->saved_data["axes"].toStringRef();
-    return {turn(g, cos, sin, pos, reinterpret_cast<const unsigned char*>(axes.data()), 1), Tensor(), Tensor(), Tensor(), Tensor()};
+    return only_once({turn(g, cos, sin, pos, reinterpret_cast<const unsigned char*>(axes.data()), 1), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 

@@ -431,3 +431,20 @@ def test_query_gradients_of_every_head_size(B, S, hq, hkv, docs, d):
     for _ in range(8):
         _close(_run(q, k, v, do, mask=mask), want)
     _status_ok()
+
+
+def test_gradients_of_gradients_are_refused(monkeypatch):
+    """With ``create_graph`` the gradients say that they cannot be differentiated again; as constants they would be left out of a sum's gradient."""
+    from lightron_b200.ops import functional as OF
+    from lightron_b200.ops import native
+    from lightron_b200.ops import reference as ref
+    cos, sin = ref.rope_tables(64, 64, device="cuda")
+    pos = torch.arange(40, device="cuda", dtype=torch.int32)[None]
+    q = _rand(1, 40, 2, 64, seed=1).requires_grad_()
+    for host in (True, False):
+        if not host:
+            monkeypatch.setattr(native, "_HOST", None)
+        for call in (lambda: OF.masked_attention(q, q, q), lambda: OF.rope_axes(q, cos, sin, pos, [0] * 32)):
+            g, = torch.autograd.grad(call().float().square().sum(), q, create_graph=True)
+            with pytest.raises(RuntimeError, match="differentiate twice"):
+                (g.float().square().sum() + q.float().sum()).backward()
