@@ -434,7 +434,6 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     const int quad = warp & 3;
     const uint32_t tdq = tmem_base + ((uint32_t)(quad * 32) << 16) + C::COL_DQ;
     uint8_t* stg = smem + C::OFF_STG + quad * 2 * C::STG_BYTES;
-    [[maybe_unused]] int turn = 0;                  // the two places in turn, over all blocks: a block may have an odd number of chunks
     bool ok = true;
     int h = h_first, mb = mb_start;
     for (int it = 0; it < total_it; it++) {
@@ -461,9 +460,12 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
 #pragma unroll
         for (int c = 0; c < D / 32; c++) {
           if (c * 32 >= p.d) break;
-          uint8_t* sp = stg + turn * C::STG_BYTES;
-          turn ^= 1;
-          if (lane == 0) bulk_wait_read_but<1>();      // this half of the staging has been read
+          uint8_t* sp = stg + (c & 1) * C::STG_BYTES;
+          // This half of the staging has been read.  (Where a block has an odd number of chunks, its first waits for both halves: the last block's last chunk left from the same one.
+          // Counting the halves through all blocks instead took registers: 68 -> 96 bytes spilled at 128 columns, in parts.)
+          if (lane == 0) {
+            if (c == 0 && ((p.d + 31) & 32)) bulk_wait_read_but<0>(); else bulk_wait_read_but<1>();
+          }
           __syncwarp();
 #pragma unroll
           for (int k = 0; k < 8; k++)
