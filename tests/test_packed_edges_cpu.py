@@ -77,9 +77,6 @@ def test_positions_outside_the_tables(outside):
     assert torch.equal(torch.isnan(dx), away)
 
 
-# ---- a model whose rotary positions have several axes, on plain text ---------------------------------
-
-
 def _model(**kw):
     from lightron_b200 import mesh
     from lightron_b200.config import ModelArgs
@@ -129,9 +126,6 @@ def test_trainer_takes_rope_sections():
                                                      "dtype": "fp32", "log_interval": 1000}}, env={}))
         losses.append([float(trainer.train_step()) for _ in range(2)])
     assert losses[1] == pytest.approx(losses[0], rel=1e-5)
-
-
-# ---- the sharded engine over library collectives -------------------------------------------------------
 
 
 def _engine(dist_kw, clip):

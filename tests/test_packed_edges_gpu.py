@@ -43,9 +43,6 @@ def _close(got, want, bound=5e-3):
         assert rel(g, w) < bound, (name, rel(g, w))
 
 
-# ---- norm and clipping ---------------------------------------------------------------------------------
-
-
 def _norm64(ts):
     return sum(t.double().square().sum() for t in ts).sqrt().item()
 
@@ -108,9 +105,6 @@ def test_second_device_of_a_process():
     assert all(torch.equal(outs[0][i], outs[1][i]) for i in (0, 2, 3))
 
 
-# ---- slopes below zero ------------------------------------------------------------------------------
-
-
 RISING = [-0.01, -0.3, -1.3, -1.4, -5.0, 0.25]
 
 
@@ -162,9 +156,6 @@ def test_text_counts_on_all_axes():
     want = both(text.expand(3, B, S).contiguous(), axes=axes)
     for got in (both(None, axes=axes), both(text, axes=axes), both(text.long(), axes=axes), both(text.expand(3, S), axes=axes), both(None)):
         assert torch.equal(got[0], want[0]) and rel(got[1], want[1]) < 2e-3         # (dq is added up as key tiles come)
-
-
-# ---- packed_attention_qkv writes to its argument -----------------------------------------------------
 
 
 def _packed(B=1, S=40, hq=2, hkv=1, d=64):
@@ -269,9 +260,6 @@ def test_whole_numbers_beyond_32_bits():
     assert torch.equal(mask.q_bounds.cpu(), want[0]) and torch.equal(mask.k_bounds.cpu(), want[1])
 
 
-# ---- caps near zero ---------------------------------------------------------------------------------
-
-
 @pytest.mark.parametrize("cap", [1e-6, 1e-9, 1e-20])
 @pytest.mark.parametrize("d", [64, 128])
 def test_caps_near_zero(d, cap):
@@ -284,9 +272,6 @@ def test_caps_near_zero(d, cap):
     _close(got, attention64(q, k, v, _see(S, S, True), d ** -0.5, cap, None, do))
 
 
-# ---- rotation -----------------------------------------------------------------------------------------
-
-
 def test_rope_axes_tables_of_any_alignment():
     from lightron_b200.ops import functional as OF
     from lightron_b200.ops import reference as ref
@@ -297,9 +282,6 @@ def test_rope_axes_tables_of_any_alignment():
     pos = torch.arange(20, device="cuda", dtype=torch.int32).expand(2, 20).contiguous()
     x = _rand(1, 20, 3, 64)
     assert torch.equal(OF.rope_axes(x, c, s, pos, [0, 1] * 16), OF.rope_axes(x, cos, sin, pos, [0, 1] * 16))
-
-
-# ---- hidden scores out of range ---------------------------------------------------------------------
 
 
 @pytest.mark.parametrize("cap,alibi", [(0.0, False), (0.0, True), (30.0, False), (200.0, True)])
@@ -320,9 +302,6 @@ def test_hidden_scores_out_of_range(cap, alibi):
         n = part.stop - part.start
         want = attention64(q[:, part], k[:, part], v[:, part], _see(n, n, True), d ** -0.5, cap, slopes, do[:, part])
         _close([g[:, part] for g in got], want)
-
-
-# ---- heads in several groups ------------------------------------------------------------------------
 
 
 def test_heads_in_several_groups_forward():
@@ -348,9 +327,6 @@ def test_heads_in_several_groups_backward():
     got = _run(q, k, v, do)
     _status_ok()
     _close(got, attention64(q, k, v, _see(S, S, True), d ** -0.5, 0.0, None, do))
-
-
-# ---- two streams at a time --------------------------------------------------------------------------
 
 
 def test_two_streams_at_a_time():
