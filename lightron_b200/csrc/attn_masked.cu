@@ -124,8 +124,17 @@ int fill(MaParams& p, const void* q, const void* k, const void* v, void* o, void
   if (!q || !k || !v || !o || (!o_lo) != (!lse) || !st || !(softcap >= 0.f && softcap < INFINITY) || !(scale > 0.f && scale < INFINITY) || (!q_bounds) != (!k_bounds)) return LB_ERR_ARG;
   if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(o) || misaligned(o_lo)) return LB_ERR_ARG;
   p = MaParams{(const bf16*)q, (const bf16*)k, (const bf16*)v, strides_at(st), strides_at(st + 3), strides_at(st + 6), (bf16*)o, (bf16*)o_lo, (float*)lse, B, Sq, Sk, hq, hkv, d,
-               scale, causal, softcap, (const float*)slopes, (const int2*)q_bounds, (const int2*)k_bounds};
+               scale, causal, softcap, (const float*)slopes, (const int2*)q_bounds, (const int2*)k_bounds, 0, 0};
   return bad_strides(p.qs) || bad_strides(p.ks) || bad_strides(p.vs) ? LB_ERR_SHAPE : LB_OK;
+}
+
+// A window over all keys is none.  (Sums of a place and the window have to stay in 32 bits.)
+int set_window(MaParams& p, int window, int sinks) {
+  if (window <= 0 || sinks < 0) return LB_ERR_ARG;
+  if (p.Sk > (1 << 29)) return LB_ERR_SHAPE;
+  p.window = window < p.Sk ? window : 0;
+  p.sinks = !p.window ? 0 : sinks < p.Sk ? sinks : p.Sk;
+  return LB_OK;
 }
 
 }  // namespace
@@ -176,6 +185,24 @@ extern "C" int lb_masked_attn_fwd(const void* q, const void* k, const void* v, v
   return ma_launch_fwd(p, ws, ws ? ws_bytes : 0, (cudaStream_t)stream);
 }
 
+// The forward under a window: of the keys of its interval a query sees those less than `window` (1 or more) positions away, and the first `sinks` of the interval.  The rest as in
+// lb_masked_attn_fwd(), with a workspace of lb_window_attn_fwd_ws_bytes().
+extern "C" long long lb_window_attn_fwd_ws_bytes(int B, int Sq, int Sk, int hq, int hkv, int d, int causal, int window, int sinks) {
+  MaParams p{};
+  if (check_sizes(B, Sq, Sk, hq, hkv, d)) return 0;
+  p.B = B; p.Sq = Sq; p.Sk = Sk; p.hq = hq; p.hkv = hkv; p.d = d; p.causal = causal;
+  return set_window(p, window, sinks) ? 0 : ma_fwd_ws_bytes(p);
+}
+extern "C" int lb_window_attn_fwd(const void* q, const void* k, const void* v, void* o, void* o_lo, void* lse, void* ws, long long ws_bytes, int B, int Sq, int Sk, int hq, int hkv,
+                                  int d, const long long* strides, float scale, int causal, float softcap, const void* slopes, const void* q_bounds, const void* k_bounds, int window, int sinks,
+                                  void* stream) {
+  MaParams p;
+  if (const int rc = fill(p, q, k, v, o, o_lo, lse, B, Sq, Sk, hq, hkv, d, strides, scale, causal, softcap, slopes, q_bounds, k_bounds)) return rc;
+  if (const int rc = set_window(p, window, sinks)) return rc;
+  if (misaligned(ws)) return LB_ERR_ARG;
+  return (p.window ? ma_launch_window_fwd : ma_launch_fwd)(p, ws, ws ? ws_bytes : 0, (cudaStream_t)stream);
+}
+
 // Bytes of the backward's workspace; 0 for sizes that it does not take.
 extern "C" long long lb_masked_attn_bwd_ws_bytes(int B, int Sq, int Sk, int hq, int hkv, int d, int causal) {
   MaParams p{};
@@ -184,16 +211,39 @@ extern "C" long long lb_masked_attn_bwd_ws_bytes(int B, int Sq, int Sk, int hq, 
   return ma_bwd_ws_bytes(p);
 }
 
-// Backward.  strides: 7 x {batch, token, head} of q, k, v, dout, dq, dk, dv; o, o_lo, lse as the forward left them; ws: lb_masked_attn_bwd_ws_bytes(), 16-byte aligned.
-extern "C" int lb_masked_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_lo, const void* dout, const void* lse, void* ws, long long ws_bytes,
-                                  void* dq, void* dk, void* dv, int B, int Sq, int Sk, int hq, int hkv, int d, const long long* strides, float scale, int causal, float softcap,
-                                  const void* slopes, const void* q_bounds, const void* k_bounds, void* stream) {
+namespace {
+int backward(const void* q, const void* k, const void* v, const void* o, const void* o_lo, const void* dout, const void* lse, void* ws, long long ws_bytes, void* dq, void* dk, void* dv, int B, int Sq,
+             int Sk, int hq, int hkv, int d, const long long* strides, float scale, int causal, float softcap, const void* slopes, const void* q_bounds, const void* k_bounds, bool windowed, int window,
+             int sinks, void* stream) {
   MaBwdParams w;
   if (const int rc = fill(w.f, q, k, v, const_cast<void*>(o), const_cast<void*>(o_lo), const_cast<void*>(lse), B, Sq, Sk, hq, hkv, d, strides, scale, causal, softcap, slopes, q_bounds, k_bounds)) return rc;
+  if (windowed)
+    if (const int rc = set_window(w.f, window, sinks)) return rc;
   if (!o_lo || !dout || !ws || !dq || !dk || !dv || misaligned(dout) || misaligned(ws) || misaligned(dq) || misaligned(dk) || misaligned(dv)) return LB_ERR_ARG;
   if (ws_bytes < ma_bwd_ws_bytes(w.f)) return LB_ERR_CAPACITY;
   w.dout = (const bf16*)dout; w.dq = (bf16*)dq; w.dk = (bf16*)dk; w.dv = (bf16*)dv; w.stats = (float*)ws;
   w.dos = strides_at(strides + 9); w.dqs = strides_at(strides + 12); w.dks = strides_at(strides + 15); w.dvs = strides_at(strides + 18);
   if (bad_strides(w.dos) || bad_strides(w.dqs) || bad_strides(w.dks) || bad_strides(w.dvs)) return LB_ERR_SHAPE;
   return ma_launch_bwd(w, (cudaStream_t)stream);
+}
+}  // namespace
+
+// Backward.  strides: 7 x {batch, token, head} of q, k, v, dout, dq, dk, dv; o, o_lo, lse as the forward left them; ws: lb_masked_attn_bwd_ws_bytes(), 16-byte aligned.
+extern "C" int lb_masked_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_lo, const void* dout, const void* lse, void* ws, long long ws_bytes,
+                                  void* dq, void* dk, void* dv, int B, int Sq, int Sk, int hq, int hkv, int d, const long long* strides, float scale, int causal, float softcap,
+                                  const void* slopes, const void* q_bounds, const void* k_bounds, void* stream) {
+  return backward(q, k, v, o, o_lo, dout, lse, ws, ws_bytes, dq, dk, dv, B, Sq, Sk, hq, hkv, d, strides, scale, causal, softcap, slopes, q_bounds, k_bounds, false, 0, 0, stream);
+}
+
+// Under a window, as lb_window_attn_fwd(); ws: lb_window_attn_bwd_ws_bytes().
+extern "C" long long lb_window_attn_bwd_ws_bytes(int B, int Sq, int Sk, int hq, int hkv, int d, int causal, int window, int sinks) {
+  MaParams p{};
+  if (check_sizes(B, Sq, Sk, hq, hkv, d)) return 0;
+  p.B = B; p.Sq = Sq; p.Sk = Sk; p.hq = hq; p.hkv = hkv; p.d = d; p.causal = causal;
+  return set_window(p, window, sinks) ? 0 : ma_bwd_ws_bytes(p);
+}
+extern "C" int lb_window_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_lo, const void* dout, const void* lse, void* ws, long long ws_bytes,
+                                  void* dq, void* dk, void* dv, int B, int Sq, int Sk, int hq, int hkv, int d, const long long* strides, float scale, int causal, float softcap,
+                                  const void* slopes, const void* q_bounds, const void* k_bounds, int window, int sinks, void* stream) {
+  return backward(q, k, v, o, o_lo, dout, lse, ws, ws_bytes, dq, dk, dv, B, Sq, Sk, hq, hkv, d, strides, scale, causal, softcap, slopes, q_bounds, k_bounds, true, window, sinks, stream);
 }

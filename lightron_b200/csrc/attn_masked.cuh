@@ -5,6 +5,8 @@
 // and the softmax of row i runs over the keys lo <= j < hi of its interval.  Documents, prefixes and causality all make such intervals, whose ends
 // never fall from one row to the next; the rows that see a key are then an interval too.  So a tile's keys follow from its first and last row,
 // a mask costs two comparisons in the tiles where an interval ends, and nothing anywhere else.
+// Under a window a row sees of its interval the keys less than `window` positions away, again an interval whose ends never fall, and the first `sinks` keys, which are those of
+// its document.  The rows that see a key stay one interval: all of the document's, where the key is one of its sinks.
 #pragma once
 #include "common.cuh"
 
@@ -21,6 +23,7 @@ struct MaParams {
   float softcap;                 // 0: none
   const float* slopes;           // null, or [hq]
   const int2 *qb, *kb;           // null, or [B, Sk]: keys that a position sees, positions that see a key
+  int window, sinks;             // 0: no window; else of those keys the ones less than `window` positions away, and the first `sinks` (both up to Sk)
 };
 
 struct MaBwdParams {
@@ -41,6 +44,7 @@ struct MaOnce {
   }
 };
 
+int ma_launch_window_fwd(const MaParams& p, void* ws, long long ws_bytes, cudaStream_t s);
 int ma_launch_fwd(const MaParams& p, void* ws, long long ws_bytes, cudaStream_t s);
 long long ma_fwd_ws_bytes(const MaParams& p);
 int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s);
@@ -94,12 +98,29 @@ __device__ __forceinline__ int2 ma_keys(const MaParams& p, int b, int i) {
   if (p.qb) return p.qb[(long long)b * p.Sk + at];
   return make_int2(0, p.causal ? at + 1 : p.Sk);
 }
-// Queries [x, y) that see key j.
-__device__ __forceinline__ int2 ma_queries(const MaParams& p, int b, int j) {
+// The same under a window: those near enough, and the sinks.  (A row of padding has an empty interval at its own place, and sees neither.)
+struct MaSees { int2 near, first; };
+__device__ __forceinline__ MaSees ma_sees(const MaParams& p, int b, int i) {
+  const int2 k = ma_keys(p, b, i);
+  const int at = i + p.Sk - p.Sq;
+  return MaSees{make_int2(max(k.x, at - p.window + 1), min(k.y, at + p.window)), make_int2(k.x, min(k.x + p.sinks, k.y))};
+}
+// First key of the document of key j.
+__device__ __forceinline__ int ma_start(const MaParams& p, int b, int j) { return p.qb ? p.qb[(long long)b * p.Sk + j].x : 0; }
+// Queries [x, y) that see key j, by its interval alone or under the window.
+__device__ __forceinline__ int2 ma_queries_all(const MaParams& p, int b, int j) {
   const int off = p.Sk - p.Sq;
   if (p.kb) {
     const int2 r = p.kb[(long long)b * p.Sk + j];
     return make_int2(max(r.x - off, 0), max(r.y - off, 0));
   }
   return make_int2(p.causal ? max(j - off, 0) : 0, p.Sq);
+}
+__device__ __forceinline__ int2 ma_queries(const MaParams& p, int b, int j) {
+  int2 r = ma_queries_all(p, b, j);
+  if (p.window && j >= ma_start(p, b, j) + p.sinks) {
+    const int at = j - (p.Sk - p.Sq);
+    r = make_int2(max(r.x, at - p.window + 1), max(min(r.y, at + p.window), 0));
+  }
+  return r;
 }

@@ -81,7 +81,10 @@ enum : int { WHOLE, PARTS, ALONE };
 // Query blocks of one head that see a key block: [x, y).
 __device__ __forceinline__ int2 query_blocks(const MaParams& p, int b, int n0, bool alone) {
   if (alone) return make_int2(0, (p.Sq + 127) / 128);      // (all are written)
-  const int lo = ma_queries(p, b, n0).x, hi = min(ma_queries(p, b, min(n0 + 128, p.Sk) - 1).y, p.Sq);
+  const int lo = ma_queries(p, b, n0).x, last = min(n0 + 128, p.Sk) - 1;
+  // (the first key's queries begin first, the last one's end last; but where the last one's document has sinks in the block, all of the document sees those)
+  const bool sinks = p.window && ma_start(p, b, last) + p.sinks > n0;
+  const int hi = min((sinks ? ma_queries_all(p, b, last) : ma_queries(p, b, last)).y, p.Sq);
   return hi > lo ? make_int2(lo / 128, (hi + 127) / 128) : make_int2(0, 0);
 }
 

@@ -61,6 +61,10 @@ struct Api {
   int (*lb_masked_attn_fwd)(P, P, P, W, W, W, W, L, int, int, int, int, int, int, const L*, float, int, float, P, P, P, W);
   L (*lb_masked_attn_bwd_ws_bytes)(int, int, int, int, int, int, int);
   int (*lb_masked_attn_bwd)(P, P, P, P, P, P, P, W, L, W, W, W, int, int, int, int, int, int, const L*, float, int, float, P, P, P, W);
+  L (*lb_window_attn_fwd_ws_bytes)(int, int, int, int, int, int, int, int, int);
+  int (*lb_window_attn_fwd)(P, P, P, W, W, W, W, L, int, int, int, int, int, int, const L*, float, int, float, P, P, P, int, int, W);
+  L (*lb_window_attn_bwd_ws_bytes)(int, int, int, int, int, int, int, int, int);
+  int (*lb_window_attn_bwd)(P, P, P, P, P, P, P, W, L, W, W, W, int, int, int, int, int, int, const L*, float, int, float, P, P, P, int, int, W);
   int (*lb_rope_axes)(P, W, P, P, P, const unsigned char*, int, int, int, int, int, int, const L*, L, L, int, W);
   int (*lb_grad_norm_parts)(int);
   int (*lb_grad_squares)(int, const P*, const L*, const int*, W, int, int*, W);
@@ -397,7 +401,7 @@ variable_list only_once(variable_list grads) {
   return (*err)(std::move(grads));
 }
 
-struct MaskedArgs { bool causal, grad; double scale, softcap; };      // one argument to autograd
+struct MaskedArgs { bool causal, grad; double scale, softcap; int window, sinks; };      // one argument to autograd; window 0: none
 struct MaskedAttention : Function<MaskedAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q0, const Tensor& k0, const Tensor& v0, const std::optional<Tensor>& slopes, const std::optional<Tensor>& qb,
                         const std::optional<Tensor>& kb, MaskedArgs a) {
@@ -410,16 +414,22 @@ struct MaskedAttention : Function<MaskedAttention> {
     }
     L st[9];
     put_strides(st, q); put_strides(st + 3, k); put_strides(st + 6, v);
-    const L bytes = api.lb_masked_attn_fwd_ws_bytes(m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d);
+    const L bytes = a.window ? api.lb_window_attn_fwd_ws_bytes(m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d, m.causal, a.window, a.sinks) : api.lb_masked_attn_fwd_ws_bytes(m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d);
     Tensor ws;
     if (bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte));
-    LB_CALL(lb_masked_attn_fwd, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.mutable_data_ptr(), const_cast<W>(ptr(lo)), const_cast<W>(ptr(lse)), const_cast<W>(ptr(ws)), bytes, m.B, m.Sq, m.Sk, m.hq,
-            m.hkv, m.d, st, m.scale, m.causal, (float)a.softcap, ptr(sl), ptr(qi), ptr(ki), stream());
+    if (a.window)
+      LB_CALL(lb_window_attn_fwd, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.mutable_data_ptr(), const_cast<W>(ptr(lo)), const_cast<W>(ptr(lse)), const_cast<W>(ptr(ws)), bytes, m.B,
+              m.Sq, m.Sk, m.hq, m.hkv, m.d, st, m.scale, m.causal, (float)a.softcap, ptr(sl), ptr(qi), ptr(ki), a.window, a.sinks, stream());
+    else
+      LB_CALL(lb_masked_attn_fwd, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.mutable_data_ptr(), const_cast<W>(ptr(lo)), const_cast<W>(ptr(lse)), const_cast<W>(ptr(ws)), bytes, m.B, m.Sq, m.Sk, m.hq,
+              m.hkv, m.d, st, m.scale, m.causal, (float)a.softcap, ptr(sl), ptr(qi), ptr(ki), stream());
     if (a.grad) {
       ctx->save_for_backward({q0, k0, v0, o, lo, lse, sl, qi, ki});
       ctx->saved_data["causal"] = a.causal;
       ctx->saved_data["scale"] = a.scale;
       ctx->saved_data["softcap"] = a.softcap;
+      ctx->saved_data["window"] = (int64_t)a.window;
+      ctx->saved_data["sinks"] = (int64_t)a.sinks;
     }
     return o;
   }
@@ -437,14 +447,21 @@ struct MaskedAttention : Function<MaskedAttention> {
     const Tensor sl = s[6].defined() ? operand(s[6], g, m.hq, m.hq, at::kFloat) : Tensor(), qi = s[7].defined() ? operand(s[7], g, ends, 2, at::kInt) : Tensor();
     const Tensor ki = s[8].defined() ? operand(s[8], g, ends, 2, at::kInt) : Tensor();
     Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(k.sizes(), k.options());
-    const L bytes = api.lb_masked_attn_bwd_ws_bytes(m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d, m.causal);
+    const int window = (int)ctx->saved_data["window"].toInt(), sinks = (int)ctx->saved_data["sinks"].toInt();
+    const float softcap = (float)ctx->saved_data["softcap"].toDouble();
+    const L bytes = window ? api.lb_window_attn_bwd_ws_bytes(m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d, m.causal, window, sinks) : api.lb_masked_attn_bwd_ws_bytes(m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d, m.causal);
     Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
     L st[21];
     const Tensor* ts[7] = {&q, &k, &v, &dout, &dq, &dk, &dv};
     for (int i = 0; i < 7; i++) put_strides(st + 3 * i, *ts[i]);
-    LB_CALL(lb_masked_attn_bwd, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.const_data_ptr(), lo.const_data_ptr(), dout.const_data_ptr(), lse.const_data_ptr(),
-            ws.mutable_data_ptr(), bytes, dq.mutable_data_ptr(), dk.mutable_data_ptr(), dv.mutable_data_ptr(), m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d, st, m.scale, m.causal,
-            (float)ctx->saved_data["softcap"].toDouble(), ptr(sl), ptr(qi), ptr(ki), stream());
+    if (window)
+      LB_CALL(lb_window_attn_bwd, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.const_data_ptr(), lo.const_data_ptr(), dout.const_data_ptr(), lse.const_data_ptr(),
+              ws.mutable_data_ptr(), bytes, dq.mutable_data_ptr(), dk.mutable_data_ptr(), dv.mutable_data_ptr(), m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d, st, m.scale, m.causal,
+              softcap, ptr(sl), ptr(qi), ptr(ki), window, sinks, stream());
+    else
+      LB_CALL(lb_masked_attn_bwd, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.const_data_ptr(), lo.const_data_ptr(), dout.const_data_ptr(), lse.const_data_ptr(),
+              ws.mutable_data_ptr(), bytes, dq.mutable_data_ptr(), dk.mutable_data_ptr(), dv.mutable_data_ptr(), m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d, st, m.scale, m.causal,
+              softcap, ptr(sl), ptr(qi), ptr(ki), stream());
     return only_once({dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
@@ -848,10 +865,12 @@ PyObject* py_attention_mask(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// masked_attention(q, k, v, q_bounds or None, k_bounds or None, slopes or None, causal, scale or None, softcap)
+constexpr int64_t MAX_WINDOW_LENGTH = 1 << 29;
+
+// masked_attention(q, k, v, q_bounds or None, k_bounds or None, slopes or None, causal, scale or None, softcap, window or None, sinks)
 PyObject* py_masked_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 9 || !unobserved()) LB_NOT_PLAIN;
+  if (n != 11 || !unobserved()) LB_NOT_PLAIN;
   const Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]);
   if (!plain(q, false) || !plain(k, false) || !plain(v, false) || q->dim() != 4 || k->dim() != 4 || !v->sizes().equals(k->sizes()) || !here(*q) || k->device() != q->device() ||
       v->device() != q->device())
@@ -875,7 +894,23 @@ PyObject* py_masked_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     LB_NOT_PLAIN;
   }
   if (!(scale >= FLT_MIN && scale <= FLT_MAX) || !(softcap == 0.0 || (softcap >= FLT_MIN && softcap <= FLT_MAX))) LB_NOT_PLAIN;
-  const MaskedArgs m{a[6] == Py_True, at::GradMode::is_enabled() && (q->requires_grad() || k->requires_grad() || v->requires_grad()), scale, softcap};
+  int64_t window = 0, sinks = 0;
+  if (a[9] != Py_None) {
+    if (!PyLong_CheckExact(a[9]) || !PyLong_CheckExact(a[10])) LB_NOT_PLAIN;
+    window = PyLong_AsLongLong(a[9]);
+    sinks = PyLong_AsLongLong(a[10]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      LB_NOT_PLAIN;
+    }
+    if (window < 1 || sinks < 0 || Sk > MAX_WINDOW_LENGTH) LB_NOT_PLAIN;
+    if (window >= Sk) window = sinks = 0;          // all keys
+    sinks = std::min(sinks, Sk);
+  } else if (!PyLong_CheckExact(a[10]) || PyLong_AsLongLong(a[10]) != 0) {
+    PyErr_Clear();
+    LB_NOT_PLAIN;
+  }
+  const MaskedArgs m{a[6] == Py_True, at::GradMode::is_enabled() && (q->requires_grad() || k->requires_grad() || v->requires_grad()), scale, softcap, (int)window, (int)sinks};
   return THPVariable_Wrap(unlocked([&, q_ = *q, k_ = *k, v_ = *v, sl = maybe(slopes), qi = maybe(qb), ki = maybe(kb)] { return MaskedAttention::apply(q_, k_, v_, sl, qi, ki, m); }));
   END_HANDLE_TH_ERRORS
 }
@@ -1032,6 +1067,7 @@ PyObject* py_init(PyObject*, PyObject* args) {
   LB_TAKE(lb_flash_fwd_tc); LB_TAKE(lb_flash_bwd_ws_bytes_kv); LB_TAKE(lb_flash_bwd_tc_ws); LB_TAKE(lb_flash_bwd); LB_TAKE(lb_embedding_fwd); LB_TAKE(lb_clear);
   LB_TAKE(lb_embedding_bwd); LB_TAKE(lb_ce_stats); LB_TAKE(lb_ce_loss); LB_TAKE(lb_ce_grad); LB_TAKE(lb_gemm_rope);
   LB_TAKE(lb_attn_mask); LB_TAKE(lb_masked_attn_fwd_ws_bytes); LB_TAKE(lb_masked_attn_fwd); LB_TAKE(lb_masked_attn_bwd_ws_bytes); LB_TAKE(lb_masked_attn_bwd); LB_TAKE(lb_rope_axes);
+  LB_TAKE(lb_window_attn_fwd_ws_bytes); LB_TAKE(lb_window_attn_fwd); LB_TAKE(lb_window_attn_bwd_ws_bytes); LB_TAKE(lb_window_attn_bwd);
   LB_TAKE(lb_grad_norm_parts); LB_TAKE(lb_grad_squares); LB_TAKE(lb_grad_total); LB_TAKE(lb_grad_scale);
   if (!ok) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "an entry point of the kernels is missing");

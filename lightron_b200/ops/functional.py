@@ -821,7 +821,7 @@ def _strides(*ts: torch.Tensor):
     return (ctypes.c_longlong * len(flat))(*flat)
 
 
-def masked_fwd_native(q, k, v, causal: bool, scale: float, softcap: float, slopes, qb, kb, grad: bool):
+def masked_fwd_native(q, k, v, causal: bool, scale: float, softcap: float, slopes, qb, kb, grad: bool, window: int = 0, sinks: int = 0):
     """(o, what rounding o to bf16 left, lse; both None without gradients): the backward's row sums of ``do * o`` need o to more than 8 bits where a row sees
     few keys, for its score gradients are differences that then all but vanish."""
     q, k, v = _strided(q), _strided(k), _strided(v)
@@ -830,43 +830,46 @@ def masked_fwd_native(q, k, v, causal: bool, scale: float, softcap: float, slope
     o = torch.empty(B, Sq, hq, d, dtype=q.dtype, device=q.device)
     o_lo = torch.empty_like(o) if grad else None
     lse = torch.empty(B, hq, Sq, dtype=torch.float32, device=q.device) if grad else None
-    nbytes = native.require().lb_masked_attn_fwd_ws_bytes(B, Sq, Sk, hq, hkv, d)
+    lib, local = native.require(), (window, sinks) if window else ()
+    nbytes = lib.lb_window_attn_fwd_ws_bytes(B, Sq, Sk, hq, hkv, d, int(causal), *local) if window else lib.lb_masked_attn_fwd_ws_bytes(B, Sq, Sk, hq, hkv, d)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    native.call("lb_masked_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), native.ptr(o_lo), native.ptr(lse), native.ptr(ws), nbytes, B, Sq, Sk, hq, hkv, d,
-                _strides(q, k, v), scale, int(causal), softcap, native.ptr(slopes), native.ptr(qb), native.ptr(kb), native.stream_ptr())
+    native.call("lb_window_attn_fwd" if window else "lb_masked_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), native.ptr(o_lo), native.ptr(lse), native.ptr(ws), nbytes, B, Sq, Sk, hq, hkv, d,
+                _strides(q, k, v), scale, int(causal), softcap, native.ptr(slopes), native.ptr(qb), native.ptr(kb), *local, native.stream_ptr())
     return o, o_lo, lse
 
 
-def masked_bwd_native(q, k, v, o, o_lo, lse, do, causal: bool, scale: float, softcap: float, slopes, qb, kb, dq=None, dk=None, dv=None):
+def masked_bwd_native(q, k, v, o, o_lo, lse, do, causal: bool, scale: float, softcap: float, slopes, qb, kb, dq=None, dk=None, dv=None, window: int = 0, sinks: int = 0):
     q, k, v, do = _strided(q), _strided(k), _strided(v), _strided(do)
     B, Sq, hq, d = q.shape
     Sk, hkv = k.shape[1], k.shape[2]
     if dq is None:
         dq, dk, dv = torch.empty_like(o), torch.empty(B, Sk, hkv, d, dtype=q.dtype, device=q.device), torch.empty(B, Sk, hkv, d, dtype=q.dtype, device=q.device)
-    ws = torch.empty(native.require().lb_masked_attn_bwd_ws_bytes(B, Sq, Sk, hq, hkv, d, int(causal)), dtype=torch.uint8, device=q.device)
-    native.call("lb_masked_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), o_lo.data_ptr(), do.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(),
+    lib, local = native.require(), (window, sinks) if window else ()
+    nbytes = (lib.lb_window_attn_bwd_ws_bytes if window else lib.lb_masked_attn_bwd_ws_bytes)(B, Sq, Sk, hq, hkv, d, int(causal), *local)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    native.call("lb_window_attn_bwd" if window else "lb_masked_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), o_lo.data_ptr(), do.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(),
                 dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, Sq, Sk, hq, hkv, d, _strides(q, k, v, do, dq, dk, dv), scale, int(causal), softcap,
-                native.ptr(slopes), native.ptr(qb), native.ptr(kb), native.stream_ptr())
+                native.ptr(slopes), native.ptr(qb), native.ptr(kb), *local, native.stream_ptr())
     return dq, dk, dv
 
 
 class _MaskedAttn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, slopes, qb, kb, causal, scale, softcap):
+    def forward(ctx, q, k, v, slopes, qb, kb, causal, scale, softcap, window, sinks):
         with native.on_device(q):
-            o, o_lo, lse = masked_fwd_native(q, k, v, causal, scale, softcap, slopes, qb, kb, not isinstance(ctx, _NoGradCtx) and any(ctx.needs_input_grad[:3]))
+            o, o_lo, lse = masked_fwd_native(q, k, v, causal, scale, softcap, slopes, qb, kb, not isinstance(ctx, _NoGradCtx) and any(ctx.needs_input_grad[:3]), window, sinks)
         ctx.save_for_backward(q, k, v, o, o_lo, lse, slopes, qb, kb)
-        ctx.args = (causal, scale, softcap)
+        ctx.args = (causal, scale, softcap, window, sinks)
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
         q, k, v, o, o_lo, lse, slopes, qb, kb = ctx.saved_tensors
-        causal, scale, softcap = ctx.args
+        causal, scale, softcap, window, sinks = ctx.args
         with native.on_device(q):
-            dq, dk, dv = masked_bwd_native(q, k, v, o, o_lo, lse, do, causal, scale, softcap, slopes, qb, kb)
-        return dq, dk, dv, None, None, None, None, None, None
+            dq, dk, dv = masked_bwd_native(q, k, v, o, o_lo, lse, do, causal, scale, softcap, slopes, qb, kb, window=window, sinks=sinks)
+        return (dq, dk, dv) + (None,) * 8
 
 
 MASKED_MAX_HEAD_DIM = 128
@@ -905,27 +908,46 @@ def _check_masked(q, k, v, mask, causal, scale, softcap, slopes) -> bool:
     return True if causal is None else bool(causal)
 
 
+def _check_window(window: Optional[int], sinks: int, length: int) -> Tuple[int, int]:
+    """Refuses what is no window; returns it with its sinks as the kernels take them: 0 for none, or one over all keys."""
+    for name, n in (("window", window), ("sinks", sinks)):
+        if n is not None and (not isinstance(n, int) or isinstance(n, bool)):
+            raise ValueError(f"{name} must be a whole number, got {n!r}")
+    if (window is not None and window < 1) or sinks is None or sinks < 0:
+        raise ValueError(f"window must be None or at least 1 and sinks at least 0, got {window} and {sinks}")
+    if window is None and sinks:
+        raise ValueError(f"{sinks} sinks have a meaning under a window only")
+    return (0, 0) if window is None or window >= length else (window, min(sinks, length))
+
+
+MAX_WINDOW_LENGTH = 1 << 29
+
+
 def _check_masked_native(d: int) -> None:
     if d % 8 or not 0 < d <= MASKED_MAX_HEAD_DIM:
         raise ValueError(f"masked_attention on the GPU takes head sizes that are multiples of 8 up to {MASKED_MAX_HEAD_DIM}, got {d}")
 
 
 def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[AttentionMask] = None, causal: Optional[bool] = None,
-                     scale: Optional[float] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     scale: Optional[float] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None, window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
     """softmax(s) v for q [B, Sq, hq, d] and k, v [B, Sk, hkv, d] in any order of the outer dimensions; query i sits at position i + Sk - Sq.
     ``s = softcap * tanh(x / softcap) - slopes[h] * |distance|`` with ``x = scale * q.k`` (``softcap`` 0: x itself; ``slopes`` fp32 [hq], constants of either sign).
-    ``mask``: see :func:`attention_mask`; without one, ``causal`` (default) or all keys.  Rows that see nothing give zeros, and gradients of zero."""
+    ``mask``: see :func:`attention_mask`; without one, ``causal`` (default) or all keys.  Rows that see nothing give zeros, and gradients of zero.
+    ``window``: of those keys a query sees the ones less than ``window`` positions away (its own is one of them) and the first ``sinks`` of its document, or of all keys."""
     if (host := native.host_ops()) is not None and (mask is None or (type(mask) is AttentionMask and causal in (None, mask.causal))):
         qb, kb, one_way = (None, None, causal is None or causal) if mask is None else (mask.q_bounds, mask.k_bounds, mask.causal)
-        if (o := host.masked_attention(q, k, v, qb, kb, slopes, one_way, scale, softcap)) is not NotImplemented:
+        if (o := host.masked_attention(q, k, v, qb, kb, slopes, one_way, scale, softcap, window, sinks)) is not NotImplemented:
             return o
     causal = _check_masked(q, k, v, mask, causal, scale, softcap, slopes)
+    local, first = _check_window(window, sinks, k.shape[1])
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
     qb, kb = (mask.q_bounds, mask.k_bounds) if mask is not None else (None, None)
     if native.use_native(q) and q.numel() and k.numel():
         _check_masked_native(q.shape[-1])
-        return _apply(_MaskedAttn, q, k, v, None if slopes is None else slopes.contiguous(), qb, kb, causal, scale, float(softcap))
-    return ref.masked_attention(q, k, v, qb, causal, scale, float(softcap), slopes)
+        if local and k.shape[1] > MAX_WINDOW_LENGTH:
+            raise ValueError(f"a window on the GPU takes up to {MAX_WINDOW_LENGTH} keys, got {k.shape[1]}")
+        return _apply(_MaskedAttn, q, k, v, None if slopes is None else slopes.contiguous(), qb, kb, causal, scale, float(softcap), local, first)
+    return ref.masked_attention(q, k, v, qb, causal, scale, float(softcap), slopes, local or None, first)
 
 
 # --------------------------------------------------------------------------------------
@@ -963,6 +985,11 @@ class _RopeAxes(torch.autograd.Function):
         return dx, None, None, None, None
 
 
+def _check_tables(d, cos, sin) -> None:
+    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != d // 2 or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise ValueError(f"cos and sin must be fp32 [positions, {d // 2}], got {cos.dtype} {tuple(cos.shape)} and {sin.dtype} {tuple(sin.shape)}")
+
+
 def _check_axes(B, S, d, cos, sin, positions, axes):
     """(positions as int32 with unit stride over the tokens, axes as a tuple), or refuses them."""
     axes = tuple(int(a) for a in axes)
@@ -972,8 +999,7 @@ def _check_axes(B, S, d, cos, sin, positions, axes):
         raise ValueError(f"positions must be [axes, {B}, {S}] or [axes, {S}] int32 / int64, got {positions.dtype} {tuple(positions.shape)}")
     if any(not 0 <= a < positions.shape[0] for a in axes):
         raise ValueError(f"axes {sorted(set(axes))} of positions with {positions.shape[0]} axes")
-    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != d // 2 or cos.dtype != torch.float32 or sin.dtype != torch.float32:
-        raise ValueError(f"cos and sin must be fp32 [positions, {d // 2}], got {cos.dtype} {tuple(cos.shape)} and {sin.dtype} {tuple(sin.shape)}")
+    _check_tables(d, cos, sin)
     if cos.shape[0] == 0 and positions.numel():
         raise ValueError("cos and sin have no rows")
     if not cos.device == sin.device == positions.device:
@@ -998,6 +1024,111 @@ def rope_axes(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: 
     if native.use_native(x) and x.numel() and d % 8 == 0 and d <= 256 and positions.shape[0] <= 8:
         return _apply(_RopeAxes, x, cos.contiguous(), sin.contiguous(), positions, axes)
     return ref.rope_axes(x, cos, sin, positions, axes)
+
+
+# --------------------------------------------------------------------------------------
+# Norms of queries and keys for each head, with the rotation in the same pass
+# --------------------------------------------------------------------------------------
+
+
+def _norm_rope_table(positions):
+    """(pointer, stride of an axis, stride of a sequence) of positions [A, B, S] / [A, S] int32, or of none."""
+    return (0, 0, 0) if positions is None else (positions.data_ptr(), positions.stride(0), positions.stride(1) if positions.dim() == 3 else 0)
+
+
+def _norm_rope_native(q, k, yq, yk, wq, wk, cos, sin, positions, axes, eps) -> None:
+    B, S, hq, d = q.shape
+    at, pos_a, pos_b = _norm_rope_table(positions)
+    native.call("lb_qk_norm_rope", q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(), wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), at, bytes(axes),
+                max(axes) + 1, B, S, hq, k.shape[2], d, cos.shape[0], _strides(q, k, yq, yk), pos_a, pos_b, eps, native.stream_ptr())
+
+
+def _norm_rope_bwd_native(q, k, dyq, dyk, dxq, dxk, wq, wk, cos, sin, positions, axes, eps, need_w: bool):
+    """(dwq, dwk), or None each."""
+    B, S, hq, d = q.shape
+    at, pos_a, pos_b = _norm_rope_table(positions)
+    ctas = native.require().lb_qk_norm_rope_bwd_ctas(B, S, hq, k.shape[2], d)
+    dwq, dwk, parts = (torch.empty_like(wq), torch.empty_like(wk), torch.empty(ctas, 2, d, dtype=torch.float32, device=q.device)) if need_w else (None, None, None)
+    native.call("lb_qk_norm_rope_bwd", q.data_ptr(), k.data_ptr(), dyq.data_ptr(), dyk.data_ptr(), dxq.data_ptr(), dxk.data_ptr(), wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+                at, bytes(axes), max(axes) + 1, native.ptr(parts), ctas, native.ptr(dwq), native.ptr(dwk), B, S, hq, k.shape[2], d, cos.shape[0], _strides(q, k, dyq, dyk, dxq, dxk), pos_a, pos_b,
+                eps, native.stream_ptr())
+    return dwq, dwk
+
+
+class _QKNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, cos, sin, positions, axes, eps):
+        ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
+        ctx.axes, ctx.eps = axes, eps
+        q, k, wq, wk = _strided(q), _strided(k), _row(wq), _row(wk)
+        yq, yk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        with native.on_device(q):
+            _norm_rope_native(q, k, yq, yk, wq, wk, cos, sin, positions, axes, eps)
+        return yq, yk
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dyq, dyk):
+        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
+        q, k, dyq, dyk, wq, wk = _strided(q), _strided(k), _strided(dyq), _strided(dyk), _row(wq), _row(wk)
+        dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        with native.on_device(q):
+            dwq, dwk = _norm_rope_bwd_native(q, k, dyq, dyk, dq, dk, wq, wk, cos, sin, positions, ctx.axes, ctx.eps, any(ctx.needs_input_grad[2:4]))
+        return dq, dk, dwq, dwk, None, None, None, None, None
+
+
+def _row(w: torch.Tensor) -> torch.Tensor:
+    """A vector where the kernels read it: in one piece, on 16 bytes."""
+    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
+
+
+NORM_ROPE_MAX_HEAD_DIM = 256
+
+
+def _check_norm_rope(q, k, q_weight, k_weight, cos, sin, eps) -> None:
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3] or q.dtype != k.dtype or q.device != k.device:
+        raise ValueError(f"qk_norm_rope takes q [B, S, hq, d] and k [B, S, hkv, d]; got {q.dtype} {tuple(q.shape)} on {q.device} and {k.dtype} {tuple(k.shape)} on {k.device}")
+    d = q.shape[3]
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if tuple(w.shape) != (d,) or w.dtype != q.dtype or w.device != q.device:
+            raise ValueError(f"{name} must be {q.dtype} [{d}] on {q.device}, got {w.dtype} {tuple(w.shape)} on {w.device}")
+    if cos.device != q.device:
+        raise ValueError(f"tables on {cos.device} for q and k on {q.device}")
+    if not 0.0 <= eps <= _FP32_MAX:
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: Optional[torch.Tensor] = None,
+                 axes: Optional[Sequence[int]] = None, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Every head of q [B, S, hq, d] and of k [B, S, hkv, d] (any order of the outer dimensions) divided by its root mean square, times ``q_weight`` / ``k_weight`` [d], and turned by its token's
+    position (interleaved pairs, as :func:`rope`), in one pass and rounded once.  ``positions``: None (each token's place), [S] or [B, S]; with ``axes`` None or [S], which count on all axes, [A, B, S]
+    or [A, S] (two dimensions are axes and tokens then), as :func:`packed_attention_qkv` takes them.  A position outside of the tables makes its heads NaN."""
+    _check_norm_rope(q, k, q_weight, k_weight, cos, sin, eps)
+    B, S, _, d = q.shape
+    positions, axes = _positions_of(positions, axes, B, S, d, cos, sin)
+    if native.use_native(q) and q.numel() and k.numel() and d % 8 == 0 and d <= NORM_ROPE_MAX_HEAD_DIM and max(axes, default=0) < 8:
+        return _apply(_QKNormRope, q, k, q_weight, k_weight, cos.contiguous(), sin.contiguous(), positions, axes, float(eps))
+    if positions is None:
+        positions = torch.arange(S, device=q.device, dtype=torch.int32).expand(max(axes, default=0) + 1, -1)
+    return ref.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, axes, eps)
+
+
+def _positions_of(positions, axes, B: int, S: int, d: int, cos, sin):
+    """(positions [A, B, S] or [A, S] int32, or None for each token's place, and the axis of each pair) from what :func:`qk_norm_rope` takes."""
+    if positions is None:
+        axes = (0,) * (d // 2) if axes is None else tuple(int(a) for a in axes)
+        if d % 2 or len(axes) != d // 2 or min(axes, default=0) < 0:
+            raise ValueError(f"axes name the axis of each of the {d // 2} pairs of a head, got {axes}")
+        _check_tables(d, cos, sin)
+        if cos.device != sin.device or (cos.shape[0] == 0 and B * S):
+            raise ValueError(f"cos [{cos.shape[0]} rows] and sin have no rows, or are on different devices: {cos.device}, {sin.device}")
+        return None, axes
+    if axes is None:
+        positions, axes = positions[None], (0,) * (d // 2)
+    elif positions.dim() == 1:
+        axes = tuple(axes)
+        positions = positions.expand(max(axes, default=0) + 1, -1)
+    return _check_axes(B, S, d, cos, sin, positions, axes)
 
 
 class _PackedAttnQKV(torch.autograd.Function):
@@ -1249,6 +1380,54 @@ def embedding(tokens: torch.Tensor, w: torch.Tensor, vocab_start: int = 0) -> to
     if vocab_start != 0 or bool(mask.any()):
         out = out.masked_fill(mask.unsqueeze(-1), 0.0)
     return out
+
+
+class _ScaledEmbedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, w, scale, vocab_start):
+        T, (V, H) = tokens.numel(), w.shape
+        tok, w_ = tokens.contiguous(), w.contiguous()
+        out = torch.empty(*tokens.shape, H, dtype=w.dtype, device=w.device)
+        with native.on_device(w):
+            native.call("lb_embed_scaled", tok.data_ptr(), tok.element_size(), w_.data_ptr(), out.data_ptr(), T, H, vocab_start, vocab_start + V, scale, native.stream_ptr())
+        ctx.save_for_backward(tokens)
+        ctx.args = (tuple(w.shape), scale, vocab_start)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        tokens, = ctx.saved_tensors
+        (V, H), scale, vocab_start = ctx.args
+        tok, dy = tokens.contiguous(), dy.contiguous()
+        with native.on_device(dy):
+            ws = torch.empty(native.require().lb_embed_sorted_ws_bytes(tok.numel(), H), dtype=torch.uint8, device=dy.device)
+            dw = torch.empty(V, H, dtype=dy.dtype, device=dy.device)
+            native.call("lb_embed_sorted_bwd", tok.data_ptr(), tok.element_size(), dy.data_ptr(), dw.data_ptr(), ws.data_ptr(), ws.numel(), tok.numel(), H, vocab_start, vocab_start + V, scale,
+                        native.stream_ptr())
+        return None, dw, None, None
+
+
+EMBED_MAX_TOKENS = 1 << 30
+
+
+def scaled_embedding(tokens: torch.Tensor, w: torch.Tensor, scale: float = 1.0, vocab_start: int = 0) -> torch.Tensor:
+    """``scale`` times the rows of ``w`` [V, H] that ``tokens`` (int32 / int64, any shape) name, rounded once; ids outside of [vocab_start, vocab_start + V) give zero rows and no gradient
+    (vocab-parallel partial result).  The gradient is dense; a row's sum runs over its tokens in their order, in 32 bits, and is rounded once: the same bits in every run, however
+    often an id comes (:func:`embedding` adds up in the weight's type, as it comes)."""
+    if w.dim() != 2 or not w.dtype.is_floating_point:
+        raise ValueError(f"scaled_embedding takes a weight [V, H], got {w.dtype} {tuple(w.shape)}")
+    if tokens.dtype not in (torch.int32, torch.int64) or tokens.device != w.device:
+        raise ValueError(f"tokens must be int32 or int64 on {w.device}, got {tokens.dtype} on {tokens.device}")
+    if not -_FP32_MAX <= scale <= _FP32_MAX:
+        raise ValueError(f"scale must be finite, in 32 bits, got {scale}")
+    if vocab_start < 0:
+        raise ValueError(f"vocab_start {vocab_start} is negative")
+    if native.use_native(w) and w.numel() and tokens.numel():
+        if tokens.numel() > EMBED_MAX_TOKENS:
+            raise ValueError(f"scaled_embedding on the GPU takes up to {EMBED_MAX_TOKENS} tokens, got {tokens.numel()}")
+        return _apply(_ScaledEmbedding, tokens, w, float(scale), int(vocab_start))
+    return ref.scaled_embedding(tokens, w, scale, vocab_start)
 
 
 # --------------------------------------------------------------------------------------

@@ -96,7 +96,18 @@ _SIGNATURES = {
     "lb_masked_attn_bwd": [_P] * 8 + [_L] + [_P] * 3 + [_I] * 6 + [_P, _F, _I, _F, _P, _P, _P, _P],
     "lb_masked_attn_bwd_ws_bytes": [_I] * 7,
     "lb_masked_attn_bwd_status": [_P],
+    "lb_window_attn_fwd_ws_bytes": [_I] * 9,
+    "lb_window_attn_fwd": [_P] * 7 + [_L] + [_I] * 6 + [_P, _F, _I, _F, _P, _P, _P, _I, _I, _P],
+    "lb_window_attn_status": [_P],
+    "lb_window_attn_bwd": [_P] * 8 + [_L] + [_P] * 3 + [_I] * 6 + [_P, _F, _I, _F, _P, _P, _P, _I, _I, _P],
+    "lb_window_attn_bwd_ws_bytes": [_I] * 9,
     "lb_rope_axes": [_P] * 6 + [_I] * 6 + [_P, _L, _L, _I, _P],
+    "lb_qk_norm_rope": [_P] * 9 + [_P] + [_I] * 7 + [_P, _L, _L, _F, _P],
+    "lb_qk_norm_rope_bwd_ctas": [_I] * 5,
+    "lb_qk_norm_rope_bwd": [_P] * 12 + [_I, _P, _I, _P, _P] + [_I] * 6 + [_P, _L, _L, _F, _P],
+    "lb_embed_scaled": [_P, _I, _P, _P, _I, _I, _L, _L, _F, _P],
+    "lb_embed_sorted_ws_bytes": [_I] * 2,
+    "lb_embed_sorted_bwd": [_P, _I, _P, _P, _P, _L, _I, _I, _L, _L, _F, _P],
     "lb_grad_norm_parts": [_I],
     "lb_grad_squares": [_I, _P, _P, _P, _P, _I, _P, _P],
     "lb_grad_total": [_P, _I, _P, _P, _P],
@@ -275,6 +286,7 @@ _HOST = False               # not looked for yet; then the extension module, or 
 _HOST_ENTRIES = ("lb_rmsnorm_fwd", "lb_rmsnorm_bwd_blocks", "lb_rmsnorm_bwd", "lb_rope", "lb_gemm_grouped_epi", "lb_flash_fwd_tc",
                  "lb_flash_bwd_ws_bytes_kv", "lb_flash_bwd_tc_ws", "lb_flash_bwd", "lb_embedding_fwd", "lb_clear", "lb_embedding_bwd", "lb_ce_stats",
                  "lb_ce_loss", "lb_ce_grad", "lb_gemm_rope", "lb_attn_mask", "lb_masked_attn_fwd_ws_bytes", "lb_masked_attn_fwd", "lb_masked_attn_bwd_ws_bytes", "lb_masked_attn_bwd", "lb_rope_axes",
+                 "lb_window_attn_fwd_ws_bytes", "lb_window_attn_fwd", "lb_window_attn_bwd_ws_bytes", "lb_window_attn_bwd",
                  "lb_grad_norm_parts", "lb_grad_squares", "lb_grad_total", "lb_grad_scale")
 
 
@@ -310,7 +322,7 @@ def _load_host_ops():
 _STATUS_READERS = (("lb_device_status", "GEMM / fused collective GEMM"), ("lb_gemm_grouped_status", "grouped GEMM"),
                    ("lb_gemm_split_status", "GEMM of small launches"),
                    ("lb_flash_status", "attention forward"), ("lb_flash_bwd_status", "attention backward"),
-                   ("lb_masked_attn_status", "masked attention forward"), ("lb_masked_attn_bwd_status", "masked attention backward"),
+                   ("lb_masked_attn_status", "masked attention forward"), ("lb_window_attn_status", "windowed attention forward"), ("lb_masked_attn_bwd_status", "masked attention backward"),
                    ("lb_dp_status", "data-parallel optimizer kernel"),
                    ("lb_moe_status", "expert-parallel routing / dispatch / combine"),
                    ("lb_coll_status", "stand-alone peer-memory collective"))

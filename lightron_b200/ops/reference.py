@@ -119,9 +119,9 @@ def mask_bounds(S: int, documents: Optional[torch.Tensor], prefix: Optional[torc
 
 
 def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bounds: Optional[torch.Tensor] = None, causal: bool = True,
-                     scale: Optional[float] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     scale: Optional[float] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None, window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
     """q [B, Sq, hq, d], k / v [B, Sk, hkv, d]; query i sits at position i + Sk - Sq and sees the keys of ``bounds`` [B, Sk, 2] there (None:
-    all keys, with ``causal`` those up to its own).  Scores are ``softcap * tanh(x / softcap) - slopes[h] * distance``; fp32 math."""
+    all keys, with ``causal`` those up to its own); with ``window`` of those the ones less than ``window`` positions away, and the first ``sinks``.  Scores are ``softcap * tanh(x / softcap) - slopes[h] * distance``; fp32 math."""
     B, Sq, hq, d = q.shape
     Sk, hkv = k.shape[1], k.shape[2]
     scale = 1.0 / math.sqrt(d) if scale is None else scale
@@ -140,6 +140,10 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bounds: 
     else:
         see = (key[None, :] <= at[:, None]) if causal else torch.ones(Sq, Sk, dtype=torch.bool, device=q.device)
         see = see[None, None, None]
+    if window is not None:
+        near = (at[:, None] - key[None, :]).abs() < window
+        first = bounds[:, Sk - Sq:].to(q.device)[..., :1][:, None, None] if bounds is not None else 0
+        see = see & (near | (key < first + sinks))
     s = s.masked_fill(~see, float("-inf"))
     top = s.amax(dim=-1, keepdim=True).detach() if Sk else s.new_zeros(*s.shape[:-1], 1)
     e = torch.exp(s - torch.where(top == float("-inf"), torch.zeros_like(top), top))
@@ -159,6 +163,27 @@ def rope_axes(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: 
     s = -s if inverse else s
     a, b = x.to(c.dtype)[..., 0::2], x.to(c.dtype)[..., 1::2]
     return torch.stack((a * c - b * s, a * s + b * c), dim=-1).flatten(-2).type_as(x)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, axes,
+                 eps: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Heads of q [B, S, hq, d] and k [B, S, hkv, d] normed, times their weights, and turned as by :func:`rope_axes`; rounded once."""
+    dt = torch.float64 if q.dtype == torch.float64 else torch.float32
+    out = []
+    for x, w in ((q, q_weight), (k, k_weight)):
+        xf = x.to(dt)
+        out.append(rope_axes(xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps) * w.to(dt), cos.to(dt), sin.to(dt), positions, axes).type_as(x))
+    return out[0], out[1]
+
+
+def scaled_embedding(tokens: torch.Tensor, w: torch.Tensor, scale: float, vocab_start: int = 0) -> torch.Tensor:
+    """``scale`` times rows of ``w``, rounded once; ids outside of [vocab_start, vocab_start + w.shape[0]) give zero rows.  The gradient is summed up in 32 bits at least."""
+    dt = torch.float64 if w.dtype == torch.float64 else torch.float32
+    local = tokens.long() - vocab_start
+    away = (local < 0) | (local >= w.shape[0])
+    if w.shape[0] == 0:
+        return w.new_zeros(*tokens.shape, w.shape[1])
+    return (F.embedding(local.masked_fill(away, 0), w.to(dt)) * scale).masked_fill(away.unsqueeze(-1), 0.0).type_as(w)
 
 
 def grad_sumsq(tensors) -> torch.Tensor:
