@@ -66,6 +66,12 @@ struct Api {
   L (*lb_window_attn_bwd_ws_bytes)(int, int, int, int, int, int, int, int, int);
   int (*lb_window_attn_bwd)(P, P, P, P, P, P, P, W, L, W, W, W, int, int, int, int, int, int, const L*, float, int, float, P, P, P, int, int, W);
   int (*lb_rope_axes)(P, W, P, P, P, const unsigned char*, int, int, int, int, int, int, const L*, L, L, int, W);
+  int (*lb_qk_norm_rope)(P, P, W, W, P, P, P, P, P, const unsigned char*, int, int, int, int, int, int, int, const L*, L, L, float, W);
+  int (*lb_qk_norm_rope_bwd_ctas)(int, int, int, int, int);
+  int (*lb_qk_norm_rope_bwd)(P, P, P, P, W, W, P, P, P, P, P, const unsigned char*, int, W, int, W, W, int, int, int, int, int, int, const L*, L, L, float, W);
+  int (*lb_embed_scaled)(P, int, P, W, int, int, L, L, float, W);
+  L (*lb_embed_sorted_ws_bytes)(int, int);
+  int (*lb_embed_sorted_bwd)(P, int, P, W, W, L, int, int, L, L, float, W);
   int (*lb_grad_norm_parts)(int);
   int (*lb_grad_squares)(int, const P*, const L*, const int*, W, int, int*, W);
   int (*lb_grad_total)(P, int, W, W, W);
@@ -497,6 +503,54 @@ struct RopeAxes : Function<RopeAxes> {
   }
 };
 
+// Axes that are all the first where there are none; the strides say how positions lie: [S], [B, S], [A, S] or [A, B, S].
+struct NormRope { Axes axes; L pos_a, pos_b; double eps; };      // one argument to autograd
+struct QKNormRope : Function<QKNormRope> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q0, const Tensor& k0, const Tensor& wq, const Tensor& wk, const Tensor& cos, const Tensor& sin, const std::optional<Tensor>& pos0,
+                               NormRope a) {
+    const Tensor q = fix_strides(q0), k = fix_strides(k0), pos = pos0.value_or(Tensor());
+    Tensor yq = at::empty(q.sizes(), q.options()), yk = at::empty(k.sizes(), k.options());
+    L st[12];
+    put_strides(st, q); put_strides(st + 3, k); put_strides(st + 6, yq); put_strides(st + 9, yk);
+    LB_CALL(lb_qk_norm_rope, q.const_data_ptr(), k.const_data_ptr(), yq.mutable_data_ptr(), yk.mutable_data_ptr(), wq.const_data_ptr(), wk.const_data_ptr(), cos.const_data_ptr(),
+            sin.const_data_ptr(), ptr(pos), a.axes.of, a.axes.n, (int)q.size(0), (int)q.size(1), (int)q.size(2), (int)k.size(2), (int)q.size(3), (int)cos.size(0), st, a.pos_a, a.pos_b, (float)a.eps,
+            stream());
+    ctx->save_for_backward({q0, k0, wq, wk, cos, sin, pos});
+    ctx->saved_data["axes"] = std::string(reinterpret_cast<const char*>(a.axes.of), q.size(3) / 2);
+    ctx->saved_data["sizes"] = std::vector<int64_t>{cos.numel(), pos.defined() ? pos.numel() : 0, a.axes.n, a.pos_a, a.pos_b};
+    ctx->saved_data["eps"] = a.eps;
+    return {yq, yk};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &gq = grads[0], &gk = grads[1];
+    const L d = gq.size(3);
+    check_saved(s[0], gq, at::kBFloat16, gq.numel(), d);
+    check_saved(s[1], gq, at::kBFloat16, gk.numel(), d);
+    TORCH_CHECK(s[0].sizes().equals(gq.sizes()) && s[1].sizes().equals(gk.sizes()), "q or k saved for backward has come back with another shape");
+    const std::vector<int64_t> n = ctx->saved_data["sizes"].toIntVector();
+    const Tensor q = fix_strides(s[0]), k = fix_strides(s[1]), dyq = fix_strides(gq), dyk = fix_strides(gk), wq = row(operand(s[2], gq, d, d)), wk = row(operand(s[3], gq, d, d));
+    const Tensor cos = operand(s[4], gq, n[0], d / 2, at::kFloat), sin = operand(s[5], gq, n[0], d / 2, at::kFloat), pos = s[6].defined() ? operand(s[6], gq, n[1], q.size(1), at::kInt) : Tensor();
+    const int B = (int)q.size(0), S = (int)q.size(1), hq = (int)q.size(2), hkv = (int)k.size(2), ctas = api.lb_qk_norm_rope_bwd_ctas(B, S, hq, hkv, (int)d);
+    Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dwq, dwk, parts;
+    if (ctx->needs_input_grad(2) || ctx->needs_input_grad(3)) {
+      dwq = at::empty({d}, q.options());
+      dwk = at::empty({d}, q.options());
+      parts = empty_f32({ctas, 2, d}, q);
+    }
+    L st[18];
+    const Tensor* ts[6] = {&q, &k, &dyq, &dyk, &dq, &dk};
+    for (int i = 0; i < 6; i++) put_strides(st + 3 * i, *ts[i]);
+    const std::string axes = ctx->saved_data["axes"].toStringRef();
+    LB_CALL(lb_qk_norm_rope_bwd, q.const_data_ptr(), k.const_data_ptr(), dyq.const_data_ptr(), dyk.const_data_ptr(), dq.mutable_data_ptr(), dk.mutable_data_ptr(), wq.const_data_ptr(),
+            wk.const_data_ptr(), cos.const_data_ptr(), sin.const_data_ptr(), ptr(pos), reinterpret_cast<const unsigned char*>(axes.data()), (int)n[2], const_cast<W>(ptr(parts)), ctas,
+            const_cast<W>(ptr(dwq)), const_cast<W>(ptr(dwk)), B, S, hq, hkv, (int)d, (int)(n[0] / (d / 2)), st, n[3], n[4], (float)ctx->saved_data["eps"].toDouble(), stream());
+    return only_once({dq, dk, dwq, dwk, Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+  // a vector where the kernels read it
+  static Tensor row(const Tensor& t) { return ((uintptr_t)t.const_data_ptr() & 15) == 0 ? t : t.clone(); }
+};
+
 // ---- embedding, loss -----------------------------------------------------------------------------
 struct Embedding : Function<Embedding> {
   static Tensor forward(AutogradContext* ctx, const Tensor& tok, const Tensor& w, int64_t v0) {
@@ -518,6 +572,29 @@ struct Embedding : Function<Embedding> {
     LB_CALL(lb_embedding_bwd, tok.const_data_ptr(), dy.const_data_ptr(), dw.mutable_data_ptr(), (int)tok.numel(), (int)s[1], (int)s[2],
             (int)(s[2] + s[0]), stream());
     return {Tensor(), dw, Tensor()};
+  }
+};
+
+struct ScaledEmbedding : Function<ScaledEmbedding> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& tok, const Tensor& w, double scale, int64_t v0) {
+    const L H = w.size(1);
+    std::vector<int64_t> sizes = tok.sizes().vec();
+    sizes.push_back(H);
+    Tensor out = empty(sizes, w);
+    LB_CALL(lb_embed_scaled, tok.const_data_ptr(), (int)tok.element_size(), w.const_data_ptr(), out.mutable_data_ptr(), (int)tok.numel(), (int)H, v0, v0 + w.size(0), (float)scale, stream());
+    ctx->save_for_backward({tok});
+    ctx->saved_data["shape"] = std::vector<int64_t>{w.size(0), H, v0};
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const std::vector<int64_t> s = ctx->saved_data["shape"].toIntVector();
+    const Tensor dy = grads[0].contiguous(), saved = ctx->get_saved_variables()[0];
+    const Tensor tok = operand(saved, dy, dy.numel() / s[1], -1, saved.defined() && saved.scalar_type() == at::kInt ? at::kInt : at::kLong);
+    Tensor dw = empty({s[0], s[1]}, dy), ws = at::empty({api.lb_embed_sorted_ws_bytes((int)tok.numel(), (int)s[1])}, dy.options().dtype(at::kByte));
+    LB_CALL(lb_embed_sorted_bwd, tok.const_data_ptr(), (int)tok.element_size(), dy.const_data_ptr(), dw.mutable_data_ptr(), ws.mutable_data_ptr(), (L)ws.numel(), (int)tok.numel(), (int)s[1], s[2],
+            s[2] + s[0], (float)ctx->saved_data["scale"].toDouble(), stream());
+    return only_once({Tensor(), dw, Tensor(), Tensor()});
   }
 };
 
@@ -945,6 +1022,71 @@ PyObject* py_rope_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions or None, axes: None, list or tuple of ints, eps)
+PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || !unobserved() || !PyFloat_CheckExact(a[8])) LB_NOT_PLAIN;
+  const Tensor *q = tensor(a[0]), *k = tensor(a[1]), *wq = tensor(a[2]), *wk = tensor(a[3]), *cos = tensor(a[4]), *sin = tensor(a[5]), *pos = a[6] == Py_None ? nullptr : tensor(a[6]);
+  if (!plain(q, false) || !plain(k, false) || q->dim() != 4 || k->dim() != 4 || !here(*q) || k->device() != q->device()) LB_NOT_PLAIN;
+  const int64_t B = q->size(0), S = q->size(1), d = q->size(3), pairs = d / 2;
+  if (k->size(0) != B || k->size(1) != S || k->size(3) != d || d % 8 || d > 256 || !fits_int({B, S, q->size(2), k->size(2)})) LB_NOT_PLAIN;
+  for (const Tensor* w : {wq, wk})
+    if (!plain(w) || w->dim() != 1 || w->size(0) != d || w->device() != q->device() || ((uintptr_t)w->const_data_ptr() & 15)) LB_NOT_PLAIN;
+  if (!sized(cos, *q, at::kFloat) || !sized(sin, *q, at::kFloat) || cos->dim() != 2 || cos->size(1) != pairs || !sin->sizes().equals(cos->sizes()) || cos->size(0) == 0 || !fits_int({cos->size(0)}))
+    LB_NOT_PLAIN;
+  NormRope r{{}, 0, 0, PyFloat_AS_DOUBLE(a[8])};
+  if (!(r.eps >= 0.0 && r.eps <= FLT_MAX)) LB_NOT_PLAIN;
+  const bool one = a[7] == Py_None;
+  r.axes.n = 1;
+  std::memset(r.axes.of, 0, sizeof(r.axes.of));
+  if (!one) {
+    if (!(PyList_CheckExact(a[7]) || PyTuple_CheckExact(a[7])) || PySequence_Fast_GET_SIZE(a[7]) != pairs) LB_NOT_PLAIN;
+    for (int64_t i = 0; i < pairs; i++) {
+      PyObject* o = PySequence_Fast_GET_ITEM(a[7], i);
+      if (!PyLong_CheckExact(o)) LB_NOT_PLAIN;
+      const long v = PyLong_AsLong(o);
+      if (v < 0 || v >= 8) {
+        PyErr_Clear();
+        LB_NOT_PLAIN;
+      }
+      r.axes.of[i] = (unsigned char)v;
+      r.axes.n = std::max(r.axes.n, (int)v + 1);
+    }
+  }
+  if (a[6] != Py_None) {
+    if (!sized(pos, *q, at::kInt)) LB_NOT_PLAIN;
+    const bool by_axis = !one && pos->dim() > 1;
+    if (by_axis && pos->size(0) < r.axes.n) LB_NOT_PLAIN;
+    if (pos->dim() == 1 ? pos->size(0) != S : one ? !pos->sizes().equals({B, S}) : !(pos->sizes().equals({pos->size(0), S}) || pos->sizes().equals({pos->size(0), B, S}))) LB_NOT_PLAIN;
+    r.pos_a = by_axis ? pos->stride(0) : 0;
+    r.pos_b = pos->dim() == 3 ? pos->stride(1) : one && pos->dim() == 2 ? pos->stride(0) : 0;
+  }
+  variable_list y = unlocked([&, q_ = *q, k_ = *k, u = *wq, w = *wk, c = *cos, s = *sin, p = maybe(pos)] { return QKNormRope::apply(q_, k_, u, w, c, s, p, r); });
+  PyObject* t = PyTuple_New(2);
+  if (!t) return nullptr;
+  for (int i = 0; i < 2; i++) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(std::move(y[i])));
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
+// scaled_embedding(tokens, w, scale, vocab_start)
+PyObject* py_scaled_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4 || !PyFloat_CheckExact(a[2]) || !PyLong_CheckExact(a[3]) || !unobserved()) LB_NOT_PLAIN;
+  const Tensor *tok = tensor(a[0]), *w = tensor(a[1]);
+  const long long v0 = PyLong_AsLongLong(a[3]);
+  const double scale = PyFloat_AS_DOUBLE(a[2]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    LB_NOT_PLAIN;
+  }
+  if (!plain(w) || w->dim() != 2 || !here(*w) || !(sized(tok, *w, at::kLong) || sized(tok, *w, at::kInt)) || tok->numel() == 0 || tok->numel() > (1 << 30) || v0 < 0 || v0 > (1LL << 40) ||
+      !fits_int({w->size(0) + 2, w->size(1)}) || !(scale >= -FLT_MAX && scale <= FLT_MAX))
+    LB_NOT_PLAIN;
+  return THPVariable_Wrap(unlocked([&, t = *tok, w_ = *w] { return ScaledEmbedding::apply(t, w_, scale, (int64_t)v0); }));
+  END_HANDLE_TH_ERRORS
+}
+
 // The list's tensors as the kernels take them: dense in one piece, all on the current device; false: not a plain list.  They are held: without the interpreter's lock
 // another thread may change the list.
 struct NormList {
@@ -1068,6 +1210,7 @@ PyObject* py_init(PyObject*, PyObject* args) {
   LB_TAKE(lb_embedding_bwd); LB_TAKE(lb_ce_stats); LB_TAKE(lb_ce_loss); LB_TAKE(lb_ce_grad); LB_TAKE(lb_gemm_rope);
   LB_TAKE(lb_attn_mask); LB_TAKE(lb_masked_attn_fwd_ws_bytes); LB_TAKE(lb_masked_attn_fwd); LB_TAKE(lb_masked_attn_bwd_ws_bytes); LB_TAKE(lb_masked_attn_bwd); LB_TAKE(lb_rope_axes);
   LB_TAKE(lb_window_attn_fwd_ws_bytes); LB_TAKE(lb_window_attn_fwd); LB_TAKE(lb_window_attn_bwd_ws_bytes); LB_TAKE(lb_window_attn_bwd);
+  LB_TAKE(lb_qk_norm_rope); LB_TAKE(lb_qk_norm_rope_bwd_ctas); LB_TAKE(lb_qk_norm_rope_bwd); LB_TAKE(lb_embed_scaled); LB_TAKE(lb_embed_sorted_ws_bytes); LB_TAKE(lb_embed_sorted_bwd);
   LB_TAKE(lb_grad_norm_parts); LB_TAKE(lb_grad_squares); LB_TAKE(lb_grad_total); LB_TAKE(lb_grad_scale);
   if (!ok) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "an entry point of the kernels is missing");
@@ -1080,7 +1223,7 @@ PyObject* py_init(PyObject*, PyObject* args) {
 
 #define LB_FAST(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {LB_FAST(linear), LB_FAST(swiglu_mlp), LB_FAST(rmsnorm), LB_FAST(attention), LB_FAST(rope_attention), LB_FAST(embedding),
-                         LB_FAST(cross_entropy), LB_FAST(decoder_layers), LB_FAST(attention_mask), LB_FAST(masked_attention), LB_FAST(rope_axes), LB_FAST(grad_norm), LB_FAST(clip_grad_norm), {"launches", py_launches, METH_NOARGS, nullptr}, {"init", py_init, METH_VARARGS, nullptr},
+                         LB_FAST(cross_entropy), LB_FAST(decoder_layers), LB_FAST(attention_mask), LB_FAST(masked_attention), LB_FAST(rope_axes), LB_FAST(qk_norm_rope), LB_FAST(scaled_embedding), LB_FAST(grad_norm), LB_FAST(clip_grad_norm), {"launches", py_launches, METH_NOARGS, nullptr}, {"init", py_init, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1103,6 +1103,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     """Every head of q [B, S, hq, d] and of k [B, S, hkv, d] (any order of the outer dimensions) divided by its root mean square, times ``q_weight`` / ``k_weight`` [d], and turned by its token's
     position (interleaved pairs, as :func:`rope`), in one pass and rounded once.  ``positions``: None (each token's place), [S] or [B, S]; with ``axes`` None or [S], which count on all axes, [A, B, S]
     or [A, S] (two dimensions are axes and tokens then), as :func:`packed_attention_qkv` takes them.  A position outside of the tables makes its heads NaN."""
+    if (host := native.host_ops()) is not None and (y := host.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, axes, eps)) is not NotImplemented:
+        return y
     _check_norm_rope(q, k, q_weight, k_weight, cos, sin, eps)
     B, S, _, d = q.shape
     positions, axes = _positions_of(positions, axes, B, S, d, cos, sin)
@@ -1415,6 +1417,8 @@ def scaled_embedding(tokens: torch.Tensor, w: torch.Tensor, scale: float = 1.0, 
     """``scale`` times the rows of ``w`` [V, H] that ``tokens`` (int32 / int64, any shape) name, rounded once; ids outside of [vocab_start, vocab_start + V) give zero rows and no gradient
     (vocab-parallel partial result).  The gradient is dense; a row's sum runs over its tokens in their order, in 32 bits, and is rounded once: the same bits in every run, however
     often an id comes (:func:`embedding` adds up in the weight's type, as it comes)."""
+    if (host := native.host_ops()) is not None and (y := host.scaled_embedding(tokens, w, scale, vocab_start)) is not NotImplemented:
+        return y
     if w.dim() != 2 or not w.dtype.is_floating_point:
         raise ValueError(f"scaled_embedding takes a weight [V, H], got {w.dtype} {tuple(w.shape)}")
     if tokens.dtype not in (torch.int32, torch.int64) or tokens.device != w.device:

@@ -287,6 +287,7 @@ _HOST_ENTRIES = ("lb_rmsnorm_fwd", "lb_rmsnorm_bwd_blocks", "lb_rmsnorm_bwd", "l
                  "lb_flash_bwd_ws_bytes_kv", "lb_flash_bwd_tc_ws", "lb_flash_bwd", "lb_embedding_fwd", "lb_clear", "lb_embedding_bwd", "lb_ce_stats",
                  "lb_ce_loss", "lb_ce_grad", "lb_gemm_rope", "lb_attn_mask", "lb_masked_attn_fwd_ws_bytes", "lb_masked_attn_fwd", "lb_masked_attn_bwd_ws_bytes", "lb_masked_attn_bwd", "lb_rope_axes",
                  "lb_window_attn_fwd_ws_bytes", "lb_window_attn_fwd", "lb_window_attn_bwd_ws_bytes", "lb_window_attn_bwd",
+                 "lb_qk_norm_rope", "lb_qk_norm_rope_bwd_ctas", "lb_qk_norm_rope_bwd", "lb_embed_scaled", "lb_embed_sorted_ws_bytes", "lb_embed_sorted_bwd",
                  "lb_grad_norm_parts", "lb_grad_squares", "lb_grad_total", "lb_grad_scale")
 
 

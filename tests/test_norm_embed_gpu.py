@@ -154,6 +154,36 @@ def test_norm_rope_same_bits_each_time():
     assert all(torch.equal(a, b) for r in runs[1:] for a, b in zip(runs[0], r))
 
 
+def test_python_nodes_are_the_same(monkeypatch):
+    from lightron_b200.ops import functional as OF, native
+    q, k, wq, wk, cos, sin = _norm_case(2, 30, 4, 2, 64)
+    w, tokens = _rand(50, 64, seed=7), torch.randint(0, 60, (5, 20), generator=torch.Generator().manual_seed(1)).cuda()
+    ins = [t.detach().requires_grad_() for t in (q, k, wq, wk, w)]
+
+    def step(**kw):
+        y = OF.qk_norm_rope(*ins[:4], cos, sin, **kw)
+        e = OF.scaled_embedding(tokens, ins[4], 1.5, 3)
+        return (*y, e, *torch.autograd.grad((*y, e), ins, (y[0].detach(), y[1].detach(), _rand(5, 20, 64, seed=9))))
+    each = torch.randint(0, 30, (3, 2, 30), generator=torch.Generator().manual_seed(2)).cuda().int()
+    axes = [0] * 10 + [1] * 11 + [2] * 11
+    cases = [{}, dict(positions=each[0, 0]), dict(positions=each[0]), dict(positions=each, axes=axes), dict(positions=each[:, 0].contiguous(), axes=axes), dict(axes=axes),
+             dict(positions=each[0, 0], axes=axes)]
+    want = [step(**kw) for kw in cases]
+    monkeypatch.setattr(native, "host_ops", lambda: None)
+    for kw, e in zip(cases, want):
+        assert all(torch.equal(a, b) for a, b in zip(step(**kw), e)), kw
+
+
+def test_nodes_refuse_a_second_derivative():
+    from lightron_b200.ops import functional as OF
+    q, k, wq, wk, cos, sin = _norm_case(1, 3, 2, 1, 64)
+    leaf, w = q.detach().requires_grad_(), _rand(5, 8).requires_grad_()
+    for y, x in ((OF.qk_norm_rope(leaf, k, wq, wk, cos, sin)[0], leaf), (OF.scaled_embedding(torch.zeros(2, dtype=torch.long, device="cuda"), w), w)):
+        g, = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+
+
 def test_norm_rope_parts_of_the_gradients():
     """One output used, or weights without gradients."""
     from lightron_b200.ops import functional as OF
@@ -190,6 +220,7 @@ def _check_embedding(tokens, V, H, scale=1.0, start=0, w=None, dy=None):
 
 @pytest.mark.parametrize("T,V,H", [
     (1, 1, 8), (1, 10, 64), (3, 5, 1), (7, 4, 2), (8, 100, 1021), (65, 30, 6), (300, 7, 264), (511, 2000, 2048), (700, 50, 4104), (2100, 900, 72), (5000, 64, 33),
+    (4096, 3000, 16), (4097, 1023, 24), (4097, 1024, 7), (9000, 140000, 8), (8191, 2, 16), (20000, 1100000, 1),
 ])
 @pytest.mark.parametrize("wide", [True, False])
 def test_embedding(T, V, H, wide):
@@ -230,6 +261,25 @@ def test_embedding_ids_outside():
     assert (_check_embedding(away, 32, 24) == 0).all()
     away[1000:] = 3
     _check_embedding(away, 32, 24)
+
+
+def test_embedding_many_rows_and_bits():
+    """Rows beyond what ten bits, and three passes of ten, hold; most of them without a token."""
+    from lightron_b200.ops import functional as OF
+    g = torch.Generator().manual_seed(3)
+    V, T = 40_000_000, 6000
+    tokens = torch.randint(0, V, (T,), generator=g)
+    tokens[::7] = V - 1
+    tokens[3::7] = 0
+    w = torch.zeros(V, 2, dtype=BF16, device="cuda").requires_grad_()
+    dy = _rand(T, 2, seed=2)
+    dw, = torch.autograd.grad(OF.scaled_embedding(tokens.cuda(), w, 3.0), w, dy)
+    ids, back = tokens.unique(return_inverse=True)
+    want = torch.zeros(ids.numel(), 2, dtype=torch.float64).index_add_(0, back, dy.double().cpu()) * 3.0
+    size = torch.zeros(ids.numel(), 2, dtype=torch.float64).index_add_(0, back, dy.double().abs().cpu()) * 3.0
+    assert ((dw[ids.cuda()].double().cpu() - want).abs() <= (HALF + 2.0 ** -23) * want.abs() + 1000 * 2.0 ** -24 * size).all()
+    dw[ids.cuda()] = 0
+    assert not dw.any()
 
 
 def test_embedding_same_bits_each_time():
