@@ -3,9 +3,9 @@
 // The weight holds vocab ids [v0, v1); ids outside give zero rows and no gradient (vocab-parallel partial result).
 //
 // Forward: memory bound, rows of w in, rows of y out.
-// Backward: the tokens are ordered by id, equal ids by their places (few by comparison, many by a radix sort of one cluster), while the other SMs clear the rows without tokens; then CTAs take runs of equal CHUNKs of that order: a row whose tokens lie inside one is summed in 32
-// bits, scaled, rounded once and written; what a chunk has of a row that begins or ends in another goes to a place of its own in 32 bits, and a last kernel adds those up in the order of
-// the chunks.  No atomics on values: the same bits in every run.  Bound by memory: every dy once, every row of dw once.
+// Backward: the tokens are ordered by id, equal ids by their places (few by comparison, many by a radix sort of one cluster); then CTAs take chunks of that order and sum rows in 32
+// bits, scale, round once and write, while others clear the rows that have no token.  What chunks have of a row that is longer than two of them goes to places of their own in 32 bits, which a
+// last kernel adds up, always in the same order.  No atomics on values: the same bits in every run.  Bound by memory: every dy once, every row of dw once.
 #include "common.cuh"
 
 namespace {
@@ -79,17 +79,13 @@ __global__ void __launch_bounds__(256) embed_scaled_kernel(const void* __restric
 }
 
 // ---- order --------------------------------------------------------------------------------------
-// One launch orders the tokens and meanwhile clears the rows of dw that have none: the first CTAs order, the others each have a share of the rows, find in all tokens which of them have
-// one, and write zeros to the rest.
 struct OrderParams {
   const void* tok;
-  int wide, T, V, H;
+  int wide, T, V;
   long long v0;
   int *ids, *place;              // [T] each: the tokens' rows in order, and their places
   int2 *a, *b;                   // [T] each: between the passes
   int passes, bits;              // of the radix sort
-  bf16* dw;
-  int order_ctas;
 };
 constexpr int ORDER_THREADS = 1024, ORDER_WARPS = ORDER_THREADS / 32;
 // Row of token t; those outside, V, come behind all others.
@@ -98,56 +94,12 @@ __device__ __forceinline__ int row_of(const OrderParams& p, int t) {
   return id >= 0 && id < p.V ? (int)id : p.V;
 }
 
-constexpr int FILL_WORDS = 4096;      // rows of a round: 32 of each word
-__device__ __forceinline__ void clear_rows(const OrderParams& p, uint32_t* marks, int cta, int ctas) {
-  const int per = (int)((p.V + (long long)ctas - 1) / ctas);
-  const long long begin = (long long)cta * per, end = min((long long)p.V, begin + per);
-  const int lane = threadIdx.x & 31;
-  const bool wide = p.H % 8 == 0 && ((uintptr_t)p.dw & 15) == 0;
-  for (long long r0 = begin; r0 < end; r0 += FILL_WORDS * 32) {
-    const int n = (int)min((long long)FILL_WORDS * 32, end - r0);
-    for (int i = threadIdx.x; i < (n + 31) / 32; i += ORDER_THREADS) marks[i] = 0;
-    __syncthreads();
-    constexpr int U = 8;
-    for (long long t = threadIdx.x; t < p.T; t += U * ORDER_THREADS) {
-      int r[U];
-#pragma unroll
-      for (int u = 0; u < U; u++) r[u] = t + u * ORDER_THREADS < p.T ? row_of(p, (int)(t + u * ORDER_THREADS)) : p.V;
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-        const long long at = r[u] - r0;
-        // (looked at first: an id that comes ten thousand times is marked once)
-        if (at >= 0 && at < n && !(reinterpret_cast<volatile uint32_t*>(marks)[at >> 5] >> (at & 31) & 1u)) atomicOr(&marks[at >> 5], 1u << (at & 31));
-      }
-    }
-    __syncthreads();
-    for (int r = threadIdx.x >> 5; r < n; r += ORDER_WARPS) {
-      if (marks[r >> 5] >> (r & 31) & 1u) continue;
-      bf16* row = p.dw + (r0 + r) * p.H;
-      if (wide) {
-        for (int c = lane; c < p.H / 8; c += 32) reinterpret_cast<uint4*>(row)[c] = make_uint4(0, 0, 0, 0);
-      } else {
-        // (a row of any alignment: whole words between its ends)
-        int c = ((uintptr_t)row & 2) ? 1 : 0;
-        if (c && lane == 0) row[0] = __float2bfloat16(0.f);
-        for (int k = lane; k < (p.H - c) / 2; k += 32) *reinterpret_cast<uint32_t*>(row + c + 2 * k) = 0u;
-        if ((p.H - c) % 2 && lane == 0) row[p.H - 1] = __float2bfloat16(0.f);
-      }
-    }
-    __syncthreads();
-  }
-}
-
 // Few tokens: each one's rank by comparison with all others, RANK_PARTS threads a token.
 constexpr int RANK_MOST = 4096, RANK_PARTS = 16, RANK_TOKENS = ORDER_THREADS / RANK_PARTS;
 __global__ void __launch_bounds__(ORDER_THREADS) embed_rank_kernel(const __grid_constant__ OrderParams p) {
   grid_go();
   grid_wait();
-  __shared__ int s[RANK_MOST];                     // (of the rows that are cleared: which have tokens)
-  if ((int)blockIdx.x >= p.order_ctas) {
-    clear_rows(p, reinterpret_cast<uint32_t*>(s), (int)blockIdx.x - p.order_ctas, (int)gridDim.x - p.order_ctas);
-    return;
-  }
+  __shared__ int s[RANK_MOST];
   for (int i = threadIdx.x; i < p.T; i += ORDER_THREADS) s[i] = row_of(p, i);
   __syncthreads();
   const int t = (int)blockIdx.x * RANK_TOKENS + (int)threadIdx.x / RANK_PARTS, part = threadIdx.x % RANK_PARTS;
@@ -162,7 +114,6 @@ __global__ void __launch_bounds__(ORDER_THREADS) embed_rank_kernel(const __grid_
     p.place[rank] = t;
   }
 }
-static_assert(FILL_WORDS <= RANK_MOST, "the marks take the place of the rows");
 
 // Many: a radix sort by one cluster, which keeps the order of equals.  A warp has a share of the elements in their order; it counts their digits 32 at a time, the lowest lane of equal digits for all of
 // them; counts of the warps ahead, then of the CTAs ahead and of the lower digits (through the cluster's shared memory), give every element its place.
@@ -183,15 +134,13 @@ __device__ __forceinline__ uint32_t peer_word(const uint32_t* at, uint32_t cta) 
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
+// KEEP: at most so many elements of a lane, which stay in its registers; 0: any number, read twice a pass.
+template <int KEEP>
 __global__ void __launch_bounds__(ORDER_THREADS, 1) embed_radix_kernel(const __grid_constant__ OrderParams p) {
   extern __shared__ __align__(16) char radix_smem[];
   RadixShared& s = *reinterpret_cast<RadixShared*>(radix_smem);
   grid_go();
   grid_wait();
-  if ((int)blockIdx.x >= CLUSTER) {
-    clear_rows(p, reinterpret_cast<uint32_t*>(radix_smem), (int)blockIdx.x - CLUSTER, (int)gridDim.x - CLUSTER);
-    return;
-  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << p.bits;
   const uint32_t me = cluster_rank(), below = (1u << lane) - 1u;
   const long long per = (p.T + 32LL * CLUSTER * ORDER_WARPS - 1) / (32LL * CLUSTER * ORDER_WARPS) * 32;
@@ -205,14 +154,38 @@ __global__ void __launch_bounds__(ORDER_THREADS, 1) embed_radix_kernel(const __g
       return pass == 0 ? make_int2(row_of(p, (int)i), (int)i) : __ldcg(from + i);
     };
     auto digit = [&](int2 x, long long i) { return i < end ? (x.x >> shift) & (digits - 1) : digits; };
-    for (int i = threadIdx.x; i < ORDER_WARPS * digits; i += ORDER_THREADS) s.count[i / digits][i % digits] = 0;
-    __syncthreads();
-    for (long long i0 = first; i0 < end; i0 += 32) {
-      const long long i = i0 + lane;
-      const int d = digit(load(i), i);
+    // rank of the lane's element among the warp's equal digits so far
+    auto count = [&](int d) {
       const uint32_t same = __match_any_sync(0xffffffffu, d);
+      uint32_t rank = 0;
+      if (d < digits) rank = s.count[warp][d] + __popc(same & below);
+      __syncwarp();
       if (d < digits && (same & below) == 0) s.count[warp][d] += __popc(same);
       __syncwarp();
+      return rank;
+    };
+    auto put = [&](int2 x, uint32_t at) {
+      if (pass + 1 < p.passes) {
+        __stcg(to + at, x);
+      } else {
+        p.ids[at] = x.x;
+        p.place[at] = x.y;
+      }
+    };
+    [[maybe_unused]] int2 x[KEEP > 0 ? KEEP : 1];
+    [[maybe_unused]] uint32_t rank[KEEP > 0 ? KEEP : 1];
+    if constexpr (KEEP > 0) {
+#pragma unroll
+      for (int u = 0; u < KEEP; u++) x[u] = load(first + 32 * u + lane);
+    }
+    for (int i = threadIdx.x; i < ORDER_WARPS * digits; i += ORDER_THREADS) s.count[i >> p.bits][i & (digits - 1)] = 0;
+    __syncthreads();
+    if constexpr (KEEP > 0) {
+#pragma unroll
+      for (int u = 0; u < KEEP; u++)
+        if (first + 32 * u < end) rank[u] = count(digit(x[u], first + 32 * u + lane));
+    } else {
+      for (long long i = first + lane; i - lane < end; i += 32) count(digit(load(i), i));
     }
     __syncthreads();
     const int d = threadIdx.x;
@@ -239,8 +212,8 @@ __global__ void __launch_bounds__(ORDER_THREADS, 1) embed_radix_kernel(const __g
     uint32_t sum = all;                            // of the lower digits
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t x = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += x;
+      const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
     }
     if (lane == 31) s.of_warps[warp] = sum;
     __syncthreads();
@@ -250,124 +223,257 @@ __global__ void __launch_bounds__(ORDER_THREADS, 1) embed_radix_kernel(const __g
     for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
     if (d < digits) s.base[d] = sum - all + w + ahead;
     __syncthreads();
-    for (long long i0 = first; i0 < end; i0 += 32) {
-      const long long i = i0 + lane;
-      const int2 x = load(i);
-      const int dx = digit(x, i);
-      const uint32_t same = __match_any_sync(0xffffffffu, dx);
-      uint32_t at = 0;
-      if (dx < digits) at = s.base[dx] + s.count[warp][dx] + __popc(same & below);
-      __syncwarp();
-      if (dx < digits) {
-        if ((same & below) == 0) s.count[warp][dx] += __popc(same);
-        if (pass + 1 < p.passes) {
-          __stcg(to + at, x);
-        } else {
-          p.ids[at] = x.x;
-          p.place[at] = x.y;
-        }
+    if constexpr (KEEP > 0) {
+#pragma unroll
+      for (int u = 0; u < KEEP; u++) {
+        const int dx = digit(x[u], first + 32 * u + lane);
+        if (dx < digits) put(x[u], s.base[dx] + s.count[warp][dx] + rank[u]);
       }
-      __syncwarp();
+    } else {
+      for (long long i = first + lane; i - lane < end; i += 32) {
+        const int2 e = load(i);
+        const int dx = digit(e, i);
+        const uint32_t at = count(dx);
+        if (dx < digits) put(e, s.base[dx] + at);
+      }
     }
     cluster_sync();                                // the elements are where the next pass reads them, and nobody reads totals any more
   }
 }
 
 // ---- sums ---------------------------------------------------------------------------------------
+// The first CTAs take a chunk of the order and a slab of columns each.  A row is summed by the chunk that it begins in, where it ends in that or the next one; a longer one leaves what each chunk has of it,
+// in 32 bits.  The other CTAs clear rows that have no token.
 struct SumParams {
   const bf16* dy;
   bf16* dw;
   const int *ids, *place;        // [T] in order of id, then place
-  float* parts;                  // [chunks][2][H]: of the row that a chunk has from the one before it, and of the one that goes on in the next
+  float* parts;                  // [chunks][2][H]: of a longer row from the chunk before, and of one that begins here
   int T, H, V, chunk;
   float scale;
+  unsigned sums, slabs;          // CTAs that sum, of a chunk
+  int clear;                     // rows of a CTA that clears
 };
-constexpr int SUM_THREADS = 256, MAX_CHUNK = 64;
+constexpr int SUM_THREADS = 256, MAX_CHUNK = 64, MOST_CLEAR = 1024;
+
+// First place in the order of row r or a later one: the warp looks in 32 places at a time.
+__device__ __forceinline__ int first_of(const int* ids, int T, long long r) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = T;                               // it is in [lo, lo + n]
+  while (n > 0) {
+    const int step = (n + 31) / 32;
+    const long long at = (long long)lo + (long long)(lane + 1) * step - 1;
+    const bool less = at < (long long)lo + n && ids[at] < r;
+    const int skip = __popc(__ballot_sync(0xffffffffu, less)) * step;
+    lo += skip;
+    n = min(step - 1, n - skip);
+  }
+  return lo;
+}
 
 template <int VEC>
-__global__ void __launch_bounds__(SUM_THREADS) embed_sum_kernel(const SumParams p) {
-  grid_go();
-  grid_wait();
+__device__ __forceinline__ void clear_rows(const SumParams& p, int cta) {
   typedef typename Vec<VEC>::type V;
-  __shared__ int ids[MAX_CHUNK + 2], place[MAX_CHUNK];
-  const long long first = (long long)blockIdx.x * p.chunk;
-  const int n = (int)min((long long)p.chunk, p.T - first);
-  for (int i = threadIdx.x; i < n + 2; i += SUM_THREADS) {
-    const long long at = first + i - 1;
-    ids[i] = at >= 0 && at < p.T ? p.ids[at] : -1;
-    if (i < n) place[i] = p.place[first + i];
+  __shared__ uint32_t marks[MOST_CLEAR / 32];      // rows that have tokens
+  __shared__ int range[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long begin = (long long)cta * p.clear, end = min((long long)p.V, begin + p.clear);
+  if (threadIdx.x < MOST_CLEAR / 32) marks[threadIdx.x] = 0;
+  if (warp < 2) {
+    const int at = first_of(p.ids, p.T, warp ? end : begin);
+    if (lane == 0) range[warp] = at;
   }
   __syncthreads();
-  const int c = (blockIdx.y * SUM_THREADS + threadIdx.x) * VEC;
-  if (c >= p.H) return;
-  constexpr int U = 8;
-  float sum[VEC];
-#pragma unroll
-  for (int k = 0; k < VEC; k++) sum[k] = 0.f;
-  int begin = 0;                                   // of the run
-  for (int i0 = 0; i0 < n && ids[i0 + 1] < p.V; i0 += U) {
-    V a[U];
-#pragma unroll
-    for (int u = 0; u < U; u++)
-      if (i0 + u < n) a[u] = *reinterpret_cast<const V*>(p.dy + (long long)place[i0 + u] * p.H + c);
+  constexpr int U = 8;                             // (a row may come ten thousand times)
+  for (int i = range[0] + (int)threadIdx.x; i < range[1]; i += U * SUM_THREADS) {
+    int r[U], before[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int i = i0 + u;
-      if (i >= n) break;
-      const int id = ids[i + 1];
-      float f[VEC];
-      unpack<VEC>(a[u], f);
+      const int at = i + u * SUM_THREADS;
+      r[u] = at < range[1] ? p.ids[at] : -1;
+      before[u] = at < range[1] && at > range[0] ? p.ids[at - 1] : -1;
+    }
 #pragma unroll
-      for (int k = 0; k < VEC; k++) sum[k] += f[k];
-      if (i + 1 < n && ids[i + 2] == id) continue;
-      if (id < p.V) {
-        const bool from = begin == 0 && ids[0] == id, on = ids[i + 2] == id;      // (on: at the chunk's end alone)
-        if (!from && !on) {
-#pragma unroll
-          for (int k = 0; k < VEC; k++) sum[k] *= p.scale;
-          *reinterpret_cast<V*>(p.dw + (long long)id * p.H + c) = packed<VEC>(sum);
-        } else {
-          float* to = p.parts + ((long long)blockIdx.x * 2 + (from ? 0 : 1)) * p.H + c;
-#pragma unroll
-          for (int k = 0; k < VEC; k++) to[k] = sum[k];
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < VEC; k++) sum[k] = 0.f;
-      begin = i + 1;
+    for (int u = 0; u < U; u++)
+      if (r[u] != before[u]) atomicOr(&marks[(r[u] - (int)begin) >> 5], 1u << ((r[u] - (int)begin) & 31));
+  }
+  __syncthreads();
+  for (int r = warp; r < (int)(end - begin); r += SUM_THREADS / 32) {
+    if (marks[r >> 5] >> (r & 31) & 1u) continue;
+    bf16* row = p.dw + (begin + r) * p.H;
+    if constexpr (VEC == 1) {
+      // (a row of any alignment: whole words between its ends)
+      const int c = ((uintptr_t)row & 2) ? 1 : 0;
+      if (c && lane == 0) row[0] = __float2bfloat16(0.f);
+      for (int k = lane; k < (p.H - c) / 2; k += 32) *reinterpret_cast<uint32_t*>(row + c + 2 * k) = 0u;
+      if ((p.H - c) % 2 && lane == 0) row[p.H - 1] = __float2bfloat16(0.f);
+    } else {
+      const float zeros[VEC] = {};
+      for (int c = lane; c < p.H / VEC; c += 32) reinterpret_cast<V*>(row)[c] = packed<VEC>(zeros);
     }
   }
 }
 
-// Rows of several chunks: the CTA of the chunk where one begins adds up its parts.  32 columns, 8 parts at a time.
-constexpr int JOIN_COLS = 32, JOIN_ROWS = 8;
-__global__ void __launch_bounds__(JOIN_COLS* JOIN_ROWS) embed_join_kernel(const SumParams p) {
+// A thread has K vectors of a row, a CTA's width apart; U places on their way.
+template <int VEC, int K, int U>
+__global__ void __launch_bounds__(SUM_THREADS, 3) embed_sum_kernel(const __grid_constant__ SumParams p) {
   grid_go();
   grid_wait();
-  const long long next = ((long long)blockIdx.x + 1) * p.chunk;
-  if (next >= p.T) return;
-  const int id = p.ids[next - 1];
-  if (id >= p.V || p.ids[next] != id) return;
-  if (p.ids[next - p.chunk] == id && next > p.chunk && p.ids[next - p.chunk - 1] == id) return;      // (began in an earlier chunk)
-  // chunks that the row goes on in: up to the last that begins with it
-  long long lo = blockIdx.x + 1, hi = (p.T - 1LL) / p.chunk;
-  while (lo < hi) {
-    const long long mid = (lo + hi + 1) / 2;
-    if (p.ids[mid * p.chunk] == id) lo = mid; else hi = mid - 1;
+  if (blockIdx.x >= p.sums) {
+    clear_rows<VEC>(p, (int)(blockIdx.x - p.sums));
+    return;
   }
-  __shared__ float s[JOIN_ROWS][JOIN_COLS];
-  const int c = blockIdx.y * JOIN_COLS + threadIdx.x;
-  float sum = 0.f;
-  if (c < p.H) {
-    if (threadIdx.y == 0) sum = p.parts[((long long)blockIdx.x * 2 + 1) * p.H + c];
-#pragma unroll 4
-    for (long long k = blockIdx.x + 1 + threadIdx.y; k <= lo; k += JOIN_ROWS) sum += p.parts[k * 2 * p.H + c];
+  typedef typename Vec<VEC>::type V;
+  __shared__ int ids[3 * MAX_CHUNK + 2], place[2 * MAX_CHUNK];      // of the chunk before (and one more), this and the next (and one more)
+  const int slab = (int)(blockIdx.x % p.slabs), chunk = (int)(blockIdx.x / p.slabs);
+  const long long first = (long long)chunk * p.chunk;
+  const int C = p.chunk, n = (int)min((long long)C, p.T - first);
+  for (int i = threadIdx.x; i < 3 * C + 2; i += SUM_THREADS) {
+    const long long at = first + i - C - 1;
+    ids[i] = at >= 0 && at < p.T ? p.ids[at] : -1;
+    if (i < 2 * C && first + i < p.T) place[i] = p.place[first + i];
   }
-  s[threadIdx.y][threadIdx.x] = sum;
   __syncthreads();
-  if (threadIdx.y || c >= p.H) return;
-  for (int r = 1; r < JOIN_ROWS; r++) sum += s[r][threadIdx.x];
-  p.dw[(long long)id * p.H + c] = __float2bfloat16(sum * p.scale);
+  const int* id_of = ids + C + 1;                  // of the chunk's places
+  // The row that goes on from the chunk before: skipped, where that one sums it (it began there, and ends here).
+  int begin = 0;
+  bool from = chunk > 0 && id_of[-1] == id_of[0];
+  if (from) {
+    int end = 1;
+    while (end < C + 1 && id_of[end] == id_of[0]) end++;
+    if (end <= C && !(id_of[-C] == id_of[0] && id_of[-C - 1] == id_of[0])) {
+      begin = end;
+      from = false;
+    }
+  }
+  // The row that goes on in the next chunk: all of it, where it began here and ends there.
+  int stop = n;
+  bool on = n == C && id_of[C] == id_of[C - 1] && begin < C;
+  if (on && !(from && id_of[0] == id_of[C - 1])) {
+    int end = C + 1;
+    while (end < 2 * C + 1 && id_of[end] == id_of[C]) end++;
+    if (end <= 2 * C) {
+      stop = end;
+      on = false;
+    }
+  }
+  const int c0 = (slab * K * SUM_THREADS + (int)threadIdx.x) * VEC;
+  constexpr int STEP = SUM_THREADS * VEC;
+  float sum[K][VEC] = {};
+  for (int i0 = begin; i0 < stop && id_of[i0] < p.V; i0 += U) {
+    V a[U][K];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int k = 0; k < K; k++)
+        if (i0 + u < stop && c0 + k * STEP < p.H) a[u][k] = *reinterpret_cast<const V*>(p.dy + (long long)place[i0 + u] * p.H + c0 + k * STEP);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = i0 + u;
+      if (i >= stop) break;
+      const int id = id_of[i];
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        float f[VEC];
+        unpack<VEC>(a[u][k], f);
+#pragma unroll
+        for (int v = 0; v < VEC; v++) sum[k][v] += f[v];
+      }
+      if (i + 1 < stop && id_of[i + 1] == id) continue;
+      const bool whole = !from && !(i + 1 == stop && on);
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        const int c = c0 + k * STEP;
+        if (id < p.V && c < p.H) {
+          if (whole) {
+#pragma unroll
+            for (int v = 0; v < VEC; v++) sum[k][v] *= p.scale;
+            *reinterpret_cast<V*>(p.dw + (long long)id * p.H + c) = packed<VEC>(sum[k]);
+          } else {
+            float* to = p.parts + ((long long)chunk * 2 + (from ? 0 : 1)) * p.H + c;
+#pragma unroll
+            for (int v = 0; v < VEC; v++) to[v] = sum[k][v];
+          }
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; v++) sum[k][v] = 0.f;
+      }
+      from = false;
+    }
+  }
+}
+
+// Rows of more than two chunks: every CTA looks for the chunks where one begins, and takes its share of (row, columns): JOIN_SLAB columns, JOIN_ROWS parts at a time.
+constexpr int JOIN_COLS = 32, JOIN_ROWS = 16, JOIN_THREADS = JOIN_COLS * JOIN_ROWS, JOIN_K = 4, JOIN_SLAB = JOIN_COLS * JOIN_K;
+__global__ void __launch_bounds__(JOIN_THREADS) embed_join_kernel(const __grid_constant__ SumParams p) {
+  grid_go();
+  grid_wait();
+  __shared__ int2 list[JOIN_THREADS];              // chunk of the round where a row begins, and the row
+  __shared__ long long ends[JOIN_THREADS];         // the last chunk that it goes on in
+  __shared__ int found;
+  __shared__ float s[JOIN_ROWS][JOIN_SLAB];
+  const int col = threadIdx.x % JOIN_COLS, r = threadIdx.x / JOIN_COLS, slabs = (p.H + JOIN_SLAB - 1) / JOIN_SLAB;
+  const long long last = (p.T - 1LL) / p.chunk;    // chunk
+  long long item = blockIdx.x;                     // of this CTA, counted over all rounds
+  for (long long c0 = 0; c0 + 2 <= last; c0 += JOIN_THREADS) {
+    if (threadIdx.x == 0) found = 0;
+    __syncthreads();
+    const long long chunk = c0 + threadIdx.x;
+    bool here = chunk + 2 <= last;
+    int id = 0;
+    if (here) {
+      const long long begin = chunk * p.chunk;
+      id = p.ids[begin + p.chunk - 1];
+      const int over = p.ids[begin + 2LL * p.chunk], head = p.ids[begin], before = begin > 0 ? p.ids[begin - 1] : -1;
+      here = id < p.V && over == id && !(head == id && before == id);
+    }
+    // (in the order of the chunks: all CTAs have the same list)
+    const uint32_t some = __ballot_sync(0xffffffffu, here);
+    __shared__ int of_warps[JOIN_THREADS / 32];
+    if ((threadIdx.x & 31) == 0) of_warps[threadIdx.x / 32] = __popc(some);
+    __syncthreads();
+    int at = __popc(some & ((1u << (threadIdx.x & 31)) - 1u));
+    for (int w = 0; w < (int)threadIdx.x / 32; w++) at += of_warps[w];
+    if (here) {
+      long long lo = chunk + 2, hi = last;
+      while (lo < hi) {                            // up to the last chunk that begins with the row
+        const long long mid = (lo + hi + 1) / 2;
+        if (p.ids[mid * p.chunk] == id) lo = mid; else hi = mid - 1;
+      }
+      list[at] = make_int2((int)threadIdx.x, id);
+      ends[at] = lo;
+    }
+    if (threadIdx.x == JOIN_THREADS - 1) found = at + (here ? 1 : 0);
+    __syncthreads();
+    const long long items = (long long)found * slabs;
+    for (; item < items; item += gridDim.x) {
+      const int2 row = list[item / slabs];
+      const long long first = c0 + row.x, end = ends[item / slabs];
+      const int c = (int)(item % slabs) * JOIN_SLAB + col;
+      float sum[JOIN_K] = {};
+#pragma unroll
+      for (int k = 0; k < JOIN_K; k++)
+        if (r == 0 && c + k * JOIN_COLS < p.H) sum[k] = p.parts[(first * 2 + 1) * p.H + c + k * JOIN_COLS];
+#pragma unroll 4
+      for (long long part = first + 1 + r; part <= end; part += JOIN_ROWS)
+#pragma unroll
+        for (int k = 0; k < JOIN_K; k++)
+          if (c + k * JOIN_COLS < p.H) sum[k] += p.parts[part * 2 * p.H + c + k * JOIN_COLS];
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < JOIN_K; k++) s[r][col + k * JOIN_COLS] = sum[k];
+      __syncthreads();
+      const int at = (int)(item % slabs) * JOIN_SLAB + (int)threadIdx.x;
+      if (threadIdx.x < JOIN_SLAB && at < p.H) {
+        float all = 0.f;
+#pragma unroll
+        for (int k = 0; k < JOIN_ROWS; k++) all += s[k][threadIdx.x];
+        p.dw[(long long)row.y * p.H + at] = __float2bfloat16(all * p.scale);
+      }
+    }
+    item -= items;
+    __syncthreads();
+  }
 }
 
 int vec_of(int H, uintptr_t at) { return H % 8 == 0 && at % 16 == 0 ? 8 : H % 2 == 0 && at % 4 == 0 ? 2 : 1; }
@@ -385,6 +491,21 @@ int passes_of(int V, int& bits) {
   return passes;
 }
 long long up(long long bytes) { return (bytes + 255) / 256 * 256; }
+template <int KEEP>
+int launch_radix(const OrderParams& o, cudaStream_t s) {
+  static bool done[64] = {false};      // (of a device: an attribute counts where it was set)
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return LB_ERR_LAUNCH;
+  if (!done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(embed_radix_kernel<KEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(RadixShared));
+    if (e != cudaSuccess) { cudaGetLastError(); g_lb_last_cuda_error = (int)e; return LB_ERR_LAUNCH; }
+    done[dev] = true;
+  }
+  return lb_launch_cluster(true, CLUSTER, embed_radix_kernel<KEEP>, CLUSTER, ORDER_THREADS, sizeof(RadixShared), s, o);
+}
+constexpr int KEPT = 4;                // elements of a lane in registers: up to 32768 tokens
+constexpr long long CLEAR_BYTES = 65536;      // of a CTA that clears
+
 int check_sizes(int T, int H, long long v0, long long v1) { return T <= 0 || T > (1 << 30) || H <= 0 || v0 < 0 || v1 <= v0 || v1 - v0 > 0x7ffffffeLL ? LB_ERR_SHAPE : LB_OK; }
 
 }  // namespace
@@ -419,43 +540,34 @@ extern "C" int lb_embed_sorted_bwd(const void* tok, int id_bytes, const void* dy
   if (ws_bytes < lb_embed_sorted_ws_bytes(T, H)) return LB_ERR_CAPACITY;
   cudaStream_t s = (cudaStream_t)stream;
   const int V = (int)(v1 - v0);
+  if ((T / 8 + 1LL) * (H / SUM_THREADS + 1LL) + V / 8 + 1LL > 0x7fffffffLL) return LB_ERR_SHAPE;      // (more CTAs than a grid has)
   char* at = (char*)ws;
-  OrderParams o{tok, id_bytes == 8 ? 1 : 0, T, V, H, v0, (int*)at, (int*)(at + up(4LL * T)), nullptr, nullptr, 0, 0, (bf16*)dw, 0};
+  OrderParams o{tok, id_bytes == 8 ? 1 : 0, T, V, v0, (int*)at, (int*)(at + up(4LL * T)), nullptr, nullptr, 0, 0};
   at += 2 * up(4LL * T);
-  // CTAs that clear: 64 KB of rows each at least
-  const long long want = ((long long)V * H * 2 + 65535) / 65536, sms = lb_num_sms();
   if (T <= RANK_MOST) {
-    o.order_ctas = (T + RANK_TOKENS - 1) / RANK_TOKENS;
-    LB_LAUNCH(embed_rank_kernel, (unsigned)(o.order_ctas + (want < 2 * sms ? want : 2 * sms)), ORDER_THREADS, 0, s, o);
+    LB_LAUNCH(embed_rank_kernel, (T + RANK_TOKENS - 1) / RANK_TOKENS, ORDER_THREADS, 0, s, o);
   } else {
     o.a = (int2*)at;
     o.b = (int2*)(at + up(8LL * T));
     at += 2 * up(8LL * T);
     o.passes = passes_of(V, o.bits);
-    static bool done[64] = {false};      // (of a device: an attribute counts where it was set)
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return LB_ERR_LAUNCH;
-    if (!done[dev]) {
-      const cudaError_t e = cudaFuncSetAttribute(embed_radix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(RadixShared));
-      if (e != cudaSuccess) { cudaGetLastError(); g_lb_last_cuda_error = (int)e; return LB_ERR_LAUNCH; }
-      done[dev] = true;
-    }
-    const long long fill = (want < sms ? want : sms) / CLUSTER, clusters = 1 + (fill < 1 ? 1 : fill);
-    const int rc = lb_launch_cluster(true, CLUSTER, embed_radix_kernel, (unsigned)(clusters * CLUSTER), ORDER_THREADS, sizeof(RadixShared), s, o);
+    const int rc = T <= KEPT * 32 * ORDER_WARPS * CLUSTER ? launch_radix<KEPT>(o, s) : launch_radix<0>(o, s);
     if (rc) return rc;
   }
-  SumParams p{(const bf16*)dy, (bf16*)dw, o.ids, o.place, (float*)at, T, H, V, chunk_of(T), scale};
-  const unsigned chunks = (unsigned)((T + p.chunk - 1LL) / p.chunk);
-  const int vec = vec_of(H, (uintptr_t)dy | (uintptr_t)dw);
-  const unsigned slabs = (unsigned)((H + SUM_THREADS * vec - 1) / (SUM_THREADS * vec));
-  if (slabs > 65535 || (H + JOIN_COLS - 1) / JOIN_COLS > 65535) return LB_ERR_SHAPE;
-#define LB_CALL(VEC) LB_LAUNCH(embed_sum_kernel<VEC>, dim3(chunks, slabs), SUM_THREADS, 0, s, p)
+  const int vec = vec_of(H, (uintptr_t)dy | (uintptr_t)dw), width = SUM_THREADS * vec * (vec == 8 ? 1 : 4);      // columns of a CTA
+  SumParams p{(const bf16*)dy, (bf16*)dw, o.ids, o.place, (float*)at, T, H, V, chunk_of(T), scale, 0, 0, 0};
+  const long long chunks = (T + p.chunk - 1LL) / p.chunk, rows = CLEAR_BYTES / (H * 2LL);
+  p.slabs = (unsigned)((H + width - 1LL) / width);
+  p.clear = (int)(rows < 8 ? 8 : rows > MOST_CLEAR ? MOST_CLEAR : rows);
+  const long long sums = chunks * p.slabs, grid = sums + ((long long)V + p.clear - 1) / p.clear;
+  p.sums = (unsigned)sums;
+#define LB_CALL(VEC, K, U) LB_LAUNCH((embed_sum_kernel<VEC, K, U>), (unsigned)grid, SUM_THREADS, 0, s, p)
   switch (vec) {
-    case 8: LB_CALL(8); break;
-    case 2: LB_CALL(2); break;
-    default: LB_CALL(1); break;
+    case 8: LB_CALL(8, 1, 8); break;
+    case 2: LB_CALL(2, 4, 4); break;
+    default: LB_CALL(1, 4, 4); break;
   }
 #undef LB_CALL
-  if (chunks > 1) LB_LAUNCH(embed_join_kernel, dim3(chunks - 1, (unsigned)((H + JOIN_COLS - 1) / JOIN_COLS)), dim3(JOIN_COLS, JOIN_ROWS), 0, s, p);
+  if (chunks > 2) LB_LAUNCH(embed_join_kernel, 2 * lb_num_sms(), JOIN_THREADS, 0, s, p);
   return LB_OK;
 }

@@ -5,9 +5,10 @@
 // x is read in the backward anyway and rstd is made anew from it, so that nothing but x is kept.  Memory bound: x in, y out; x and dy in, dx out.
 // Sums of a head are over the lanes that have it, in 32 bits; dw is added up in 32 bits by every thread over its tokens, then over the CTA's threads and over the CTAs, in
 // their order: the same bits in every run.  y, dx and dw are rounded once.
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace {
+using namespace bw;
 
 constexpr int MAX_AXES = 8, MAX_PAIRS = 128;
 
@@ -21,12 +22,18 @@ struct NormRopeParams {
   const int* positions;          // null: a token's place in its sequence; else axis a of token (b, s) at a * pos_a + b * pos_b + s
   long long pos_a, pos_b;
   float* partial;                // backward, null or [CTAs][2][d]
-  int B, S, hq, hkv, d, rows, share;
+  int B, S, hq, hkv, d, rows;
   float eps;
+  int of_q, groups, share, items;      // groups of q, of a token, of a warp; warps' shares of all tokens
+  FastDiv by_parts, by_S;
+  int plain;                     // one axis, and tables on 16 bytes: a lane's angles are two vectors
   unsigned char axis[MAX_PAIRS];
 };
 
-// A head is P2 lanes', 8 columns each (d / 8 of them, up to the next power of two, work); a warp takes 32 / P2 heads of a token at a time, ROUND loads of each lane in flight.
+// A head is P2 lanes', 8 columns each (d / 8 of them, up to the next power of two, work); a warp takes 32 / P2 heads of q or of k at a time, a group: what is decided for a group is decided
+// for the warp.  Two groups make a round, and the next round (of the next token, behind a token's last) is on its way while one is worked on.
+// The first columns of a lane's four pairs are two pairs of numbers, the second ones two more: everything but sums over lanes is done two numbers at a time.  (One at a time the
+// backward took 305 instructions a group and was bound by them: 16384 tokens, 36 heads of 64 61 us.)
 template <int P2>
 struct Lanes {
   static constexpr int G = 32 / P2;
@@ -46,159 +53,238 @@ __device__ __forceinline__ float head_sum(float x) {
   return x;
 }
 
-// Cosines and sines of the lane's four pairs of a token; a position outside of the tables gives NaN, no access.
-__device__ __forceinline__ void angles(const NormRopeParams& p, int b, int s, int v, bool works, float* cs) {
+struct Pairs { f32x2 a[2], b[2]; };      // first and second columns of four pairs
+__device__ __forceinline__ Pairs pairs_of(const uint4& u) {
+  auto lo = [](uint32_t w) { return __uint_as_float(w << 16); };
+  auto hi = [](uint32_t w) { return __uint_as_float(w & 0xffff0000u); };
+  return Pairs{{pack2(lo(u.x), lo(u.y)), pack2(lo(u.z), lo(u.w))}, {pack2(hi(u.x), hi(u.y)), pack2(hi(u.z), hi(u.w))}};
+}
+__device__ __forceinline__ uint4 packed(const Pairs& p) {
+  uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int pair = works ? v * 4 + i : 0;
-    const int pos = p.positions ? p.positions[p.axis[pair] * p.pos_a + b * p.pos_b + s] : s;
-    const bool there = (unsigned)pos < (unsigned)p.rows;
-    const long long at = (long long)pos * (p.d >> 1) + pair;
-    cs[i] = there ? p.cosT[at] : __int_as_float(0x7fffffff);
-    cs[4 + i] = there ? p.sinT[at] : __int_as_float(0x7fffffff);
+  for (int i = 0; i < 2; i++) {
+    float a0, a1, b0, b1;
+    unpack2(p.a[i], a0, a1);
+    unpack2(p.b[i], b0, b1);
+    const bf162 x = __floats2bfloat162_rn(a0, b0), y = __floats2bfloat162_rn(a1, b1);
+    w[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
+    w[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ Pairs times(const Pairs& x, const Pairs& y) { return Pairs{{mul2(x.a[0], y.a[0]), mul2(x.a[1], y.a[1])}, {mul2(x.b[0], y.b[0]), mul2(x.b[1], y.b[1])}}; }
+__device__ __forceinline__ Pairs times(const Pairs& x, float y) {
+  const f32x2 t = pack2(y, y);
+  return Pairs{{mul2(x.a[0], t), mul2(x.a[1], t)}, {mul2(x.b[0], t), mul2(x.b[1], t)}};
+}
+__device__ __forceinline__ Pairs plus(const Pairs& x, const Pairs& y, const Pairs& z) {      // x y + z
+  return Pairs{{fma2(x.a[0], y.a[0], z.a[0]), fma2(x.a[1], y.a[1], z.a[1])}, {fma2(x.b[0], y.b[0], z.b[0]), fma2(x.b[1], y.b[1], z.b[1])}};
+}
+__device__ __forceinline__ float dot(const Pairs& x, const Pairs& y) {
+  float a, b;
+  unpack2(add2(fma2(x.a[0], y.a[0], mul2(x.b[0], y.b[0])), fma2(x.a[1], y.a[1], mul2(x.b[1], y.b[1]))), a, b);
+  return a + b;
+}
+// Turned by the angles, whose sines are in minus with the other sign; back: the two in each other's place.
+struct Angles { f32x2 c[2], s[2], minus[2]; };
+__device__ __forceinline__ Pairs turned(const Pairs& x, const Angles& t, bool back) {
+  Pairs y;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    y.a[i] = fma2(x.a[i], t.c[i], mul2(x.b[i], back ? t.s[i] : t.minus[i]));
+    y.b[i] = fma2(x.b[i], t.c[i], mul2(x.a[i], back ? t.minus[i] : t.s[i]));
+  }
+  return y;
+}
+// Of the lane's four pairs of a token; a position outside of the tables gives NaN, no access.
+__device__ __forceinline__ Angles angles(const NormRopeParams& p, int b, int s, int v, bool works) {
+  float4 c, n;
+  if (p.plain) {
+    const int pos = p.positions ? p.positions[b * p.pos_b + s] : s;
+    c = n = make_float4(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff), __int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
+    if ((unsigned)pos < (unsigned)p.rows) {
+      const long long at = (long long)pos * (p.d >> 1) + (works ? v * 4 : 0);
+      c = *reinterpret_cast<const float4*>(p.cosT + at);
+      n = *reinterpret_cast<const float4*>(p.sinT + at);
+    }
+  } else {
+    float cs[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int pair = works ? v * 4 + i : 0;
+      const int pos = p.positions ? p.positions[p.axis[pair] * p.pos_a + b * p.pos_b + s] : s;
+      const bool there = (unsigned)pos < (unsigned)p.rows;
+      const long long at = (long long)pos * (p.d >> 1) + pair;
+      cs[i] = there ? p.cosT[at] : __int_as_float(0x7fffffff);
+      cs[4 + i] = there ? p.sinT[at] : __int_as_float(0x7fffffff);
+    }
+    c = make_float4(cs[0], cs[1], cs[2], cs[3]);
+    n = make_float4(cs[4], cs[5], cs[6], cs[7]);
+  }
+  return Angles{{pack2(c.x, c.y), pack2(c.z, c.w)}, {pack2(n.x, n.y), pack2(n.z, n.w)}, {pack2(-n.x, -n.y), pack2(-n.z, -n.w)}};
 }
 
-constexpr int ROUND = 4;
+// Groups [g0, g1) of a token: those of q, then those of k.
+struct Item { int b, s, g0, g1; };
+__device__ __forceinline__ Item item_of(const NormRopeParams& p, int i) {
+  Item t;
+  const int tok = p.by_parts.div(i), part = i - tok * (int)p.by_parts.d;
+  t.b = p.by_S.div(tok);
+  t.s = tok - t.b * p.S;
+  t.g0 = part * p.share;
+  t.g1 = min(p.groups, t.g0 + p.share);
+  return t;
+}
+// Where the lane's vectors of a token lie in one tensor of queries and one of keys.
+template <typename T>
+struct Places {
+  T *q, *k;
+  __device__ Places(T* of_q, T* of_k, const NormRopeHeads& qs, const NormRopeHeads& ks, const Item& t, int mine, int v)
+      : q(of_q + t.b * qs.b + t.s * qs.s + mine * qs.h + v * 8), k(of_k + t.b * ks.b + t.s * ks.s + mine * ks.h + v * 8) {}
+  template <int G>
+  __device__ T* at(bool is_q, int g, const NormRopeHeads& qs, const NormRopeHeads& ks) const { return is_q ? q + g * (G * qs.h) : k + g * (G * ks.h); }
+};
+
+constexpr int THREADS = 256, WARPS = THREADS / 32, ROUND = 2;
 
 template <int P2>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
+__global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
   grid_go();
   grid_wait();
   const Lanes<P2> l(p.d);
   constexpr int G = Lanes<P2>::G;
-  const long long tok = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (tok >= (long long)p.B * p.S) return;
-  const int b = (int)(tok / p.S), s = (int)(tok - (long long)b * p.S), heads = p.hq + p.hkv;
-  const int h0 = (int)blockIdx.y * p.share, h1 = min(heads, h0 + p.share);
-  const bf16 *q = p.q + b * p.qs.b + s * p.qs.s + l.v * 8, *k = p.k + b * p.ks.b + s * p.ks.s + l.v * 8;
-  uint4 a[ROUND];
-  auto load = [&](int h) {
+  const int item = (int)blockIdx.x * WARPS + (int)(threadIdx.x >> 5);
+  if (item >= p.items) return;
+  const Item t = item_of(p, item);
+  // groups where the lane has a head
+  const int nq = l.works ? (p.hq - l.mine + G - 1) / G : 0, nk = l.works ? (p.hkv - l.mine + G - 1) / G : 0;
+  const Places<const bf16> in(p.q, p.k, p.qs, p.ks, t, l.mine, l.v);
+  const Places<bf16> out(p.oq, p.ok, p.oqs, p.oks, t, l.mine, l.v);
+  auto load = [&](uint4* x, int g0) {
 #pragma unroll
     for (int i = 0; i < ROUND; i++) {
-      const int at = h + i * G;
-      a[i] = make_uint4(0, 0, 0, 0);
-      if (at < h1 && l.works) a[i] = __ldcs(reinterpret_cast<const uint4*>(at < p.hq ? q + at * p.qs.h : k + (at - p.hq) * p.ks.h));
+      const bool is_q = g0 + i < p.of_q;
+      const int g = is_q ? g0 + i : g0 + i - p.of_q;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (g0 + i < t.g1 && g < (is_q ? nq : nk)) x[i] = __ldcs(reinterpret_cast<const uint4*>(in.at<G>(is_q, g, p.qs, p.ks)));
     }
   };
-  load(h0 + l.mine);
-  float cs[8], wq[8], wk[8];
+  uint4 x[ROUND], next[ROUND];
+  load(x, t.g0);
   const int col = l.works ? l.v * 8 : 0;
-  unpack8(*reinterpret_cast<const uint4*>(p.wq + col), wq);
-  unpack8(*reinterpret_cast<const uint4*>(p.wk + col), wk);
-  angles(p, b, s, l.v, l.works, cs);
+  const uint4 wq = *reinterpret_cast<const uint4*>(p.wq + col), wk = *reinterpret_cast<const uint4*>(p.wk + col);
+  const Angles turn = angles(p, t.b, t.s, l.v, l.works);
   const float inv_d = 1.f / (float)p.d;
-  bf16 *oq = p.oq + b * p.oqs.b + s * p.oqs.s + l.v * 8, *ok = p.ok + b * p.oks.b + s * p.oks.s + l.v * 8;
-  for (int h = h0; h < h1; h += ROUND * G) {        // (the same for all lanes: they meet in the sums)
-    if (h != h0) load(h + l.mine);
+  for (int g0 = t.g0; g0 < t.g1; g0 += ROUND) {
+    if (g0 + ROUND < t.g1) load(next, g0 + ROUND);
 #pragma unroll
     for (int i = 0; i < ROUND; i++) {
-      if (h + i * G >= h1) break;
-      const int at = h + i * G + l.mine;
-      float f[8], ss = 0.f;
-      unpack8(a[i], f);
-#pragma unroll
-      for (int j = 0; j < 8; j++) ss += f[j] * f[j];
-      const float rstd = rsqrtf(head_sum<P2>(ss) * inv_d + p.eps);
-      const bool is_q = at < p.hq;
-#pragma unroll
-      for (int j = 0; j < 8; j++) f[j] = f[j] * rstd * (is_q ? wq[j] : wk[j]);
-      rope_rotate8(cs, f);
-      if (at < h1 && l.works) *reinterpret_cast<uint4*>(is_q ? oq + at * p.oqs.h : ok + (at - p.hq) * p.oks.h) = pack8(f);
+      if (g0 + i >= t.g1) break;
+      const bool is_q = g0 + i < p.of_q;
+      const int g = is_q ? g0 + i : g0 + i - p.of_q;
+      const Pairs f = pairs_of(x[i]);
+      const float rstd = rsqrtf(head_sum<P2>(dot(f, f)) * inv_d + p.eps);
+      const Pairs y = turned(times(times(f, rstd), pairs_of(is_q ? wq : wk)), turn, false);
+      if (g < (is_q ? nq : nk)) *reinterpret_cast<uint4*>(out.at<G>(is_q, g, p.oqs, p.oks)) = packed(y);
     }
+#pragma unroll
+    for (int i = 0; i < ROUND; i++) x[i] = next[i];
   }
 }
 
 // A warp walks over tokens; every thread keeps its share of dw.
-constexpr int BWD_ROUND = 2, BWD_THREADS = 256;
 template <int P2>
-__global__ void __launch_bounds__(BWD_THREADS, 2) qk_norm_rope_bwd_kernel(const __grid_constant__ NormRopeParams p) {
+__global__ void __launch_bounds__(THREADS, 2) qk_norm_rope_bwd_kernel(const __grid_constant__ NormRopeParams p) {
   grid_go();
   grid_wait();
   const Lanes<P2> l(p.d);
-  constexpr int G = Lanes<P2>::G, WARPS = BWD_THREADS / 32;
-  const int heads = p.hq + p.hkv, parts = (heads + p.share - 1) / p.share;
-  const long long items = (long long)p.B * p.S * parts;
+  constexpr int G = Lanes<P2>::G;
+  const int step = (int)gridDim.x * WARPS;
   const float inv_d = 1.f / (float)p.d;
-  float wq[8], wk[8], aq[8], ak[8];
   const int col = l.works ? l.v * 8 : 0;
-  unpack8(*reinterpret_cast<const uint4*>(p.wq + col), wq);
-  unpack8(*reinterpret_cast<const uint4*>(p.wk + col), wk);
+  const uint4 wq = *reinterpret_cast<const uint4*>(p.wq + col), wk = *reinterpret_cast<const uint4*>(p.wk + col);
+  const int nq = l.works ? (p.hq - l.mine + G - 1) / G : 0, nk = l.works ? (p.hkv - l.mine + G - 1) / G : 0;
+  Pairs aq, ak;
 #pragma unroll
-  for (int j = 0; j < 8; j++) aq[j] = ak[j] = 0.f;
-  for (long long item = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5); item < items; item += (long long)gridDim.x * WARPS) {
-    const long long tok = item / parts;
-    const int part = (int)(item - tok * parts), b = (int)(tok / p.S), s = (int)(tok - (long long)b * p.S);
-    const int h0 = part * p.share, h1 = min(heads, h0 + p.share);
-    const bf16 *q = p.q + b * p.qs.b + s * p.qs.s + l.v * 8, *k = p.k + b * p.ks.b + s * p.ks.s + l.v * 8;
-    const bf16 *dq = p.dq + b * p.dqs.b + s * p.dqs.s + l.v * 8, *dk = p.dk + b * p.dks.b + s * p.dks.s + l.v * 8;
-    bf16 *oq = p.oq + b * p.oqs.b + s * p.oqs.s + l.v * 8, *ok = p.ok + b * p.oks.b + s * p.oks.s + l.v * 8;
-    uint4 x[BWD_ROUND], y[BWD_ROUND];
-    auto load = [&](int h) {
+  for (int i = 0; i < 2; i++) aq.a[i] = aq.b[i] = ak.a[i] = ak.b[i] = 0;
+  auto load = [&](uint4* x, uint4* y, const Item& t, int g0) {
+    const Places<const bf16> in(p.q, p.k, p.qs, p.ks, t, l.mine, l.v), dy(p.dq, p.dk, p.dqs, p.dks, t, l.mine, l.v);
 #pragma unroll
-      for (int i = 0; i < BWD_ROUND; i++) {
-        const int at = h + i * G;
-        x[i] = y[i] = make_uint4(0, 0, 0, 0);
-        if (at < h1 && l.works) {
-          x[i] = __ldcs(reinterpret_cast<const uint4*>(at < p.hq ? q + at * p.qs.h : k + (at - p.hq) * p.ks.h));
-          y[i] = __ldcs(reinterpret_cast<const uint4*>(at < p.hq ? dq + at * p.dqs.h : dk + (at - p.hq) * p.dks.h));
-        }
-      }
-    };
-    load(h0 + l.mine);
-    float cs[8];
-    angles(p, b, s, l.v, l.works, cs);
-    for (int h = h0; h < h1; h += BWD_ROUND * G) {
-      if (h != h0) load(h + l.mine);
-#pragma unroll
-      for (int i = 0; i < BWD_ROUND; i++) {
-        if (h + i * G >= h1) break;
-        const int at = h + i * G + l.mine;
-        const bool is_q = at < p.hq, in = at < h1 && l.works;
-        float f[8], g[8], ss = 0.f, dot = 0.f;
-        unpack8(x[i], f);
-        unpack8(y[i], g);
-        if (in) rope_rotate8(cs, g, true);          // (elsewhere zeros, which a NaN of the tables leaves alone)
-#pragma unroll
-        for (int j = 0; j < 8; j++) ss += f[j] * f[j];
-        ss = head_sum<P2>(ss);                      // (all lanes meet here)
-        const float rstd = in ? rsqrtf(ss * inv_d + p.eps) : 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          f[j] *= rstd;
-          const float gx = g[j] * f[j];
-          if (in) (is_q ? aq[j] : ak[j]) += gx;
-          const float w = is_q ? wq[j] : wk[j];
-          dot += gx * w;
-          g[j] *= w;
-        }
-        dot = head_sum<P2>(dot) * inv_d;
-#pragma unroll
-        for (int j = 0; j < 8; j++) g[j] = rstd * (g[j] - f[j] * dot);
-        if (in) *reinterpret_cast<uint4*>(is_q ? oq + at * p.oqs.h : ok + (at - p.hq) * p.oks.h) = pack8(g);
+    for (int i = 0; i < ROUND; i++) {
+      const bool is_q = g0 + i < p.of_q;
+      const int g = is_q ? g0 + i : g0 + i - p.of_q;
+      x[i] = y[i] = make_uint4(0, 0, 0, 0);
+      if (g0 + i < t.g1 && g < (is_q ? nq : nk)) {
+        x[i] = __ldcs(reinterpret_cast<const uint4*>(in.at<G>(is_q, g, p.qs, p.ks)));
+        y[i] = __ldcs(reinterpret_cast<const uint4*>(dy.at<G>(is_q, g, p.dqs, p.dks)));
       }
     }
+  };
+  // (32 bits of an item: the step goes past the end at most once)
+  unsigned item = blockIdx.x * WARPS + (threadIdx.x >> 5);
+  uint4 x[ROUND], y[ROUND];
+  Angles turn;
+  Item t;
+  if (item < (unsigned)p.items) {
+    t = item_of(p, (int)item);
+    load(x, y, t, t.g0);
+    turn = angles(p, t.b, t.s, l.v, l.works);
+  }
+  while (item < (unsigned)p.items) {
+    const bool more = item + step < (unsigned)p.items;
+    const Item then = more ? item_of(p, (int)(item + step)) : t;
+    const Places<bf16> out(p.oq, p.ok, p.oqs, p.oks, t, l.mine, l.v);
+    for (int g0 = t.g0; g0 < t.g1; g0 += ROUND) {
+      uint4 nx[ROUND], ny[ROUND];
+      if (g0 + ROUND < t.g1) load(nx, ny, t, g0 + ROUND);
+      else if (more) load(nx, ny, then, then.g0);
+#pragma unroll
+      for (int i = 0; i < ROUND; i++) {
+        if (g0 + i >= t.g1) break;
+        const bool is_q = g0 + i < p.of_q;
+        const int g = is_q ? g0 + i : g0 + i - p.of_q;
+        const bool in = g < (is_q ? nq : nk);
+        Pairs f = pairs_of(x[i]);
+        const float ss = head_sum<P2>(dot(f, f));
+        // (0 where the lane has no head, of which there would be NaN with an eps of zero)
+        const float rstd = in ? rsqrtf(ss * inv_d + p.eps) : 0.f;
+        f = times(f, rstd);                                                    // xhat
+        Pairs gx = turned(pairs_of(y[i]), turn, true);
+        if (is_q) aq = plus(gx, f, aq); else ak = plus(gx, f, ak);
+        gx = times(gx, pairs_of(is_q ? wq : wk));
+        const float mean = head_sum<P2>(dot(gx, f)) * inv_d;
+        const f32x2 off = pack2(-mean, -mean);
+        gx = times(Pairs{{fma2(f.a[0], off, gx.a[0]), fma2(f.a[1], off, gx.a[1])}, {fma2(f.b[0], off, gx.b[0]), fma2(f.b[1], off, gx.b[1])}}, rstd);
+        if (in) *reinterpret_cast<uint4*>(out.at<G>(is_q, g, p.oqs, p.oks)) = packed(gx);
+      }
+#pragma unroll
+      for (int i = 0; i < ROUND; i++) { x[i] = nx[i]; y[i] = ny[i]; }
+    }
+    if (more) turn = angles(p, then.b, then.s, l.v, l.works);
+    t = then;
+    item += step;
   }
   if (!p.partial) return;
   // over the heads of a warp, then over the warps of the CTA
   __shared__ float sums[2][WARPS][P2 * 8];
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
+  for (int of = 0; of < 2; of++) {
+    const Pairs& from = of ? ak : aq;
+    float c[8];
 #pragma unroll
-    for (int o = P2; o < 32; o <<= 1) {
-      aq[j] += __shfl_xor_sync(0xffffffffu, aq[j], o);
-      ak[j] += __shfl_xor_sync(0xffffffffu, ak[j], o);
+    for (int i = 0; i < 2; i++) {
+      unpack2(from.a[i], c[4 * i], c[4 * i + 2]);
+      unpack2(from.b[i], c[4 * i + 1], c[4 * i + 3]);
     }
-  }
-  if (l.mine == 0) {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      sums[0][threadIdx.x >> 5][l.v * 8 + j] = aq[j];
-      sums[1][threadIdx.x >> 5][l.v * 8 + j] = ak[j];
+#pragma unroll
+      for (int o = P2; o < 32; o <<= 1) c[j] += __shfl_xor_sync(0xffffffffu, c[j], o);
+      if (l.mine == 0) sums[of][threadIdx.x >> 5][l.v * 8 + j] = c[j];
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * p.d; i += BWD_THREADS) {
+  for (int i = threadIdx.x; i < 2 * p.d; i += THREADS) {
     const int of = i / p.d, c = i - of * p.d;
     float t = 0.f;
 #pragma unroll
@@ -228,12 +314,29 @@ int padded(int d) {
   while (p2 * 8 < d) p2 *= 2;
   return p2;
 }
-// Heads of a warp: all of a token's, or fewer where there are few tokens: one round of loads each at least, eight warps per SM.
-int share_of(long long tokens, int heads, int d, int round) {
-  const int per = 32 / padded(d) * round, most = (heads + per - 1) / per;
+// Groups of a token, and of a warp: all of a token's, or fewer where there are few tokens: one round of loads each at least, eight warps per SM.
+int groups_of(int hq, int hkv, int d) {
+  const int G = 32 / padded(d);
+  return (hq + G - 1) / G + (hkv + G - 1) / G;
+}
+int share_of(long long tokens, int groups) {
+  const int most = (groups + ROUND - 1) / ROUND;
   const long long want = (8LL * lb_num_sms() + tokens - 1) / tokens;
   const int parts = (int)(want < most ? want : most);
-  return (heads + parts - 1) / parts;
+  return (groups + parts - 1) / parts;
+}
+long long items_of(long long tokens, int groups, int share) { return tokens * ((groups + share - 1) / share); }
+int set_items(NormRopeParams& p) {
+  const long long tokens = (long long)p.B * p.S;
+  const int G = 32 / padded(p.d);
+  p.of_q = (p.hq + G - 1) / G;
+  p.groups = groups_of(p.hq, p.hkv, p.d);
+  p.share = share_of(tokens, p.groups);
+  if (items_of(tokens, p.groups, p.share) > 0x7fffffffLL) return LB_ERR_SHAPE;
+  p.items = (int)items_of(tokens, p.groups, p.share);
+  p.by_parts.set((unsigned)((p.groups + p.share - 1) / p.share));
+  p.by_S.set((unsigned)p.S);
+  return LB_OK;
 }
 
 bool bad(const NormRopeHeads& s) { return (s.b | s.s | s.h) % 8 != 0; }
@@ -251,6 +354,8 @@ int fill(NormRopeParams& p, const void* q, const void* k, const void* wq, const 
     if (axes[i] >= n_axes) return LB_ERR_ARG;
     p.axis[i] = axes[i];
   }
+  p.plain = (((uintptr_t)cosT | (uintptr_t)sinT) & 15) == 0;
+  for (int i = 0; i < d / 2; i++) p.plain &= axes[i] == 0;
   return LB_OK;
 }
 
@@ -277,12 +382,8 @@ extern "C" int lb_qk_norm_rope(const void* q, const void* k, void* yq, void* yk,
   p.oq = (bf16*)yq; p.ok = (bf16*)yk;
   p.qs = heads_at(strides); p.ks = heads_at(strides + 3); p.oqs = heads_at(strides + 6); p.oks = heads_at(strides + 9);
   if (bad(p.qs) || bad(p.ks) || bad(p.oqs) || bad(p.oks)) return LB_ERR_SHAPE;
-  const long long tokens = (long long)B * S, blocks = (tokens + 7) / 8;
-  if (blocks > 2147483647LL) return LB_ERR_SHAPE;
-  p.share = share_of(tokens, hq + hkv, d, ROUND);
-  const int parts = (hq + hkv + p.share - 1) / p.share;
-  if (parts > 65535) return LB_ERR_SHAPE;
-#define LB_CALL(P) LB_LAUNCH(qk_norm_rope_kernel<P>, dim3((unsigned)blocks, (unsigned)parts), 256, 0, (cudaStream_t)stream, p)
+  if (const int rc = set_items(p)) return rc;
+#define LB_CALL(P) LB_LAUNCH(qk_norm_rope_kernel<P>, (p.items + WARPS - 1) / WARPS, THREADS, 0, (cudaStream_t)stream, p)
   LB_BY_LANES(d, LB_CALL)
 #undef LB_CALL
   return LB_OK;
@@ -292,8 +393,8 @@ extern "C" int lb_qk_norm_rope(const void* q, const void* k, void* yq, void* yk,
 extern "C" int lb_qk_norm_rope_bwd_ctas(int B, int S, int hq, int hkv, int d) {
   if (B <= 0 || S <= 0 || hq <= 0 || hkv <= 0 || d <= 0 || d % 8 || d > 2 * MAX_PAIRS || (long long)hq + hkv > 0x3fffffff) return 0;
   const long long tokens = (long long)B * S;
-  const int share = share_of(tokens, hq + hkv, d, BWD_ROUND), parts = (hq + hkv + share - 1) / share;
-  const long long want = (tokens * parts + 7) / 8, most = 2LL * lb_num_sms();
+  const int groups = groups_of(hq, hkv, d);
+  const long long want = (items_of(tokens, groups, share_of(tokens, groups)) + WARPS - 1) / WARPS, most = 2LL * lb_num_sms();
   return (int)(want < most ? want : most);
 }
 
@@ -309,8 +410,8 @@ extern "C" int lb_qk_norm_rope_bwd(const void* q, const void* k, const void* dyq
   p.dq = (const bf16*)dyq; p.dk = (const bf16*)dyk; p.oq = (bf16*)dxq; p.ok = (bf16*)dxk; p.partial = (float*)partial;
   p.qs = heads_at(strides); p.ks = heads_at(strides + 3); p.dqs = heads_at(strides + 6); p.dks = heads_at(strides + 9); p.oqs = heads_at(strides + 12); p.oks = heads_at(strides + 15);
   if (bad(p.qs) || bad(p.ks) || bad(p.dqs) || bad(p.dks) || bad(p.oqs) || bad(p.oks)) return LB_ERR_SHAPE;
-  p.share = share_of((long long)B * S, hq + hkv, d, BWD_ROUND);
-#define LB_CALL(P) LB_LAUNCH(qk_norm_rope_bwd_kernel<P>, ctas, BWD_THREADS, 0, (cudaStream_t)stream, p)
+  if (const int rc = set_items(p)) return rc;
+#define LB_CALL(P) LB_LAUNCH(qk_norm_rope_bwd_kernel<P>, ctas, THREADS, 0, (cudaStream_t)stream, p)
   LB_BY_LANES(d, LB_CALL)
 #undef LB_CALL
   if (partial) LB_LAUNCH(qk_norm_rope_dw_kernel, (2 * d + 31) / 32, dim3(32, 32), 0, (cudaStream_t)stream, (const float*)partial, (bf16*)dwq, (bf16*)dwk, ctas, d);
