@@ -30,10 +30,10 @@ struct NormRopeParams {
   unsigned char axis[MAX_PAIRS];
 };
 
-// A head is P2 lanes', 8 columns each (d / 8 of them, up to the next power of two, work); a warp takes 32 / P2 heads of q or of k at a time, a group: what is decided for a group is decided
-// for the warp.  Two groups make a round, and the next round (of the next token, behind a token's last) is on its way while one is worked on.
-// The first columns of a lane's four pairs are two pairs of numbers, the second ones two more: everything but sums over lanes is done two numbers at a time.  (One at a time the
-// backward took 305 instructions a group and was bound by them: 16384 tokens, 36 heads of 64 61 us.)
+// A head is P2 lanes', 8 columns each (d / 8 of them, up to the next power of two, work); a warp takes 32 / P2 heads of q or of k at a time, a group, first those of q, then those of k: what differs
+// between the two is decided outside of the loops.  AHEAD groups are on their way, and pointers are counted up: what bounds simpler forms is instructions, not memory (16384 tokens, 36 heads of
+// 64: heads of q and k in one loop, strides multiplied out and numbers one at a time, 156 a group forward and 305 backward, 32 and 61 us).
+// The first columns of a lane's four pairs are two pairs of numbers, the second ones two more: all but the forward's rotation and sums over lanes is done two numbers at a time.
 template <int P2>
 struct Lanes {
   static constexpr int G = 32 / P2;
@@ -72,31 +72,13 @@ __device__ __forceinline__ uint4 packed(const Pairs& p) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ Pairs times(const Pairs& x, const Pairs& y) { return Pairs{{mul2(x.a[0], y.a[0]), mul2(x.a[1], y.a[1])}, {mul2(x.b[0], y.b[0]), mul2(x.b[1], y.b[1])}}; }
-__device__ __forceinline__ Pairs times(const Pairs& x, float y) {
-  const f32x2 t = pack2(y, y);
-  return Pairs{{mul2(x.a[0], t), mul2(x.a[1], t)}, {mul2(x.b[0], t), mul2(x.b[1], t)}};
-}
-__device__ __forceinline__ Pairs plus(const Pairs& x, const Pairs& y, const Pairs& z) {      // x y + z
-  return Pairs{{fma2(x.a[0], y.a[0], z.a[0]), fma2(x.a[1], y.a[1], z.a[1])}, {fma2(x.b[0], y.b[0], z.b[0]), fma2(x.b[1], y.b[1], z.b[1])}};
-}
 __device__ __forceinline__ float dot(const Pairs& x, const Pairs& y) {
   float a, b;
   unpack2(add2(fma2(x.a[0], y.a[0], mul2(x.b[0], y.b[0])), fma2(x.a[1], y.a[1], mul2(x.b[1], y.b[1]))), a, b);
   return a + b;
 }
-// Turned by the angles, whose sines are in minus with the other sign; back: the two in each other's place.
-struct Angles { f32x2 c[2], s[2], minus[2]; };
-__device__ __forceinline__ Pairs turned(const Pairs& x, const Angles& t, bool back) {
-  Pairs y;
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    y.a[i] = fma2(x.a[i], t.c[i], mul2(x.b[i], back ? t.s[i] : t.minus[i]));
-    y.b[i] = fma2(x.b[i], t.c[i], mul2(x.a[i], back ? t.minus[i] : t.s[i]));
-  }
-  return y;
-}
-// Of the lane's four pairs of a token; a position outside of the tables gives NaN, no access.
+// Angles of the lane's four pairs of a token; a position outside of the tables gives NaN, no access.
+struct Angles { f32x2 c[2], s[2]; };
 __device__ __forceinline__ Angles angles(const NormRopeParams& p, int b, int s, int v, bool works) {
   float4 c, n;
   if (p.plain) {
@@ -121,7 +103,7 @@ __device__ __forceinline__ Angles angles(const NormRopeParams& p, int b, int s, 
     c = make_float4(cs[0], cs[1], cs[2], cs[3]);
     n = make_float4(cs[4], cs[5], cs[6], cs[7]);
   }
-  return Angles{{pack2(c.x, c.y), pack2(c.z, c.w)}, {pack2(n.x, n.y), pack2(n.z, n.w)}, {pack2(-n.x, -n.y), pack2(-n.z, -n.w)}};
+  return Angles{{pack2(c.x, c.y), pack2(c.z, c.w)}, {pack2(n.x, n.y), pack2(n.z, n.w)}};
 }
 
 // Groups [g0, g1) of a token: those of q, then those of k.
@@ -135,161 +117,168 @@ __device__ __forceinline__ Item item_of(const NormRopeParams& p, int i) {
   t.g1 = min(p.groups, t.g0 + p.share);
   return t;
 }
-// Where the lane's vectors of a token lie in one tensor of queries and one of keys.
+// The lane's columns of the first group of a walk.
 template <typename T>
-struct Places {
-  T *q, *k;
-  __device__ Places(T* of_q, T* of_k, const NormRopeHeads& qs, const NormRopeHeads& ks, const Item& t, int mine, int v)
-      : q(of_q + t.b * qs.b + t.s * qs.s + mine * qs.h + v * 8), k(of_k + t.b * ks.b + t.s * ks.s + mine * ks.h + v * 8) {}
-  template <int G>
-  __device__ T* at(bool is_q, int g, const NormRopeHeads& qs, const NormRopeHeads& ks) const { return is_q ? q + g * (G * qs.h) : k + g * (G * ks.h); }
-};
+__device__ __forceinline__ T* place(T* base, const NormRopeHeads& st, const Item& t, int head, int v) { return base + (t.b * st.b + t.s * st.s + head * st.h + v * 8); }
 
-constexpr int THREADS = 256, WARPS = THREADS / 32, ROUND = 2;
+constexpr int THREADS = 256, WARPS = THREADS / 32;
 
 template <int P2>
 __global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
   grid_go();
   grid_wait();
+  constexpr int G = Lanes<P2>::G, AHEAD = 4;
   const Lanes<P2> l(p.d);
-  constexpr int G = Lanes<P2>::G;
   const int item = (int)blockIdx.x * WARPS + (int)(threadIdx.x >> 5);
   if (item >= p.items) return;
   const Item t = item_of(p, item);
-  // groups where the lane has a head
-  const int nq = l.works ? (p.hq - l.mine + G - 1) / G : 0, nk = l.works ? (p.hkv - l.mine + G - 1) / G : 0;
-  const Places<const bf16> in(p.q, p.k, p.qs, p.ks, t, l.mine, l.v);
-  const Places<bf16> out(p.oq, p.ok, p.oqs, p.oks, t, l.mine, l.v);
-  auto load = [&](uint4* x, int g0) {
+  const float inv_d = 1.f / (float)p.d;
+  Angles turn;
+  // groups [lo, hi) of one tensor of `heads` heads
+  auto walk = [&](const bf16* in, const NormRopeHeads& is, bf16* out, const NormRopeHeads& os, const bf16* weight, int heads, int lo, int hi, bool first) {
+    if (lo >= hi) return;
+    const bf16* from = place(in, is, t, lo * G + l.mine, l.v);
+    bf16* to = place(out, os, t, lo * G + l.mine, l.v);
+    const long long from_step = G * is.h, to_step = G * os.h;
+    const int mine = l.works ? min(hi, (heads - l.mine + G - 1) / G) : 0;       // groups up to here have a head of the lane's
+    uint4 x[AHEAD];
+    auto load = [&](uint4& x, int g) {
+      x = make_uint4(0, 0, 0, 0);
+      if (g < mine) x = __ldcs(reinterpret_cast<const uint4*>(from));
+      from += from_step;
+    };
 #pragma unroll
-    for (int i = 0; i < ROUND; i++) {
-      const bool is_q = g0 + i < p.of_q;
-      const int g = is_q ? g0 + i : g0 + i - p.of_q;
-      x[i] = make_uint4(0, 0, 0, 0);
-      if (g0 + i < t.g1 && g < (is_q ? nq : nk)) x[i] = __ldcs(reinterpret_cast<const uint4*>(in.at<G>(is_q, g, p.qs, p.ks)));
+    for (int u = 0; u < AHEAD; u++) load(x[u], lo + u);
+    const Pairs w = pairs_of(*reinterpret_cast<const uint4*>(weight + (l.works ? l.v * 8 : 0)));
+    if (first) turn = angles(p, t.b, t.s, l.v, l.works);
+    // a weight and an angle are one number: y = (w a) c - (w b) s, (w b) c + (w a) s
+    f32x2 ac[2], as[2], bc[2], bs[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      ac[k] = mul2(w.a[k], turn.c[k]);
+      as[k] = mul2(w.a[k], turn.s[k]);
+      bc[k] = mul2(w.b[k], turn.c[k]);
+      bs[k] = mul2(w.b[k], turn.s[k]);
+    }
+    for (int g0 = lo; g0 < hi; g0 += AHEAD) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; u++) {
+        const int g = g0 + u;
+        if (g >= hi) break;
+        const Pairs f = pairs_of(x[u]);
+        if (g0 + AHEAD < hi) load(x[u], g + AHEAD);
+        const float rstd = rsqrtf(head_sum<P2>(dot(f, f)) * inv_d + p.eps);
+        const f32x2 by = pack2(rstd, rstd);
+        Pairs y;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          y.a[k] = mul2(sub2(mul2(f.a[k], ac[k]), mul2(f.b[k], bs[k])), by);
+          y.b[k] = mul2(fma2(f.b[k], bc[k], mul2(f.a[k], as[k])), by);
+        }
+        if (g < mine) *reinterpret_cast<uint4*>(to) = packed(y);
+        to += to_step;
+      }
     }
   };
-  uint4 x[ROUND], next[ROUND];
-  load(x, t.g0);
-  const int col = l.works ? l.v * 8 : 0;
-  const uint4 wq = *reinterpret_cast<const uint4*>(p.wq + col), wk = *reinterpret_cast<const uint4*>(p.wk + col);
-  const Angles turn = angles(p, t.b, t.s, l.v, l.works);
-  const float inv_d = 1.f / (float)p.d;
-  for (int g0 = t.g0; g0 < t.g1; g0 += ROUND) {
-    if (g0 + ROUND < t.g1) load(next, g0 + ROUND);
-#pragma unroll
-    for (int i = 0; i < ROUND; i++) {
-      if (g0 + i >= t.g1) break;
-      const bool is_q = g0 + i < p.of_q;
-      const int g = is_q ? g0 + i : g0 + i - p.of_q;
-      const Pairs f = pairs_of(x[i]);
-      const float rstd = rsqrtf(head_sum<P2>(dot(f, f)) * inv_d + p.eps);
-      const Pairs y = turned(times(times(f, rstd), pairs_of(is_q ? wq : wk)), turn, false);
-      if (g < (is_q ? nq : nk)) *reinterpret_cast<uint4*>(out.at<G>(is_q, g, p.oqs, p.oks)) = packed(y);
-    }
-#pragma unroll
-    for (int i = 0; i < ROUND; i++) x[i] = next[i];
-  }
+  walk(p.q, p.qs, p.oq, p.oqs, p.wq, p.hq, t.g0, min(t.g1, p.of_q), true);
+  walk(p.k, p.ks, p.ok, p.oks, p.wk, p.hkv, max(t.g0 - p.of_q, 0), t.g1 - p.of_q, t.g0 >= p.of_q);
 }
 
-// A warp walks over tokens; every thread keeps its share of dw.
+// A warp walks over tokens.  A thread adds up its share of dw in registers over the heads of q or of k of a token, and over tokens in shared memory.
 template <int P2>
-__global__ void __launch_bounds__(THREADS, 2) qk_norm_rope_bwd_kernel(const __grid_constant__ NormRopeParams p) {
+__global__ void __launch_bounds__(THREADS, 3) qk_norm_rope_bwd_kernel(const __grid_constant__ NormRopeParams p) {
   grid_go();
   grid_wait();
+  constexpr int G = Lanes<P2>::G, AHEAD = 2;
+  __shared__ float2 kept[2][4][THREADS];
   const Lanes<P2> l(p.d);
-  constexpr int G = Lanes<P2>::G;
-  const int step = (int)gridDim.x * WARPS;
   const float inv_d = 1.f / (float)p.d;
-  const int col = l.works ? l.v * 8 : 0;
-  const uint4 wq = *reinterpret_cast<const uint4*>(p.wq + col), wk = *reinterpret_cast<const uint4*>(p.wk + col);
-  const int nq = l.works ? (p.hq - l.mine + G - 1) / G : 0, nk = l.works ? (p.hkv - l.mine + G - 1) / G : 0;
-  Pairs aq, ak;
 #pragma unroll
-  for (int i = 0; i < 2; i++) aq.a[i] = aq.b[i] = ak.a[i] = ak.b[i] = 0;
-  auto load = [&](uint4* x, uint4* y, const Item& t, int g0) {
-    const Places<const bf16> in(p.q, p.k, p.qs, p.ks, t, l.mine, l.v), dy(p.dq, p.dk, p.dqs, p.dks, t, l.mine, l.v);
+  for (int i = 0; i < 4; i++) kept[0][i][threadIdx.x] = kept[1][i][threadIdx.x] = make_float2(0.f, 0.f);
+  // (the step goes past the end once, within 32 bits)
+  for (unsigned item = blockIdx.x * WARPS + (threadIdx.x >> 5); item < (unsigned)p.items; item += gridDim.x * WARPS) {
+    const Item t = item_of(p, (int)item);
+    Angles turn;
+    auto walk = [&](const bf16* in, const NormRopeHeads& is, const bf16* dy, const NormRopeHeads& ds, bf16* out, const NormRopeHeads& os, const bf16* weight, int heads, int lo, int hi, bool first,
+                    float2 (*sums)[THREADS]) {
+      if (lo >= hi) return;
+      const bf16 *from = place(in, is, t, lo * G + l.mine, l.v), *from_dy = place(dy, ds, t, lo * G + l.mine, l.v);
+      bf16* to = place(out, os, t, lo * G + l.mine, l.v);
+      const int mine = l.works ? min(hi, (heads - l.mine + G - 1) / G) : 0;
+      uint4 x[AHEAD], y[AHEAD];
+      auto load = [&](uint4& x, uint4& y, int g) {
+        x = y = make_uint4(0, 0, 0, 0);
+        if (g < mine) {
+          x = __ldcs(reinterpret_cast<const uint4*>(from));
+          y = __ldcs(reinterpret_cast<const uint4*>(from_dy));
+        }
+        from += G * is.h;
+        from_dy += G * ds.h;
+      };
 #pragma unroll
-    for (int i = 0; i < ROUND; i++) {
-      const bool is_q = g0 + i < p.of_q;
-      const int g = is_q ? g0 + i : g0 + i - p.of_q;
-      x[i] = y[i] = make_uint4(0, 0, 0, 0);
-      if (g0 + i < t.g1 && g < (is_q ? nq : nk)) {
-        x[i] = __ldcs(reinterpret_cast<const uint4*>(in.at<G>(is_q, g, p.qs, p.ks)));
-        y[i] = __ldcs(reinterpret_cast<const uint4*>(dy.at<G>(is_q, g, p.dqs, p.dks)));
+      for (int u = 0; u < AHEAD; u++) load(x[u], y[u], lo + u);
+      const Pairs w = pairs_of(*reinterpret_cast<const uint4*>(weight + (l.works ? l.v * 8 : 0)));
+      if (first) turn = angles(p, t.b, t.s, l.v, l.works);
+      Pairs sum;
+#pragma unroll
+      for (int k = 0; k < 2; k++) sum.a[k] = sum.b[k] = 0;
+      for (int g0 = lo; g0 < hi; g0 += AHEAD) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+          const int g = g0 + u;
+          if (g >= hi) break;
+          Pairs f = pairs_of(x[u]), gx;
+          const Pairs r = pairs_of(y[u]);
+          if (g0 + AHEAD < hi) load(x[u], y[u], g + AHEAD);
+          const float ss = head_sum<P2>(dot(f, f));
+          // (0 where the lane has no head, of which there would be NaN with an eps of zero)
+          const float rstd = g < mine ? rsqrtf(ss * inv_d + p.eps) : 0.f;
+          const f32x2 by = pack2(rstd, rstd);
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            f.a[k] = mul2(f.a[k], by);             // xhat
+            f.b[k] = mul2(f.b[k], by);
+            gx.a[k] = fma2(r.a[k], turn.c[k], mul2(r.b[k], turn.s[k]));        // dy turned back
+            gx.b[k] = sub2(mul2(r.b[k], turn.c[k]), mul2(r.a[k], turn.s[k]));
+            sum.a[k] = fma2(gx.a[k], f.a[k], sum.a[k]);
+            sum.b[k] = fma2(gx.b[k], f.b[k], sum.b[k]);
+            gx.a[k] = mul2(gx.a[k], w.a[k]);
+            gx.b[k] = mul2(gx.b[k], w.b[k]);
+          }
+          const float mean = head_sum<P2>(dot(gx, f)) * inv_d;
+          const f32x2 off = pack2(-mean, -mean);
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            gx.a[k] = mul2(fma2(f.a[k], off, gx.a[k]), by);
+            gx.b[k] = mul2(fma2(f.b[k], off, gx.b[k]), by);
+          }
+          if (g < mine) *reinterpret_cast<uint4*>(to) = packed(gx);
+          to += G * os.h;
+        }
       }
-    }
-  };
-  // (32 bits of an item: the step goes past the end at most once)
-  unsigned item = blockIdx.x * WARPS + (threadIdx.x >> 5);
-  uint4 x[ROUND], y[ROUND];
-  Angles turn;
-  Item t;
-  if (item < (unsigned)p.items) {
-    t = item_of(p, (int)item);
-    load(x, y, t, t.g0);
-    turn = angles(p, t.b, t.s, l.v, l.works);
-  }
-  while (item < (unsigned)p.items) {
-    const bool more = item + step < (unsigned)p.items;
-    const Item then = more ? item_of(p, (int)(item + step)) : t;
-    const Places<bf16> out(p.oq, p.ok, p.oqs, p.oks, t, l.mine, l.v);
-    for (int g0 = t.g0; g0 < t.g1; g0 += ROUND) {
-      uint4 nx[ROUND], ny[ROUND];
-      if (g0 + ROUND < t.g1) load(nx, ny, t, g0 + ROUND);
-      else if (more) load(nx, ny, then, then.g0);
+      if (!p.partial) return;
 #pragma unroll
-      for (int i = 0; i < ROUND; i++) {
-        if (g0 + i >= t.g1) break;
-        const bool is_q = g0 + i < p.of_q;
-        const int g = is_q ? g0 + i : g0 + i - p.of_q;
-        const bool in = g < (is_q ? nq : nk);
-        Pairs f = pairs_of(x[i]);
-        const float ss = head_sum<P2>(dot(f, f));
-        // (0 where the lane has no head, of which there would be NaN with an eps of zero)
-        const float rstd = in ? rsqrtf(ss * inv_d + p.eps) : 0.f;
-        f = times(f, rstd);                                                    // xhat
-        Pairs gx = turned(pairs_of(y[i]), turn, true);
-        if (is_q) aq = plus(gx, f, aq); else ak = plus(gx, f, ak);
-        gx = times(gx, pairs_of(is_q ? wq : wk));
-        const float mean = head_sum<P2>(dot(gx, f)) * inv_d;
-        const f32x2 off = pack2(-mean, -mean);
-        gx = times(Pairs{{fma2(f.a[0], off, gx.a[0]), fma2(f.a[1], off, gx.a[1])}, {fma2(f.b[0], off, gx.b[0]), fma2(f.b[1], off, gx.b[1])}}, rstd);
-        if (in) *reinterpret_cast<uint4*>(out.at<G>(is_q, g, p.oqs, p.oks)) = packed(gx);
+      for (int k = 0; k < 4; k++) {
+        float a, b;
+        unpack2(k < 2 ? sum.a[k] : sum.b[k - 2], a, b);
+        const float2 old = sums[k][threadIdx.x];
+        sums[k][threadIdx.x] = make_float2(old.x + a, old.y + b);
       }
-#pragma unroll
-      for (int i = 0; i < ROUND; i++) { x[i] = nx[i]; y[i] = ny[i]; }
-    }
-    if (more) turn = angles(p, then.b, then.s, l.v, l.works);
-    t = then;
-    item += step;
+    };
+    walk(p.q, p.qs, p.dq, p.dqs, p.oq, p.oqs, p.wq, p.hq, t.g0, min(t.g1, p.of_q), true, kept[0]);
+    walk(p.k, p.ks, p.dk, p.dks, p.ok, p.oks, p.wk, p.hkv, max(t.g0 - p.of_q, 0), t.g1 - p.of_q, t.g0 >= p.of_q, kept[1]);
   }
   if (!p.partial) return;
-  // over the heads of a warp, then over the warps of the CTA
-  __shared__ float sums[2][WARPS][P2 * 8];
-#pragma unroll
-  for (int of = 0; of < 2; of++) {
-    const Pairs& from = of ? ak : aq;
-    float c[8];
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      unpack2(from.a[i], c[4 * i], c[4 * i + 2]);
-      unpack2(from.b[i], c[4 * i + 1], c[4 * i + 3]);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-#pragma unroll
-      for (int o = P2; o < 32; o <<= 1) c[j] += __shfl_xor_sync(0xffffffffu, c[j], o);
-      if (l.mine == 0) sums[of][threadIdx.x >> 5][l.v * 8 + j] = c[j];
-    }
-  }
+  // over the heads of a group and the warps: a column is that of the same lane and place in all of them
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * p.d; i += THREADS) {
-    const int of = i / p.d, c = i - of * p.d;
-    float t = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; w++) t += sums[of][w][c];
-    p.partial[(long long)blockIdx.x * 2 * p.d + i] = t;
+    const int of = i / p.d, c = i - of * p.d, pair = (c & 7) >> 1, k = (c & 1) * 2 + (pair >> 1);
+    float total = 0.f;
+    for (int j = c / 8; j < THREADS; j += P2) {
+      const float2 s = kept[of][k][j];
+      total += pair & 1 ? s.y : s.x;
+    }
+    p.partial[(long long)blockIdx.x * 2 * p.d + i] = total;
   }
 }
 
@@ -314,13 +303,13 @@ int padded(int d) {
   while (p2 * 8 < d) p2 *= 2;
   return p2;
 }
-// Groups of a token, and of a warp: all of a token's, or fewer where there are few tokens: one round of loads each at least, eight warps per SM.
+// Groups of a token, and of a warp: all of a token's, or fewer where there are few tokens: two at least, eight warps per SM.
 int groups_of(int hq, int hkv, int d) {
   const int G = 32 / padded(d);
   return (hq + G - 1) / G + (hkv + G - 1) / G;
 }
 int share_of(long long tokens, int groups) {
-  const int most = (groups + ROUND - 1) / ROUND;
+  const int most = (groups + 1) / 2;
   const long long want = (8LL * lb_num_sms() + tokens - 1) / tokens;
   const int parts = (int)(want < most ? want : most);
   return (groups + parts - 1) / parts;
@@ -394,7 +383,7 @@ extern "C" int lb_qk_norm_rope_bwd_ctas(int B, int S, int hq, int hkv, int d) {
   if (B <= 0 || S <= 0 || hq <= 0 || hkv <= 0 || d <= 0 || d % 8 || d > 2 * MAX_PAIRS || (long long)hq + hkv > 0x3fffffff) return 0;
   const long long tokens = (long long)B * S;
   const int groups = groups_of(hq, hkv, d);
-  const long long want = (items_of(tokens, groups, share_of(tokens, groups)) + WARPS - 1) / WARPS, most = 2LL * lb_num_sms();
+  const long long want = (items_of(tokens, groups, share_of(tokens, groups)) + WARPS - 1) / WARPS, most = 3LL * lb_num_sms();      // as many as are resident
   return (int)(want < most ? want : most);
 }
 
