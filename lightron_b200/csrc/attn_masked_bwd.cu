@@ -35,6 +35,11 @@ struct BwdParams {
   float *dq_acc, *dk_acc, *dv_acc;
   int* order;                    // null, or the key blocks (sequence * blocks + block) in the order of their CTAs
   int parts;                     // CTAs of a key block
+  // LIST: pieces of the key blocks' walks {key block, first, length, place of its sums or -1}, longest first; of every key block {place of the first, pieces that leave sums}
+  int4* items;
+  int2* joined;
+  int *n_items, *cut_blocks;     // {how many pieces, how many key blocks in several}, and those
+  int chunk, extra;              // longest piece wanted, pieces beyond one per key block that there is room for
   int acc_d;                     // columns of dq_acc: head_dim in whole pieces of 32
   MaTerms f;
   f32x2 scale2;                  // the scale, twice
@@ -75,8 +80,9 @@ struct Cfg {
 };
 static_assert(Cfg<128>::SMEM <= 232448, "shared memory of a CTA");
 
-// What a CTA leaves: WHOLE dK and dV of a key block, and its share of dQ, added to the fp32 sums; PARTS that, and its share of dK and dV; ALONE all three.
-enum : int { WHOLE, PARTS, ALONE };
+// What a CTA leaves: WHOLE dK and dV of a key block, and its share of dQ, added to the fp32 sums; PARTS that, and its share of dK and dV; ALONE all three; LIST, under a window, dK and dV or its share
+// of them: sinks are seen by all queries of their document, many times those of other keys, and such walks are cut.
+enum : int { WHOLE, PARTS, ALONE, LIST };
 
 // Query blocks of one head that see a key block: [x, y).
 __device__ __forceinline__ int2 query_blocks(const MaParams& p, int b, int n0, bool alone) {
@@ -90,18 +96,125 @@ __device__ __forceinline__ int2 query_blocks(const MaParams& p, int b, int n0, b
 
 // Row statistics, one 1 KB record per (b, h, 128-query block): 128 x -lse * log2(e), then 128 x -scale * D.  Rows without a sum, and rows past Sq, get (-inf, 0), which
 // makes their P and dS zero.  Also clears dQ's accumulator.  D/8 threads per (token, head).
-// With `order`, the last CTA instead sorts the key blocks by the query blocks that see them, most first, for the longest walks to begin first whatever the documents are
+// With `order`, the first CTA instead sorts the key blocks by the query blocks that see them, most first, for the longest walks to begin first whatever the documents are
 // (walks of more than MOST blocks count as equal).  Against the order of a causal mask, main kernel: 8 x 2048, documents of 300, 32 / 4 heads, d 64 199 -> 188 us; 3 x 1531 of
 // 500, 32 / 8 heads, d 128 95 -> 86.
 constexpr int MOST = 1023;
-template <int D>
-__global__ void ma_bwd_prep_kernel(const __grid_constant__ BwdParams pp, const int clear) {
+
+// Entries ahead of each size: count[i + 1] holds how many have size i.
+__device__ __forceinline__ void count_ahead(int* count) {
+  if (threadIdx.x < 32) {
+    int run = 0;
+    for (int k = 0; k < MOST + 2; k += 32) {
+      const int i = k + (int)threadIdx.x;
+      int v = i < MOST + 2 ? count[i] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, v, o);
+        if ((int)threadIdx.x >= o) v += x;
+      }
+      if (i < MOST + 2) count[i] = run + v;
+      run += __shfl_sync(0xffffffffu, v, 31);
+    }
+  }
+}
+
+// One CTA lists the pieces of all walks.  Which of equal pieces comes first is left open; what they are is not.
+__device__ void list_pieces(const BwdParams& pp, int* count) {
+  const MaParams& p = pp.w.f;
+  constexpr int KEPT = 2048;                                   // walks that are looked up once
+  __shared__ int of_warps[32], kept[KEPT], n_cut;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, rep = p.hq / p.hkv;
+  const int n_nblk = (p.Sk + 127) / 128, n = p.B * n_nblk;
+  auto walk_of = [&](int e) {
+    const int2 mb = query_blocks(p, e / n_nblk, (e % n_nblk) * 128, false);
+    return (mb.y - mb.x) * rep;
+  };
+  for (int e = threadIdx.x; e < min(n, KEPT); e += blockDim.x) kept[e] = walk_of(e);
+  if (threadIdx.x == 0) n_cut = 0;
+  __syncthreads();
+  auto walk = [&](int e) { return e < KEPT ? kept[e] : walk_of(e); };
+  // of all threads; in `before`: of those before this one
+  auto sum_of = [&](int v, int& before) {
+    int run = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += x;
+    }
+    __syncthreads();
+    if (lane == 31) of_warps[warp] = run;
+    __syncthreads();
+    int all = 0, ahead = 0;
+    for (int w = 0; w < warps; w++) {
+      if (w == warp) ahead = all;
+      all += of_warps[w];
+    }
+    before = ahead + run - v;
+    return all;
+  };
+  const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x, a = min(n, (int)threadIdx.x * per), end = min(n, a + per);
+  // pieces twice as long until there is room for all
+  int length = pp.chunk, beyond = 0, before;
+  for (;; length *= 2) {
+    int more = 0;
+    for (int e = a; e < end; e++) more += max((walk(e) + length - 1) / length - 1, 0);
+    beyond = sum_of(more, before);
+    if (beyond <= pp.extra) break;
+  }
+  auto cut = [&](int e, int& its, int& pieces, int& share) {
+    its = walk(e);
+    pieces = max((its + length - 1) / length, 1);
+    share = (its + pieces - 1) / pieces;
+  };
+  auto bucket = [&](int size) { return MOST - min(size, MOST); };
+  for (int i = threadIdx.x; i < MOST + 2; i += blockDim.x) count[i] = 0;
+  __syncthreads();
+  int sums = 0, its, pieces, share;
+  for (int e = a; e < end; e++) {
+    cut(e, its, pieces, share);
+    if (pieces > 1) {
+      atomicAdd(&count[bucket(share) + 1], pieces - 1);
+      sums += pieces;
+    }
+    atomicAdd(&count[bucket(its - (pieces - 1) * share) + 1], 1);
+  }
+  sum_of(sums, before);
+  count_ahead(count);
+  __syncthreads();
+  for (int e = a; e < end; e++) {
+    cut(e, its, pieces, share);
+    if (pieces > 1) {
+      const int at = atomicAdd(&count[bucket(share)], pieces - 1);
+      for (int k = 0; k + 1 < pieces; k++) pp.items[at + k] = make_int4(e, k * share, share, before + k);
+    }
+    pp.items[atomicAdd(&count[bucket(its - (pieces - 1) * share)], 1)] = make_int4(e, (pieces - 1) * share, its - (pieces - 1) * share, pieces > 1 ? before + pieces - 1 : -1);
+    pp.joined[e] = make_int2(before, pieces > 1 ? pieces : 0);
+    if (pieces > 1) {
+      before += pieces;
+      pp.cut_blocks[atomicAdd(&n_cut, 1)] = e;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    pp.n_items[0] = n + beyond;
+    pp.n_items[1] = n_cut;
+  }
+}
+
+// LISTED: the first CTA lists the pieces (its registers spill: with as many as it would like, 60 for 32, the others, which are memory's, took 66 us instead of 52 at 1 x 8192, 32 heads, d 128).
+template <int D, bool LISTED>
+__global__ void __launch_bounds__(256, LISTED ? 8 : 1) ma_bwd_prep_kernel(const __grid_constant__ BwdParams pp, const int clear) {
   grid_go();
   grid_wait();
   const MaParams& p = pp.w.f;
-  const int workers = (int)gridDim.x - (pp.order ? 1 : 0);
-  if ((int)blockIdx.x == workers) {
+  const int planners = LISTED || pp.order ? 1 : 0, workers = (int)gridDim.x - planners;
+  if ((int)blockIdx.x < planners) {                            // (the first: what it does is a chain)
     __shared__ int count[MOST + 2];
+    if constexpr (LISTED) {
+      list_pieces(pp, count);
+      return;
+    }
     const int n_nblk = (p.Sk + 127) / 128, n = p.B * n_nblk;
     auto size = [&](int e) {
       const int2 mb = query_blocks(p, e / n_nblk, (e % n_nblk) * 128, false);
@@ -111,20 +224,7 @@ __global__ void ma_bwd_prep_kernel(const __grid_constant__ BwdParams pp, const i
     __syncthreads();
     for (int e = threadIdx.x; e < n; e += blockDim.x) atomicAdd(&count[size(e) + 1], 1);
     __syncthreads();
-    if (threadIdx.x < 32) {                                    // entries ahead of each size
-      int run = 0;
-      for (int k = 0; k < MOST + 2; k += 32) {
-        const int i = k + (int)threadIdx.x;
-        int v = i < MOST + 2 ? count[i] : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int x = __shfl_up_sync(0xffffffffu, v, o);
-          if ((int)threadIdx.x >= o) v += x;
-        }
-        if (i < MOST + 2) count[i] = run + v;
-        run += __shfl_sync(0xffffffffu, v, 31);
-      }
-    }
+    count_ahead(count);
     __syncthreads();
     for (int e = threadIdx.x; e < n; e += blockDim.x) pp.order[atomicAdd(&count[size(e)], 1)] = e;
     return;
@@ -135,7 +235,7 @@ __global__ void ma_bwd_prep_kernel(const __grid_constant__ BwdParams pp, const i
   const int rpb = blockDim.x / TPR;                            // rows per block and iteration
   const int sub = threadIdx.x % TPR;
   // every thread of the block runs the same number of iterations, so the shuffles see whole warps
-  for (long long base = (long long)blockIdx.x * rpb; base < total; base += (long long)workers * rpb) {
+  for (long long base = (long long)((int)blockIdx.x - planners) * rpb; base < total; base += (long long)workers * rpb) {
     const long long idx = base + threadIdx.x / TPR;
     const bool live = idx < total;
     float s = 0.f;
@@ -185,24 +285,42 @@ __global__ void ma_convert_kernel(const __grid_constant__ BwdParams pp) {
     const int lane = threadIdx.x & 31;
     constexpr int G = D / 8;
     const int n_nblk = (p.Sk + 127) / 128, rep = p.hq / p.hkv, pairs = p.hkv * p.B;
-    const long long pieces = 2LL * pairs * n_nblk * 4 * G;
+    const long long pieces = (pp.items ? 2LL * p.hkv * pp.n_items[1] : 2LL * pairs * n_nblk) * 4 * G;
     for (; start < 32 * pieces; start += threads) {            // (dK or dV, key block, pair, quad, 8 columns)
       const long long w = start >> 5;
       const int g = (int)(w % G), quad = (int)((w / G) & 3);
       const long long tile = w / (4 * G);
-      const int pair = (int)(tile % pairs), block = (int)((tile / pairs) % n_nblk), dv = (int)(tile / pairs / n_nblk), b = pair / p.hkv;
+      int pair = (int)(tile % pairs), block = (int)((tile / pairs) % n_nblk), dv = (int)(tile / pairs / n_nblk);
+      if (pp.items) {
+        const long long of = tile / p.hkv;                     // (key blocks in several pieces alone)
+        const int e = pp.cut_blocks[of >> 1];
+        dv = (int)(of & 1);
+        block = e % n_nblk;
+        pair = e / n_nblk * p.hkv + (int)(tile % p.hkv);
+      }
+      const int b = pair / p.hkv;
       const int row = block * 128 + quad * 32 + lane;
       if (row >= p.Sk || g * 8 >= p.d) continue;
-      const int2 mb = query_blocks(p, b, block * 128, false);
-      const int its = (mb.y - mb.x) * rep, share = (its + pp.parts - 1) / pp.parts;
-      const int used = share ? (its + share - 1) / share : 0;
-      const float4* from = reinterpret_cast<const float4*>(dv ? pp.dv_acc : pp.dk_acc) + ((long long)block * pairs + pair) * pp.parts * (32 * D) + (quad * (D / 4) + 2 * g) * 32 + lane;
+      int used;
+      long long first, apart = 1;                              // place of the first part, and from one to the next
+      if (pp.items) {
+        const int2 j = pp.joined[b * n_nblk + block];
+        used = j.y;
+        apart = p.hkv;
+        first = (long long)j.x * p.hkv + pair % p.hkv;
+      } else {
+        const int2 mb = query_blocks(p, b, block * 128, false);
+        const int its = (mb.y - mb.x) * rep, share = (its + pp.parts - 1) / pp.parts;
+        used = share ? (its + share - 1) / share : 0;
+        first = ((long long)block * pairs + pair) * pp.parts;
+      }
+      const float4* from = reinterpret_cast<const float4*>(dv ? pp.dv_acc : pp.dk_acc) + first * (32 * D) + (quad * (D / 4) + 2 * g) * 32 + lane;
       float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       for (int part = 0; part < used; part += 4) {
         float4 x[4][2];
 #pragma unroll
         for (int u = 0; u < 4; u++)
-          if (part + u < used) { x[u][0] = from[(long long)(part + u) * (32 * D)]; x[u][1] = from[(long long)(part + u) * (32 * D) + 32]; }
+          if (part + u < used) { x[u][0] = from[(part + u) * apart * (32 * D)]; x[u][1] = from[(part + u) * apart * (32 * D) + 32]; }
 #pragma unroll
         for (int u = 0; u < 4; u++)
           if (part + u < used) {
@@ -312,6 +430,13 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
   volatile int* abort_flag = s_abort;
   grid_wait();
 
+  [[maybe_unused]] int4 piece = make_int4(0, 0, 0, 0);          // (a CTA without one leaves nothing)
+  if constexpr (FORM == LIST) {
+    const int i = (int)blockIdx.x / p.hkv;
+    if (i < *pp.n_items) piece = pp.items[i];
+    nblk = piece.x % n_nblk;
+    pair = piece.x / n_nblk * p.hkv + (int)blockIdx.x % p.hkv;
+  }
   if (FORM == WHOLE && pp.order) {
     const int e = pp.order[(int)blockIdx.x / p.hkv];
     nblk = e % n_nblk;
@@ -328,8 +453,14 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     it_first = min(total_it, part * share);
     total_it = min(share, total_it - it_first);
   }
-  const int h_first = hk * rep + (FORM == PARTS && total_it ? it_first / per_head : 0);
-  const int mb_start = mb_first + (FORM == PARTS && total_it ? it_first % per_head : 0);
+  if constexpr (FORM == LIST) {
+    it_first = piece.y;
+    total_it = piece.z;
+  }
+  constexpr bool CUT = FORM == PARTS || FORM == LIST;
+  const int h_first = hk * rep + (CUT && total_it ? it_first / per_head : 0);
+  const int mb_start = mb_first + (CUT && total_it ? it_first % per_head : 0);
+  const bool leaves_sums = FORM == PARTS || (FORM == LIST && piece.w >= 0);
 
   if (warp < 4) reg_dec<C::REGS_ISSUE>();
   if (warp == 0) {
@@ -643,10 +774,11 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     }
     // dQ of the last block is the last MMA: everything has finished
     if (ok && total_it > 0) ok = mbar_wait(dq_full, (uint32_t)(total_it - 1) & 1u, abort_flag);
-    if (FORM == PARTS && ok && total_it > 0) {
+    if (CUT && leaves_sums && ok && total_it > 0) {
       // to this CTA's place, 32 columns at a time
       fence_after();
-      float* sum = (wg ? pp.dk_acc : pp.dv_acc) + (((long long)nblk * p.hkv * p.B + pair) * pp.parts + part) * (128 * D) + quad * (32 * D);
+      const long long place = FORM == LIST ? (long long)piece.w * p.hkv + hk : ((long long)nblk * p.hkv * p.B + pair) * pp.parts + part;
+      float* sum = (wg ? pp.dk_acc : pp.dv_acc) + place * (128 * D) + quad * (32 * D);
       uint8_t* out = smem + (wg ? C::OFF_V : C::OFF_K) + quad * C::STG_BYTES;
 #pragma unroll 1
       for (int c = 0; c < D / 32 && c * 32 < p.d; c++) {
@@ -666,7 +798,7 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         }
       }
       if (lane == 0) bulk_wait_read_but<0>();        // nothing reads shared memory after the CTA's end
-    } else if (FORM != PARTS && ok && total_it > 0) {
+    } else if (FORM != PARTS && !leaves_sums && ok && total_it > 0) {
       // through shared memory (K's tile for dV, V's for dK: nothing reads them any more), 64 columns of 32 keys at a time
       fence_after();
 #pragma unroll 1
@@ -691,7 +823,7 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         }
       }
       if (lane == 0) bulk_wait_read_but<0>();        // nothing reads shared memory after the CTA's end
-    } else if (FORM != PARTS && total_it == 0 && key < p.Sk) {
+    } else if (FORM != PARTS && !leaves_sums && total_it == 0 && key < p.Sk) {
       // no query sees these keys: their gradients are zero
       const MaStrides& s = wg ? pp.w.dks : pp.w.dvs;
       bf16* orow = (wg ? pp.w.dk : pp.w.dv) + b * s.b + key * s.s + hk * s.h;
@@ -731,6 +863,8 @@ int launch_form(const CUtensorMap* m, const BwdParams& p, unsigned grid, cudaStr
   return bias ? launch<D, FORM, false, true>(m, p, grid, s) : launch<D, FORM, false, false>(m, p, grid, s);
 }
 
+long long order_ints(const MaParams& p) { return (long long)p.B * ((p.Sk + 127) / 128); }
+
 // CTAs of a key block, for its walk over query blocks of all heads of the group.  In query blocks: a CTA's fixed part is some 6, leaving dK / dV in fp32 instead of
 // writing them 3 and their conversion 2 more (the figures of the causal backward's model); where the mask comes from the device its lengths are not known
 // here, and those of a causal mask are taken.  Whole / parts, all kernels as a graph, us, causal: 2 x 2000, 16 / 2 heads, d 64 213 / 78; 1 x 2000, 16 / 4, d 128 156 / 79; 1 x 8192, 8 / 2, d 128
@@ -751,6 +885,33 @@ int parts_of(int B, int Sq, int Sk, int hq, int hkv, int causal, int sms) {
   return best;
 }
 
+// Under a window: the longest piece of a walk, and how many pieces there may be beyond one per key block.  By the model of parts_of(), for keys that queries near them see and for blocks of sinks,
+// which all queries behind them see; where the mask comes from the device documents cut the walks shorter, and there are more, shorter ones of sinks: then pieces may get twice as long.
+struct Pieces { int length, extra; };
+Pieces pieces_of(const MaParams& p, int sms) {
+  const int n_mblocks = (p.Sq + 127) / 128, n_nblk = (p.Sk + 127) / 128, rep = p.hq / p.hkv;
+  const long long pairs = (long long)p.hkv * p.B, span = 128 + (p.causal ? 1LL : 2LL) * (p.window - 1LL);
+  // (key and query blocks that begin at the same places meet in one block fewer)
+  const long long most = (span + 127) / 128 + ((p.Sk - p.Sq) % 128 || !p.causal ? 1 : 0);
+  const long long near = std::min<long long>(most, n_mblocks) * rep, far = (long long)n_mblocks * rep;
+  const long long n_far = std::min<long long>((p.sinks + 127) / 128, n_nblk), n_near = n_nblk - n_far;
+  double best_time = 0.0;
+  Pieces best{(int)far, 0};
+  auto look = [&](long long length) {
+    const long long a = (near + length - 1) / length, b = (far + length - 1) / length;
+    const long long extra = n_near * (a - 1) + n_far * (b - 1);
+    const double work = (double)(n_near * (near + a * (a > 1 ? 9 : 6)) + n_far * (far + b * (b > 1 ? 9 : 6))) * pairs / sms;
+    const double time = std::max(std::max((near + a - 1) / a, n_far ? (far + b - 1) / b : 0) + 9.0, 1.1 * work) + (extra ? 1.0 : 0.0);
+    if (best_time == 0.0 || time < best_time) {
+      best_time = time;
+      best = Pieces{(int)length, (int)std::min<long long>((2 * extra + (p.sinks ? 4 : 0)) * p.B, 1 << 24)};
+    }
+  };
+  for (long long parts = 1; parts <= std::min<long long>(far, 64); parts++) look((far + parts - 1) / parts);
+  for (long long parts = 1; parts <= std::min<long long>(near, 32); parts++) look((near + parts - 1) / parts);
+  return best;
+}
+
 template <int D>
 int launch_bwd(BwdParams& p, cudaStream_t s) {
   const MaParams& a = p.w.f;
@@ -767,17 +928,18 @@ int launch_bwd(BwdParams& p, cudaStream_t s) {
   // Up to 128 keys a query block's dQ comes from one CTA, which writes it: nothing to clear, to add to and to convert.  Added / written, as a graph, us: 4 x 128, 12 heads, d 64 13.2 / 10.3,
   // 8 x 128, 32 heads 24.6 / 18.5, 32 x 128, 32 / 8 heads 54 / 41; 8 x 100, 16 heads, d 128 18.6 / 14.4.
   const bool alone = a.Sk <= 128;
-  const long long grid = (long long)((a.Sk + 127) / 128) * a.hkv * a.B * p.parts;
+  const long long grid = p.items ? (order_ints(a) + p.extra) * a.hkv : (long long)((a.Sk + 127) / 128) * a.hkv * a.B * p.parts;
   if (grid > 2147483647LL) return LB_ERR_SHAPE;
   const long long rows = (long long)a.B * ((a.Sq + 127) / 128 * 128) * a.hq;
   const long long rows_per_block = 256 / (D / 8), cap = lb_num_sms() * 16;
   const long long pblocks = (rows + rows_per_block - 1) / rows_per_block;
-  LB_LAUNCH(ma_bwd_prep_kernel<D>, (int)(pblocks < cap ? pblocks : cap) + (p.order ? 1 : 0), 256, 0, s, p, !alone);
-  rc = p.parts > 1 ? launch_form<D, PARTS>(m, p, (unsigned)grid, s) : alone ? launch_form<D, ALONE>(m, p, (unsigned)grid, s) : launch_form<D, WHOLE>(m, p, (unsigned)grid, s);
+  LB_LAUNCH((p.items ? ma_bwd_prep_kernel<D, true> : ma_bwd_prep_kernel<D, false>), (int)(pblocks < cap ? pblocks : cap) + (p.order || p.items ? 1 : 0), 256, 0, s, p, !alone);
+  rc = p.items ? launch_form<D, LIST>(m, p, (unsigned)grid, s) : p.parts > 1 ? launch_form<D, PARTS>(m, p, (unsigned)grid, s) : alone ? launch_form<D, ALONE>(m, p, (unsigned)grid, s) : launch_form<D, WHOLE>(m, p, (unsigned)grid, s);
   if (rc || alone) return rc;
-  const long long part_rows = p.parts > 1 ? 2LL * a.B * ((a.Sk + 127) / 128 * 128) * a.hkv : 0;
+  const bool cut = p.parts > 1 || p.items;
+  const long long part_rows = cut ? 2LL * a.B * ((a.Sk + 127) / 128 * 128) * a.hkv : 0;
   const long long cblocks = (rows * (D / 32) + part_rows * (D / 8) + 255) / 256;      // (a thread takes 32 values of dQ)
-  LB_LAUNCH(p.parts > 1 ? ma_convert_kernel<D, true> : ma_convert_kernel<D, false>, (int)(cblocks < cap ? cblocks : cap), 256, 0, s, p);
+  LB_LAUNCH(cut ? ma_convert_kernel<D, true> : ma_convert_kernel<D, false>, (int)(cblocks < cap ? cblocks : cap), 256, 0, s, p);
   return LB_OK;
 }
 
@@ -789,11 +951,18 @@ long long part_floats(const MaParams& p, int parts) {
   return parts > 1 ? (long long)p.B * p.hkv * ((p.Sk + 127) / 128) * parts * 128 * (p.d <= 64 ? 64 : 128) : 0;
 }
 
-long long order_ints(const MaParams& p) { return (long long)p.B * ((p.Sk + 127) / 128); }
+// (pieces that leave sums: two for each one beyond the first of its key block, at most)
+long long piece_floats(const MaParams& p, const Pieces& c) { return 2LL * c.extra * p.hkv * 128 * (p.d <= 64 ? 64 : 128); }
+// (without a mask and with nothing to cut, the key blocks' order is known)
+bool listed(const MaParams& p, const Pieces& c) { return p.window > 0 && p.Sk > 128 && (c.extra > 0 || p.qb); }
 
 }  // namespace
 
 long long ma_bwd_ws_bytes(const MaParams& p) {
+  if (p.window > 0) {
+    const Pieces c = pieces_of(p, lb_num_sms());
+    return (stats_floats(p) + dq_floats(p) + 2 * piece_floats(p, c) + 4 * (order_ints(p) + c.extra) + 3 * order_ints(p) + 4) * (long long)sizeof(float);
+  }
   return (stats_floats(p) + dq_floats(p) + 2 * part_floats(p, parts_of(p.B, p.Sq, p.Sk, p.hq, p.hkv, p.causal, lb_num_sms())) + order_ints(p)) * (long long)sizeof(float);
 }
 
@@ -801,14 +970,28 @@ int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s) {
   const MaParams& a = w.f;
   BwdParams p;
   p.w = w;
-  p.parts = parts_of(a.B, a.Sq, a.Sk, a.hq, a.hkv, a.causal, lb_num_sms());
+  p.items = nullptr;
   p.acc_d = acc_columns(a.d);
   p.dq_acc = w.stats + stats_floats(a);
   p.dk_acc = p.dq_acc + dq_floats(a);
-  p.dv_acc = p.dk_acc + part_floats(a, p.parts);
-  p.order = a.kb && p.parts == 1 && a.Sk > 128 ? reinterpret_cast<int*>(p.dv_acc + part_floats(a, p.parts)) : nullptr;
   p.f.set(a, false, twice);
   p.scale2 = twice(a.scale);
+  const Pieces c = a.window > 0 ? pieces_of(a, lb_num_sms()) : Pieces{0, 0};
+  p.parts = 1;
+  p.order = nullptr;
+  if (listed(a, c)) {
+    p.chunk = c.length;
+    p.extra = c.extra;
+    p.dv_acc = p.dk_acc + piece_floats(a, c);
+    p.items = reinterpret_cast<int4*>(p.dv_acc + piece_floats(a, c));
+    p.joined = reinterpret_cast<int2*>(p.items + order_ints(a) + c.extra);
+    p.n_items = reinterpret_cast<int*>(p.joined + order_ints(a));
+    p.cut_blocks = p.n_items + 4;
+    return a.d <= 64 ? launch_bwd<64>(p, s) : launch_bwd<128>(p, s);
+  }
+  if (!a.window) p.parts = parts_of(a.B, a.Sq, a.Sk, a.hq, a.hkv, a.causal, lb_num_sms());
+  p.dv_acc = p.dk_acc + part_floats(a, p.parts);
+  p.order = a.kb && p.parts == 1 && a.Sk > 128 ? reinterpret_cast<int*>(p.dv_acc + part_floats(a, p.parts)) : nullptr;
   return a.d <= 64 ? launch_bwd<64>(p, s) : launch_bwd<128>(p, s);
 }
 

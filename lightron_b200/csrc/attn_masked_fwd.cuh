@@ -31,6 +31,7 @@
 // Under a window (WINDOW) a tile's keys are at most two ranges: the window's, from the first key near its first row to the last that any of its rows sees, and before it the sinks of the document
 // that the tile begins in (a document that begins inside of the tile has its sinks in the window's range).  Their blocks come one after the other; a block of the sinks is cut off where
 // the window's range begins.  Where one range over both takes no more blocks, it is one.
+// Few queries (WINDOW, less than 128 of them): a tile's rows are the 2^shift heads of a group for each query, so that K and V are read once for all of them.
 #pragma once
 #include "attn_masked.cuh"
 #include "tcgen05.cuh"
@@ -51,7 +52,8 @@ struct FwdParams {
   int tiles_x;                   // query tiles (128 rows) per (batch, head)
   int steal;                     // CTAs go on with entries that have not been started
   int group;                     // (batch, head) pairs whose tiles are ordered together
-  FastDiv by_grp, by_group, by_last, by_hq, by_rep;    // entries of a group, heads of a group / of the last one, hq, hq / hkv
+  FastDiv by_grp, by_group, by_last, by_hq, by_rep;    // entries of a group, heads of a group / of the last one, heads, heads / hkv
+  int shift, heads;              // rows of a query, as a power of two; hq >> shift
   MaTerms f;
   int splits;                    // CTAs of a tile, each with a share of its key blocks, which leave parts
   float *part_o, *part_s;        // [tile][split] x [D / 4][128 rows][4] fp32, and x [reference, sum, rounded sum][128 rows]
@@ -180,7 +182,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
   // One entry per (batch, head, query tile): the last tiles, which see most under a causal mask, of all heads of a group first; a group is as many heads as keep
   // their K / V in L2 together.  A resident CTA goes on with entries that have not been started (cluster launch control).
   volatile int* abort_flag = s_abort;
-  const int off = p.Sk - p.Sq;
+  const int off = p.Sk - p.Sq, shift = WINDOW ? pp.shift : 0;
   struct Tile { int m0, b, h, hk, key0, nb, split, skip, far0, nf; };      // WINDOW: blocks left to other CTAs; sinks: first key and blocks, of all
   auto tile_of = [&](int cid) {
     Tile t;
@@ -188,15 +190,15 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     if (pp.splits > 1) { t.split = cid % pp.splits; cid /= pp.splits; }
     const int grp = pp.by_grp.div(cid);
     const int in_grp = cid - grp * (int)pp.by_grp.d;
-    const FastDiv& heads = (grp + 1) * pp.group <= p.hq * p.B ? pp.by_group : pp.by_last;
+    const FastDiv& heads = (grp + 1) * pp.group <= pp.heads * p.B ? pp.by_group : pp.by_last;
     const int row = heads.div(in_grp);
     const int bh = grp * pp.group + in_grp - row * (int)heads.d;
     t.m0 = (pp.tiles_x - 1 - row) * C::BM;
     t.b = pp.by_hq.div(bh);
-    t.h = bh - t.b * p.hq;
+    t.h = bh - t.b * pp.heads;
     t.hk = pp.by_rep.div(t.h);
     if constexpr (WINDOW) {
-      const MaSees first = ma_sees(p, t.b, t.m0), last = ma_sees(p, t.b, min(t.m0 + C::BM, p.Sq) - 1);
+      const MaSees first = ma_sees(p, t.b, t.m0 >> pp.shift), last = ma_sees(p, t.b, min((t.m0 + C::BM - 1) >> pp.shift, p.Sq - 1));
       const int end = max(last.near.y, last.first.y), far_end = min(first.first.y, first.near.x);
       t.far0 = first.first.x;
       t.key0 = first.near.x;
@@ -287,7 +289,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           if (!mbar_wait(q_empty, (uint32_t)(n & 1) ^ 1u, abort_flag)) { ok = false; break; }
           mbar_expect_tx(q_full, C::ATOMS * C::SLOT_BYTES);
 #pragma unroll
-          for (int a = 0; a < C::ATOMS; a++) tma_load_4d(sbase + C::OFF_Q + a * C::SLOT_BYTES, &tq, a * 64, t.h, t.m0, t.b, q_full);
+          for (int a = 0; a < C::ATOMS; a++) tma_load_4d(sbase + C::OFF_Q + a * C::SLOT_BYTES, &tq, a * 64, t.h << shift, t.m0 >> shift, t.b, q_full);
           for (int j = 0; j < t.nb && ok; j++) {
             const int key0 = key_of(t, j);
 #pragma unroll
@@ -489,7 +491,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     Tile t = tile_of((int)blockIdx.x);
     // (rows past the last one are never stored: they are left unmasked)
     auto keys_of = [&](const Tile& at) {
-      const int row = at.m0 + quad * 32 + lane;
+      const int row = (at.m0 + quad * 32 + lane) >> shift;
       if (row >= p.Sq) return MaSees{make_int2(0, 0x7fffffff), make_int2(0, 0)};
       if constexpr (WINDOW) return ma_sees(p, at.b, row);
       return MaSees{ma_keys(p, at.b, row), make_int2(0, 0)};
@@ -497,11 +499,13 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     MaSees sees = keys_of(t);
     for (int n = 0; ok; n++) {
       const int2 see = sees.near;
-      const int nb = t.nb, row = t.m0 + quad * 32 + lane, warp_at = t.m0 + quad * 32 + off;      // the row's place is row + off
+      // (row: of the queries; its place is row + off)
+      const int nb = t.nb, row = (t.m0 + quad * 32 + lane) >> shift, warp_at = ((t.m0 + quad * 32) >> shift) + off;
+      [[maybe_unused]] const int warp_end = warp_at + (31 >> shift), head = (t.h << shift) + (lane & ((1 << shift) - 1));
       [[maybe_unused]] float slope2 = 0.f;
       [[maybe_unused]] bool left_only = true;      // no row of the warp sees a key behind its own
       if constexpr (BIAS) {
-        slope2 = p.slopes ? p.slopes[t.h] * LOG2E : 0.f;
+        slope2 = p.slopes ? p.slopes[head] * LOG2E : 0.f;
         left_only = __all_sync(0xffffffffu, row >= p.Sq || (WINDOW ? max(see.y, sees.first.y) : see.y) <= row + off + 1);
       }
       if (lane == 0) bulk_wait_read_but<0>();      // the last tile's O has left the place of the meetings
@@ -535,7 +539,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         if (!C::P_ALIAS) arrive(s_free);                 // S may be overwritten by the next key block
         const bool pv_ready = !C::P_ALIAS && j > 0 && mbar_test_wait(pv_done, (g - 1) & 1u);   // asked ahead of its use
         if constexpr (MADE) {
-          const int side = left_only || c0 + 63 <= warp_at ? 1 : c0 >= warp_at + 31 ? -1 : 0;
+          const int side = left_only || c0 + 63 <= warp_at ? 1 : c0 >= warp_end ? -1 : 0;
           scores64<CAP, BIAS>(r, pp, slope2, side, c0 - (row + off), top);
         }
         if (need_mask) {
@@ -551,7 +555,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         // LINEAR: bias at column i is slope * (c0 + i - place); with keys on both sides of a row (slope 0) it is in r from here on
         [[maybe_unused]] float slope = 0.f;
         if constexpr (LINEAR) {
-          slope = left_only || c0 + 63 <= warp_at ? slope2 : c0 >= warp_at + 31 ? -slope2 : 0.f;
+          slope = left_only || c0 + 63 <= warp_at ? slope2 : c0 >= warp_end ? -slope2 : 0.f;
           if (slope == 0.f) {
             const float by = -__fdividef(slope2, pp.f.scale1), d0 = (float)(c0 - (row + off));
 #pragma unroll
@@ -685,7 +689,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       fence_after();
       if (pp.splits > 1) {                         // (one tile per CTA)
-        const long long part = (((long long)t.b * p.hq + t.h) * pp.tiles_x + t.m0 / C::BM) * pp.splits + t.split;
+        const long long part = (((long long)t.b * pp.heads + t.h) * pp.tiles_x + t.m0 / C::BM) * pp.splits + t.split;
         float4* o = reinterpret_cast<float4*>(pp.part_o + part * (C::BM * D)) + set * (D / 8) * C::BM + quad * 32 + lane;
 #pragma unroll 1
         for (int c = 0; c < D / 2; c += 32) {
@@ -714,8 +718,8 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(out + at + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = v[i];      // (64-byte swizzle)
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0 && t.m0 + quad * 32 < p.Sq) {
-          tma_store_4d(map, smem_u32(out) + at, col, t.h, t.m0 + quad * 32, t.b);
+        if (lane == 0 && (t.m0 + quad * 32) >> shift < p.Sq) {
+          tma_store_4d(map, smem_u32(out) + at, col, t.h << shift, (t.m0 + quad * 32) >> shift, t.b);
           bulk_commit();
         }
       };
@@ -742,7 +746,7 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           leave(&to_lo, hi, set * (D / 2) + c, C::OUT_BYTES - 2048);
         }
       }
-      if (GRAD && set == 0 && row < p.Sq) p.lse[((long long)t.b * p.hq + t.h) * p.Sq + row] = l_i != 0.f ? m_s * (MADE || LINEAR ? LN2 : p.scale) + logf(l_i) : -INFINITY;
+      if (GRAD && set == 0 && row < p.Sq) p.lse[((long long)t.b * p.hq + head) * p.Sq + row] = l_i != 0.f ? m_s * (MADE || LINEAR ? LN2 : p.scale) + logf(l_i) : -INFINITY;
       if (cta < 0) break;
       t = next;
       sees = next_sees;
@@ -769,8 +773,9 @@ __global__ void ma_join_kernel(const __grid_constant__ FwdParams pp) {
   const int c = threadIdx.x % TPR, rows = blockDim.x / TPR;
   const long long total = (long long)p.B * p.hq * p.Sq;
   for (long long at = (long long)blockIdx.x * rows + threadIdx.x / TPR; at < total; at += (long long)gridDim.x * rows) {
-    const int i = (int)(at % p.Sq), h = (int)(at / p.Sq % p.hq), b = (int)(at / p.Sq / p.hq), r = i & 127;
-    const long long part = (((long long)b * p.hq + h) * pp.tiles_x + i / 128) * pp.splits;
+    const int i = (int)(at % p.Sq), h = (int)(at / p.Sq % p.hq), b = (int)(at / p.Sq / p.hq);
+    const int row = (i << pp.shift) + (h & ((1 << pp.shift) - 1)), r = row & 127;
+    const long long part = (((long long)b * pp.heads + (h >> pp.shift)) * pp.tiles_x + row / 128) * pp.splits;
     const float* s = pp.part_s + part * 384 + r;
     float m = -INFINITY;
     for (int k = 0; k < pp.splits; k++) m = max2(m, s[k * 384]);
@@ -808,8 +813,16 @@ __global__ void ma_join_kernel(const __grid_constant__ FwdParams pp) {
 // CTAs of a tile: one where there is a tile for each SM, else as many as find room (two per SM), with four key blocks or more each.  Whole / split, us, causal: 8192 queries and keys, 1 head,
 // d 64 97 / 45; 2 heads, d 128, cap 121 / 74; 4 x 4096 of 4 heads, d 128, cap 68 / 46; 2048, 4 heads, d 64 27 / 22; one query, 32 / 8 heads, d 128, 8192 keys 118 / 37, 4 x 32768 keys
 // 557 / 296; left whole 1024, 8 heads, d 128 19.7 / 20.4 and 2 x 1024, 8 heads, d 64 19.5 / 19.2.  (Where the mask comes from the device the length of the walks is not known here: that of all keys is taken.)
+// Rows of a query under a window, as a power of two: the heads of its group, where there are few queries.
+int shift_of(const MaParams& p) {
+  const int rep = p.hq / p.hkv;
+  int shift = 0;
+  while ((1 << shift) < rep) shift++;
+  return p.window && p.Sq < 128 && shift <= 5 && (1 << shift) == rep ? shift : 0;
+}
+int tiles_of(const MaParams& p) { return (int)((((long long)p.Sq << shift_of(p)) + 127) / 128); }      // of the heads of a group, or of one
 int splits_of(const MaParams& p, int sms) {
-  const long long tiles = (long long)((p.Sq + 127) / 128) * p.hq * p.B;
+  const long long tiles = (long long)tiles_of(p) * (p.hq >> shift_of(p)) * p.B;
   const int all = (p.Sk + 127) / 128, rows = p.Sq < 128 ? p.Sq : 128;
   // (under a window: of the keys near to a tile's rows, and the sinks)
   const long long near = p.window ? ((p.causal ? 1LL : 2LL) * p.window + rows + 126) / 128 + (p.sinks + 127) / 128 : all;
@@ -818,14 +831,12 @@ int splits_of(const MaParams& p, int sms) {
   const long long room = 2LL * sms / tiles;
   return (int)(room < blocks / 4 ? room : blocks / 4);
 }
-long long part_floats(int B, int Sq, int hq, int d, int splits) {
-  return splits > 1 ? (long long)((Sq + 127) / 128) * hq * B * splits * 128 : 0;
-}
+long long part_floats(const MaParams& p, int splits) { return splits > 1 ? (long long)tiles_of(p) * (p.hq >> shift_of(p)) * p.B * splits * 128 : 0; }
 
 // Bytes of the parts' workspace: 0 where tiles are not split.
 long long fwd_ws_bytes(const MaParams& p) {
   const int splits = splits_of(p, lb_num_sms());
-  return part_floats(p.B, p.Sq, p.hq, p.d, splits) * ((p.d <= 64 ? 64 : 128) + 3) * (long long)sizeof(float);
+  return part_floats(p, splits) * ((p.d <= 64 ? 64 : 128) + 3) * (long long)sizeof(float);
 }
 
 template <int D, int CAP, bool BIAS, bool GRAD, bool WINDOW>
@@ -862,28 +873,31 @@ int launch_fwd(const MaParams& a, void* ws, long long ws_bytes, cudaStream_t s) 
   CUtensorMap maps[5];      // q, k, v, o, o_lo
   int rc;
   const uint64_t B = a.B, Sq = a.Sq, Sk = a.Sk, hq = a.hq, hkv = a.hkv, d = a.d;
-  if ((rc = make_map_bf16_4d(maps, a.q, d, hq, Sq, B, a.qs.h, a.qs.s, a.qs.b, 128))) return rc;
+  FwdParams p;
+  p.shift = WINDOW ? shift_of(a) : 0;
+  p.heads = a.hq >> p.shift;
+  const uint32_t rows = 1u << p.shift;      // of a query
+  if ((rc = make_map_bf16_4d(maps, a.q, d, hq, Sq, B, a.qs.h, a.qs.s, a.qs.b, 128 / rows, 64, rows))) return rc;
   if ((rc = make_map_bf16_4d(maps + 1, a.k, d, hkv, Sk, B, a.ks.h, a.ks.s, a.ks.b, 128))) return rc;
   if ((rc = make_map_bf16_4d(maps + 2, a.v, d, hkv, Sk, B, a.vs.h, a.vs.s, a.vs.b, 64))) return rc;
-  if ((rc = make_map_bf16_4d(maps + 3, a.o, d, hq, Sq, B, d, hq * d, Sq * hq * d, 32, 32))) return rc;
-  if ((rc = make_map_bf16_4d(maps + 4, a.o_lo ? a.o_lo : a.o, d, hq, Sq, B, d, hq * d, Sq * hq * d, 32, 32))) return rc;
-  FwdParams p;
+  if ((rc = make_map_bf16_4d(maps + 3, a.o, d, hq, Sq, B, d, hq * d, Sq * hq * d, 32 / rows, 32, rows))) return rc;
+  if ((rc = make_map_bf16_4d(maps + 4, a.o_lo ? a.o_lo : a.o, d, hq, Sq, B, d, hq * d, Sq * hq * d, 32 / rows, 32, rows))) return rc;
   p.a = a;
-  p.tiles_x = (a.Sq + 127) / 128;
+  p.tiles_x = tiles_of(a);
   // heads ordered together: as many as have their K / V in 48 MB (of 126 MB of L2), whole GQA groups
-  const long long kv_bytes = 4LL * D * a.Sk, pairs = (long long)a.hq * a.B;
+  const long long kv_bytes = 4LL * D * a.Sk, pairs = (long long)p.heads * a.B;
   const long long kv_heads = kv_bytes >= (48LL << 20) ? 1 : (48LL << 20) / kv_bytes;
-  p.group = (int)(kv_heads * (a.hq / a.hkv) < pairs ? kv_heads * (a.hq / a.hkv) : pairs);
+  p.group = (int)(kv_heads * (p.heads / a.hkv) < pairs ? kv_heads * (p.heads / a.hkv) : pairs);
   p.splits = ws_bytes > 0 && ws_bytes >= fwd_ws_bytes(a) ? splits_of(a, lb_num_sms()) : 1;
   p.part_o = (float*)ws;
-  p.part_s = p.part_o + part_floats(a.B, a.Sq, a.hq, a.d, p.splits) * D;
+  p.part_s = p.part_o + part_floats(a, p.splits) * D;
   const long long grid = p.tiles_x * pairs * p.splits;
   if (grid > 2147483647LL) return LB_ERR_SHAPE;
   p.by_grp.set((unsigned)(p.tiles_x * p.group));
   p.by_group.set((unsigned)p.group);
   p.by_last.set((unsigned)(pairs % p.group ? pairs % p.group : p.group));
-  p.by_hq.set((unsigned)a.hq);
-  p.by_rep.set((unsigned)(a.hq / a.hkv));
+  p.by_hq.set((unsigned)p.heads);
+  p.by_rep.set((unsigned)(p.heads / a.hkv));
   p.steal = p.splits == 1 && grid > 2 * lb_num_sms();      // (with all tiles resident at once there is none to take)
   p.f.set(a, true, twice);
   const bool bias = a.slopes != nullptr;

@@ -501,9 +501,9 @@ inline int make_map_bf16_3d(CUtensorMap* m, const void* base, uint64_t inner, ui
 // [batches, rows, heads, d] with strides of sb, ss and sh elements (multiples of 8); box = box_rows rows of 64 columns of one head, or of 32 (64-byte swizzle).  What lies outside of d or of
 // the rows is loaded as zeros and not stored.
 inline int make_map_bf16_4d(CUtensorMap* m, const void* base, uint64_t d, uint64_t heads, uint64_t rows, uint64_t batches, uint64_t sh, uint64_t ss, uint64_t sb,
-                            uint32_t box_rows, uint32_t box_cols = 64) {
+                            uint32_t box_rows, uint32_t box_cols = 64, uint32_t box_heads = 1) {
   const cuuint64_t dims[4] = {d, heads, rows, batches}, strides[3] = {sh * 2, ss * 2, sb * 2};
-  const cuuint32_t box[4] = {box_cols, 1, box_rows, 1};
+  const cuuint32_t box[4] = {box_cols, box_heads, box_rows, 1};
   return make_map_bf16_nd(m, base, 4, dims, strides, box, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
