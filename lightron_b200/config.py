@@ -46,6 +46,11 @@ class ModelArgs:
     attn_softcap: float = 0.0                 # scores are capped at softcap * tanh(score / softcap); 0: not
     attn_alibi: bool = False                  # scores fall with distance, head h by 2^(-8 (h + 1) / n_heads) a token
     rope_sections: Optional[tuple] = None     # pairs of a head that turn by each axis of positions [axes, B, S]
+    attn_window: Optional[int] = None         # a position sees the keys less than so many positions before it
+    attn_sinks: int = 0                       # and the first so many of its document
+    attn_global_freq: int = 0                 # every so many-th layer sees all keys in spite of the window; 0: none
+    qk_norm: bool = False                     # heads of queries and keys are normed ahead of the rotation
+    embed_scale: Optional[float] = None       # embeddings are multiplied by it, and their gradients summed in 32 bits
 
     def __post_init__(self):
         if self.rope_sections is not None:
@@ -54,8 +59,16 @@ class ModelArgs:
                 raise ValueError(f"rope_sections {self.rope_sections} do not add up to the {self.head_dim // 2} pairs of a head")
         if not 0.0 <= self.attn_softcap < float("inf"):
             raise ValueError(f"attn_softcap must be zero (none) or positive and finite, got {self.attn_softcap}")
+        if self.attn_window is not None and (type(self.attn_window) is not int or self.attn_window < 1):
+            raise ValueError(f"attn_window must be at least 1, or null, got {self.attn_window!r}")
+        if type(self.attn_sinks) is not int or self.attn_sinks < 0 or (self.attn_sinks and self.attn_window is None):
+            raise ValueError(f"attn_sinks must be at least 0, and have a meaning with attn_window only, got {self.attn_sinks!r}")
+        if type(self.attn_global_freq) is not int or self.attn_global_freq < 0 or (self.attn_global_freq and self.attn_window is None):
+            raise ValueError(f"attn_global_freq must be at least 0, and has a meaning with attn_window only, got {self.attn_global_freq!r}")
+        if self.embed_scale is not None and not abs(self.embed_scale) < float("inf"):
+            raise ValueError(f"embed_scale must be finite, got {self.embed_scale}")
         if self.cp_size > 1 and self.packed_attention:
-            raise ValueError("attn_softcap, attn_alibi and rope_sections are not built for context parallelism")
+            raise ValueError("attn_softcap, attn_alibi, rope_sections, attn_window and qk_norm are not built for context parallelism")
         if self.n_kv_heads is None:
             self.n_kv_heads = self.n_heads
         if self.dim % self.n_heads:
@@ -68,7 +81,11 @@ class ModelArgs:
     @property
     def packed_attention(self) -> bool:
         """Whether the attention differs from plain causal attention with rotary positions on one axis."""
-        return bool(self.attn_softcap or self.attn_alibi or self.rope_sections)
+        return bool(self.attn_softcap or self.attn_alibi or self.rope_sections or self.attn_window or self.qk_norm)
+
+    def window_of(self, layer_id: int) -> Optional[int]:
+        """Window of a layer's attention, or None: it sees all keys."""
+        return None if self.attn_global_freq and (layer_id + 1) % self.attn_global_freq == 0 else self.attn_window
 
     @property
     def head_dim(self) -> int:
@@ -100,7 +117,7 @@ class ModelArgs:
 
     def num_params(self) -> int:
         d, kv = self.dim, self.n_kv_heads * self.head_dim
-        attn = 2 * d * d + 2 * d * kv
+        attn = 2 * d * d + 2 * d * kv + (2 * self.head_dim if self.qk_norm else 0)
         mlp = 3 * d * self.ffn_hidden
         total = 2 * self.vocab_size * d + d
         for i in range(self.n_layers):

@@ -50,12 +50,13 @@ class RMSNorm(nn.Module):
 
 
 class Embedding(nn.Module):
-    def __init__(self, num_embeddings: int, dim: int, dtype=None, device=None):
+    def __init__(self, num_embeddings: int, dim: int, dtype=None, device=None, scale: Optional[float] = None):
         super().__init__()
+        self.scale = scale
         self.weight = nn.Parameter(torch.empty(num_embeddings, dim, dtype=dtype, device=device))
 
     def forward(self, tokens):
-        return OF.embedding(tokens, self.weight, 0)
+        return OF.embedding(tokens, self.weight, 0) if self.scale is None else OF.scaled_embedding(tokens, self.weight, self.scale)
 
 
 def _col(args: ModelArgs, i, o, ctx, **kw):
@@ -95,7 +96,7 @@ class MLP(nn.Module):
 
 
 class Attention(nn.Module):
-    def __init__(self, args: ModelArgs, ctx, **kw):
+    def __init__(self, args: ModelArgs, ctx, layer_id: int = 0, **kw):
         super().__init__()
         tp = args.tp_size
         assert args.n_heads % tp == 0, f"n_heads ({args.n_heads}) must be divisible by tp_size ({tp})"
@@ -116,6 +117,11 @@ class Attention(nn.Module):
         self.packed = args.packed_attention
         self.softcap = args.attn_softcap
         self.axes = None if args.rope_sections is None else tuple(a for a, n in enumerate(args.rope_sections) for _ in range(n))
+        self.window = args.window_of(layer_id)
+        self.sinks = args.attn_sinks if self.window is not None else 0
+        self.qk_norm = args.qk_norm
+        if args.qk_norm:              # of all heads, on every rank of the TP group
+            self.q_norm, self.k_norm = RMSNorm(d, eps=args.norm_eps, **kw), RMSNorm(d, eps=args.norm_eps, **kw)
         self._slopes = None
         if args.attn_alibi:           # of this rank's heads
             first = ctx.tp_rank * self.n_heads if tp > 1 else 0
@@ -134,7 +140,14 @@ class Attention(nn.Module):
             qkv = OF.linear(comm.copy_to_group(x, self.tp_group), self.wq.weight, self.wk.weight, self.wv.weight)
         hq, hkv, d = self.n_heads, self.n_kv_heads, self.head_dim
         if self.cp_group is None and (self.packed or mask is not None or (positions is not None and positions.dim() > 1)):
-            o = OF.packed_attention_qkv(qkv, cos, sin, positions, B, S, hq, hkv, d, axes=self.axes, mask=mask, softcap=self.softcap, slopes=self.slopes(qkv.device))
+            norms = {}
+            if self.qk_norm:
+                wq, wk = self.q_norm.weight, self.k_norm.weight
+                if not self.sp:       # each rank's heads give a part of the weights' gradients (under sequence parallelism the optimizer adds those of all norms up)
+                    wq, wk = comm.copy_to_group(wq, self.tp_group), comm.copy_to_group(wk, self.tp_group)
+                norms = dict(q_norm=wq, k_norm=wk, norm_eps=self.q_norm.eps)
+            o = OF.packed_attention_qkv(qkv, cos, sin, positions, B, S, hq, hkv, d, axes=self.axes, mask=mask, softcap=self.softcap, slopes=self.slopes(qkv.device), window=self.window,
+                                        sinks=self.sinks, **norms)
         elif mask is not None:
             raise ValueError("packed batches are not built for context parallelism")
         elif self.cp_group is None:
@@ -151,7 +164,7 @@ class TransformerBlock(nn.Module):
     def __init__(self, args: ModelArgs, layer_id: int, ctx, **kw):
         super().__init__()
         self.layer_id = layer_id
-        self.attention = Attention(args, ctx, **kw)
+        self.attention = Attention(args, ctx, layer_id=layer_id, **kw)
         if args.is_moe_layer(layer_id):
             from .moe import MoEFeedForward
             self.feed_forward = MoEFeedForward(args, ctx, **kw)
@@ -224,7 +237,7 @@ class LightronTransformer(nn.Module):
                 self.tok_embeddings = VocabParallelEmbedding(args.vocab_size, args.dim, group=ctx.tp_group,
                                                              sequence_parallel=False, **kw)
             else:
-                self.tok_embeddings = Embedding(args.vocab_size, args.dim, **kw)
+                self.tok_embeddings = Embedding(args.vocab_size, args.dim, scale=args.embed_scale, **kw)
         self.layers = nn.ModuleDict({str(i): TransformerBlock(args, i, ctx, **kw) for i in range(lo, hi)})
         if last_stage:
             self.norm = RMSNorm(args.dim, eps=args.norm_eps, **kw)
@@ -247,17 +260,19 @@ class LightronTransformer(nn.Module):
     def embed(self, tokens: torch.Tensor) -> torch.Tensor:
         """tokens [B, S] -> [T, H] (rows sharded over TP under sequence parallelism)."""
         flat = tokens.reshape(-1)
+        scale = self.args.embed_scale
         if self.args.tp_size > 1:
             from ..parallel import embed_fused
-            if embed_fused.fused_ok(self.tok_embeddings.weight, self.tp_group, flat.numel(), self.sp):
+            if scale is None and embed_fused.fused_ok(self.tok_embeddings.weight, self.tp_group, flat.numel(), self.sp):
                 # the owner of a token's id stores its row straight into the rank that needs it
                 return embed_fused.vocab_parallel_embedding(flat, self.tok_embeddings.weight, self.tp_group,
                                                             self.tok_embeddings.vocab_start, self.sp)
-            part = OF.embedding(flat, self.tok_embeddings.weight, self.tok_embeddings.vocab_start)
+            w, start = self.tok_embeddings.weight, self.tok_embeddings.vocab_start
+            part = OF.embedding(flat, w, start) if scale is None else OF.scaled_embedding(flat, w, scale, start)
             if self.sp:
                 return comm.scatter_rows(part, self.tp_group)
             return comm.reduce_from_group(part, self.tp_group)
-        return OF.embedding(flat, self.tok_embeddings.weight, 0)
+        return OF.embedding(flat, self.tok_embeddings.weight, 0) if scale is None else OF.scaled_embedding(flat, self.tok_embeddings.weight, scale)
 
     def run_layers(self, h, delta, B, S, positions, mask=None):
         cos, sin = self.rope_tables(h.device)

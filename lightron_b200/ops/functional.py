@@ -1143,61 +1143,104 @@ class _PackedAttnQKV(torch.autograd.Function):
         return heads[:, :, :hq + hkv], heads[:, :, :hq], heads[:, :, hq:hq + hkv], heads[:, :, hq + hkv:]
 
     @staticmethod
-    def forward(ctx, qkv, cos, sin, positions, slopes, qb, kb, axes, dims, causal, scale, softcap):
+    def forward(ctx, qkv, cos, sin, positions, slopes, qb, kb, axes, dims, causal, scale, softcap, window, sinks):
         qk, q, k, v = _PackedAttnQKV._views(qkv, *dims)
         with native.on_device(qkv):
             _rope_axes_native(qk, qk, cos, sin, positions, axes, False)
             torch.autograd.graph.increment_version(qkv)
-            o, o_lo, lse = masked_fwd_native(q, k, v, causal, scale, softcap, slopes, qb, kb, not isinstance(ctx, _NoGradCtx) and ctx.needs_input_grad[0])
+            o, o_lo, lse = masked_fwd_native(q, k, v, causal, scale, softcap, slopes, qb, kb, not isinstance(ctx, _NoGradCtx) and ctx.needs_input_grad[0], window, sinks)
         # (detached: the version still counts, but nobody asks how a view that was written to was made)
         ctx.save_for_backward(qkv.detach(), o, o_lo, lse, cos, sin, positions, slopes, qb, kb)
-        ctx.args = (axes, dims, causal, scale, softcap)
+        ctx.args = (axes, dims, causal, scale, softcap, window, sinks)
         return o.view(qkv.shape[0], -1)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
         qkv, o, o_lo, lse, cos, sin, positions, slopes, qb, kb = ctx.saved_tensors
-        axes, dims, causal, scale, softcap = ctx.args
+        axes, dims, causal, scale, softcap, window, sinks = ctx.args
         dqkv = torch.empty_like(qkv)
         _, q, k, v = _PackedAttnQKV._views(qkv, *dims)
         dqk, dq, dk, dv = _PackedAttnQKV._views(dqkv, *dims)
         with native.on_device(qkv):
-            masked_bwd_native(q, k, v, o, o_lo, lse, do.reshape(o.shape), causal, scale, softcap, slopes, qb, kb, dq, dk, dv)
+            masked_bwd_native(q, k, v, o, o_lo, lse, do.reshape(o.shape), causal, scale, softcap, slopes, qb, kb, dq, dk, dv, window, sinks)
             _rope_axes_native(dqk, dqk, cos, sin, positions, axes, True)
-        return (dqkv,) + (None,) * 11
+        return (dqkv,) + (None,) * 13
+
+
+class _NormAttnQKV(torch.autograd.Function):
+    """:func:`qk_norm_rope` + masked attention on the fused projection output, which stays as it is; backward writes one dqkv tensor."""
+
+    @staticmethod
+    def forward(ctx, qkv, wq, wk, cos, sin, positions, slopes, qb, kb, axes, dims, eps, causal, scale, softcap, window, sinks):
+        B, S, hq, hkv, d = dims
+        _, q, k, v = _PackedAttnQKV._views(qkv, *dims)
+        turned = torch.empty(B, S, hq + hkv, d, dtype=qkv.dtype, device=qkv.device)
+        with native.on_device(qkv):
+            _norm_rope_native(q, k, turned[:, :, :hq], turned[:, :, hq:], _row(wq), _row(wk), cos, sin, positions, axes, eps)
+            o, o_lo, lse = masked_fwd_native(turned[:, :, :hq], turned[:, :, hq:], v, causal, scale, softcap, slopes, qb, kb,
+                                             not isinstance(ctx, _NoGradCtx) and any(ctx.needs_input_grad[:3]), window, sinks)
+        ctx.save_for_backward(qkv, wq, wk, turned, o, o_lo, lse, cos, sin, positions, slopes, qb, kb)
+        ctx.args = (axes, dims, eps, causal, scale, softcap, window, sinks)
+        return o.view(B * S, hq * d)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        qkv, wq, wk, turned, o, o_lo, lse, cos, sin, positions, slopes, qb, kb = ctx.saved_tensors
+        axes, dims, eps, causal, scale, softcap, window, sinks = ctx.args
+        hq = dims[2]
+        _, q, k, v = _PackedAttnQKV._views(qkv, *dims)
+        dqkv, dturned = torch.empty_like(qkv), torch.empty_like(turned)
+        _, dq, dk, dv = _PackedAttnQKV._views(dqkv, *dims)
+        with native.on_device(qkv):
+            masked_bwd_native(turned[:, :, :hq], turned[:, :, hq:], v, o, o_lo, lse, do.reshape(o.shape), causal, scale, softcap, slopes, qb, kb, dturned[:, :, :hq], dturned[:, :, hq:], dv,
+                              window, sinks)
+            dwq, dwk = _norm_rope_bwd_native(q, k, dturned[:, :, :hq], dturned[:, :, hq:], dq, dk, _row(wq), _row(wk), cos, sin, positions, axes, eps, any(ctx.needs_input_grad[1:3]))
+        return (dqkv, dwq, dwk) + (None,) * 14
 
 
 def packed_attention_qkv(qkv: torch.Tensor, cos, sin, positions, B: int, S: int, hq: int, hkv: int, d: int, axes: Optional[Sequence[int]] = None,
-                         mask: Optional[AttentionMask] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """:func:`rope_attention_qkv` for packed batches: qkv [B*S, (hq+2hkv)*d] -> [B*S, hq*d] by :func:`rope_axes` on q and k and :func:`masked_attention`.
+                         mask: Optional[AttentionMask] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None, window: Optional[int] = None, sinks: int = 0,
+                         q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, norm_eps: float = 1e-6) -> torch.Tensor:
+    """:func:`rope_attention_qkv` for packed batches and local attention: qkv [B*S, (hq+2hkv)*d] -> [B*S, hq*d] by :func:`rope_axes` on q and k, or with ``q_norm`` and ``k_norm`` [d] by
+    :func:`qk_norm_rope`, and :func:`masked_attention`.
     ``positions``: None (each token's place), [S], [B, S] (as of documents that count from zero).  With ``axes``: None or [S], which count on all axes together as text
-    does, [A, B, S] or [A, S] (two dimensions are axes and tokens then, never sequences and tokens).  On the GPU the caller hands ``qkv`` over: q and k are rotated where
+    does, [A, B, S] or [A, S] (two dimensions are axes and tokens then, never sequences and tokens).  On the GPU the caller hands ``qkv`` over: without norms q and k are rotated where
     they lie (its version counts up); only a leaf that requires a gradient, or one whose memory does not suit the kernels, is copied first and stays as it was."""
-    if positions is None:
+    if (q_norm is None) != (k_norm is None):
+        raise ValueError("q_norm and k_norm come together")
+    if positions is None and q_norm is None:
         positions = torch.arange(S, device=qkv.device, dtype=torch.int32)
-    if axes is None:
-        positions, axes = positions[None], (0,) * (d // 2)
-    elif positions.dim() == 1:
-        axes = tuple(axes)
-        positions = positions.expand(max(axes, default=0) + 1, -1)
     if qkv.dim() != 2 or qkv.shape != (B * S, (hq + 2 * hkv) * d):
         raise ValueError(f"qkv {tuple(qkv.shape)} is not [{B} * {S}, ({hq} + 2 * {hkv}) * {d}]")
     if cos.device != qkv.device:
         raise ValueError(f"tables on {cos.device} for qkv on {qkv.device}")
-    positions, axes = _check_axes(B, S, d, cos, sin, positions, axes)
+    positions, axes = _positions_of(positions, axes, B, S, d, cos, sin)
     heads = qkv.view(B, S, hq + 2 * hkv, d)
     q, k, v = heads[:, :, :hq], heads[:, :, hq:hq + hkv], heads[:, :, hq + hkv:]
     causal = _check_masked(q, k, v, mask, None, None, softcap, slopes)
-    if native.use_native(qkv) and qkv.numel() and positions.shape[0] <= 8:
+    local, first = _check_window(window, sinks, S)
+    if q_norm is not None:
+        _check_norm_rope(q, k, q_norm, k_norm, cos, sin, norm_eps)
+    if native.use_native(qkv) and qkv.numel() and max(axes, default=0) < 8 and (positions is None or positions.shape[0] <= 8):
         _check_masked_native(d)
-        if not qkv.is_contiguous() or qkv.data_ptr() % 16 or (qkv.requires_grad and qkv.is_leaf):
+        if local and S > MAX_WINDOW_LENGTH:
+            raise ValueError(f"a window on the GPU takes up to {MAX_WINDOW_LENGTH} keys, got {S}")
+        suits = qkv.is_contiguous() and qkv.data_ptr() % 16 == 0
+        if not suits or (q_norm is None and qkv.requires_grad and qkv.is_leaf):
             qkv = qkv.clone(memory_format=torch.contiguous_format)
         qb, kb = (mask.q_bounds, mask.k_bounds) if mask is not None else (None, None)
-        return _apply(_PackedAttnQKV, qkv, cos.contiguous(), sin.contiguous(), positions, None if slopes is None else slopes.contiguous(), qb, kb, axes, (B, S, hq, hkv, d), causal,
-                      1.0 / math.sqrt(d), float(softcap))
-    q, k = rope_axes(q, cos, sin, positions, axes), rope_axes(k, cos, sin, positions, axes)
-    return masked_attention(q, k, v, mask=mask, softcap=softcap, slopes=slopes).reshape(B * S, hq * d)
+        cos, sin, slopes = cos.contiguous(), sin.contiguous(), None if slopes is None else slopes.contiguous()
+        rest = (causal, 1.0 / math.sqrt(d), float(softcap), local, first)
+        if q_norm is not None:
+            return _apply(_NormAttnQKV, qkv, q_norm, k_norm, cos, sin, positions, slopes, qb, kb, axes, (B, S, hq, hkv, d), float(norm_eps), *rest)
+        return _apply(_PackedAttnQKV, qkv, cos, sin, positions, slopes, qb, kb, axes, (B, S, hq, hkv, d), *rest)
+    if q_norm is not None:
+        q, k = qk_norm_rope(q, k, q_norm, k_norm, cos, sin, positions=positions, axes=axes, eps=norm_eps)
+    else:
+        q, k = rope_axes(q, cos, sin, positions, axes), rope_axes(k, cos, sin, positions, axes)
+    return masked_attention(q, k, v, mask=mask, softcap=softcap, slopes=slopes, window=window, sinks=sinks).reshape(B * S, hq * d)
 
 
 # --------------------------------------------------------------------------------------

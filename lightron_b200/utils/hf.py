@@ -21,6 +21,7 @@ _LAYER_MAP = {
     "mlp.gate_proj.weight": "feed_forward.w1.weight", "mlp.up_proj.weight": "feed_forward.w3.weight",
     "mlp.down_proj.weight": "feed_forward.w2.weight", "input_layernorm.weight": "attention_norm.weight",
     "post_attention_layernorm.weight": "ffn_norm.weight",
+    "self_attn.q_norm.weight": "attention.q_norm.weight", "self_attn.k_norm.weight": "attention.k_norm.weight",      # of a head, with ``model.qk_norm``
 }
 _TOP_MAP = {"model.embed_tokens.weight": "tok_embeddings.weight", "model.norm.weight": "norm.weight",
             "lm_head.weight": "output.weight"}
@@ -51,6 +52,8 @@ def convert_hf_llama_state_dict(hf_sd: Dict[str, torch.Tensor], n_heads: int, n_
                     t = _to_interleaved(v, n_heads)
                 elif permute_rope and rest == "self_attn.k_proj.weight":
                     t = _to_interleaved(v, n_kv_heads)
+                elif permute_rope and rest in ("self_attn.q_norm.weight", "self_attn.k_norm.weight"):
+                    t = _to_interleaved(v, 1)
                 out[f"layers.{idx}.{_LAYER_MAP[rest]}"] = t
     if "output.weight" not in out and "tok_embeddings.weight" in out:       # tied embeddings
         out["output.weight"] = out["tok_embeddings.weight"]
@@ -73,6 +76,8 @@ def export_hf_llama_state_dict(sd: Dict[str, torch.Tensor], n_heads: int, n_kv_h
                     t = _from_interleaved(v, n_heads)
                 elif permute_rope and rest == "attention.wk.weight":
                     t = _from_interleaved(v, n_kv_heads)
+                elif permute_rope and rest in ("attention.q_norm.weight", "attention.k_norm.weight"):
+                    t = _from_interleaved(v, 1)
                 out[f"model.layers.{idx}.{inv_layer[rest]}"] = t
     return out
 
