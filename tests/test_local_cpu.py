@@ -113,3 +113,137 @@ def _embed(**kw):
 def test_refusals(call):
     with pytest.raises(ValueError):
         call()
+
+
+# ---- in the model -----------------------------------------------------------------------------------
+
+LOCAL = dict(attn_window=4, attn_sinks=2, qk_norm=True, embed_scale=3.0)
+
+
+def _model(ctx=None, **kw):
+    from lightron_b200 import mesh
+    from lightron_b200.config import ModelArgs
+    from lightron_b200.models import LightronTransformer, init_weights
+    if ctx is None:
+        mesh.set_context(None)
+    args = ModelArgs(**{**dict(dim=32, n_layers=3, n_heads=4, n_kv_heads=2, vocab_size=64, intermediate_size=48, max_seq_len=64), **kw})
+    model = LightronTransformer(args, ctx=ctx, dtype=torch.float32, device="cpu")
+    init_weights(model, 0, std=0.2)
+    with torch.no_grad():
+        for n, p in model.named_parameters():
+            if p.dim() == 1:                                       # the same on every rank
+                p.add_(0.3 * torch.randn(p.shape, generator=torch.Generator().manual_seed(len(n))))
+    return model
+
+
+@pytest.mark.parametrize("kw", [dict(attn_window=4), LOCAL, dict(LOCAL, attn_global_freq=2, attn_softcap=5.0), dict(qk_norm=True, rope_sections=(2, 1, 1)), dict(embed_scale=0.5)])
+def test_model_of_documents_is_each_alone(kw):
+    model = _model(**kw)
+    lens = [5, 14, 9]
+    tokens = torch.randint(0, 64, (1, sum(lens)), generator=torch.Generator().manual_seed(0))
+    ids = torch.cat([torch.full((n,), i) for i, n in enumerate(lens)])[None]
+    pos = torch.cat([torch.arange(n) for n in lens])[None]
+    packed = model(tokens, positions=pos, mask=OF.attention_mask(documents=ids))
+    at = 0
+    for n in lens:
+        assert torch.allclose(packed[:, at:at + n], model(tokens[:, at:at + n]), atol=1e-5)
+        at += n
+    model.loss(tokens, tokens, positions=pos, mask=OF.attention_mask(documents=ids)).backward()
+    assert all(torch.isfinite(p.grad).all() and p.grad.abs().sum() > 0 for p in model.parameters())
+
+
+def test_model_layers_see_their_windows():
+    """A change of one token reaches as far as the windows of the layers and the layers without one let it."""
+    tokens = torch.randint(0, 64, (1, 40), generator=torch.Generator().manual_seed(1))
+    other = tokens.clone()
+    other[0, 10] = (other[0, 10] + 1) % 64
+    for kw, last in ((dict(attn_window=4), 10 + 3 * 3), (dict(attn_window=4, attn_global_freq=3), 39), (dict(attn_window=64), 39), (dict(attn_window=1), 10)):
+        model = _model(**kw)
+        changed = (model(tokens) - model(other)).abs().amax(-1)[0] > 1e-6
+        assert changed.nonzero().max() == last and not changed[:10].any()
+    sinks = _model(attn_window=2, attn_sinks=11)                   # position 10 is a sink
+    assert ((sinks(tokens) - sinks(other)).abs().amax(-1)[0, 10:] > 1e-7).all()
+
+
+def test_scaled_embedding_in_the_model():
+    """Embeddings that are multiplied by c are those of weights c times as large."""
+    tokens = torch.randint(0, 64, (2, 9), generator=torch.Generator().manual_seed(1))
+    a, b = _model(embed_scale=3.0), _model()
+    with torch.no_grad():
+        b.tok_embeddings.weight.mul_(3.0)
+    assert torch.allclose(a(tokens), b(tokens), atol=1e-5)
+    assert torch.allclose(a.tok_embeddings(tokens), b.tok_embeddings(tokens), atol=1e-6)
+
+
+def test_model_arguments_are_checked():
+    from lightron_b200.config import ModelArgs
+    for bad in (dict(attn_window=0), dict(attn_window=1.5), dict(attn_sinks=2), dict(attn_window=4, attn_sinks=-1), dict(attn_global_freq=2), dict(attn_window=4, attn_global_freq=-1),
+                dict(embed_scale=float("inf")), dict(attn_window=4, cp_size=2), dict(qk_norm=True, cp_size=2)):
+        with pytest.raises(ValueError):
+            ModelArgs(dim=32, n_heads=4, **bad)
+    args = ModelArgs(dim=32, n_heads=4, n_layers=2, attn_window=4, attn_global_freq=2, qk_norm=True)
+    assert [args.window_of(i) for i in range(4)] == [4, None, 4, None] and args.packed_attention
+    assert args.num_params() == ModelArgs(dim=32, n_heads=4, n_layers=2).num_params() + 2 * 2 * 8
+
+
+def test_norm_weights_of_other_layouts():
+    """Weights of heads whose pairs lie half a head apart, there and back, and what they compute."""
+    from lightron_b200.utils.hf import convert_hf_llama_state_dict, export_hf_llama_state_dict
+    model = _model(qk_norm=True)
+    sd = model.state_dict()
+    out = export_hf_llama_state_dict(sd, 4, 2)
+    assert "model.layers.0.self_attn.q_norm.weight" in out
+    assert torch.equal(out["model.layers.0.self_attn.q_norm.weight"], torch.cat((sd["layers.0.attention.q_norm.weight"][0::2], sd["layers.0.attention.q_norm.weight"][1::2])))
+    back = convert_hf_llama_state_dict(out, 4, 2)
+    assert back.keys() == sd.keys() and all(torch.equal(back[k], sd[k]) for k in sd)
+
+
+def _local_worker(rank, world, sp):
+    import torch.distributed as dist
+    from lightron_b200 import mesh
+    ctx = mesh.setup_distributed(tp_size=world, backend="gloo")
+    model = _model(ctx=ctx, tp_size=world, sequence_parallel=sp, **LOCAL)
+    tokens = torch.randint(0, 64, (2, 12), generator=torch.Generator().manual_seed(1))
+    loss = model.loss(tokens, tokens.roll(-1, 1))
+    loss.backward()
+    grads = {}
+    for n, p in model.named_parameters():
+        if p.dim() == 1:
+            g = p.grad.clone()
+            if sp:                                                 # parts, which the optimizers add up
+                dist.all_reduce(g, group=ctx.tp_group)
+            grads[n] = g.numpy()
+    grads["tok_embeddings.weight"] = model.tok_embeddings.weight.grad.numpy()
+    return float(loss.detach()), grads
+
+
+@pytest.mark.parametrize("sp", [False, True])
+def test_tensor_parallel_gradients(sp):
+    """Norm weights of heads that are spread over ranks, and embeddings of parts of the vocabulary: the gradients of one process."""
+    from dist_utils import run_distributed
+    got = run_distributed(_local_worker, 2, sp)
+    model = _model(**LOCAL)
+    tokens = torch.randint(0, 64, (2, 12), generator=torch.Generator().manual_seed(1))
+    loss = model.loss(tokens, tokens.roll(-1, 1))
+    loss.backward()
+    for rank, (value, grads) in enumerate(got):
+        assert abs(value - float(loss.detach())) < 1e-5
+        for n, g in grads.items():
+            want = dict(model.named_parameters())[n].grad
+            want = want if n != "tok_embeddings.weight" else want[rank * 32:(rank + 1) * 32]
+            assert torch.allclose(torch.from_numpy(g), want, atol=1e-5, rtol=1e-4), n
+
+
+def test_trainer_takes_the_keys():
+    """The run configuration's section, with clipping and two pipeline-free steps."""
+    from lightron_b200 import mesh
+    from lightron_b200.config import parse_config
+    from lightron_b200.trainer import Trainer
+    mesh.set_context(None)
+    raw = {"distributed": {}, "model": {"name": "tiny", "attn_window": 16, "attn_sinks": 2, "attn_global_freq": 4, "qk_norm": True, "embed_scale": 16.0}, "dataset": {"name": "synthetic"},
+           "training": {"micro_batch_size": 2, "gradient_accumulation_steps": 1, "seq_length": 64, "learning_rate": 3e-4, "total_steps": 2, "seed": 0, "dtype": "fp32", "grad_clip": 1.0,
+                        "log_interval": 1000}}
+    tr = Trainer(parse_config(raw, env={}))
+    losses = [float(tr.train_step()) for _ in range(2)]
+    mesh.set_context(None)
+    assert all(0 < x < 20 for x in losses)
