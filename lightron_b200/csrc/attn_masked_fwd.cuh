@@ -778,18 +778,31 @@ __global__ void ma_join_kernel(const __grid_constant__ FwdParams pp) {
     const long long part = (((long long)b * pp.heads + (h >> pp.shift)) * pp.tiles_x + row / 128) * pp.splits;
     const float* s = pp.part_s + part * 384 + r;
     float m = -INFINITY;
+#pragma unroll 4
     for (int k = 0; k < pp.splits; k++) m = max2(m, s[k * 384]);
     float l = 0.f, lp = 0.f, f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     const float4* o = reinterpret_cast<const float4*>(pp.part_o + part * (128 * D)) + 2 * c * 128 + r;
-    for (int k = 0; k < pp.splits; k++) {
-      const float from = s[k * 384];
-      if (from == -INFINITY) continue;                       // (has seen nothing)
-      const float w = exp2f(from - m);
-      const float4 x = o[(long long)k * (32 * D)], y = o[(long long)k * (32 * D) + 128];
-      l += w * s[k * 384 + 128];
-      lp += w * s[k * 384 + 256];
-      f[0] += w * x.x; f[1] += w * x.y; f[2] += w * x.z; f[3] += w * x.w;
-      f[4] += w * y.x; f[5] += w * y.y; f[6] += w * y.z; f[7] += w * y.w;
+    for (int k0 = 0; k0 < pp.splits; k0 += 4) {
+      float4 x[4], y[4];
+      float from[4], sl[4], sp[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int k = min(k0 + u, pp.splits - 1);
+        x[u] = o[(long long)k * (32 * D)];
+        y[u] = o[(long long)k * (32 * D) + 128];
+        from[u] = s[k * 384];
+        sl[u] = s[k * 384 + 128];
+        sp[u] = s[k * 384 + 256];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        if (k0 + u >= pp.splits || from[u] == -INFINITY) continue;      // (has seen nothing)
+        const float w = exp2f(from[u] - m);
+        l += w * sl[u];
+        lp += w * sp[u];
+        f[0] += w * x[u].x; f[1] += w * x[u].y; f[2] += w * x[u].z; f[3] += w * x[u].w;
+        f[4] += w * y[u].x; f[5] += w * y[u].y; f[6] += w * y[u].z; f[7] += w * y[u].w;
+      }
     }
     const float inv = lp != 0.f ? 1.f / lp : 0.f;
     if (c * 8 < p.d) {

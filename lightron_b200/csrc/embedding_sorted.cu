@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(256) embed_scaled_kernel(const void* __restric
   grid_go();
   grid_wait();
   typedef typename Vec<VEC>::type V;
-  constexpr int U = 4;
+  constexpr int U = VEC == 8 ? 4 : 8;
   const int lane = threadIdx.x & 31, nvec = H / VEC;
   for (long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); t < T; t += (long long)gridDim.x * 8) {
     const long long id = id_at(tok, wide, t);
@@ -314,7 +314,8 @@ __device__ __forceinline__ void clear_rows(const SumParams& p, int cta) {
   }
 }
 
-// A thread has K vectors of a row, a CTA's width apart; U places on their way.
+// A thread has K vectors of a row, a CTA's width apart; U places on their way.  (Rows of odd length are taken by single columns, 34 instructions each: 15001 x 1021 36 us.  By pairs from
+// two words each, every second row being askew, loads no longer go out together: 46.)
 template <int VEC, int K, int U>
 __global__ void __launch_bounds__(SUM_THREADS, 3) embed_sum_kernel(const __grid_constant__ SumParams p) {
   grid_go();
@@ -392,7 +393,8 @@ __global__ void __launch_bounds__(SUM_THREADS, 3) embed_sum_kernel(const __grid_
           } else {
             float* to = p.parts + ((long long)chunk * 2 + (from ? 0 : 1)) * p.H + c;
 #pragma unroll
-            for (int v = 0; v < VEC; v++) to[v] = sum[k][v];
+            for (int v = 0; v < VEC; v++)
+              to[v] = sum[k][v];
           }
         }
 #pragma unroll
@@ -410,16 +412,15 @@ __global__ void __launch_bounds__(JOIN_THREADS) embed_join_kernel(const __grid_c
   grid_wait();
   __shared__ int2 list[JOIN_THREADS];              // chunk of the round where a row begins, and the row
   __shared__ long long ends[JOIN_THREADS];         // the last chunk that it goes on in
-  __shared__ int found;
+  __shared__ int found, heads[JOIN_THREADS];       // rows that the round's chunks begin with
   __shared__ float s[JOIN_ROWS][JOIN_SLAB];
   const int col = threadIdx.x % JOIN_COLS, r = threadIdx.x / JOIN_COLS, slabs = (p.H + JOIN_SLAB - 1) / JOIN_SLAB;
   const long long last = (p.T - 1LL) / p.chunk;    // chunk
   long long item = blockIdx.x;                     // of this CTA, counted over all rounds
   for (long long c0 = 0; c0 + 2 <= last; c0 += JOIN_THREADS) {
-    if (threadIdx.x == 0) found = 0;
-    __syncthreads();
     const long long chunk = c0 + threadIdx.x;
     bool here = chunk + 2 <= last;
+    heads[threadIdx.x] = chunk <= last ? p.ids[chunk * p.chunk] : -1;
     int id = 0;
     if (here) {
       const long long begin = chunk * p.chunk;
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) embed_join_kernel(const __grid_c
       long long lo = chunk + 2, hi = last;
       while (lo < hi) {                            // up to the last chunk that begins with the row
         const long long mid = (lo + hi + 1) / 2;
-        if (p.ids[mid * p.chunk] == id) lo = mid; else hi = mid - 1;
+        if ((mid - c0 < JOIN_THREADS ? heads[mid - c0] : p.ids[mid * p.chunk]) == id) lo = mid; else hi = mid - 1;
       }
       list[at] = make_int2((int)threadIdx.x, id);
       ends[at] = lo;
@@ -477,9 +478,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) embed_join_kernel(const __grid_c
 }
 
 int vec_of(int H, uintptr_t at) { return H % 8 == 0 && at % 16 == 0 ? 8 : H % 2 == 0 && at % 4 == 0 ? 2 : 1; }
-// Tokens of a chunk: four chunks per SM, at least 8 tokens
+// Tokens of a chunk: three chunks per SM, as many as are resident, at least 8 tokens
 int chunk_of(int T) {
-  const int most = (T + 4 * lb_num_sms() - 1) / (4 * lb_num_sms());
+  const int most = (T + 3 * lb_num_sms() - 1) / (3 * lb_num_sms());
   return most < 8 ? 8 : most > MAX_CHUNK ? MAX_CHUNK : most;
 }
 // Bits of a row or V, in passes of up to ten
@@ -491,17 +492,17 @@ int passes_of(int V, int& bits) {
   return passes;
 }
 long long up(long long bytes) { return (bytes + 255) / 256 * 256; }
-template <int KEEP>
-int launch_radix(const OrderParams& o, cudaStream_t s) {
-  static bool done[64] = {false};      // (of a device: an attribute counts where it was set)
+// (an attribute counts on the device where it was set)
+int launch_order(void (*fn)(const OrderParams), bool* done, const OrderParams& o, cudaStream_t s) {
+  constexpr int smem = (int)sizeof(RadixShared);
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return LB_ERR_LAUNCH;
   if (!done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(embed_radix_kernel<KEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(RadixShared));
+    const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) { cudaGetLastError(); g_lb_last_cuda_error = (int)e; return LB_ERR_LAUNCH; }
     done[dev] = true;
   }
-  return lb_launch_cluster(true, CLUSTER, embed_radix_kernel<KEEP>, CLUSTER, ORDER_THREADS, sizeof(RadixShared), s, o);
+  return lb_launch_cluster(true, CLUSTER, fn, CLUSTER, ORDER_THREADS, smem, s, o);
 }
 constexpr int KEPT = 4;                // elements of a lane in registers: up to 32768 tokens
 constexpr long long CLEAR_BYTES = 65536;      // of a CTA that clears
@@ -551,10 +552,12 @@ extern "C" int lb_embed_sorted_bwd(const void* tok, int id_bytes, const void* dy
     o.b = (int2*)(at + up(8LL * T));
     at += 2 * up(8LL * T);
     o.passes = passes_of(V, o.bits);
-    const int rc = T <= KEPT * 32 * ORDER_WARPS * CLUSTER ? launch_radix<KEPT>(o, s) : launch_radix<0>(o, s);
+    static bool done[2][64] = {};
+    const int rc = T <= KEPT * 32 * ORDER_WARPS * CLUSTER ? launch_order(embed_radix_kernel<KEPT>, done[0], o, s) : launch_order(embed_radix_kernel<0>, done[1], o, s);
     if (rc) return rc;
   }
-  const int vec = vec_of(H, (uintptr_t)dy | (uintptr_t)dw), width = SUM_THREADS * vec * (vec == 8 ? 1 : 4);      // columns of a CTA
+  const int vec = vec_of(H, (uintptr_t)dy | (uintptr_t)dw);
+  const int width = SUM_THREADS * (vec == 8 ? 8 : vec * 4);      // columns of a CTA
   SumParams p{(const bf16*)dy, (bf16*)dw, o.ids, o.place, (float*)at, T, H, V, chunk_of(T), scale, 0, 0, 0};
   const long long chunks = (T + p.chunk - 1LL) / p.chunk, rows = CLEAR_BYTES / (H * 2LL);
   p.slabs = (unsigned)((H + width - 1LL) / width);
@@ -564,8 +567,8 @@ extern "C" int lb_embed_sorted_bwd(const void* tok, int id_bytes, const void* dy
 #define LB_CALL(VEC, K, U) LB_LAUNCH((embed_sum_kernel<VEC, K, U>), (unsigned)grid, SUM_THREADS, 0, s, p)
   switch (vec) {
     case 8: LB_CALL(8, 1, 8); break;
-    case 2: LB_CALL(2, 4, 4); break;
-    default: LB_CALL(1, 4, 4); break;
+    case 2: LB_CALL(2, 4, 8); break;
+    default: LB_CALL(1, 4, 8); break;
   }
 #undef LB_CALL
   if (chunks > 2) LB_LAUNCH(embed_join_kernel, 2 * lb_num_sms(), JOIN_THREADS, 0, s, p);

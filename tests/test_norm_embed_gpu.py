@@ -220,7 +220,7 @@ def _check_embedding(tokens, V, H, scale=1.0, start=0, w=None, dy=None):
 
 @pytest.mark.parametrize("T,V,H", [
     (1, 1, 8), (1, 10, 64), (3, 5, 1), (7, 4, 2), (8, 100, 1021), (65, 30, 6), (300, 7, 264), (511, 2000, 2048), (700, 50, 4104), (2100, 900, 72), (5000, 64, 33),
-    (4096, 3000, 16), (4097, 1023, 24), (4097, 1024, 7), (9000, 140000, 8), (8191, 2, 16), (20000, 1100000, 1),
+    (4096, 3000, 16), (4097, 1023, 24), (4097, 1024, 7), (9000, 140000, 8), (8191, 2, 16), (20000, 1100000, 1), (16384, 32000, 8), (16385, 1000, 5), (16383, 70000, 3), (12000, 1, 9), (33000, 300, 2),
 ])
 @pytest.mark.parametrize("wide", [True, False])
 def test_embedding(T, V, H, wide):
