@@ -697,7 +697,8 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           tmem_ld32(to_addr + c, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 8; i++) o[(c / 4 + i) * C::BM] = reinterpret_cast<const float4*>(r)[i];
+          for (int i = 0; i < 8; i++)
+            if (row < p.Sq) o[(c / 4 + i) * C::BM] = reinterpret_cast<const float4*>(r)[i];
         }
         if (set == 0) {
           float* s = pp.part_s + part * (3 * C::BM) + quad * 32 + lane;
