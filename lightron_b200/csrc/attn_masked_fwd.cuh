@@ -595,7 +595,8 @@ ma_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           float2 theirs;
           meet(make_float2(m_new, 0.f), theirs);
           m_new = max2(m_new, theirs.x);
-          const bool grow = !(m_i != -INFINITY && (m_new - m_i) * unit <= 8.f);
+          constexpr float LAG = WINDOW && GRAD && CAP == CAP_MAX ? 0.f : 8.f;
+          const bool grow = !(m_i != -INFINITY && (m_new - m_i) * unit <= LAG);
           if (__any_sync(0xffffffffu, grow)) {
             // (where a row has seen nothing yet there is nothing to rescale)
             rescale = __any_sync(0xffffffffu, grow && m_i != -INFINITY);
@@ -916,10 +917,18 @@ int launch_fwd(const MaParams& a, void* ws, long long ws_bytes, cudaStream_t s) 
   p.f.set(a, true, twice);
   const bool bias = a.slopes != nullptr;
   if (a.softcap <= 0.f) return bias ? launch<D, NO_CAP, true, WINDOW>(maps, p, (unsigned)grid, s) : launch<D, NO_CAP, false, WINDOW>(maps, p, (unsigned)grid, s);
-  if (p.f.cap1 <= 80.f) return bias ? launch<D, CAP_ZERO, true, WINDOW>(maps, p, (unsigned)grid, s) : launch<D, CAP_ZERO, false, WINDOW>(maps, p, (unsigned)grid, s);
-  // (above 55 the running maximum is kept, with and without slopes by the form that has the bias: such caps are rare, and four forms fewer are built.  Without slopes a form of its own
-  // is faster: cap 200, this one / its own, 8 x 2048, 32 / 4 heads, d 64 412 / 362 us, both ways 710 / 645; 1 x 8192, 32 / 8 heads, d 128 830 / 740, both ways 1710 / 1585.)
-  return launch<D, CAP_MAX, true, WINDOW>(maps, p, (unsigned)grid, s);
+  if constexpr (WINDOW) {
+    // For gradients the weights are relative to the row's maximum, as it stands: the largest is 1 and is not rounded, and D is nearer to what it stands for.  (Distance to 64 bits relative to zero /
+    // to the maximum that may lag by 2^8 / to the maximum: 3 x 1531, window 333, cap 30, 16 / 4 heads, d 96, o 1.90e-3 / 1.83e-3 / 1.74e-3, dq 2.57e-3 / 2.51e-3 / 2.45e-3; the kernel 53 / 55 / 57 us.)
+    if (a.o_lo) return bias ? launch_form<D, CAP_MAX, true, true, true>(maps, p, (unsigned)grid, s) : launch_form<D, CAP_MAX, false, true, true>(maps, p, (unsigned)grid, s);
+    if (p.f.cap1 <= 80.f) return bias ? launch_form<D, CAP_ZERO, true, false, true>(maps, p, (unsigned)grid, s) : launch_form<D, CAP_ZERO, false, false, true>(maps, p, (unsigned)grid, s);
+    return launch_form<D, CAP_MAX, true, false, true>(maps, p, (unsigned)grid, s);
+  } else {
+    if (p.f.cap1 <= 80.f) return bias ? launch<D, CAP_ZERO, true, false>(maps, p, (unsigned)grid, s) : launch<D, CAP_ZERO, false, false>(maps, p, (unsigned)grid, s);
+    // (above 55 the running maximum is kept, with and without slopes by the form that has the bias: such caps are rare, and four forms fewer are built.  Without slopes a form of its own
+    // is faster: cap 200, this one / its own, 8 x 2048, 32 / 4 heads, d 64 412 / 362 us, both ways 710 / 645; 1 x 8192, 32 / 8 heads, d 128 830 / 740, both ways 1710 / 1585.)
+    return launch<D, CAP_MAX, true, false>(maps, p, (unsigned)grid, s);
+  }
 }
 
 // Copies the status words of the forward to host memory and clears them.
