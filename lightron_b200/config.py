@@ -65,8 +65,10 @@ class ModelArgs:
             raise ValueError(f"attn_sinks must be at least 0, and have a meaning with attn_window only, got {self.attn_sinks!r}")
         if type(self.attn_global_freq) is not int or self.attn_global_freq < 0 or (self.attn_global_freq and self.attn_window is None):
             raise ValueError(f"attn_global_freq must be at least 0, and has a meaning with attn_window only, got {self.attn_global_freq!r}")
-        if self.embed_scale is not None and not abs(self.embed_scale) < float("inf"):
-            raise ValueError(f"embed_scale must be finite, got {self.embed_scale}")
+        if self.embed_scale is not None:
+            if not abs(self.embed_scale) < float("inf"):
+                raise ValueError(f"embed_scale must be finite, got {self.embed_scale}")
+            self.embed_scale = float(self.embed_scale)
         if self.cp_size > 1 and self.packed_attention:
             raise ValueError("attn_softcap, attn_alibi, rope_sections, attn_window and qk_norm are not built for context parallelism")
         if self.n_kv_heads is None:

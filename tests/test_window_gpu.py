@@ -111,6 +111,49 @@ def test_last_queries_of_a_longer_sequence(Sq, Sk, window, sinks, hq, hkv, d):
     assert (got[2][:, hidden] == 0).all() and (got[3][:, hidden] == 0).all()
 
 
+@pytest.mark.parametrize("Sq,Sk,window,sinks,causal,docs", [(70, 1100, 90, 5, False, 0), (5, 900, 200, 140, False, 0), (3, 700, 60, 4, True, 250), (100, 700, 150, 3, True, 300), (40, 640, 33, 200, False, 200),
+                                                            (1, 300, 40, 2, True, 90)])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 64), (32, 1, 128), (64, 1, 64), (6, 2, 96)])
+def test_few_queries_with_documents_and_both_ways(Sq, Sk, window, sinks, causal, docs, hq, hkv, d):
+    """The heads of a group as a tile's rows, two to 32 of them, and groups that are not taken so."""
+    _check(2, Sq, Sk, hq, hkv, d, window, sinks, causal=causal, docs=docs, seed=3)
+
+
+def test_many_key_heads_and_pieces():
+    """Walks of sinks in many pieces, more key blocks than are listed at once, and fewer pieces than there is room for."""
+    _check(1, 2000, 2000, 16, 1, 64, 40, 300)
+    _check(5, 900, 900, 2, 2, 64, 20, 3, docs=40)
+    q, k, v, do = _inputs(3, 130000, 130000, 1, 1, 8)
+    got = _run(q, k, v, do, window=5, sinks=2)
+    _status_ok()
+    at = torch.arange(130000, device="cuda")
+    keys = torch.stack([torch.zeros_like(at), torch.ones_like(at)] + [at - 4 + i for i in range(5)], dim=1)      # sinks, and the window where it does not hold them
+    see = (keys >= 0) & (keys <= at[:, None])
+    see[:, 2:] &= keys[:, 2:] >= 2
+    pick = keys.clamp_min(0)
+    qd, kd, vd = (t[:, :, 0].double().requires_grad_() for t in (q, k, v))
+    s = (qd[:, :, None] * kd[:, pick]).sum(-1) * 8 ** -0.5
+    p = s.masked_fill(~see, -1e300).softmax(-1)
+    o = (p[..., None] * vd[:, pick]).sum(2)
+    want = (o.detach(), *torch.autograd.grad(o, (qd, kd, vd), do[:, :, 0].double()))
+    _close([g[:, :, 0] for g in got], want)
+
+
+def test_on_two_streams():
+    cases = [(_inputs(1, 1500, 1500, 8, 2, 64, seed=i), dict(window=200, sinks=140 * i)) for i in range(2)]
+    want = [_run(*t, **kw) for t, kw in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cases], [[], []]
+    for _ in range(4):
+        for st, (t, kw), g in zip(streams, cases, got):
+            with torch.cuda.stream(st):
+                g.append(_run(*t, **kw))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for r in g:
+            assert all(torch.equal(r[i], w[i]) for i in (0, 2, 3)) and rel(r[1], w[1]) < 2e-3
+
+
 @pytest.mark.parametrize("cap", [0.0, 20.0, 200.0])
 @pytest.mark.parametrize("slopes", [None, [0.5, 0.01, 0.0, 0.25], [-0.01, -0.3, -1.3, 0.25]])
 @pytest.mark.parametrize("Sq,Sk,d,window,sinks,causal,docs", [
