@@ -35,7 +35,7 @@ struct NormRopeParams {
 // A head is P2 lanes', 8 columns each (d / 8 of them, up to the next power of two, work); a warp takes 32 / P2 heads of q or of k at a time, a group, first those of q, then those of k: what differs
 // between the two is decided outside of the loops.  AHEAD groups are on their way, and pointers are counted up: what bounds simpler forms is instructions, not memory (16384 tokens, 36 heads of
 // 64: heads of q and k in one loop, strides multiplied out and numbers one at a time, 156 a group forward and 305 backward, 32 and 61 us).
-// The first columns of a lane's four pairs are two pairs of numbers, the second ones two more: all but the forward's rotation and sums over lanes is done two numbers at a time.
+// The first columns of a lane's four pairs are two pairs of numbers, the second ones two more: all but sums over lanes is done two numbers at a time.
 template <int P2>
 struct Lanes {
   static constexpr int G = 32 / P2;
