@@ -44,6 +44,7 @@ struct BwdParams {
   int2* joined;
   int *n_items, *cut_blocks;     // {how many pieces, how many key blocks in several}, and those
   int chunk, extra;              // longest piece wanted, pieces beyond one per key block that there is room for
+  int by_head;                   // all pieces of a head, then the next head's; else those of all heads together
   int acc_d;                     // columns of dq_acc: head_dim in whole pieces of 32
   MaTerms f;
   f32x2 scale2;                  // the scale, twice
@@ -402,11 +403,13 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     pair = t % pairs;
     nblk = t / pairs;
   } else {
-    const int grp = (int)blockIdx.x / (n_nblk * GROUP);
-    const int in_grp = (int)blockIdx.x - grp * n_nblk * GROUP;
-    const int gsize = min(GROUP, p.hkv * p.B - grp * GROUP);
+    // (under a window all walks are as long, and a pair's share most when they run together)
+    const int group = p.window ? 1 : GROUP;
+    const int grp = (int)blockIdx.x / (n_nblk * group);
+    const int in_grp = (int)blockIdx.x - grp * n_nblk * group;
+    const int gsize = min(group, p.hkv * p.B - grp * group);
     nblk = in_grp / gsize;
-    pair = grp * GROUP + in_grp % gsize;
+    pair = grp * group + in_grp % gsize;
   }
   const int off = p.Sk - p.Sq;
   const int rep = p.hq / p.hkv;
@@ -436,10 +439,11 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
 
   [[maybe_unused]] int4 piece = make_int4(0, 0, 0, 0);          // (a CTA without one leaves nothing)
   if constexpr (FORM == LIST) {
-    const int i = (int)blockIdx.x / p.hkv;
+    const int of_head = (int)gridDim.x / p.hkv, head = pp.by_head ? (int)blockIdx.x / of_head : (int)blockIdx.x % p.hkv;
+    const int i = pp.by_head ? (int)blockIdx.x - head * of_head : (int)blockIdx.x / p.hkv;
     if (i < *pp.n_items) piece = pp.items[i];
     nblk = piece.x % n_nblk;
-    pair = piece.x / n_nblk * p.hkv + (int)blockIdx.x % p.hkv;
+    pair = piece.x / n_nblk * p.hkv + head;
   }
   if (FORM == WHOLE && pp.order) {
     const int e = pp.order[(int)blockIdx.x / p.hkv];
@@ -891,16 +895,19 @@ int parts_of(int B, int Sq, int Sk, int hq, int hkv, int causal, int sms) {
 
 // Under a window: the longest piece of a walk, and how many pieces there may be beyond one per key block.  By the model of parts_of(), for keys that queries near them see and for blocks of sinks,
 // which all queries behind them see; where the mask comes from the device documents cut the walks shorter, and there are more, shorter ones of sinks: then pieces may get twice as long.
-struct Pieces { int length, extra; };
-Pieces pieces_of(const MaParams& p, int sms) {
+// Without a mask, and with two CTAs for each SM or more, pieces go head by head and none is longer than the walk of other keys: 148 CTAs then work on two heads or three, whose Q, dO and dQ's sums stay in L2 (1 x 8192,
+// window 1024, 4 sinks, 32 / 8 heads, d 128, longest of all heads first / head by head: 912 / 472 MB of DRAM, the kernel 400 / 381 us; 3 x 1531, window 333, 130 sinks, one wave of CTAs: all kernels 168 / 190).
+struct Pieces { int length, extra; bool by_head; };
+Pieces pieces_of(const MaParams& p, bool masked, int sms) {
   const int n_mblocks = (p.Sq + 127) / 128, n_nblk = (p.Sk + 127) / 128, rep = p.hq / p.hkv;
   const long long pairs = (long long)p.hkv * p.B, span = 128 + (p.causal ? 1LL : 2LL) * (p.window - 1LL);
   // (key and query blocks that begin at the same places meet in one block fewer)
   const long long most = (span + 127) / 128 + ((p.Sk - p.Sq) % 128 || !p.causal ? 1 : 0);
   const long long near = std::min<long long>(most, n_mblocks) * rep, far = (long long)n_mblocks * rep;
   const long long n_far = std::min<long long>((p.sinks + 127) / 128, n_nblk), n_near = n_nblk - n_far;
+  const bool by_head = !masked && n_nblk * pairs >= 2LL * sms;
   double best_time = 0.0;
-  Pieces best{(int)far, 0};
+  Pieces best{(int)far, 0, by_head};
   auto look = [&](long long length) {
     const long long a = (near + length - 1) / length, b = (far + length - 1) / length;
     const long long extra = n_near * (a - 1) + n_far * (b - 1);
@@ -908,10 +915,11 @@ Pieces pieces_of(const MaParams& p, int sms) {
     const double time = std::max(std::max((near + a - 1) / a, n_far ? (far + b - 1) / b : 0) + 9.0, 1.1 * work) + (extra ? 1.0 : 0.0);
     if (best_time == 0.0 || time < best_time) {
       best_time = time;
-      best = Pieces{(int)length, (int)std::min<long long>((2 * extra + (p.sinks ? 4 : 0)) * p.B, 1 << 24)};
+      best = Pieces{(int)length, (int)std::min<long long>((2 * extra + (p.sinks ? 4 : 0)) * p.B, 1 << 24), by_head};
     }
   };
-  for (long long parts = 1; parts <= std::min<long long>(far, 64); parts++) look((far + parts - 1) / parts);
+  for (long long parts = 1; parts <= std::min<long long>(far, 64); parts++)
+    if (!by_head || (far + parts - 1) / parts <= near) look((far + parts - 1) / parts);
   for (long long parts = 1; parts <= std::min<long long>(near, 32); parts++) look((near + parts - 1) / parts);
   return best;
 }
@@ -964,7 +972,9 @@ bool listed(const MaParams& p, const Pieces& c) { return p.window > 0 && p.Sk > 
 
 long long ma_bwd_ws_bytes(const MaParams& p) {
   if (p.window > 0) {
-    const Pieces c = pieces_of(p, lb_num_sms());
+    // (with a mask or without, which is not known here)
+    Pieces c = pieces_of(p, false, lb_num_sms());
+    c.extra = std::max(c.extra, pieces_of(p, true, lb_num_sms()).extra);
     return (stats_floats(p) + dq_floats(p) + 2 * piece_floats(p, c) + 4 * (order_ints(p) + c.extra) + 3 * order_ints(p) + 4) * (long long)sizeof(float);
   }
   return (stats_floats(p) + dq_floats(p) + 2 * part_floats(p, parts_of(p.B, p.Sq, p.Sk, p.hq, p.hkv, p.causal, lb_num_sms())) + order_ints(p)) * (long long)sizeof(float);
@@ -980,12 +990,13 @@ int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s) {
   p.dk_acc = p.dq_acc + dq_floats(a);
   p.f.set(a, false, twice);
   p.scale2 = twice(a.scale);
-  const Pieces c = a.window > 0 ? pieces_of(a, lb_num_sms()) : Pieces{0, 0};
+  const Pieces c = a.window > 0 ? pieces_of(a, a.qb != nullptr, lb_num_sms()) : Pieces{0, 0, false};
   p.parts = 1;
   p.order = nullptr;
   if (listed(a, c)) {
     p.chunk = c.length;
     p.extra = c.extra;
+    p.by_head = c.by_head;
     p.dv_acc = p.dk_acc + piece_floats(a, c);
     p.items = reinterpret_cast<int4*>(p.dv_acc + piece_floats(a, c));
     p.joined = reinterpret_cast<int2*>(p.items + order_ints(a) + c.extra);

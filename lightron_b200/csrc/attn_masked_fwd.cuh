@@ -33,8 +33,8 @@
 // the window's range begins.  Where one range over both takes no more blocks, it is one.  So a window of w keys costs (w + 127) / 128 blocks, rounded up, and a few sinks one more: of 1024 keys and 4 sinks ten,
 // for eight of visible pairs.  1 x 8192, 32 / 8 heads, d 128 182 to 201 us (causal without a window 595); 8 x 2048, window 512 over documents of 900, 4 sinks each, 32 / 4 heads, d 64 177 to 193.
 // Few queries (WINDOW, less than 128 of them): a tile's rows are the 2^shift heads of a group for each query, so that K and V are read once for all of them: one token of 8 sequences, window 4096,
-// 32 / 8 heads, d 128, a tile for each head / for each group, 85 / 35 us (33 once rows without a query left no parts) and 6 for the join of four splits.  (Splits for twice as many CTAs as
-// find room: 42, for each CTA's fixed part is some 4 us.)
+// 32 / 8 heads, d 128, a tile for each head / for each group, 85 / 35 us (33 once rows without a query left no parts) and 6 for the join of four splits.  (Splits for two and a half to four times
+// as many CTAs as find room, both kernels: 37 -> 48, for each CTA's fixed part is some 4 us.)
 #pragma once
 #include "attn_masked.cuh"
 #include "tcgen05.cuh"
