@@ -373,3 +373,78 @@ def test_on_two_streams():
     torch.cuda.synchronize()
     for g, e in zip(got, want):
         assert all(torch.equal(x, e) for x in g[::2]) and all(torch.equal(x, y[0]) for x in g[1::2])
+
+
+# ---- refusals, hooks ------------------------------------------------------------------------------
+
+
+def test_refusals_on_the_gpu():
+    from lightron_b200.ops import functional as OF
+    q, k, wq, wk, cos, sin = _norm_case(1, 4, 2, 1, 64)
+    w, tokens = _rand(5, 8), torch.zeros(3, dtype=torch.long, device="cuda")
+    for call in (lambda: OF.qk_norm_rope(q, k, wq.float(), wk, cos, sin), lambda: OF.qk_norm_rope(q, k, wq, wk.cpu(), cos, sin), lambda: OF.qk_norm_rope(q, k, wq, wk, cos.cpu(), sin.cpu()),
+                 lambda: OF.qk_norm_rope(q, k.cpu(), wq, wk, cos, sin), lambda: OF.qk_norm_rope(q, k, wq, wk, cos, sin, eps=float("nan")),
+                 lambda: OF.qk_norm_rope(q, k, wq, wk, cos, sin, positions=torch.zeros(4, dtype=torch.int32)), lambda: OF.qk_norm_rope(q, k[:, :3], wq, wk, cos, sin),
+                 lambda: OF.scaled_embedding(tokens.cpu(), w), lambda: OF.scaled_embedding(tokens.to(torch.int16), w), lambda: OF.scaled_embedding(tokens, w, float("inf")),
+                 lambda: OF.scaled_embedding(tokens, w, 1.0, -1), lambda: OF.scaled_embedding(tokens, w[0]),
+                 lambda: OF.masked_attention(q, k, k, window=0), lambda: OF.masked_attention(q, k, k, window=2, sinks=-1), lambda: OF.masked_attention(q, k, k, sinks=2),
+                 lambda: OF.masked_attention(q, k, k, window=True), lambda: OF.masked_attention(_rand(1, 4, 2, 136), _rand(1, 4, 2, 136), _rand(1, 4, 2, 136), window=2)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_other_types_and_sizes_run_without_the_kernels():
+    """fp32, fp16 and head sizes that the kernels do not take, by PyTorch operations."""
+    from lightron_b200.ops import functional as OF
+    from lightron_b200.ops import reference as ref
+    for d, dtype, bound in ((64, torch.float32, 1e-5), (64, torch.float16, 2.0 ** -11 + 1e-5), (6, BF16, HALF + 1e-4), (264, BF16, HALF + 1e-4)):
+        q, k, wq, wk = _rand(2, 5, 4, d, seed=1, dtype=dtype), _rand(2, 5, 2, d, seed=2, dtype=dtype), _rand(d, seed=3, dtype=dtype), _rand(d, seed=4, dtype=dtype)
+        cos, sin = ref.rope_tables(d, 9, device="cuda")
+        y = OF.qk_norm_rope(q, k, wq, wk, cos, sin)
+        at = torch.arange(5, device="cuda").expand(1, 2, 5)
+        for got, x, w in ((y[0], q, wq), (y[1], k, wk)):
+            assert got.dtype == dtype and rel(got, norm_rope64(x.double(), w.double(), cos, sin, at, [0] * (d // 2), 1e-6)) < bound
+    w = _rand(5, 8, dtype=torch.float32).requires_grad_()
+    tokens = torch.tensor([1, 1, 4, 9], device="cuda")
+    y = OF.scaled_embedding(tokens, w, 3.0)
+    dw, = torch.autograd.grad(y.sum(), w)
+    assert torch.equal(y, torch.cat((w.detach()[tokens[:3]] * 3, torch.zeros(1, 8, device="cuda")))) and dw[1].eq(6).all() and dw[4].eq(3).all() and dw[[0, 2, 3]].eq(0).all()
+
+
+def test_saved_tensors_may_wait_on_the_cpu():
+    from lightron_b200.ops import functional as OF
+    q, k, wq, wk, cos, sin = _norm_case(2, 30, 4, 2, 64)
+    v = _rand(2, 30, 2, 64, seed=6)
+    w, tokens = _rand(50, 64, seed=7), torch.randint(0, 60, (300,), generator=torch.Generator().manual_seed(1)).cuda()
+    ins = [t.detach().requires_grad_() for t in (q, k, wq, wk, v, w)]
+
+    def step():
+        tq, tk = OF.qk_norm_rope(*ins[:4], cos, sin)
+        o = OF.masked_attention(tq, tk, ins[4], window=7, sinks=2)
+        e = OF.scaled_embedding(tokens, ins[5], 1.5)
+        return (o, e), lambda: torch.autograd.grad((o, e), ins, (_rand(*o.shape, seed=8), _rand(*e.shape, seed=9)))
+    out, back = step()
+    want = back()
+    with torch.autograd.graph.save_on_cpu():
+        other, back = step()
+    got = back()
+    assert all(torch.equal(a, b) for a, b in zip(out, other)) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_arguments_written_to_are_noticed():
+    """What backward needs is not what it was: an error, no other gradient."""
+    from lightron_b200.ops import functional as OF
+    q, k, wq, wk, cos, sin = _norm_case(1, 3, 2, 1, 64)
+    leaf = q.detach().requires_grad_()
+    x = leaf * 1
+    y, _ = OF.qk_norm_rope(x, k, wq, wk, cos, sin)
+    with torch.no_grad():
+        x.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    tokens = torch.zeros(3, dtype=torch.long, device="cuda")
+    w = _rand(5, 8).requires_grad_()
+    e = OF.scaled_embedding(tokens, w)
+    tokens.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        e.sum().backward()
