@@ -874,6 +874,7 @@ class _MaskedAttn(torch.autograd.Function):
 
 MASKED_MAX_HEAD_DIM = 128
 _FP32_TINY, _FP32_MAX = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
+_INT_MAX = (1 << 31) - 1
 
 
 def _check_masked(q, k, v, mask, causal, scale, softcap, slopes) -> bool:
@@ -1109,6 +1110,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     B, S, _, d = q.shape
     positions, axes = _positions_of(positions, axes, B, S, d, cos, sin)
     if native.use_native(q) and q.numel() and k.numel() and d % 8 == 0 and d <= NORM_ROPE_MAX_HEAD_DIM and max(axes, default=0) < 8:
+        if max(B, S, q.shape[2], k.shape[2], cos.shape[0]) > _INT_MAX:
+            raise ValueError(f"qk_norm_rope on the GPU takes sizes up to {_INT_MAX}, got {tuple(q.shape)}, {tuple(k.shape)} and tables of {cos.shape[0]} rows")
         return _apply(_QKNormRope, q, k, q_weight, k_weight, cos.contiguous(), sin.contiguous(), positions, axes, float(eps))
     if positions is None:
         positions = torch.arange(S, device=q.device, dtype=torch.int32).expand(max(axes, default=0) + 1, -1)
@@ -1454,6 +1457,7 @@ class _ScaledEmbedding(torch.autograd.Function):
 
 
 EMBED_MAX_TOKENS = 1 << 30
+EMBED_MAX_START = 1 << 62
 
 
 def scaled_embedding(tokens: torch.Tensor, w: torch.Tensor, scale: float = 1.0, vocab_start: int = 0) -> torch.Tensor:
@@ -1468,11 +1472,11 @@ def scaled_embedding(tokens: torch.Tensor, w: torch.Tensor, scale: float = 1.0, 
         raise ValueError(f"tokens must be int32 or int64 on {w.device}, got {tokens.dtype} on {tokens.device}")
     if not -_FP32_MAX <= scale <= _FP32_MAX:
         raise ValueError(f"scale must be finite, in 32 bits, got {scale}")
-    if vocab_start < 0:
-        raise ValueError(f"vocab_start {vocab_start} is negative")
+    if not isinstance(vocab_start, int) or isinstance(vocab_start, bool) or not 0 <= vocab_start <= EMBED_MAX_START:
+        raise ValueError(f"vocab_start must be a whole number from 0 to {EMBED_MAX_START}, got {vocab_start!r}")
     if native.use_native(w) and w.numel() and tokens.numel():
-        if tokens.numel() > EMBED_MAX_TOKENS:
-            raise ValueError(f"scaled_embedding on the GPU takes up to {EMBED_MAX_TOKENS} tokens, got {tokens.numel()}")
+        if tokens.numel() > EMBED_MAX_TOKENS or max(w.shape) >= _INT_MAX:
+            raise ValueError(f"scaled_embedding on the GPU takes up to {EMBED_MAX_TOKENS} tokens, and rows and columns below {_INT_MAX}, got {tokens.numel()} and {tuple(w.shape)}")
         return _apply(_ScaledEmbedding, tokens, w, float(scale), int(vocab_start))
     return ref.scaled_embedding(tokens, w, scale, vocab_start)
 

@@ -115,6 +115,12 @@ def test_refusals(call):
         call()
 
 
+@pytest.mark.parametrize("start", [1 << 63, (1 << 64) + 2, 1.5, True, None])
+def test_a_vocab_start_that_is_no_id_is_refused(start):
+    with pytest.raises(ValueError):
+        _embed(vocab_start=start)()
+
+
 # ---- in the model -----------------------------------------------------------------------------------
 
 LOCAL = dict(attn_window=4, attn_sinks=2, qk_norm=True, embed_scale=3.0)

@@ -393,6 +393,18 @@ def test_refusals_on_the_gpu():
             call()
 
 
+def test_sizes_past_31_bits_are_refused():
+    """Views of one row, so that nothing of such a size is there."""
+    from lightron_b200.ops import functional as OF
+    q, k, wq, wk, cos, sin = _norm_case(1, 1, 1, 1, 8)
+    w, tokens, most = _rand(1, 8), torch.zeros(3, dtype=torch.long, device="cuda"), 1 << 31
+    for call in (lambda: OF.qk_norm_rope(q.expand(1, most, 1, 8), k.expand(1, most, 1, 8), wq, wk, cos, sin), lambda: OF.qk_norm_rope(q, k.expand(1, 1, most + 1, 8), wq, wk, cos, sin),
+                 lambda: OF.scaled_embedding(tokens, w.expand(most, 8)), lambda: OF.scaled_embedding(tokens, w[:, :1].expand(1, most + 8)),
+                 lambda: OF.scaled_embedding(tokens[:1].expand(most), w), lambda: OF.scaled_embedding(tokens, w, 1.0, (1 << 64) + 1)):
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_other_types_and_sizes_run_without_the_kernels():
     """fp32, fp16 and head sizes that the kernels do not take, by PyTorch operations."""
     from lightron_b200.ops import functional as OF
