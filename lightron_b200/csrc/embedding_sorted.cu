@@ -509,7 +509,11 @@ int launch_order(void (*fn)(const OrderParams), bool* done, const OrderParams& o
 constexpr int KEPT = 4;                // elements of a lane in registers: up to 32768 tokens
 constexpr long long CLEAR_BYTES = 65536;      // of a CTA that clears
 
-int check_sizes(int T, int H, long long v0, long long v1) { return T <= 0 || T > (1 << 30) || H <= 0 || v0 < 0 || v1 <= v0 || v1 - v0 > 0x7ffffffeLL ? LB_ERR_SHAPE : LB_OK; }
+// (columns are counted in 32 bits, in steps of up to 2048 past the last one)
+constexpr int MOST_COLUMNS = 1 << 30;
+int check_sizes(int T, int H, long long v0, long long v1) {
+  return T <= 0 || T > (1 << 30) || H <= 0 || H > MOST_COLUMNS || v0 < 0 || v1 <= v0 || v1 - v0 > 0x7ffffffeLL ? LB_ERR_SHAPE : LB_OK;
+}
 
 }  // namespace
 

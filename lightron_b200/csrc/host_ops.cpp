@@ -1081,7 +1081,7 @@ PyObject* py_scaled_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
     LB_NOT_PLAIN;
   }
   if (!plain(w) || w->dim() != 2 || !here(*w) || !(sized(tok, *w, at::kLong) || sized(tok, *w, at::kInt)) || tok->numel() == 0 || tok->numel() > (1 << 30) || v0 < 0 || v0 > (1LL << 40) ||
-      !fits_int({w->size(0) + 2, w->size(1)}) || !(scale >= -FLT_MAX && scale <= FLT_MAX))
+      !fits_int({w->size(0) + 2}) || w->size(1) > (1 << 30) || !(scale >= -FLT_MAX && scale <= FLT_MAX))
     LB_NOT_PLAIN;
   return THPVariable_Wrap(unlocked([&, t = *tok, w_ = *w] { return ScaledEmbedding::apply(t, w_, scale, (int64_t)v0); }));
   END_HANDLE_TH_ERRORS

@@ -1457,6 +1457,7 @@ class _ScaledEmbedding(torch.autograd.Function):
 
 
 EMBED_MAX_TOKENS = 1 << 30
+EMBED_MAX_COLUMNS = 1 << 30
 EMBED_MAX_START = 1 << 62
 
 
@@ -1475,8 +1476,8 @@ def scaled_embedding(tokens: torch.Tensor, w: torch.Tensor, scale: float = 1.0, 
     if not isinstance(vocab_start, int) or isinstance(vocab_start, bool) or not 0 <= vocab_start <= EMBED_MAX_START:
         raise ValueError(f"vocab_start must be a whole number from 0 to {EMBED_MAX_START}, got {vocab_start!r}")
     if native.use_native(w) and w.numel() and tokens.numel():
-        if tokens.numel() > EMBED_MAX_TOKENS or max(w.shape) >= _INT_MAX:
-            raise ValueError(f"scaled_embedding on the GPU takes up to {EMBED_MAX_TOKENS} tokens, and rows and columns below {_INT_MAX}, got {tokens.numel()} and {tuple(w.shape)}")
+        if tokens.numel() > EMBED_MAX_TOKENS or w.shape[0] >= _INT_MAX or w.shape[1] > EMBED_MAX_COLUMNS:
+            raise ValueError(f"scaled_embedding on the GPU takes up to {EMBED_MAX_TOKENS} tokens, {EMBED_MAX_COLUMNS} columns and rows below {_INT_MAX}, got {tokens.numel()} and {tuple(w.shape)}")
         return _apply(_ScaledEmbedding, tokens, w, float(scale), int(vocab_start))
     return ref.scaled_embedding(tokens, w, scale, vocab_start)
 
