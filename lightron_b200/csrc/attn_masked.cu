@@ -208,7 +208,7 @@ extern "C" long long lb_masked_attn_bwd_ws_bytes(int B, int Sq, int Sk, int hq, 
   MaParams p{};
   if (check_sizes(B, Sq, Sk, hq, hkv, d)) return 0;
   p.B = B; p.Sq = Sq; p.Sk = Sk; p.hq = hq; p.hkv = hkv; p.d = d; p.causal = causal;
-  return ma_bwd_ws_bytes(p);
+  return ma_bwd_ws_bytes(p, false);
 }
 
 namespace {
@@ -220,7 +220,7 @@ int backward(const void* q, const void* k, const void* v, const void* o, const v
   if (windowed)
     if (const int rc = set_window(w.f, window, sinks)) return rc;
   if (!o_lo || !dout || !ws || !dq || !dk || !dv || misaligned(dout) || misaligned(ws) || misaligned(dq) || misaligned(dk) || misaligned(dv)) return LB_ERR_ARG;
-  if (ws_bytes < ma_bwd_ws_bytes(w.f)) return LB_ERR_CAPACITY;
+  if (ws_bytes < ma_bwd_ws_bytes(w.f, w.f.qb != nullptr)) return LB_ERR_CAPACITY;
   w.dout = (const bf16*)dout; w.dq = (bf16*)dq; w.dk = (bf16*)dk; w.dv = (bf16*)dv; w.stats = (float*)ws;
   w.dos = strides_at(strides + 9); w.dqs = strides_at(strides + 12); w.dks = strides_at(strides + 15); w.dvs = strides_at(strides + 18);
   if (bad_strides(w.dos) || bad_strides(w.dqs) || bad_strides(w.dks) || bad_strides(w.dvs)) return LB_ERR_SHAPE;
@@ -235,12 +235,12 @@ extern "C" int lb_masked_attn_bwd(const void* q, const void* k, const void* v, c
   return backward(q, k, v, o, o_lo, dout, lse, ws, ws_bytes, dq, dk, dv, B, Sq, Sk, hq, hkv, d, strides, scale, causal, softcap, slopes, q_bounds, k_bounds, false, 0, 0, stream);
 }
 
-// Under a window, as lb_window_attn_fwd(); ws: lb_window_attn_bwd_ws_bytes().
-extern "C" long long lb_window_attn_bwd_ws_bytes(int B, int Sq, int Sk, int hq, int hkv, int d, int causal, int window, int sinks) {
+// Under a window, as lb_window_attn_fwd(); ws: lb_window_attn_bwd_ws_bytes(), of calls with bounds (masked 1) or without (0).
+extern "C" long long lb_window_attn_bwd_ws_bytes(int B, int Sq, int Sk, int hq, int hkv, int d, int causal, int window, int sinks, int masked) {
   MaParams p{};
   if (check_sizes(B, Sq, Sk, hq, hkv, d)) return 0;
   p.B = B; p.Sq = Sq; p.Sk = Sk; p.hq = hq; p.hkv = hkv; p.d = d; p.causal = causal;
-  return set_window(p, window, sinks) ? 0 : ma_bwd_ws_bytes(p);
+  return set_window(p, window, sinks) ? 0 : ma_bwd_ws_bytes(p, masked != 0);
 }
 extern "C" int lb_window_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_lo, const void* dout, const void* lse, void* ws, long long ws_bytes,
                                   void* dq, void* dk, void* dv, int B, int Sq, int Sk, int hq, int hkv, int d, const long long* strides, float scale, int causal, float softcap,

@@ -48,7 +48,7 @@ int ma_launch_window_fwd(const MaParams& p, void* ws, long long ws_bytes, cudaSt
 int ma_launch_fwd(const MaParams& p, void* ws, long long ws_bytes, cudaStream_t s);
 long long ma_fwd_ws_bytes(const MaParams& p);
 int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s);
-long long ma_bwd_ws_bytes(const MaParams& p);
+long long ma_bwd_ws_bytes(const MaParams& p, bool masked);
 
 // What the kernels need of the scores' form, in units of log2: x * scale without a cap; with one, tanh(u) * times, u = x * by, as x * (c[0] + c[1] x^2 + c[2] x^4 + c[3] x^6) while
 // |x| <= limit: relative error 2.2e-6 up to u = 0.6 (coefficients of tanh(u) / u in u^2, found by least squares over Chebyshev points with weights that were raised

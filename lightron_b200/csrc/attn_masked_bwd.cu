@@ -970,11 +970,9 @@ bool listed(const MaParams& p, const Pieces& c) { return p.window > 0 && p.Sk > 
 
 }  // namespace
 
-long long ma_bwd_ws_bytes(const MaParams& p) {
+long long ma_bwd_ws_bytes(const MaParams& p, bool masked) {
   if (p.window > 0) {
-    // (with a mask or without, which is not known here)
-    Pieces c = pieces_of(p, false, lb_num_sms());
-    c.extra = std::max(c.extra, pieces_of(p, true, lb_num_sms()).extra);
+    const Pieces c = pieces_of(p, masked, lb_num_sms());
     return (stats_floats(p) + dq_floats(p) + 2 * piece_floats(p, c) + 4 * (order_ints(p) + c.extra) + 3 * order_ints(p) + 4) * (long long)sizeof(float);
   }
   return (stats_floats(p) + dq_floats(p) + 2 * part_floats(p, parts_of(p.B, p.Sq, p.Sk, p.hq, p.hkv, p.causal, lb_num_sms())) + order_ints(p)) * (long long)sizeof(float);

@@ -63,7 +63,7 @@ struct Api {
   int (*lb_masked_attn_bwd)(P, P, P, P, P, P, P, W, L, W, W, W, int, int, int, int, int, int, const L*, float, int, float, P, P, P, W);
   L (*lb_window_attn_fwd_ws_bytes)(int, int, int, int, int, int, int, int, int);
   int (*lb_window_attn_fwd)(P, P, P, W, W, W, W, L, int, int, int, int, int, int, const L*, float, int, float, P, P, P, int, int, W);
-  L (*lb_window_attn_bwd_ws_bytes)(int, int, int, int, int, int, int, int, int);
+  L (*lb_window_attn_bwd_ws_bytes)(int, int, int, int, int, int, int, int, int, int);
   int (*lb_window_attn_bwd)(P, P, P, P, P, P, P, W, L, W, W, W, int, int, int, int, int, int, const L*, float, int, float, P, P, P, int, int, W);
   int (*lb_rope_axes)(P, W, P, P, P, const unsigned char*, int, int, int, int, int, int, const L*, L, L, int, W);
   int (*lb_qk_norm_rope)(P, P, W, W, P, P, P, P, P, const unsigned char*, int, int, int, int, int, int, int, const L*, L, L, float, W);
@@ -455,7 +455,8 @@ struct MaskedAttention : Function<MaskedAttention> {
     Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(k.sizes(), k.options());
     const int window = (int)ctx->saved_data["window"].toInt(), sinks = (int)ctx->saved_data["sinks"].toInt();
     const float softcap = (float)ctx->saved_data["softcap"].toDouble();
-    const L bytes = window ? api.lb_window_attn_bwd_ws_bytes(m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d, m.causal, window, sinks) : api.lb_masked_attn_bwd_ws_bytes(m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d, m.causal);
+    const L bytes = window ? api.lb_window_attn_bwd_ws_bytes(m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d, m.causal, window, sinks, qi.defined())
+                           : api.lb_masked_attn_bwd_ws_bytes(m.B, m.Sq, m.Sk, m.hq, m.hkv, m.d, m.causal);
     Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
     L st[21];
     const Tensor* ts[7] = {&q, &k, &v, &dout, &dq, &dk, &dv};

@@ -845,7 +845,7 @@ def masked_bwd_native(q, k, v, o, o_lo, lse, do, causal: bool, scale: float, sof
     if dq is None:
         dq, dk, dv = torch.empty_like(o), torch.empty(B, Sk, hkv, d, dtype=q.dtype, device=q.device), torch.empty(B, Sk, hkv, d, dtype=q.dtype, device=q.device)
     lib, local = native.require(), (window, sinks) if window else ()
-    nbytes = (lib.lb_window_attn_bwd_ws_bytes if window else lib.lb_masked_attn_bwd_ws_bytes)(B, Sq, Sk, hq, hkv, d, int(causal), *local)
+    nbytes = lib.lb_window_attn_bwd_ws_bytes(B, Sq, Sk, hq, hkv, d, int(causal), *local, int(qb is not None)) if window else lib.lb_masked_attn_bwd_ws_bytes(B, Sq, Sk, hq, hkv, d, int(causal))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     native.call("lb_window_attn_bwd" if window else "lb_masked_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), o_lo.data_ptr(), do.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(),
                 dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, Sq, Sk, hq, hkv, d, _strides(q, k, v, do, dq, dk, dv), scale, int(causal), softcap,

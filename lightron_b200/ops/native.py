@@ -100,7 +100,7 @@ _SIGNATURES = {
     "lb_window_attn_fwd": [_P] * 7 + [_L] + [_I] * 6 + [_P, _F, _I, _F, _P, _P, _P, _I, _I, _P],
     "lb_window_attn_status": [_P],
     "lb_window_attn_bwd": [_P] * 8 + [_L] + [_P] * 3 + [_I] * 6 + [_P, _F, _I, _F, _P, _P, _P, _I, _I, _P],
-    "lb_window_attn_bwd_ws_bytes": [_I] * 9,
+    "lb_window_attn_bwd_ws_bytes": [_I] * 10,
     "lb_rope_axes": [_P] * 6 + [_I] * 6 + [_P, _L, _L, _I, _P],
     "lb_qk_norm_rope": [_P] * 9 + [_P] + [_I] * 7 + [_P, _L, _L, _F, _P],
     "lb_qk_norm_rope_bwd_ctas": [_I] * 5,

@@ -35,3 +35,21 @@ def test_rows_past_30_bits_are_refused(H, monkeypatch):
     monkeypatch.setattr(torch.Tensor, "contiguous", lambda t, *a, **kw: t)      # (one number stands for all of them)
     with pytest.raises(ValueError, match="columns"):
         OF.scaled_embedding(torch.zeros(1, dtype=torch.long), torch.zeros(1, 1).expand(1, H))
+
+
+# ---- the windowed backward's workspace -------------------------------------------------------------
+
+
+def _window_bytes(B, S, hq, hkv, d, window, sinks, masked, Sq=None, causal=True):
+    """(bytes of the workspace, of the row statistics and dQ's sums in it)."""
+    Sq = S if Sq is None else Sq
+    rows = B * hq * -(-Sq // 128) * 128
+    return _library().lb_window_attn_bwd_ws_bytes(B, Sq, S, hq, hkv, d, int(causal), window, sinks, int(masked)), 4 * rows * (2 + (-(-d // 32) * 32 if S > 128 else 0))
+
+
+def test_workspace_of_a_mask_is_its_own():
+    """Packed documents do not pay for the pieces of a call without a mask, whose sinks are seen by all queries."""
+    size, fixed = _window_bytes(4, 8192, 32, 32, 128, 256, 4096, masked=True)
+    assert size - fixed < 1 << 29
+    size, fixed = _window_bytes(4, 8192, 32, 8, 128, 128, 4096, masked=True)
+    assert size - fixed < 1 << 28
