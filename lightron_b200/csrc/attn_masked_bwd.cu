@@ -16,10 +16,10 @@
 // What bounds it.  d 64: a block takes 2890 cycles, most of them the math warps' (tensor pipe 44 %, exponentials 36 % of the active cycles), and a CTA's fixed part is some 6 blocks, a fifth
 // of a walk of documents of 300 tokens.  d 128: 4300 cycles, the chain dS - dK, dQ - drain - dP; with a cap the math warps again (5100; tensor pipe 50 %).  All kernels, us: 8 x 2048, 32 / 4 heads, d 64
 // causal 505, bias 525, cap 660, documents of 300 288; 1 x 8192, 32 / 8 heads, d 128 causal 1400 to 1450, bias 1340 to 1390, cap 1605 to 1630.
-// Under a window a key block's walk is short, but a block of sinks is seen by all queries behind it: 256 query blocks instead of 38 at 1 x 8192, window 1024, 32 / 8 heads.  Walks are then cut into pieces
-// of a length that is chosen here and listed on the device, longest first, where the lengths are known (documents cut them); pieces of one block leave dK and dV in fp32 in places of their own, as parts
-// do.  Main kernel, whole / cut: that case, 4 sinks, d 128 647 / 385 to 400 us; 3 x 1531, window 333, 130 sinks, cap 30, 16 / 4 heads, d 96 128 / 74 to 82; 8 x 2048, window 512 over documents of 900,
-// 4 sinks, 32 / 4 heads, d 64 247 / 239 to 257 (documents leave little to cut).  What bounds it is what bounds the others, the block's chain and a CTA's fixed part.
+// Under a window a key block's walk is short, but a block of sinks is seen by all queries behind it: 256 query blocks instead of 38 at 1 x 8192, window 1024, 32 / 8 heads.  Where they would
+// leave the others waiting, walks are then cut into pieces of a length that is chosen here and listed on the device, longest first, where the lengths are known (documents cut them); pieces of one block
+// leave dK and dV in fp32 in places of their own, as parts do.  Main kernel, whole / cut: that case, 4 sinks, d 128 647 / 385 to 400 us; 3 x 1531, window 333, 130 sinks, cap 30, 16 / 4 heads, d 96
+// 128 / 74 to 82.  What bounds it is what bounds the others, the block's chain and a CTA's fixed part.
 // Warp roles (512 threads): warp 0 TMA producer, warp 1 MMA issuer + TMEM owner, warps 4-11 math, 12-15 dQ drain.
 // All waits are bounded; on expiry a status word is set and the CTA drains and frees its TMEM.
 #include <algorithm>
@@ -43,7 +43,7 @@ struct BwdParams {
   int4* items;
   int2* joined;
   int *n_items, *cut_blocks;     // {how many pieces, how many key blocks in several}, and those
-  int chunk, extra;              // longest piece wanted, pieces beyond one per key block that there is room for
+  int chunk, extra, sums;        // longest piece wanted, pieces beyond one per key block that there is room for, and pieces that leave sums
   int by_head;                   // all pieces of a head, then the next head's; else those of all heads together
   int acc_d;                     // columns of dq_acc: head_dim in whole pieces of 32
   MaTerms f;
@@ -128,7 +128,8 @@ __device__ __forceinline__ void count_ahead(int* count) {
 __device__ void list_pieces(const BwdParams& pp, int* count) {
   const MaParams& p = pp.w.f;
   constexpr int KEPT = 2048;                                   // walks that are looked up once
-  __shared__ int of_warps[32], kept[KEPT], n_cut;
+  __shared__ long long of_warps[32];
+  __shared__ int kept[KEPT], n_cut;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, rep = p.hq / p.hkv;
   const int n_nblk = (p.Sk + 127) / 128, n = p.B * n_nblk;
   auto walk_of = [&](int e) {
@@ -140,17 +141,17 @@ __device__ void list_pieces(const BwdParams& pp, int* count) {
   __syncthreads();
   auto walk = [&](int e) { return e < KEPT ? kept[e] : walk_of(e); };
   // of all threads; in `before`: of those before this one
-  auto sum_of = [&](int v, int& before) {
-    int run = v;
+  auto sum_of = [&](long long v, long long& before) {
+    long long run = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, run, o);
+      const long long x = __shfl_up_sync(0xffffffffu, run, o);
       if (lane >= o) run += x;
     }
     __syncthreads();
     if (lane == 31) of_warps[warp] = run;
     __syncthreads();
-    int all = 0, ahead = 0;
+    long long all = 0, ahead = 0;
     for (int w = 0; w < warps; w++) {
       if (w == warp) ahead = all;
       all += of_warps[w];
@@ -159,13 +160,18 @@ __device__ void list_pieces(const BwdParams& pp, int* count) {
     return all;
   };
   const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x, a = min(n, (int)threadIdx.x * per), end = min(n, a + per);
-  // pieces twice as long until there is room for all
-  int length = pp.chunk, beyond = 0, before;
+  // pieces twice as long until there is room for all, and for the sums that they leave
+  int length = pp.chunk, beyond = 0;
+  long long ahead;
   for (;; length *= 2) {
-    int more = 0;
-    for (int e = a; e < end; e++) more += max((walk(e) + length - 1) / length - 1, 0);
-    beyond = sum_of(more, before);
-    if (beyond <= pp.extra) break;
+    long long more = 0;                                        // pieces beyond one per walk; walks in several, 32 bits up
+    for (int e = a; e < end; e++) {
+      const int of_walk = max((walk(e) + length - 1) / length - 1, 0);
+      more += of_walk + (of_walk ? 1LL << 32 : 0);
+    }
+    const long long all = sum_of(more, ahead);
+    beyond = (int)all;
+    if (beyond <= pp.extra && beyond + (all >> 32) <= pp.sums) break;
   }
   auto cut = [&](int e, int& its, int& pieces, int& share) {
     its = walk(e);
@@ -184,7 +190,8 @@ __device__ void list_pieces(const BwdParams& pp, int* count) {
     }
     atomicAdd(&count[bucket(its - (pieces - 1) * share) + 1], 1);
   }
-  sum_of(sums, before);
+  sum_of(sums, ahead);
+  int before = (int)ahead;                                     // places of the sums
   count_ahead(count);
   __syncthreads();
   for (int e = a; e < end; e++) {
@@ -893,11 +900,22 @@ int parts_of(int B, int Sq, int Sk, int hq, int hkv, int causal, int sms) {
   return best;
 }
 
-// Under a window: the longest piece of a walk, and how many pieces there may be beyond one per key block.  By the model of parts_of(), for keys that queries near them see and for blocks of sinks,
-// which all queries behind them see; where the mask comes from the device documents cut the walks shorter, and there are more, shorter ones of sinks: then pieces may get twice as long.
-// Without a mask, and with two CTAs for each SM or more, pieces go head by head and none is longer than the walk of other keys: 148 CTAs then work on two heads or three, whose Q, dO and dQ's sums stay in L2 (1 x 8192,
-// window 1024, 4 sinks, 32 / 8 heads, d 128, longest of all heads first / head by head: 912 / 472 MB of DRAM, the kernel 400 / 381 us; 3 x 1531, window 333, 130 sinks, one wave of CTAs: all kernels 168 / 190).
-struct Pieces { int length, extra; bool by_head; };
+long long stats_floats(const MaParams& p) { return (long long)p.B * p.hq * ((p.Sq + 127) / 128) * 256; }
+int acc_columns(int d) { return (d + 31) / 32 * 32; }
+long long dq_floats(const MaParams& p) { return p.Sk <= 128 ? 0 : stats_floats(p) / 2 * acc_columns(p.d); }
+
+// Under a window: the longest piece of a walk, how many pieces there may be beyond one per key block, and how many leave sums (of one kv head).  By the model of parts_of(), for keys that queries near
+// them see and for blocks of sinks, which all queries behind them see.  Without a mask that is what the walks are at most; documents cut them shorter, and make more, shorter ones of sinks: then there is
+// room for more pieces, and where it does not do the list makes them twice as long.  What pieces leave takes no more memory than dQ's sums, or 64 MB.  Without pieces there is no list; key blocks are
+// sorted then by their walks where these differ.
+// Without a mask, with several kv heads and two CTAs for each SM or more, the order may be head by head: 148 CTAs then work on two heads or three, whose Q, dO and dQ's sums stay in L2, which is worth a
+// twentieth of the time; but a walk that is longer than the others then begins in the last head, too, and ends behind them.
+// The whole backward, us, longest of all heads first / head by head, for the longest piece that is taken (the first one) and others; 32 / 8 heads, d 128: 1 x 8192, window 1024, 4 sinks, of 36 query blocks
+// 484 / 468, of 128 484 / 679, whole 796 / 948; window 128, 150 sinks, of 64 293 / 373, of 8 356 / 308, whole 723 / 777; 1024 sinks, of 128 482 / 591, of 64 499 / 516, of 8 745 / 589, whole 701 / 758;
+// 1 x 16384, window 256, 2048 sinks, whole 1665 / 2040, of 64 1784 / 1643, of 12 2532 / 1992; 4 x 8192, window 128, 4096 sinks, whole 4796 / 4705, of 8 7818 / 6290; 32 / 32 heads: 32 x 2048, window 512,
+// 4 sinks, whole 3369 / 3030, of 5 3362 / 3401.  With a mask, whole and sorted / in the pieces that were taken for no mask: 8 x 2048, window 512, 4 sinks, 32 / 4 heads, d 64, documents of 900 330 / 340,
+// of 300 295 / 306; in pieces where one sequence has few: 1 x 8192, window 1024, 4 sinks, 32 / 8 heads, d 128, one document 493, whole 740, documents of 3000 473, whole 672.
+struct Pieces { int length, extra, sums; bool by_head, sorted; };
 Pieces pieces_of(const MaParams& p, bool masked, int sms) {
   const int n_mblocks = (p.Sq + 127) / 128, n_nblk = (p.Sk + 127) / 128, rep = p.hq / p.hkv;
   const long long pairs = (long long)p.hkv * p.B, span = 128 + (p.causal ? 1LL : 2LL) * (p.window - 1LL);
@@ -905,22 +923,29 @@ Pieces pieces_of(const MaParams& p, bool masked, int sms) {
   const long long most = (span + 127) / 128 + ((p.Sk - p.Sq) % 128 || !p.causal ? 1 : 0);
   const long long near = std::min<long long>(most, n_mblocks) * rep, far = (long long)n_mblocks * rep;
   const long long n_far = std::min<long long>((p.sinks + 127) / 128, n_nblk), n_near = n_nblk - n_far;
-  const bool by_head = !masked && n_nblk * pairs >= 2LL * sms;
+  const long long room = std::max(dq_floats(p), 1LL << 24) / (2LL * p.hkv * 128 * (p.d <= 64 ? 64 : 128));      // pieces that leave sums
+  const bool heads = !masked && p.hkv > 1 && n_nblk * pairs >= 2LL * sms;
   double best_time = 0.0;
-  Pieces best{(int)far, 0, by_head};
+  Pieces best{(int)far, 0, 0, false, false};
+  if (p.Sk <= 128) return best;
   auto look = [&](long long length) {
     const long long a = (near + length - 1) / length, b = (far + length - 1) / length;
-    const long long extra = n_near * (a - 1) + n_far * (b - 1);
+    long long extra = (n_near * (a - 1) + n_far * (b - 1)) * p.B, sums = extra + ((a > 1 ? n_near : 0) + (b > 1 ? n_far : 0)) * p.B;
+    if (sums > room) return;
     const double work = (double)(n_near * (near + a * (a > 1 ? 9 : 6)) + n_far * (far + b * (b > 1 ? 9 : 6))) * pairs / sms;
-    const double time = std::max(std::max((near + a - 1) / a, n_far ? (far + b - 1) / b : 0) + 9.0, 1.1 * work) + (extra ? 1.0 : 0.0);
-    if (best_time == 0.0 || time < best_time) {
-      best_time = time;
-      best = Pieces{(int)length, (int)std::min<long long>((2 * extra + (p.sinks ? 4 : 0)) * p.B, 1 << 24), by_head};
+    const double other = (double)((near + a - 1) / a), longest = std::max(other, n_far ? (double)((far + b - 1) / b) : 0.0);
+    const double together = std::max(longest + 9.0, 1.1 * work), apart = 1.045 * work + longest - other, time = (heads ? std::min(together, apart) : together) + (extra ? 1.0 : 0.0);
+    if (best_time != 0.0 && time >= best_time) return;
+    best_time = time;
+    if (masked && extra) {
+      extra = std::min(2 * extra + (p.sinks ? 4LL * p.B : 0), room / 2);
+      sums = extra + std::min(extra, (long long)p.B * n_nblk);
     }
+    best = Pieces{(int)length, (int)std::min(extra, 1LL << 24), (int)std::min(sums, 1LL << 25), heads && apart < together, false};
   };
-  for (long long parts = 1; parts <= std::min<long long>(far, 64); parts++)
-    if (!by_head || (far + parts - 1) / parts <= near) look((far + parts - 1) / parts);
+  for (long long parts = 1; parts <= std::min<long long>(far, 64); parts++) look((far + parts - 1) / parts);
   for (long long parts = 1; parts <= std::min<long long>(near, 32); parts++) look((near + parts - 1) / parts);
+  best.sorted = masked || (n_far > 0 && n_near > 0 && far > near && !best.by_head);
   return best;
 }
 
@@ -955,27 +980,21 @@ int launch_bwd(BwdParams& p, cudaStream_t s) {
   return LB_OK;
 }
 
-// Bytes of the workspace: row statistics, fp32 dQ (up to 128 keys: none), fp32 dK and dV of the parts, the order of the key blocks.
-long long stats_floats(const MaParams& p) { return (long long)p.B * p.hq * ((p.Sq + 127) / 128) * 256; }
-int acc_columns(int d) { return (d + 31) / 32 * 32; }
-long long dq_floats(const MaParams& p) { return p.Sk <= 128 ? 0 : stats_floats(p) / 2 * acc_columns(p.d); }
 long long part_floats(const MaParams& p, int parts) {
   return parts > 1 ? (long long)p.B * p.hkv * ((p.Sk + 127) / 128) * parts * 128 * (p.d <= 64 ? 64 : 128) : 0;
 }
-
-// (pieces that leave sums: two for each one beyond the first of its key block, at most)
-long long piece_floats(const MaParams& p, const Pieces& c) { return 2LL * c.extra * p.hkv * 128 * (p.d <= 64 ? 64 : 128); }
-// (without a mask and with nothing to cut, the key blocks' order is known)
-bool listed(const MaParams& p, const Pieces& c) { return p.window > 0 && p.Sk > 128 && (c.extra > 0 || p.qb); }
+long long piece_floats(const MaParams& p, const Pieces& c) { return (long long)c.sums * p.hkv * 128 * (p.d <= 64 ? 64 : 128); }
 
 }  // namespace
 
+// Bytes of the workspace: row statistics, fp32 dQ (up to 128 keys: none), fp32 dK and dV of parts or pieces, the order of the key blocks or the list of the pieces.
 long long ma_bwd_ws_bytes(const MaParams& p, bool masked) {
+  const long long all = stats_floats(p) + dq_floats(p);
   if (p.window > 0) {
     const Pieces c = pieces_of(p, masked, lb_num_sms());
-    return (stats_floats(p) + dq_floats(p) + 2 * piece_floats(p, c) + 4 * (order_ints(p) + c.extra) + 3 * order_ints(p) + 4) * (long long)sizeof(float);
+    return (all + (c.extra ? 2 * piece_floats(p, c) + 4 * (order_ints(p) + c.extra) + 3 * order_ints(p) + 4 : order_ints(p))) * (long long)sizeof(float);
   }
-  return (stats_floats(p) + dq_floats(p) + 2 * part_floats(p, parts_of(p.B, p.Sq, p.Sk, p.hq, p.hkv, p.causal, lb_num_sms())) + order_ints(p)) * (long long)sizeof(float);
+  return (all + 2 * part_floats(p, parts_of(p.B, p.Sq, p.Sk, p.hq, p.hkv, p.causal, lb_num_sms())) + order_ints(p)) * (long long)sizeof(float);
 }
 
 int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s) {
@@ -988,12 +1007,13 @@ int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s) {
   p.dk_acc = p.dq_acc + dq_floats(a);
   p.f.set(a, false, twice);
   p.scale2 = twice(a.scale);
-  const Pieces c = a.window > 0 ? pieces_of(a, a.qb != nullptr, lb_num_sms()) : Pieces{0, 0, false};
+  const Pieces c = a.window > 0 ? pieces_of(a, a.qb != nullptr, lb_num_sms()) : Pieces{};
   p.parts = 1;
   p.order = nullptr;
-  if (listed(a, c)) {
+  if (c.extra) {
     p.chunk = c.length;
     p.extra = c.extra;
+    p.sums = c.sums;
     p.by_head = c.by_head;
     p.dv_acc = p.dk_acc + piece_floats(a, c);
     p.items = reinterpret_cast<int4*>(p.dv_acc + piece_floats(a, c));
@@ -1004,7 +1024,7 @@ int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s) {
   }
   if (!a.window) p.parts = parts_of(a.B, a.Sq, a.Sk, a.hq, a.hkv, a.causal, lb_num_sms());
   p.dv_acc = p.dk_acc + part_floats(a, p.parts);
-  p.order = a.kb && p.parts == 1 && a.Sk > 128 ? reinterpret_cast<int*>(p.dv_acc + part_floats(a, p.parts)) : nullptr;
+  p.order = (a.window > 0 ? c.sorted : a.kb && p.parts == 1) && a.Sk > 128 ? reinterpret_cast<int*>(p.dv_acc + part_floats(a, p.parts)) : nullptr;
   return a.d <= 64 ? launch_bwd<64>(p, s) : launch_bwd<128>(p, s);
 }
 

@@ -53,3 +53,40 @@ def test_workspace_of_a_mask_is_its_own():
     assert size - fixed < 1 << 29
     size, fixed = _window_bytes(4, 8192, 32, 8, 128, 128, 4096, masked=True)
     assert size - fixed < 1 << 28
+
+
+@pytest.mark.parametrize("B,S,hq,hkv,d,window,sinks", [
+    (4, 8192, 32, 32, 128, 256, 4096), (1, 32768, 32, 8, 128, 512, 4096), (1, 65536, 32, 8, 128, 128, 4096), (1, 131072, 32, 8, 128, 128, 8192), (4, 8192, 32, 8, 128, 128, 4096),
+    (8, 8192, 32, 8, 128, 1024, 1024), (1, 8192, 32, 8, 128, 128, 1024), (32, 2048, 32, 32, 128, 512, 4), (1024, 256, 32, 32, 128, 64, 4), (1, 131072, 32, 8, 128, 4096, 4096),
+    (3, 130000, 1, 1, 8, 5, 2), (1, 2000, 16, 1, 64, 40, 300), (1, 500, 4, 2, 64, 130, 130), (2, 129, 1, 1, 8, 1, 1), (7, 128, 4, 4, 64, 5, 1), (5, 1, 4, 4, 64, 1, 0),
+])
+@pytest.mark.parametrize("masked,causal", [(False, True), (True, True), (False, False), (True, False)])
+def test_workspace_of_pieces_has_a_bound(B, S, hq, hkv, d, window, sinks, masked, causal):
+    """What pieces of walks leave, for dK and dV together, takes no more than dQ's sums or 64 MB, however many sinks there are; the list itself 28 bytes a key block and 16 a piece."""
+    size, fixed = _window_bytes(B, S, hq, hkv, d, window, sinks, masked, causal=causal)
+    blocks = B * -(-S // 128)
+    most = max(fixed, 1 << 26)
+    assert 0 <= size - fixed <= most + 28 * blocks + 16 * (most // (2 * 4 * 128 * 64 * hkv) + 1) + 16
+
+
+def test_workspace_without_a_mask_is_what_is_used():
+    """1 x 8192 with a window of 1024 and four sinks: the sinks' walk of 256 blocks in eight pieces of each of 8 heads, nothing else."""
+    size, fixed = _window_bytes(1, 8192, 32, 8, 128, 1024, 4, masked=False)
+    assert size - fixed == 2 * 8 * 8 * 128 * 128 * 4 + 16 * (64 + 7) + 12 * 64 + 16
+
+
+def test_walks_are_no_longer_than_the_plan_of_the_pieces_takes_them_for():
+    """Query blocks that see a key block, counted, against the bound that sizes lists without a mask: blocks of sinks may be seen by all, others by the window's span."""
+    for Sq, Sk, window, sinks, causal in [(700, 700, 1, 0, True), (700, 700, 130, 4, True), (700, 700, 129, 200, True), (600, 700, 64, 3, True), (601, 900, 257, 0, True), (700, 700, 130, 4, False),
+                                          (640, 640, 1, 0, False), (500, 900, 300, 129, False), (129, 1000, 128, 1, True)]:
+        off = Sk - Sq
+        at, key = torch.arange(Sq)[:, None] + off, torch.arange(Sk)[None]
+        see = ((at - key).abs() < window) | (key < sinks)
+        if causal:
+            see &= key <= at
+        span = 128 + (1 if causal else 2) * (window - 1)
+        near = min(-(-span // 128) + (1 if off % 128 or not causal else 0), -(-Sq // 128))
+        for n0 in range(0, Sk, 128):
+            rows = see[:, n0:n0 + 128].any(1).nonzero()
+            walk = 0 if not len(rows) else int(rows[-1]) // 128 - int(rows[0]) // 128 + 1
+            assert walk <= (-(-Sq // 128) if n0 < sinks else near)
