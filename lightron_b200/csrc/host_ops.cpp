@@ -1055,7 +1055,7 @@ PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
   }
   if (a[6] != Py_None) {
-    if (!sized(pos, *q, at::kInt)) LB_NOT_PLAIN;
+    if (!sized(pos, *q, at::kInt) || pos->dim() == 0) LB_NOT_PLAIN;
     const bool by_axis = !one && pos->dim() > 1;
     if (by_axis && pos->size(0) < r.axes.n) LB_NOT_PLAIN;
     if (pos->dim() == 1 ? pos->size(0) != S : one ? !pos->sizes().equals({B, S}) : !(pos->sizes().equals({pos->size(0), S}) || pos->sizes().equals({pos->size(0), B, S}))) LB_NOT_PLAIN;
