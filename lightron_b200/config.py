@@ -89,6 +89,17 @@ class ModelArgs:
         """Window of a layer's attention, or None: it sees all keys."""
         return None if self.attn_global_freq and (layer_id + 1) % self.attn_global_freq == 0 else self.attn_window
 
+    def flops_per_token(self, seq_length: int) -> float:
+        """Operations of a training step per token, forward and backward: 6 for each parameter that a token visits, and 12 * dim for each key that a position sees in the mean, layer by layer:
+        half of the sequence, or under a window what the window and the sinks leave of it."""
+        def visible(window) -> float:
+            if window is None or window >= seq_length:
+                return seq_length / 2
+            hidden = seq_length - window                      # positions that do not see their first key, and how many keys the last of them does not see
+            shown = min(self.attn_sinks, hidden)              # of those, by the sinks
+            return (window * (window + 1) / 2 + hidden * window + shown * (shown + 1) / 2 + (hidden - shown) * shown) / seq_length
+        return 6.0 * self.num_active_params() + 12.0 * self.dim * sum(visible(self.window_of(i)) for i in range(self.n_layers))
+
     @property
     def head_dim(self) -> int:
         return self.dim // self.n_heads

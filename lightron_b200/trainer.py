@@ -263,10 +263,8 @@ class Trainer:
                 if is_log:
                     tps_wall = (self.tokens_seen - tokens0) / max(time.time() - start, 1e-9)
                     tps_dev = tokens_per_step / (ms / 1e3) if ms > 0 else float("nan")
-                    # model FLOPs: 6 N per token for the matmuls + causal attention (fwd + bwd)
-                    a = self.args
-                    flops_tok = 6.0 * a.num_active_params() + 6.0 * a.n_layers * a.dim * t.seq_length
-                    mfu = flops_tok * tps_dev / (ctx.world_size * self.peak_flops) if ms > 0 else float("nan")
+                    # model FLOPs: 6 N per token for the matmuls + causal attention under the layers' windows (fwd + bwd)
+                    mfu = self.args.flops_per_token(t.seq_length) * tps_dev / (ctx.world_size * self.peak_flops) if ms > 0 else float("nan")
                     print(f"Step {self.step}/{t.total_steps} | Loss: {last_loss:.4f} | TPS: {tps_wall:.2f} tokens/s"
                           f" | device TPS: {tps_dev:.2f} | step {ms:.2f} ms | MFU {mfu * 100:.1f}%", flush=True)
                     if log_f:

@@ -90,3 +90,41 @@ def test_walks_are_no_longer_than_the_plan_of_the_pieces_takes_them_for():
             rows = see[:, n0:n0 + 128].any(1).nonzero()
             walk = 0 if not len(rows) else int(rows[-1]) // 128 - int(rows[0]) // 128 + 1
             assert walk <= (-(-Sq // 128) if n0 < sinks else near)
+
+
+# ---- figures of a run ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("S,window,sinks,freq", [(64, 16, 0, 0), (64, 16, 3, 2), (64, 16, 60, 0), (64, 1, 5, 3), (64, 64, 2, 0), (64, 200, 0, 0), (50, 49, 1, 0), (64, None, 0, 0)])
+def test_operations_of_a_step_count_visible_keys(S, window, sinks, freq):
+    from lightron_b200.config import ModelArgs
+    args = ModelArgs(dim=32, n_heads=4, n_layers=4, vocab_size=64, attn_window=window, attn_sinks=sinks, attn_global_freq=freq)
+    keys = 0.0
+    for layer in range(4):
+        w = args.window_of(layer)
+        if w is None or w >= S:
+            keys += S / 2
+        else:
+            keys += sum(1 for i in range(S) for j in range(i + 1) if i - j < w or j < sinks) / S
+    assert args.flops_per_token(S) == pytest.approx(6.0 * args.num_active_params() + 12.0 * 32 * keys, rel=1e-12)
+    if window is None:
+        assert args.flops_per_token(S) == 6.0 * args.num_active_params() + 6.0 * 4 * 32 * S
+
+
+def test_logged_mfu_counts_the_window(tmp_path):
+    import json
+    from lightron_b200 import mesh
+    from lightron_b200.config import parse_config
+    from lightron_b200.trainer import Trainer
+    mesh.set_context(None)
+    log = tmp_path / "run.jsonl"
+    raw = {"distributed": {}, "model": {"name": "tiny", "attn_window": 16, "attn_sinks": 2, "attn_global_freq": 4}, "dataset": {"name": "synthetic"},
+           "training": {"micro_batch_size": 1, "gradient_accumulation_steps": 1, "seq_length": 128, "learning_rate": 3e-4, "total_steps": 1, "seed": 0, "dtype": "fp32", "log_interval": 1,
+                        "jsonl_log": str(log), "save_interval": 0, "save_final": False}}
+    tr = Trainer(parse_config(raw, env={}))
+    tr.fit()
+    mesh.set_context(None)
+    row = json.loads(log.read_text().splitlines()[-1])
+    keys = 64 + 3 * sum(1 for i in range(128) for j in range(i + 1) if i - j < 16 or j < 2) / 128
+    want = (6.0 * tr.args.num_active_params() + 12.0 * tr.args.dim * keys) * row["tokens_per_s_device"] / (row["mfu_peak_tflops"] * 1e12)
+    assert row["mfu"] == pytest.approx(want, rel=1e-9)
