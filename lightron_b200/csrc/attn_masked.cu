@@ -128,12 +128,20 @@ int fill(MaParams& p, const void* q, const void* k, const void* v, void* o, void
   return bad_strides(p.qs) || bad_strides(p.ks) || bad_strides(p.vs) ? LB_ERR_SHAPE : LB_OK;
 }
 
-// A window over all keys is none.  (Sums of a place and the window have to stay in 32 bits.)
-int set_window(MaParams& p, int window, int sinks) {
+// Whether the forward takes a window over all keys as one of their number, which has the heads of a group as a tile's rows, instead of as none: where heads fill the SMs by themselves, or the cache is
+// long.  One key short of all / as none, us, hq / hkv, d 128, one query: 8 sequences of 32 / 8 heads, 256 keys 14 / 16, 4096 43 / 88, 65536 352 / 1182; one sequence, 1024 keys 25 / 25, 4096 27 / 39; 32 of
+// 16 / 1, 4096 keys 33 / 166; 64 queries, 8 sequences of 32 / 8, 4096 keys 70 / 90; left as none: one sequence of 16 / 1, 512 keys 20 / 18; 64 queries over 16384 70 / 53; 100 queries, 8 sequences of 32 / 8,
+// 4096 keys 92 / 90.
+bool rows_of_heads(const MaParams& p) {
+  const int shift = ma_group_shift(p);
+  return shift > 0 && p.Sq <= 64 && ((long long)p.hq * p.B >= lb_num_sms() || (p.Sq << shift <= 128 && p.Sk >= 2048));
+}
+// A window over all keys is none, but for that.  (Sums of a place and the window have to stay in 32 bits.)
+int set_window(MaParams& p, int window, int sinks, bool forward) {
   if (window <= 0 || sinks < 0) return LB_ERR_ARG;
   if (p.Sk > (1 << 29)) return LB_ERR_SHAPE;
-  p.window = window < p.Sk ? window : 0;
-  p.sinks = !p.window ? 0 : sinks < p.Sk ? sinks : p.Sk;
+  p.window = window < p.Sk ? window : forward && rows_of_heads(p) ? p.Sk : 0;
+  p.sinks = !p.window || p.window == p.Sk ? 0 : sinks < p.Sk ? sinks : p.Sk;
   return LB_OK;
 }
 
@@ -191,14 +199,14 @@ extern "C" long long lb_window_attn_fwd_ws_bytes(int B, int Sq, int Sk, int hq, 
   MaParams p{};
   if (check_sizes(B, Sq, Sk, hq, hkv, d)) return 0;
   p.B = B; p.Sq = Sq; p.Sk = Sk; p.hq = hq; p.hkv = hkv; p.d = d; p.causal = causal;
-  return set_window(p, window, sinks) ? 0 : ma_fwd_ws_bytes(p);
+  return set_window(p, window, sinks, true) ? 0 : ma_fwd_ws_bytes(p);
 }
 extern "C" int lb_window_attn_fwd(const void* q, const void* k, const void* v, void* o, void* o_lo, void* lse, void* ws, long long ws_bytes, int B, int Sq, int Sk, int hq, int hkv,
                                   int d, const long long* strides, float scale, int causal, float softcap, const void* slopes, const void* q_bounds, const void* k_bounds, int window, int sinks,
                                   void* stream) {
   MaParams p;
   if (const int rc = fill(p, q, k, v, o, o_lo, lse, B, Sq, Sk, hq, hkv, d, strides, scale, causal, softcap, slopes, q_bounds, k_bounds)) return rc;
-  if (const int rc = set_window(p, window, sinks)) return rc;
+  if (const int rc = set_window(p, window, sinks, true)) return rc;
   if (misaligned(ws)) return LB_ERR_ARG;
   return (p.window ? ma_launch_window_fwd : ma_launch_fwd)(p, ws, ws ? ws_bytes : 0, (cudaStream_t)stream);
 }
@@ -218,7 +226,7 @@ int backward(const void* q, const void* k, const void* v, const void* o, const v
   MaBwdParams w;
   if (const int rc = fill(w.f, q, k, v, const_cast<void*>(o), const_cast<void*>(o_lo), const_cast<void*>(lse), B, Sq, Sk, hq, hkv, d, strides, scale, causal, softcap, slopes, q_bounds, k_bounds)) return rc;
   if (windowed)
-    if (const int rc = set_window(w.f, window, sinks)) return rc;
+    if (const int rc = set_window(w.f, window, sinks, false)) return rc;
   if (!o_lo || !dout || !ws || !dq || !dk || !dv || misaligned(dout) || misaligned(ws) || misaligned(dq) || misaligned(dk) || misaligned(dv)) return LB_ERR_ARG;
   if (ws_bytes < ma_bwd_ws_bytes(w.f, w.f.qb != nullptr)) return LB_ERR_CAPACITY;
   w.dout = (const bf16*)dout; w.dq = (bf16*)dq; w.dk = (bf16*)dk; w.dv = (bf16*)dv; w.stats = (float*)ws;
@@ -240,7 +248,7 @@ extern "C" long long lb_window_attn_bwd_ws_bytes(int B, int Sq, int Sk, int hq, 
   MaParams p{};
   if (check_sizes(B, Sq, Sk, hq, hkv, d)) return 0;
   p.B = B; p.Sq = Sq; p.Sk = Sk; p.hq = hq; p.hkv = hkv; p.d = d; p.causal = causal;
-  return set_window(p, window, sinks) ? 0 : ma_bwd_ws_bytes(p, masked != 0);
+  return set_window(p, window, sinks, false) ? 0 : ma_bwd_ws_bytes(p, masked != 0);
 }
 extern "C" int lb_window_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_lo, const void* dout, const void* lse, void* ws, long long ws_bytes,
                                   void* dq, void* dk, void* dv, int B, int Sq, int Sk, int hq, int hkv, int d, const long long* strides, float scale, int causal, float softcap,

@@ -26,6 +26,14 @@ struct MaParams {
   int window, sinks;             // 0: no window; else of those keys the ones less than `window` positions away, and the first `sinks` (both up to Sk)
 };
 
+// The heads of a group as a power of two, where there are few queries: such calls may have them as a tile's rows.
+inline int ma_group_shift(const MaParams& p) {
+  const int rep = p.hq / p.hkv;
+  int shift = 0;
+  while ((1 << shift) < rep) shift++;
+  return p.Sq < 128 && shift <= 5 && (1 << shift) == rep ? shift : 0;
+}
+
 struct MaBwdParams {
   MaParams f;
   const bf16* dout;

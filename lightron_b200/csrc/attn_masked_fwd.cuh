@@ -831,13 +831,8 @@ __global__ void ma_join_kernel(const __grid_constant__ FwdParams pp) {
 // CTAs of a tile: one where there is a tile for each SM, else as many as find room (two per SM), with four key blocks or more each.  Whole / split, us, causal: 8192 queries and keys, 1 head,
 // d 64 97 / 45; 2 heads, d 128, cap 121 / 74; 4 x 4096 of 4 heads, d 128, cap 68 / 46; 2048, 4 heads, d 64 27 / 22; one query, 32 / 8 heads, d 128, 8192 keys 118 / 37, 4 x 32768 keys
 // 557 / 296; left whole 1024, 8 heads, d 128 19.7 / 20.4 and 2 x 1024, 8 heads, d 64 19.5 / 19.2.  (Where the mask comes from the device the length of the walks is not known here: that of all keys is taken.)
-// Rows of a query under a window, as a power of two: the heads of its group, where there are few queries.
-int shift_of(const MaParams& p) {
-  const int rep = p.hq / p.hkv;
-  int shift = 0;
-  while ((1 << shift) < rep) shift++;
-  return p.window && p.Sq < 128 && shift <= 5 && (1 << shift) == rep ? shift : 0;
-}
+// Rows of a query, as a power of two: under a window the heads of its group, where there are few queries.
+int shift_of(const MaParams& p) { return p.window ? ma_group_shift(p) : 0; }
 int tiles_of(const MaParams& p) { return (int)((((long long)p.Sq << shift_of(p)) + 127) / 128); }      // of the heads of a group, or of one
 int splits_of(const MaParams& p, int sms) {
   const long long tiles = (long long)tiles_of(p) * (p.hq >> shift_of(p)) * p.B;

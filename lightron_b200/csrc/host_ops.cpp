@@ -982,7 +982,7 @@ PyObject* py_masked_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       LB_NOT_PLAIN;
     }
     if (window < 1 || sinks < 0 || Sk > MAX_WINDOW_LENGTH) LB_NOT_PLAIN;
-    if (window >= Sk) window = sinks = 0;          // all keys
+    window = std::min(window, Sk);
     sinks = std::min(sinks, Sk);
   } else if (!PyLong_CheckExact(a[10]) || PyLong_AsLongLong(a[10]) != 0) {
     PyErr_Clear();

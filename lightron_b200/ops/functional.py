@@ -910,7 +910,7 @@ def _check_masked(q, k, v, mask, causal, scale, softcap, slopes) -> bool:
 
 
 def _check_window(window: Optional[int], sinks: int, length: int) -> Tuple[int, int]:
-    """Refuses what is no window; returns it with its sinks as the kernels take them: 0 for none, or one over all keys."""
+    """Refuses what is no window; returns it with its sinks as the kernels take them: 0 for none, or one over more keys than they count."""
     for name, n in (("window", window), ("sinks", sinks)):
         if n is not None and (not isinstance(n, int) or isinstance(n, bool)):
             raise ValueError(f"{name} must be a whole number, got {n!r}")
@@ -918,7 +918,7 @@ def _check_window(window: Optional[int], sinks: int, length: int) -> Tuple[int, 
         raise ValueError(f"window must be None or at least 1 and sinks at least 0, got {window} and {sinks}")
     if window is None and sinks:
         raise ValueError(f"{sinks} sinks have a meaning under a window only")
-    return (0, 0) if window is None or window >= length else (window, min(sinks, length))
+    return (0, 0) if window is None or window >= length > MAX_WINDOW_LENGTH else (min(window, length), min(sinks, length))
 
 
 MAX_WINDOW_LENGTH = 1 << 29

@@ -128,3 +128,19 @@ def test_logged_mfu_counts_the_window(tmp_path):
     keys = 64 + 3 * sum(1 for i in range(128) for j in range(i + 1) if i - j < 16 or j < 2) / 128
     want = (6.0 * tr.args.num_active_params() + 12.0 * tr.args.dim * keys) * row["tokens_per_s_device"] / (row["mfu_peak_tflops"] * 1e12)
     assert row["mfu"] == pytest.approx(want, rel=1e-9)
+
+
+@pytest.mark.parametrize("B,hq,hkv,d", [(8, 32, 8, 128), (8, 32, 8, 64), (1, 32, 4, 128)])
+@pytest.mark.parametrize("S", [2048, 4095, 4096, 20000])
+def test_single_tokens_are_split_alike_where_the_cache_fills_the_window(B, hq, hkv, d, S):
+    """The heads of a group as a tile's rows, and walks split over keys, for a window of all keys as for one that is a key short of them."""
+    lib = _library()
+    size = [lib.lb_window_attn_fwd_ws_bytes(B, 1, S, hq, hkv, d, 1, window, 0) for window in (S - 1, S, S + 1, 1 << 30)]
+    assert size[0] > 0 and size == size[:1] * 4
+
+
+def test_many_queries_take_a_window_over_all_keys_as_none():
+    lib = _library()
+    for S, Sq in ((700, 700), (9000, 300), (20000, 128), (40000, 100)):
+        assert lib.lb_window_attn_fwd_ws_bytes(1, Sq, S, 8, 2, 64, 1, S, 3) == lib.lb_masked_attn_fwd_ws_bytes(1, Sq, S, 8, 2, 64)
+        assert lib.lb_window_attn_bwd_ws_bytes(1, Sq, S, 8, 2, 64, 1, S, 3, 0) == lib.lb_masked_attn_bwd_ws_bytes(1, Sq, S, 8, 2, 64, 1)
