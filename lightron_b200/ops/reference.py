@@ -183,7 +183,10 @@ def scaled_embedding(tokens: torch.Tensor, w: torch.Tensor, scale: float, vocab_
     away = (local < 0) | (local >= w.shape[0])
     if w.shape[0] == 0:
         return w.new_zeros(*tokens.shape, w.shape[1])
-    return (F.embedding(local.masked_fill(away, 0), w.to(dt)) * scale).masked_fill(away.unsqueeze(-1), 0.0).type_as(w)
+    local = local.masked_fill(away, 0)
+    # (the gradient is summed up in the type that rows are gathered in; without one only the rows are cast)
+    rows = F.embedding(local, w.to(dt)) if w.requires_grad and torch.is_grad_enabled() else F.embedding(local, w).to(dt)
+    return (rows * scale).masked_fill(away.unsqueeze(-1), 0.0).type_as(w)
 
 
 def grad_sumsq(tensors) -> torch.Tensor:

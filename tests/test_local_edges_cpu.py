@@ -37,6 +37,21 @@ def test_rows_past_30_bits_are_refused(H, monkeypatch):
         OF.scaled_embedding(torch.zeros(1, dtype=torch.long), torch.zeros(1, 1).expand(1, H))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_rows_alone_are_cast_without_gradients(dtype, monkeypatch):
+    """The same values with and without a gradient, and no copy of the table in another type where none is asked for."""
+    from lightron_b200.ops import reference as ref
+    w = torch.randn(11, 6, generator=torch.Generator().manual_seed(1)).to(dtype).requires_grad_()
+    tokens = torch.tensor([[3, 4, 13], [2, 9, 3]])
+    want = OF.scaled_embedding(tokens, w, 1.7, 3)
+    gather, tables = ref.F.embedding, []
+    monkeypatch.setattr(ref.F, "embedding", lambda i, t: tables.append(t) or gather(i, t))
+    with torch.no_grad():
+        assert torch.equal(OF.scaled_embedding(tokens, w, 1.7, 3), want)
+    assert torch.equal(OF.scaled_embedding(tokens, w.detach(), 1.7, 3), want)
+    assert len(tables) == 2 and all(t.dtype == dtype and t.data_ptr() == w.data_ptr() for t in tables)
+
+
 # ---- the windowed backward's workspace -------------------------------------------------------------
 
 
