@@ -21,6 +21,7 @@
 // leave dK and dV in fp32 in places of their own, as parts do.  Main kernel, whole / cut: that case, 4 sinks, d 128 647 / 385 to 400 us; 3 x 1531, window 333, 130 sinks, cap 30, 16 / 4 heads, d 96
 // 128 / 74 to 82.  What bounds it is what bounds the others, the block's chain and a CTA's fixed part.
 // Warp roles (512 threads): warp 0 TMA producer, warp 1 MMA issuer + TMEM owner, warps 4-11 math, 12-15 dQ drain.
+// P^T and dS^T are rounded to bf16, the type of Q, K and dO, as operands of the tensor cores: 1.7e-3 of a gradient in the 2-norm beside the 1.7e-3 of its own rounding; all sums are fp32.
 // All waits are bounded; on expiry a status word is set and the CTA drains and frees its TMEM.
 #include <algorithm>
 #include <type_traits>
