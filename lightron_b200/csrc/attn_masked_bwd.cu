@@ -129,8 +129,7 @@ __device__ __forceinline__ void count_ahead(int* count) {
 __device__ void list_pieces(const BwdParams& pp, int* count) {
   const MaParams& p = pp.w.f;
   constexpr int KEPT = 2048;                                   // walks that are looked up once
-  __shared__ long long of_warps[32];
-  __shared__ int kept[KEPT], n_cut;
+  __shared__ int of_warps[32], kept[KEPT], n_cut;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, rep = p.hq / p.hkv;
   const int n_nblk = (p.Sk + 127) / 128, n = p.B * n_nblk;
   auto walk_of = [&](int e) {
@@ -142,17 +141,17 @@ __device__ void list_pieces(const BwdParams& pp, int* count) {
   __syncthreads();
   auto walk = [&](int e) { return e < KEPT ? kept[e] : walk_of(e); };
   // of all threads; in `before`: of those before this one
-  auto sum_of = [&](long long v, long long& before) {
-    long long run = v;
+  auto sum_of = [&](int v, int& before) {
+    int run = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, run, o);
+      const int x = __shfl_up_sync(0xffffffffu, run, o);
       if (lane >= o) run += x;
     }
     __syncthreads();
     if (lane == 31) of_warps[warp] = run;
     __syncthreads();
-    long long all = 0, ahead = 0;
+    int all = 0, ahead = 0;
     for (int w = 0; w < warps; w++) {
       if (w == warp) ahead = all;
       all += of_warps[w];
@@ -162,17 +161,16 @@ __device__ void list_pieces(const BwdParams& pp, int* count) {
   };
   const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x, a = min(n, (int)threadIdx.x * per), end = min(n, a + per);
   // pieces twice as long until there is room for all, and for the sums that they leave
-  int length = pp.chunk, beyond = 0;
-  long long ahead;
+  int length = pp.chunk, beyond = 0, before = 0;               // before: place of this thread's first sums
   for (;; length *= 2) {
-    long long more = 0;                                        // pieces beyond one per walk; walks in several, 32 bits up
+    int more = 0, sums = 0;
     for (int e = a; e < end; e++) {
       const int of_walk = max((walk(e) + length - 1) / length - 1, 0);
-      more += of_walk + (of_walk ? 1LL << 32 : 0);
+      more += of_walk;
+      if (of_walk) sums += of_walk + 1;
     }
-    const long long all = sum_of(more, ahead);
-    beyond = (int)all;
-    if (beyond <= pp.extra && beyond + (all >> 32) <= pp.sums) break;
+    beyond = sum_of(more, before);
+    if (beyond <= pp.extra && sum_of(sums, before) <= pp.sums) break;
   }
   auto cut = [&](int e, int& its, int& pieces, int& share) {
     its = walk(e);
@@ -182,17 +180,13 @@ __device__ void list_pieces(const BwdParams& pp, int* count) {
   auto bucket = [&](int size) { return MOST - min(size, MOST); };
   for (int i = threadIdx.x; i < MOST + 2; i += blockDim.x) count[i] = 0;
   __syncthreads();
-  int sums = 0, its, pieces, share;
+  int its, pieces, share;
   for (int e = a; e < end; e++) {
     cut(e, its, pieces, share);
-    if (pieces > 1) {
-      atomicAdd(&count[bucket(share) + 1], pieces - 1);
-      sums += pieces;
-    }
+    if (pieces > 1) atomicAdd(&count[bucket(share) + 1], pieces - 1);
     atomicAdd(&count[bucket(its - (pieces - 1) * share) + 1], 1);
   }
-  sum_of(sums, ahead);
-  int before = (int)ahead;                                     // places of the sums
+  __syncthreads();
   count_ahead(count);
   __syncthreads();
   for (int e = a; e < end; e++) {
