@@ -940,7 +940,9 @@ Pieces pieces_of(const MaParams& p, bool masked, int sms) {
   };
   for (long long parts = 1; parts <= std::min<long long>(far, 64); parts++) look((far + parts - 1) / parts);
   for (long long parts = 1; parts <= std::min<long long>(near, 32); parts++) look((near + parts - 1) / parts);
-  best.sorted = masked || (n_far > 0 && n_near > 0 && far > near && !best.by_head);
+  // (walks differ where there are sinks, and where a window is so long that many of them end with the queries; both passes, in order of their places / sorted, us: 16 x 1500, 8 / 1 heads, d 64, window 800
+  // 278 / 234, 400 left 234; 8 x 2000, 8 / 2 heads, window 1900, 4 sinks 275 / 217)
+  best.sorted = masked || (!best.by_head && n_nblk * pairs > sms && ((n_far > 0 && far > near) || 2 * near > far));
   return best;
 }
 
