@@ -24,6 +24,7 @@
 // P^T and dS^T are rounded to bf16, the type of Q, K and dO, as operands of the tensor cores: 1.7e-3 of a gradient in the 2-norm beside the 1.7e-3 of its own rounding; all sums are fp32.
 // All waits are bounded; on expiry a status word is set and the CTA drains and frees its TMEM.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 #include "attn_masked.cuh"
 #include "tcgen05.cuh"
@@ -43,13 +44,20 @@ struct BwdParams {
   // LIST: pieces of the key blocks' walks {key block, first, length, place of its sums or -1}, longest first; of every key block {place of the first, pieces that leave sums}
   int4* items;
   int2* joined;
-  int *n_items, *cut_blocks;     // {how many pieces, how many key blocks in several}, and those
+  int *n_items, *cut_blocks;     // {how many pieces, how many key blocks in several, how many pieces come first}, and those
   int chunk, extra, sums;        // longest piece wanted, pieces beyond one per key block that there is room for, and pieces that leave sums
-  int by_head;                   // all pieces of a head, then the next head's; else those of all heads together
+  int ordinary, lead;            // LIST: pieces longer than this come first, of all heads, then the others head by head; of `order`: how many key blocks come so
   int acc_d;                     // columns of dq_acc: head_dim in whole pieces of 32
   MaTerms f;
   f32x2 scale2;                  // the scale, twice
 };
+
+// Entry and head of a CTA: the first `lead` entries of a list for all heads, longest first, then the others head by head.
+__device__ __forceinline__ int2 entry_and_head(int cta, int grid, int heads, int lead) {
+  if (cta < lead * heads) return make_int2(cta / heads, cta % heads);
+  const int rest = cta - lead * heads, each = grid / heads - lead;
+  return make_int2(lead + rest % each, rest / each);
+}
 
 // (batch, kv head) pairs whose key blocks are ordered together: enough to keep the chip busy to the end, few enough that several key blocks of a pair run
 // at a time and share its Q / dO / dQ traffic in L2.
@@ -189,6 +197,8 @@ __device__ void list_pieces(const BwdParams& pp, int* count) {
   __syncthreads();
   count_ahead(count);
   __syncthreads();
+  const int lead = count[bucket(pp.ordinary)];                 // (pieces longer than that are in the buckets ahead)
+  __syncthreads();
   for (int e = a; e < end; e++) {
     cut(e, its, pieces, share);
     if (pieces > 1) {
@@ -206,6 +216,7 @@ __device__ void list_pieces(const BwdParams& pp, int* count) {
   if (threadIdx.x == 0) {
     pp.n_items[0] = n + beyond;
     pp.n_items[1] = n_cut;
+    pp.n_items[2] = lead;
   }
 }
 
@@ -441,16 +452,16 @@ ma_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
 
   [[maybe_unused]] int4 piece = make_int4(0, 0, 0, 0);          // (a CTA without one leaves nothing)
   if constexpr (FORM == LIST) {
-    const int of_head = (int)gridDim.x / p.hkv, head = pp.by_head ? (int)blockIdx.x / of_head : (int)blockIdx.x % p.hkv;
-    const int i = pp.by_head ? (int)blockIdx.x - head * of_head : (int)blockIdx.x / p.hkv;
-    if (i < *pp.n_items) piece = pp.items[i];
+    const int2 at = entry_and_head((int)blockIdx.x, (int)gridDim.x, p.hkv, pp.n_items[2]);
+    if (at.x < pp.n_items[0]) piece = pp.items[at.x];
     nblk = piece.x % n_nblk;
-    pair = piece.x / n_nblk * p.hkv + head;
+    pair = piece.x / n_nblk * p.hkv + at.y;
   }
   if (FORM == WHOLE && pp.order) {
-    const int e = pp.order[(int)blockIdx.x / p.hkv];
+    const int2 at = entry_and_head((int)blockIdx.x, (int)gridDim.x, p.hkv, pp.lead);
+    const int e = pp.order[at.x];
     nblk = e % n_nblk;
-    pair = e / n_nblk * p.hkv + (int)blockIdx.x % p.hkv;
+    pair = e / n_nblk * p.hkv + at.y;
   }
   const int hk = pair % p.hkv, b = pair / p.hkv;
   const int n0 = nblk * C::BN;
@@ -903,14 +914,15 @@ long long dq_floats(const MaParams& p) { return p.Sk <= 128 ? 0 : stats_floats(p
 // them see and for blocks of sinks, which all queries behind them see.  Without a mask that is what the walks are at most; documents cut them shorter, and make more, shorter ones of sinks: then there is
 // room for more pieces, and where it does not do the list makes them twice as long.  What pieces leave takes no more memory than dQ's sums, or 64 MB.  Without pieces there is no list; key blocks are
 // sorted then by their walks where these differ.
-// Without a mask, with several kv heads and two CTAs for each SM or more, the order may be head by head: 148 CTAs then work on two heads or three, whose Q, dO and dQ's sums stay in L2, which is worth a
-// twentieth of the time; but a walk that is longer than the others then begins in the last head, too, and ends behind them.
-// The whole backward, us, longest of all heads first / head by head, for the longest piece that is taken (the first one) and others; 32 / 8 heads, d 128: 1 x 8192, window 1024, 4 sinks, of 36 query blocks
-// 484 / 468, of 128 484 / 679, whole 796 / 948; window 128, 150 sinks, of 64 293 / 373, of 8 356 / 308, whole 723 / 777; 1024 sinks, of 128 482 / 591, of 64 499 / 516, of 8 745 / 589, whole 701 / 758;
-// 1 x 16384, window 256, 2048 sinks, whole 1665 / 2040, of 64 1784 / 1643, of 12 2532 / 1992; 4 x 8192, window 128, 4096 sinks, whole 4796 / 4705, of 8 7818 / 6290; 32 / 32 heads: 32 x 2048, window 512,
-// 4 sinks, whole 3369 / 3030, of 5 3362 / 3401.  With a mask, whole and sorted / in the pieces that were taken for no mask: 8 x 2048, window 512, 4 sinks, 32 / 4 heads, d 64, documents of 900 330 / 340,
-// of 300 295 / 306; in pieces where one sequence has few: 1 x 8192, window 1024, 4 sinks, 32 / 8 heads, d 128, one document 493, whole 740, documents of 3000 473, whole 672.
-struct Pieces { int length, extra, sums; bool by_head, sorted; };
+// Without a mask, with several kv heads and two CTAs for each SM or more, the rest of the walks go head by head: 148 CTAs then work on two heads or three, whose Q, dO and dQ's sums stay in L2.  What is
+// longer, of the sinks, goes head by head, too, and what begins with the last head may end behind all others; or it comes first, of all heads, and is slower, most where it is cut, for pieces that are
+// at different queries share nothing.  The whole backward, us, in the order: longest first of all heads / head by head / the sinks' first and the rest head by head, for lengths of pieces in query blocks;
+// 32 / 8 heads, d 128: 2 x 8208, window 103, 1 sink, 8 blocks 553 / 519 / 519, 65 508 / 589 / 514, 130 596 / 742 / 590, whole 887 / 1016 / 870; 1 x 8192, window 128, 1024 sinks, 32 blocks 547 / 496 / 548,
+// 128 500 / 619 / 502, whole 725 / 828 / 684; 1 x 8192, window 1024, 4 sinks, 36 blocks 542 / 512 / 510, 128 516 / 724 / 508, whole 768 / 970 / 771; 1 x 32768, window 512, 4096 sinks, 20 blocks
+// 9524 / 7947 / 7839, 256 7058 / 6215 / 6457, whole 6270 / 6669 / 5764; 4 x 8192, window 128, 4096 sinks, 43 blocks 6505 / 5609 / 6651, whole 5077 / 5024 / 4768; 16 x 742, 64 / 8 heads, window 337,
+// 4 sinks, 32 blocks 890 / 792 / 827, whole 880 / 802 / 837.  With a mask, 32 / 8 heads, d 128, whole and sorted / in pieces: 1 x 8192, window 1024, 4 sinks, one document 740 / 493, documents of 3000
+// 672 / 473; 32 / 4 heads, d 64: 8 x 2048, window 512, documents of 900, where none is cut, 330 / 340.
+struct Pieces { int length, extra, sums, ordinary, lead; bool sorted; };
 Pieces pieces_of(const MaParams& p, bool masked, int sms) {
   const int n_mblocks = (p.Sq + 127) / 128, n_nblk = (p.Sk + 127) / 128, rep = p.hq / p.hkv;
   const long long pairs = (long long)p.hkv * p.B, span = 128 + (p.causal ? 1LL : 2LL) * (p.window - 1LL);
@@ -921,28 +933,32 @@ Pieces pieces_of(const MaParams& p, bool masked, int sms) {
   const long long room = std::max(dq_floats(p), 1LL << 24) / (2LL * p.hkv * 128 * (p.d <= 64 ? 64 : 128));      // pieces that leave sums
   const bool heads = !masked && p.hkv > 1 && n_nblk * pairs >= 2LL * sms;
   double best_time = 0.0;
-  Pieces best{(int)far, 0, 0, false, false};
+  Pieces best{(int)far, 0, 0, 0, 0, false};
   if (p.Sk <= 128) return best;
   auto look = [&](long long length) {
     const long long a = (near + length - 1) / length, b = (far + length - 1) / length;
     long long extra = (n_near * (a - 1) + n_far * (b - 1)) * p.B, sums = extra + ((a > 1 ? n_near : 0) + (b > 1 ? n_far : 0)) * p.B;
     if (sums > room) return;
-    const double work = (double)(n_near * (near + a * (a > 1 ? 9 : 6)) + n_far * (far + b * (b > 1 ? 9 : 6))) * pairs / sms;
-    const double other = (double)((near + a - 1) / a), longest = std::max(other, n_far ? (double)((far + b - 1) / b) : 0.0);
-    const double together = std::max(longest + 9.0, 1.1 * work), apart = 1.045 * work + longest - other, time = (heads ? std::min(together, apart) : together) + (extra ? 1.0 : 0.0);
+    const double work = (double)(n_near * (near + a * (a > 1 ? 9 : 6))) * pairs / sms, sinks = (double)(n_far * (far + b * (b > 1 ? 9 : 6))) * pairs / sms;
+    const double other = (double)((near + a - 1) / a), sink = n_far ? (double)((far + b - 1) / b) : 0.0, longest = std::max(other, sink);
+    const double apart = 1.045 * (work + sinks) + std::max(0.0, longest - std::max(other, (work + sinks) / p.hkv));
+    const double first = heads ? std::max(std::max(other, 1.2 * sink) + 9.0, 1.045 * work + (b > 1 ? 1.4 : 1.1) * sinks) : std::max(longest + 9.0, 1.1 * (work + sinks));
+    const bool by_head = heads && (longest == other || apart <= first);
+    const double time = (by_head ? apart : first) + (extra ? 1.0 : 0.0);
     if (best_time != 0.0 && time >= best_time) return;
     best_time = time;
     if (masked && extra) {
       extra = std::min(2 * extra + (p.sinks ? 4LL * p.B : 0), room / 2);
       sums = extra + std::min(extra, (long long)p.B * n_nblk);
     }
-    best = Pieces{(int)length, (int)std::min(extra, 1LL << 24), (int)std::min(sums, 1LL << 25), heads && apart < together, false};
+    best = Pieces{(int)length, (int)std::min(extra, 1LL << 24), (int)std::min(sums, 1LL << 25), by_head ? INT_MAX : heads ? (int)other : 0, 0, false};
   };
   for (long long parts = 1; parts <= std::min<long long>(far, 64); parts++) look((far + parts - 1) / parts);
   for (long long parts = 1; parts <= std::min<long long>(near, 32); parts++) look((near + parts - 1) / parts);
   // (walks differ where there are sinks, and where a window is so long that many of them end with the queries; both passes, in order of their places / sorted, us: 16 x 1500, 8 / 1 heads, d 64, window 800
   // 278 / 234, 400 left 234; 8 x 2000, 8 / 2 heads, window 1900, 4 sinks 275 / 217)
-  best.sorted = masked || (!best.by_head && n_nblk * pairs > sms && ((n_far > 0 && far > near) || 2 * near > far));
+  best.sorted = masked || (n_nblk * pairs > sms && ((n_far > 0 && far > near) || 2 * near > far));
+  best.lead = (int)((best.ordinary == INT_MAX ? 0 : heads ? n_far : n_nblk) * p.B);
   return best;
 }
 
@@ -1011,7 +1027,7 @@ int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s) {
     p.chunk = c.length;
     p.extra = c.extra;
     p.sums = c.sums;
-    p.by_head = c.by_head;
+    p.ordinary = c.ordinary;
     p.dv_acc = p.dk_acc + piece_floats(a, c);
     p.items = reinterpret_cast<int4*>(p.dv_acc + piece_floats(a, c));
     p.joined = reinterpret_cast<int2*>(p.items + order_ints(a) + c.extra);
@@ -1021,6 +1037,7 @@ int ma_launch_bwd(const MaBwdParams& w, cudaStream_t s) {
   }
   if (!a.window) p.parts = parts_of(a.B, a.Sq, a.Sk, a.hq, a.hkv, a.causal, lb_num_sms());
   p.dv_acc = p.dk_acc + part_floats(a, p.parts);
+  p.lead = a.window > 0 ? c.lead : (int)order_ints(a);
   p.order = (a.window > 0 ? c.sorted : a.kb && p.parts == 1) && a.Sk > 128 ? reinterpret_cast<int*>(p.dv_acc + part_floats(a, p.parts)) : nullptr;
   return a.d <= 64 ? launch_bwd<64>(p, s) : launch_bwd<128>(p, s);
 }
