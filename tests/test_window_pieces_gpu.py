@@ -47,3 +47,13 @@ def test_memory_of_many_sinks():
     n = q.numel()
     # o, what its rounding left, dq, dk, dv in bf16; lse and two row statistics in fp32; dQ's sums, and what pieces leave
     assert torch.cuda.max_memory_allocated() - before < 10 * n + 12 * n // 64 + 4 * n + max(4 * n, 1 << 26) + (8 << 20)
+
+
+@pytest.mark.parametrize("B,S,hq,hkv,d,window,sinks,causal", [
+    (6, 700, 16, 16, 64, 600, 4, True), (8, 600, 16, 8, 64, 100, 3, True), (4, 900, 16, 16, 64, 300, 700, True), (8, 513, 12, 12, 128, 500, 0, True), (3, 2000, 8, 8, 64, 64, 1500, True),
+    (4, 1000, 12, 12, 64, 100, 900, False),
+])
+def test_whole_walks_in_their_order(B, S, hq, hkv, d, window, sinks, causal):
+    """Nothing cut: key blocks sorted by their walks, head by head or those of the sinks ahead of all heads."""
+    _check(B, S, S, hq, hkv, d, window, sinks, causal=causal)
+    _again(B, S, hq, hkv, d, window, sinks, causal)
